@@ -14,6 +14,7 @@ import atexit
 import collections
 import ctypes
 import functools
+import itertools
 import os
 import sys
 
@@ -1441,6 +1442,127 @@ def attention_replay_key(step, n_heads: int, n_kv_heads: int, window: int = 0):
                                    for d in ((64, 128) if window > 0 else ()))
 
 
+# ----------------------------------------------------------------------------- sequences that share pages
+
+@functools.lru_cache(maxsize=4096)
+def _prefix_scratch(n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own) -> tuple:
+    """(floats of scratch, launches) of a prefix_attention of these sizes."""
+    lib, kernels = load_library("prefix_attention"), ctypes.c_int(0)
+    lib.llmb_prefix_attention_scratch_floats.restype = ctypes.c_longlong
+    floats = lib.llmb_prefix_attention_scratch_floats(*map(_c_int, (n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new,
+                                                                    max_group, max_shared, max_own)), ctypes.byref(kernels))
+    return floats, kernels.value
+
+
+def _page_bucket(pages: int) -> int:
+    """The least power of two that is no less than `pages` (0 for 0): what a launch depends on of a number of pages."""
+    return 1 << (pages - 1).bit_length() if pages > 0 else 0
+
+
+def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, n_heads, n_kv_heads, head_dim,
+                     scale, *, max_new, max_group, max_shared, max_own, out=None):
+    """Causal grouped-query attention, as `attention` without its options, for a batch whose sequences share pages: the
+    sequences group_first[g] .. group_first[g + 1] - 1 have the same pages in the first group_pages[g] places of their rows of
+    `block_table`, and those keys and values are read once for all of them. `group_first` (int32 [G + 1], from 0 to the
+    number of sequences) and `group_pages` (int32 [G]) are on the device, as `seq_lens` [B] (with the new tokens) and
+    `cu_seqlens` [B + 1] are; a sequence that shares nothing is a group of its own with 0 pages. The cache already holds the
+    new tokens' keys and values. Returns [T, Hq * D] in qkv's dtype.
+
+    max_new, max_group: most new tokens of a sequence, of a group; max_shared: most pages that a group shares; max_own: most
+    positions of a sequence behind those. Upper bounds, which size the launches."""
+    _require_cuda(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages)
+    n, dtype = qkv.shape[0], qkv.dtype
+    n_seqs, n_groups = seq_lens.numel(), group_pages.numel()
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < n_heads * head_dim:
+        raise KernelError(f"prefix_attention: queries must be rows of at least {n_heads * head_dim} contiguous values")
+    for cache in (k_cache, v_cache):
+        if (cache.dim() != 4 or tuple(cache.shape[1:]) != (n_kv_heads, PAGE, head_dim) or cache.dtype != dtype
+                or not cache.is_contiguous()):
+            raise KernelError(f"prefix_attention: caches must be contiguous {dtype} [pages, {n_kv_heads}, {PAGE}, {head_dim}]")
+    for name, ints, count in (("seq_lens", seq_lens, n_seqs), ("cu_seqlens", cu_seqlens, n_seqs + 1),
+                              ("group_first", group_first, n_groups + 1), ("group_pages", group_pages, n_groups)):
+        if ints.dtype != torch.int32 or ints.numel() != count or not ints.is_contiguous():
+            raise KernelError(f"prefix_attention: {name} must be contiguous int32 [{count}]")
+    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n_seqs or block_table.stride(1) != 1
+            or max_shared > block_table.shape[1]):
+        raise KernelError(f"prefix_attention: the page table must be int32 [{n_seqs}, at least {max_shared}]")
+    if max_new < 1 or max_group < max_new or max_shared < 0 or max_own < 0:
+        raise KernelError(f"prefix_attention: no bounds of a step: max_new {max_new}, max_group {max_group}, max_shared {max_shared}, "
+                          f"max_own {max_own}")
+    _check_out(out, (n, n_heads * head_dim), dtype, "prefix_attention")
+    if out is None:
+        out = torch.empty((n, n_heads * head_dim), dtype=dtype, device=qkv.device)
+    if n == 0:
+        return out
+    shared, own = _page_bucket(max_shared), _page_bucket(-(-max_own // PAGE)) * PAGE
+    floats, kernels = _prefix_scratch(n, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, shared, own)
+    parts = _scratch(qkv.device, "attention", floats)[0] if floats else None
+    _call("prefix_attention", "llmb_prefix_attention", _ptr(qkv), _c_int(qkv.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(block_table),
+          _c_int(block_table.stride(0)), _ptr(seq_lens), _ptr(cu_seqlens), _ptr(group_first), _ptr(group_pages), _ptr(out),
+          _c_int(out.stride(0)), _ptr(parts), ctypes.c_longlong(floats), _c_int(_code(dtype)), _c_int(n), _c_int(n_seqs), _c_int(n_groups),
+          _c_int(n_heads), _c_int(n_kv_heads), _c_int(head_dim), _c_float(scale), _c_int(max_new), _c_int(max_group), _c_int(shared),
+          _c_int(own), _stream(), kernels=kernels)
+    return out
+
+
+def _copy_items(shapes, n_items: int, source, target, rows, what: str) -> None:
+    source, target = list(source), list(target)
+    rows = [1] * len(source) if rows is None else list(rows)
+    if not len(source) == len(target) == len(rows):
+        raise KernelError(f"{what}: {len(source)} sources, {len(target)} targets, {len(rows)} numbers of rows")
+    if not source or not shapes:
+        return
+    if min(source) < 0 or max(source) >= n_items or min(target) < 0 or max(target) >= n_items:
+        raise KernelError(f"{what}: an item is outside the {n_items} there are")
+    targets = set(target)
+    if len(targets) != len(target) or not targets.isdisjoint(source):
+        raise KernelError(f"{what}: every target is written once and no target is a source")
+    triples = sorted(zip(source, target, rows))                      # the targets of a source stand together
+    pairs = (_c_int * (3 * len(triples)))(*itertools.chain.from_iterable(triples))
+    flat = (ctypes.c_longlong * (7 * len(shapes)))(*itertools.chain.from_iterable(shapes))
+    launches = -(-len(shapes) // 16) * -(-len(triples) // 240)
+    _call("page_copy", "llmb_page_copy", _c_int(len(shapes)), flat, _c_int(len(triples)), pairs, _stream(), kernels=launches)
+
+
+def copy_pages(pools, source, target, rows=None) -> None:
+    """pools[..., target[i], :, :rows[i], :] = pools[..., source[i], :, :rows[i], :] for all i, in place and in one launch: what
+    forking a sequence does with its last page and compacting a cache with whole pages. `pools`: a tensor [..., pages, heads,
+    64, dim] (all layers of keys and values), or a list of such tensors with the same number of pages; `source`, `target`, `rows`:
+    whole numbers on the host. rows[i] (1 to 64; all rows if None) positions are copied. A page may be the source of many, but no page is
+    written twice, and no page is both a source and a target."""
+    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    _require_cuda(*pools)
+    shapes = []
+    for pool in pools:
+        if pool.dim() < 4 or not pool.is_contiguous() or pool.shape[-2] != PAGE or pool.shape[-4] != pools[0].shape[-4]:
+            raise KernelError(f"copy_pages: a pool must be contiguous [..., pages, heads, {PAGE}, dim], all with the same pages")
+        pages, heads, _, dim = pool.shape[-4:]
+        row = dim * pool.element_size()
+        if pool.numel():
+            shapes.append((pool.data_ptr(), pool.numel() // (pages * heads * PAGE * dim), heads, pages * heads * PAGE * row, heads * PAGE * row,
+                           PAGE * row, row))
+    if rows is None:
+        rows = [PAGE] * len(source)
+    elif len(rows) and (min(rows) < 1 or max(rows) > PAGE):
+        raise KernelError(f"copy_pages: a page has 1 to {PAGE} rows to copy")
+    _copy_items(shapes, pools[0].shape[-4] if pools else 0, source, target, rows, "copy_pages")
+
+
+def copy_slots(states, source, target) -> None:
+    """states[..][target[i]] = states[..][source[i]] for all i, in place: what layers keep for a sequence at a fixed size, copied to other
+    slots. `states`: a list of contiguous tensors [slots, ...]; the rest as in `copy_pages`."""
+    states = [states] if isinstance(states, torch.Tensor) else list(states)
+    _require_cuda(*states)
+    shapes = []
+    for state in states:
+        if state.dim() < 1 or not state.is_contiguous() or state.shape[0] != states[0].shape[0]:
+            raise KernelError("copy_slots: a state must be contiguous [slots, ...], all with the same slots")
+        if state.numel():
+            size = state.numel() // state.shape[0] * state.element_size()
+            shapes.append((state.data_ptr(), 1, 1, 0, size, 0, size))
+    _copy_items(shapes, states[0].shape[0] if states else 0, source, target, None, "copy_slots")
+
+
 # ----------------------------------------------------------------------------- latent attention, shared rotated keys
 
 def latent_write(u, n_heads, dim, rot, rank, gain, eps, rope_table, interleaved, tok_pos, tok_seq, block_table, ring_pages,
@@ -1894,7 +2016,7 @@ def required_libraries() -> list:
             "attention_decode", "attention_prefill", "attention_prefill_tc", "sampling"]
 
 
-__all__ = ["PAGE", "GLU_BLOCK", "glu_fusable", "embed", "scale_", "random_normal_", "begin_recording", "end_recording", "RecordedPass", "StepScope", "scratch_generation", "Emit", "FoldedNorm", "RopeWrite", "cast_sumsq", "SUMSQ_LD", "rmsnorm", "swiglu", "rope_cache_write", "linear", "attention",
+__all__ = ["PAGE", "GLU_BLOCK", "glu_fusable", "embed", "scale_", "random_normal_", "begin_recording", "end_recording", "RecordedPass", "StepScope", "scratch_generation", "Emit", "FoldedNorm", "RopeWrite", "cast_sumsq", "SUMSQ_LD", "rmsnorm", "swiglu", "rope_cache_write", "linear", "attention", "prefix_attention", "copy_pages", "copy_slots",
            "softcap_", "add_rows_", "conv_rope_cache_write", "diff_attention", "tanh_norm", "norm_rope_cache_write",
            "sigmoid_attention", "gated_recurrence", "state_space", "attention_replay_key", "layernorm", "input_conv", "output_norm_add_", "forget_recurrence",
            "latent_write", "head_products", "latent_attention", "latent_prefill", "attention_decode_splits", "sigmoid_attention_replay_key", "sigmoid_decode_splits", "sigmoid_mixed_heads", "sigmoid_mixed_elements",
