@@ -15,9 +15,10 @@
 // bounds (most tokens of a group, most pages) and a block beyond the real work leaves. A key beyond a row's position has no
 // weight whatever is stored there, and values beyond a tile's last position are taken for zero, so that what an earlier sequence
 // left in a page (infinities and NaN too) does not reach a result. A row that sees no key is zero.
-#include "common.cuh"
+#include "tc.cuh"
 
 using namespace llmb;
+using namespace llmb::tc;
 
 LLMB_DEFINE_LAST_ERROR(llmb_prefix_attention)
 
@@ -40,7 +41,8 @@ struct Args {
     int q_stride, out_stride, table_stride, n_seqs, n_groups, n_heads, n_kv_heads, head_dim;
     float scale_log2;
     int prefix_tiles, prefix_splits, own_tiles, own_splits, slots;
-    int vectors;                     // the caches' rows and the queries can be read 16 bytes at a time
+    int vectors;                     // the caches' rows can be read 16 bytes at a time
+    int whole;                       // a tile of a group walks its sequences' own pages behind the shared ones (tensor cores)
 };
 
 // A block's share of the work: rows of a range of tokens against a slice of pages.
@@ -48,6 +50,7 @@ struct Item {
     int kv_head, tile, tiles, slot;
     int seq_first, seq_last;         // the sequences whose tokens are the rows
     int first_token, n_rows;
+    int page_first;                  // the first page that is not shared (own parts)
     int page_begin, page_end;        // of the table of seq_first
 };
 
@@ -75,6 +78,7 @@ __device__ __forceinline__ bool item_of(const Args& a, int x, Item& w) {
         w.seq_first = a.group_first[group];
         w.seq_last = a.group_first[group + 1];
         int pages = a.group_pages[group], per = (pages + a.prefix_splits - 1) / a.prefix_splits;
+        w.page_first = 0;
         w.page_begin = min(split * per, pages);
         w.page_end = min(w.page_begin + per, pages);
         w.slot = split;
@@ -88,6 +92,7 @@ __device__ __forceinline__ bool item_of(const Args& a, int x, Item& w) {
         w.seq_last = seq + 1;
         int first = a.group_pages[group_of(a, seq)], last = (a.seq_lens[seq] + LLMB_PAGE - 1) / LLMB_PAGE;
         int pages = max(last - first, 0), per = (pages + a.own_splits - 1) / a.own_splits;
+        w.page_first = first;
         w.page_begin = first + min(split * per, pages);
         w.page_end = first + min(split * per + per, pages);
         w.slot = a.prefix_splits + split;
@@ -98,15 +103,19 @@ __device__ __forceinline__ bool item_of(const Args& a, int x, Item& w) {
     return true;
 }
 
-// the position of a token of the item's sequences
-__device__ __forceinline__ int position_of(const Args& a, const Item& w, int token) {
+// which of the item's sequences a token belongs to, and its position there
+__device__ __forceinline__ int sequence_of(const Args& a, const Item& w, int token) {
     int low = w.seq_first, high = w.seq_last - 1;             // the last sequence whose tokens do not start behind this one
     while (low < high) {
         int mid = (low + high + 1) >> 1;
         if (a.cu_seqlens[mid] <= token) low = mid;
         else high = mid - 1;
     }
-    return a.seq_lens[low] - a.cu_seqlens[low + 1] + token;
+    return low;
+}
+__device__ __forceinline__ int position_of(const Args& a, const Item& w, int token) {
+    int seq = sequence_of(a, w, token);
+    return a.seq_lens[seq] - a.cu_seqlens[seq + 1] + token;
 }
 
 // ------------------------------------------------------------------------------------------------ any type, any head size
@@ -302,6 +311,392 @@ __global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(con
     }
 }
 
+// ------------------------------------------------------------------------------------------------ bfloat16, head sizes 64 and 128
+//
+// The products on the fifth-generation tensor cores. A block holds 128 rows and walks its pages one by one:
+//
+// * warps 0 and 6: the page's keys and values by TMA (64 x 64 boxes with the 128-byte swizzle), two buffers each;
+// * warp 1: S[128, 64 keys] = Q K^T into one of two buffers of scores in tensor memory, O[128, D] += P V with P from tensor memory. The
+//   scores of the page after the next are issued behind P V of this one, so that products and softmax work on different buffers;
+// * warps 2 to 5: thread r owns row r. It puts the tile's queries into shared memory (rows are token and head, which no box of a
+//   tensor map follows for every share), then per page reads 64 scores, forms the weights and writes them over the scores as pairs
+//   of bfloat16 (rounded to 8 bits: what the tensor cores take; their sum is of the unrounded ones). The maximum that the exponents refer to
+//   moves only when a page exceeds it by more than 2^8; O is then rescaled in place.
+//
+// A walk is the shared pages, or a sequence's own ones, or both: behind the shared pages those of each sequence that the tile has rows of,
+// whose rows alone see them (`whole`).
+
+constexpr int TC_ROWS = 128, TC_THREADS = 224;
+constexpr int Q_PIECE = TC_ROWS * 64 * 2;         // the tile's rows, 64 columns of the head: 16 KB
+constexpr int KV_PIECE = LLMB_PAGE * 64 * 2;      // a page, 64 columns of the head: 8 KB
+// tensor memory: two buffers of scores (64 columns of 32-bit values, the weights over the first 32), O beside them
+constexpr uint32_t S_COL = 0, O_COL = 128, TMEM_COLS = 256;
+
+// The pages of an item, one after the other: the shared ones, then those of each sequence in turn.
+struct Walk {
+    int seq;                          // whose own pages these are, or -1 for shared ones
+    int logical, end;                 // place in the table of the sequence (of the first one where shared), end of this stretch
+    int limit;                        // the last position of the stretch that a row of the tile sees
+};
+
+// the tile's rows are tokens first .. last of sequences seq_first .. seq_last
+struct TileRange {
+    int seq_first, seq_last, token_first, token_last, shared;
+    bool own;                         // own pages behind the shared ones
+};
+
+__device__ __forceinline__ void own_stretch(const Args& a, const TileRange& t, int seq, Walk& w) {
+    w.seq = seq;
+    int end = a.cu_seqlens[seq + 1];
+    w.limit = a.seq_lens[seq] - end + min(end - 1, t.token_last);         // position of the sequence's last token in the tile
+    w.logical = t.shared;
+    w.end = w.limit / LLMB_PAGE + 1;
+    if (a.cu_seqlens[seq] == end || w.limit < 0) w.end = 0;                 // brings nothing
+}
+__device__ __forceinline__ bool next_stretch(const Args& a, const TileRange& t, Walk& w) {
+    while (t.own) {
+        int seq = w.seq < 0 ? t.seq_first : w.seq + 1;
+        if (seq > t.seq_last) return false;
+        own_stretch(a, t, seq, w);
+        if (w.logical < w.end) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ bool step(const Args& a, const TileRange& t, Walk& w) { return ++w.logical < w.end || next_stretch(a, t, w); }
+// to the page `skip` pages behind the walk's first
+__device__ __forceinline__ void start(const Args& a, const TileRange& t, Walk& w, int skip) {
+    w.seq = -1;
+    w.logical = 0;
+    w.end = t.shared;
+    w.limit = t.shared * LLMB_PAGE - 1;
+    while (skip >= w.end - w.logical) {
+        skip -= max(w.end - w.logical, 0);
+        if (!next_stretch(a, t, w)) return;
+    }
+    w.logical += skip;
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+template <int HD>
+__global__ void __launch_bounds__(TC_THREADS, 2)
+prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                           const __grid_constant__ Args a, int* status) {
+    constexpr int PIECES = HD / 64;
+    constexpr int KV_BYTES = PIECES * KV_PIECE;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* q_tile = base;
+    unsigned char* k_tile = base + PIECES * Q_PIECE;
+    unsigned char* v_tile = k_tile + 2 * KV_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(v_tile + 2 * KV_BYTES);
+    uint64_t* q_full = bars;                  // the queries are in shared memory
+    uint64_t* k_full = bars + 1;              // [2]
+    uint64_t* k_empty = bars + 3;             // [2]
+    uint64_t* v_full = bars + 5;              // [2]
+    uint64_t* v_empty = bars + 7;             // [2]
+    uint64_t* s_full = bars + 9;              // [2] a buffer's scores are complete
+    uint64_t* p_full = bars + 11;             // [2] its weights are written and O has been rescaled
+    uint64_t* o_full = bars + 13;             // a page's P V has been added to O
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    griddep_launch();
+    griddep_wait();
+    Item w;
+    if (!item_of(a, blockIdx.x, w)) return;                  // uniform for the block, here and below: nothing is allocated yet
+    const int share = a.n_heads / a.n_kv_heads;
+    const int row0 = w.tile * TC_ROWS, n_rows = min(TC_ROWS, w.n_rows - row0);
+    if (n_rows <= 0) return;
+    const bool of_group = w.slot < a.prefix_splits;
+    TileRange range;
+    range.token_first = w.first_token + row0 / share;
+    range.token_last = w.first_token + (row0 + n_rows - 1) / share;
+    range.seq_first = of_group ? sequence_of(a, w, range.token_first) : w.seq_first;
+    range.seq_last = of_group ? sequence_of(a, w, range.token_last) : w.seq_first;
+    range.own = !of_group || a.whole;
+    range.shared = of_group ? a.group_pages[group_of(a, w.seq_first)] : w.page_first;
+    // the slice of the walk that is this block's
+    int skip, n_blocks;
+    if (of_group) {
+        int total = range.shared;
+        if (a.whole) {
+            Walk all;
+            all.seq = -1;
+            while (next_stretch(a, range, all)) total += all.end - all.logical;
+        }
+        int per = (total + a.prefix_splits - 1) / a.prefix_splits;
+        skip = min(w.slot * per, total);
+        n_blocks = min(per, total - skip);
+    } else {
+        skip = w.page_begin - w.page_first;
+        n_blocks = w.page_end - w.page_begin;
+        Walk all;
+        own_stretch(a, range, w.seq_first, all);
+        n_blocks = max(0, min(n_blocks, all.end - w.page_begin));
+    }
+    const int* shared_pages = a.block_table + (size_t)w.seq_first * a.table_stride;
+    Walk walk;
+    auto start_walk = [&]() {
+        if (of_group) {
+            start(a, range, walk, skip);
+        } else {
+            own_stretch(a, range, w.seq_first, walk);
+            walk.logical += skip;
+        }
+    };
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 14; ++i) mbar_init(smem_u32(&bars[i]), (i == 0 || i == 11 || i == 12) ? 128 : 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0 || warp == 6) {
+        const bool keys = warp == 0;
+        const CUtensorMap* map = keys ? &map_k : &map_v;
+        unsigned char* tiles = keys ? k_tile : v_tile;
+        uint64_t* full = keys ? k_full : v_full;
+        uint64_t* empty = keys ? k_empty : v_empty;
+        if (n_blocks > 0) start_walk();
+        for (int kb = 0; kb < n_blocks; ++kb) {
+            int b = kb & 1;
+            const int* pages = walk.seq < 0 ? shared_pages : a.block_table + (size_t)walk.seq * a.table_stride;
+            int page = pages[walk.logical];
+            step(a, range, walk);
+            if (kb >= 2 && !mbar_wait_warp(smem_u32(&empty[b]), ((kb >> 1) - 1) & 1, abort_flag, status, keys ? 11 : 12)) break;
+            if (elect_one()) {
+                uint32_t bar = smem_u32(&full[b]);
+                mbar_expect_tx(bar, KV_BYTES);
+                int row = (page * a.n_kv_heads + w.kv_head) * LLMB_PAGE;
+                for (int h = 0; h < PIECES; ++h)
+                    tma_load_2d(smem_u32(tiles + b * KV_BYTES + h * KV_PIECE), map, bar, h * 64, row);
+            }
+            __syncwarp();
+        }
+    } else if (warp == 1) {
+        // D 32-bit, A and B bfloat16, M = 128; S has N = 64 keys, O has N = HD with B MN-major
+        constexpr uint32_t idesc_qk = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LLMB_PAGE >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
+        constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
+        const uint64_t q_desc = smem_desc(smem_u32(q_tile));
+        const uint64_t k_desc0 = smem_desc(smem_u32(k_tile)), v_desc0 = smem_desc_mn(smem_u32(v_tile), KV_PIECE);
+        constexpr uint64_t BUFFER = (uint64_t)(KV_BYTES >> 4);       // the second buffer, in the address field
+        auto issue_qk = [&](int kb) -> bool {
+            int b = kb & 1;
+            if (!mbar_wait_warp(smem_u32(&k_full[b]), (kb >> 1) & 1, abort_flag, status, 14)) return false;
+            tcgen05_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int j = 0; j < HD / 16; ++j) {
+                    uint64_t q_off = (uint64_t)(((j >> 2) * Q_PIECE + (j & 3) * 32) >> 4);
+                    uint64_t k_off = (uint64_t)(((j >> 2) * KV_PIECE + (j & 3) * 32) >> 4);
+                    tcgen05_mma(tmem_base + S_COL + b * LLMB_PAGE, q_desc + q_off, k_desc0 + b * BUFFER + k_off, idesc_qk, j > 0 ? 1u : 0u);
+                }
+                tcgen05_commit(smem_u32(&s_full[b]));
+                tcgen05_commit(smem_u32(&k_empty[b]));
+            }
+            __syncwarp();
+            return true;
+        };
+        bool ok = n_blocks > 0 && mbar_wait_warp(smem_u32(q_full), 0, abort_flag, status, 13) && issue_qk(0);
+        if (ok && n_blocks > 1) ok = issue_qk(1);
+        for (int kb = 0; kb < n_blocks && ok; ++kb) {
+            int b = kb & 1, phase = (kb >> 1) & 1;
+            ok = mbar_wait_warp(smem_u32(&p_full[b]), phase, abort_flag, status, 15);
+            ok = ok && mbar_wait_warp(smem_u32(&v_full[b]), phase, abort_flag, status, 16);
+            if (!ok) break;
+            tcgen05_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int j = 0; j < LLMB_PAGE / 16; ++j)    // 16 keys a step: 8 columns of P, 2048 bytes of V rows
+                    tcgen05_mma_ts(tmem_base + O_COL, tmem_base + S_COL + b * LLMB_PAGE + j * 8,
+                                   v_desc0 + b * BUFFER + (uint64_t)((j * 2048) >> 4), idesc_pv, (kb > 0 || j > 0) ? 1u : 0u);
+                tcgen05_commit(smem_u32(o_full));
+                tcgen05_commit(smem_u32(&v_empty[b]));
+            }
+            __syncwarp();
+            if (kb + 2 < n_blocks) ok = issue_qk(kb + 2);
+        }
+    } else {
+        const int t = threadIdx.x - 64;                      // 0 .. 127
+        {   // the queries, 16 bytes at a time, where the 128-byte swizzle has them
+            constexpr int CHUNKS = HD / 8;
+            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q);
+#pragma unroll 4
+            for (int i = t; i < TC_ROWS * CHUNKS; i += 128) {
+                int r = i / CHUNKS, c = i - r * CHUNKS;
+                uint4 value = make_uint4(0u, 0u, 0u, 0u);
+                if (r < n_rows) {
+                    int token = w.first_token + (row0 + r) / share, head = w.kv_head * share + (row0 + r) % share;
+                    value = *reinterpret_cast<const uint4*>(q + (size_t)token * a.q_stride + (size_t)head * HD + c * 8);
+                }
+                *reinterpret_cast<uint4*>(q_tile + (c >> 3) * Q_PIECE + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = value;
+            }
+            fence_async_shared();
+            mbar_arrive(smem_u32(q_full));
+        }
+        int quarter = warp & 3;
+        int row = quarter * 32 + lane;                       // row of the tile = lane of tensor memory
+        const int token = w.first_token + (row0 + min(row, n_rows - 1)) / share;
+        const int my_seq = of_group ? sequence_of(a, w, token) : w.seq_first;
+        const int my_pos = row < n_rows ? a.seq_lens[my_seq] - a.cu_seqlens[my_seq + 1] + token : -1;
+        uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        float run_max = -INFINITY, run_sum = 0.f;
+        bool ok = true;
+        if (n_blocks > 0) start_walk();
+        for (int kb = 0; kb < n_blocks && ok; ++kb) {
+            int b = kb & 1;
+            const int key0 = walk.logical * LLMB_PAGE, limit = walk.limit;
+            const int pos = walk.seq < 0 || walk.seq == my_seq ? my_pos : -1;         // what the row sees of this stretch
+            step(a, range, walk);
+            ok = mbar_wait(smem_u32(&s_full[b]), (kb >> 1) & 1, abort_flag, status, 17);
+            if (!ok) break;
+            __syncwarp();
+            tcgen05_fence_after();
+            bool whole = key0 + LLMB_PAGE - 1 <= pos;        // no key of the page is hidden from this row
+            uint32_t s_addr = lane_addr + S_COL + b * LLMB_PAGE;
+            uint32_t ra[32], rb[32];
+            tmem_ld32_start(s_addr, ra);
+            tmem_ld32_start(s_addr + 32, rb);
+            tmem_ld32_wait(ra);
+            tmem_ld32_wait(rb);
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    if (key0 + j > pos) ra[j] = __float_as_uint(-INFINITY);
+                    if (key0 + 32 + j > pos) rb[j] = __float_as_uint(-INFINITY);
+                }
+            }
+            float block_max = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) block_max = max3(block_max, __uint_as_float(ra[j]), __uint_as_float(ra[j + 1]));
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) block_max = max3(block_max, __uint_as_float(rb[j]), __uint_as_float(rb[j + 1]));
+            // (a row that has seen no key yet keeps -inf, and all its weights are zero)
+            bool move = (block_max - run_max) * a.scale_log2 > 8.f;
+            float new_max = move ? block_max : run_max;
+            float alpha = move && kb > 0 ? fast_exp2((run_max - new_max) * a.scale_log2) : 1.f;
+            float shift = new_max == -INFINITY ? 0.f : new_max * a.scale_log2;
+            run_max = new_max;
+            float add = 0.f;
+            auto to_weights = [&](const uint32_t (&r)[32], int c) {
+                uint32_t packed[16];
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                    float p0 = fast_exp2(fmaf(__uint_as_float(r[j]), a.scale_log2, -shift));
+                    float p1 = fast_exp2(fmaf(__uint_as_float(r[j + 1]), a.scale_log2, -shift));
+                    add += p0 + p1;
+                    packed[j >> 1] = pack2(p0, p1);
+                }
+                tmem_st16(s_addr + (c >> 1), packed);
+            };
+            to_weights(ra, 0);
+            to_weights(rb, 32);
+            run_sum = run_sum * alpha + add;
+            if (kb > 0) {
+                ok = mbar_wait(smem_u32(o_full), (kb - 1) & 1, abort_flag, status, 18);
+                if (!ok) break;
+                __syncwarp();
+                tcgen05_fence_after();
+                if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t r[32];
+                        tmem_ld32(lane_addr + O_COL + c, r);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
+                        tmem_st32(lane_addr + O_COL + c, r);
+                    }
+                }
+            }
+            if (key0 + LLMB_PAGE - 1 > limit) {              // values behind the last position are whatever a page held: zero here
+                ok = mbar_wait(smem_u32(&v_full[b]), (kb >> 1) & 1, abort_flag, status, 20);
+                if (!ok) break;
+                int first = limit + 1 - key0;                // (a row of a piece is 128 bytes, its swizzle stays inside)
+                for (int i = t; i < PIECES * (LLMB_PAGE - first) * 8; i += 128) {
+                    int piece = i / ((LLMB_PAGE - first) * 8), rest = i - piece * (LLMB_PAGE - first) * 8;
+                    *reinterpret_cast<uint4*>(v_tile + b * KV_BYTES + piece * KV_PIECE + first * 128 + rest * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_async_shared();
+            }
+            tmem_st_wait();
+            tcgen05_fence_before();
+            mbar_arrive(smem_u32(&p_full[b]));
+        }
+        if (ok && n_blocks > 0) ok = mbar_wait(smem_u32(o_full), (n_blocks - 1) & 1, abort_flag, status, 19);
+        if (ok) {
+            __syncwarp();
+            tcgen05_fence_after();
+            const bool valid = row < n_rows;
+            const int head = w.kv_head * share + (row0 + row) % share;
+            const bool direct = a.slots == 1;
+            float inv = run_sum != 0.f ? 1.0f / run_sum : 0.f;
+            size_t slot = ((size_t)token * a.n_heads + head) * a.slots + w.slot;
+            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD;
+            float* acc = a.acc + slot * HD;
+            if (valid && !direct) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(run_sum != 0.f ? run_max * a.scale_log2 : -INFINITY, run_sum);
+            if (direct || n_blocks > 0) {
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t r[32];
+                    if (n_blocks > 0) {
+                        tmem_ld32(lane_addr + O_COL + c, r);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) r[j] = 0u;
+                    }
+                    if (valid && direct) {
+#pragma unroll
+                        for (int d = 0; d < 32; d += 8) {
+                            uint4 packed;
+                            packed.x = pack2(__uint_as_float(r[d]) * inv, __uint_as_float(r[d + 1]) * inv);
+                            packed.y = pack2(__uint_as_float(r[d + 2]) * inv, __uint_as_float(r[d + 3]) * inv);
+                            packed.z = pack2(__uint_as_float(r[d + 4]) * inv, __uint_as_float(r[d + 5]) * inv);
+                            packed.w = pack2(__uint_as_float(r[d + 6]) * inv, __uint_as_float(r[d + 7]) * inv);
+                            *reinterpret_cast<uint4*>(o + c + d) = packed;
+                        }
+                    } else if (valid) {
+#pragma unroll
+                        for (int d = 0; d < 32; d += 4)
+                            *reinterpret_cast<uint4*>(acc + c + d) = make_uint4(r[d], r[d + 1], r[d + 2], r[d + 3]);
+                    }
+                }
+            }
+        }
+    }
+
+    tcgen05_fence_before();
+    __syncthreads();
+    if (*abort_flag) {                                       // a wait ran out: copies in flight get their time before the block leaves
+        for (int i = 0; i < 100; ++i) __nanosleep(10000);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tcgen05_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ the parts joined
 //
 // A warp a row: each lane reads one part's maximum and sum, the weights are shared by shuffles, and the lanes take columns.
@@ -349,27 +744,18 @@ __global__ void __launch_bounds__(128) prefix_attention_join_kernel(const __grid
 // ------------------------------------------------------------------------------------------------ the call
 
 struct Plan {
+    bool tc;                         // tensor cores
+    bool whole;                      // a group's tiles walk the shared and the own pages, nothing is left for own parts
     int prefix_tiles, prefix_splits, own_tiles, own_splits, slots;
 };
 
 constexpr int SMS = 148;
+constexpr int MAX_SPLITS = 64;
 
-// Into how many parts the shared and the own pages are cut: as many pages a block as make all blocks come to about `wave`,
-// two pages at least.
-Plan plan_of(int n_seqs, int n_groups, int share, int n_kv_heads, int rows, int max_new, int max_group, int shared_pages, int own_pages, int wave) {
-    Plan p;
-    p.prefix_tiles = shared_pages > 0 ? ceil_div((long long)max_group * share, rows) : 0;
-    p.own_tiles = ceil_div((long long)max_new * share, rows);
-    long long prefix = (long long)n_groups * p.prefix_tiles * n_kv_heads, own = (long long)n_seqs * p.own_tiles * n_kv_heads;
-    long long per = (prefix * shared_pages + own * own_pages + wave - 1) / wave;
-    if (per < 2) per = 2;
-    p.prefix_splits = shared_pages > 0 ? ceil_div(shared_pages, per) : 0;
-    p.own_splits = ceil_div(own_pages, per);
-    if (p.prefix_splits > 64) p.prefix_splits = 64;
-    if (p.own_splits > 64) p.own_splits = 64;
-    p.slots = p.prefix_splits + p.own_splits;
-    return p;
-}
+struct Sizes {
+    int n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own;
+    bool tc;                         // the tensor-core kernel can take the call
+};
 
 // the least power of two that is no less than n: replayed steps of one bucket make the same launches
 int bucket(int n) {
@@ -378,52 +764,111 @@ int bucket(int n) {
     return b;
 }
 
-Plan plan_for(int n_seqs, int n_groups, int n_heads, int n_kv_heads, int head_dim, int max_new, int max_group, int max_shared, int max_own) {
-    int shared = max_shared > 0 ? bucket(max_shared) : 0, own = bucket(ceil_div(max_own > 0 ? max_own : 1, LLMB_PAGE));
-    int an_sm = head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1;
-    return plan_of(n_seqs, n_groups, n_heads / n_kv_heads, n_kv_heads, SIMT_ROWS, max_new, max_group, shared, own, an_sm * SMS);
+// Into how many parts the shared and the own pages are cut: as many pages a block as make all blocks come to about the blocks that the
+// SMs hold at once, two pages at least.
+Plan plan_for(const Sizes& z) {
+    Plan p;
+    int share = z.n_heads / z.n_kv_heads;
+    int shared = z.max_shared > 0 ? bucket(z.max_shared) : 0, own = bucket(ceil_div(z.max_own > 0 ? z.max_own : 1, LLMB_PAGE));
+    p.tc = z.tc;
+    int rows = p.tc ? TC_ROWS : SIMT_ROWS;
+    long long wave = (long long)SMS * (p.tc ? 2 : z.head_dim <= 64 ? 4 : z.head_dim <= 128 ? 2 : 1);
+    // sequences that bring few rows each would leave a tile of a group to walk many sequences' pages for a few of its rows
+    p.whole = p.tc && (long long)z.max_new * share > 16;
+    p.prefix_tiles = shared > 0 || p.whole ? ceil_div((long long)z.max_group * share, rows) : 0;
+    p.own_tiles = p.whole ? 0 : ceil_div((long long)z.max_new * share, rows);
+    long long prefix = (long long)z.n_groups * p.prefix_tiles * z.n_kv_heads, owns = (long long)z.n_seqs * p.own_tiles * z.n_kv_heads;
+    int walk = shared + (p.whole ? own : 0);
+    long long per = (prefix * walk + owns * own + wave - 1) / wave;
+    if (per < 2) per = 2;
+    p.prefix_splits = p.prefix_tiles > 0 ? ceil_div(walk, per) : 0;
+    p.own_splits = p.own_tiles > 0 ? ceil_div(own, per) : 0;
+    if (p.prefix_splits > MAX_SPLITS) p.prefix_splits = MAX_SPLITS;
+    if (p.own_splits > MAX_SPLITS) p.own_splits = MAX_SPLITS;
+    p.slots = p.prefix_splits + p.own_splits;
+    return p;
 }
 
 template <typename T, int DMAX>
-int launch_simt(const Args& a, long long blocks, cudaStream_t stream) {
+int launch_simt(const Args& a, unsigned blocks, cudaStream_t stream) {
     constexpr size_t smem = simt_floats<DMAX>() * sizeof(float);
     static bool configured = false;
     if (!configured) {
         LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_simt_kernel<T, DMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         configured = true;
     }
-    llmb::launch(prefix_attention_simt_kernel<T, DMAX>, dim3((unsigned)blocks), SIMT_THREADS, smem, stream, true, a);
+    llmb::launch(prefix_attention_simt_kernel<T, DMAX>, dim3(blocks), SIMT_THREADS, smem, stream, true, a);
     return check_launch("prefix_attention_simt");
 }
 
-template <typename T>
-int run(const Args& a, int n_tokens, cudaStream_t stream) {
+template <int HD>
+int launch_tc(const Args& a, int n_pages, unsigned blocks, cudaStream_t stream) {
+    // never less than 80 KB, so that no third block lands on an SM and waits for tensor memory
+    constexpr size_t need = 1024 + (HD / 64) * (Q_PIECE + 4 * KV_PIECE) + 16 * 8 + 16, smem = need < 80 * 1024 ? 80 * 1024 : need;
+    static bool configured = false;
+    if (!configured) {
+        LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        configured = true;
+    }
+    CUtensorMap map_k, map_v;
+    long long cache_rows = (long long)n_pages * a.n_kv_heads * LLMB_PAGE;
+    int code = make_map_2d(&map_k, a.k_cache, cache_rows, HD, HD, 64, LLMB_PAGE);
+    if (!code) code = make_map_2d(&map_v, a.v_cache, cache_rows, HD, HD, 64, LLMB_PAGE);
+    if (code) return code;
+    int* status = status_word();
+    int* status_dev = nullptr;
+    if (status) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status_dev, status, 0));
+    llmb::launch(prefix_attention_tc_kernel<HD>, dim3(blocks), TC_THREADS, smem, stream, true, map_k, map_v, a, status_dev);
+    return check_launch("prefix_attention_tc");
+}
+
+int run(const Args& a, const Plan& p, int dtype, int n_pages, int n_tokens, cudaStream_t stream) {
     long long blocks = (long long)a.n_kv_heads * ((long long)a.n_groups * a.prefix_tiles * a.prefix_splits + (long long)a.n_seqs * a.own_tiles * a.own_splits);
     LLMB_REQUIRE(blocks < (1ll << 31), "prefix_attention: too many blocks");
-    int code = a.head_dim <= 64 ? launch_simt<T, 64>(a, blocks, stream)
-             : a.head_dim <= 128 ? launch_simt<T, 128>(a, blocks, stream) : launch_simt<T, 256>(a, blocks, stream);
+    const bool f32 = dtype == LLMB_DTYPE_F32;
+    int code;
+    if (p.tc) code = a.head_dim == 64 ? launch_tc<64>(a, n_pages, (unsigned)blocks, stream) : launch_tc<128>(a, n_pages, (unsigned)blocks, stream);
+    else if (a.head_dim <= 64) code = f32 ? launch_simt<float, 64>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 64>(a, (unsigned)blocks, stream);
+    else if (a.head_dim <= 128) code = f32 ? launch_simt<float, 128>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 128>(a, (unsigned)blocks, stream);
+    else code = f32 ? launch_simt<float, 256>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 256>(a, (unsigned)blocks, stream);
     if (code || a.slots == 1) return code;
     int rows = n_tokens * a.n_heads;
-    llmb::launch(prefix_attention_join_kernel<T>, dim3((rows + 3) / 4), 128, 0, stream, true, a, rows);
+    if (f32) llmb::launch(prefix_attention_join_kernel<float>, dim3((rows + 3) / 4), 128, 0, stream, true, a, rows);
+    else llmb::launch(prefix_attention_join_kernel<__nv_bfloat16>, dim3((rows + 3) / 4), 128, 0, stream, true, a, rows);
     return check_launch("prefix_attention_join");
 }
 
 }  // namespace
 
+LLMB_EXPORT int llmb_prefix_attention_status() {
+    int* s = status_word();
+    if (!s) return -1;
+    int v = *s;
+    *s = 0;
+    return v;
+}
+
+// Whether the tensor-core kernel takes these operands (rows and caches on 16-byte boundaries, a positive scale).
+LLMB_EXPORT int llmb_prefix_attention_tc_serves(int dtype, int head_dim, int aligned, float scale) {
+    return dtype == LLMB_DTYPE_BF16 && (head_dim == 64 || head_dim == 128) && aligned && scale > 0.f ? 1 : 0;
+}
+
 // Floats of scratch that a call of these sizes needs, and the number of its launches in *kernels.
 LLMB_EXPORT long long llmb_prefix_attention_scratch_floats(int n_tokens, int n_seqs, int n_groups, int n_heads, int n_kv_heads, int head_dim,
-                                                           int max_new, int max_group, int max_shared, int max_own, int* kernels) {
+                                                           int max_new, int max_group, int max_shared, int max_own, int tc, int* kernels) {
+    *kernels = 1;
     if (n_tokens <= 0 || n_seqs <= 0 || n_groups <= 0 || n_kv_heads <= 0 || n_heads < n_kv_heads) return 0;
-    Plan p = plan_for(n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own);
-    *kernels = p.slots > 1 ? 2 : 1;
+    Plan p = plan_for(Sizes{n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own, tc != 0});
+    if (p.slots > 1) ++*kernels;
     return p.slots > 1 ? (long long)n_tokens * n_heads * p.slots * (head_dim + 2) : 0;
 }
 
-LLMB_EXPORT int llmb_prefix_attention(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int* block_table,
+// tc: what llmb_prefix_attention_tc_serves said, 0 to keep to the CUDA cores.
+LLMB_EXPORT int llmb_prefix_attention(const void* q, int q_stride, const void* k_cache, const void* v_cache, int n_pages, const int* block_table,
                                       int table_stride, const int* seq_lens, const int* cu_seqlens, const int* group_first,
                                       const int* group_pages, void* out, int out_stride, float* scratch, long long scratch_floats, int dtype,
                                       int n_tokens, int n_seqs, int n_groups, int n_heads, int n_kv_heads, int head_dim, float scale,
-                                      int max_new, int max_group, int max_shared, int max_own, cudaStream_t stream) {
+                                      int max_new, int max_group, int max_shared, int max_own, int tc, cudaStream_t stream) {
     if (n_tokens == 0 || n_seqs == 0) return LLMB_OK;
     LLMB_REQUIRE(n_tokens > 0 && n_seqs > 0 && n_groups > 0 && n_groups <= n_seqs, "prefix_attention: %d tokens of %d sequences in %d groups",
                  n_tokens, n_seqs, n_groups);
@@ -431,15 +876,21 @@ LLMB_EXPORT int llmb_prefix_attention(const void* q, int q_stride, const void* k
     LLMB_REQUIRE(head_dim > 0 && head_dim <= LLMB_MAX_HEAD_DIM, "prefix_attention: head_dim %d (served: up to %d)", head_dim, LLMB_MAX_HEAD_DIM);
     LLMB_REQUIRE(max_new > 0 && max_group >= max_new && max_shared >= 0 && max_own >= 0, "prefix_attention: bad sizes");
     LLMB_REQUIRE((long long)n_tokens * n_heads < (1ll << 31), "prefix_attention: %d tokens of %d heads", n_tokens, n_heads);
-    Plan p = plan_for(n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own);
+    auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+    LLMB_REQUIRE(!tc || llmb_prefix_attention_tc_serves(dtype, head_dim, aligned(q) && q_stride % 8 == 0 && aligned(out) && out_stride % 8 == 0 &&
+                                                        aligned(k_cache) && aligned(v_cache), scale),
+                 "prefix_attention: the tensor-core kernel does not take these operands");
+    LLMB_REQUIRE(n_pages > 0 && (long long)n_pages * n_kv_heads * LLMB_PAGE < (1ll << 31), "prefix_attention: %d pages", n_pages);
+    Plan p = plan_for(Sizes{n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own, tc != 0});
     long long rows = (long long)n_tokens * n_heads;
-    LLMB_REQUIRE(p.slots == 1 || (scratch != nullptr && scratch_floats >= rows * p.slots * (head_dim + 2)), "prefix_attention: scratch too small");
+    LLMB_REQUIRE(p.slots == 1 || (scratch != nullptr && aligned(scratch) && scratch_floats >= rows * p.slots * (head_dim + 2)),
+                 "prefix_attention: scratch too small");
     int size = dtype == LLMB_DTYPE_F32 ? 4 : 2;
-    bool vectors = (head_dim * size) % 16 == 0 && ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) == 0;
+    bool vectors = (head_dim * size) % 16 == 0 && aligned(k_cache) && aligned(v_cache);
     Args a{q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, out, scratch, scratch + rows * p.slots * head_dim,
            q_stride, out_stride, table_stride, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, scale * LOG2E,
-           p.prefix_tiles, p.prefix_splits, p.own_tiles, p.own_splits, p.slots, vectors ? 1 : 0};
-    return dtype == LLMB_DTYPE_F32 ? run<float>(a, n_tokens, stream) : run<__nv_bfloat16>(a, n_tokens, stream);
+           p.prefix_tiles, p.prefix_splits, p.own_tiles, p.own_splits, p.slots, vectors ? 1 : 0, p.whole ? 1 : 0};
+    return run(a, p, dtype, n_pages, n_tokens, stream);
 }
 
 // the packed doors of the launching entry points (common.cuh)

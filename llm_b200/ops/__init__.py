@@ -1105,7 +1105,7 @@ def check_device_status() -> None:
     reads a word of host memory); meaningful after the stream was synchronised."""
     from .build import _loaded
     for name in ("gemm_tc", "attention_prefill_tc", "routed_experts", "latent_prefill_tc", "latent_attention",
-                 "sigmoid_attention_tc", "diff_attention_tc", "gated_recurrence"):
+                 "sigmoid_attention_tc", "diff_attention_tc", "gated_recurrence", "prefix_attention"):
         if name in _loaded:
             code = getattr(_loaded[name], f"llmb_{name}_status")()
             if code != 0:
@@ -1445,12 +1445,13 @@ def attention_replay_key(step, n_heads: int, n_kv_heads: int, window: int = 0):
 # ----------------------------------------------------------------------------- sequences that share pages
 
 @functools.lru_cache(maxsize=4096)
-def _prefix_scratch(n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own) -> tuple:
-    """(floats of scratch, launches) of a prefix_attention of these sizes."""
+def _prefix_scratch(n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own,
+                    tc) -> tuple:
+    """(floats of scratch, launches) of a prefix_attention of these sizes, on the tensor cores or not."""
     lib, kernels = load_library("prefix_attention"), ctypes.c_int(0)
     lib.llmb_prefix_attention_scratch_floats.restype = ctypes.c_longlong
     floats = lib.llmb_prefix_attention_scratch_floats(*map(_c_int, (n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new,
-                                                                    max_group, max_shared, max_own)), ctypes.byref(kernels))
+                                                                    max_group, max_shared, max_own, tc)), ctypes.byref(kernels))
     return floats, kernels.value
 
 
@@ -1495,13 +1496,15 @@ def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, g
     if n == 0:
         return out
     shared, own = _page_bucket(max_shared), _page_bucket(-(-max_own // PAGE)) * PAGE
-    floats, kernels = _prefix_scratch(n, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, shared, own)
+    aligned = qkv.stride(0) % 8 == 0 and not (qkv.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) & 15
+    tc = int(dtype == torch.bfloat16 and head_dim in (64, 128) and scale > 0 and aligned and not tactics.is_disabled("prefix_attention_tc"))
+    floats, kernels = _prefix_scratch(n, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, shared, own, tc)
     parts = _scratch(qkv.device, "attention", floats)[0] if floats else None
-    _call("prefix_attention", "llmb_prefix_attention", _ptr(qkv), _c_int(qkv.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(block_table),
-          _c_int(block_table.stride(0)), _ptr(seq_lens), _ptr(cu_seqlens), _ptr(group_first), _ptr(group_pages), _ptr(out),
+    _call("prefix_attention", "llmb_prefix_attention", _ptr(qkv), _c_int(qkv.stride(0)), _ptr(k_cache), _ptr(v_cache),
+          _c_int(k_cache.shape[0]), _ptr(block_table), _c_int(block_table.stride(0)), _ptr(seq_lens), _ptr(cu_seqlens), _ptr(group_first), _ptr(group_pages), _ptr(out),
           _c_int(out.stride(0)), _ptr(parts), ctypes.c_longlong(floats), _c_int(_code(dtype)), _c_int(n), _c_int(n_seqs), _c_int(n_groups),
           _c_int(n_heads), _c_int(n_kv_heads), _c_int(head_dim), _c_float(scale), _c_int(max_new), _c_int(max_group), _c_int(shared),
-          _c_int(own), _stream(), kernels=kernels)
+          _c_int(own), _c_int(tc), _stream(), kernels=kernels)
     return out
 
 
