@@ -49,21 +49,31 @@ class LLM:
     def generate(self, prompts, max_tokens: int = DEFAULT_MAX_TOKENS, temperature: float = 0.7,
                  top_k: int = 40, top_p: float = 0.75, min_p: float = 0.25,
                  repeat_penalty: float = 1.1, repeat_last_n: int = 64, seed: int = DEFAULT_SEED,
-                 stop_tokens=None, on_token=None, details: bool = False):
+                 stop_tokens=None, on_token=None, details: bool = False, samples: int = 1, share_prefix: bool = False):
         """Generate for every prompt (a list of token ids each). The i-th
         prompt samples with seed + i. `stop_tokens` defaults to the model's
         eos ids. Returns the generated ids per prompt, or GenerationResult
-        objects with `details=True`."""
+        objects with `details=True`.
+
+        `samples` > 1 draws that many continuations of every prompt, which is prefilled and held
+        once; each prompt's result is then a list of them, sample j of prompt i draws with
+        seed + i * samples + j, and `on_token` gets i * samples + j. `share_prefix`: neighbouring
+        prompts that begin alike (one document, several questions) share what they have in common."""
         if prompts and isinstance(prompts[0], int):
             prompts = [prompts]
+        if samples < 1:
+            raise FormatError(f"{samples} samples of a prompt")
+        count = len(prompts)
+        prompts = [p for p in prompts for _ in range(samples)]
         stops = tuple(self.default_stop_tokens if stop_tokens is None else stop_tokens)
         requests = [GenerationRequest(
             prompt=list(p), max_tokens=max_tokens, stop_tokens=stops,
             params=SamplingParams(temperature, top_k, top_p, min_p, repeat_penalty, repeat_last_n,
                                   (seed + i) & ((1 << 64) - 1)))
             for i, p in enumerate(prompts)]
-        results = _generate(self.engine, requests, on_token=on_token)
-        return results if details else [r.tokens for r in results]
+        results = _generate(self.engine, requests, on_token=on_token, share_prefix=share_prefix or samples > 1)
+        results = results if details else [r.tokens for r in results]
+        return results if samples == 1 else [results[i * samples:(i + 1) * samples] for i in range(count)]
 
 
 def load(model, **options) -> LLM:

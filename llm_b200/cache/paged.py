@@ -17,6 +17,10 @@ serves a batch:
 * `state` tensors [slots, ...] hold what a mixer keeps per sequence at a fixed
   size; a slot's rows are zeroed when the slot is taken.
 
+A slot can be forked: its children share its full pages (a page goes back when its last
+holder is released) and get copies of what is still written: the last, partly filled page,
+the rings of `window` groups and the rows of `state`.
+
 Slots and pages are given back by `release` and reused. Which page holds what is
 decided by the native host library (`csrc/host/cache.cpp`); this class owns the
 tensors and hands out views of them.
@@ -161,6 +165,7 @@ class PagedCache:
                     for request in wanted]
         self.states = tensors_of(states)
         self.block_states = tensors_of(block_states or [])
+        self.forked = False                  # whether slots may share pages
 
     def __del__(self):
         handle = getattr(self, "_handle", None)
@@ -183,6 +188,48 @@ class PagedCache:
         """Give the slot and all of its pages back."""
         native.check(native.lib().llmh_cache_release(self._handle, int(slot)))
 
+    def fork(self, slot: int, count: int = 1) -> list:
+        """`count` new slots that hold what `slot` holds: the same full pages, and copies (queued on the current stream) of the
+        rest. Raises CacheFull before anything is changed."""
+        from .. import ops
+        most = max(int(count), 0) * sum(g.ring_pages if g.window else 1 for g in self.groups)
+        children, copies, n_copies = (c_int * max(int(count), 1))(), (c_int * max(4 * most, 1))(), c_int()
+        native.check(native.lib().llmh_cache_fork(self._handle, int(slot), int(count), children, copies, most, byref(n_copies)))
+        children = list(children)
+        self.forked = True
+        try:
+            flat = copies[:4 * n_copies.value]
+            for g in set(flat[0::4]):
+                mine = [i for i in range(0, len(flat), 4) if flat[i] == g]
+                ops.copy_pages(self._pools(g), [flat[i + 1] for i in mine], [flat[i + 2] for i in mine], [flat[i + 3] for i in mine])
+            states = [s for s in self.states + self.block_states if s is not None]
+            if states:
+                ops.copy_slots(states, [int(slot)] * len(children), children)
+        except BaseException:
+            for child in children:
+                self.release(child)
+            raise
+        return children
+
+    def compact(self) -> int:
+        """Move the held pages of every group to the front of its pool, on the current stream: the first `pool.n_held` pages of a group's
+        tensors are then all that is held (a cache to be saved or moved is one piece). Returns the number of pages moved."""
+        from .. import ops
+        moved = 0
+        for g, group in enumerate(self.groups):
+            n = group.pool.count
+            source, target, count = (c_int * n)(), (c_int * n)(), c_int()
+            native.check(native.lib().llmh_cache_plan_compact(self._handle, g, source, target, byref(count)))
+            if count.value:
+                ops.copy_pages(self._pools(g), source[:count.value], target[:count.value])
+                native.check(native.lib().llmh_cache_apply_moves(self._handle, g, count, source, target))
+                moved += count.value
+        return moved
+
+    def _pools(self, group_index: int) -> list:
+        group = self.groups[group_index]
+        return [t for t in (group.storage, group.keys, group.values if group.values is not group.keys else None) if t is not None]
+
     def reserve(self, slot: int, new_length: int) -> None:
         """Make sure the slot has pages for positions < new_length. Raises
         ContextFull or CacheFull before anything is changed."""
@@ -199,6 +246,12 @@ class PagedCache:
         """Whether new sequences of these final lengths fit beside what is held."""
         lengths = list(lengths)
         return bool(native.lib().llmh_cache_can_hold(self._handle, len(lengths), native.ints(lengths, c_longlong)))
+
+    def can_hold_shared(self, lengths, shared) -> bool:
+        """`can_hold` for sequences whose first shared[i] positions (whole pages) are pages of the sequence before them in the list."""
+        lengths, shared = list(lengths), list(shared)
+        return bool(native.lib().llmh_cache_can_hold_shared(self._handle, len(lengths), native.ints(lengths, c_longlong),
+                                                            native.ints(shared, c_longlong)))
 
     def set_length(self, slot: int, length: int) -> None:
         native.check(native.lib().llmh_cache_set_length(self._handle, int(slot), int(length)))
@@ -251,5 +304,5 @@ class PagedCache:
         return total
 
     def check(self) -> None:
-        """No slot or page lost, held twice, or shared between two slots."""
+        """No slot or page lost, or held by more or other slots than share it."""
         native.check(native.lib().llmh_cache_check(self._handle))

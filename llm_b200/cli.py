@@ -1,13 +1,14 @@
 """Command line of the library, in the manner of MythEclipse/llm's `llm-cli`.
 
-    python -m llm_b200 [--model DIR] [--context 4096] [--max-tokens 256] [--temperature 0.7] ID ...
+    python -m llm_b200 [--model DIR] [--context 4096] [--max-tokens 256] [--temperature 0.7] [--samples 1] ID ...
     python -m llm_b200 bench [-m DIR | --random SHAPE] [-c 4096] [-p 512] [-n 128] [-b 1] [-r 5] [-o json]
     python -m llm_b200 inspect DIR
     python -m llm_b200 random (--shape NAME | --config FILE) --out DIR [--seed S]
 
 The first form completes a prompt given as token ids and prints the generated
 ids and the run's statistics (apps/cli/src/main.rs:55-76: the same flags and
-defaults; text and tokenizers are outside this library). `bench` keeps the
+defaults; text and tokenizers are outside this library); with --samples N that many
+continuations of it, a line each, drawn in one batch whose prompt is prefilled and held once. `bench` keeps the
 flags of apps/cli/src/bench.rs:45-71 (-m, -c, -p, -n, -r, -o with comma lists)
 and its two tests: `pp<N>` times the prefill of N tokens and nothing else,
 `tg<N>` prefills a 16-token prompt and times only the decoding of N tokens
@@ -59,7 +60,7 @@ def main(argv=None) -> int:
 
 def complete(args) -> int:
     model, context, max_tokens, temperature, dtype = None, DEFAULT_CONTEXT, DEFAULT_MAX_TOKENS, 0.7, "bfloat16"
-    seed, prompt = None, []
+    seed, prompt, samples = None, [], 1
     while args:
         a = args.pop(0)
         if a == "--model":
@@ -74,14 +75,26 @@ def complete(args) -> int:
             dtype = _value(args, a)
         elif a == "--seed":
             seed = int(_value(args, a))
+        elif a == "--samples":
+            samples = int(_value(args, a))
         else:
             prompt += _int_list(a, "the prompt")
     if model is None or not prompt:
         raise SystemExit("usage: python -m llm_b200 --model DIR [--context N] [--max-tokens N] "
-                         "[--temperature T] [--dtype bfloat16|float32] [--seed S] TOKEN_ID ...")
+                         "[--temperature T] [--dtype bfloat16|float32] [--seed S] [--samples N] TOKEN_ID ...")
+    if samples < 1:
+        raise SystemExit("--samples needs a number of at least 1")
     import llm_b200
-    llm = llm_b200.LLM(model, dtype=dtype, context=context, batch=1)
+    llm = llm_b200.LLM(model, dtype=dtype, context=context, batch=samples)
     options = {} if seed is None else {"seed": seed}
+    if samples > 1:
+        (results,) = llm.generate([prompt], max_tokens=max_tokens, temperature=temperature, details=True, samples=samples, **options)
+        for result in results:
+            print(" ".join(map(str, result.tokens)))
+        drawn = sum(r.generated_tokens for r in results)
+        print(f"[{results[0].prompt_tokens} prompt tokens, {drawn} generated in {samples} samples, ttft {results[0].ttft_ms:.0f} ms, "
+              f"{sum(r.tokens_per_second for r in results):.1f} tok/s]", file=sys.stderr)
+        return 0
     (result,) = llm.generate([prompt], max_tokens=max_tokens, temperature=temperature, details=True,
                              on_token=lambda i, t: print(t, end=" ", flush=True), **options)
     print()

@@ -46,7 +46,8 @@ int Cache::acquire() {
 void Cache::release(int slot) {
     require_held(slot);
     for (Group& group : groups) {
-        for (int page : group.slot_pages[slot]) group.pool.give_back(page);
+        for (int page : group.slot_pages[slot])
+            if (--group.holders[page] == 0) group.pool.give_back(page);
         group.slot_pages[slot].clear();
     }
     lengths_[slot] = 0;
@@ -69,11 +70,7 @@ void Cache::reserve(int slot, long long new_length) {
     }
     for (size_t g = 0; g < groups.size(); ++g) {
         Group& group = groups[g];
-        for (int i = 0; i < needs[g]; ++i) {
-            int page = group.pool.take();
-            group.table[(size_t)slot * group.ring_pages + group.slot_pages[slot].size()] = page;
-            group.slot_pages[slot].push_back(page);
-        }
+        for (int i = 0; i < needs[g]; ++i) group.give(slot, group.pool.take());
     }
 }
 
@@ -114,13 +111,13 @@ long long Cache::held_tokens() const {
     return total;
 }
 
-// No slot or page lost, held twice, or shared between two slots; the table mirrors the lists.
+// No slot or page lost or held by more slots than it counts; a page that several slots hold is a full one of a `full` group, at the
+// same place in all of them; the table mirrors the lists.
 void Cache::check() const {
     slots.check();
     for (const Group& group : groups) {
         group.pool.check();
-        std::vector<int> owner(group.pool.count(), -1);
-        int owned = 0;
+        std::vector<int> owners(group.pool.count(), 0), place(group.pool.count(), -1);
         for (int slot = 0; slot < max_slots; ++slot) {
             const std::vector<int>& pages = group.slot_pages[slot];
             if (!pages.empty() && !slots.is_held(slot))
@@ -130,15 +127,21 @@ void Cache::check() const {
                 if (page < 0 || page >= group.pool.count() || !group.pool.is_held(page))
                     throw Failure{LLMH_INVARIANT, "slot " + std::to_string(slot) + " lists page " +
                                                       std::to_string(page) + " that is on the free list"};
-                if (owner[page] >= 0)
-                    throw Failure{LLMH_INVARIANT, "page " + std::to_string(page) + " is held by slots " +
-                                                      std::to_string(owner[page]) + " and " + std::to_string(slot)};
+                if (owners[page]++ && (group.window || place[page] != (int)i))
+                    throw Failure{LLMH_INVARIANT, "page " + std::to_string(page) + " is held by slot " + std::to_string(slot) +
+                                                      " and by another that cannot share it"};
                 if (group.table[(size_t)slot * group.ring_pages + i] != page)
                     throw Failure{LLMH_INVARIANT, "the page table of slot " + std::to_string(slot) +
                                                       " does not list its page " + std::to_string(i)};
-                owner[page] = slot;
-                ++owned;
+                place[page] = (int)i;
             }
+        }
+        int owned = 0;
+        for (int page = 0; page < group.pool.count(); ++page) {
+            owned += owners[page] > 0;
+            if (owners[page] != group.holders[page])
+                throw Failure{LLMH_INVARIANT, "page " + std::to_string(page) + " counts " + std::to_string(group.holders[page]) +
+                                                  " holders and has " + std::to_string(owners[page])};
         }
         if (owned != group.pool.n_held())
             throw Failure{LLMH_INVARIANT, std::to_string(group.pool.n_held() - owned) + " pages are held by no slot"};

@@ -43,6 +43,18 @@ public:
         free_.push_back(item);
         std::push_heap(free_.begin(), free_.end(), std::greater<int>());
     }
+    // Held items change places: from[i], held, is free afterwards, and to[i], free, is held.
+    void exchange(const std::vector<int>& from, const std::vector<int>& to) {
+        for (size_t i = 0; i < from.size(); ++i) {
+            if (!is_held(from[i]) || to[i] < 0 || to[i] >= count_ || held_[to[i]])
+                throw Failure{LLMH_INVARIANT, what_ + " " + std::to_string(from[i]) + " cannot move to " + std::to_string(to[i])};
+            held_[from[i]] = 0;
+            held_[to[i]] = 1;
+        }
+        free_.clear();
+        for (int i = 0; i < count_; ++i)
+            if (!held_[i]) free_.push_back(i);
+    }
     // Every item is either free once or held, never both or neither.
     void check() const {
         std::vector<int> seen(count_, 0);

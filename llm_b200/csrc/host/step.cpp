@@ -73,6 +73,7 @@ void check_batch(const Cache& cache, int n, const int* slots, const int* counts,
         }
         long long new_length = (long long)cache.length(slot) + counts[i];
         if (new_length > max_seq_len) throw Failure{LLMH_CONTEXT_FULL, "", new_length, max_seq_len};
+        cache.require_writable(slot, cache.length(slot));
         token_at += counts[i];
         want_at += want_counts[i];
     }

@@ -12,16 +12,22 @@ are those of generate.rs:20-49,129-160. Who is live, who goes on and who leaves
 for which reason is decided by the native host library
 (`csrc/host/generation.cpp`); this module owns slots, steps, sampling, timing
 and callbacks.
+
+With `share_prefix`, neighbouring requests whose prompts begin alike begin together: what they
+have in common is prefilled once and forked (equal prompts as a whole: several samples of one
+prompt), and the steps read the shared pages once.
 """
 from __future__ import annotations
 
 import time
+from array import array
 from ctypes import byref, c_int, c_void_p
 from dataclasses import dataclass, field
 
 import torch
 
 from .. import native
+from ..cache import PAGE
 from ..errors import ContextFull, FormatError
 from ..sampling import BatchSampler, SamplingParams
 from .step import Entry
@@ -59,7 +65,7 @@ def plan_batches(requests, fits, max_batch: int) -> list:
             batches.append(current)
             current, lengths = [], []
         if not fits([final_length]):
-            raise ContextFull(final_length, 0)
+            raise ContextFull(final_length if isinstance(final_length, int) else final_length[0], 0)
         current.append(index)
         lengths.append(final_length)
     if current:
@@ -67,11 +73,80 @@ def plan_batches(requests, fits, max_batch: int) -> list:
     return batches
 
 
-def generate(engine, requests, max_batch: int | None = None, on_token=None, cancel=None) -> list:
+class _Prompts:
+    """How the prompts of neighbouring requests begin alike. `twin[i]`: prompt i is the one before it. The others fall into runs
+    of neighbours that start with the same `common` tokens, whole pages that leave each of them at least a token (0: a prompt alone)."""
+
+    def __init__(self, prompts):
+        self.twin = [i > 0 and prompts[i] == prompts[i - 1] for i in range(len(prompts))]
+        alone = [i for i, t in enumerate(self.twin) if not t]
+        try:
+            tokens = array("i", [t for i in alone for t in prompts[i]])
+        except (OverflowError, TypeError) as error:
+            raise FormatError(f"token ids must be 32-bit integers ({error})") from None
+        n = len(alone)
+        first, common, runs = (c_int * (n + 1))(), (c_int * n)(), c_int()
+        native.check(native.lib().llmh_prompt_runs(n, native.ints(len(prompts[i]) for i in alone),
+                                                   (c_int * len(tokens)).from_buffer(tokens), PAGE, first, common, byref(runs)))
+        self.run, self.common = [0] * len(prompts), [0] * len(prompts)
+        for k in range(runs.value):
+            for j in range(first[k], first[k + 1]):
+                self.run[alone[j]], self.common[alone[j]] = k, common[k]
+        for i, t in enumerate(self.twin):
+            if t:
+                self.run[i], self.common[i] = self.run[i - 1], self.common[i - 1]
+        self.lengths = [len(p) for p in prompts]
+
+    def shared(self, i: int) -> int:
+        """Positions (whole pages) of request i's prompt that are pages of the request before it."""
+        if self.twin[i]:
+            return self.lengths[i] // PAGE * PAGE
+        return self.common[i] if i > 0 and self.run[i] == self.run[i - 1] else 0
+
+
+def _start(engine, reqs, batch, prompts, slots):
+    """Prefill a batch: a slot a request is put into `slots`, and the logits of every prompt's last token are returned. `prompts`: what the
+    prompts have in common (a _Prompts of all requests; `batch` are their indices), or None."""
+    if prompts is None:
+        slots += engine.acquire(len(reqs))
+        return engine.step([Entry(slot, r.prompt, [len(r.prompt) - 1]) for slot, r in zip(slots, reqs)])
+    alone = [b for b, i in enumerate(batch) if b == 0 or not prompts.twin[i]]
+    slot_of, done = {}, {}
+    at = 0
+    while at < len(alone):                               # runs of prompts that begin alike
+        end = at + 1
+        while end < len(alone) and prompts.run[batch[alone[end]]] == prompts.run[batch[alone[at]]]:
+            end += 1
+        common = prompts.common[batch[alone[at]]] if end - at > 1 else 0
+        (first,) = engine.acquire()
+        slots.append(first)
+        members = [first]
+        if common:
+            engine.step([Entry(first, reqs[alone[at]].prompt[:common], [])])
+            members += engine.fork(first, end - at - 1)
+            slots += members[1:]
+        for b, slot in zip(alone[at:end], members):
+            slot_of[b], done[b] = slot, common
+        at = end
+    logits = engine.step([Entry(slot_of[b], reqs[b].prompt[done[b]:], [len(reqs[b].prompt) - done[b] - 1]) for b in alone])
+    rows = []
+    for k, b in enumerate(alone):                        # equal prompts: the rest of them
+        end = alone[k + 1] if k + 1 < len(alone) else len(reqs)
+        rows += [k] * (end - b)
+        if end - b > 1:
+            children = engine.fork(slot_of[b], end - b - 1)
+            slots += children
+            slot_of.update(zip(range(b + 1, end), children))
+    slots[:] = [slot_of[b] for b in range(len(reqs))]
+    return logits if len(alone) == len(reqs) else logits[torch.tensor(rows, dtype=torch.long, device=logits.device)]
+
+
+def generate(engine, requests, max_batch: int | None = None, on_token=None, cancel=None, share_prefix: bool = False) -> list:
     """Run every request to its end and return one GenerationResult each, in
     the order of the requests. `on_token(request index, token)` is called for
     every emitted token; `cancel()` returning True ends all live sequences with
-    reason 'cancelled'."""
+    reason 'cancelled'. `share_prefix`: what the prompts of neighbouring requests have
+    in common at their beginning is prefilled and held once (see the module text)."""
     requests = list(requests)
     context = engine.max_seq_len
     for i, r in enumerate(requests):
@@ -82,9 +157,16 @@ def generate(engine, requests, max_batch: int | None = None, on_token=None, canc
         r.params.check(engine.vocab)
     results = [None] * len(requests)
     final = [(i, min(len(r.prompt) + max(r.max_tokens, 0), context)) for i, r in enumerate(requests)]
-    batches = plan_batches(final, engine.cache.can_hold, max_batch or engine.max_slots)
+    fits, prompts = engine.cache.can_hold, None
+    if share_prefix and requests:
+        prompts = _Prompts([list(r.prompt) for r in requests])
+        final = [(i, (length, prompts.shared(i))) for i, length in final]
+
+        def fits(items):                                 # (a batch's first sequence has nobody to share with)
+            return engine.cache.can_hold_shared([n for n, _ in items], [0] + [shared for _, shared in items[1:]])
+    batches = plan_batches(final, fits, max_batch or engine.max_slots)
     for batch in batches:
-        _run_batch(engine, requests, batch, results, on_token, cancel)
+        _run_batch(engine, requests, batch, results, on_token, cancel, prompts)
     return results
 
 
@@ -141,9 +223,9 @@ class _Schedule:
         return list(self._a[:done.value])
 
 
-def _run_batch(engine, requests, batch, results, on_token, cancel) -> None:
+def _run_batch(engine, requests, batch, results, on_token, cancel, prompts=None) -> None:
     started = time.perf_counter()
-    slots = engine.acquire(len(batch))
+    slots = []
     reqs = [requests[i] for i in batch]
     emitted = [[] for _ in batch]
     reason = ["max_tokens"] * len(batch)
@@ -167,8 +249,7 @@ def _run_batch(engine, requests, batch, results, on_token, cancel) -> None:
 
     try:
         live = schedule.live()
-        logits = engine.step([Entry(slots[b], reqs[b].prompt, [len(reqs[b].prompt) - 1])
-                              for b in live])
+        logits = _start(engine, reqs, batch, prompts, slots)
         prefill_done = None
         while live:
             if cancel is not None and cancel():
@@ -223,10 +304,8 @@ def _run_batch(engine, requests, batch, results, on_token, cancel) -> None:
             if live:
                 logits = next_logits if len(going_rows) == len(onward) else next_logits[going_rows]
     finally:
-        for b in range(len(batch)):
-            if b not in released:
-                engine.release([slots[b]])
-                released.add(b)
+        # (a prefill that failed has taken some of the slots)
+        engine.release([slot for b, slot in enumerate(slots) if b not in released])
     ended = time.perf_counter()
     for b, index in enumerate(batch):
         n = len(emitted[b])

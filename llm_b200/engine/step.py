@@ -22,7 +22,7 @@ import torch
 from .. import native, ops
 from ..cache import PAGE, PagedCache, round_up
 from ..errors import FormatError, LlmError
-from ..parts.base import StepContext
+from ..parts.base import SharedPages, StepContext
 from .workspace import Workspace
 
 
@@ -144,6 +144,11 @@ class Engine:
         for slot in slots:
             self.cache.release(slot)
 
+    def fork(self, slot: int, count: int = 1) -> list:
+        """`count` new sequences that stand where `slot` stands: they share its full pages, and attention reads those once
+        for all of them in steps where they stand next to each other (ops.prefix_attention)."""
+        return self.cache.fork(slot, count)
+
     def length(self, slot: int) -> int:
         return self.cache.length(slot)
 
@@ -223,12 +228,16 @@ class Engine:
                 self._layouts.clear()
             plan = self._layouts[shape] = (offsets, sizes, list(offsets), list(sizes), total.value)
         c_offsets, c_sizes, offsets, sizes, total = plan
-        host = self._host_buffer(total)
+        host = self._host_buffer(total + (2 * self._group_room(batch.n) if self.cache.forked else 0))
         summary = (c_longlong * 5)()
         native.check(lib.llmh_step_pack(cache, *batch.arguments(), host.data_ptr(), host.numel(),
                                         c_offsets, c_sizes, summary))
         n_tokens, decode, max_len = summary[0], bool(summary[2]), summary[3]
         n_groups = len(offsets) - 8
+        groups_at = total
+        sharing = self._groups(batch, host[total:]) if self.cache.forked else None
+        if sharing is not None:
+            total += 2 * self._group_room(batch.n)
 
         def lengths():
             """New tokens and the length before the step, per entry (a replayed step does not ask)."""
@@ -241,23 +250,29 @@ class Engine:
                 return dev[offsets[i]:offsets[i] + sizes[i]]
             n_seqs = batch.n
             counts, starts = lengths()
+            shared = None
+            if sharing is not None:
+                pages_at = groups_at + self._group_room(n_seqs)
+                shared = SharedPages(dev[groups_at:groups_at + sharing[0] + 1], dev[pages_at:pages_at + sharing[0]], *sharing[1:])
             ctx = StepContext(
                 n_tokens=n_tokens, n_seqs=n_seqs, dtype=self.dtype, device=self.device,
                 tok_pos=view(1), tok_seq=view(2), cu_seqlens=view(3), seq_lens=view(4),
                 slot_ids=view(5), seq_order=view(7), cache=self.cache,
                 block_tables=[view(8 + g).view(n_seqs, -1) for g in range(n_groups)],
-                decode=decode, new_counts=counts, starts=starts, max_len=max_len,
+                decode=decode, new_counts=counts, starts=starts, max_len=max_len, sharing=shared,
                 workspace=self.workspace.for_tokens(n_tokens))
             return ctx, view(0), view(6)
 
         logits = None
         graphable = self.use_graphs and decode and all(e.want == [0] for e in entries)
         if graphable:
-            logits = self._replay(len(entries), max_len, host, total, context, device_tokens)
+            logits = self._replay(len(entries), max_len, host, total, context, device_tokens, sharing)
         if logits is None and self.use_records and not graphable:
             step = _HostStep(n_tokens, batch.n, decode, *lengths(), max_len)
             key = self.model.replay_key(step, sizes[6])
             if key is not None and sizes[6] * self.vocab <= MAX_RECORDED_LOGITS:
+                if sharing is not None:
+                    key = (key, sharing)
                 logits = self._run_recorded(key, batch.n, host, total, context, device_tokens)
         if logits is None:
             dev = host[:max(total, 4)].to(self.device, non_blocking=True)
@@ -270,6 +285,25 @@ class Engine:
         native.check(lib.llmh_step_commit(cache, batch.n, batch.slots, batch.counts))
         self.steps_run += 1
         return logits
+
+    @staticmethod
+    def _group_room(n_seqs: int) -> int:
+        """Integers of the step buffer for one array of the sequences' groups, a multiple of 16 bytes."""
+        return (n_seqs + 1 + 3) // 4 * 4
+
+    def _groups(self, batch, room):
+        """Which of the batch's sequences share pages, written behind the step's sections: (groups, and the bounds of
+        SharedPages, numbers of pages as the launches know them: rounded up to a power of two), or None."""
+        first, pages, summary = (c_int * (batch.n + 1))(), (c_int * batch.n)(), (c_int * 5)()
+        native.check(native.lib().llmh_step_groups(self.cache._handle, batch.n, batch.slots, batch.counts, first, pages, summary))
+        n_groups, max_new, max_group, max_shared, max_own = summary
+        if n_groups == 0:
+            return None
+        at = self._group_room(batch.n)
+        room[:n_groups + 1] = torch.tensor(first[:n_groups + 1], dtype=torch.int32)
+        room[at:at + n_groups] = torch.tensor(pages[:n_groups], dtype=torch.int32)
+        widest = min(g.ring_pages for g in self.cache.groups if not g.window)
+        return (n_groups, max_new, max_group, min(ops.page_bucket(max_shared), widest), ops.page_bucket(-(-max_own // PAGE)) * PAGE)
 
     # ------------------------------------------------------------------ recorded passes
 
@@ -345,7 +379,7 @@ class Engine:
 
     # ------------------------------------------------------------------ captured decode steps
 
-    def _replay(self, n_seqs, max_len, host, total, context, device_tokens=None):
+    def _replay(self, n_seqs, max_len, host, total, context, device_tokens=None, sharing=None):
         """Decode steps of one shape (sequences, power-of-two bucket of pages)
         run from a CUDA graph once that shape has been seen GRAPH_AFTER_STEPS
         times, as the decode graphs of apps/engine/src/model.rs:699-729 are
@@ -354,7 +388,7 @@ class Engine:
         by the kernels from one device buffer that is refreshed before the
         replay."""
         pages = max(1, (max_len + PAGE - 1) // PAGE)
-        key = (n_seqs, (pages - 1).bit_length())        # buckets (2^(k-1), 2^k] pages: a context of 2^k pages ends in its bucket
+        key = (n_seqs, (pages - 1).bit_length(), sharing)        # buckets (2^(k-1), 2^k] pages: a context of 2^k pages ends in its bucket
         graph = self._graphs.get(key)
         if graph is None:
             seen = self._graph_seen.get(key, 0) + 1

@@ -53,6 +53,12 @@ _SIGNATURES = {
     "llmh_cache_slot_pages": (c_int, [_P, c_int, c_int, _INTS, c_int, _INTS]),
     "llmh_cache_table_rows": (c_int, [_P, c_int, c_int, _INTS, _P]),
     "llmh_cache_check": (c_int, [_P]),
+    "llmh_cache_fork": (c_int, [_P, c_int, c_int, _INTS, _INTS, c_int, _INTS]),
+    "llmh_cache_can_hold_shared": (c_int, [_P, c_int, _LONGS, _LONGS]),
+    "llmh_cache_plan_compact": (c_int, [_P, c_int, _INTS, _INTS, _INTS]),
+    "llmh_cache_apply_moves": (c_int, [_P, c_int, c_int, _INTS, _INTS]),
+    "llmh_step_groups": (c_int, [_P, c_int, _INTS, _INTS, _INTS, _INTS, _INTS]),
+    "llmh_prompt_runs": (c_int, [c_int, _INTS, _INTS, c_int, _INTS, _INTS, _INTS]),
     "llmh_step_check": (c_int, [_P, *_BATCH, c_int, c_int]),
     "llmh_step_reserve": (c_int, [_P, c_int, _INTS, _INTS]),
     "llmh_step_begin": (c_int, [_P, *_BATCH, c_int, c_int]),

@@ -1455,9 +1455,14 @@ def _prefix_scratch(n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, m
     return floats, kernels.value
 
 
-def _page_bucket(pages: int) -> int:
+def page_bucket(pages: int) -> int:
     """The least power of two that is no less than `pages` (0 for 0): what a launch depends on of a number of pages."""
     return 1 << (pages - 1).bit_length() if pages > 0 else 0
+
+
+def prefix_attention_pays(max_shared: int) -> bool:
+    """Whether a step whose sequences share pages reads them once for each group (`prefix_attention`) or for each sequence (`attention`)."""
+    return max_shared > 0 and not tactics.is_disabled("prefix_attention")
 
 
 def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, n_heads, n_kv_heads, head_dim,
@@ -1495,7 +1500,7 @@ def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, g
         out = torch.empty((n, n_heads * head_dim), dtype=dtype, device=qkv.device)
     if n == 0:
         return out
-    shared, own = _page_bucket(max_shared), _page_bucket(-(-max_own // PAGE)) * PAGE
+    shared, own = page_bucket(max_shared), page_bucket(-(-max_own // PAGE)) * PAGE
     aligned = qkv.stride(0) % 8 == 0 and not (qkv.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) & 15
     tc = int(dtype == torch.bfloat16 and head_dim in (64, 128) and scale > 0 and aligned and not tactics.is_disabled("prefix_attention_tc"))
     floats, kernels = _prefix_scratch(n, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, shared, own, tc)
@@ -2019,7 +2024,7 @@ def required_libraries() -> list:
             "attention_decode", "attention_prefill", "attention_prefill_tc", "sampling"]
 
 
-__all__ = ["PAGE", "GLU_BLOCK", "glu_fusable", "embed", "scale_", "random_normal_", "begin_recording", "end_recording", "RecordedPass", "StepScope", "scratch_generation", "Emit", "FoldedNorm", "RopeWrite", "cast_sumsq", "SUMSQ_LD", "rmsnorm", "swiglu", "rope_cache_write", "linear", "attention", "prefix_attention", "copy_pages", "copy_slots",
+__all__ = ["PAGE", "GLU_BLOCK", "glu_fusable", "embed", "scale_", "random_normal_", "begin_recording", "end_recording", "RecordedPass", "StepScope", "scratch_generation", "Emit", "FoldedNorm", "RopeWrite", "cast_sumsq", "SUMSQ_LD", "rmsnorm", "swiglu", "rope_cache_write", "linear", "attention", "prefix_attention", "prefix_attention_pays", "page_bucket", "copy_pages", "copy_slots",
            "softcap_", "add_rows_", "conv_rope_cache_write", "diff_attention", "tanh_norm", "norm_rope_cache_write",
            "sigmoid_attention", "gated_recurrence", "state_space", "attention_replay_key", "layernorm", "input_conv", "output_norm_add_", "forget_recurrence",
            "latent_write", "head_products", "latent_attention", "latent_prefill", "attention_decode_splits", "sigmoid_attention_replay_key", "sigmoid_decode_splits", "sigmoid_mixed_heads", "sigmoid_mixed_elements",

@@ -17,7 +17,7 @@ class AttentionMixer(Mixer):
     scale, the window, the biases and the position encoding as parameters."""
     graph_safe = True
     emits = True
-    libraries = ("elementwise", "gemm_simt", "gemm_skinny", "gemm_tc", "attention_generic", "attention_decode", "attention_decode_window", "attention_prefill", "attention_prefill_tc")
+    libraries = ("elementwise", "gemm_simt", "gemm_skinny", "gemm_tc", "attention_generic", "attention_decode", "attention_decode_window", "attention_prefill", "attention_prefill_tc", "prefix_attention")
 
     def __init__(self, spec):
         self.spec = spec
@@ -118,12 +118,18 @@ class AttentionMixer(Mixer):
             ops.rope_cache_write(qkv, angles, ctx.tok_pos, ctx.tok_seq, table, ring, keys, values, s.n_heads,
                                  s.n_kv_heads, s.head_dim, interleaved=interleaved,
                                  write_cache=(entry == cache_entry))
-        mixed = ops.attention(qkv, keys, values, table, ring, ctx.tok_pos, ctx.tok_seq, s.n_heads,
-                              s.n_kv_heads, s.head_dim, s.scale, s.window, out=ctx.scratch("mixed", (n, self.q_width), h.dtype),
-                              decode=ctx.decode,
-                              seq_lens=ctx.seq_lens, max_len=ctx.max_len,
-                              cu_seqlens=ctx.cu_seqlens, max_new=max(ctx.new_counts),
-                              seq_order=ctx.seq_order)
+        mixed = ctx.scratch("mixed", (n, self.q_width), h.dtype)
+        share = ctx.sharing if s.window == 0 else None
+        if share is not None and ops.prefix_attention_pays(share.max_shared):
+            mixed = ops.prefix_attention(qkv, keys, values, table, ctx.seq_lens, ctx.cu_seqlens, share.group_first, share.group_pages,
+                                         s.n_heads, s.n_kv_heads, s.head_dim, s.scale, max_new=share.max_new, max_group=share.max_group,
+                                         max_shared=share.max_shared, max_own=share.max_own, out=mixed)
+        else:
+            mixed = ops.attention(qkv, keys, values, table, ring, ctx.tok_pos, ctx.tok_seq, s.n_heads,
+                                  s.n_kv_heads, s.head_dim, s.scale, s.window, out=mixed, decode=ctx.decode,
+                                  seq_lens=ctx.seq_lens, max_len=ctx.max_len,
+                                  cu_seqlens=ctx.cu_seqlens, max_new=max(ctx.new_counts),
+                                  seq_order=ctx.seq_order)
         ops.linear(mixed, self.w_o, self.b_o, residual=residual, emit=emit)
 
 

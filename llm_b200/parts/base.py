@@ -24,6 +24,18 @@ from ..errors import Unsupported
 
 
 @dataclass
+class SharedPages:
+    """The groups of a step's sequences that share the first pages of their tables in the cache's `full` groups (ops.prefix_attention):
+    device arrays, and upper bounds for the launches."""
+    group_first: torch.Tensor      # [G + 1] first sequence of each group
+    group_pages: torch.Tensor      # [G] pages that its members share
+    max_new: int                   # most new tokens of a sequence,
+    max_group: int                 # of a group
+    max_shared: int                # most pages that a group shares
+    max_own: int                   # most positions of a sequence behind them
+
+
+@dataclass
 class StepContext:
     """One step's batch as the parts see it. Device tensors are int32."""
     n_tokens: int                  # T: tokens of this step, packed sequence after sequence
@@ -43,6 +55,7 @@ class StepContext:
     max_len: int                   # host: longest sequence after this step
     workspace: object = None       # engine.workspace.Views of this step, or None
     seq_order: torch.Tensor = None # [B] the sequences by falling length (work lists start the longest first)
+    sharing: SharedPages = None    # which sequences share pages, or None: every part may read each sequence's pages for itself
     extras: dict = field(default_factory=dict)
 
     def scratch(self, name: str, shape=None, dtype=None):

@@ -174,6 +174,37 @@ def attention(qkv, k_cache, v_cache, block_table, ring_pages, tok_pos, tok_seq, 
     return result.to(qkv.dtype)
 
 
+def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, n_heads, n_kv_heads, head_dim,
+                     scale, *, max_new, max_group, max_shared, max_own, out=None):
+    """The groups say what is stored once, nothing of the result."""
+    first, pages, width = group_first.tolist(), group_pages.tolist(), block_table.shape[1]
+    assert first[0] == 0 and first[-1] == seq_lens.numel() and max(pages) <= max_shared <= width
+    for g, shared in enumerate(pages):
+        for s in range(first[g], first[g + 1]):
+            assert block_table[s, :shared].tolist() == block_table[first[g], :shared].tolist()
+            assert int(seq_lens[s]) - shared * PAGE <= max_own and int(cu_seqlens[s + 1] - cu_seqlens[s]) <= max_new
+            assert int(cu_seqlens[s + 1] - cu_seqlens[s]) + shared * PAGE <= int(seq_lens[s])
+        assert int(cu_seqlens[first[g + 1]] - cu_seqlens[first[g]]) <= max_group
+    new = (cu_seqlens[1:] - cu_seqlens[:-1]).tolist()
+    tok_seq = torch.tensor([s for s, n in enumerate(new) for _ in range(n)], dtype=torch.int32, device=qkv.device)
+    tok_pos = torch.tensor([int(seq_lens[s]) - n + t for s, n in enumerate(new) for t in range(n)], dtype=torch.int32, device=qkv.device)
+    return attention(qkv, k_cache, v_cache, block_table, width, tok_pos, tok_seq, n_heads, n_kv_heads, head_dim, scale, out=out)
+
+
+def copy_pages(pools, source, target, rows=None):
+    assert len(set(target)) == len(target) and not set(source) & set(target)
+    for pool in [pools] if isinstance(pools, torch.Tensor) else pools:
+        for s, t, r in zip(source, target, rows or [PAGE] * len(source)):
+            pool[..., t, :, :r, :] = pool[..., s, :, :r, :]
+
+
+def copy_slots(states, source, target):
+    assert len(set(target)) == len(target) and not set(source) & set(target)
+    for state in states:
+        for s, t in zip(source, target):
+            state[t] = state[s]
+
+
 def tanh_norm(x, alpha, gain, bias, out_dtype, rows=None, out=None, second=None):
     if rows is not None:
         x = x[rows.long()]
@@ -899,7 +930,7 @@ def sample_rows(logits, params, iparams, recent, recent_len, rng_state, out, sta
 
 
 
-OPS = {"embed": embed, "scale_": scale_, "cast_sumsq": cast_sumsq, "rmsnorm": rmsnorm, "swiglu": swiglu, "linear": linear,
+OPS = {"prefix_attention": prefix_attention, "copy_pages": copy_pages, "copy_slots": copy_slots, "embed": embed, "scale_": scale_, "cast_sumsq": cast_sumsq, "rmsnorm": rmsnorm, "swiglu": swiglu, "linear": linear,
        "rope_cache_write": rope_cache_write, "attention": attention, "argmax_rows": argmax_rows,
        "softcap_": softcap_, "add_rows_": add_rows_, "conv_rope_cache_write": conv_rope_cache_write,
        "diff_attention": diff_attention, "tanh_norm": tanh_norm, "norm_rope_cache_write": norm_rope_cache_write,
