@@ -15,6 +15,7 @@
 // bounds (most tokens of a group, most pages) and a block beyond the real work leaves. A key beyond a row's position has no
 // weight whatever is stored there, and values beyond a tile's last position are taken for zero, so that what an earlier sequence
 // left in a page (infinities and NaN too) does not reach a result. A row that sees no key is zero.
+#include "mma.cuh"
 #include "tc.cuh"
 
 using namespace llmb;
@@ -25,6 +26,7 @@ LLMB_DEFINE_LAST_ERROR(llmb_prefix_attention)
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int MAX_SPLITS = 64, MAX_SLOTS = 2 * MAX_SPLITS;      // parts of the shared pages, of own ones; of a row
 
 struct Args {
     const void* q;
@@ -325,8 +327,13 @@ __global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(con
 //
 // A walk is the shared pages, or a sequence's own ones, or both: behind the shared pages those of each sequence that the tile has rows of,
 // whose rows alone see them (`whole`).
+//
+// Items of 16 rows or fewer (a sequence's own pages in a decode step; the shared pages of a few samples) are bound by reading their
+// pages and would leave seven eighths of the tile empty: warp 0 keeps a ring of pages in flight and warps 2 to 5 take 16 of
+// a page's 64 keys each with mma.sync.m16n8k16, keep a maximum, a sum and weighted values of their own and are merged at the end.
 
 constexpr int TC_ROWS = 128, TC_THREADS = 224;
+constexpr int FEW_ROWS = 16;                      // rows of an item that go through mma.sync
 constexpr int Q_PIECE = TC_ROWS * 64 * 2;         // the tile's rows, 64 columns of the head: 16 KB
 constexpr int KV_PIECE = LLMB_PAGE * 64 * 2;      // a page, 64 columns of the head: 8 KB
 // tensor memory: two buffers of scores (64 columns of 32-bit values, the weights over the first 32), O beside them
@@ -388,10 +395,232 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         : "memory");
 }
 
+// where element (row, col) of a page lies in shared memory: pieces of 64 columns, 16-byte chunks swizzled by the row
+__device__ __forceinline__ const unsigned char* swizzled(const unsigned char* page, int row, int col) {
+    return page + (col >> 6) * KV_PIECE + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4);
+}
+
+template <int HD> struct Ring {                              // of the items of few rows
+    static constexpr int STAGE = 2 * (HD / 64) * KV_PIECE;   // a page's keys and values
+    static constexpr int STAGES = HD == 64 ? 5 : 3;          // two blocks an SM: 160 and 192 KB in flight
+};
+template <int HD>
+__host__ __device__ constexpr int tile_bytes() {
+    return (HD / 64) * (Q_PIECE + 4 * KV_PIECE) > Ring<HD>::STAGE * Ring<HD>::STAGES ? (HD / 64) * (Q_PIECE + 4 * KV_PIECE)
+                                                                                  : Ring<HD>::STAGE * Ring<HD>::STAGES;
+}
+
+// An item of up to 16 rows over the pages [page_begin, page_end) of one table. Rows g and g + 8 of the mma tile are this lane's.
+template <int HD>
+__device__ __forceinline__ void few_rows(const Args& a, const Item& w, const CUtensorMap& map_k, const CUtensorMap& map_v, unsigned char* base,
+                                         uint64_t* bars, volatile int* abort_flag, int* status) {
+    constexpr int STAGES = Ring<HD>::STAGES, STAGE = Ring<HD>::STAGE, PIECES = HD / 64;
+    uint64_t* full = bars;
+    uint64_t* empty = bars + STAGES;
+    const int warp = warp_index(), lane = threadIdx.x & 31, share = a.n_heads / a.n_kv_heads;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(smem_u32(&full[i]), 1);
+            mbar_init(smem_u32(&empty[i]), 4);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    griddep_launch();
+    griddep_wait();
+    const bool own = w.slot >= a.prefix_splits;
+    const int last_token = w.first_token + (w.n_rows - 1) / share;
+    // the last position that a row sees of these pages
+    int limit = w.page_end * LLMB_PAGE - 1;
+    if (own) limit = min(limit, a.seq_lens[w.seq_first] - a.cu_seqlens[w.seq_first + 1] + last_token);
+    const int n_pages = min(w.page_end, limit < 0 ? 0 : limit / LLMB_PAGE + 1) - w.page_begin;
+    bool ok = true;
+    if (warp == 0) {
+        const int* pages = a.block_table + (size_t)w.seq_first * a.table_stride + w.page_begin;
+        for (int i = 0; i < n_pages; ++i) {
+            int stage = i % STAGES;
+            int row = (pages[i] * a.n_kv_heads + w.kv_head) * LLMB_PAGE;
+            if (i >= STAGES && !mbar_wait_warp(smem_u32(&empty[stage]), (i / STAGES - 1) & 1, abort_flag, status, 21)) break;
+            if (elect_one()) {
+                uint32_t bar = smem_u32(&full[stage]);
+                mbar_expect_tx(bar, STAGE);
+                for (int h = 0; h < PIECES; ++h) {
+                    tma_load_2d(smem_u32(base + stage * STAGE + h * KV_PIECE), &map_k, bar, h * 64, row);
+                    tma_load_2d(smem_u32(base + stage * STAGE + (PIECES + h) * KV_PIECE), &map_v, bar, h * 64, row);
+                }
+            }
+            __syncwarp();
+        }
+    }
+    const int g = lane >> 2, t = lane & 3, part = warp - 2;          // warps 2 .. 5: 16 keys of every page
+    float acc[HD / 8][4], run_max[2] = {-INFINITY, -INFINITY}, run_sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+    if (part >= 0 && part < 4) {
+        uint32_t qa[HD / 16][4];
+        int pos[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            int r = g + half * 8;
+            bool valid = r < w.n_rows;
+            int token = w.first_token + (valid ? r : 0) / share, head = w.kv_head * share + (valid ? r : 0) % share;
+            pos[half] = valid ? position_of(a, w, token) : -1;
+            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + (size_t)token * a.q_stride + (size_t)head * HD;
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks) {
+                qa[ks][half] = valid ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 2 * t) : 0u;
+                qa[ks][2 + half] = valid ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8 + 2 * t) : 0u;
+            }
+        }
+        for (int i = 0; i < n_pages; ++i) {
+            int stage = i % STAGES;
+            ok = mbar_wait_warp(smem_u32(&full[stage]), (i / STAGES) & 1, abort_flag, status, 22);
+            if (!ok) break;
+            const unsigned char* ks_ = base + stage * STAGE;
+            const unsigned char* vs_ = ks_ + PIECES * KV_PIECE;
+            const int key0 = (w.page_begin + i) * LLMB_PAGE + part * 16;
+            if (key0 <= limit) {
+                float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    uint32_t b[4];
+                    ldmatrix_x4(b, swizzled(ks_, part * 16 + (lane >> 4) * 8 + (lane & 7), ks * 16 + ((lane >> 3) & 1) * 8));
+                    mma_bf16(s0, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[0], b[1]);
+                    mma_bf16(s1, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[2], b[3]);
+                }
+                // this lane's keys: key0 + 2t, +1 (s0), +8, +9 (s1); elements 0, 1 of row g, 2, 3 of row g + 8
+                uint32_t pa[4];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float v[4] = {s0[2 * half], s0[2 * half + 1], s1[2 * half], s1[2 * half + 1]};
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        int key = key0 + 2 * t + (j & 1) + (j >> 1) * 8;
+                        v[j] = key <= pos[half] ? v[j] * a.scale_log2 : -INFINITY;
+                        top = fmaxf(top, v[j]);
+                    }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    float new_max = fmaxf(run_max[half], top), against = new_max == -INFINITY ? 0.f : new_max;
+                    float alpha = fast_exp2(run_max[half] - against);
+                    float p[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[j] = fast_exp2(v[j] - against);
+                    run_sum[half] = run_sum[half] * alpha + ((p[0] + p[1]) + (p[2] + p[3]));       // of this lane's keys
+                    run_max[half] = new_max;
+                    pa[half] = pack_bf16(p[0], p[1]);
+                    pa[2 + half] = pack_bf16(p[2], p[3]);
+#pragma unroll
+                    for (int n = 0; n < HD / 8; ++n) {
+                        acc[n][2 * half] *= alpha;
+                        acc[n][2 * half + 1] *= alpha;
+                    }
+                }
+                const bool cut = key0 + 15 > limit;          // values behind the last position are whatever the page held: zero here
+                const int left = limit + 1 - key0 - 2 * t;   // of this lane's keys 0, 1, 8, 9
+                const uint32_t keep_low = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+                const uint32_t keep_high = left >= 10 ? 0xffffffffu : left == 9 ? 0xffffu : 0u;
+#pragma unroll
+                for (int n = 0; n < HD / 8; n += 2) {
+                    uint32_t b[4];
+                    ldmatrix_x4_trans(b, swizzled(vs_, part * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), (n + (lane >> 4)) * 8));
+                    if (cut) {
+                        b[0] &= keep_low;
+                        b[1] &= keep_high;
+                        b[2] &= keep_low;
+                        b[3] &= keep_high;
+                    }
+                    mma_bf16(acc[n], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
+                    mma_bf16(acc[n + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&empty[stage]));
+        }
+    }
+    __syncthreads();                                         // every page has been read: its room is free
+    if (*abort_flag) {                                       // a wait ran out: copies in flight get their time before the block leaves
+        for (int i = 0; i < 100; ++i) __nanosleep(10000);
+        return;
+    }
+    constexpr int LD = HD + 8;                               // (rows of the merge in different banks)
+    float* merge_acc = reinterpret_cast<float*>(base);       // [4][16][LD]
+    float* merge_max = merge_acc + 4 * FEW_ROWS * LD;        // [4][16], and the sums
+    float* merge_sum = merge_max + 4 * FEW_ROWS;
+    if (part >= 0 && part < 4) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            run_sum[half] += __shfl_xor_sync(0xffffffffu, run_sum[half], 1);
+            run_sum[half] += __shfl_xor_sync(0xffffffffu, run_sum[half], 2);
+            int r = part * FEW_ROWS + g + half * 8;
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n)
+                *reinterpret_cast<float2*>(merge_acc + r * LD + n * 8 + 2 * t) = make_float2(acc[n][2 * half], acc[n][2 * half + 1]);
+            if (t == 0) {
+                merge_max[r] = run_max[half];
+                merge_sum[r] = run_sum[half];
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < w.n_rows * (HD / 4); i += TC_THREADS) {
+        int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = fmaxf(m, merge_max[k * FEW_ROWS + r]);
+        float against = m == -INFINITY ? 0.f : m, sum = 0.f;
+        float4 value = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float weight = fast_exp2(merge_max[k * FEW_ROWS + r] - against);
+            float4 x = *reinterpret_cast<const float4*>(merge_acc + (k * FEW_ROWS + r) * LD + d);
+            value.x = fmaf(x.x, weight, value.x);
+            value.y = fmaf(x.y, weight, value.y);
+            value.z = fmaf(x.z, weight, value.z);
+            value.w = fmaf(x.w, weight, value.w);
+            sum += merge_sum[k * FEW_ROWS + r] * weight;
+        }
+        int token = w.first_token + r / share, head = w.kv_head * share + r % share;
+        if (a.slots == 1) {
+            float inv = sum != 0.f ? 1.f / sum : 0.f;
+            uint2 packed = make_uint2(pack2(value.x * inv, value.y * inv), pack2(value.z * inv, value.w * inv));
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD + d) = packed;
+        } else {
+            size_t slot = ((size_t)token * a.n_heads + head) * a.slots + w.slot;
+            if (sum != 0.f) *reinterpret_cast<float4*>(a.acc + slot * HD + d) = value;
+            if (d == 0) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(m, sum);
+        }
+    }
+}
+
+// The arrays that say which sequences there are, in shared memory (one round of loads) where there is room.
+constexpr int STAGED_SEQS = 128;
+struct Staged {
+    int seq_lens[STAGED_SEQS], cu_seqlens[STAGED_SEQS + 1], group_first[STAGED_SEQS + 1], group_pages[STAGED_SEQS];
+};
+__device__ __forceinline__ void stage_arrays(Args& a, Staged& s) {
+    if (a.n_seqs > STAGED_SEQS) return;
+    for (int i = threadIdx.x; i <= a.n_seqs; i += blockDim.x) {
+        s.cu_seqlens[i] = a.cu_seqlens[i];
+        if (i < a.n_seqs) s.seq_lens[i] = a.seq_lens[i];
+        if (i <= a.n_groups) s.group_first[i] = a.group_first[i];
+        if (i < a.n_groups) s.group_pages[i] = a.group_pages[i];
+    }
+    __syncthreads();
+    a.seq_lens = s.seq_lens;
+    a.cu_seqlens = s.cu_seqlens;
+    a.group_first = s.group_first;
+    a.group_pages = s.group_pages;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(TC_THREADS, 2)
 prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                           const __grid_constant__ Args a, int* status) {
+                           const __grid_constant__ Args args, int* status) {
     constexpr int PIECES = HD / 64;
     constexpr int KV_BYTES = PIECES * KV_PIECE;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -399,7 +628,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     unsigned char* q_tile = base;
     unsigned char* k_tile = base + PIECES * Q_PIECE;
     unsigned char* v_tile = k_tile + 2 * KV_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(v_tile + 2 * KV_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + tile_bytes<HD>());
     uint64_t* q_full = bars;                  // the queries are in shared memory
     uint64_t* k_full = bars + 1;              // [2]
     uint64_t* k_empty = bars + 3;             // [2]
@@ -411,10 +640,15 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    griddep_launch();
-    griddep_wait();
+    __shared__ Staged staged;
+    Args a = args;
+    stage_arrays(a, staged);                                 // (lengths, groups and tables are not written by the kernels of a step)
     Item w;
     if (!item_of(a, blockIdx.x, w)) return;                  // uniform for the block, here and below: nothing is allocated yet
+    if (!a.whole && w.n_rows <= FEW_ROWS) {
+        if (w.n_rows > 0 && w.tile == 0) few_rows<HD>(a, w, map_k, map_v, base, bars, abort_flag, status);
+        return;
+    }
     const int share = a.n_heads / a.n_kv_heads;
     const int row0 = w.tile * TC_ROWS, n_rows = min(TC_ROWS, w.n_rows - row0);
     if (n_rows <= 0) return;
@@ -462,6 +696,9 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // Tensor memory is taken when the kernel in front is done with it, and the next kernel may take some only when this one has it: two
+    // that wait for one another's would stand still.
+    griddep_wait();
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
@@ -470,6 +707,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
+    griddep_launch();
     uint32_t tmem_base = *tmem_slot;
 
     if (warp == 0 || warp == 6) {
@@ -573,6 +811,11 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
             if (!ok) break;
             __syncwarp();
             tcgen05_fence_after();
+            const bool cut = key0 + LLMB_PAGE - 1 > limit;
+            if (quarter * 32 >= n_rows && !cut) {            // a warp without rows: its lanes' weights reach nobody's result
+                mbar_arrive(smem_u32(&p_full[b]));
+                continue;
+            }
             bool whole = key0 + LLMB_PAGE - 1 <= pos;        // no key of the page is hidden from this row
             uint32_t s_addr = lane_addr + S_COL + b * LLMB_PAGE;
             uint32_t ra[32], rb[32];
@@ -629,7 +872,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
                     }
                 }
             }
-            if (key0 + LLMB_PAGE - 1 > limit) {              // values behind the last position are whatever a page held: zero here
+            if (cut) {                                       // values behind the last position are whatever a page held: zero here
                 ok = mbar_wait(smem_u32(&v_full[b]), (kb >> 1) & 1, abort_flag, status, 20);
                 if (!ok) break;
                 int first = limit + 1 - key0;                // (a row of a piece is 128 bytes, its swizzle stays inside)
@@ -644,7 +887,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
             mbar_arrive(smem_u32(&p_full[b]));
         }
         if (ok && n_blocks > 0) ok = mbar_wait(smem_u32(o_full), (n_blocks - 1) & 1, abort_flag, status, 19);
-        if (ok) {
+        if (ok && quarter * 32 < n_rows) {
             __syncwarp();
             tcgen05_fence_after();
             const bool valid = row < n_rows;
@@ -699,46 +942,101 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 
 // ------------------------------------------------------------------------------------------------ the parts joined
 //
-// A warp a row: each lane reads one part's maximum and sum, the weights are shared by shuffles, and the lanes take columns.
-template <typename T>
-__global__ void __launch_bounds__(128) prefix_attention_join_kernel(const __grid_constant__ Args a, int n_rows) {
+// WARPS warps a row: each reads all the maxima and sums, a lane a part, and takes every WARPS-th part, several of them in flight; their
+// sums are added in order. With one warp that read part after part the join of 34 parts of 512 rows took 25 us, more than the parts.
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(256) prefix_attention_join_kernel(const __grid_constant__ Args a, int n_rows) {
+    constexpr int ROWS = 8 / WARPS, CHUNKS = LLMB_MAX_HEAD_DIM / 128, AHEAD = 4;
+    __shared__ float4 shared_value[8][LLMB_MAX_HEAD_DIM / 4];
     griddep_launch();
     griddep_wait();
-    int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (row >= n_rows) return;
-    const int D = a.head_dim;
-    const float* acc = behind_wait(a.acc) + (size_t)row * a.slots * D;
-    const float* stats = behind_wait(a.stats) + (size_t)row * a.slots * 2;
-    float m = -INFINITY;
-    for (int s = lane; s < a.slots; s += 32) m = fmaxf(m, stats[s * 2]);
-    m = warp_max(m);
-    float against = m == -INFINITY ? 0.f : m, sum = 0.f;
-    constexpr int COLS = LLMB_MAX_HEAD_DIM / 32;
-    float value[COLS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp % WARPS;
+    const int row = blockIdx.x * ROWS + warp / WARPS;
+    const int D = a.head_dim, slots = a.slots, width = (D + 3) / 4;
+    const bool valid = row < n_rows, vectors = D % 4 == 0;
+    float4 value[CHUNKS];
+    float sum = 0.f;
 #pragma unroll
-    for (int c = 0; c < COLS; ++c) value[c] = 0.f;
-    for (int s0 = 0; s0 < a.slots; s0 += 32) {
-        float weight = 0.f;
-        if (s0 + lane < a.slots) {
-            float l = stats[(s0 + lane) * 2 + 1];
-            weight = l != 0.f ? exp2f(stats[(s0 + lane) * 2] - against) : 0.f;
-            sum += l * weight;
+    for (int c = 0; c < CHUNKS; ++c) value[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (valid) {
+        const float* acc = behind_wait(a.acc) + (size_t)row * slots * D;
+        const float2* stats = reinterpret_cast<const float2*>(behind_wait(a.stats)) + (size_t)row * slots;
+        static_assert(MAX_SLOTS <= 128, "four parts a lane");
+        float2 part[4];
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            part[k] = lane + 32 * k < slots ? stats[lane + 32 * k] : make_float2(-INFINITY, 0.f);
+            m = fmaxf(m, part[k].x);
         }
-        int count = min(32, a.slots - s0);
-        for (int s = 0; s < count; ++s) {
-            float part = __shfl_sync(0xffffffffu, weight, s);
-            if (part == 0.f) continue;                             // a part without keys has written no values
+        m = warp_max(m);
+        const float against = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int c = 0; c < COLS; ++c)
-                if (c * 32 + lane < D) value[c] = fmaf(part, acc[(size_t)(s0 + s) * D + c * 32 + lane], value[c]);
+        for (int k = 0; k < 4; ++k) {
+            // (a part without keys has written no values; a sum that is not a number stays one)
+            part[k].x = part[k].y != 0.f ? exp2f(part[k].x - against) : 0.f;
+            sum += part[k].x * part[k].y;
+        }
+        sum = warp_sum(sum);
+        auto at = [&](int s, int c) {
+            int col = (c * 32 + lane) * 4;
+            const float* from = acc + (size_t)s * D + col;
+            if (vectors) return col < D ? *reinterpret_cast<const float4*>(from) : make_float4(0.f, 0.f, 0.f, 0.f);
+            return make_float4(col < D ? from[0] : 0.f, col + 1 < D ? from[1] : 0.f, col + 2 < D ? from[2] : 0.f, col + 3 < D ? from[3] : 0.f);
+        };
+        for (int s0 = mine; s0 < slots; s0 += WARPS * AHEAD) {
+            float weight[AHEAD];
+            float4 x[AHEAD][CHUNKS];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                int s = s0 + j * WARPS, k = s >> 5;
+                float w = k == 0 ? part[0].x : k == 1 ? part[1].x : k == 2 ? part[2].x : part[3].x;
+                weight[j] = __shfl_sync(0xffffffffu, w, s & 31);
+                if (s >= slots) weight[j] = 0.f;
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c)
+                    x[j][c] = weight[j] != 0.f && c * 128 < D ? at(s, c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) {
+                    value[c].x = fmaf(weight[j], x[j][c].x, value[c].x);
+                    value[c].y = fmaf(weight[j], x[j][c].y, value[c].y);
+                    value[c].z = fmaf(weight[j], x[j][c].z, value[c].z);
+                    value[c].w = fmaf(weight[j], x[j][c].w, value[c].w);
+                }
         }
     }
-    sum = warp_sum(sum);
-    float inv = sum != 0.f ? 1.f / sum : 0.f;
+    if (WARPS > 1) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+            if (c * 32 + lane < width) shared_value[warp][c * 32 + lane] = value[c];
+        __syncthreads();
+        if (mine) return;
+#pragma unroll
+        for (int k = 1; k < WARPS; ++k)
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+                if (c * 32 + lane < width) {
+                    float4 x = shared_value[warp + k][c * 32 + lane];
+                    value[c].x += x.x;
+                    value[c].y += x.y;
+                    value[c].z += x.z;
+                    value[c].w += x.w;
+                }
+    }
+    if (!valid) return;
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
     T* out = static_cast<T*>(a.out) + (size_t)(row / a.n_heads) * a.out_stride + (size_t)(row % a.n_heads) * D;
 #pragma unroll
-    for (int c = 0; c < COLS; ++c)
-        if (c * 32 + lane < D) out[c * 32 + lane] = from_float<T>(value[c] * inv);
+    for (int c = 0; c < CHUNKS; ++c) {
+        int col = (c * 32 + lane) * 4;
+        float x[4] = {value[c].x * inv, value[c].y * inv, value[c].z * inv, value[c].w * inv};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (col + k < D) out[col + k] = from_float<T>(x[k]);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ the call
@@ -750,7 +1048,6 @@ struct Plan {
 };
 
 constexpr int SMS = 148;
-constexpr int MAX_SPLITS = 64;
 
 struct Sizes {
     int n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own;
@@ -789,6 +1086,10 @@ Plan plan_for(const Sizes& z) {
     return p;
 }
 
+// of the parts' weighted values (their maxima and sums start on 16 bytes behind them), and of both
+long long value_floats(long long parts, int head_dim) { return (parts * head_dim + 3) / 4 * 4; }
+long long scratch_floats_of(long long parts, int head_dim) { return value_floats(parts, head_dim) + 2 * parts; }
+
 template <typename T, int DMAX>
 int launch_simt(const Args& a, unsigned blocks, cudaStream_t stream) {
     constexpr size_t smem = simt_floats<DMAX>() * sizeof(float);
@@ -803,8 +1104,9 @@ int launch_simt(const Args& a, unsigned blocks, cudaStream_t stream) {
 
 template <int HD>
 int launch_tc(const Args& a, int n_pages, unsigned blocks, cudaStream_t stream) {
-    // never less than 80 KB, so that no third block lands on an SM and waits for tensor memory
-    constexpr size_t need = 1024 + (HD / 64) * (Q_PIECE + 4 * KV_PIECE) + 16 * 8 + 16, smem = need < 80 * 1024 ? 80 * 1024 : need;
+    // (more than 80 KB: no third block lands on an SM and waits for tensor memory)
+    constexpr size_t smem = 1024 + tile_bytes<HD>() + 16 * 8;
+    static_assert(smem > 80 * 1024 && 2 * (smem + sizeof(Staged) + 1024) <= 227 * 1024, "two blocks an SM");
     static bool configured = false;
     if (!configured) {
         LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -822,6 +1124,15 @@ int launch_tc(const Args& a, int n_pages, unsigned blocks, cudaStream_t stream) 
     return check_launch("prefix_attention_tc");
 }
 
+// a warp for four parts, as many as fit
+template <typename T>
+void launch_join(const Args& a, int rows, cudaStream_t stream) {
+    if (a.slots <= 4) llmb::launch(prefix_attention_join_kernel<T, 1>, dim3((rows + 7) / 8), 256, 0, stream, true, a, rows);
+    else if (a.slots <= 8) llmb::launch(prefix_attention_join_kernel<T, 2>, dim3((rows + 3) / 4), 256, 0, stream, true, a, rows);
+    else if (a.slots <= 16) llmb::launch(prefix_attention_join_kernel<T, 4>, dim3((rows + 1) / 2), 256, 0, stream, true, a, rows);
+    else llmb::launch(prefix_attention_join_kernel<T, 8>, dim3(rows), 256, 0, stream, true, a, rows);
+}
+
 int run(const Args& a, const Plan& p, int dtype, int n_pages, int n_tokens, cudaStream_t stream) {
     long long blocks = (long long)a.n_kv_heads * ((long long)a.n_groups * a.prefix_tiles * a.prefix_splits + (long long)a.n_seqs * a.own_tiles * a.own_splits);
     LLMB_REQUIRE(blocks < (1ll << 31), "prefix_attention: too many blocks");
@@ -833,8 +1144,8 @@ int run(const Args& a, const Plan& p, int dtype, int n_pages, int n_tokens, cuda
     else code = f32 ? launch_simt<float, 256>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 256>(a, (unsigned)blocks, stream);
     if (code || a.slots == 1) return code;
     int rows = n_tokens * a.n_heads;
-    if (f32) llmb::launch(prefix_attention_join_kernel<float>, dim3((rows + 3) / 4), 128, 0, stream, true, a, rows);
-    else llmb::launch(prefix_attention_join_kernel<__nv_bfloat16>, dim3((rows + 3) / 4), 128, 0, stream, true, a, rows);
+    if (f32) launch_join<float>(a, rows, stream);
+    else launch_join<__nv_bfloat16>(a, rows, stream);
     return check_launch("prefix_attention_join");
 }
 
@@ -860,7 +1171,7 @@ LLMB_EXPORT long long llmb_prefix_attention_scratch_floats(int n_tokens, int n_s
     if (n_tokens <= 0 || n_seqs <= 0 || n_groups <= 0 || n_kv_heads <= 0 || n_heads < n_kv_heads) return 0;
     Plan p = plan_for(Sizes{n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own, tc != 0});
     if (p.slots > 1) ++*kernels;
-    return p.slots > 1 ? (long long)n_tokens * n_heads * p.slots * (head_dim + 2) : 0;
+    return p.slots > 1 ? scratch_floats_of((long long)n_tokens * n_heads * p.slots, head_dim) : 0;
 }
 
 // tc: what llmb_prefix_attention_tc_serves said, 0 to keep to the CUDA cores.
@@ -883,11 +1194,11 @@ LLMB_EXPORT int llmb_prefix_attention(const void* q, int q_stride, const void* k
     LLMB_REQUIRE(n_pages > 0 && (long long)n_pages * n_kv_heads * LLMB_PAGE < (1ll << 31), "prefix_attention: %d pages", n_pages);
     Plan p = plan_for(Sizes{n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own, tc != 0});
     long long rows = (long long)n_tokens * n_heads;
-    LLMB_REQUIRE(p.slots == 1 || (scratch != nullptr && aligned(scratch) && scratch_floats >= rows * p.slots * (head_dim + 2)),
+    LLMB_REQUIRE(p.slots == 1 || (scratch != nullptr && aligned(scratch) && scratch_floats >= scratch_floats_of(rows * p.slots, head_dim)),
                  "prefix_attention: scratch too small");
     int size = dtype == LLMB_DTYPE_F32 ? 4 : 2;
     bool vectors = (head_dim * size) % 16 == 0 && aligned(k_cache) && aligned(v_cache);
-    Args a{q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, out, scratch, scratch + rows * p.slots * head_dim,
+    Args a{q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, out, scratch, scratch + value_floats(rows * p.slots, head_dim),
            q_stride, out_stride, table_stride, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, scale * LOG2E,
            p.prefix_tiles, p.prefix_splits, p.own_tiles, p.own_splits, p.slots, vectors ? 1 : 0, p.whole ? 1 : 0};
     return run(a, p, dtype, n_pages, n_tokens, stream);
