@@ -1117,9 +1117,8 @@ int launch_tc(const Args& a, int n_pages, unsigned blocks, cudaStream_t stream) 
     int code = make_map_2d(&map_k, a.k_cache, cache_rows, HD, HD, 64, LLMB_PAGE);
     if (!code) code = make_map_2d(&map_v, a.v_cache, cache_rows, HD, HD, 64, LLMB_PAGE);
     if (code) return code;
-    int* status = status_word();
-    int* status_dev = nullptr;
-    if (status) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status_dev, status, 0));
+    static int* status_dev = nullptr;
+    if (!status_dev && status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status_dev, status_word(), 0));
     llmb::launch(prefix_attention_tc_kernel<HD>, dim3(blocks), TC_THREADS, smem, stream, true, map_k, map_v, a, status_dev);
     return check_launch("prefix_attention_tc");
 }

@@ -180,6 +180,10 @@ class RecordedPass:
         """The 8-byte slot of a ctypes argument: an address, a widened integer, or a double's bits."""
         if a is None:
             return 0
+        if type(a) is int:                                # (an entry point whose argument types are declared takes plain numbers)
+            return a & 0xFFFFFFFFFFFFFFFF
+        if type(a) is float:
+            return ctypes.c_ulonglong.from_buffer_copy(ctypes.c_double(a)).value
         if isinstance(a, ctypes.c_void_p):
             return a.value or 0
         if isinstance(a, (ctypes.c_int, ctypes.c_longlong, ctypes.c_ulonglong)):
@@ -1444,14 +1448,25 @@ def attention_replay_key(step, n_heads: int, n_kv_heads: int, window: int = 0):
 
 # ----------------------------------------------------------------------------- sequences that share pages
 
-@functools.lru_cache(maxsize=4096)
-def _prefix_scratch(n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own,
-                    tc) -> tuple:
-    """(floats of scratch, launches) of a prefix_attention of these sizes, on the tensor cores or not."""
-    lib, kernels = load_library("prefix_attention"), ctypes.c_int(0)
+_prefix_declared = False
+
+
+def _declare_prefix():
+    """The argument types of prefix_attention's entry points, so that a call hands over plain numbers: its launches are short, and a
+    ctypes object for each of 30 arguments costs the host as much as they do."""
+    global _prefix_declared
+    lib, p, i = load_library("prefix_attention"), ctypes.c_void_p, _c_int
     lib.llmb_prefix_attention_scratch_floats.restype = ctypes.c_longlong
-    floats = lib.llmb_prefix_attention_scratch_floats(*map(_c_int, (n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new,
-                                                                    max_group, max_shared, max_own, tc)), ctypes.byref(kernels))
+    lib.llmb_prefix_attention_scratch_floats.argtypes = [i] * 11 + [ctypes.POINTER(i)]
+    lib.llmb_prefix_attention.argtypes = [p, i, p, p, i, p, i, p, p, p, p, p, i, p, ctypes.c_longlong] + [i] * 7 + [_c_float] + [i] * 5 + [p]
+    _prefix_declared = True
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefix_scratch(*sizes) -> tuple:
+    """(floats of scratch, launches) of a prefix_attention of these sizes, the last of which says whether it runs on the tensor cores."""
+    kernels = ctypes.c_int(0)
+    floats = load_library("prefix_attention").llmb_prefix_attention_scratch_floats(*sizes, ctypes.byref(kernels))
     return floats, kernels.value
 
 
@@ -1476,40 +1491,53 @@ def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, g
 
     max_new, max_group: most new tokens of a sequence, of a group; max_shared: most pages that a group shares; max_own: most
     positions of a sequence behind those. Upper bounds, which size the launches."""
-    _require_cuda(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages)
-    n, dtype = qkv.shape[0], qkv.dtype
-    n_seqs, n_groups = seq_lens.numel(), group_pages.numel()
-    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < n_heads * head_dim:
+    if not _prefix_declared:
+        _declare_prefix()
+    dtype, int32 = qkv.dtype, torch.int32
+    tensors = (qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages)
+    if not (qkv.is_cuda and k_cache.is_cuda and v_cache.is_cuda and block_table.is_cuda and seq_lens.is_cuda and cu_seqlens.is_cuda
+            and group_first.is_cuda and group_pages.is_cuda):
+        _require_cuda(*tensors)
+    if qkv.dim() != 2:
+        raise KernelError("prefix_attention: queries must be rows")
+    (n, width), (q_stride, inner) = qkv.shape, qkv.stride()
+    if inner != 1 or width < n_heads * head_dim:
         raise KernelError(f"prefix_attention: queries must be rows of at least {n_heads * head_dim} contiguous values")
-    for cache in (k_cache, v_cache):
-        if (cache.dim() != 4 or tuple(cache.shape[1:]) != (n_kv_heads, PAGE, head_dim) or cache.dtype != dtype
-                or not cache.is_contiguous()):
-            raise KernelError(f"prefix_attention: caches must be contiguous {dtype} [pages, {n_kv_heads}, {PAGE}, {head_dim}]")
-    for name, ints, count in (("seq_lens", seq_lens, n_seqs), ("cu_seqlens", cu_seqlens, n_seqs + 1),
-                              ("group_first", group_first, n_groups + 1), ("group_pages", group_pages, n_groups)):
-        if ints.dtype != torch.int32 or ints.numel() != count or not ints.is_contiguous():
-            raise KernelError(f"prefix_attention: {name} must be contiguous int32 [{count}]")
-    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n_seqs or block_table.stride(1) != 1
-            or max_shared > block_table.shape[1]):
+    paged = k_cache.shape
+    if (len(paged) != 4 or paged[1:] != (n_kv_heads, PAGE, head_dim) or v_cache.shape != paged or k_cache.dtype is not dtype
+            or v_cache.dtype is not dtype or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
+        raise KernelError(f"prefix_attention: caches must be contiguous {dtype} [pages, {n_kv_heads}, {PAGE}, {head_dim}], both with the same pages")
+    n_seqs, n_groups = seq_lens.numel(), group_pages.numel()
+    if not (seq_lens.dtype is int32 and cu_seqlens.dtype is int32 and group_first.dtype is int32 and group_pages.dtype is int32
+            and cu_seqlens.numel() == n_seqs + 1 and group_first.numel() == n_groups + 1 and seq_lens.is_contiguous()
+            and cu_seqlens.is_contiguous() and group_first.is_contiguous() and group_pages.is_contiguous()):
+        raise KernelError("prefix_attention: seq_lens [B], cu_seqlens [B + 1], group_first [G + 1] and group_pages [G] must be contiguous int32")
+    if block_table.dtype is not int32 or block_table.dim() != 2:
+        raise KernelError("prefix_attention: the page table must be int32 [B, pages]")
+    (table_rows, table_width), (table_stride, table_inner) = block_table.shape, block_table.stride()
+    if table_rows != n_seqs or table_inner != 1 or max_shared > table_width:
         raise KernelError(f"prefix_attention: the page table must be int32 [{n_seqs}, at least {max_shared}]")
     if max_new < 1 or max_group < max_new or max_shared < 0 or max_own < 0:
         raise KernelError(f"prefix_attention: no bounds of a step: max_new {max_new}, max_group {max_group}, max_shared {max_shared}, "
                           f"max_own {max_own}")
-    _check_out(out, (n, n_heads * head_dim), dtype, "prefix_attention")
     if out is None:
         out = torch.empty((n, n_heads * head_dim), dtype=dtype, device=qkv.device)
+    else:
+        _check_out(out, (n, n_heads * head_dim), dtype, "prefix_attention")
     if n == 0:
         return out
     shared, own = page_bucket(max_shared), page_bucket(-(-max_own // PAGE)) * PAGE
-    aligned = qkv.stride(0) % 8 == 0 and not (qkv.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) & 15
-    tc = int(dtype == torch.bfloat16 and head_dim in (64, 128) and scale > 0 and aligned and not tactics.is_disabled("prefix_attention_tc"))
+    at_q, at_k, at_v, at_out = qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+    tc = int(dtype is torch.bfloat16 and head_dim in (64, 128) and scale > 0 and q_stride % 8 == 0 and not (at_q | at_k | at_v | at_out) & 15
+             and not tactics.is_disabled("prefix_attention_tc"))
     floats, kernels = _prefix_scratch(n, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, shared, own, tc)
     parts = _scratch(qkv.device, "attention", floats)[0] if floats else None
-    _call("prefix_attention", "llmb_prefix_attention", _ptr(qkv), _c_int(qkv.stride(0)), _ptr(k_cache), _ptr(v_cache),
-          _c_int(k_cache.shape[0]), _ptr(block_table), _c_int(block_table.stride(0)), _ptr(seq_lens), _ptr(cu_seqlens), _ptr(group_first), _ptr(group_pages), _ptr(out),
-          _c_int(out.stride(0)), _ptr(parts), ctypes.c_longlong(floats), _c_int(_code(dtype)), _c_int(n), _c_int(n_seqs), _c_int(n_groups),
-          _c_int(n_heads), _c_int(n_kv_heads), _c_int(head_dim), _c_float(scale), _c_int(max_new), _c_int(max_group), _c_int(shared),
-          _c_int(own), _c_int(tc), _stream(), kernels=kernels)
+    if _recording is not None:
+        _recording.keep += [*tensors, out, parts]
+    _call("prefix_attention", "llmb_prefix_attention", at_q, q_stride, at_k, at_v, k_cache.shape[0], block_table.data_ptr(), table_stride,
+          seq_lens.data_ptr(), cu_seqlens.data_ptr(), group_first.data_ptr(), group_pages.data_ptr(), at_out, out.stride(0),
+          parts.data_ptr() if floats else None, floats, _code(dtype), n, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, scale, max_new,
+          max_group, shared, own, tc, _stream(), kernels=kernels)
     return out
 
 
