@@ -38,12 +38,14 @@ struct Args {
     const int* group_first;          // [n_groups + 1] the first sequence of each group
     const int* group_pages;          // [n_groups] pages that the group's members share
     void* out;
-    float* acc;                      // [tokens * heads, slots, head_dim]
-    float* stats;                    // [tokens * heads, slots, 2]: maximum in base-2 units, sum
+    float* acc;                      // [rows, slots, head_dim], a row a (token, head), or a row of the tiles that are cut (`whole`)
+    float* stats;                    // [rows, slots, 2]: maximum in base-2 units, sum
     int q_stride, out_stride, table_stride, n_seqs, n_groups, n_heads, n_kv_heads, head_dim;
     float scale_log2;
     int prefix_tiles, prefix_splits, own_tiles, own_splits, slots;
     int vectors;                     // the caches' rows can be read 16 bytes at a time
+    int full_tiles;                  // tiles of the wide kernel whose walk is one block's; the others are cut into prefix_splits pieces
+    int behind;                      // own parts launched behind the wide kernel, which has waited for all that they read
     int whole;                       // a tile of a group walks its sequences' own pages behind the shared ones (tensor cores)
 };
 
@@ -313,31 +315,282 @@ __global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(con
     }
 }
 
-// ------------------------------------------------------------------------------------------------ bfloat16, head sizes 64 and 128
+// ------------------------------------------------------------------------------------------------ bfloat16, few rows
 //
-// The products on the fifth-generation tensor cores. A block holds 128 rows and walks its pages one by one:
-//
-// * warps 0 and 6: the page's keys and values by TMA (64 x 64 boxes with the 128-byte swizzle), two buffers each;
-// * warp 1: S[128, 64 keys] = Q K^T into one of two buffers of scores in tensor memory, O[128, D] += P V with P from tensor memory. The
-//   scores of the page after the next are issued behind P V of this one, so that products and softmax work on different buffers;
-// * warps 2 to 5: thread r owns row r. It puts the tile's queries into shared memory (rows are token and head, which no box of a
-//   tensor map follows for every share), then per page reads 64 scores, forms the weights and writes them over the scores as pairs
-//   of bfloat16 (rounded to 8 bits: what the tensor cores take; their sum is of the unrounded ones). The maximum that the exponents refer to
-//   moves only when a page exceeds it by more than 2^8; O is then rescaled in place.
-//
-// A walk is the shared pages, or a sequence's own ones, or both: behind the shared pages those of each sequence that the tile has rows of,
-// whose rows alone see them (`whole`).
-//
-// Items of 16 rows or fewer (a sequence's own pages in a decode step; the shared pages of a few samples) are bound by reading their
-// pages and would leave seven eighths of the tile empty: warp 0 keeps a ring of pages in flight and warps 2 to 5 take 16 of
-// a page's 64 keys each with mma.sync.m16n8k16, keep a maximum, a sum and weighted values of their own and are merged at the end.
+// Items of 64 rows or fewer (a sequence's own pages in a decode step; the shared pages of a few samples) are bound by reading their pages.
+// Warp 4 keeps a ring of pages in flight (TMA, 64 x 64 boxes with the 128-byte swizzle); warps 0 to 3 take 16 rows and a share of a
+// page's keys each with mma.sync.m16n8k16: 16 keys where the item has up to 16 rows, 32 up to 32, all 64 above. Each keeps a maximum,
+// a sum and weighted values of its own, in 32 bits, and those of the same rows are merged at the end. Weights are rounded to 8 bits, what the
+// tensor cores take; their sum is of the unrounded ones.
 
-constexpr int TC_ROWS = 128, TC_THREADS = 224;
-constexpr int FEW_ROWS = 16;                      // rows of an item that go through mma.sync
-constexpr int Q_PIECE = TC_ROWS * 64 * 2;         // the tile's rows, 64 columns of the head: 16 KB
 constexpr int KV_PIECE = LLMB_PAGE * 64 * 2;      // a page, 64 columns of the head: 8 KB
-// tensor memory: two buffers of scores (64 columns of 32-bit values, the weights over the first 32), O beside them
-constexpr uint32_t S_COL = 0, O_COL = 128, TMEM_COLS = 256;
+constexpr int FEW_ROWS = 64, FEW_THREADS = 160;
+constexpr int FEW_WARPS = 4;
+
+// where element (row, col) of a page lies in shared memory: pieces of 64 columns, 16-byte chunks swizzled by the row
+__device__ __forceinline__ const unsigned char* swizzled(const unsigned char* page, int row, int col) {
+    return page + (col >> 6) * KV_PIECE + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4);
+}
+
+template <int HD> struct Ring {
+    static constexpr int STAGE = 2 * (HD / 64) * KV_PIECE;   // a page's keys and values
+    static constexpr int STAGES = HD == 64 ? 6 : 3;          // two blocks an SM: 192 KB in flight
+    static constexpr int MERGE = FEW_WARPS * 16 * (HD + 8 + 2) * 4;
+    static constexpr int BYTES = STAGE * STAGES;
+    static_assert(MERGE <= BYTES, "the merge takes the ring's place");
+};
+
+// The arrays that say which sequences there are, in shared memory (one round of loads) where there is room.
+constexpr int STAGED_SEQS = 128;
+struct Staged {
+    int seq_lens[STAGED_SEQS], cu_seqlens[STAGED_SEQS + 1], group_first[STAGED_SEQS + 1], group_pages[STAGED_SEQS];
+};
+__device__ __forceinline__ void stage_arrays(Args& a, Staged& s) {
+    if (a.n_seqs > STAGED_SEQS) return;
+    for (int i = threadIdx.x; i <= a.n_seqs; i += blockDim.x) {
+        s.cu_seqlens[i] = a.cu_seqlens[i];
+        if (i < a.n_seqs) s.seq_lens[i] = a.seq_lens[i];
+        if (i <= a.n_groups) s.group_first[i] = a.group_first[i];
+        if (i < a.n_groups) s.group_pages[i] = a.group_pages[i];
+    }
+    __syncthreads();
+    a.seq_lens = s.seq_lens;
+    a.cu_seqlens = s.cu_seqlens;
+    a.group_first = s.group_first;
+    a.group_pages = s.group_pages;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(FEW_THREADS, 2)
+prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                            const __grid_constant__ Args args, int* status) {
+    constexpr int STAGES = Ring<HD>::STAGES, STAGE = Ring<HD>::STAGE, PIECES = HD / 64;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(base + Ring<HD>::BYTES);
+    uint64_t* empty = full + STAGES;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + STAGES);
+    __shared__ Staged staged;
+
+    griddep_launch();
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(smem_u32(&full[i]), 1);
+            mbar_init(smem_u32(&empty[i]), FEW_WARPS);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    Args a = args;
+    stage_arrays(a, staged);                                 // (lengths, groups and tables are not written by the kernels of a step)
+    Item w;
+    bool work = item_of(a, blockIdx.x, w);                   // uniform for the block
+    work = work && w.n_rows > 0 && w.n_rows <= FEW_ROWS;
+    __syncthreads();
+    // Behind the wide kernel's shared parts the own ones may run beside them: that kernel lets them start when the one in front of it is
+    // complete. Each block waits for it at its end, so that the join waits for both.
+    if (!a.behind || !work) griddep_wait();
+    if (!work) return;
+    const int share = a.n_heads / a.n_kv_heads;
+    const bool own = w.slot >= a.prefix_splits;
+    const int last_token = w.first_token + (w.n_rows - 1) / share;
+    int limit = w.page_end * LLMB_PAGE - 1;                  // the last position that a row sees of these pages
+    if (own) limit = min(limit, a.seq_lens[w.seq_first] - a.cu_seqlens[w.seq_first + 1] + last_token);
+    const int n_pages = min(w.page_end, limit < 0 ? 0 : limit / LLMB_PAGE + 1) - w.page_begin;
+    const int row_groups = w.n_rows <= 16 ? 1 : w.n_rows <= 32 ? 2 : 4;
+
+    const int g = lane >> 2, t = lane & 3;
+    const int rows0 = warp % row_groups * 16, keys0 = warp / row_groups * 16 * row_groups;      // this warp's rows and keys of a page
+    float acc[HD / 8][4], run_max[2] = {-INFINITY, -INFINITY}, run_sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+    if (warp == FEW_WARPS) {
+        const int* pages = a.block_table + (size_t)w.seq_first * a.table_stride + w.page_begin;
+        int numbers = lane < n_pages ? pages[lane] : 0;      // 32 places of the table at once
+        for (int i = 0; i < n_pages; ++i) {
+            if (i > 0 && (i & 31) == 0) numbers = i + lane < n_pages ? pages[i + lane] : 0;
+            int stage = i % STAGES;
+            int row = (__shfl_sync(0xffffffffu, numbers, i & 31) * a.n_kv_heads + w.kv_head) * LLMB_PAGE;
+            if (i >= STAGES && !mbar_wait_warp(smem_u32(&empty[stage]), (i / STAGES - 1) & 1, abort_flag, status, 21)) break;
+            if (elect_one()) {
+                uint32_t bar = smem_u32(&full[stage]);
+                mbar_expect_tx(bar, STAGE);
+                for (int h = 0; h < PIECES; ++h) tma_load_2d(smem_u32(base + stage * STAGE + h * KV_PIECE), &map_k, bar, h * 64, row);
+                for (int h = 0; h < PIECES; ++h) tma_load_2d(smem_u32(base + stage * STAGE + (PIECES + h) * KV_PIECE), &map_v, bar, h * 64, row);
+            }
+            __syncwarp();
+        }
+    } else {
+        // rows g and g + 8 of the mma tile are this lane's
+        uint32_t qa[HD / 16][4];
+        int pos[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            int r = rows0 + g + half * 8;
+            bool valid = r < w.n_rows;
+            int token = w.first_token + (valid ? r : 0) / share, head = w.kv_head * share + (valid ? r : 0) % share;
+            pos[half] = valid ? position_of(a, w, token) : -1;
+            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + (size_t)token * a.q_stride + (size_t)head * HD;
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks) {
+                qa[ks][half] = valid ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 2 * t) : 0u;
+                qa[ks][2 + half] = valid ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8 + 2 * t) : 0u;
+            }
+        }
+        bool ok = rows0 < w.n_rows;                          // (a warp without rows only lets the ring go on)
+        for (int i = 0; i < n_pages; ++i) {
+            int stage = i % STAGES;
+            if (!mbar_wait_warp(smem_u32(&full[stage]), (i / STAGES) & 1, abort_flag, status, 22)) break;
+            const unsigned char* k_page = base + stage * STAGE;
+            const unsigned char* v_page = k_page + PIECES * KV_PIECE;
+#pragma unroll 1
+            for (int part = 0; part < row_groups; ++part) {
+                const int in_page = keys0 + part * 16, key0 = (w.page_begin + i) * LLMB_PAGE + in_page;
+                if (!ok || key0 > limit) break;
+                float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    uint32_t b[4];
+                    ldmatrix_x4(b, swizzled(k_page, in_page + (lane >> 4) * 8 + (lane & 7), ks * 16 + ((lane >> 3) & 1) * 8));
+                    mma_bf16(s0, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[0], b[1]);
+                    mma_bf16(s1, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[2], b[3]);
+                }
+                // this lane's keys: key0 + 2t, +1 (s0), +8, +9 (s1); elements 0, 1 of row g, 2, 3 of row g + 8
+                uint32_t pa[4];
+                float alpha[2];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float v[4] = {s0[2 * half], s0[2 * half + 1], s1[2 * half], s1[2 * half + 1]};
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        int key = key0 + 2 * t + (j & 1) + (j >> 1) * 8;
+                        v[j] = key <= pos[half] ? v[j] * a.scale_log2 : -INFINITY;
+                        top = fmaxf(top, v[j]);
+                    }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    float new_max = fmaxf(run_max[half], top), against = new_max == -INFINITY ? 0.f : new_max;
+                    alpha[half] = fast_exp2(run_max[half] - against);
+                    float p[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[j] = fast_exp2(v[j] - against);
+                    run_sum[half] = run_sum[half] * alpha[half] + ((p[0] + p[1]) + (p[2] + p[3]));       // of this lane's keys
+                    run_max[half] = new_max;
+                    pa[half] = pack_bf16(p[0], p[1]);
+                    pa[2 + half] = pack_bf16(p[2], p[3]);
+                }
+                if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {       // a maximum has moved
+#pragma unroll
+                    for (int n = 0; n < HD / 8; ++n) {
+                        acc[n][0] *= alpha[0];
+                        acc[n][1] *= alpha[0];
+                        acc[n][2] *= alpha[1];
+                        acc[n][3] *= alpha[1];
+                    }
+                }
+                const bool cut = key0 + 15 > limit;          // values behind the last position are whatever the page held: zero here
+                const int left = limit + 1 - key0 - 2 * t;   // of this lane's keys 0, 1, 8, 9
+                const uint32_t keep_low = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+                const uint32_t keep_high = left >= 10 ? 0xffffffffu : left == 9 ? 0xffffu : 0u;
+#pragma unroll
+                for (int n = 0; n < HD / 8; n += 2) {
+                    uint32_t b[4];
+                    ldmatrix_x4_trans(b, swizzled(v_page, in_page + ((lane >> 3) & 1) * 8 + (lane & 7), (n + (lane >> 4)) * 8));
+                    if (cut) {
+                        b[0] &= keep_low;
+                        b[1] &= keep_high;
+                        b[2] &= keep_low;
+                        b[3] &= keep_high;
+                    }
+                    mma_bf16(acc[n], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
+                    mma_bf16(acc[n + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&empty[stage]));
+        }
+    }
+    __syncthreads();                                         // every page has been read: its room is free
+    if (*abort_flag) {                                       // a wait ran out: copies in flight get their time before the block leaves
+        for (int i = 0; i < 100; ++i) __nanosleep(10000);
+        if (a.behind) griddep_wait();
+        return;
+    }
+    constexpr int LD = HD + 8;                               // (rows of the merge in different banks)
+    float* merge_acc = reinterpret_cast<float*>(base);       // [warps][16][LD]
+    float* merge_max = merge_acc + FEW_WARPS * 16 * LD;      // [warps][16], and the sums
+    float* merge_sum = merge_max + FEW_WARPS * 16;
+    if (warp < FEW_WARPS) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            run_sum[half] += __shfl_xor_sync(0xffffffffu, run_sum[half], 1);
+            run_sum[half] += __shfl_xor_sync(0xffffffffu, run_sum[half], 2);
+            int r = warp * 16 + g + half * 8;
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n)
+                *reinterpret_cast<float2*>(merge_acc + r * LD + n * 8 + 2 * t) = make_float2(acc[n][2 * half], acc[n][2 * half + 1]);
+            if (t == 0) {
+                merge_max[r] = run_max[half];
+                merge_sum[r] = run_sum[half];
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < w.n_rows * (HD / 4); i += FEW_THREADS) {
+        int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
+        int at = (r >> 4) * 16 + (r & 15);                   // of the row's first warp; its others follow row_groups warps behind
+        float m = -INFINITY;
+        for (int k = r >> 4; k < FEW_WARPS; k += row_groups) m = fmaxf(m, merge_max[k * 16 + (r & 15)]);
+        float against = m == -INFINITY ? 0.f : m, sum = 0.f;
+        float4 value = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = r >> 4; k < FEW_WARPS; k += row_groups, at += row_groups * 16) {
+            float weight = fast_exp2(merge_max[at] - against);
+            float4 x = *reinterpret_cast<const float4*>(merge_acc + at * LD + d);
+            value.x = fmaf(x.x, weight, value.x);
+            value.y = fmaf(x.y, weight, value.y);
+            value.z = fmaf(x.z, weight, value.z);
+            value.w = fmaf(x.w, weight, value.w);
+            sum += merge_sum[at] * weight;
+        }
+        int token = w.first_token + r / share, head = w.kv_head * share + r % share;
+        if (a.slots == 1) {
+            float inv = sum != 0.f ? 1.f / sum : 0.f;
+            uint2 packed = make_uint2(pack2(value.x * inv, value.y * inv), pack2(value.z * inv, value.w * inv));
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD + d) = packed;
+        } else {
+            size_t slot = ((size_t)token * a.n_heads + head) * a.slots + w.slot;
+            if (sum != 0.f) *reinterpret_cast<float4*>(a.acc + slot * HD + d) = value;
+            if (d == 0) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(m, sum);
+        }
+    }
+    if (a.behind) griddep_wait();
+}
+
+// ------------------------------------------------------------------------------------------------ bfloat16, many rows
+//
+// 256 rows a block, one block an SM: two tiles of 128 rows with four softmax warps each share the keys and values of 128 positions (two
+// pages). Per tile one buffer of scores [128, 128] and O [128, D] fill tensor memory; the two tiles take turns: while the softmax of one
+// works on its scores, the products of the other run (P V of these keys, then Q K^T of the next). Against two blocks an SM of 128 rows and 64 keys
+// each step has half the waits per score, Q K^T reads 8 KB of shared memory for 64 cycles of products (with 64 keys 6 KB for 32: the
+// reads, not the products, set its pace), and every page is read once for 256 rows.
+//
+// When a tile's scores are there, its last P V is complete too (the products were issued behind it), so O can be rescaled at once. The maximum
+// that the exponents refer to moves only when it is exceeded by more than 2^8. Weights are rounded to 8 bits, what the tensor cores
+// take; their sum is of the unrounded ones.
+//
+// A walk is a group's shared pages and, where the sequences bring many tokens (`whole`), behind them the own pages of each sequence that the
+// block has rows of. Only the rows of that sequence see those: the others' weights are zero, and the products leave their lanes of O
+// alone (a value that is not finite times a weight of zero would reach them).
+
+constexpr int TC_ROWS = 128;                                 // lanes of tensor memory
+constexpr int Q_PIECE = TC_ROWS * 64 * 2;                    // a tile's rows, 64 columns of the head: 16 KB
+constexpr int WIDE_ROWS = 256, WIDE_THREADS = 384;           // warps 0 keys, 1 products, 2 values, 4-7 and 8-11 a tile's softmax
+constexpr int PAIR_PIECE = 128 * 128;                        // 128 positions, 64 columns of the head: 16 KB
+constexpr int WIDE_REGS_FEW = 104, WIDE_REGS_MANY = 200;      // 128 x 64 + 256 x 216 <= 384 x 168, what the block is launched with
 
 // The pages of an item, one after the other: the shared ones, then those of each sequence in turn.
 struct Walk {
@@ -383,316 +636,119 @@ __device__ __forceinline__ void start(const Args& a, const TileRange& t, Walk& w
     w.logical += skip;
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+// a block's tile and its piece of the tile's walk
+struct Piece {
+    int tile_index, piece, pieces;
+};
+__device__ __forceinline__ Piece piece_of(const Args& a, int x) {
+    if (x < a.full_tiles) return Piece{x, 0, 1};
+    x -= a.full_tiles;
+    return Piece{a.full_tiles + x / a.prefix_splits, x % a.prefix_splits, a.prefix_splits};
+}
+
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+
+// A from tensor memory, B from shared memory; lanes whose bit is set in `off` keep their rows of D
+__device__ __forceinline__ void mma_ts_lanes(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, const uint32_t (&off)[4]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(1u), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]) : "memory");
 }
-
-// where element (row, col) of a page lies in shared memory: pieces of 64 columns, 16-byte chunks swizzled by the row
-__device__ __forceinline__ const unsigned char* swizzled(const unsigned char* page, int row, int col) {
-    return page + (col >> 6) * KV_PIECE + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4);
-}
-
-template <int HD> struct Ring {                              // of the items of few rows
-    static constexpr int STAGE = 2 * (HD / 64) * KV_PIECE;   // a page's keys and values
-    static constexpr int STAGES = HD == 64 ? 5 : 3;          // two blocks an SM: 160 and 192 KB in flight
-};
-template <int HD>
-__host__ __device__ constexpr int tile_bytes() {
-    return (HD / 64) * (Q_PIECE + 4 * KV_PIECE) > Ring<HD>::STAGE * Ring<HD>::STAGES ? (HD / 64) * (Q_PIECE + 4 * KV_PIECE)
-                                                                                  : Ring<HD>::STAGE * Ring<HD>::STAGES;
-}
-
-// An item of up to 16 rows over the pages [page_begin, page_end) of one table. Rows g and g + 8 of the mma tile are this lane's.
-template <int HD>
-__device__ __forceinline__ void few_rows(const Args& a, const Item& w, const CUtensorMap& map_k, const CUtensorMap& map_v, unsigned char* base,
-                                         uint64_t* bars, volatile int* abort_flag, int* status) {
-    constexpr int STAGES = Ring<HD>::STAGES, STAGE = Ring<HD>::STAGE, PIECES = HD / 64;
-    uint64_t* full = bars;
-    uint64_t* empty = bars + STAGES;
-    const int warp = warp_index(), lane = threadIdx.x & 31, share = a.n_heads / a.n_kv_heads;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) {
-            mbar_init(smem_u32(&full[i]), 1);
-            mbar_init(smem_u32(&empty[i]), 4);
-        }
-        *abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+// the lanes of a tile that are not among rows first .. last - 1
+__device__ __forceinline__ void lanes_off(int first, int last, uint32_t (&off)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        int from = min(max(first - 32 * k, 0), 32), to = min(max(last - 32 * k, 0), 32);
+        uint32_t below_to = to >= 32 ? 0xffffffffu : (1u << to) - 1u, below_from = from >= 32 ? 0xffffffffu : (1u << from) - 1u;
+        off[k] = ~(below_to & ~below_from);
     }
-    __syncthreads();
-    griddep_launch();
-    griddep_wait();
-    const bool own = w.slot >= a.prefix_splits;
-    const int last_token = w.first_token + (w.n_rows - 1) / share;
-    // the last position that a row sees of these pages
-    int limit = w.page_end * LLMB_PAGE - 1;
-    if (own) limit = min(limit, a.seq_lens[w.seq_first] - a.cu_seqlens[w.seq_first + 1] + last_token);
-    const int n_pages = min(w.page_end, limit < 0 ? 0 : limit / LLMB_PAGE + 1) - w.page_begin;
-    bool ok = true;
-    if (warp == 0) {
-        const int* pages = a.block_table + (size_t)w.seq_first * a.table_stride + w.page_begin;
-        for (int i = 0; i < n_pages; ++i) {
-            int stage = i % STAGES;
-            int row = (pages[i] * a.n_kv_heads + w.kv_head) * LLMB_PAGE;
-            if (i >= STAGES && !mbar_wait_warp(smem_u32(&empty[stage]), (i / STAGES - 1) & 1, abort_flag, status, 21)) break;
-            if (elect_one()) {
-                uint32_t bar = smem_u32(&full[stage]);
-                mbar_expect_tx(bar, STAGE);
-                for (int h = 0; h < PIECES; ++h) {
-                    tma_load_2d(smem_u32(base + stage * STAGE + h * KV_PIECE), &map_k, bar, h * 64, row);
-                    tma_load_2d(smem_u32(base + stage * STAGE + (PIECES + h) * KV_PIECE), &map_v, bar, h * 64, row);
-                }
-            }
-            __syncwarp();
-        }
-    }
-    const int g = lane >> 2, t = lane & 3, part = warp - 2;          // warps 2 .. 5: 16 keys of every page
-    float acc[HD / 8][4], run_max[2] = {-INFINITY, -INFINITY}, run_sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-    if (part >= 0 && part < 4) {
-        uint32_t qa[HD / 16][4];
-        int pos[2];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            int r = g + half * 8;
-            bool valid = r < w.n_rows;
-            int token = w.first_token + (valid ? r : 0) / share, head = w.kv_head * share + (valid ? r : 0) % share;
-            pos[half] = valid ? position_of(a, w, token) : -1;
-            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + (size_t)token * a.q_stride + (size_t)head * HD;
-#pragma unroll
-            for (int ks = 0; ks < HD / 16; ++ks) {
-                qa[ks][half] = valid ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 2 * t) : 0u;
-                qa[ks][2 + half] = valid ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8 + 2 * t) : 0u;
-            }
-        }
-        for (int i = 0; i < n_pages; ++i) {
-            int stage = i % STAGES;
-            ok = mbar_wait_warp(smem_u32(&full[stage]), (i / STAGES) & 1, abort_flag, status, 22);
-            if (!ok) break;
-            const unsigned char* ks_ = base + stage * STAGE;
-            const unsigned char* vs_ = ks_ + PIECES * KV_PIECE;
-            const int key0 = (w.page_begin + i) * LLMB_PAGE + part * 16;
-            if (key0 <= limit) {
-                float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) {
-                    uint32_t b[4];
-                    ldmatrix_x4(b, swizzled(ks_, part * 16 + (lane >> 4) * 8 + (lane & 7), ks * 16 + ((lane >> 3) & 1) * 8));
-                    mma_bf16(s0, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[0], b[1]);
-                    mma_bf16(s1, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[2], b[3]);
-                }
-                // this lane's keys: key0 + 2t, +1 (s0), +8, +9 (s1); elements 0, 1 of row g, 2, 3 of row g + 8
-                uint32_t pa[4];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    float v[4] = {s0[2 * half], s0[2 * half + 1], s1[2 * half], s1[2 * half + 1]};
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        int key = key0 + 2 * t + (j & 1) + (j >> 1) * 8;
-                        v[j] = key <= pos[half] ? v[j] * a.scale_log2 : -INFINITY;
-                        top = fmaxf(top, v[j]);
-                    }
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    float new_max = fmaxf(run_max[half], top), against = new_max == -INFINITY ? 0.f : new_max;
-                    float alpha = fast_exp2(run_max[half] - against);
-                    float p[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) p[j] = fast_exp2(v[j] - against);
-                    run_sum[half] = run_sum[half] * alpha + ((p[0] + p[1]) + (p[2] + p[3]));       // of this lane's keys
-                    run_max[half] = new_max;
-                    pa[half] = pack_bf16(p[0], p[1]);
-                    pa[2 + half] = pack_bf16(p[2], p[3]);
-#pragma unroll
-                    for (int n = 0; n < HD / 8; ++n) {
-                        acc[n][2 * half] *= alpha;
-                        acc[n][2 * half + 1] *= alpha;
-                    }
-                }
-                const bool cut = key0 + 15 > limit;          // values behind the last position are whatever the page held: zero here
-                const int left = limit + 1 - key0 - 2 * t;   // of this lane's keys 0, 1, 8, 9
-                const uint32_t keep_low = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
-                const uint32_t keep_high = left >= 10 ? 0xffffffffu : left == 9 ? 0xffffu : 0u;
-#pragma unroll
-                for (int n = 0; n < HD / 8; n += 2) {
-                    uint32_t b[4];
-                    ldmatrix_x4_trans(b, swizzled(vs_, part * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), (n + (lane >> 4)) * 8));
-                    if (cut) {
-                        b[0] &= keep_low;
-                        b[1] &= keep_high;
-                        b[2] &= keep_low;
-                        b[3] &= keep_high;
-                    }
-                    mma_bf16(acc[n], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
-                    mma_bf16(acc[n + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
-                }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&empty[stage]));
-        }
-    }
-    __syncthreads();                                         // every page has been read: its room is free
-    if (*abort_flag) {                                       // a wait ran out: copies in flight get their time before the block leaves
-        for (int i = 0; i < 100; ++i) __nanosleep(10000);
-        return;
-    }
-    constexpr int LD = HD + 8;                               // (rows of the merge in different banks)
-    float* merge_acc = reinterpret_cast<float*>(base);       // [4][16][LD]
-    float* merge_max = merge_acc + 4 * FEW_ROWS * LD;        // [4][16], and the sums
-    float* merge_sum = merge_max + 4 * FEW_ROWS;
-    if (part >= 0 && part < 4) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            run_sum[half] += __shfl_xor_sync(0xffffffffu, run_sum[half], 1);
-            run_sum[half] += __shfl_xor_sync(0xffffffffu, run_sum[half], 2);
-            int r = part * FEW_ROWS + g + half * 8;
-#pragma unroll
-            for (int n = 0; n < HD / 8; ++n)
-                *reinterpret_cast<float2*>(merge_acc + r * LD + n * 8 + 2 * t) = make_float2(acc[n][2 * half], acc[n][2 * half + 1]);
-            if (t == 0) {
-                merge_max[r] = run_max[half];
-                merge_sum[r] = run_sum[half];
-            }
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < w.n_rows * (HD / 4); i += TC_THREADS) {
-        int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
-        float m = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) m = fmaxf(m, merge_max[k * FEW_ROWS + r]);
-        float against = m == -INFINITY ? 0.f : m, sum = 0.f;
-        float4 value = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float weight = fast_exp2(merge_max[k * FEW_ROWS + r] - against);
-            float4 x = *reinterpret_cast<const float4*>(merge_acc + (k * FEW_ROWS + r) * LD + d);
-            value.x = fmaf(x.x, weight, value.x);
-            value.y = fmaf(x.y, weight, value.y);
-            value.z = fmaf(x.z, weight, value.z);
-            value.w = fmaf(x.w, weight, value.w);
-            sum += merge_sum[k * FEW_ROWS + r] * weight;
-        }
-        int token = w.first_token + r / share, head = w.kv_head * share + r % share;
-        if (a.slots == 1) {
-            float inv = sum != 0.f ? 1.f / sum : 0.f;
-            uint2 packed = make_uint2(pack2(value.x * inv, value.y * inv), pack2(value.z * inv, value.w * inv));
-            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD + d) = packed;
-        } else {
-            size_t slot = ((size_t)token * a.n_heads + head) * a.slots + w.slot;
-            if (sum != 0.f) *reinterpret_cast<float4*>(a.acc + slot * HD + d) = value;
-            if (d == 0) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(m, sum);
-        }
-    }
-}
-
-// The arrays that say which sequences there are, in shared memory (one round of loads) where there is room.
-constexpr int STAGED_SEQS = 128;
-struct Staged {
-    int seq_lens[STAGED_SEQS], cu_seqlens[STAGED_SEQS + 1], group_first[STAGED_SEQS + 1], group_pages[STAGED_SEQS];
-};
-__device__ __forceinline__ void stage_arrays(Args& a, Staged& s) {
-    if (a.n_seqs > STAGED_SEQS) return;
-    for (int i = threadIdx.x; i <= a.n_seqs; i += blockDim.x) {
-        s.cu_seqlens[i] = a.cu_seqlens[i];
-        if (i < a.n_seqs) s.seq_lens[i] = a.seq_lens[i];
-        if (i <= a.n_groups) s.group_first[i] = a.group_first[i];
-        if (i < a.n_groups) s.group_pages[i] = a.group_pages[i];
-    }
-    __syncthreads();
-    a.seq_lens = s.seq_lens;
-    a.cu_seqlens = s.cu_seqlens;
-    a.group_first = s.group_first;
-    a.group_pages = s.group_pages;
 }
 
 template <int HD>
-__global__ void __launch_bounds__(TC_THREADS, 2)
-prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                           const __grid_constant__ Args args, int* status) {
+__global__ void __launch_bounds__(WIDE_THREADS, 1)
+prefix_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                             const __grid_constant__ Args args, int* status) {
     constexpr int PIECES = HD / 64;
-    constexpr int KV_BYTES = PIECES * KV_PIECE;
+    constexpr int Q_BYTES = PIECES * Q_PIECE, PAIR_BYTES = PIECES * PAIR_PIECE, PAGE_BYTES = PIECES * KV_PIECE;
+    constexpr uint32_t SCORES = 128, O_FIRST = 256, COLS = 512;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char* q_tile = base;
-    unsigned char* k_tile = base + PIECES * Q_PIECE;
-    unsigned char* v_tile = k_tile + 2 * KV_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base + tile_bytes<HD>());
-    uint64_t* q_full = bars;                  // the queries are in shared memory
-    uint64_t* k_full = bars + 1;              // [2]
-    uint64_t* k_empty = bars + 3;             // [2]
-    uint64_t* v_full = bars + 5;              // [2]
-    uint64_t* v_empty = bars + 7;             // [2]
-    uint64_t* s_full = bars + 9;              // [2] a buffer's scores are complete
-    uint64_t* p_full = bars + 11;             // [2] its weights are written and O has been rescaled
-    uint64_t* o_full = bars + 13;             // a page's P V has been added to O
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+    unsigned char* q_tile = base;                             // [2]
+    unsigned char* k_tile = base + 2 * Q_BYTES;               // [2] pairs of pages
+    unsigned char* v_tile = k_tile + 2 * PAIR_BYTES;          // [2]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(v_tile + 2 * PAIR_BYTES);
+    uint64_t* q_full = bars;                  // [2] a tile's queries are in shared memory
+    uint64_t* k_full = bars + 2;              // [2]
+    uint64_t* k_empty = bars + 4;             // [2]
+    uint64_t* v_full = bars + 6;              // [2]
+    uint64_t* v_empty = bars + 8;             // [2]
+    uint64_t* s_full = bars + 10;             // [2] a tile's scores are complete (and all its products before)
+    uint64_t* p_full = bars + 12;             // [2][2] its weights of 64 positions are written and O has been rescaled
+    uint64_t* o_full = bars + 16;             // [2] its last P V is complete
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     __shared__ Staged staged;
     Args a = args;
-    stage_arrays(a, staged);                                 // (lengths, groups and tables are not written by the kernels of a step)
-    Item w;
-    if (!item_of(a, blockIdx.x, w)) return;                  // uniform for the block, here and below: nothing is allocated yet
-    if (!a.whole && w.n_rows <= FEW_ROWS) {
-        if (w.n_rows > 0 && w.tile == 0) few_rows<HD>(a, w, map_k, map_v, base, bars, abort_flag, status);
-        return;
-    }
+    stage_arrays(a, staged);
+    const Piece piece = piece_of(a, blockIdx.x);
     const int share = a.n_heads / a.n_kv_heads;
-    const int row0 = w.tile * TC_ROWS, n_rows = min(TC_ROWS, w.n_rows - row0);
+    Item w;
+    w.kv_head = piece.tile_index % a.n_kv_heads;
+    w.tile = piece.tile_index / a.n_kv_heads % a.prefix_tiles;
+    const int group = piece.tile_index / a.n_kv_heads / a.prefix_tiles;
+    if (group >= a.n_groups) return;                          // uniform for the block, here and below: nothing is allocated yet
+    w.seq_first = a.group_first[group];
+    w.seq_last = a.group_first[group + 1];
+    if (w.seq_first >= w.seq_last) return;
+    w.first_token = a.cu_seqlens[w.seq_first];
+    w.n_rows = (a.cu_seqlens[w.seq_last] - w.first_token) * share;
+    const int row0 = w.tile * WIDE_ROWS, n_rows = min(WIDE_ROWS, w.n_rows - row0);
     if (n_rows <= 0) return;
-    const bool of_group = w.slot < a.prefix_splits;
+    const int n_tiles = n_rows > TC_ROWS ? 2 : 1;
     TileRange range;
     range.token_first = w.first_token + row0 / share;
     range.token_last = w.first_token + (row0 + n_rows - 1) / share;
-    range.seq_first = of_group ? sequence_of(a, w, range.token_first) : w.seq_first;
-    range.seq_last = of_group ? sequence_of(a, w, range.token_last) : w.seq_first;
-    range.own = !of_group || a.whole;
-    range.shared = of_group ? a.group_pages[group_of(a, w.seq_first)] : w.page_first;
-    // the slice of the walk that is this block's
-    int skip, n_blocks;
-    if (of_group) {
-        int total = range.shared;
-        if (a.whole) {
-            Walk all;
-            all.seq = -1;
-            while (next_stretch(a, range, all)) total += all.end - all.logical;
-        }
-        int per = (total + a.prefix_splits - 1) / a.prefix_splits;
-        skip = min(w.slot * per, total);
-        n_blocks = min(per, total - skip);
-    } else {
-        skip = w.page_begin - w.page_first;
-        n_blocks = w.page_end - w.page_begin;
+    range.seq_first = sequence_of(a, w, range.token_first);
+    range.seq_last = sequence_of(a, w, range.token_last);
+    range.own = a.whole;
+    range.shared = a.group_pages[group];
+    int total = range.shared;
+    if (a.whole) {
         Walk all;
-        own_stretch(a, range, w.seq_first, all);
-        n_blocks = max(0, min(n_blocks, all.end - w.page_begin));
+        all.seq = -1;
+        while (next_stretch(a, range, all)) total += all.end - all.logical;
     }
+    // pieces of whole pairs of pages
+    const int pairs = (total + 1) / 2, per = (pairs + piece.pieces - 1) / piece.pieces;
+    const int skip = min(piece.piece * per * 2, total), n_pages = min(per * 2, total - skip), n_blocks = (n_pages + 1) / 2;
     const int* shared_pages = a.block_table + (size_t)w.seq_first * a.table_stride;
-    Walk walk;
-    auto start_walk = [&]() {
-        if (of_group) {
-            start(a, range, walk, skip);
-        } else {
-            own_stretch(a, range, w.seq_first, walk);
-            walk.logical += skip;
-        }
-    };
     const int warp = warp_index(), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 14; ++i) mbar_init(smem_u32(&bars[i]), (i == 0 || i == 11 || i == 12) ? 128 : 1);
+        for (int i = 0; i < 18; ++i) {
+            bool by_softmax = i < 2 || (i >= 12 && i < 16);
+            mbar_init(smem_u32(&bars[i]), by_softmax ? 128 : 1);
+        }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -700,8 +756,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     // that wait for one another's would stand still.
     griddep_wait();
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tcgen05_fence_before();
@@ -710,218 +765,341 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     griddep_launch();
     uint32_t tmem_base = *tmem_slot;
 
-    if (warp == 0 || warp == 6) {
-        const bool keys = warp == 0;
-        const CUtensorMap* map = keys ? &map_k : &map_v;
-        unsigned char* tiles = keys ? k_tile : v_tile;
-        uint64_t* full = keys ? k_full : v_full;
-        uint64_t* empty = keys ? k_empty : v_empty;
-        if (n_blocks > 0) start_walk();
-        for (int kb = 0; kb < n_blocks; ++kb) {
-            int b = kb & 1;
-            const int* pages = walk.seq < 0 ? shared_pages : a.block_table + (size_t)walk.seq * a.table_stride;
-            int page = pages[walk.logical];
-            step(a, range, walk);
-            if (kb >= 2 && !mbar_wait_warp(smem_u32(&empty[b]), ((kb >> 1) - 1) & 1, abort_flag, status, keys ? 11 : 12)) break;
-            if (elect_one()) {
-                uint32_t bar = smem_u32(&full[b]);
-                mbar_expect_tx(bar, KV_BYTES);
-                int row = (page * a.n_kv_heads + w.kv_head) * LLMB_PAGE;
-                for (int h = 0; h < PIECES; ++h)
-                    tma_load_2d(smem_u32(tiles + b * KV_BYTES + h * KV_PIECE), map, bar, h * 64, row);
-            }
-            __syncwarp();
-        }
-    } else if (warp == 1) {
-        // D 32-bit, A and B bfloat16, M = 128; S has N = 64 keys, O has N = HD with B MN-major
-        constexpr uint32_t idesc_qk = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LLMB_PAGE >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
-        constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
-        const uint64_t q_desc = smem_desc(smem_u32(q_tile));
-        const uint64_t k_desc0 = smem_desc(smem_u32(k_tile)), v_desc0 = smem_desc_mn(smem_u32(v_tile), KV_PIECE);
-        constexpr uint64_t BUFFER = (uint64_t)(KV_BYTES >> 4);       // the second buffer, in the address field
-        auto issue_qk = [&](int kb) -> bool {
-            int b = kb & 1;
-            if (!mbar_wait_warp(smem_u32(&k_full[b]), (kb >> 1) & 1, abort_flag, status, 14)) return false;
-            tcgen05_fence_after();
-            if (elect_one()) {
-#pragma unroll
-                for (int j = 0; j < HD / 16; ++j) {
-                    uint64_t q_off = (uint64_t)(((j >> 2) * Q_PIECE + (j & 3) * 32) >> 4);
-                    uint64_t k_off = (uint64_t)(((j >> 2) * KV_PIECE + (j & 3) * 32) >> 4);
-                    tcgen05_mma(tmem_base + S_COL + b * LLMB_PAGE, q_desc + q_off, k_desc0 + b * BUFFER + k_off, idesc_qk, j > 0 ? 1u : 0u);
+    // page i of the piece: shared ones first, then what the walk finds behind them
+    struct Place {
+        int seq, logical, limit;
+    };
+    const int n_shared = max(0, min(n_pages, range.shared - skip));
+    Walk walk;
+    if (n_shared < n_pages) start(a, range, walk, skip + n_shared);
+    auto next_place = [&](int i) -> Place {
+        if (i < n_shared) return Place{-1, skip + i, 0x7fffffff};
+        Place at{walk.seq, walk.logical, walk.limit};
+        step(a, range, walk);
+        return at;
+    };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(WIDE_REGS_FEW));
+        if (warp == 0 || warp == 2) {
+            const bool keys = warp == 0;
+            const CUtensorMap* map = keys ? &map_k : &map_v;
+            unsigned char* tiles = keys ? k_tile : v_tile;
+            uint64_t* full = keys ? k_full : v_full;
+            uint64_t* empty = keys ? k_empty : v_empty;
+            auto next_page = [&](int i) {
+                Place at = next_place(i);
+                return (at.seq < 0 ? shared_pages : a.block_table + (size_t)at.seq * a.table_stride)[at.logical];
+            };
+            int first = n_pages > 0 ? next_page(0) : 0, second = n_pages > 1 ? next_page(1) : -1;
+            for (int kb = 0; kb < n_blocks; ++kb) {
+                int b = kb & 1, page0 = first, page1 = second;
+                // the numbers of the next pages are fetched under the wait for room
+                if (2 * kb + 2 < n_pages) first = next_page(2 * kb + 2);
+                second = 2 * kb + 3 < n_pages ? next_page(2 * kb + 3) : -1;
+                if (kb >= 2 && !mbar_wait_warp(smem_u32(&empty[b]), ((kb >> 1) - 1) & 1, abort_flag, status, keys ? 31 : 32)) break;
+                if (elect_one()) {
+                    uint32_t bar = smem_u32(&full[b]);
+                    mbar_expect_tx(bar, page1 >= 0 ? 2 * PAGE_BYTES : PAGE_BYTES);
+                    for (int h = 0; h < PIECES; ++h) {
+                        uint32_t to = smem_u32(tiles + b * PAIR_BYTES + h * PAIR_PIECE);
+                        tma_load_2d(to, map, bar, h * 64, (page0 * a.n_kv_heads + w.kv_head) * LLMB_PAGE);
+                        if (page1 >= 0) tma_load_2d(to + KV_PIECE, map, bar, h * 64, (page1 * a.n_kv_heads + w.kv_head) * LLMB_PAGE);
+                    }
                 }
-                tcgen05_commit(smem_u32(&s_full[b]));
-                tcgen05_commit(smem_u32(&k_empty[b]));
+                __syncwarp();
             }
-            __syncwarp();
-            return true;
-        };
-        bool ok = n_blocks > 0 && mbar_wait_warp(smem_u32(q_full), 0, abort_flag, status, 13) && issue_qk(0);
-        if (ok && n_blocks > 1) ok = issue_qk(1);
-        for (int kb = 0; kb < n_blocks && ok; ++kb) {
-            int b = kb & 1, phase = (kb >> 1) & 1;
-            ok = mbar_wait_warp(smem_u32(&p_full[b]), phase, abort_flag, status, 15);
-            ok = ok && mbar_wait_warp(smem_u32(&v_full[b]), phase, abort_flag, status, 16);
-            if (!ok) break;
-            tcgen05_fence_after();
-            if (elect_one()) {
+        } else if (warp == 1) {
+            // The tiles' products in turn, which keeps them half a period apart: with a warp for each both softmaxes ran at the same time
+            // and shared the special-function units while the tensor cores stood still (4,350 cycles a pair of pages).
+            constexpr uint32_t idesc_qk = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
+            constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
+            const uint64_t q_desc = smem_desc(smem_u32(q_tile));
+            const uint64_t k_desc0 = smem_desc(smem_u32(k_tile)), v_desc0 = smem_desc_mn(smem_u32(v_tile), PAIR_PIECE);
+            constexpr uint64_t BUFFER = (uint64_t)(PAIR_BYTES >> 4), Q_TILE = (uint64_t)(Q_BYTES >> 4);
+            auto issue_qk = [&](int tile, int kb) {
+                int b = kb & 1;
+                if (elect_one()) {
 #pragma unroll
-                for (int j = 0; j < LLMB_PAGE / 16; ++j)    // 16 keys a step: 8 columns of P, 2048 bytes of V rows
-                    tcgen05_mma_ts(tmem_base + O_COL, tmem_base + S_COL + b * LLMB_PAGE + j * 8,
-                                   v_desc0 + b * BUFFER + (uint64_t)((j * 2048) >> 4), idesc_pv, (kb > 0 || j > 0) ? 1u : 0u);
-                tcgen05_commit(smem_u32(o_full));
-                tcgen05_commit(smem_u32(&v_empty[b]));
+                    for (int j = 0; j < HD / 16; ++j) {
+                        uint64_t q_off = (uint64_t)(((j >> 2) * Q_PIECE + (j & 3) * 32) >> 4);
+                        uint64_t k_off = (uint64_t)(((j >> 2) * PAIR_PIECE + (j & 3) * 32) >> 4);
+                        tcgen05_mma(tmem_base + tile * SCORES, q_desc + tile * Q_TILE + q_off, k_desc0 + b * BUFFER + k_off, idesc_qk, j > 0 ? 1u : 0u);
+                    }
+                    tcgen05_commit(smem_u32(&s_full[tile]));
+                    if (tile == n_tiles - 1) tcgen05_commit(smem_u32(&k_empty[b]));
+                }
+                __syncwarp();
+            };
+            // the values of pair kb and the keys of the pair behind it are in shared memory
+            auto arrived = [&](int kb) {
+                return mbar_wait_warp(smem_u32(&v_full[kb & 1]), (kb >> 1) & 1, abort_flag, status, 36) &&
+                       (kb + 1 >= n_blocks || mbar_wait_warp(smem_u32(&k_full[(kb + 1) & 1]), ((kb + 1) >> 1) & 1, abort_flag, status, 37));
+            };
+            bool ok = n_blocks > 0 && mbar_wait_warp(smem_u32(&k_full[0]), 0, abort_flag, status, 34);
+            for (int tile = 0; tile < n_tiles && ok; ++tile) {
+                ok = mbar_wait_warp(smem_u32(&q_full[tile]), 0, abort_flag, status, 33);
+                if (!ok) break;
+                tcgen05_fence_after();
+                issue_qk(tile, 0);
             }
-            __syncwarp();
-            if (kb + 2 < n_blocks) ok = issue_qk(kb + 2);
+            ok = ok && arrived(0);
+            // A tile's products of pair kb, then its scores of the next pair. `masked`: pages that not all rows of the tile may be touched by, or a
+            // single page at the end; otherwise nothing is worked out between the waits (the tensor cores have work for some 500 cycles).
+            auto turn = [&](int tile, int kb, bool masked, bool two, const uint32_t (&off)[2][4]) -> bool {
+                const int b = kb & 1;
+                const uint32_t o = tmem_base + O_FIRST + tile * HD, p = tmem_base + tile * SCORES;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {        // 64 positions each: the first are multiplied while the others' weights are formed
+                    if (!mbar_wait_warp(smem_u32(&p_full[2 * tile + half]), kb & 1, abort_flag, status, 35)) return false;
+                    tcgen05_fence_after();
+                    // 16 positions a step: 8 columns of weights, 2048 bytes of value rows
+                    if (!masked) {
+                        if (elect_one()) {
+#pragma unroll
+                            for (int j = 4 * half; j < 4 * half + 4; ++j)
+                                tcgen05_mma_ts(o, p + j * 8, v_desc0 + b * BUFFER + (uint64_t)((j * 2048) >> 4), idesc_pv, 1u);
+                        }
+                    } else if ((half == 0 || two) && elect_one()) {
+#pragma unroll
+                        for (int j = 4 * half; j < 4 * half + 4; ++j)
+                            mma_ts_lanes(o, p + j * 8, v_desc0 + b * BUFFER + (uint64_t)((j * 2048) >> 4), idesc_pv, off[half]);
+                    }
+                    __syncwarp();
+                }
+                if (elect_one()) {
+                    if (kb == n_blocks - 1) tcgen05_commit(smem_u32(&o_full[tile]));
+                    if (tile == n_tiles - 1) tcgen05_commit(smem_u32(&v_empty[b]));
+                }
+                __syncwarp();
+                if (kb + 1 < n_blocks) {
+                    issue_qk(tile, kb + 1);
+                    // the next keys and values are waited for where products are under way
+                    if (tile == 0) return arrived(kb + 1);
+                }
+                return true;
+            };
+            // the rows of a tile that do not see a page, where the block has rows of several sequences
+            const bool mixed = range.seq_first != range.seq_last;
+            const int n_plain = mixed ? n_shared / 2 : n_pages / 2;              // pairs that every row may be touched by
+            uint32_t none[2][4] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
+            int kb = 0;
+            if (n_tiles == 2) {
+                for (; kb < n_plain && ok; ++kb) ok = turn(0, kb, false, true, none) && turn(1, kb, false, true, none);
+            } else {
+                for (; kb < n_plain && ok; ++kb) ok = turn(0, kb, false, true, none);
+            }
+            for (; kb < n_blocks && ok; ++kb) {
+                const bool two = 2 * kb + 1 < n_pages;
+                Place at[2];
+                at[0] = next_place(2 * kb);
+                if (two) at[1] = next_place(2 * kb + 1);
+                for (int tile = 0; tile < n_tiles && ok; ++tile) {
+                    uint32_t off[2][4] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if ((half && !two) || !mixed || at[half].seq < 0) continue;
+                        lanes_off((a.cu_seqlens[at[half].seq] - w.first_token) * share - row0 - tile * TC_ROWS,
+                                  (a.cu_seqlens[at[half].seq + 1] - w.first_token) * share - row0 - tile * TC_ROWS, off[half]);
+                    }
+                    ok = turn(tile, kb, true, two, off);
+                }
+            }
         }
     } else {
-        const int t = threadIdx.x - 64;                      // 0 .. 127
-        {   // the queries, 16 bytes at a time, where the 128-byte swizzle has them
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(WIDE_REGS_MANY));
+        const int tile = (warp >> 2) - 1, quarter = warp & 3, t = threadIdx.x & 127;
+        const int tile_rows = n_rows - tile * TC_ROWS;        // of this tile, above 128 where it is full
+        if (tile < n_tiles) {
             constexpr int CHUNKS = HD / 8;
             const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q);
+            unsigned char* to = q_tile + tile * Q_BYTES;
 #pragma unroll 4
             for (int i = t; i < TC_ROWS * CHUNKS; i += 128) {
                 int r = i / CHUNKS, c = i - r * CHUNKS;
                 uint4 value = make_uint4(0u, 0u, 0u, 0u);
-                if (r < n_rows) {
-                    int token = w.first_token + (row0 + r) / share, head = w.kv_head * share + (row0 + r) % share;
+                if (r < tile_rows) {
+                    int at = row0 + tile * TC_ROWS + r, token = w.first_token + at / share, head = w.kv_head * share + at % share;
                     value = *reinterpret_cast<const uint4*>(q + (size_t)token * a.q_stride + (size_t)head * HD + c * 8);
                 }
-                *reinterpret_cast<uint4*>(q_tile + (c >> 3) * Q_PIECE + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = value;
+                *reinterpret_cast<uint4*>(to + (c >> 3) * Q_PIECE + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = value;
             }
             fence_async_shared();
-            mbar_arrive(smem_u32(q_full));
-        }
-        int quarter = warp & 3;
-        int row = quarter * 32 + lane;                       // row of the tile = lane of tensor memory
-        const int token = w.first_token + (row0 + min(row, n_rows - 1)) / share;
-        const int my_seq = of_group ? sequence_of(a, w, token) : w.seq_first;
-        const int my_pos = row < n_rows ? a.seq_lens[my_seq] - a.cu_seqlens[my_seq + 1] + token : -1;
-        uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-        float run_max = -INFINITY, run_sum = 0.f;
-        bool ok = true;
-        if (n_blocks > 0) start_walk();
-        for (int kb = 0; kb < n_blocks && ok; ++kb) {
-            int b = kb & 1;
-            const int key0 = walk.logical * LLMB_PAGE, limit = walk.limit;
-            const int pos = walk.seq < 0 || walk.seq == my_seq ? my_pos : -1;         // what the row sees of this stretch
-            step(a, range, walk);
-            ok = mbar_wait(smem_u32(&s_full[b]), (kb >> 1) & 1, abort_flag, status, 17);
-            if (!ok) break;
-            __syncwarp();
-            tcgen05_fence_after();
-            const bool cut = key0 + LLMB_PAGE - 1 > limit;
-            if (quarter * 32 >= n_rows && !cut) {            // a warp without rows: its lanes' weights reach nobody's result
-                mbar_arrive(smem_u32(&p_full[b]));
-                continue;
+            mbar_arrive(smem_u32(&q_full[tile]));
+
+            const int r = quarter * 32 + lane;                // row of the tile = lane of tensor memory
+            const bool valid = r < tile_rows;
+            const int at = row0 + tile * TC_ROWS + (valid ? r : 0);
+            const int token = w.first_token + at / share, head = w.kv_head * share + at % share;
+            const int my_seq = sequence_of(a, w, token);
+            const int my_pos = valid ? a.seq_lens[my_seq] - a.cu_seqlens[my_seq + 1] + token : -1;
+            const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+            const uint32_t s_addr = lane_addr + tile * SCORES, o_addr = lane_addr + O_FIRST + tile * HD;
+            const bool idle = quarter * 32 >= tile_rows;      // a warp without rows: its lanes' weights reach nobody's result
+            {   // every product adds to O: it starts from zero
+                uint32_t zero[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) zero[j] = 0u;
+#pragma unroll
+                for (int c = 0; c < HD; c += 16) tmem_st16(o_addr + c, zero);
+                tmem_st_wait();
             }
-            bool whole = key0 + LLMB_PAGE - 1 <= pos;        // no key of the page is hidden from this row
-            uint32_t s_addr = lane_addr + S_COL + b * LLMB_PAGE;
-            uint32_t ra[32], rb[32];
-            tmem_ld32_start(s_addr, ra);
-            tmem_ld32_start(s_addr + 32, rb);
-            tmem_ld32_wait(ra);
-            tmem_ld32_wait(rb);
-            if (!whole) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    if (key0 + j > pos) ra[j] = __float_as_uint(-INFINITY);
-                    if (key0 + 32 + j > pos) rb[j] = __float_as_uint(-INFINITY);
+            const uint64_t scale2 = pair_of(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
+            float run_max = -INFINITY, run_sum = 0.f;
+            bool ok = true;
+            for (int kb = 0; kb < n_blocks && ok; ++kb) {
+                // the last key that the row sees of each of the two pages, from the page's first; positions stored behind it that no row sees
+                int pos0 = my_pos - (skip + 2 * kb) * LLMB_PAGE, pos1 = pos0 - LLMB_PAGE, stored0 = LLMB_PAGE, stored1 = LLMB_PAGE;
+                if (2 * kb + 1 >= n_shared) {
+                    Place at = next_place(2 * kb);
+                    pos0 = (at.seq < 0 || at.seq == my_seq ? my_pos : -1) - at.logical * LLMB_PAGE;
+                    stored0 = min(at.limit - at.logical * LLMB_PAGE, LLMB_PAGE - 1) + 1;
+                    pos1 = -1;
+                    if (2 * kb + 1 < n_pages) {
+                        at = next_place(2 * kb + 1);
+                        pos1 = (at.seq < 0 || at.seq == my_seq ? my_pos : -1) - at.logical * LLMB_PAGE;
+                        stored1 = min(at.limit - at.logical * LLMB_PAGE, LLMB_PAGE - 1) + 1;
+                    }
                 }
-            }
-            float block_max = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) block_max = max3(block_max, __uint_as_float(ra[j]), __uint_as_float(ra[j + 1]));
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) block_max = max3(block_max, __uint_as_float(rb[j]), __uint_as_float(rb[j + 1]));
-            // (a row that has seen no key yet keeps -inf, and all its weights are zero)
-            bool move = (block_max - run_max) * a.scale_log2 > 8.f;
-            float new_max = move ? block_max : run_max;
-            float alpha = move && kb > 0 ? fast_exp2((run_max - new_max) * a.scale_log2) : 1.f;
-            float shift = new_max == -INFINITY ? 0.f : new_max * a.scale_log2;
-            run_max = new_max;
-            float add = 0.f;
-            auto to_weights = [&](const uint32_t (&r)[32], int c) {
-                uint32_t packed[16];
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    float p0 = fast_exp2(fmaf(__uint_as_float(r[j]), a.scale_log2, -shift));
-                    float p1 = fast_exp2(fmaf(__uint_as_float(r[j + 1]), a.scale_log2, -shift));
-                    add += p0 + p1;
-                    packed[j >> 1] = pack2(p0, p1);
-                }
-                tmem_st16(s_addr + (c >> 1), packed);
-            };
-            to_weights(ra, 0);
-            to_weights(rb, 32);
-            run_sum = run_sum * alpha + add;
-            if (kb > 0) {
-                ok = mbar_wait(smem_u32(o_full), (kb - 1) & 1, abort_flag, status, 18);
+                ok = mbar_wait(smem_u32(&s_full[tile]), kb & 1, abort_flag, status, 38);
                 if (!ok) break;
                 __syncwarp();
                 tcgen05_fence_after();
-                if (__any_sync(0xffffffffu, alpha != 1.f)) {
+                if (stored0 < LLMB_PAGE || stored1 < LLMB_PAGE) {     // values behind the last position are whatever a page held: zero here
+                    ok = mbar_wait(smem_u32(&v_full[kb & 1]), (kb >> 1) & 1, abort_flag, status, 39);
+                    if (!ok) break;
+                    for (int half = 0; half < 2 && tile == 0; ++half) {       // (the first tile's products are issued first)
+                        int first = max(half ? stored1 : stored0, 0), chunks = (LLMB_PAGE - first) * 8;
+                        for (int i = t; i < PIECES * chunks; i += 128) {
+                            int h = i / chunks, rest = i - h * chunks;
+                            *reinterpret_cast<uint4*>(v_tile + (kb & 1) * PAIR_BYTES + h * PAIR_PIECE + half * KV_PIECE + first * 128 + rest * 16) =
+                                make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    }
+                    fence_async_shared();
+                }
+                if (idle) {
+                    mbar_arrive(smem_u32(&p_full[2 * tile]));
+                    mbar_arrive(smem_u32(&p_full[2 * tile + 1]));
+                } else {
+                    uint32_t r0[32], r1[32], r2[32], r3[32];
+                    // the second half of the scores comes while the first one's maximum is taken
+                    tmem_ld32_start(s_addr, r0);
+                    tmem_ld32_start(s_addr + 32, r1);
+                    tmem_ld32_wait(r0);
+                    tmem_ld32_wait(r1);
+                    tmem_ld32_start(s_addr + 64, r2);
+                    tmem_ld32_start(s_addr + 96, r3);
+                    if (pos0 < LLMB_PAGE - 1) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            if (j > pos0) r0[j] = __float_as_uint(-INFINITY);
+                            if (j + 32 > pos0) r1[j] = __float_as_uint(-INFINITY);
+                        }
+                    }
+                    float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        top0 = max3(top0, __uint_as_float(r0[j]), __uint_as_float(r0[j + 1]));
+                        top1 = max3(top1, __uint_as_float(r1[j]), __uint_as_float(r1[j + 1]));
+                    }
+                    tmem_ld32_wait(r2);
+                    tmem_ld32_wait(r3);
+                    if (pos1 < LLMB_PAGE - 1) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            if (j > pos1) r2[j] = __float_as_uint(-INFINITY);
+                            if (j + 32 > pos1) r3[j] = __float_as_uint(-INFINITY);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        top0 = max3(top0, __uint_as_float(r2[j]), __uint_as_float(r2[j + 1]));
+                        top1 = max3(top1, __uint_as_float(r3[j]), __uint_as_float(r3[j + 1]));
+                    }
+                    const float top = fmaxf(top0, top1);
+                    // (a row that has seen no key yet keeps -inf, and all its weights are zero)
+                    const bool move = (top - run_max) * a.scale_log2 > 8.f;
+                    const float new_max = move ? top : run_max;
+                    const float alpha = move ? fast_exp2((run_max - new_max) * a.scale_log2) : 1.f;
+                    const float shift = new_max == -INFINITY ? 0.f : -new_max * a.scale_log2;
+                    run_max = new_max;
+                    if (kb > 0 && __any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o_addr + c, o);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                            tmem_st16(o_addr + c, o);
+                        }
+                    }
+                    const uint64_t shift2 = pair_of(__float_as_uint(shift), __float_as_uint(shift));
+                    uint64_t add = pair_of(0u, 0u);
+                    auto to_weights = [&](const uint32_t (&x)[32], int c) {
+                        uint32_t packed[16];
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float p0, p1;
+                            unpair(fma2(pair_of(x[j], x[j + 1]), scale2, shift2), p0, p1);
+                            p0 = fast_exp2(p0);
+                            p1 = fast_exp2(p1);
+                            add = add2(add, pair_of(__float_as_uint(p0), __float_as_uint(p1)));
+                            packed[j >> 1] = pack2(p0, p1);
+                        }
+                        tmem_st16(s_addr + (c >> 1), packed);
+                    };
+                    to_weights(r0, 0);
+                    to_weights(r1, 32);
+                    tmem_st_wait();
+                    tcgen05_fence_before();
+                    mbar_arrive(smem_u32(&p_full[2 * tile]));
+                    to_weights(r2, 64);
+                    to_weights(r3, 96);
+                    float add_lo, add_hi;
+                    unpair(add, add_lo, add_hi);
+                    run_sum = run_sum * alpha + (add_lo + add_hi);
+                    tmem_st_wait();
+                    tcgen05_fence_before();
+                    mbar_arrive(smem_u32(&p_full[2 * tile + 1]));
+                }
+            }
+            if (ok && n_blocks > 0) ok = mbar_wait(smem_u32(&o_full[tile]), 0, abort_flag, status, 40);
+            if (ok && !idle) {
+                __syncwarp();
+                tcgen05_fence_after();
+                const bool direct = piece.pieces == 1 && a.whole;
+                const float inv = run_sum != 0.f ? 1.0f / run_sum : 0.f;
+                const size_t part_row = a.whole ? (size_t)(piece.tile_index - a.full_tiles) * WIDE_ROWS + (at - row0) : (size_t)token * a.n_heads + head;
+                const size_t slot = part_row * a.slots + piece.piece;
+                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD;
+                float* acc = a.acc + slot * HD;
+                if (valid && !direct) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(run_sum != 0.f ? run_max * a.scale_log2 : -INFINITY, run_sum);
+                if (direct || n_blocks > 0) {
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 32) {
-                        uint32_t r[32];
-                        tmem_ld32(lane_addr + O_COL + c, r);
+                        uint32_t x[32];
+                        if (n_blocks > 0) {
+                            tmem_ld32(o_addr + c, x);
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
-                        tmem_st32(lane_addr + O_COL + c, r);
-                    }
-                }
-            }
-            if (cut) {                                       // values behind the last position are whatever a page held: zero here
-                ok = mbar_wait(smem_u32(&v_full[b]), (kb >> 1) & 1, abort_flag, status, 20);
-                if (!ok) break;
-                int first = limit + 1 - key0;                // (a row of a piece is 128 bytes, its swizzle stays inside)
-                for (int i = t; i < PIECES * (LLMB_PAGE - first) * 8; i += 128) {
-                    int piece = i / ((LLMB_PAGE - first) * 8), rest = i - piece * (LLMB_PAGE - first) * 8;
-                    *reinterpret_cast<uint4*>(v_tile + b * KV_BYTES + piece * KV_PIECE + first * 128 + rest * 16) = make_uint4(0u, 0u, 0u, 0u);
-                }
-                fence_async_shared();
-            }
-            tmem_st_wait();
-            tcgen05_fence_before();
-            mbar_arrive(smem_u32(&p_full[b]));
-        }
-        if (ok && n_blocks > 0) ok = mbar_wait(smem_u32(o_full), (n_blocks - 1) & 1, abort_flag, status, 19);
-        if (ok && quarter * 32 < n_rows) {
-            __syncwarp();
-            tcgen05_fence_after();
-            const bool valid = row < n_rows;
-            const int head = w.kv_head * share + (row0 + row) % share;
-            const bool direct = a.slots == 1;
-            float inv = run_sum != 0.f ? 1.0f / run_sum : 0.f;
-            size_t slot = ((size_t)token * a.n_heads + head) * a.slots + w.slot;
-            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD;
-            float* acc = a.acc + slot * HD;
-            if (valid && !direct) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(run_sum != 0.f ? run_max * a.scale_log2 : -INFINITY, run_sum);
-            if (direct || n_blocks > 0) {
-#pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
-                    uint32_t r[32];
-                    if (n_blocks > 0) {
-                        tmem_ld32(lane_addr + O_COL + c, r);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = 0u;
-                    }
-                    if (valid && direct) {
-#pragma unroll
-                        for (int d = 0; d < 32; d += 8) {
-                            uint4 packed;
-                            packed.x = pack2(__uint_as_float(r[d]) * inv, __uint_as_float(r[d + 1]) * inv);
-                            packed.y = pack2(__uint_as_float(r[d + 2]) * inv, __uint_as_float(r[d + 3]) * inv);
-                            packed.z = pack2(__uint_as_float(r[d + 4]) * inv, __uint_as_float(r[d + 5]) * inv);
-                            packed.w = pack2(__uint_as_float(r[d + 6]) * inv, __uint_as_float(r[d + 7]) * inv);
-                            *reinterpret_cast<uint4*>(o + c + d) = packed;
+                            for (int j = 0; j < 32; ++j) x[j] = 0u;
                         }
-                    } else if (valid) {
+                        if (valid && direct) {
 #pragma unroll
-                        for (int d = 0; d < 32; d += 4)
-                            *reinterpret_cast<uint4*>(acc + c + d) = make_uint4(r[d], r[d + 1], r[d + 2], r[d + 3]);
+                            for (int d = 0; d < 32; d += 8) {
+                                uint4 packed;
+                                packed.x = pack2(__uint_as_float(x[d]) * inv, __uint_as_float(x[d + 1]) * inv);
+                                packed.y = pack2(__uint_as_float(x[d + 2]) * inv, __uint_as_float(x[d + 3]) * inv);
+                                packed.z = pack2(__uint_as_float(x[d + 4]) * inv, __uint_as_float(x[d + 5]) * inv);
+                                packed.w = pack2(__uint_as_float(x[d + 6]) * inv, __uint_as_float(x[d + 7]) * inv);
+                                *reinterpret_cast<uint4*>(o + c + d) = packed;
+                            }
+                        } else if (valid) {
+#pragma unroll
+                            for (int d = 0; d < 32; d += 4)
+                                *reinterpret_cast<uint4*>(acc + c + d) = make_uint4(x[d], x[d + 1], x[d + 2], x[d + 3]);
+                        }
                     }
                 }
             }
@@ -936,12 +1114,24 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     }
     if (warp == 1) {
         tcgen05_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(COLS) : "memory");
     }
 }
 
 // ------------------------------------------------------------------------------------------------ the parts joined
 //
+// The (token, head) of a row of parts, -1 if it has none: `whole` walks have parts for the tiles that are cut only.
+__device__ __forceinline__ int row_of_parts(const Args& a, int row, int n_rows) {
+    if (row >= n_rows) return -1;
+    if (!a.whole) return row;
+    int tile = a.full_tiles + row / WIDE_ROWS, share = a.n_heads / a.n_kv_heads;
+    int kv_head = tile % a.n_kv_heads, group = tile / a.n_kv_heads / a.prefix_tiles;
+    int at = tile / a.n_kv_heads % a.prefix_tiles * WIDE_ROWS + row % WIDE_ROWS;
+    int first = a.cu_seqlens[a.group_first[group]], last = a.cu_seqlens[a.group_first[group + 1]];
+    if (at >= (last - first) * share) return -1;
+    return (first + at / share) * a.n_heads + kv_head * share + at % share;
+}
+
 // WARPS warps a row: each reads all the maxima and sums, a lane a part, and takes every WARPS-th part, several of them in flight; their
 // sums are added in order. With one warp that read part after part the join of 34 parts of 512 rows took 25 us, more than the parts.
 template <typename T, int WARPS>
@@ -953,7 +1143,8 @@ __global__ void __launch_bounds__(256) prefix_attention_join_kernel(const __grid
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp % WARPS;
     const int row = blockIdx.x * ROWS + warp / WARPS;
     const int D = a.head_dim, slots = a.slots, width = (D + 3) / 4;
-    const bool valid = row < n_rows, vectors = D % 4 == 0;
+    const int of = row_of_parts(a, row, n_rows);
+    const bool valid = of >= 0, vectors = D % 4 == 0;
     float4 value[CHUNKS];
     float sum = 0.f;
 #pragma unroll
@@ -1028,7 +1219,7 @@ __global__ void __launch_bounds__(256) prefix_attention_join_kernel(const __grid
     }
     if (!valid) return;
     const float inv = sum != 0.f ? 1.f / sum : 0.f;
-    T* out = static_cast<T*>(a.out) + (size_t)(row / a.n_heads) * a.out_stride + (size_t)(row % a.n_heads) * D;
+    T* out = static_cast<T*>(a.out) + (size_t)(of / a.n_heads) * a.out_stride + (size_t)(of % a.n_heads) * D;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
         int col = (c * 32 + lane) * 4;
@@ -1041,17 +1232,20 @@ __global__ void __launch_bounds__(256) prefix_attention_join_kernel(const __grid
 
 // ------------------------------------------------------------------------------------------------ the call
 
+enum Kernel { CUDA_CORES, FEW, WIDE };
+
 struct Plan {
-    bool tc;                         // tensor cores
+    Kernel kernel;                   // of the shared pages
     bool whole;                      // a group's tiles walk the shared and the own pages, nothing is left for own parts
-    int prefix_tiles, prefix_splits, own_tiles, own_splits, slots;
+    int prefix_tiles, prefix_splits, own_tiles, own_splits, slots, full_tiles;
+    long long part_rows;             // rows that are joined from parts
 };
 
 constexpr int SMS = 148;
 
 struct Sizes {
     int n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own;
-    bool tc;                         // the tensor-core kernel can take the call
+    bool tc;                         // the tensor-core kernels can take the call
 };
 
 // the least power of two that is no less than n: replayed steps of one bucket make the same launches
@@ -1061,28 +1255,47 @@ int bucket(int n) {
     return b;
 }
 
-// Into how many parts the shared and the own pages are cut: as many pages a block as make all blocks come to about the blocks that the
-// SMs hold at once, two pages at least.
+// Which kernel, and into how many parts the shared and the own pages are cut: as many pages a block as make all blocks come to about the blocks
+// that the SMs hold at once, two pages at least.
 Plan plan_for(const Sizes& z) {
     Plan p;
     int share = z.n_heads / z.n_kv_heads;
     int shared = z.max_shared > 0 ? bucket(z.max_shared) : 0, own = bucket(ceil_div(z.max_own > 0 ? z.max_own : 1, LLMB_PAGE));
-    p.tc = z.tc;
-    int rows = p.tc ? TC_ROWS : SIMT_ROWS;
-    long long wave = (long long)SMS * (p.tc ? 2 : z.head_dim <= 64 ? 4 : z.head_dim <= 128 ? 2 : 1);
     // sequences that bring few rows each would leave a tile of a group to walk many sequences' pages for a few of its rows
-    p.whole = p.tc && (long long)z.max_new * share > 16;
+    p.whole = z.tc && (long long)z.max_new * share > FEW_ROWS;
+    p.kernel = !z.tc ? CUDA_CORES : p.whole || (shared > 0 && (long long)z.max_group * share > FEW_ROWS) ? WIDE : FEW;
+    int rows = p.kernel == WIDE ? WIDE_ROWS : p.kernel == FEW ? FEW_ROWS : SIMT_ROWS;
     p.prefix_tiles = shared > 0 || p.whole ? ceil_div((long long)z.max_group * share, rows) : 0;
-    p.own_tiles = p.whole ? 0 : ceil_div((long long)z.max_new * share, rows);
+    p.own_tiles = p.whole ? 0 : ceil_div((long long)z.max_new * share, z.tc ? FEW_ROWS : SIMT_ROWS);
+    p.full_tiles = 0;
     long long prefix = (long long)z.n_groups * p.prefix_tiles * z.n_kv_heads, owns = (long long)z.n_seqs * p.own_tiles * z.n_kv_heads;
     int walk = shared + (p.whole ? own : 0);
-    long long per = (prefix * walk + owns * own + wave - 1) / wave;
-    if (per < 2) per = 2;
-    p.prefix_splits = p.prefix_tiles > 0 ? ceil_div(walk, per) : 0;
-    p.own_splits = p.own_tiles > 0 ? ceil_div(own, per) : 0;
+    if (p.kernel == WIDE) {
+        // whole rounds of tiles as they are, the tiles of the last round cut so that they fill one, into four pages at least
+        p.full_tiles = p.whole ? (int)(prefix / SMS * SMS) : 0;
+        long long rest = prefix - p.full_tiles, best = 0;
+        p.prefix_splits = 1;
+        for (int n = 1; n <= MAX_SPLITS && (n == 1 || 4 * n <= walk) && rest > 0; ++n) {
+            // rounds of blocks times what one takes: its pages, and about eight pages' time for its start, its end and the join of a part more
+            long long time = (rest * n + SMS - 1) / SMS * (ceil_div(walk, n) + 8) + n;
+            if (n == 1 || time < best) {
+                best = time;
+                p.prefix_splits = n;
+            }
+        }
+        // own pages: a launch of their own, 32 pages a block at most
+        p.own_splits = p.own_tiles > 0 ? ceil_div(own, 32) : 0;
+    } else {
+        long long wave = (long long)SMS * (z.tc ? 2 : z.head_dim <= 64 ? 4 : z.head_dim <= 128 ? 2 : 1);
+        long long per = (prefix * walk + owns * own + wave - 1) / wave;
+        if (per < 2) per = 2;
+        p.prefix_splits = p.prefix_tiles > 0 ? ceil_div(walk, per) : 0;
+        p.own_splits = p.own_tiles > 0 ? ceil_div(own, per) : 0;
+    }
     if (p.prefix_splits > MAX_SPLITS) p.prefix_splits = MAX_SPLITS;
     if (p.own_splits > MAX_SPLITS) p.own_splits = MAX_SPLITS;
     p.slots = p.prefix_splits + p.own_splits;
+    p.part_rows = p.slots == 1 ? 0 : p.whole ? (prefix - p.full_tiles) * WIDE_ROWS : (long long)z.n_tokens * z.n_heads;
     return p;
 }
 
@@ -1103,13 +1316,16 @@ int launch_simt(const Args& a, unsigned blocks, cudaStream_t stream) {
 }
 
 template <int HD>
-int launch_tc(const Args& a, int n_pages, unsigned blocks, cudaStream_t stream) {
-    // (more than 80 KB: no third block lands on an SM and waits for tensor memory)
-    constexpr size_t smem = 1024 + tile_bytes<HD>() + 16 * 8;
-    static_assert(smem > 80 * 1024 && 2 * (smem + sizeof(Staged) + 1024) <= 227 * 1024, "two blocks an SM");
+int launch_tc(const Args& a, const Plan& p, int n_pages, unsigned blocks, cudaStream_t stream) {
+    constexpr size_t few = 1024 + Ring<HD>::BYTES + (2 * Ring<HD>::STAGES + 1) * 8;
+    static_assert(2 * (few + sizeof(Staged) + 1024) <= 227 * 1024, "two blocks an SM");
+    // (more than half of an SM's shared memory for the smaller head size too: tensor memory has room for one block)
+    constexpr size_t wide_need = 1024 + (HD / 64) * (2 * Q_PIECE + 4 * PAIR_PIECE) + 19 * 8, wide = wide_need < 120 * 1024 ? 120 * 1024 : wide_need;
+    static_assert(wide + sizeof(Staged) + 1024 <= 227 * 1024, "one block an SM");
     static bool configured = false;
     if (!configured) {
-        LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few));
+        LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_wide_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wide));
         configured = true;
     }
     CUtensorMap map_k, map_v;
@@ -1119,8 +1335,21 @@ int launch_tc(const Args& a, int n_pages, unsigned blocks, cudaStream_t stream) 
     if (code) return code;
     static int* status_dev = nullptr;
     if (!status_dev && status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status_dev, status_word(), 0));
-    llmb::launch(prefix_attention_tc_kernel<HD>, dim3(blocks), TC_THREADS, smem, stream, true, map_k, map_v, a, status_dev);
-    return check_launch("prefix_attention_tc");
+    if (p.kernel == WIDE) {
+        long long tiles = (long long)a.n_groups * a.prefix_tiles * a.n_kv_heads, wide_blocks = a.full_tiles + (tiles - a.full_tiles) * a.prefix_splits;
+        LLMB_REQUIRE(wide_blocks < (1ll << 31), "prefix_attention: too many blocks");
+        llmb::launch(prefix_attention_wide_kernel<HD>, dim3((unsigned)wide_blocks), WIDE_THREADS, wide, stream, true, map_k, map_v, a, status_dev);
+        if ((code = check_launch("prefix_attention_wide")) || a.own_tiles == 0) return code;
+        // the own parts: the blocks of the other kernel for them, the slots of the shared parts in front of theirs
+        Args own = a;
+        own.prefix_tiles = 0;
+        own.behind = pdl_enabled() ? 1 : 0;
+        blocks = (unsigned)((long long)a.n_kv_heads * a.n_seqs * a.own_tiles * a.own_splits);
+        llmb::launch(prefix_attention_few_kernel<HD>, dim3(blocks), FEW_THREADS, few, stream, true, map_k, map_v, own, status_dev);
+        return check_launch("prefix_attention_few");
+    }
+    llmb::launch(prefix_attention_few_kernel<HD>, dim3(blocks), FEW_THREADS, few, stream, true, map_k, map_v, a, status_dev);
+    return check_launch("prefix_attention_few");
 }
 
 // a warp for four parts, as many as fit
@@ -1132,19 +1361,18 @@ void launch_join(const Args& a, int rows, cudaStream_t stream) {
     else llmb::launch(prefix_attention_join_kernel<T, 8>, dim3(rows), 256, 0, stream, true, a, rows);
 }
 
-int run(const Args& a, const Plan& p, int dtype, int n_pages, int n_tokens, cudaStream_t stream) {
+int run(const Args& a, const Plan& p, int dtype, int n_pages, cudaStream_t stream) {
     long long blocks = (long long)a.n_kv_heads * ((long long)a.n_groups * a.prefix_tiles * a.prefix_splits + (long long)a.n_seqs * a.own_tiles * a.own_splits);
     LLMB_REQUIRE(blocks < (1ll << 31), "prefix_attention: too many blocks");
     const bool f32 = dtype == LLMB_DTYPE_F32;
     int code;
-    if (p.tc) code = a.head_dim == 64 ? launch_tc<64>(a, n_pages, (unsigned)blocks, stream) : launch_tc<128>(a, n_pages, (unsigned)blocks, stream);
+    if (p.kernel != CUDA_CORES) code = a.head_dim == 64 ? launch_tc<64>(a, p, n_pages, (unsigned)blocks, stream) : launch_tc<128>(a, p, n_pages, (unsigned)blocks, stream);
     else if (a.head_dim <= 64) code = f32 ? launch_simt<float, 64>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 64>(a, (unsigned)blocks, stream);
     else if (a.head_dim <= 128) code = f32 ? launch_simt<float, 128>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 128>(a, (unsigned)blocks, stream);
     else code = f32 ? launch_simt<float, 256>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 256>(a, (unsigned)blocks, stream);
     if (code || a.slots == 1) return code;
-    int rows = n_tokens * a.n_heads;
-    if (f32) launch_join<float>(a, rows, stream);
-    else launch_join<__nv_bfloat16>(a, rows, stream);
+    if (f32) launch_join<float>(a, (int)p.part_rows, stream);
+    else launch_join<__nv_bfloat16>(a, (int)p.part_rows, stream);
     return check_launch("prefix_attention_join");
 }
 
@@ -1170,7 +1398,8 @@ LLMB_EXPORT long long llmb_prefix_attention_scratch_floats(int n_tokens, int n_s
     if (n_tokens <= 0 || n_seqs <= 0 || n_groups <= 0 || n_kv_heads <= 0 || n_heads < n_kv_heads) return 0;
     Plan p = plan_for(Sizes{n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own, tc != 0});
     if (p.slots > 1) ++*kernels;
-    return p.slots > 1 ? scratch_floats_of((long long)n_tokens * n_heads * p.slots, head_dim) : 0;
+    if (p.kernel == WIDE && p.own_tiles > 0) ++*kernels;
+    return scratch_floats_of(p.part_rows * p.slots, head_dim);
 }
 
 // tc: what llmb_prefix_attention_tc_serves said, 0 to keep to the CUDA cores.
@@ -1192,15 +1421,17 @@ LLMB_EXPORT int llmb_prefix_attention(const void* q, int q_stride, const void* k
                  "prefix_attention: the tensor-core kernel does not take these operands");
     LLMB_REQUIRE(n_pages > 0 && (long long)n_pages * n_kv_heads * LLMB_PAGE < (1ll << 31), "prefix_attention: %d pages", n_pages);
     Plan p = plan_for(Sizes{n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own, tc != 0});
-    long long rows = (long long)n_tokens * n_heads;
-    LLMB_REQUIRE(p.slots == 1 || (scratch != nullptr && aligned(scratch) && scratch_floats >= scratch_floats_of(rows * p.slots, head_dim)),
+    const long long parts = p.part_rows * p.slots;
+    LLMB_REQUIRE(p.part_rows < (1ll << 31), "prefix_attention: %lld rows of parts", p.part_rows);
+    LLMB_REQUIRE(parts == 0 || (scratch != nullptr && aligned(scratch) && scratch_floats >= scratch_floats_of(parts, head_dim)),
                  "prefix_attention: scratch too small");
     int size = dtype == LLMB_DTYPE_F32 ? 4 : 2;
     bool vectors = (head_dim * size) % 16 == 0 && aligned(k_cache) && aligned(v_cache);
-    Args a{q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, out, scratch, scratch + value_floats(rows * p.slots, head_dim),
+    Args a{q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, out, scratch, scratch + value_floats(parts, head_dim),
            q_stride, out_stride, table_stride, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, scale * LOG2E,
-           p.prefix_tiles, p.prefix_splits, p.own_tiles, p.own_splits, p.slots, vectors ? 1 : 0, p.whole ? 1 : 0};
-    return run(a, p, dtype, n_pages, n_tokens, stream);
+           p.prefix_tiles, p.prefix_splits, p.own_tiles, p.own_splits, p.slots, vectors ? 1 : 0, p.full_tiles,
+           0, p.whole ? 1 : 0};
+    return run(a, p, dtype, n_pages, stream);
 }
 
 // the packed doors of the launching entry points (common.cuh)
