@@ -45,6 +45,7 @@ struct Args {
     int prefix_tiles, prefix_splits, own_tiles, own_splits, slots;
     int vectors;                     // the caches' rows can be read 16 bytes at a time
     int full_tiles;                  // tiles of the wide kernel whose walk is one block's; the others are cut into prefix_splits pieces
+    int even_blocks;                 // > 0: so many blocks share the groups' pages in slices of equal length, else every group is cut into prefix_splits
     int behind;                      // own parts launched behind the wide kernel, which has waited for all that they read
     int whole;                       // a tile of a group walks its sequences' own pages behind the shared ones (tensor cores)
 };
@@ -72,7 +73,7 @@ __device__ __forceinline__ int group_of(const Args& a, int seq) {
 __device__ __forceinline__ bool item_of(const Args& a, int x, Item& w) {
     w.kv_head = x % a.n_kv_heads;
     x /= a.n_kv_heads;
-    int prefix_blocks = a.n_groups * a.prefix_tiles * a.prefix_splits;
+    int prefix_blocks = a.even_blocks ? 0 : a.n_groups * a.prefix_tiles * a.prefix_splits;
     int share = a.n_heads / a.n_kv_heads;
     if (x < prefix_blocks) {
         w.tiles = a.prefix_tiles;
@@ -315,17 +316,29 @@ __global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(con
     }
 }
 
-// ------------------------------------------------------------------------------------------------ bfloat16, few rows
+// ------------------------------------------------------------------------------------------------ bfloat16, up to 128 rows
 //
-// Items of 64 rows or fewer (a sequence's own pages in a decode step; the shared pages of a few samples) are bound by reading their pages.
-// Warp 4 keeps a ring of pages in flight (TMA, 64 x 64 boxes with the 128-byte swizzle); warps 0 to 3 take 16 rows and a share of a
-// page's keys each with mma.sync.m16n8k16: 16 keys where the item has up to 16 rows, 32 up to 32, all 64 above. Each keeps a maximum,
-// a sum and weighted values of its own, in 32 bits, and those of the same rows are merged at the end. Weights are rounded to 8 bits, what the
-// tensor cores take; their sum is of the unrounded ones.
+// What a decode step brings: a group's shared pages against up to 128 rows, a sequence's own pages against up to 16. Reading the pages is the
+// work; two blocks an SM hold a slice of pages each.
+//
+// Items of 16 rows or fewer (prefix_attention_few_kernel): warp 4 keeps a ring of pages in flight (TMA, 64 x 64 boxes with the 128-byte
+// swizzle); warps 0 to 3 take 16 of a page's 64 keys each with mma.sync.m16n8k16 and keep a maximum, a sum and weighted values of their own, in
+// 32 bits, which are merged at the end. mma.sync stands up to that many rows: with 64 rows a page took four times as long as on tcgen05.
+//
+// Items of more rows (prefix_attention_tile_kernel): S[128, 64 keys] = Q K^T into one of two buffers of scores in tensor memory (warp 1), the
+// weights written over them by a thread a row (warps 2 to 5; those without rows only pass the word on), O[128, D] += P V with P from tensor
+// memory. The scores of the page after the next are issued behind P V of this one.
+//
+// In both, weights are rounded to 8 bits, what the tensor cores take, and their sum is of the unrounded ones. The two are kernels of their own:
+// as branches of one, the own pages of a step took a third longer.
 
+constexpr int TC_ROWS = 128;                      // lanes of tensor memory
 constexpr int KV_PIECE = LLMB_PAGE * 64 * 2;      // a page, 64 columns of the head: 8 KB
-constexpr int FEW_ROWS = 64, FEW_THREADS = 160;
+constexpr int Q_PIECE = TC_ROWS * 64 * 2;         // 128 rows, 64 columns of the head: 16 KB
+constexpr int FEW_ROWS = 16, FEW_THREADS = 160, TILE_THREADS = 192;
 constexpr int FEW_WARPS = 4;
+// tensor memory of an item: two buffers of scores (64 columns of 32-bit values, the weights over the first 32), O beside them
+constexpr uint32_t S_COL = 0, O_COL = 128, TMEM_COLS = 256;
 
 // where element (row, col) of a page lies in shared memory: pieces of 64 columns, 16-byte chunks swizzled by the row
 __device__ __forceinline__ const unsigned char* swizzled(const unsigned char* page, int row, int col) {
@@ -338,10 +351,11 @@ template <int HD> struct Ring {
     static constexpr int MERGE = FEW_WARPS * 16 * (HD + 8 + 2) * 4;
     static constexpr int BYTES = STAGE * STAGES;
     static_assert(MERGE <= BYTES, "the merge takes the ring's place");
+    static_assert((HD / 64) * (Q_PIECE + 4 * KV_PIECE) <= BYTES, "the queries and two pages");
 };
 
 // The arrays that say which sequences there are, in shared memory (one round of loads) where there is room.
-constexpr int STAGED_SEQS = 128;
+constexpr int STAGED_SEQS = 512;
 struct Staged {
     int seq_lens[STAGED_SEQS], cu_seqlens[STAGED_SEQS + 1], group_first[STAGED_SEQS + 1], group_pages[STAGED_SEQS];
 };
@@ -360,6 +374,75 @@ __device__ __forceinline__ void stage_arrays(Args& a, Staged& s) {
     a.group_pages = s.group_pages;
 }
 
+// Slices of equal length of groups of unequal ones: `per` pages each, the least number (two at least) with which all groups' slices fit into the
+// blocks that there are for a key head, or a group's all. Each warp finds out for itself, a lane a group. w: the slice's group and pages; *pieces:
+// the slices of the group; false where nothing is left for the block.
+__device__ __forceinline__ bool even_slice_of(const Args& a, int x, int lane, Item& w, int& pieces) {
+    const unsigned all = 0xffffffffu;
+    const int share = a.n_heads / a.n_kv_heads, heads = a.even_blocks / a.n_kv_heads;          // blocks of a key head
+    auto pages_of = [&](int g) { return g < a.n_groups && a.cu_seqlens[a.group_first[g + 1]] > a.cu_seqlens[a.group_first[g]] ? a.group_pages[g] : 0; };
+    int work = 0, items = 0, most = 0;
+    for (int g0 = 0; g0 < a.n_groups; g0 += 32) {
+        int pages = pages_of(g0 + lane);
+        work += __reduce_add_sync(all, pages);
+        items += __popc(__ballot_sync(all, pages > 0));
+        most = max(most, __reduce_max_sync(all, pages));
+    }
+    int per = items < heads ? (work + heads - items - 1) / (heads - items) : most;
+    per = max(max(per, 2), (most + a.prefix_splits - 1) / a.prefix_splits);
+    w.kv_head = x % a.n_kv_heads;
+    x /= a.n_kv_heads;
+    for (int g0 = 0; g0 < a.n_groups; g0 += 32) {
+        int pages = pages_of(g0 + lane), mine = (pages + per - 1) / per, before = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            int left = __shfl_up_sync(all, before, d);
+            if (lane >= d) before += left;
+        }
+        unsigned beyond = __ballot_sync(all, x < before);
+        if (!beyond) {
+            x -= __shfl_sync(all, before, 31);
+            continue;
+        }
+        int at = __ffs(beyond) - 1;
+        pieces = __shfl_sync(all, mine, at);
+        x -= __shfl_sync(all, before - mine, at);
+        pages = __shfl_sync(all, pages, at);
+        w.seq_first = a.group_first[g0 + at];
+        w.seq_last = a.group_first[g0 + at + 1];
+        w.page_first = 0;
+        w.page_begin = min(x * per, pages);
+        w.page_end = min(x * per + per, pages);
+        w.slot = x;
+        w.tile = 0;
+        w.tiles = 1;
+        w.first_token = a.cu_seqlens[w.seq_first];
+        w.n_rows = (a.cu_seqlens[w.seq_last] - w.first_token) * share;
+        return true;
+    }
+    return false;
+}
+
+// A part's maximum and sum. Where slices are of equal length, the last one of a group leaves the parts that it has fewer than there is room for, and
+// the own part of a sequence that shares nothing those of the shared pages.
+__device__ __forceinline__ void put_stats(const Args& a, const Item& w, int pieces, size_t row, float m, float sum) {
+    float2* stats = reinterpret_cast<float2*>(a.stats) + row * a.slots;
+    stats[w.slot] = make_float2(sum != 0.f ? m : -INFINITY, sum);
+    if (!a.even_blocks) return;
+    int first = a.prefix_splits;
+    if (w.slot == a.prefix_splits && w.page_first == 0) first = 0;
+    else if (w.slot == pieces - 1) first = pieces;
+    for (int i = first; i < a.prefix_splits; ++i) stats[i] = make_float2(-INFINITY, 0.f);
+}
+
+// The block's slice; uniform for the block. *pieces: of a group whose slices are dealt out.
+__device__ __forceinline__ bool slice_of(const Args& a, Item& w, int& pieces) {
+    int x = blockIdx.x - (a.prefix_tiles > 0 ? a.even_blocks : 0);
+    pieces = 0;
+    return (x < 0 ? even_slice_of(a, blockIdx.x, threadIdx.x & 31, w, pieces) : item_of(a, x, w)) && w.n_rows > 0;
+}
+
+// Up to 16 rows over the pages [page_begin, page_end) of one table.
 template <int HD>
 __global__ void __launch_bounds__(FEW_THREADS, 2)
 prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -385,10 +468,10 @@ prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __g
     Args a = args;
     stage_arrays(a, staged);                                 // (lengths, groups and tables are not written by the kernels of a step)
     Item w;
-    bool work = item_of(a, blockIdx.x, w);                   // uniform for the block
-    work = work && w.n_rows > 0 && w.n_rows <= FEW_ROWS;
+    int pieces;
+    const bool work = slice_of(a, w, pieces);
     __syncthreads();
-    // Behind the wide kernel's shared parts the own ones may run beside them: that kernel lets them start when the one in front of it is
+    // Behind the kernel of the shared parts the own ones may run beside them: that kernel lets them start when the one in front of it is
     // complete. Each block waits for it at its end, so that the join waits for both.
     if (!a.behind || !work) griddep_wait();
     if (!work) return;
@@ -398,10 +481,8 @@ prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __g
     int limit = w.page_end * LLMB_PAGE - 1;                  // the last position that a row sees of these pages
     if (own) limit = min(limit, a.seq_lens[w.seq_first] - a.cu_seqlens[w.seq_first + 1] + last_token);
     const int n_pages = min(w.page_end, limit < 0 ? 0 : limit / LLMB_PAGE + 1) - w.page_begin;
-    const int row_groups = w.n_rows <= 16 ? 1 : w.n_rows <= 32 ? 2 : 4;
 
-    const int g = lane >> 2, t = lane & 3;
-    const int rows0 = warp % row_groups * 16, keys0 = warp / row_groups * 16 * row_groups;      // this warp's rows and keys of a page
+    const int g = lane >> 2, t = lane & 3, part = warp;      // warps 0 to 3: 16 keys of every page
     float acc[HD / 8][4], run_max[2] = {-INFINITY, -INFINITY}, run_sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n)
@@ -429,7 +510,7 @@ prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         int pos[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            int r = rows0 + g + half * 8;
+            int r = g + half * 8;
             bool valid = r < w.n_rows;
             int token = w.first_token + (valid ? r : 0) / share, head = w.kv_head * share + (valid ? r : 0) % share;
             pos[half] = valid ? position_of(a, w, token) : -1;
@@ -440,21 +521,18 @@ prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __g
                 qa[ks][2 + half] = valid ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8 + 2 * t) : 0u;
             }
         }
-        bool ok = rows0 < w.n_rows;                          // (a warp without rows only lets the ring go on)
         for (int i = 0; i < n_pages; ++i) {
             int stage = i % STAGES;
             if (!mbar_wait_warp(smem_u32(&full[stage]), (i / STAGES) & 1, abort_flag, status, 22)) break;
             const unsigned char* k_page = base + stage * STAGE;
             const unsigned char* v_page = k_page + PIECES * KV_PIECE;
-#pragma unroll 1
-            for (int part = 0; part < row_groups; ++part) {
-                const int in_page = keys0 + part * 16, key0 = (w.page_begin + i) * LLMB_PAGE + in_page;
-                if (!ok || key0 > limit) break;
+            const int key0 = (w.page_begin + i) * LLMB_PAGE + part * 16;
+            if (key0 <= limit) {
                 float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks) {
                     uint32_t b[4];
-                    ldmatrix_x4(b, swizzled(k_page, in_page + (lane >> 4) * 8 + (lane & 7), ks * 16 + ((lane >> 3) & 1) * 8));
+                    ldmatrix_x4(b, swizzled(k_page, part * 16 + (lane >> 4) * 8 + (lane & 7), ks * 16 + ((lane >> 3) & 1) * 8));
                     mma_bf16(s0, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[0], b[1]);
                     mma_bf16(s1, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[2], b[3]);
                 }
@@ -499,7 +577,7 @@ prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __g
 #pragma unroll
                 for (int n = 0; n < HD / 8; n += 2) {
                     uint32_t b[4];
-                    ldmatrix_x4_trans(b, swizzled(v_page, in_page + ((lane >> 3) & 1) * 8 + (lane & 7), (n + (lane >> 4)) * 8));
+                    ldmatrix_x4_trans(b, swizzled(v_page, part * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), (n + (lane >> 4)) * 8));
                     if (cut) {
                         b[0] &= keep_low;
                         b[1] &= keep_high;
@@ -529,7 +607,7 @@ prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         for (int half = 0; half < 2; ++half) {
             run_sum[half] += __shfl_xor_sync(0xffffffffu, run_sum[half], 1);
             run_sum[half] += __shfl_xor_sync(0xffffffffu, run_sum[half], 2);
-            int r = warp * 16 + g + half * 8;
+            int r = part * 16 + g + half * 8;
 #pragma unroll
             for (int n = 0; n < HD / 8; ++n)
                 *reinterpret_cast<float2*>(merge_acc + r * LD + n * 8 + 2 * t) = make_float2(acc[n][2 * half], acc[n][2 * half + 1]);
@@ -542,19 +620,20 @@ prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __g
     __syncthreads();
     for (int i = threadIdx.x; i < w.n_rows * (HD / 4); i += FEW_THREADS) {
         int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
-        int at = (r >> 4) * 16 + (r & 15);                   // of the row's first warp; its others follow row_groups warps behind
         float m = -INFINITY;
-        for (int k = r >> 4; k < FEW_WARPS; k += row_groups) m = fmaxf(m, merge_max[k * 16 + (r & 15)]);
+#pragma unroll
+        for (int k = 0; k < FEW_WARPS; ++k) m = fmaxf(m, merge_max[k * 16 + r]);
         float against = m == -INFINITY ? 0.f : m, sum = 0.f;
         float4 value = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = r >> 4; k < FEW_WARPS; k += row_groups, at += row_groups * 16) {
-            float weight = fast_exp2(merge_max[at] - against);
-            float4 x = *reinterpret_cast<const float4*>(merge_acc + at * LD + d);
+#pragma unroll
+        for (int k = 0; k < FEW_WARPS; ++k) {
+            float weight = fast_exp2(merge_max[k * 16 + r] - against);
+            float4 x = *reinterpret_cast<const float4*>(merge_acc + (k * 16 + r) * LD + d);
             value.x = fmaf(x.x, weight, value.x);
             value.y = fmaf(x.y, weight, value.y);
             value.z = fmaf(x.z, weight, value.z);
             value.w = fmaf(x.w, weight, value.w);
-            sum += merge_sum[at] * weight;
+            sum += merge_sum[k * 16 + r] * weight;
         }
         int token = w.first_token + r / share, head = w.kv_head * share + r % share;
         if (a.slots == 1) {
@@ -562,12 +641,265 @@ prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __g
             uint2 packed = make_uint2(pack2(value.x * inv, value.y * inv), pack2(value.z * inv, value.w * inv));
             *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD + d) = packed;
         } else {
-            size_t slot = ((size_t)token * a.n_heads + head) * a.slots + w.slot;
-            if (sum != 0.f) *reinterpret_cast<float4*>(a.acc + slot * HD + d) = value;
-            if (d == 0) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(m, sum);
+            size_t row = (size_t)token * a.n_heads + head;
+            if (sum != 0.f) *reinterpret_cast<float4*>(a.acc + (row * a.slots + w.slot) * HD + d) = value;
+            if (d == 0) put_stats(a, w, pieces, row, m, sum);
         }
     }
     if (a.behind) griddep_wait();
+}
+
+// Up to 128 rows over a group's shared pages [page_begin, page_end).
+template <int HD>
+__global__ void __launch_bounds__(TILE_THREADS, 2)
+prefix_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                             const __grid_constant__ Args args, int* status) {
+    constexpr int PIECES = HD / 64, KV_BYTES = PIECES * KV_PIECE;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + Ring<HD>::BYTES);         // 14 barriers and two words
+    unsigned char* q_tile = base;
+    unsigned char* k_tile = base + PIECES * Q_PIECE;
+    unsigned char* v_tile = k_tile + 2 * KV_BYTES;
+    uint64_t* q_full = bars;                  // the queries are in shared memory
+    uint64_t* k_full = bars + 1;              // [2]
+    uint64_t* k_empty = bars + 3;             // [2]
+    uint64_t* v_full = bars + 5;              // [2]
+    uint64_t* v_empty = bars + 7;             // [2]
+    uint64_t* s_full = bars + 9;              // [2] a buffer's scores are complete
+    uint64_t* p_full = bars + 11;             // [2] its weights are written and O has been rescaled
+    uint64_t* o_full = bars + 13;             // a page's P V has been added to O
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+#pragma unroll 1
+        for (int i = 0; i < 14; ++i) mbar_init(smem_u32(&bars[i]), (i == 0 || i == 11 || i == 12) ? 128 : 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __shared__ Staged staged;
+    Args a = args;
+    stage_arrays(a, staged);
+    Item w;
+    int pieces;
+    const bool work = slice_of(a, w, pieces);                // nothing is allocated where a block leaves
+    const int share = a.n_heads / a.n_kv_heads, n_pages = work ? w.page_end - w.page_begin : 0;
+    // Tensor memory is taken when the kernel in front is done with it, and the next kernel may take some only when this one has it: two
+    // that wait for one another's would stand still.
+    griddep_wait();
+    if (n_pages <= 0) {                                      // a slice beyond the group's pages, where all groups are cut alike
+        for (int r = threadIdx.x; work && r < w.n_rows; r += TILE_THREADS)
+            put_stats(a, w, pieces, (size_t)(w.first_token + r / share) * a.n_heads + w.kv_head * share + r % share, -INFINITY, 0.f);
+        return;
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    griddep_launch();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        const int* pages = a.block_table + (size_t)w.seq_first * a.table_stride + w.page_begin;
+        int numbers = lane < n_pages ? pages[lane] : 0;      // 32 places of the table at once
+        for (int kb = 0; kb < n_pages; ++kb) {
+            const int b = kb & 1, phase = ((kb >> 1) - 1) & 1;
+            if (kb > 0 && (kb & 31) == 0) numbers = kb + lane < n_pages ? pages[kb + lane] : 0;
+            const int row = (__shfl_sync(0xffffffffu, numbers, kb & 31) * a.n_kv_heads + w.kv_head) * LLMB_PAGE;
+            for (int of = 0; of < 2; ++of) {                 // keys, values
+                if (kb >= 2 && !mbar_wait_warp(smem_u32(of ? &v_empty[b] : &k_empty[b]), phase, abort_flag, status, 11 + of)) break;
+                if (elect_one()) {
+                    uint32_t bar = smem_u32(of ? &v_full[b] : &k_full[b]);
+                    mbar_expect_tx(bar, KV_BYTES);
+                    for (int h = 0; h < PIECES; ++h)
+                        tma_load_2d(smem_u32((of ? v_tile : k_tile) + b * KV_BYTES + h * KV_PIECE), of ? &map_v : &map_k, bar, h * 64, row);
+                }
+                __syncwarp();
+            }
+            if (*abort_flag) break;
+        }
+    } else if (warp == 1) {
+        // D 32-bit, A and B bfloat16, M = 128; S has N = 64 keys, O has N = HD with B MN-major
+        constexpr uint32_t idesc_qk = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(LLMB_PAGE >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
+        constexpr uint32_t idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(TC_ROWS >> 4) << 24);
+        const uint64_t q_desc = smem_desc(smem_u32(q_tile));
+        const uint64_t k_desc0 = smem_desc(smem_u32(k_tile)), v_desc0 = smem_desc_mn(smem_u32(v_tile), KV_PIECE);
+        constexpr uint64_t BUFFER = (uint64_t)(KV_BYTES >> 4);       // the second buffer, in the address field
+        auto issue_qk = [&](int kb) -> bool {
+            int b = kb & 1;
+            if (!mbar_wait_warp(smem_u32(&k_full[b]), (kb >> 1) & 1, abort_flag, status, 14)) return false;
+            tcgen05_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int j = 0; j < HD / 16; ++j) {
+                    uint64_t q_off = (uint64_t)(((j >> 2) * Q_PIECE + (j & 3) * 32) >> 4);
+                    uint64_t k_off = (uint64_t)(((j >> 2) * KV_PIECE + (j & 3) * 32) >> 4);
+                    tcgen05_mma(tmem_base + S_COL + b * LLMB_PAGE, q_desc + q_off, k_desc0 + b * BUFFER + k_off, idesc_qk, j > 0 ? 1u : 0u);
+                }
+                tcgen05_commit(smem_u32(&s_full[b]));
+                tcgen05_commit(smem_u32(&k_empty[b]));
+            }
+            __syncwarp();
+            return true;
+        };
+        bool ok = mbar_wait_warp(smem_u32(q_full), 0, abort_flag, status, 13) && issue_qk(0);
+        if (ok && n_pages > 1) ok = issue_qk(1);
+        for (int kb = 0; kb < n_pages && ok; ++kb) {
+            int b = kb & 1, phase = (kb >> 1) & 1;
+            ok = mbar_wait_warp(smem_u32(&p_full[b]), phase, abort_flag, status, 15);
+            ok = ok && mbar_wait_warp(smem_u32(&v_full[b]), phase, abort_flag, status, 16);
+            if (!ok) break;
+            tcgen05_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int j = 0; j < LLMB_PAGE / 16; ++j)    // 16 keys a step: 8 columns of weights, 2048 bytes of value rows
+                    tcgen05_mma_ts(tmem_base + O_COL, tmem_base + S_COL + b * LLMB_PAGE + j * 8,
+                                   v_desc0 + b * BUFFER + (uint64_t)((j * 2048) >> 4), idesc_pv, (kb > 0 || j > 0) ? 1u : 0u);
+                tcgen05_commit(smem_u32(o_full));
+                tcgen05_commit(smem_u32(&v_empty[b]));
+            }
+            __syncwarp();
+            if (kb + 2 < n_pages) ok = issue_qk(kb + 2);
+        }
+    } else {
+        constexpr int CHUNKS = HD / 8, STEP = 128 / CHUNKS;
+        const int t = threadIdx.x - 64;                      // 0 .. 127
+        {   // the queries, 16 bytes at a time, where the 128-byte swizzle has them
+            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q);
+            const int c = t % CHUNKS, more_tokens = STEP / share, more_heads = STEP % share;
+            int token0 = w.first_token + t / CHUNKS / share, head0 = t / CHUNKS % share;
+#pragma unroll 1
+            for (int r = t / CHUNKS; r < TC_ROWS; r += STEP) {
+                unsigned char* chunk = q_tile + (c >> 3) * Q_PIECE + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                if (r < w.n_rows) cp_async16(chunk, q + (size_t)token0 * a.q_stride + (size_t)(w.kv_head * share + head0) * HD + c * 8);
+                else *reinterpret_cast<uint4*>(chunk) = make_uint4(0u, 0u, 0u, 0u);
+                token0 += more_tokens;
+                head0 += more_heads;
+                if (head0 >= share) {
+                    head0 -= share;
+                    ++token0;
+                }
+            }
+            cp_async_commit();
+        }
+        const int quarter = warp & 3, row = quarter * 32 + lane;             // row of the tile = lane of tensor memory
+        const int token = w.first_token + min(row, w.n_rows - 1) / share;
+        const int my_pos = row < w.n_rows ? position_of(a, w, token) : -1;
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        const bool idle = quarter * 32 >= w.n_rows;          // a warp without rows: its lanes' weights reach nobody's result
+        float run_max = -INFINITY, run_sum = 0.f;
+        cp_async_wait<0>();
+        fence_async_shared();
+        mbar_arrive(smem_u32(q_full));
+        bool ok = true;
+        for (int kb = 0; kb < n_pages && ok; ++kb) {
+            const int b = kb & 1, pos = my_pos - (w.page_begin + kb) * LLMB_PAGE;        // the last key that the row sees, from the page's first
+            ok = mbar_wait(smem_u32(&s_full[b]), (kb >> 1) & 1, abort_flag, status, 17);
+            if (!ok) break;
+            __syncwarp();
+            if (idle) {
+                mbar_arrive(smem_u32(&p_full[b]));
+                continue;
+            }
+            tcgen05_fence_after();
+            const uint32_t s_addr = lane_addr + S_COL + b * LLMB_PAGE;
+            uint32_t ra[32], rb[32];
+            tmem_ld32_start(s_addr, ra);
+            tmem_ld32_start(s_addr + 32, rb);
+            tmem_ld32_wait(ra);
+            tmem_ld32_wait(rb);
+            if (pos < LLMB_PAGE - 1) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    if (j > pos) ra[j] = __float_as_uint(-INFINITY);
+                    if (j + 32 > pos) rb[j] = __float_as_uint(-INFINITY);
+                }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) top = max3(top, __uint_as_float(ra[j]), __uint_as_float(ra[j + 1]));
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) top = max3(top, __uint_as_float(rb[j]), __uint_as_float(rb[j + 1]));
+            // The maximum that the exponents refer to moves only when it is exceeded by more than 2^8; a row that has seen no key keeps -inf.
+            const bool move = (top - run_max) * a.scale_log2 > 8.f;
+            const float new_max = move ? top : run_max;
+            const float alpha = move && kb > 0 ? fast_exp2((run_max - new_max) * a.scale_log2) : 1.f;
+            const float shift = new_max == -INFINITY ? 0.f : new_max * a.scale_log2;
+            run_max = new_max;
+            float add = 0.f;
+            auto to_weights = [&](const uint32_t (&x)[32], int c) {
+                uint32_t packed[16];
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                    float p0 = fast_exp2(fmaf(__uint_as_float(x[j]), a.scale_log2, -shift));
+                    float p1 = fast_exp2(fmaf(__uint_as_float(x[j + 1]), a.scale_log2, -shift));
+                    add += p0 + p1;
+                    packed[j >> 1] = pack2(p0, p1);
+                }
+                tmem_st16(s_addr + (c >> 1), packed);
+            };
+            to_weights(ra, 0);
+            to_weights(rb, 32);
+            run_sum = run_sum * alpha + add;
+            if (kb > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                ok = mbar_wait_warp(smem_u32(o_full), (kb - 1) & 1, abort_flag, status, 18);
+                if (!ok) break;
+                tcgen05_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 16) {
+                    uint32_t x[16];
+                    tmem_ld16(lane_addr + O_COL + c, x);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * alpha);
+                    tmem_st16(lane_addr + O_COL + c, x);
+                }
+            }
+            tmem_st_wait();
+            tcgen05_fence_before();
+            mbar_arrive(smem_u32(&p_full[b]));
+        }
+        if (ok) ok = mbar_wait(smem_u32(o_full), (n_pages - 1) & 1, abort_flag, status, 19);
+        if (ok && !idle) {
+            __syncwarp();
+            tcgen05_fence_after();
+            // All products are complete, the pages' room is free: a row goes out from there in one bulk copy. Rows lie 16 bytes further
+            // apart than they are long.
+            constexpr int ROOM = HD * 4 + 16;
+            static_assert(TC_ROWS * ROOM <= Ring<HD>::BYTES, "a row a thread");
+            unsigned char* room = base + row * ROOM;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+                uint32_t x[16];
+                tmem_ld16(lane_addr + O_COL + c, x);
+#pragma unroll
+                for (int d = 0; d < 16; d += 4) *reinterpret_cast<uint4*>(room + (c + d) * 4) = make_uint4(x[d], x[d + 1], x[d + 2], x[d + 3]);
+            }
+            if (row < w.n_rows) {
+                const size_t at = (size_t)token * a.n_heads + w.kv_head * share + row % share;
+                put_stats(a, w, pieces, at, run_max * a.scale_log2, run_sum);
+                fence_async_shared();
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                             ::"l"(a.acc + (at * a.slots + w.slot) * HD), "r"(smem_u32(room)), "r"(HD * 4) : "memory");
+                bulk_commit();
+                bulk_wait<0>();
+            }
+        }
+    }
+
+    tcgen05_fence_before();
+    __syncthreads();
+    if (*abort_flag) {                                       // a wait ran out: copies in flight get their time before the block leaves
+        for (int i = 0; i < 100; ++i) __nanosleep(10000);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tcgen05_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ bfloat16, many rows
@@ -586,8 +918,6 @@ prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __g
 // block has rows of. Only the rows of that sequence see those: the others' weights are zero, and the products leave their lanes of O
 // alone (a value that is not finite times a weight of zero would reach them).
 
-constexpr int TC_ROWS = 128;                                 // lanes of tensor memory
-constexpr int Q_PIECE = TC_ROWS * 64 * 2;                    // a tile's rows, 64 columns of the head: 16 KB
 constexpr int WIDE_ROWS = 256, WIDE_THREADS = 384;           // warps 0 keys, 1 products, 2 values, 4-7 and 8-11 a tile's softmax
 constexpr int PAIR_PIECE = 128 * 128;                        // 128 positions, 64 columns of the head: 16 KB
 constexpr int WIDE_REGS_FEW = 104, WIDE_REGS_MANY = 200;      // 128 x 64 + 256 x 216 <= 384 x 168, what the block is launched with
@@ -636,14 +966,71 @@ __device__ __forceinline__ void start(const Args& a, const TileRange& t, Walk& w
     w.logical += skip;
 }
 
-// a block's tile and its piece of the tile's walk
+// a block's tile, its piece of the tile's walk, and how many pieces that has
 struct Piece {
-    int tile_index, piece, pieces;
+    int kv_head, group, tile, tile_index, piece, pieces;
 };
+// Every tile is cut alike (`whole`, and batches too large for the arrays in shared memory).
 __device__ __forceinline__ Piece piece_of(const Args& a, int x) {
-    if (x < a.full_tiles) return Piece{x, 0, 1};
-    x -= a.full_tiles;
-    return Piece{a.full_tiles + x / a.prefix_splits, x % a.prefix_splits, a.prefix_splits};
+    Piece p{0, 0, 0, x, 0, 1};
+    if (x >= a.full_tiles) {
+        x -= a.full_tiles;
+        p.tile_index = a.full_tiles + x / a.prefix_splits;
+        p.piece = x % a.prefix_splits;
+        p.pieces = a.prefix_splits;
+    }
+    int rest = p.tile_index / a.n_kv_heads;
+    p.kv_head = p.tile_index - rest * a.n_kv_heads;
+    p.group = rest / a.prefix_tiles;
+    p.tile = rest - p.group * a.prefix_tiles;
+    return p;
+}
+// Groups of unequal lengths: pieces of `per` pairs of pages, the least number with which all tiles' pieces fit into the grid. Each warp finds out
+// for itself, a lane a group. group = n_groups where nothing is left for the block.
+__device__ __forceinline__ Piece even_piece_of(const Args& a, int x, int blocks, int lane) {
+    const unsigned all = 0xffffffffu;
+    const int share = a.n_heads / a.n_kv_heads, heads = blocks / a.n_kv_heads;      // blocks of a key head
+    auto tiles_and_pairs = [&](int g, int& tiles, int& pairs) {
+        tiles = 0;
+        pairs = 0;
+        if (g < a.n_groups) {
+            tiles = ((a.cu_seqlens[a.group_first[g + 1]] - a.cu_seqlens[a.group_first[g]]) * share + WIDE_ROWS - 1) / WIDE_ROWS;
+            pairs = (a.group_pages[g] + 1) / 2;
+            if (pairs == 0 || tiles < 0) tiles = 0;
+        }
+    };
+    int work = 0, items = 0, most = 0, tiles, pairs;
+    for (int g0 = 0; g0 < a.n_groups; g0 += 32) {
+        tiles_and_pairs(g0 + lane, tiles, pairs);
+        work += __reduce_add_sync(all, tiles * pairs);
+        items += __reduce_add_sync(all, tiles);
+        most = max(most, __reduce_max_sync(all, tiles > 0 ? pairs : 0));
+    }
+    int per = items < heads ? (work + heads - items - 1) / (heads - items) : most;
+    per = max(max(per, (most + a.prefix_splits - 1) / a.prefix_splits), 1);
+    Piece p{x % a.n_kv_heads, a.n_groups, 0, 0, 0, 1};
+    x /= a.n_kv_heads;
+    for (int g0 = 0; g0 < a.n_groups; g0 += 32) {
+        tiles_and_pairs(g0 + lane, tiles, pairs);
+        int pieces = (pairs + per - 1) / per, before = tiles * pieces;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            int left = __shfl_up_sync(all, before, d);
+            if (lane >= d) before += left;
+        }
+        unsigned beyond = __ballot_sync(all, x < before);
+        if (beyond) {
+            int at = __ffs(beyond) - 1;
+            p.group = g0 + at;
+            p.pieces = __shfl_sync(all, pieces, at);
+            x -= __shfl_sync(all, before - tiles * pieces, at);
+            p.tile = x / p.pieces;
+            p.piece = x - p.tile * p.pieces;
+            break;
+        }
+        x -= __shfl_sync(all, before, 31);
+    }
+    return p;
 }
 
 __device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
@@ -710,12 +1097,12 @@ prefix_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __
     __shared__ Staged staged;
     Args a = args;
     stage_arrays(a, staged);
-    const Piece piece = piece_of(a, blockIdx.x);
+    const Piece piece = a.even_blocks ? even_piece_of(a, blockIdx.x, gridDim.x, threadIdx.x & 31) : piece_of(a, blockIdx.x);
     const int share = a.n_heads / a.n_kv_heads;
     Item w;
-    w.kv_head = piece.tile_index % a.n_kv_heads;
-    w.tile = piece.tile_index / a.n_kv_heads % a.prefix_tiles;
-    const int group = piece.tile_index / a.n_kv_heads / a.prefix_tiles;
+    w.kv_head = piece.kv_head;
+    w.tile = piece.tile;
+    const int group = piece.group;
     if (group >= a.n_groups) return;                          // uniform for the block, here and below: nothing is allocated yet
     w.seq_first = a.group_first[group];
     w.seq_last = a.group_first[group + 1];
@@ -745,6 +1132,7 @@ prefix_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __
     const int warp = warp_index(), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
+#pragma unroll 1
         for (int i = 0; i < 18; ++i) {
             bool by_softmax = i < 2 || (i >= 12 && i < 16);
             mbar_init(smem_u32(&bars[i]), by_softmax ? 128 : 1);
@@ -914,19 +1302,30 @@ prefix_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __
             constexpr int CHUNKS = HD / 8;
             const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q);
             unsigned char* to = q_tile + tile * Q_BYTES;
-#pragma unroll 4
-            for (int i = t; i < TC_ROWS * CHUNKS; i += 128) {
-                int r = i / CHUNKS, c = i - r * CHUNKS;
-                uint4 value = make_uint4(0u, 0u, 0u, 0u);
-                if (r < tile_rows) {
-                    int at = row0 + tile * TC_ROWS + r, token = w.first_token + at / share, head = w.kv_head * share + at % share;
-                    value = *reinterpret_cast<const uint4*>(q + (size_t)token * a.q_stride + (size_t)head * HD + c * 8);
+            // All 16-byte chunks in flight at once, and no division for each (the queries took 11,000 to 18,000 cycles with both).
+            constexpr int STEP = 128 / CHUNKS;
+            const int c = t % CHUNKS, at0 = row0 + tile * TC_ROWS + t / CHUNKS, more_tokens = STEP / share, more_heads = STEP % share;
+            int token0 = w.first_token + at0 / share, head0 = at0 % share;
+#pragma unroll 1
+            for (int k = 0; k < CHUNKS; ++k) {
+                int r = t / CHUNKS + k * STEP;
+                unsigned char* chunk = to + (c >> 3) * Q_PIECE + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                const __nv_bfloat16* from = q + (size_t)token0 * a.q_stride + (size_t)(w.kv_head * share + head0) * HD + c * 8;
+                token0 += more_tokens;
+                head0 += more_heads;
+                if (head0 >= share) {
+                    head0 -= share;
+                    ++token0;
                 }
-                *reinterpret_cast<uint4*>(to + (c >> 3) * Q_PIECE + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = value;
+                if (r < tile_rows) {
+                    cp_async16(chunk, from);
+                } else {
+                    *reinterpret_cast<uint4*>(chunk) = make_uint4(0u, 0u, 0u, 0u);
+                }
             }
-            fence_async_shared();
-            mbar_arrive(smem_u32(&q_full[tile]));
+            cp_async_commit();
 
+            // what a row needs besides, while the queries are on their way
             const int r = quarter * 32 + lane;                // row of the tile = lane of tensor memory
             const bool valid = r < tile_rows;
             const int at = row0 + tile * TC_ROWS + (valid ? r : 0);
@@ -940,10 +1339,13 @@ prefix_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 uint32_t zero[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) zero[j] = 0u;
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < HD; c += 16) tmem_st16(o_addr + c, zero);
                 tmem_st_wait();
             }
+            cp_async_wait<0>();
+            fence_async_shared();
+            mbar_arrive(smem_u32(&q_full[tile]));
             const uint64_t scale2 = pair_of(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
             float run_max = -INFINITY, run_sum = 0.f;
             bool ok = true;
@@ -1064,7 +1466,8 @@ prefix_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     mbar_arrive(smem_u32(&p_full[2 * tile + 1]));
                 }
             }
-            if (ok && n_blocks > 0) ok = mbar_wait(smem_u32(&o_full[tile]), 0, abort_flag, status, 40);
+            // both tiles' products are complete: the pages' room is free
+            for (int i = 0; i < n_tiles && ok && n_blocks > 0; ++i) ok = mbar_wait(smem_u32(&o_full[i]), 0, abort_flag, status, 40);
             if (ok && !idle) {
                 __syncwarp();
                 tcgen05_fence_after();
@@ -1072,34 +1475,37 @@ prefix_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 const float inv = run_sum != 0.f ? 1.0f / run_sum : 0.f;
                 const size_t part_row = a.whole ? (size_t)(piece.tile_index - a.full_tiles) * WIDE_ROWS + (at - row0) : (size_t)token * a.n_heads + head;
                 const size_t slot = part_row * a.slots + piece.piece;
-                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD;
-                float* acc = a.acc + slot * HD;
                 if (valid && !direct) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(run_sum != 0.f ? run_max * a.scale_log2 : -INFINITY, run_sum);
+                if (valid && a.even_blocks && piece.piece == piece.pieces - 1)           // the parts that this tile has fewer than others
+                    for (int i = piece.pieces; i < a.prefix_splits; ++i)
+                        *reinterpret_cast<float2*>(a.stats + (part_row * a.slots + i) * 2) = make_float2(-INFINITY, 0.f);
+                // O goes out by way of shared memory, a bulk copy a row: written from its thread, a row's 16 bytes each went to another line
+                // (9,000 to 15,000 cycles). Rows lie 16 bytes further apart than they are long: eight lanes' chunks in different banks.
+                constexpr int ROOM = HD * 4 + 16;
+                static_assert(2 * TC_ROWS * ROOM <= 2 * Q_BYTES + 4 * PAIR_BYTES, "rows of both tiles");
+                unsigned char* room = base + (tile * TC_ROWS + r) * ROOM;
                 if (direct || n_blocks > 0) {
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 32) {
                         uint32_t x[32];
-                        if (n_blocks > 0) {
-                            tmem_ld32(o_addr + c, x);
+                        tmem_ld32(o_addr + c, x);
+                        if (direct) {
+#pragma unroll
+                            for (int d = 0; d < 32; d += 8)
+                                *reinterpret_cast<uint4*>(room + (c + d) * 2) = make_uint4(
+                                    pack2(__uint_as_float(x[d]) * inv, __uint_as_float(x[d + 1]) * inv), pack2(__uint_as_float(x[d + 2]) * inv, __uint_as_float(x[d + 3]) * inv),
+                                    pack2(__uint_as_float(x[d + 4]) * inv, __uint_as_float(x[d + 5]) * inv), pack2(__uint_as_float(x[d + 6]) * inv, __uint_as_float(x[d + 7]) * inv));
                         } else {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) x[j] = 0u;
+                            for (int d = 0; d < 32; d += 4) *reinterpret_cast<uint4*>(room + (c + d) * 4) = make_uint4(x[d], x[d + 1], x[d + 2], x[d + 3]);
                         }
-                        if (valid && direct) {
-#pragma unroll
-                            for (int d = 0; d < 32; d += 8) {
-                                uint4 packed;
-                                packed.x = pack2(__uint_as_float(x[d]) * inv, __uint_as_float(x[d + 1]) * inv);
-                                packed.y = pack2(__uint_as_float(x[d + 2]) * inv, __uint_as_float(x[d + 3]) * inv);
-                                packed.z = pack2(__uint_as_float(x[d + 4]) * inv, __uint_as_float(x[d + 5]) * inv);
-                                packed.w = pack2(__uint_as_float(x[d + 6]) * inv, __uint_as_float(x[d + 7]) * inv);
-                                *reinterpret_cast<uint4*>(o + c + d) = packed;
-                            }
-                        } else if (valid) {
-#pragma unroll
-                            for (int d = 0; d < 32; d += 4)
-                                *reinterpret_cast<uint4*>(acc + c + d) = make_uint4(x[d], x[d + 1], x[d + 2], x[d + 3]);
-                        }
+                    }
+                    if (valid) {
+                        fence_async_shared();
+                        void* to = direct ? (void*)(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD) : (void*)(a.acc + slot * HD);
+                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_u32(room)), "r"(direct ? HD * 2 : HD * 4) : "memory");
+                        bulk_commit();
+                        bulk_wait<0>();
                     }
                 }
             }
@@ -1232,12 +1638,14 @@ __global__ void __launch_bounds__(256) prefix_attention_join_kernel(const __grid
 
 // ------------------------------------------------------------------------------------------------ the call
 
-enum Kernel { CUDA_CORES, FEW, WIDE };
+enum Kernel { CUDA_CORES, FEW, TILE, WIDE };
 
 struct Plan {
     Kernel kernel;                   // of the shared pages
     bool whole;                      // a group's tiles walk the shared and the own pages, nothing is left for own parts
     int prefix_tiles, prefix_splits, own_tiles, own_splits, slots, full_tiles;
+    long long prefix_blocks, own_blocks;      // one launch, or two with TILE and WIDE
+    long long even_blocks;           // > 0: the blocks that deal out unequal groups' pages
     long long part_rows;             // rows that are joined from parts
 };
 
@@ -1263,37 +1671,55 @@ Plan plan_for(const Sizes& z) {
     int shared = z.max_shared > 0 ? bucket(z.max_shared) : 0, own = bucket(ceil_div(z.max_own > 0 ? z.max_own : 1, LLMB_PAGE));
     // sequences that bring few rows each would leave a tile of a group to walk many sequences' pages for a few of its rows
     p.whole = z.tc && (long long)z.max_new * share > FEW_ROWS;
-    p.kernel = !z.tc ? CUDA_CORES : p.whole || (shared > 0 && (long long)z.max_group * share > FEW_ROWS) ? WIDE : FEW;
-    int rows = p.kernel == WIDE ? WIDE_ROWS : p.kernel == FEW ? FEW_ROWS : SIMT_ROWS;
+    const long long group_rows = shared > 0 ? (long long)z.max_group * share : 0;
+    p.kernel = !z.tc ? CUDA_CORES : p.whole || group_rows > TC_ROWS ? WIDE : group_rows > FEW_ROWS ? TILE : FEW;
+    int rows = p.kernel == WIDE ? WIDE_ROWS : z.tc ? TC_ROWS : SIMT_ROWS;
     p.prefix_tiles = shared > 0 || p.whole ? ceil_div((long long)z.max_group * share, rows) : 0;
-    p.own_tiles = p.whole ? 0 : ceil_div((long long)z.max_new * share, z.tc ? FEW_ROWS : SIMT_ROWS);
+    p.own_tiles = p.whole ? 0 : ceil_div((long long)z.max_new * share, z.tc ? TC_ROWS : SIMT_ROWS);
     p.full_tiles = 0;
+    p.even_blocks = 0;
+    long long wide_blocks = 0;
     long long prefix = (long long)z.n_groups * p.prefix_tiles * z.n_kv_heads, owns = (long long)z.n_seqs * p.own_tiles * z.n_kv_heads;
     int walk = shared + (p.whole ? own : 0);
+    // Several groups: their pages are dealt out on the device, where their lengths are known. Below is then the most that a group is cut into, and the blocks
+    // for it: the wide kernel's in one round, the other's as many again as there are groups.
+    const bool even = z.tc && !p.whole && z.n_groups > 1 && shared > 0 && z.n_seqs <= STAGED_SEQS;
     if (p.kernel == WIDE) {
         // whole rounds of tiles as they are, the tiles of the last round cut so that they fill one, into four pages at least
         p.full_tiles = p.whole ? (int)(prefix / SMS * SMS) : 0;
         long long rest = prefix - p.full_tiles, best = 0;
         p.prefix_splits = 1;
         for (int n = 1; n <= MAX_SPLITS && (n == 1 || 4 * n <= walk) && rest > 0; ++n) {
-            // rounds of blocks times what one takes: its pages, and about eight pages' time for its start, its end and the join of a part more
-            long long time = (rest * n + SMS - 1) / SMS * (ceil_div(walk, n) + 8) + n;
+            // rounds of blocks times what one takes: its pages, and about eight pages' time for its start and its end
+            long long time = (rest * n + SMS - 1) / SMS * (ceil_div(walk, n) + 8);
             if (n == 1 || time < best) {
                 best = time;
                 p.prefix_splits = n;
             }
         }
-        // own pages: a launch of their own, 32 pages a block at most
-        p.own_splits = p.own_tiles > 0 ? ceil_div(own, 32) : 0;
+        wide_blocks = p.full_tiles + rest * p.prefix_splits;
+        p.own_splits = p.own_tiles > 0 ? ceil_div(own, 32) : 0;      // own pages: a launch of their own, 32 pages a block at most
+        if (even) {
+            p.prefix_splits = ceil_div(SMS, z.n_kv_heads);
+            wide_blocks = prefix > SMS ? prefix : SMS;
+            p.even_blocks = wide_blocks;
+        }
     } else {
         long long wave = (long long)SMS * (z.tc ? 2 : z.head_dim <= 64 ? 4 : z.head_dim <= 128 ? 2 : 1);
         long long per = (prefix * walk + owns * own + wave - 1) / wave;
         if (per < 2) per = 2;
         p.prefix_splits = p.prefix_tiles > 0 ? ceil_div(walk, per) : 0;
         p.own_splits = p.own_tiles > 0 ? ceil_div(own, per) : 0;
+        if (even) {
+            p.prefix_splits = ceil_div(2 * SMS, z.n_kv_heads);
+            if (p.prefix_splits > ceil_div(shared, 2)) p.prefix_splits = ceil_div(shared, 2);
+            p.even_blocks = prefix + 2 * SMS;
+        }
     }
     if (p.prefix_splits > MAX_SPLITS) p.prefix_splits = MAX_SPLITS;
     if (p.own_splits > MAX_SPLITS) p.own_splits = MAX_SPLITS;
+    p.prefix_blocks = p.kernel == WIDE ? wide_blocks : even ? p.even_blocks : prefix * p.prefix_splits;
+    p.own_blocks = owns * p.own_splits;
     p.slots = p.prefix_splits + p.own_splits;
     p.part_rows = p.slots == 1 ? 0 : p.whole ? (prefix - p.full_tiles) * WIDE_ROWS : (long long)z.n_tokens * z.n_heads;
     return p;
@@ -1316,15 +1742,17 @@ int launch_simt(const Args& a, unsigned blocks, cudaStream_t stream) {
 }
 
 template <int HD>
-int launch_tc(const Args& a, const Plan& p, int n_pages, unsigned blocks, cudaStream_t stream) {
-    constexpr size_t few = 1024 + Ring<HD>::BYTES + (2 * Ring<HD>::STAGES + 1) * 8;
-    static_assert(2 * (few + sizeof(Staged) + 1024) <= 227 * 1024, "two blocks an SM");
+int launch_tc(const Args& a, const Plan& p, int n_pages, cudaStream_t stream) {
+    // (more than a third of an SM's shared memory: no third block lands there and waits for tensor memory)
+    constexpr size_t tiles = 1024 + Ring<HD>::BYTES + 16 * 8;
+    static_assert(2 * (tiles + sizeof(Staged) + 1024) <= 227 * 1024 && 2 * Ring<HD>::STAGES <= 14, "two blocks an SM");
     // (more than half of an SM's shared memory for the smaller head size too: tensor memory has room for one block)
     constexpr size_t wide_need = 1024 + (HD / 64) * (2 * Q_PIECE + 4 * PAIR_PIECE) + 19 * 8, wide = wide_need < 120 * 1024 ? 120 * 1024 : wide_need;
     static_assert(wide + sizeof(Staged) + 1024 <= 227 * 1024, "one block an SM");
     static bool configured = false;
     if (!configured) {
-        LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few));
+        LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tiles));
+        LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_tile_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tiles));
         LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_wide_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wide));
         configured = true;
     }
@@ -1335,20 +1763,18 @@ int launch_tc(const Args& a, const Plan& p, int n_pages, unsigned blocks, cudaSt
     if (code) return code;
     static int* status_dev = nullptr;
     if (!status_dev && status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status_dev, status_word(), 0));
-    if (p.kernel == WIDE) {
-        long long tiles = (long long)a.n_groups * a.prefix_tiles * a.n_kv_heads, wide_blocks = a.full_tiles + (tiles - a.full_tiles) * a.prefix_splits;
-        LLMB_REQUIRE(wide_blocks < (1ll << 31), "prefix_attention: too many blocks");
-        llmb::launch(prefix_attention_wide_kernel<HD>, dim3((unsigned)wide_blocks), WIDE_THREADS, wide, stream, true, map_k, map_v, a, status_dev);
-        if ((code = check_launch("prefix_attention_wide")) || a.own_tiles == 0) return code;
-        // the own parts: the blocks of the other kernel for them, the slots of the shared parts in front of theirs
-        Args own = a;
-        own.prefix_tiles = 0;
-        own.behind = pdl_enabled() ? 1 : 0;
-        blocks = (unsigned)((long long)a.n_kv_heads * a.n_seqs * a.own_tiles * a.own_splits);
-        llmb::launch(prefix_attention_few_kernel<HD>, dim3(blocks), FEW_THREADS, few, stream, true, map_k, map_v, own, status_dev);
+    const unsigned prefix = (unsigned)p.prefix_blocks, own = (unsigned)p.own_blocks;
+    if (p.kernel == FEW) {
+        llmb::launch(prefix_attention_few_kernel<HD>, dim3(prefix + own), FEW_THREADS, tiles, stream, true, map_k, map_v, a, status_dev);
         return check_launch("prefix_attention_few");
     }
-    llmb::launch(prefix_attention_few_kernel<HD>, dim3(blocks), FEW_THREADS, few, stream, true, map_k, map_v, a, status_dev);
+    if (p.kernel == WIDE) llmb::launch(prefix_attention_wide_kernel<HD>, dim3(prefix), WIDE_THREADS, wide, stream, true, map_k, map_v, a, status_dev);
+    else llmb::launch(prefix_attention_tile_kernel<HD>, dim3(prefix), TILE_THREADS, tiles, stream, true, map_k, map_v, a, status_dev);
+    if ((code = check_launch("prefix_attention_shared")) || own == 0) return code;
+    Args behind = a;                          // the own parts, their slots behind those of the shared ones
+    behind.prefix_tiles = 0;
+    behind.behind = pdl_enabled() ? 1 : 0;
+    llmb::launch(prefix_attention_few_kernel<HD>, dim3(own), FEW_THREADS, tiles, stream, true, map_k, map_v, behind, status_dev);
     return check_launch("prefix_attention_few");
 }
 
@@ -1362,11 +1788,11 @@ void launch_join(const Args& a, int rows, cudaStream_t stream) {
 }
 
 int run(const Args& a, const Plan& p, int dtype, int n_pages, cudaStream_t stream) {
-    long long blocks = (long long)a.n_kv_heads * ((long long)a.n_groups * a.prefix_tiles * a.prefix_splits + (long long)a.n_seqs * a.own_tiles * a.own_splits);
+    const long long blocks = p.prefix_blocks + p.own_blocks;
     LLMB_REQUIRE(blocks < (1ll << 31), "prefix_attention: too many blocks");
     const bool f32 = dtype == LLMB_DTYPE_F32;
     int code;
-    if (p.kernel != CUDA_CORES) code = a.head_dim == 64 ? launch_tc<64>(a, p, n_pages, (unsigned)blocks, stream) : launch_tc<128>(a, p, n_pages, (unsigned)blocks, stream);
+    if (p.kernel != CUDA_CORES) code = a.head_dim == 64 ? launch_tc<64>(a, p, n_pages, stream) : launch_tc<128>(a, p, n_pages, stream);
     else if (a.head_dim <= 64) code = f32 ? launch_simt<float, 64>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 64>(a, (unsigned)blocks, stream);
     else if (a.head_dim <= 128) code = f32 ? launch_simt<float, 128>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 128>(a, (unsigned)blocks, stream);
     else code = f32 ? launch_simt<float, 256>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 256>(a, (unsigned)blocks, stream);
@@ -1398,7 +1824,7 @@ LLMB_EXPORT long long llmb_prefix_attention_scratch_floats(int n_tokens, int n_s
     if (n_tokens <= 0 || n_seqs <= 0 || n_groups <= 0 || n_kv_heads <= 0 || n_heads < n_kv_heads) return 0;
     Plan p = plan_for(Sizes{n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own, tc != 0});
     if (p.slots > 1) ++*kernels;
-    if (p.kernel == WIDE && p.own_tiles > 0) ++*kernels;
+    if ((p.kernel == TILE || p.kernel == WIDE) && p.own_blocks > 0) ++*kernels;
     return scratch_floats_of(p.part_rows * p.slots, head_dim);
 }
 
@@ -1430,7 +1856,7 @@ LLMB_EXPORT int llmb_prefix_attention(const void* q, int q_stride, const void* k
     Args a{q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, out, scratch, scratch + value_floats(parts, head_dim),
            q_stride, out_stride, table_stride, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, scale * LOG2E,
            p.prefix_tiles, p.prefix_splits, p.own_tiles, p.own_splits, p.slots, vectors ? 1 : 0, p.full_tiles,
-           0, p.whole ? 1 : 0};
+           (int)p.even_blocks, 0, p.whole ? 1 : 0};
     return run(a, p, dtype, n_pages, stream);
 }
 
