@@ -123,22 +123,44 @@ __device__ __forceinline__ int position_of(const Args& a, const Item& w, int tok
     return a.seq_lens[seq] - a.cu_seqlens[seq + 1] + token;
 }
 
+// The arrays that say which sequences there are, in shared memory (one round of loads) where there is room.
+constexpr int STAGED_SEQS = 512;
+struct Staged {
+    int seq_lens[STAGED_SEQS], cu_seqlens[STAGED_SEQS + 1], group_first[STAGED_SEQS + 1], group_pages[STAGED_SEQS];
+};
+__device__ __forceinline__ void stage_arrays(Args& a, Staged& s) {
+    if (a.n_seqs > STAGED_SEQS) return;
+    for (int i = threadIdx.x; i <= a.n_seqs; i += blockDim.x) {
+        s.cu_seqlens[i] = a.cu_seqlens[i];
+        if (i < a.n_seqs) s.seq_lens[i] = a.seq_lens[i];
+        if (i <= a.n_groups) s.group_first[i] = a.group_first[i];
+        if (i < a.n_groups) s.group_pages[i] = a.group_pages[i];
+    }
+    __syncthreads();
+    a.seq_lens = s.seq_lens;
+    a.cu_seqlens = s.cu_seqlens;
+    a.group_first = s.group_first;
+    a.group_pages = s.group_pages;
+}
+
 // ------------------------------------------------------------------------------------------------ any type, any head size
 //
 // 32-bit arithmetic on the CUDA cores: the path of 32-bit caches, and of the head sizes that the tensor-core kernel is not built for.
 // A block holds 32 rows and walks its pages one by one: 64 keys and values in shared memory (as 32-bit values), thread
-// (ty, tx) of a half-warp ty owns rows 4 ty .. 4 ty + 3. It forms their scores with keys tx, tx + 16, tx + 32, tx + 48 (4 x 4 products a
-// pair of 16-byte loads), shares maxima and sums with the 15 other threads of its rows, and adds the weighted values of columns
-// 4 tx + 64 c. Rows of a key or value are 4 words longer than the head, so that the 16 rows that a half-warp reads lie in
-// different banks.
+// (ty, tx) of a half-warp ty owns rows 2 ty and 2 ty + 1. It forms their scores with keys tx, tx + 16, tx + 32, tx + 48, shares maxima
+// and sums with the 15 other threads of its rows, and adds the weighted values of columns 4 tx + 64 c. Rows of a key or value are 4 words
+// longer than the head, so that the 16 rows that a half-warp reads lie in different banks. 32-bit pages come by cp.async.
+//
+// Eight sequences behind 4,096 positions (32 heads of 64, 32-bit): 27 us; the products alone are 4. Loaded through registers row by row it took 36, with
+// four rows a thread and half the threads 30, with the next page under way during this one (and two blocks an SM instead of three) 27.
 
-constexpr int SIMT_ROWS = 32, SIMT_THREADS = 128;
+constexpr int SIMT_ROWS = 32, SIMT_THREADS = 256, RT = SIMT_ROWS / (SIMT_THREADS / 16);     // RT: rows of a thread
 
 template <int DMAX>
-constexpr int simt_floats() { return (SIMT_ROWS + 2 * LLMB_PAGE) * (DMAX + 4) + SIMT_ROWS * (LLMB_PAGE + 4) + SIMT_ROWS; }
+constexpr int simt_floats() { return (SIMT_ROWS + 2 * LLMB_PAGE) * (DMAX + 4) + SIMT_ROWS * (LLMB_PAGE + 4) + SIMT_ROWS + 4; }
 
 template <typename T, int DMAX>
-__global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(const __grid_constant__ Args args) {
     constexpr int LD = DMAX + 4, LP = LLMB_PAGE + 4, COLS = DMAX / 64;
     extern __shared__ __align__(16) float smem[];
     float* qs = smem;                              // [32][LD], scaled
@@ -146,11 +168,16 @@ __global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(con
     float* vs = ks + LLMB_PAGE * LD;               // [64][LD]
     float* ps = vs + LLMB_PAGE * LD;               // [32][LP]
     int* row_pos = reinterpret_cast<int*>(ps + SIMT_ROWS * LP);
+    int* last_pos = row_pos + SIMT_ROWS;
+    __shared__ Staged staged;
 
     griddep_launch();
-    griddep_wait();
+    Args a = args;
+    stage_arrays(a, staged);
     Item w;
-    if (!item_of(a, blockIdx.x, w)) return;
+    const bool work = item_of(a, blockIdx.x, w);
+    griddep_wait();
+    if (!work) return;
     const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
     const int D = a.head_dim, share = a.n_heads / a.n_kv_heads;
     const T* q = static_cast<const T*>(a.q);
@@ -158,84 +185,106 @@ __global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(con
     const T* v_cache = static_cast<const T*>(a.v_cache);
     const int* pages = a.block_table + (size_t)w.seq_first * a.table_stride;
 
+    constexpr int V = 16 / sizeof(T);
+    const int width = a.vectors ? D / V : (D + 3) & ~3;        // of a row, in vectors or in single values (the scores read four at a time)
+    const int row_step = SIMT_THREADS / width, first_row = tid / width, col = (tid - first_row * width) * (a.vectors ? V : 1);
+    // a page's keys and values: thread tid takes column `col` of every row_step-th row (rows wider than the block: all columns in turn)
+    auto load_page = [&](int logical) {
+        const size_t base = ((size_t)pages[logical] * a.n_kv_heads + w.kv_head) * LLMB_PAGE * D;
+        if (!a.vectors) {
+            for (int i = tid; i < LLMB_PAGE * width; i += SIMT_THREADS) {
+                int row = i / width, c = i - row * width;
+                ks[row * LD + c] = c < D ? to_float(k_cache[base + (size_t)row * D + c]) : 0.f;
+                vs[row * LD + c] = c < D ? to_float(v_cache[base + (size_t)row * D + c]) : 0.f;
+            }
+        } else if (first_row < row_step) {
+#pragma unroll 4
+            for (int row = first_row; row < LLMB_PAGE; row += row_step) {
+                const T* from_k = k_cache + base + (size_t)row * D + col;
+                const T* from_v = v_cache + base + (size_t)row * D + col;
+                if constexpr (sizeof(T) == 4) {
+                    cp_async16(ks + row * LD + col, from_k);
+                    cp_async16(vs + row * LD + col, from_v);
+                } else {
+                    __align__(16) T kk[V], vv[V];
+                    *reinterpret_cast<uint4*>(kk) = *reinterpret_cast<const uint4*>(from_k);
+                    *reinterpret_cast<uint4*>(vv) = *reinterpret_cast<const uint4*>(from_v);
+#pragma unroll
+                    for (int j = 0; j < V; j += 4) {
+                        *reinterpret_cast<float4*>(ks + row * LD + col + j) = make_float4(to_float(kk[j]), to_float(kk[j + 1]), to_float(kk[j + 2]), to_float(kk[j + 3]));
+                        *reinterpret_cast<float4*>(vs + row * LD + col + j) = make_float4(to_float(vv[j]), to_float(vv[j + 1]), to_float(vv[j + 2]), to_float(vv[j + 3]));
+                    }
+                }
+            }
+        }
+    };
+
     for (int tile = w.tile; tile * SIMT_ROWS < w.n_rows; tile += w.tiles) {
         int row0 = tile * SIMT_ROWS, rows = min(SIMT_ROWS, w.n_rows - row0);
         __syncthreads();                           // the tile before is done with shared memory
-        for (int i = tid; i < SIMT_ROWS * DMAX; i += SIMT_THREADS) {
-            int r = i / DMAX, d = i - r * DMAX;
-            float value = 0.f;
-            if (r < rows && d < D) {
-                int token = w.first_token + (row0 + r) / share, head = w.kv_head * share + (row0 + r) % share;
-                value = to_float(q[(size_t)token * a.q_stride + (size_t)head * D + d]) * a.scale_log2;
-            }
-            qs[r * LD + d] = value;
-        }
-        if (tid < SIMT_ROWS) row_pos[tid] = tid < rows ? position_of(a, w, w.first_token + (row0 + tid) / share) : -1;
-        __syncthreads();
-        int last = -1;                             // the last position that a row of the tile sees
-        for (int r = 0; r < rows; ++r) last = max(last, row_pos[r]);
-        int end = min(w.page_end, last < 0 ? 0 : last / LLMB_PAGE + 1);
-
-        float m[4], l[4], o[4][COLS * 4];
-        int pos[4];
+#pragma unroll 4
+        for (int r = tid >> 5; r < SIMT_ROWS; r += SIMT_THREADS / 32) {          // a warp a row
+            const bool valid = r < rows;
+            const int token = w.first_token + (row0 + (valid ? r : 0)) / share, head = w.kv_head * share + (row0 + (valid ? r : 0)) % share;
+            const T* from = q + (size_t)token * a.q_stride + (size_t)head * D;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+            for (int d = tid & 31; d < DMAX; d += 32) qs[r * LD + d] = valid && d < D ? to_float(from[d]) * a.scale_log2 : 0.f;
+        }
+        if (tid < SIMT_ROWS) {
+            int p = tid < rows ? position_of(a, w, w.first_token + (row0 + tid) / share) : -1;
+            row_pos[tid] = p;
+            p = __reduce_max_sync(0xffffffffu, p);
+            if (tid == 0) *last_pos = p;
+        }
+        __syncthreads();
+        const int last = *last_pos;                // the last position that a row of the tile sees
+        const int end = min(w.page_end, last < 0 ? 0 : last / LLMB_PAGE + 1);
+
+        float m[RT], l[RT], o[RT][COLS * 4];
+        int pos[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
             m[i] = -INFINITY;
             l[i] = 0.f;
-            pos[i] = row_pos[ty * 4 + i];
+            pos[i] = row_pos[ty * RT + i];
 #pragma unroll
             for (int c = 0; c < COLS * 4; ++c) o[i][c] = 0.f;
         }
+        const bool idle = (tid >> 5) * 2 * RT >= rows;         // a warp without rows
         for (int logical = w.page_begin; logical < end; ++logical) {
-            size_t base = ((size_t)pages[logical] * a.n_kv_heads + w.kv_head) * LLMB_PAGE * D;
-            int key0 = logical * LLMB_PAGE, stored = min(LLMB_PAGE, last + 1 - key0);
+            const int key0 = logical * LLMB_PAGE, stored = min(LLMB_PAGE, last + 1 - key0);
             __syncthreads();                       // everyone is done with the page before
-            constexpr int V = 16 / sizeof(T);
-            if (a.vectors) {
-                int per_row = D / V;
-                for (int i = tid; i < LLMB_PAGE * per_row; i += SIMT_THREADS) {
-                    int row = i / per_row, col = (i - row * per_row) * V;
-                    __align__(16) T kk[V], vv[V];
-                    *reinterpret_cast<uint4*>(kk) = *reinterpret_cast<const uint4*>(k_cache + base + (size_t)row * D + col);
-                    *reinterpret_cast<uint4*>(vv) = *reinterpret_cast<const uint4*>(v_cache + base + (size_t)row * D + col);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        ks[row * LD + col + j] = to_float(kk[j]);
-                        vs[row * LD + col + j] = row < stored ? to_float(vv[j]) : 0.f;
-                    }
-                }
-            } else {
-                int width = (D + 3) & ~3;          // (the scores read four columns at a time)
-                for (int i = tid; i < LLMB_PAGE * width; i += SIMT_THREADS) {
-                    int row = i / width, col = i - row * width;
-                    bool in = col < D;
-                    ks[row * LD + col] = in ? to_float(k_cache[base + (size_t)row * D + col]) : 0.f;
-                    vs[row * LD + col] = in && row < stored ? to_float(v_cache[base + (size_t)row * D + col]) : 0.f;
-                }
-            }
+            load_page(logical);
+            cp_async_commit();
+            cp_async_wait<0>();
             __syncthreads();
-            if (ty * 4 >= rows) continue;          // (the same answer in a half-warp, whose threads alone share the rows)
-            unsigned mates = 0xffffu << (tid & 16);
+            if (stored < LLMB_PAGE) {              // values behind the last position are whatever the page held: zero here
+                for (int row = stored + (tid >> 5); row < LLMB_PAGE; row += SIMT_THREADS / 32)
+                    for (int d = tid & 31; d < D; d += 32) vs[row * LD + d] = 0.f;
+                __syncthreads();
+            }
+            if (idle) continue;
 
-            float s[4][4];
+            float s[RT][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < RT; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
             for (int d = 0; d < D; d += 4) {
-                float4 qv[4], kv[4];
+                float4 qv[RT], kv[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(qs + (ty * 4 + i) * LD + d);
+                for (int i = 0; i < RT; ++i) qv[i] = *reinterpret_cast<const float4*>(qs + (ty * RT + i) * LD + d);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * LD + d);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < RT; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         s[i][j] = fmaf(qv[i].x, kv[j].x, fmaf(qv[i].y, kv[j].y, fmaf(qv[i].z, kv[j].z, fmaf(qv[i].w, kv[j].w, s[i][j]))));
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < RT; ++i) {
                 float top = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -243,7 +292,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(con
                     top = fmaxf(top, s[i][j]);
                 }
 #pragma unroll
-                for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(mates, top, x));
+                for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                 float new_m = fmaxf(m[i], top), against = new_m == -INFINITY ? 0.f : new_m;
                 float alpha = exp2f(m[i] - against);
                 m[i] = new_m;
@@ -252,17 +301,18 @@ __global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(con
                 for (int j = 0; j < 4; ++j) {
                     float p = exp2f(s[i][j] - against);
                     add += p;
-                    ps[(ty * 4 + i) * LP + tx + 16 * j] = p;
+                    ps[(ty * RT + i) * LP + tx + 16 * j] = p;
                 }
                 l[i] = l[i] * alpha + add;         // of this thread's keys
 #pragma unroll
                 for (int c = 0; c < COLS * 4; ++c) o[i][c] *= alpha;
             }
-            __syncwarp(mates);
+            __syncwarp();
+#pragma unroll 2
             for (int j = 0; j < LLMB_PAGE; j += 4) {
-                float4 pv[4];
+                float4 pv[RT];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(ps + (ty * 4 + i) * LP + j);
+                for (int i = 0; i < RT; ++i) pv[i] = *reinterpret_cast<const float4*>(ps + (ty * RT + i) * LP + j);
 #pragma unroll
                 for (int c = 0; c < COLS; ++c) {
                     if (c * 64 + tx * 4 >= D) break;
@@ -270,7 +320,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(con
                     for (int jj = 0; jj < 4; ++jj) {
                         float4 v = *reinterpret_cast<const float4*>(vs + (j + jj) * LD + c * 64 + tx * 4);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
+                        for (int i = 0; i < RT; ++i) {
                             float p = jj == 0 ? pv[i].x : jj == 1 ? pv[i].y : jj == 2 ? pv[i].z : pv[i].w;
                             o[i][c * 4] = fmaf(p, v.x, o[i][c * 4]);
                             o[i][c * 4 + 1] = fmaf(p, v.y, o[i][c * 4 + 1]);
@@ -280,15 +330,14 @@ __global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(con
                     }
                 }
             }
-            __syncwarp(mates);                     // the weights are read before the next page's are written
+            __syncwarp();                     // the weights are read before the next page's are written
         }
-        if (ty * 4 < rows) {
-            unsigned mates = 0xffffu << (tid & 16);
+        if (!idle) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < RT; ++i) {
 #pragma unroll
-                for (int x = 8; x > 0; x >>= 1) l[i] += __shfl_xor_sync(mates, l[i], x);
-                int r = ty * 4 + i;
+                for (int x = 8; x > 0; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+                int r = ty * RT + i;
                 if (r >= rows) continue;
                 int token = w.first_token + (row0 + r) / share, head = w.kv_head * share + (row0 + r) % share;
                 if (a.slots == 1) {
@@ -353,26 +402,6 @@ template <int HD> struct Ring {
     static_assert(MERGE <= BYTES, "the merge takes the ring's place");
     static_assert((HD / 64) * (Q_PIECE + 4 * KV_PIECE) <= BYTES, "the queries and two pages");
 };
-
-// The arrays that say which sequences there are, in shared memory (one round of loads) where there is room.
-constexpr int STAGED_SEQS = 512;
-struct Staged {
-    int seq_lens[STAGED_SEQS], cu_seqlens[STAGED_SEQS + 1], group_first[STAGED_SEQS + 1], group_pages[STAGED_SEQS];
-};
-__device__ __forceinline__ void stage_arrays(Args& a, Staged& s) {
-    if (a.n_seqs > STAGED_SEQS) return;
-    for (int i = threadIdx.x; i <= a.n_seqs; i += blockDim.x) {
-        s.cu_seqlens[i] = a.cu_seqlens[i];
-        if (i < a.n_seqs) s.seq_lens[i] = a.seq_lens[i];
-        if (i <= a.n_groups) s.group_first[i] = a.group_first[i];
-        if (i < a.n_groups) s.group_pages[i] = a.group_pages[i];
-    }
-    __syncthreads();
-    a.seq_lens = s.seq_lens;
-    a.cu_seqlens = s.cu_seqlens;
-    a.group_first = s.group_first;
-    a.group_pages = s.group_pages;
-}
 
 // Slices of equal length of groups of unequal ones: `per` pages each, the least number (two at least) with which all groups' slices fit into the
 // blocks that there are for a key head, or a group's all. Each warp finds out for itself, a lane a group. w: the slice's group and pages; *pieces:
@@ -657,7 +686,7 @@ prefix_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __
     constexpr int PIECES = HD / 64, KV_BYTES = PIECES * KV_PIECE;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base + Ring<HD>::BYTES);         // 14 barriers and two words
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + Ring<HD>::BYTES);         // 15 barriers and two words
     unsigned char* q_tile = base;
     unsigned char* k_tile = base + PIECES * Q_PIECE;
     unsigned char* v_tile = k_tile + 2 * KV_BYTES;
@@ -668,13 +697,14 @@ prefix_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __
     uint64_t* v_empty = bars + 7;             // [2]
     uint64_t* s_full = bars + 9;              // [2] a buffer's scores are complete
     uint64_t* p_full = bars + 11;             // [2] its weights are written and O has been rescaled
-    uint64_t* o_full = bars + 13;             // a page's P V has been added to O
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+    uint64_t* o_full = bars + 13;             // a page's P V has been added to O (asked for at the next page only: a parity tells two states apart)
+    uint64_t* o_last = bars + 14;             // the last one's has
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = warp_index(), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
 #pragma unroll 1
-        for (int i = 0; i < 14; ++i) mbar_init(smem_u32(&bars[i]), (i == 0 || i == 11 || i == 12) ? 128 : 1);
+        for (int i = 0; i < 15; ++i) mbar_init(smem_u32(&bars[i]), (i == 0 || i == 11 || i == 12) ? 128 : 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -759,7 +789,7 @@ prefix_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 for (int j = 0; j < LLMB_PAGE / 16; ++j)    // 16 keys a step: 8 columns of weights, 2048 bytes of value rows
                     tcgen05_mma_ts(tmem_base + O_COL, tmem_base + S_COL + b * LLMB_PAGE + j * 8,
                                    v_desc0 + b * BUFFER + (uint64_t)((j * 2048) >> 4), idesc_pv, (kb > 0 || j > 0) ? 1u : 0u);
-                tcgen05_commit(smem_u32(o_full));
+                tcgen05_commit(smem_u32(kb == n_pages - 1 ? o_last : o_full));
                 tcgen05_commit(smem_u32(&v_empty[b]));
             }
             __syncwarp();
@@ -862,7 +892,7 @@ prefix_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __
             tcgen05_fence_before();
             mbar_arrive(smem_u32(&p_full[b]));
         }
-        if (ok) ok = mbar_wait(smem_u32(o_full), (n_pages - 1) & 1, abort_flag, status, 19);
+        if (ok) ok = mbar_wait(smem_u32(o_last), 0, abort_flag, status, 19);
         if (ok && !idle) {
             __syncwarp();
             tcgen05_fence_after();
@@ -1540,10 +1570,11 @@ __device__ __forceinline__ int row_of_parts(const Args& a, int row, int n_rows) 
 
 // WARPS warps a row: each reads all the maxima and sums, a lane a part, and takes every WARPS-th part, several of them in flight; their
 // sums are added in order. With one warp that read part after part the join of 34 parts of 512 rows took 25 us, more than the parts.
-template <typename T, int WARPS>
-__global__ void __launch_bounds__(256) prefix_attention_join_kernel(const __grid_constant__ Args a, int n_rows) {
-    constexpr int ROWS = 8 / WARPS, CHUNKS = LLMB_MAX_HEAD_DIM / 128, AHEAD = 4;
-    __shared__ float4 shared_value[8][LLMB_MAX_HEAD_DIM / 4];
+// CHUNKS: 128 columns of the head each; with two for all sizes the registers let three blocks on an SM, and 2,048 rows of 19 parts took 14 us.
+template <typename T, int WARPS, int CHUNKS>
+__global__ void __launch_bounds__(256, CHUNKS == 1 ? 5 : 3) prefix_attention_join_kernel(const __grid_constant__ Args a, int n_rows) {
+    constexpr int ROWS = 8 / WARPS, AHEAD = 4;
+    __shared__ float4 shared_value[8][CHUNKS * 32];
     griddep_launch();
     griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp % WARPS;
@@ -1690,8 +1721,9 @@ Plan plan_for(const Sizes& z) {
         long long rest = prefix - p.full_tiles, best = 0;
         p.prefix_splits = 1;
         for (int n = 1; n <= MAX_SPLITS && (n == 1 || 4 * n <= walk) && rest > 0; ++n) {
-            // rounds of blocks times what one takes: its pages, and about eight pages' time for its start and its end
-            long long time = (rest * n + SMS - 1) / SMS * (ceil_div(walk, n) + 8);
+            // In pages' time (0.85 us): rounds of blocks times what one takes, its pages and about twelve for its start and its end, and the parts
+            // written and read again at some 5 TB/s.
+            long long time = (rest * n + SMS - 1) / SMS * (ceil_div(walk, n) + 12) + (n > 1 ? rest * n * WIDE_ROWS * z.head_dim * 8 / 4300000 : 0);
             if (n == 1 || time < best) {
                 best = time;
                 p.prefix_splits = n;
@@ -1705,7 +1737,7 @@ Plan plan_for(const Sizes& z) {
             p.even_blocks = wide_blocks;
         }
     } else {
-        long long wave = (long long)SMS * (z.tc ? 2 : z.head_dim <= 64 ? 4 : z.head_dim <= 128 ? 2 : 1);
+        long long wave = (long long)SMS * (z.tc ? 2 : z.head_dim <= 64 ? 3 : z.head_dim <= 128 ? 2 : 1);
         long long per = (prefix * walk + owns * own + wave - 1) / wave;
         if (per < 2) per = 2;
         p.prefix_splits = p.prefix_tiles > 0 ? ceil_div(walk, per) : 0;
@@ -1779,12 +1811,12 @@ int launch_tc(const Args& a, const Plan& p, int n_pages, cudaStream_t stream) {
 }
 
 // a warp for four parts, as many as fit
-template <typename T>
+template <typename T, int CHUNKS>
 void launch_join(const Args& a, int rows, cudaStream_t stream) {
-    if (a.slots <= 4) llmb::launch(prefix_attention_join_kernel<T, 1>, dim3((rows + 7) / 8), 256, 0, stream, true, a, rows);
-    else if (a.slots <= 8) llmb::launch(prefix_attention_join_kernel<T, 2>, dim3((rows + 3) / 4), 256, 0, stream, true, a, rows);
-    else if (a.slots <= 16) llmb::launch(prefix_attention_join_kernel<T, 4>, dim3((rows + 1) / 2), 256, 0, stream, true, a, rows);
-    else llmb::launch(prefix_attention_join_kernel<T, 8>, dim3(rows), 256, 0, stream, true, a, rows);
+    if (a.slots <= 4) llmb::launch(prefix_attention_join_kernel<T, 1, CHUNKS>, dim3((rows + 7) / 8), 256, 0, stream, true, a, rows);
+    else if (a.slots <= 8) llmb::launch(prefix_attention_join_kernel<T, 2, CHUNKS>, dim3((rows + 3) / 4), 256, 0, stream, true, a, rows);
+    else if (a.slots <= 16) llmb::launch(prefix_attention_join_kernel<T, 4, CHUNKS>, dim3((rows + 1) / 2), 256, 0, stream, true, a, rows);
+    else llmb::launch(prefix_attention_join_kernel<T, 8, CHUNKS>, dim3(rows), 256, 0, stream, true, a, rows);
 }
 
 int run(const Args& a, const Plan& p, int dtype, int n_pages, cudaStream_t stream) {
@@ -1797,8 +1829,9 @@ int run(const Args& a, const Plan& p, int dtype, int n_pages, cudaStream_t strea
     else if (a.head_dim <= 128) code = f32 ? launch_simt<float, 128>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 128>(a, (unsigned)blocks, stream);
     else code = f32 ? launch_simt<float, 256>(a, (unsigned)blocks, stream) : launch_simt<__nv_bfloat16, 256>(a, (unsigned)blocks, stream);
     if (code || a.slots == 1) return code;
-    if (f32) launch_join<float>(a, (int)p.part_rows, stream);
-    else launch_join<__nv_bfloat16>(a, (int)p.part_rows, stream);
+    const bool narrow = a.head_dim <= 128;
+    if (f32) narrow ? launch_join<float, 1>(a, (int)p.part_rows, stream) : launch_join<float, 2>(a, (int)p.part_rows, stream);
+    else narrow ? launch_join<__nv_bfloat16, 1>(a, (int)p.part_rows, stream) : launch_join<__nv_bfloat16, 2>(a, (int)p.part_rows, stream);
     return check_launch("prefix_attention_join");
 }
 

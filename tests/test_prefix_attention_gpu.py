@@ -84,6 +84,8 @@ def check(b, got):
     """The whole result against the definition in 64 bits, each row within its own bound."""
     heads, dim, share, u = b["heads"], b["dim"], b["heads"] // b["kv_heads"], 2.0 ** -24
     half = 0.0 if b["dtype"] == F32 else 2.0 ** -9
+    torch.cuda.synchronize()
+    ops().check_device_status()                                        # no wait in a kernel has run out
     assert got.dtype == b["dtype"] and tuple(got.shape) == (b["cu"][-1], heads * dim)
     got = got.double().view(-1, heads, dim)
     for s, length in enumerate(b["lengths"]):
@@ -113,6 +115,8 @@ SHARED = [                                  # (shared pages, members' (held, new
     [(2, [(0, 3), (9, 65), (70, 1), (0, 0), (3, 40)]), (0, [(0, 0)]), (1, [(0, 130), (64, 2)])],      # unequal, some bring nothing
     [(0, [(0, 1)]), (0, [(62, 1)]), (0, [(0, 70)])],                            # nothing is shared
     [(40, [(200, 1), (10, 1), (1500, 1)])],                                     # long enough to be cut into parts
+    [(9, [(i, 1) for i in range(5)]), (49, [(40 + i, 1) for i in range(7)]), (20, [(100 * i, 1) for i in range(9)]),
+     (33, [(63, 1)] * 11)],                                                     # unequal groups, dealt out in slices of equal length
 ]
 HEADS = [(4, 4, 64), (8, 2, 128), (6, 1, 32), (4, 2, 16), (12, 4, 80), (2, 2, 256), (40, 2, 64), (3, 1, 18), (8, 1, 96)]
 
@@ -122,6 +126,17 @@ HEADS = [(4, 4, 64), (8, 2, 128), (6, 1, 32), (4, 2, 16), (12, 4, 80), (2, 2, 25
 @pytest.mark.parametrize("groups", range(len(SHARED)))
 def test_against_the_definition(dtype, heads, kv_heads, dim, groups):
     b = make(SHARED[groups], heads, kv_heads, dim, dtype, seed=groups)
+    check(b, call(b))
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim", [(32, 16, 64), (48, 24, 128), (64, 32, 128), (8, 8, 64), (40, 10, 128)])
+@pytest.mark.parametrize("members, new", [(9, 1), (24, 1), (70, 1), (4, 25), (3, 130)])
+def test_slices_of_many_pages(heads, kv_heads, dim, members, new):
+    """Many key heads leave few blocks for each: a block walks many pages, over every number of them."""
+    for pages in (67, 130):
+        b = make([(pages, [(17 * i % 90, new) for i in range(members)])], heads, kv_heads, dim, BF16, seed=pages, spread=1.5)
+        check(b, call(b))
+    b = make([(61 - 13 * g, [(11 * i % 140, new) for i in range(members // 3 + g)]) for g in range(4)], heads, kv_heads, dim, BF16, seed=12, spread=1.5)
     check(b, call(b))
 
 
