@@ -1845,52 +1845,64 @@ LLMB_EXPORT int llmb_prefix_attention_status() {
     return v;
 }
 
-// Whether the tensor-core kernel takes these operands (rows and caches on 16-byte boundaries, a positive scale).
+// Whether the tensor-core kernels take these operands (rows and caches on 16-byte boundaries, a positive scale).
 LLMB_EXPORT int llmb_prefix_attention_tc_serves(int dtype, int head_dim, int aligned, float scale) {
     return dtype == LLMB_DTYPE_BF16 && (head_dim == 64 || head_dim == 128) && aligned && scale > 0.f ? 1 : 0;
 }
 
+// The sizes of a call, one integer each.
+struct llmb_prefix_sizes {
+    int q_stride, n_pages, table_stride, out_stride;         // elements between rows, pages of the caches
+    int dtype, n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim;
+    int max_new, max_group, max_shared, max_own;             // upper bounds (ops.prefix_attention)
+    int tc;                                                  // what llmb_prefix_attention_tc_serves said, 0 to keep to the CUDA cores
+};
+
+namespace {
+Sizes sizes_of(const llmb_prefix_sizes& z) {
+    return Sizes{z.n_tokens, z.n_seqs, z.n_groups, z.n_heads, z.n_kv_heads, z.head_dim, z.max_new, z.max_group, z.max_shared, z.max_own, z.tc != 0};
+}
+}  // namespace
+
 // Floats of scratch that a call of these sizes needs, and the number of its launches in *kernels.
-LLMB_EXPORT long long llmb_prefix_attention_scratch_floats(int n_tokens, int n_seqs, int n_groups, int n_heads, int n_kv_heads, int head_dim,
-                                                           int max_new, int max_group, int max_shared, int max_own, int tc, int* kernels) {
+LLMB_EXPORT long long llmb_prefix_attention_scratch_floats(const llmb_prefix_sizes* z, int* kernels) {
     *kernels = 1;
-    if (n_tokens <= 0 || n_seqs <= 0 || n_groups <= 0 || n_kv_heads <= 0 || n_heads < n_kv_heads) return 0;
-    Plan p = plan_for(Sizes{n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own, tc != 0});
+    if (z->n_tokens <= 0 || z->n_seqs <= 0 || z->n_groups <= 0 || z->n_kv_heads <= 0 || z->n_heads < z->n_kv_heads) return 0;
+    Plan p = plan_for(sizes_of(*z));
     if (p.slots > 1) ++*kernels;
     if ((p.kernel == TILE || p.kernel == WIDE) && p.own_blocks > 0) ++*kernels;
-    return scratch_floats_of(p.part_rows * p.slots, head_dim);
+    return scratch_floats_of(p.part_rows * p.slots, z->head_dim);
 }
 
-// tc: what llmb_prefix_attention_tc_serves said, 0 to keep to the CUDA cores.
-LLMB_EXPORT int llmb_prefix_attention(const void* q, int q_stride, const void* k_cache, const void* v_cache, int n_pages, const int* block_table,
-                                      int table_stride, const int* seq_lens, const int* cu_seqlens, const int* group_first,
-                                      const int* group_pages, void* out, int out_stride, float* scratch, long long scratch_floats, int dtype,
-                                      int n_tokens, int n_seqs, int n_groups, int n_heads, int n_kv_heads, int head_dim, float scale,
-                                      int max_new, int max_group, int max_shared, int max_own, int tc, cudaStream_t stream) {
-    if (n_tokens == 0 || n_seqs == 0) return LLMB_OK;
-    LLMB_REQUIRE(n_tokens > 0 && n_seqs > 0 && n_groups > 0 && n_groups <= n_seqs, "prefix_attention: %d tokens of %d sequences in %d groups",
-                 n_tokens, n_seqs, n_groups);
-    LLMB_REQUIRE(n_kv_heads > 0 && n_heads % n_kv_heads == 0, "prefix_attention: %d heads are no multiple of %d kv heads", n_heads, n_kv_heads);
-    LLMB_REQUIRE(head_dim > 0 && head_dim <= LLMB_MAX_HEAD_DIM, "prefix_attention: head_dim %d (served: up to %d)", head_dim, LLMB_MAX_HEAD_DIM);
-    LLMB_REQUIRE(max_new > 0 && max_group >= max_new && max_shared >= 0 && max_own >= 0, "prefix_attention: bad sizes");
-    LLMB_REQUIRE((long long)n_tokens * n_heads < (1ll << 31), "prefix_attention: %d tokens of %d heads", n_tokens, n_heads);
+LLMB_EXPORT int llmb_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const int* block_table, const int* seq_lens,
+                                      const int* cu_seqlens, const int* group_first, const int* group_pages, void* out, float* scratch,
+                                      long long scratch_floats, float scale, const llmb_prefix_sizes* sizes, cudaStream_t stream) {
+    const llmb_prefix_sizes& z = *sizes;
+    if (z.n_tokens == 0 || z.n_seqs == 0) return LLMB_OK;
+    LLMB_REQUIRE(z.dtype == LLMB_DTYPE_F32 || z.dtype == LLMB_DTYPE_BF16, "prefix_attention: float32 and bfloat16 are built");
+    LLMB_REQUIRE(z.n_tokens > 0 && z.n_seqs > 0 && z.n_groups > 0 && z.n_groups <= z.n_seqs, "prefix_attention: %d tokens of %d sequences in %d groups",
+                 z.n_tokens, z.n_seqs, z.n_groups);
+    LLMB_REQUIRE(z.n_kv_heads > 0 && z.n_heads > 0 && z.n_heads % z.n_kv_heads == 0, "prefix_attention: %d heads are no multiple of %d kv heads",
+                 z.n_heads, z.n_kv_heads);
+    LLMB_REQUIRE(z.head_dim > 0 && z.head_dim <= LLMB_MAX_HEAD_DIM, "prefix_attention: head_dim %d (served: up to %d)", z.head_dim, LLMB_MAX_HEAD_DIM);
+    LLMB_REQUIRE(z.max_new > 0 && z.max_group >= z.max_new && z.max_shared >= 0 && z.max_own >= 0, "prefix_attention: bad sizes");
+    LLMB_REQUIRE((long long)z.n_tokens * z.n_heads < (1ll << 31), "prefix_attention: %d tokens of %d heads", z.n_tokens, z.n_heads);
     auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-    LLMB_REQUIRE(!tc || llmb_prefix_attention_tc_serves(dtype, head_dim, aligned(q) && q_stride % 8 == 0 && aligned(out) && out_stride % 8 == 0 &&
-                                                        aligned(k_cache) && aligned(v_cache), scale),
-                 "prefix_attention: the tensor-core kernel does not take these operands");
-    LLMB_REQUIRE(n_pages > 0 && (long long)n_pages * n_kv_heads * LLMB_PAGE < (1ll << 31), "prefix_attention: %d pages", n_pages);
-    Plan p = plan_for(Sizes{n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own, tc != 0});
+    LLMB_REQUIRE(!z.tc || llmb_prefix_attention_tc_serves(z.dtype, z.head_dim, aligned(q) && z.q_stride % 8 == 0 && aligned(out) && z.out_stride % 8 == 0 &&
+                                                          aligned(k_cache) && aligned(v_cache), scale),
+                 "prefix_attention: the tensor-core kernels do not take these operands");
+    LLMB_REQUIRE(z.n_pages > 0 && (long long)z.n_pages * z.n_kv_heads * LLMB_PAGE < (1ll << 31), "prefix_attention: %d pages", z.n_pages);
+    Plan p = plan_for(sizes_of(z));
     const long long parts = p.part_rows * p.slots;
     LLMB_REQUIRE(p.part_rows < (1ll << 31), "prefix_attention: %lld rows of parts", p.part_rows);
-    LLMB_REQUIRE(parts == 0 || (scratch != nullptr && aligned(scratch) && scratch_floats >= scratch_floats_of(parts, head_dim)),
+    LLMB_REQUIRE(parts == 0 || (scratch != nullptr && aligned(scratch) && scratch_floats >= scratch_floats_of(parts, z.head_dim)),
                  "prefix_attention: scratch too small");
-    int size = dtype == LLMB_DTYPE_F32 ? 4 : 2;
-    bool vectors = (head_dim * size) % 16 == 0 && aligned(k_cache) && aligned(v_cache);
-    Args a{q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, out, scratch, scratch + value_floats(parts, head_dim),
-           q_stride, out_stride, table_stride, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, scale * LOG2E,
+    bool vectors = (z.head_dim * (z.dtype == LLMB_DTYPE_F32 ? 4 : 2)) % 16 == 0 && aligned(k_cache) && aligned(v_cache);
+    Args a{q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, out, scratch, scratch + value_floats(parts, z.head_dim),
+           z.q_stride, z.out_stride, z.table_stride, z.n_seqs, z.n_groups, z.n_heads, z.n_kv_heads, z.head_dim, scale * LOG2E,
            p.prefix_tiles, p.prefix_splits, p.own_tiles, p.own_splits, p.slots, vectors ? 1 : 0, p.full_tiles,
            (int)p.even_blocks, 0, p.whole ? 1 : 0};
-    return run(a, p, dtype, n_pages, stream);
+    return run(a, p, z.dtype, z.n_pages, stream);
 }
 
 // the packed doors of the launching entry points (common.cuh)

@@ -1448,26 +1448,25 @@ def attention_replay_key(step, n_heads: int, n_kv_heads: int, window: int = 0):
 
 # ----------------------------------------------------------------------------- sequences that share pages
 
-_prefix_declared = False
+_prefix_entry = None
 
 
 def _declare_prefix():
-    """The argument types of prefix_attention's entry points, so that a call hands over plain numbers: its launches are short, and a
-    ctypes object for each of 30 arguments costs the host as much as they do."""
-    global _prefix_declared
-    lib, p, i = load_library("prefix_attention"), ctypes.c_void_p, _c_int
+    """prefix_attention's entry point with its argument types, so that a call hands over plain numbers: its launches are short, and a
+    ctypes object for each argument costs the host as much as they do."""
+    global _prefix_entry
+    lib, p = load_library("prefix_attention"), ctypes.c_void_p
     lib.llmb_prefix_attention_scratch_floats.restype = ctypes.c_longlong
-    lib.llmb_prefix_attention_scratch_floats.argtypes = [i] * 11 + [ctypes.POINTER(i)]
-    lib.llmb_prefix_attention.argtypes = [p, i, p, p, i, p, i, p, p, p, p, p, i, p, ctypes.c_longlong] + [i] * 7 + [_c_float] + [i] * 5 + [p]
-    _prefix_declared = True
+    lib.llmb_prefix_attention.argtypes = [p] * 10 + [ctypes.c_longlong, _c_float, p, p]
+    _prefix_entry = lib.llmb_prefix_attention
 
 
 @functools.lru_cache(maxsize=4096)
-def _prefix_scratch(*sizes) -> tuple:
-    """(floats of scratch, launches) of a prefix_attention of these sizes, the last of which says whether it runs on the tensor cores."""
-    kernels = ctypes.c_int(0)
-    floats = load_library("prefix_attention").llmb_prefix_attention_scratch_floats(*sizes, ctypes.byref(kernels))
-    return floats, kernels.value
+def _prefix_plan(*sizes) -> tuple:
+    """(the sizes of a call as the library takes them, floats of scratch, launches)."""
+    kernels, packed = ctypes.c_int(0), (_c_int * len(sizes))(*sizes)
+    floats = load_library("prefix_attention").llmb_prefix_attention_scratch_floats(packed, ctypes.byref(kernels))
+    return packed, ctypes.addressof(packed), floats, kernels.value
 
 
 def page_bucket(pages: int) -> int:
@@ -1491,7 +1490,7 @@ def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, g
 
     max_new, max_group: most new tokens of a sequence, of a group; max_shared: most pages that a group shares; max_own: most
     positions of a sequence behind those. Upper bounds, which size the launches."""
-    if not _prefix_declared:
+    if _prefix_entry is None:
         _declare_prefix()
     dtype, int32 = qkv.dtype, torch.int32
     tensors = (qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages)
@@ -1521,7 +1520,7 @@ def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, g
         raise KernelError(f"prefix_attention: no bounds of a step: max_new {max_new}, max_group {max_group}, max_shared {max_shared}, "
                           f"max_own {max_own}")
     if out is None:
-        out = torch.empty((n, n_heads * head_dim), dtype=dtype, device=qkv.device)
+        out = qkv.new_empty((n, n_heads * head_dim))
     else:
         _check_out(out, (n, n_heads * head_dim), dtype, "prefix_attention")
     if n == 0:
@@ -1530,14 +1529,14 @@ def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, g
     at_q, at_k, at_v, at_out = qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
     tc = int(dtype is torch.bfloat16 and head_dim in (64, 128) and scale > 0 and q_stride % 8 == 0 and not (at_q | at_k | at_v | at_out) & 15
              and not tactics.is_disabled("prefix_attention_tc"))
-    floats, kernels = _prefix_scratch(n, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, shared, own, tc)
+    packed, at_sizes, floats, kernels = _prefix_plan(q_stride, paged[0], table_stride, n_heads * head_dim, _DTYPE_CODE.get(dtype, -1), n, n_seqs, n_groups,
+                                                     n_heads, n_kv_heads, head_dim, max_new, max_group, shared, own, tc)
     parts = _scratch(qkv.device, "attention", floats)[0] if floats else None
     if _recording is not None:
-        _recording.keep += [*tensors, out, parts]
-    _call("prefix_attention", "llmb_prefix_attention", at_q, q_stride, at_k, at_v, k_cache.shape[0], block_table.data_ptr(), table_stride,
-          seq_lens.data_ptr(), cu_seqlens.data_ptr(), group_first.data_ptr(), group_pages.data_ptr(), at_out, out.stride(0),
-          parts.data_ptr() if floats else None, floats, _code(dtype), n, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, scale, max_new,
-          max_group, shared, own, tc, _stream(), kernels=kernels)
+        _recording.keep += [*tensors, out, parts, packed]
+    _call("prefix_attention", "llmb_prefix_attention", at_q, at_k, at_v, block_table.data_ptr(), seq_lens.data_ptr(), cu_seqlens.data_ptr(),
+          group_first.data_ptr(), group_pages.data_ptr(), at_out, parts.data_ptr() if floats else None, floats, float(scale), at_sizes, _stream(),
+          kernels=kernels)
     return out
 
 
