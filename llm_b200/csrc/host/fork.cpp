@@ -197,8 +197,8 @@ LLMH_EXPORT int llmh_cache_apply_moves(void* cache, int group, int count, const 
 }
 
 // The groups of a step's entries that share pages: entries first[g] .. first[g + 1] - 1 have pages[g] pages in common (first: room for
-// n + 1, pages: for n). summary: [groups, most new tokens of an entry, of a group, most shared pages, most positions behind them];
-// groups = 0: nothing is shared.
+// n + 1, pages: for n). summary: [groups, most new tokens of an entry, of a group, most shared pages, most positions behind them, pages that are
+// read once less for each further member of a group]; groups = 0: nothing is shared.
 LLMH_EXPORT int llmh_step_groups(void* cache, int n, const int* slots, const int* counts, int* first, int* pages, int* summary) {
     return guarded([&] {
         const Cache& c = *static_cast<Cache*>(cache);
@@ -206,7 +206,7 @@ LLMH_EXPORT int llmh_step_groups(void* cache, int n, const int* slots, const int
         for (int i = 0; i < n; ++i) c.require_held(slots[i]);
         for (int i = 0; i + 1 < n; ++i) common[i] = c.common_pages(slots[i], slots[i + 1]);
         int groups = best_runs(n, common.data(), first);
-        int max_new = 0, max_group = 0, max_shared = 0, max_own = 0;
+        int max_new = 0, max_group = 0, max_shared = 0, max_own = 0, saved = 0;
         for (int g = 0; g < groups; ++g) {
             int shared = first[g + 1] - first[g] > 1 ? 0x7fffffff : 0, tokens = 0;
             for (int i = first[g]; i + 1 < first[g + 1]; ++i) shared = std::min(shared, common[i]);
@@ -218,7 +218,9 @@ LLMH_EXPORT int llmh_step_groups(void* cache, int n, const int* slots, const int
             }
             max_group = std::max(max_group, tokens);
             max_shared = std::max(max_shared, shared);
+            saved += (first[g + 1] - first[g] - 1) * shared;
         }
+        summary[5] = saved;
         summary[0] = max_shared > 0 ? groups : 0;
         summary[1] = max_new;
         summary[2] = max_group;

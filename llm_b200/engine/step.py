@@ -294,16 +294,16 @@ class Engine:
     def _groups(self, batch, room):
         """Which of the batch's sequences share pages, written behind the step's sections: (groups, and the bounds of
         SharedPages, numbers of pages as the launches know them: rounded up to a power of two), or None."""
-        first, pages, summary = (c_int * (batch.n + 1))(), (c_int * batch.n)(), (c_int * 5)()
+        first, pages, summary = (c_int * (batch.n + 1))(), (c_int * batch.n)(), (c_int * 6)()
         native.check(native.lib().llmh_step_groups(self.cache._handle, batch.n, batch.slots, batch.counts, first, pages, summary))
-        n_groups, max_new, max_group, max_shared, max_own = summary
+        n_groups, max_new, max_group, max_shared, max_own, saved = summary
         if n_groups == 0:
             return None
         at = self._group_room(batch.n)
         room[:n_groups + 1] = torch.tensor(first[:n_groups + 1], dtype=torch.int32)
         room[at:at + n_groups] = torch.tensor(pages[:n_groups], dtype=torch.int32)
         widest = min(g.ring_pages for g in self.cache.groups if not g.window)
-        return (n_groups, max_new, max_group, min(ops.page_bucket(max_shared), widest), ops.page_bucket(-(-max_own // PAGE)) * PAGE)
+        return (n_groups, max_new, max_group, min(ops.page_bucket(max_shared), widest), ops.page_bucket(-(-max_own // PAGE)) * PAGE, saved)
 
     # ------------------------------------------------------------------ recorded passes
 

@@ -120,7 +120,8 @@ class AttentionMixer(Mixer):
                                  write_cache=(entry == cache_entry))
         mixed = ctx.scratch("mixed", (n, self.q_width), h.dtype)
         share = ctx.sharing if s.window == 0 else None
-        if share is not None and ops.prefix_attention_pays(share.max_shared):
+        if share is not None and ops.prefix_attention_pays(h.dtype, s.n_heads, s.n_kv_heads, s.head_dim, ctx.n_seqs, share.max_new,
+                                                           share.max_shared, share.saved_pages):
             mixed = ops.prefix_attention(qkv, keys, values, table, ctx.seq_lens, ctx.cu_seqlens, share.group_first, share.group_pages,
                                          s.n_heads, s.n_kv_heads, s.head_dim, s.scale, max_new=share.max_new, max_group=share.max_group,
                                          max_shared=share.max_shared, max_own=share.max_own, out=mixed)

@@ -33,6 +33,7 @@ class SharedPages:
     max_group: int                 # of a group
     max_shared: int                # most pages that a group shares
     max_own: int                   # most positions of a sequence behind them
+    saved_pages: int               # pages that are read once less for each further member of a group
 
 
 @dataclass

@@ -210,7 +210,7 @@ def test_forked_sequences_go_their_own_ways(tmp_path, plain_kernels, monkeypatch
     import llm_b200.ops as ops
     config, weights, engine = _setup(tmp_path, "A")
     calls = []
-    plain = ops.prefix_attention
+    plain = ops.prefix_attention                           # (32-bit steps always read shared pages once)
     monkeypatch.setattr(ops, "prefix_attention", lambda *a, **k: calls.append((a[6].tolist(), a[7].tolist(), k)) or plain(*a, **k))
     prompt = random_tokens(70, config["vocab_size"], 1)
     (slot,) = engine.acquire()

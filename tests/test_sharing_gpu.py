@@ -22,8 +22,12 @@ def engine_for(folder, dtype, **options):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("which", sorted(CONFIGS))
-def test_forked_sequences_against_the_plain_implementation(tmp_path, dtype, which):
+def test_forked_sequences_against_the_plain_implementation(tmp_path, monkeypatch, dtype, which):
     from llm_b200 import ops
+    used = []
+    kernel = ops.prefix_attention
+    monkeypatch.setattr(ops, "prefix_attention", lambda *a, **k: used.append(1) or kernel(*a, **k))
+    monkeypatch.setattr(ops, "prefix_attention_pays", lambda *a: not ops.tactics.is_disabled("prefix_attention"))      # however little is shared
     from llm_b200.engine import Entry
     folder = make_folder(tmp_path, which, BF16)
     config, weights = plain_llama.read_model_folder(folder)
@@ -50,11 +54,11 @@ def test_forked_sequences_against_the_plain_implementation(tmp_path, dtype, whic
         texts = [t + n for t, n in zip(texts, new)]
         step(new)
     assert engine.graph_replays >= 4
-    before = ops.launch_count()
+    assert used
     new = [[5]] * 6
     texts = [t + [5] for t in texts]
     shared = step(new)
-    assert ops.launch_count() > before
+    del used[:]
     for s, t in zip(slots, texts):                         # the same step with every sequence's pages read for itself
         engine.cache.set_length(s, len(t) - 1)
     ops.tactics.disable("prefix_attention")
@@ -63,6 +67,7 @@ def test_forked_sequences_against_the_plain_implementation(tmp_path, dtype, whic
         apart = step(new)
     finally:
         ops.tactics.enable("prefix_attention")
+    assert not used
     assert close(shared, apart.cpu(), dtype)
     engine.release(slots[:2])
     engine.cache.compact()
@@ -114,3 +119,39 @@ def test_samples_of_a_prompt(tmp_path, which):
         for j in range(3):
             assert llm.generate([p], seed=7 + 3 * i + j, **options)[0] == together[i][j]
     llm.engine.cache.check()
+
+
+def test_what_is_read_once_pays_from_some_bytes_on():
+    from llm_b200 import ops
+    pays = ops.prefix_attention_pays
+    assert not pays(BF16, 32, 8, 128, 4, 1, 8, 24) and pays(BF16, 32, 8, 128, 4, 1, 32, 96)
+    assert not pays(BF16, 32, 8, 128, 64, 1, 4, 252) and pays(BF16, 32, 8, 128, 64, 1, 8, 504)
+    assert not pays(BF16, 32, 8, 128, 8, 20, 16, 112) and pays(BF16, 32, 8, 128, 8, 20, 32, 224)
+    assert not pays(BF16, 32, 32, 128, 8, 90, 64, 448) and pays(BF16, 32, 32, 128, 8, 90, 128, 896)
+    assert pays(F32, 4, 2, 16, 2, 1, 1, 1) and not pays(F32, 4, 2, 16, 2, 1, 0, 0)
+    assert not pays(BF16, 4, 2, 96, 8, 1, 128, 896) and pays(BF16, 4, 2, 80, 8, 1, 1, 7)
+
+
+def test_a_long_prompt_is_read_once_by_rule(tmp_path):
+    """Eight samples of 1,600 positions on the small model with heads of 128: the step chooses the kernel for itself, in a prompt step and
+    in replayed decode steps."""
+    from llm_b200 import ops
+    from llm_b200.engine import Entry
+    folder = make_folder(tmp_path, "F", BF16)
+    config, weights = plain_llama.read_model_folder(folder)
+    engine = engine_for(folder, F32)
+    common = random_tokens(1600, config["vocab_size"], 1)
+    (slot,) = engine.acquire()
+    engine.step([Entry(slot, common, [])])
+    slots = [slot] + engine.fork(slot, 7)
+    want = plain_llama.forward(config, weights, common + [3, 4, 5])
+    logits = engine.step([Entry(s, [3, 4], [0, 1]) for s in slots])
+    for s in range(8):
+        assert close(logits[2 * s:2 * s + 2], want[1600:1602], F32)
+    for _ in range(4):
+        logits = engine.step([Entry(s, [5], [0]) for s in slots])
+        for s, row in zip(slots, logits):
+            assert close(row[None], want[1602:1603], F32)
+            engine.cache.set_length(s, 1602)
+    engine.check()
+    engine.cache.check()
