@@ -1741,7 +1741,9 @@ Plan plan_for(const Sizes& z) {
         long long per = (prefix * walk + owns * own + wave - 1) / wave;
         if (per < 2) per = 2;
         p.prefix_splits = p.prefix_tiles > 0 ? ceil_div(walk, per) : 0;
-        p.own_splits = p.own_tiles > 0 ? ceil_div(own, per) : 0;
+        // own pages beside the tile kernel: a launch of their own, cut only where they are long (16 sequences behind 8,192 positions 17.8 us, with
+        // two blocks for one to four own pages 21.9)
+        p.own_splits = p.own_tiles == 0 ? 0 : ceil_div(own, p.kernel == TILE ? 32 : per);
         if (even) {
             p.prefix_splits = ceil_div(2 * SMS, z.n_kv_heads);
             if (p.prefix_splits > ceil_div(shared, 2)) p.prefix_splits = ceil_div(shared, 2);
