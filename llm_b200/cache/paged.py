@@ -185,8 +185,10 @@ class PagedCache:
         return slot.value
 
     def release(self, slot: int) -> None:
-        """Give the slot and all of its pages back."""
+        """Give the slot and all of its pages back (a page that other slots hold stays theirs)."""
         native.check(native.lib().llmh_cache_release(self._handle, int(slot)))
+        if self.forked and self.slots.n_held <= 1:
+            self.forked = False              # nobody is left to share with
 
     def fork(self, slot: int, count: int = 1) -> list:
         """`count` new slots that hold what `slot` holds: the same full pages, and copies (queued on the current stream) of the

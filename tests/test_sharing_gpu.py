@@ -155,3 +155,15 @@ def test_a_long_prompt_is_read_once_by_rule(tmp_path):
             engine.cache.set_length(s, 1602)
     engine.check()
     engine.cache.check()
+
+
+def test_the_command_line_prints_a_line_a_sample(tmp_path, capsys):
+    from llm_b200.cli import main
+    import llm_b200
+    folder = make_folder(tmp_path, "A", F32)
+    assert main(["--model", str(folder), "--dtype", "float32", "--context", "100", "--max-tokens", "6", "--samples", "3", "--seed", "5", "7", "8", "9"]) == 0
+    lines = [[int(t) for t in line.split()] for line in capsys.readouterr().out.splitlines()]
+    llm = llm_b200.LLM(str(folder), dtype="float32", context=100, batch=1)
+    assert lines == [llm.generate([[7, 8, 9]], max_tokens=6, seed=5 + j)[0] for j in range(3)]
+    with pytest.raises(SystemExit):
+        main(["--model", str(folder), "--samples", "0", "7"])
