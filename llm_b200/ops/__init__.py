@@ -10,6 +10,7 @@ The parts call these functions as attributes of this module
 """
 from __future__ import annotations
 
+import array
 import atexit
 import collections
 import ctypes
@@ -1573,10 +1574,11 @@ def _copy_items(shapes, n_items: int, source, target, rows, what: str) -> None:
     if len(targets) != len(target) or not targets.isdisjoint(source):
         raise KernelError(f"{what}: every target is written once and no target is a source")
     triples = sorted(zip(source, target, rows))                      # the targets of a source stand together
-    pairs = (_c_int * (3 * len(triples)))(*itertools.chain.from_iterable(triples))
-    flat = (ctypes.c_longlong * (7 * len(shapes)))(*itertools.chain.from_iterable(shapes))
+    pairs = array.array("i", itertools.chain.from_iterable(triples))
+    flat = array.array("q", itertools.chain.from_iterable(shapes))
     launches = -(-len(shapes) // 16) * -(-len(triples) // 240)
-    _call("page_copy", "llmb_page_copy", _c_int(len(shapes)), flat, _c_int(len(triples)), pairs, _stream(), kernels=launches)
+    _call("page_copy", "llmb_page_copy", _c_int(len(shapes)), ctypes.c_void_p(flat.buffer_info()[0]), _c_int(len(triples)),
+          ctypes.c_void_p(pairs.buffer_info()[0]), _stream(), kernels=launches)
 
 
 def copy_pages(pools, source, target, rows=None) -> None:
@@ -1587,20 +1589,21 @@ def copy_pages(pools, source, target, rows=None) -> None:
     written twice, and no page is both a source and a target."""
     pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
     _require_cuda(*pools)
-    shapes = []
+    shapes, pages = [], None
     for pool in pools:
-        if pool.dim() < 4 or not pool.is_contiguous() or pool.shape[-2] != PAGE or pool.shape[-4] != pools[0].shape[-4]:
+        sizes = pool.shape
+        if len(sizes) < 4 or sizes[-2] != PAGE or pages not in (None, sizes[-4]) or not pool.is_contiguous():
             raise KernelError(f"copy_pages: a pool must be contiguous [..., pages, heads, {PAGE}, dim], all with the same pages")
-        pages, heads, _, dim = pool.shape[-4:]
-        row = dim * pool.element_size()
-        if pool.numel():
-            shapes.append((pool.data_ptr(), pool.numel() // (pages * heads * PAGE * dim), heads, pages * heads * PAGE * row, heads * PAGE * row,
+        pages, heads, _, dim = sizes[-4:]
+        row, count = dim * pool.element_size(), pool.numel()
+        if count:
+            shapes.append((pool.data_ptr(), count // (pages * heads * PAGE * dim), heads, pages * heads * PAGE * row, heads * PAGE * row,
                            PAGE * row, row))
     if rows is None:
         rows = [PAGE] * len(source)
     elif len(rows) and (min(rows) < 1 or max(rows) > PAGE):
         raise KernelError(f"copy_pages: a page has 1 to {PAGE} rows to copy")
-    _copy_items(shapes, pools[0].shape[-4] if pools else 0, source, target, rows, "copy_pages")
+    _copy_items(shapes, pages or 0, source, target, rows, "copy_pages")
 
 
 def copy_slots(states, source, target) -> None:
