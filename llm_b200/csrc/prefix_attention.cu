@@ -1707,14 +1707,19 @@ Plan plan_for(const Sizes& z) {
     int shared = z.max_shared > 0 ? bucket(z.max_shared) : 0, own = bucket(ceil_div(z.max_own > 0 ? z.max_own : 1, LLMB_PAGE));
     // sequences that bring few rows each would leave a tile of a group to walk many sequences' pages for a few of its rows
     p.whole = z.tc && (long long)z.max_new * share > FEW_ROWS;
-    // One shared page is read by every sequence itself: with one own page besides, that is a single launch without parts. Three sequences of a
-    // small 32-bit model take 14.5 us from the host for 22, the same 7.1 on the device.
-    p.alone = !p.whole && shared == 1;
+    long long group_rows = shared > 0 ? (long long)z.max_group * share : 0;
+    // A few shared pages are read by every sequence itself: they come from L2, and a launch, its start and its parts are saved. One page always (three
+    // sequences of a small 32-bit model 14.5 us from the host for 22). Instead of the wide kernel up to 4,096 pages of a key head in all: heads of 128
+    // over 8, 64 sequences behind 2, 4 and 8 pages 12.3, 15.0, 20.3 us for 20.5, 22.5, 22.8; behind 16 pages 24 either way. Instead of the tile kernel up to
+    // 512, while no SM has two sequences: 8 behind 4, 8 and 16 pages 7.1, 7.7 and 12.7 for 9.3, 9.6 and 10.1; 32 behind 2 pages 12.7 for 11.2.
+    const long long walks = (long long)z.n_seqs * z.n_kv_heads;
+    p.alone = !p.whole && (shared == 1 || (z.tc && shared > 0 && group_rows > FEW_ROWS &&
+                                           (group_rows > TC_ROWS ? walks * shared <= 4096 : walks * shared <= 512 && walks <= SMS)));
     if (p.alone) {
+        own = bucket(own + shared);
         shared = 0;
-        own = bucket(own + 1);
+        group_rows = 0;
     }
-    const long long group_rows = shared > 0 ? (long long)z.max_group * share : 0;
     p.kernel = !z.tc ? CUDA_CORES : p.whole || group_rows > TC_ROWS ? WIDE : group_rows > FEW_ROWS ? TILE : FEW;
     int rows = p.kernel == WIDE ? WIDE_ROWS : z.tc ? TC_ROWS : SIMT_ROWS;
     p.prefix_tiles = shared > 0 || p.whole ? ceil_div((long long)z.max_group * share, rows) : 0;

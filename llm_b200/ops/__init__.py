@@ -1479,13 +1479,14 @@ def prefix_attention_pays(dtype, n_heads, n_kv_heads, head_dim, n_seqs, max_new,
     """Whether a step whose sequences share pages reads them once for each group (`prefix_attention`) or for each sequence
     (`attention`); saved_pages: pages that are read once less for each further member of a group.
 
-    In 32 bits always (two sequences behind one page 12 us for 39, eight behind 32 pages 20 for 362). In bfloat16 where
+    In 32 bits always (two sequences behind one page 8 us for 33, eight behind 32 pages 19 for 361). In bfloat16 where
     `attention` has a tensor-core kernel and this has none (32, 96) never, where neither has one always. Head sizes 64 and 128,
     measured at 32 heads over 8 and over 32, with 2 to 64 sequences behind 1 to 128 pages; microseconds without and with:
 
-    * single tokens: reading a page again is cheap until the saved bytes outweigh the join, some 6 MB and 1.5 MB for every
-      sequence. Heads of 128 over 8: 4 sequences behind 8 pages 6.1 / 7.4, 32 pages 10.9 / 9.0; 16 behind 4 pages 8.9 / 10.5, 16 pages
-      16.6 / 13.1; 64 behind 4 pages 19 / 22, 8 pages 30 / 23, 128 pages 305 / 38.
+    * single tokens: reading a page again is cheap until the saved bytes outweigh the join, some 10 MB and 0.8 MB for every
+      sequence. Heads of 128 over 8: 4 sequences behind 8 pages 6.1 / 7.4, 32 pages 10.9 / 9.0; 16 behind 4 pages 9.0 / 8.8, 16 pages
+      16.7 / 11.1; 64 behind 2 pages 14.5 / 12.3, 4 pages 19 / 15, 8 pages 30 / 20, 128 pages 305 / 38; heads of 64: 8 behind 16 pages 6.7 / 9.2, 64
+      behind 8 pages 17 / 15.
     * several tokens: tiles of several sequences' rows fill up where query heads share a key head, so 32 pages pay (8 sequences
       of 5 to 20 tokens 38 / 27, of 200 to 300 106 / 86; behind 8 pages 16 / 24 and 48 / 46); with a key head for each query head
       128 pages do (8 sequences of 40 to 90 tokens 136 / 125, behind 32 pages 40 / 56)."""
@@ -1497,7 +1498,7 @@ def prefix_attention_pays(dtype, n_heads, n_kv_heads, head_dim, n_seqs, max_new,
         return head_dim not in (32, 64, 96, 128)
     if max_new > 1:
         return max_shared >= (32 if n_heads > n_kv_heads else 128)
-    return saved_pages * PAGE * n_kv_heads * head_dim * 4 >= 6e6 + 1.5e6 * n_seqs
+    return saved_pages * PAGE * n_kv_heads * head_dim * 4 >= 10e6 + 0.8e6 * n_seqs
 
 
 def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, n_heads, n_kv_heads, head_dim,

@@ -201,6 +201,27 @@ def test_more_sequences_than_shared_memory_lists(heads, kv_heads, dim):
     check(b, call(b))
 
 
+@pytest.mark.parametrize("heads, kv_heads, dim", [(8, 2, 64), (32, 8, 128), (16, 2, 128), (4, 2, 64)])
+@pytest.mark.parametrize("members, shared", [(9, 2), (9, 9), (9, 70), (40, 1), (40, 2), (40, 33), (70, 7), (70, 17), (140, 3), (140, 40)])
+def test_shared_pages_read_by_every_sequence_or_once(heads, kv_heads, dim, members, shared):
+    """Few shared pages are read by every sequence itself, many once for all: sizes on both sides, one group and several."""
+    b = make([(shared, [(23 * i % 140, 1) for i in range(members)])], heads, kv_heads, dim, BF16, seed=30 + shared)
+    check(b, call(b))
+    b = make([(shared, [(31 * i % 90, 1) for i in range(members)]), (0, [(5, 1), (0, 0)]), (shared // 2, [(i, 1) for i in range(members // 2)])],
+             heads, kv_heads, dim, BF16, seed=31 + shared)
+    check(b, call(b))
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim", [(4, 2, 64), (16, 2, 128)])
+def test_more_sequences_than_shared_memory_lists_behind_many_pages(heads, kv_heads, dim):
+    """Shared pages that are read once: groups of more rows than a tile holds, and small ones."""
+    b = make([(5, [(i % 70, 1) for i in range(300)]), (9, [(i % 40, 1) for i in range(200)])] + [(0, [(i % 50, 1)]) for i in range(60)],
+             heads, kv_heads, dim, BF16, seed=41)
+    check(b, call(b))
+    b = make([(3 + g % 4, [(i * 9 + g, 1) for i in range(7 + g % 5)]) for g in range(62)], heads, kv_heads, dim, BF16, seed=42)
+    check(b, call(b))
+
+
 def test_same_result_twice_and_on_another_stream():
     b = make(SHARED[5], 32, 8, 128, BF16, seed=7)
     first = call(b)

@@ -125,7 +125,7 @@ def test_what_is_read_once_pays_from_some_bytes_on():
     from llm_b200 import ops
     pays = ops.prefix_attention_pays
     assert not pays(BF16, 32, 8, 128, 4, 1, 8, 24) and pays(BF16, 32, 8, 128, 4, 1, 32, 96)
-    assert not pays(BF16, 32, 8, 128, 64, 1, 4, 252) and pays(BF16, 32, 8, 128, 64, 1, 8, 504)
+    assert not pays(BF16, 32, 8, 128, 64, 1, 1, 63) and pays(BF16, 32, 8, 128, 64, 1, 4, 252) and pays(BF16, 32, 8, 128, 64, 1, 8, 504)
     assert not pays(BF16, 32, 8, 128, 8, 20, 16, 112) and pays(BF16, 32, 8, 128, 8, 20, 32, 224)
     assert not pays(BF16, 32, 32, 128, 8, 90, 64, 448) and pays(BF16, 32, 32, 128, 8, 90, 128, 896)
     assert pays(F32, 4, 2, 16, 2, 1, 1, 1) and not pays(F32, 4, 2, 16, 2, 1, 0, 0)
