@@ -222,6 +222,18 @@ def test_more_sequences_than_shared_memory_lists_behind_many_pages(heads, kv_hea
     check(b, call(b))
 
 
+@pytest.mark.parametrize("members, shared", [(40, 17), (40, 1), (70, 33), (70, 2), (61, 0)])
+def test_own_pages_of_unequal_sequences(members, shared):
+    """One to two rounds of blocks for own pages, from none to many: long sequences start first, behind each way of reading the shared pages."""
+    b = make([(shared, [(137 * i % 900, 1) for i in range(members)])], 16, 8, 64, BF16, seed=50 + shared)
+    check(b, call(b))
+    b = make([(shared, [(97 * i % 700, 1) for i in range(members - 20)]), (0, [(3, 1), (0, 0), (650, 1)]), (shared // 3, [(200 * i, 1) for i in range(4)])],
+             16, 8, 64, BF16, seed=51 + shared)
+    check(b, call(b))
+    b = make([(shared, [(0, 1)] * (members - 1) + [(600, 1)])], 16, 8, 64, BF16, seed=52 + shared)
+    check(b, call(b))
+
+
 def test_same_result_twice_and_on_another_stream():
     b = make(SHARED[5], 32, 8, 128, BF16, seed=7)
     first = call(b)
