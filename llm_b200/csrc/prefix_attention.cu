@@ -1,6 +1,7 @@
 // Attention of a batch whose sequences share their first pages of the cache: several samples of one prompt, several questions
 // behind one document. Sequences that stand together in the batch form groups; the members of a group have the same pages in the
-// first `group_pages` places of their page tables. The keys and values of those pages are read once for all queries of the group.
+// first `group_pages` places of their page tables. The keys and values of those pages are read once for all queries of the group, or by
+// each sequence where they are few pages (plan_for).
 //
 //   out[t, a] = sum_j p_j v_j,  p = softmax_j(scale * q[t, a] . k_j),  j <= position of t,  keys of head a * kv_heads / heads
 //
