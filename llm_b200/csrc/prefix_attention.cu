@@ -1172,14 +1172,16 @@ prefix_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __
     w.kv_head = piece.kv_head;
     w.tile = piece.tile;
     const int group = piece.group;
-    if (group >= a.n_groups) return;                          // uniform for the block, here and below: nothing is allocated yet
+    // A block without work leaves here (the block as a whole, nothing is allocated yet), behind the kernel in front all the same: if
+    // none has any (a step whose groups turn out to share nothing), the own parts that follow rely on these waits alone.
+    if (group >= a.n_groups) return griddep_wait();
     w.seq_first = a.group_first[group];
     w.seq_last = a.group_first[group + 1];
-    if (w.seq_first >= w.seq_last) return;
+    if (w.seq_first >= w.seq_last) return griddep_wait();
     w.first_token = a.cu_seqlens[w.seq_first];
     w.n_rows = (a.cu_seqlens[w.seq_last] - w.first_token) * share;
     const int row0 = w.tile * WIDE_ROWS, n_rows = min(WIDE_ROWS, w.n_rows - row0);
-    if (n_rows <= 0) return;
+    if (n_rows <= 0) return griddep_wait();
     const int n_tiles = n_rows > TC_ROWS ? 2 : 1;
     TileRange range;
     range.token_first = w.first_token + row0 / share;
