@@ -886,9 +886,8 @@ prefix_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __
         bool ok = true;
         for (int kb = 0; kb < n_pages && ok; ++kb) {
             const int b = kb & 1, pos = my_pos - (w.page_begin + kb) * LLMB_PAGE;        // the last key that the row sees, from the page's first
-            ok = mbar_wait(smem_u32(&s_full[b]), (kb >> 1) & 1, abort_flag, status, 17);
+            ok = mbar_wait_warp(smem_u32(&s_full[b]), (kb >> 1) & 1, abort_flag, status, 17);      // one answer for the warp: its loads are the whole warp's
             if (!ok) break;
-            __syncwarp();
             if (idle) {
                 mbar_arrive(smem_u32(&p_full[b]));
                 continue;
@@ -950,9 +949,8 @@ prefix_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __
             tcgen05_fence_before();
             mbar_arrive(smem_u32(&p_full[b]));
         }
-        if (ok) ok = mbar_wait(smem_u32(o_last), 0, abort_flag, status, 19);
+        if (ok) ok = mbar_wait_warp(smem_u32(o_last), 0, abort_flag, status, 19);
         if (ok && !idle) {
-            __syncwarp();
             tcgen05_fence_after();
             // All products are complete, the pages' room is free: a row goes out from there in one bulk copy. Rows lie 16 bytes further
             // apart than they are long.
@@ -1434,12 +1432,11 @@ prefix_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __
                         stored1 = min(at.limit - at.logical * LLMB_PAGE, LLMB_PAGE - 1) + 1;
                     }
                 }
-                ok = mbar_wait(smem_u32(&s_full[tile]), kb & 1, abort_flag, status, 38);
+                ok = mbar_wait_warp(smem_u32(&s_full[tile]), kb & 1, abort_flag, status, 38);
                 if (!ok) break;
-                __syncwarp();
                 tcgen05_fence_after();
                 if (stored0 < LLMB_PAGE || stored1 < LLMB_PAGE) {     // values behind the last position are whatever a page held: zero here
-                    ok = mbar_wait(smem_u32(&v_full[kb & 1]), (kb >> 1) & 1, abort_flag, status, 39);
+                    ok = mbar_wait_warp(smem_u32(&v_full[kb & 1]), (kb >> 1) & 1, abort_flag, status, 39);
                     if (!ok) break;
                     for (int half = 0; half < 2 && tile == 0; ++half) {       // (the first tile's products are issued first)
                         int first = max(half ? stored1 : stored0, 0), chunks = (LLMB_PAGE - first) * 8;
@@ -1538,9 +1535,8 @@ prefix_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 }
             }
             // both tiles' products are complete: the pages' room is free
-            for (int i = 0; i < n_tiles && ok && n_blocks > 0; ++i) ok = mbar_wait(smem_u32(&o_full[i]), 0, abort_flag, status, 40);
+            for (int i = 0; i < n_tiles && ok && n_blocks > 0; ++i) ok = mbar_wait_warp(smem_u32(&o_full[i]), 0, abort_flag, status, 40);
             if (ok && !idle) {
-                __syncwarp();
                 tcgen05_fence_after();
                 const bool direct = piece.pieces == 1 && a.whole;
                 const float inv = run_sum != 0.f ? 1.0f / run_sum : 0.f;

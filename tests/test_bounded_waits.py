@@ -19,3 +19,10 @@ def test_no_thread_leaves_its_warps_on_its_own_wait(name):
         statement = source[max(source.rfind(c, 0, at) for c in ";{}") + 1:source.index(";", at)].strip()
         assert statement.startswith("mbar_wait("), f"{name}: the answer of `{statement}` is used"
     assert "mbar_wait_warp(" in source
+
+
+def test_prefix_attention_asks_as_a_warp():
+    """Behind every wait of its kernels come loads of whole warps or barriers of the block: no thread may go its own way on an answer of its own."""
+    source = re.sub(r"//[^\n]*", "", (CSRC / "prefix_attention.cu").read_text())
+    assert not re.findall(r"\bmbar_wait\(", source)
+    assert source.count("mbar_wait_warp(") >= 15
