@@ -520,11 +520,23 @@ __device__ __forceinline__ void put_stats(const Args& a, const Item& w, int piec
     for (int i = first; i < a.prefix_splits; ++i) stats[i] = make_float2(-INFINITY, 0.f);
 }
 
-// The block's slice; uniform for the block. *pieces: of a group whose slices are dealt out.
-__device__ __forceinline__ bool slice_of(const Args& a, Item& w, int& pieces) {
+// What a kernel reports of a step that brings more tokens than the bounds of its call say (no wait has this code).
+constexpr int BEYOND_BOUNDS = 50;
+__device__ __forceinline__ void report_beyond_bounds(int* status) {
+    if (threadIdx.x == 0 && status) atomicCAS(status, 0, BEYOND_BOUNDS);
+}
+
+// The block's slice; uniform for the block. *pieces: of a group whose slices are dealt out. The kernels have room for `most` rows, which the launch has
+// chosen them for by max_new and max_group; the lengths are on the device only, so that it shows here whether they keep to those.
+__device__ __forceinline__ bool slice_of(const Args& a, Item& w, int& pieces, int most, int* status) {
     int x = blockIdx.x - (a.prefix_tiles > 0 ? a.even_blocks : 0);
     pieces = 0;
-    return (x < 0 ? even_slice_of(a, blockIdx.x, threadIdx.x & 31, w, pieces) : item_of(a, x, w)) && w.n_rows > 0;
+    bool work = (x < 0 ? even_slice_of(a, blockIdx.x, threadIdx.x & 31, w, pieces) : item_of(a, x, w)) && w.n_rows > 0;
+    if (work && w.n_rows > most) {
+        report_beyond_bounds(status);
+        w.n_rows = most;
+    }
+    return work;
 }
 
 // Up to 16 rows over the pages [page_begin, page_end) of one table.
@@ -556,7 +568,7 @@ prefix_attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __g
     order_sequences(a, order);
     Item w;
     int pieces;
-    const bool work = slice_of(a, w, pieces);
+    const bool work = slice_of(a, w, pieces, FEW_ROWS, status);
     __syncthreads();
     // Behind the kernel of the shared parts the own ones may run beside them: that kernel lets them start when the one in front of it is
     // complete. Each block waits for it at its end, so that the join waits for both.
@@ -771,7 +783,7 @@ prefix_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __
     stage_arrays(a, staged);
     Item w;
     int pieces;
-    const bool work = slice_of(a, w, pieces);                // nothing is allocated where a block leaves
+    const bool work = slice_of(a, w, pieces, TC_ROWS, status);                // nothing is allocated where a block leaves
     const int share = a.n_heads / a.n_kv_heads, n_pages = work ? w.page_end - w.page_begin : 0;
     // Tensor memory is taken when the kernel in front is done with it, and the next kernel may take some only when this one has it: two
     // that wait for one another's would stand still.
@@ -1178,6 +1190,7 @@ prefix_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k, const __
     if (w.seq_first >= w.seq_last) return griddep_wait();
     w.first_token = a.cu_seqlens[w.seq_first];
     w.n_rows = (a.cu_seqlens[w.seq_last] - w.first_token) * share;
+    if (w.n_rows > a.prefix_tiles * WIDE_ROWS) report_beyond_bounds(status);       // (tiles that no block has)
     const int row0 = w.tile * WIDE_ROWS, n_rows = min(WIDE_ROWS, w.n_rows - row0);
     if (n_rows <= 0) return griddep_wait();
     const int n_tiles = n_rows > TC_ROWS ? 2 : 1;

@@ -1106,13 +1106,15 @@ def tensor_core_status() -> int:
 
 
 def check_device_status() -> None:
-    """Raise if a kernel of a loaded library reported a wait that ran out. Cheap (it
-    reads a word of host memory); meaningful after the stream was synchronised."""
+    """Raise if a kernel of a loaded library reported a wait that ran out, or a step beyond its call's
+    bounds (prefix_attention). Cheap (it reads a word of host memory); meaningful after the stream was synchronised."""
     from .build import _loaded
     for name in ("gemm_tc", "attention_prefill_tc", "routed_experts", "latent_prefill_tc", "latent_attention",
                  "sigmoid_attention_tc", "diff_attention_tc", "gated_recurrence", "prefix_attention"):
         if name in _loaded:
             code = getattr(_loaded[name], f"llmb_{name}_status")()
+            if name == "prefix_attention" and code == _BEYOND_BOUNDS:
+                raise KernelError("prefix_attention: a step brought more tokens than max_new or max_group said; its results are not valid")
             if code != 0:
                 raise KernelError(f"{name}: a bounded wait ran out (code {code}); the results of the "
                                   "last steps are not valid")
@@ -1450,6 +1452,7 @@ def attention_replay_key(step, n_heads: int, n_kv_heads: int, window: int = 0):
 # ----------------------------------------------------------------------------- sequences that share pages
 
 _prefix_entry = None
+_BEYOND_BOUNDS = 50             # its report of a step larger than its bounds (csrc/prefix_attention.cu)
 
 
 def _declare_prefix():
@@ -1511,7 +1514,8 @@ def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, g
     new tokens' keys and values. Returns [T, Hq * D] in qkv's dtype.
 
     max_new, max_group: most new tokens of a sequence, of a group; max_shared: most pages that a group shares; max_own: most
-    positions of a sequence behind those. Upper bounds, which size the launches."""
+    positions of a sequence behind those. Upper bounds, which size the launches. A step that brings more tokens than max_new or max_group
+    say is reported by `check_device_status`; its results are not valid."""
     if _prefix_entry is None:
         _declare_prefix()
     dtype, int32 = qkv.dtype, torch.int32

@@ -46,3 +46,19 @@ def test_groups_that_share_nothing_where_many_pages_are_allowed():
     behind_a_kernel_in_front(with_bounds(b, max_shared=8), 3)
     b = make([(0, members)], 32, 8, 128, BF16, seed=61, extra_width=40)
     behind_a_kernel_in_front(with_bounds(b, max_shared=32), 3)
+
+
+@pytest.mark.parametrize("members, new, bounds", [
+    ([30, 1, 3], 1, dict(max_new=1, max_group=3)),                     # own parts of more rows than their kernel holds
+    ([1] * 40, 1, dict(max_new=1, max_group=4)),                       # and groups, for each of the kernels that may be chosen
+    ([1] * 40, 1, dict(max_new=1, max_group=16)),
+    ([90] * 5, 90, dict(max_new=30, max_group=40)),
+])
+def test_a_step_beyond_its_bounds_is_reported(members, new, bounds):
+    from llm_b200.errors import KernelError
+    b = make([(9, [(17 * i % 100, n) for i, n in enumerate(members)])], 8, 2, 64, BF16, seed=62)
+    call(with_bounds(b, **bounds))
+    torch.cuda.synchronize()
+    with pytest.raises(KernelError, match="max_new"):
+        ops().check_device_status()
+    check(b, call(b))                                                  # and the next call is as it was
