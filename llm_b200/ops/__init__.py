@@ -1551,6 +1551,8 @@ def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, g
         _check_out(out, (n, n_heads * head_dim), dtype, "prefix_attention")
     if n == 0:
         return out
+    # no step goes beyond its tokens and its tables: wider bounds choose the same launches, and sizes stay within 32 bits
+    max_new, max_group, max_own = min(max_new, n), min(max_group, n), min(max_own, table_width * PAGE)
     shared, own = page_bucket(max_shared), page_bucket(-(-max_own // PAGE)) * PAGE
     at_q, at_k, at_v, at_out = qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
     tc = int(dtype is torch.bfloat16 and head_dim in (64, 128) and scale > 0 and q_stride % 8 == 0 and not (at_q | at_k | at_v | at_out) & 15

@@ -62,3 +62,11 @@ def test_a_step_beyond_its_bounds_is_reported(members, new, bounds):
     with pytest.raises(KernelError, match="max_new"):
         ops().check_device_status()
     check(b, call(b))                                                  # and the next call is as it was
+
+
+@pytest.mark.parametrize("wide", [2 ** 31 - 1, 2 ** 32 + 1, 2 ** 40])
+@pytest.mark.parametrize("new", [1, 30])
+def test_bounds_of_any_size(wide, new):
+    """Bounds are no sizes of anything: the widest serve."""
+    b = make([(3, [(17 * i % 100, new) for i in range(7)]), (0, [(150, new)])], 8, 2, 64, BF16, seed=63)
+    check(b, call(with_bounds(b, max_new=wide, max_group=wide, max_own=wide)))
