@@ -103,6 +103,10 @@ class DecoderModel:
             return None
         return (step.n_tokens, step.n_seqs, n_rows, tuple(keys), final)
 
+    def sharing_shapes(self) -> tuple:
+        """The distinct attentions that can read pages which sequences share once (Part.sharing_shapes)."""
+        return tuple(dict.fromkeys(shape for block in self.blocks for part in block.parts for shape in part.sharing_shapes()))
+
     def graph_safe(self) -> bool:
         return all(b.graph_safe for b in self.blocks) and self.final_norm.graph_safe
 

@@ -31,6 +31,7 @@ MAX_GRAPHS = 128           # captured shapes (batch size, bucket of pages) an en
 RECORD_AFTER_PASSES = 1    # plain passes of a shape before the next one is recorded
 MAX_RECORDS = 32           # recorded passes an engine keeps
 MAX_LAYOUTS = 4096         # shapes whose sections an engine knows
+MAX_SEEN = 4096            # shapes that an engine counts until they are captured or recorded
 MAX_RECORDED_LOGITS = 1 << 25   # a recorded pass holds its logits buffer: none for more values than this
 
 
@@ -124,6 +125,7 @@ class Engine:
                            and os.environ.get("LLMB_NO_GRAPHS", "0") in ("", "0")
                            and not ops.PROFILING
                            and getattr(model, "graph_safe", lambda: False)())
+        self.sharing_shapes = model.sharing_shapes()      # the attentions that can read shared pages once
         self._graphs, self._graph_seen, self._graph_pool = {}, {}, None
         self.graph_replays = 0            # decode steps run from a captured graph so far
         # passes that are not replayed from a graph (prompts, mixed steps, the first steps of a
@@ -228,14 +230,15 @@ class Engine:
                 self._layouts.clear()
             plan = self._layouts[shape] = (offsets, sizes, list(offsets), list(sizes), total.value)
         c_offsets, c_sizes, offsets, sizes, total = plan
-        host = self._host_buffer(total + (2 * self._group_room(batch.n) if self.cache.forked else 0))
+        may_share = self.cache.forked and bool(self.sharing_shapes)
+        host = self._host_buffer(total + (2 * self._group_room(batch.n) if may_share else 0))
         summary = (c_longlong * 5)()
         native.check(lib.llmh_step_pack(cache, *batch.arguments(), host.data_ptr(), host.numel(),
                                         c_offsets, c_sizes, summary))
         n_tokens, decode, max_len = summary[0], bool(summary[2]), summary[3]
         n_groups = len(offsets) - 8
         groups_at = total
-        sharing = self._groups(batch, host[total:]) if self.cache.forked else None
+        sharing = self._groups(batch, host[total:]) if may_share else None
         if sharing is not None:
             total += 2 * self._group_room(batch.n)
 
@@ -292,18 +295,26 @@ class Engine:
         return (n_seqs + 1 + 3) // 4 * 4
 
     def _groups(self, batch, room):
-        """Which of the batch's sequences share pages, written behind the step's sections: (groups, and the bounds of
-        SharedPages, numbers of pages as the launches know them: rounded up to a power of two), or None."""
+        """Which of the batch's sequences share pages, written behind the step's sections: (groups, and the bounds and shapes of
+        SharedPages), or None where no attention gains by reading them once. The tuple is part of what captured and recorded steps are kept under:
+        it holds what launches depend on and no more, numbers of pages (and of a group's tokens, in steps of single
+        tokens) rounded up to a power of two."""
         first, pages, summary = (c_int * (batch.n + 1))(), (c_int * batch.n)(), (c_int * 6)()
         native.check(native.lib().llmh_step_groups(self.cache._handle, batch.n, batch.slots, batch.counts, first, pages, summary))
         n_groups, max_new, max_group, max_shared, max_own, saved = summary
         if n_groups == 0:
             return None
+        shapes = tuple(s for s in self.sharing_shapes
+                       if ops.prefix_attention_pays(self.dtype, *s, batch.n, max_new, max_shared, saved))
+        if not shapes:
+            return None
         at = self._group_room(batch.n)
         room[:n_groups + 1] = torch.tensor(first[:n_groups + 1], dtype=torch.int32)
         room[at:at + n_groups] = torch.tensor(pages[:n_groups], dtype=torch.int32)
         widest = min(g.ring_pages for g in self.cache.groups if not g.window)
-        return (n_groups, max_new, max_group, min(ops.page_bucket(max_shared), widest), ops.page_bucket(-(-max_own // PAGE)) * PAGE, saved)
+        if max_new == 1:
+            max_group = min(ops.page_bucket(max_group), batch.n)
+        return (n_groups, max_new, max_group, min(ops.page_bucket(max_shared), widest), ops.page_bucket(-(-max_own // PAGE)) * PAGE, shapes)
 
     # ------------------------------------------------------------------ recorded passes
 
@@ -325,7 +336,7 @@ class Engine:
         if held is None:
             seen = self._record_seen.get(key, 0) + 1
             self._record_seen[key] = seen
-            if len(self._record_seen) > 4096:
+            if len(self._record_seen) > MAX_SEEN:
                 self._record_seen.clear()
             if seen <= RECORD_AFTER_PASSES:
                 return None
@@ -392,6 +403,8 @@ class Engine:
         graph = self._graphs.get(key)
         if graph is None:
             seen = self._graph_seen.get(key, 0) + 1
+            if len(self._graph_seen) >= MAX_SEEN:
+                self._graph_seen.clear()
             self._graph_seen[key] = seen
             if seen <= GRAPH_AFTER_STEPS:
                 return None

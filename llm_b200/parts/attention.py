@@ -45,6 +45,10 @@ class AttentionMixer(Mixer):
             out[t["o_bias"]] = ParamSpec((s.hidden,), "bias")
         return out
 
+    def sharing_shapes(self):
+        s = self.spec
+        return ((s.n_heads, s.n_kv_heads, s.head_dim),) if s.window == 0 else ()
+
     def bind(self, tensors, dtype, device):
         t = self.spec.tensor
         self.w_qkv = torch.cat([to_run_dtype(tensors[t[r]], dtype, device) for r in ("q", "k", "v")])
@@ -119,9 +123,8 @@ class AttentionMixer(Mixer):
                                  s.n_kv_heads, s.head_dim, interleaved=interleaved,
                                  write_cache=(entry == cache_entry))
         mixed = ctx.scratch("mixed", (n, self.q_width), h.dtype)
-        share = ctx.sharing if s.window == 0 else None
-        if share is not None and ops.prefix_attention_pays(h.dtype, s.n_heads, s.n_kv_heads, s.head_dim, ctx.n_seqs, share.max_new,
-                                                           share.max_shared, share.saved_pages):
+        share = ctx.sharing
+        if share is not None and s.window == 0 and (s.n_heads, s.n_kv_heads, s.head_dim) in share.shapes:
             mixed = ops.prefix_attention(qkv, keys, values, table, ctx.seq_lens, ctx.cu_seqlens, share.group_first, share.group_pages,
                                          s.n_heads, s.n_kv_heads, s.head_dim, s.scale, max_new=share.max_new, max_group=share.max_group,
                                          max_shared=share.max_shared, max_own=share.max_own, out=mixed)

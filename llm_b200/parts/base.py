@@ -33,7 +33,7 @@ class SharedPages:
     max_group: int                 # of a group
     max_shared: int                # most pages that a group shares
     max_own: int                   # most positions of a sequence behind them
-    saved_pages: int               # pages that are read once less for each further member of a group
+    shapes: tuple                  # (query heads, key heads, head size) of the attentions for which reading them once pays
 
 
 @dataclass
@@ -101,6 +101,10 @@ class Part:
         same launches with the same arguments, and the engine may run the second from the record
         of the first, walked by the native host library."""
         return None
+
+    def sharing_shapes(self) -> tuple:
+        """(query heads, key heads, head size) of this part's attentions that can read shared pages once (StepContext.sharing)."""
+        return ()
 
     def fold_input_norm(self, gain) -> bool:
         """Offered by the block after `bind`, where the norm in front of this part is an RMS norm

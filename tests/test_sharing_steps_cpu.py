@@ -1,0 +1,85 @@
+"""Which steps read shared pages once, and what captured steps are kept under, on the CPU."""
+import pytest
+import torch
+
+from tiny import make_folder
+
+from llm_b200.cache import PAGE
+from llm_b200.engine import Engine, Entry, load_model
+from llm_b200.engine import step as step_module
+
+
+@pytest.fixture
+def engine(tmp_path, plain_kernels):
+    return Engine(load_model(make_folder(tmp_path, "F", torch.float32), torch.float32, "cpu"), max_tokens=64 * PAGE, max_slots=16)
+
+
+def forked(engine, pages, members, behind=5):
+    """`members` sequences that share `pages` pages and hold `behind` positions each behind them (nothing is computed)."""
+    (slot,) = engine.acquire()
+    engine.cache.reserve(slot, pages * PAGE + behind)
+    engine.cache.set_length(slot, pages * PAGE + behind)
+    return [slot] + (engine.fork(slot, members - 1) if members > 1 else [])
+
+
+def sharing(engine, *groups, new=1):
+    """What the engine makes of a step over groups of (pages, members)."""
+    slots = [s for pages, members in groups for s in forked(engine, pages, members)]
+    batch = step_module._Batch([Entry(s, [1] * new, [0]) for s in slots])
+    room = torch.zeros(2 * engine._group_room(batch.n), dtype=torch.int32)
+    found = engine._groups(batch, room)
+    engine.release(slots)
+    return found
+
+
+def test_captured_steps_are_kept_under_what_launches_depend_on(engine):
+    """Not under the pages that are saved: other numbers of pages within the same bounds are the same step."""
+    first = sharing(engine, (5, 3))
+    assert first == sharing(engine, (6, 3)) == sharing(engine, (8, 3)) and first != sharing(engine, (9, 3))
+    assert sharing(engine, (5, 3), (2, 4)) == sharing(engine, (3, 3), (6, 4))
+    assert sharing(engine, (5, 3), (2, 3), (2, 2)) == sharing(engine, (5, 4), (2, 2), (2, 2))     # groups of four at most
+    # a prompt step's launches have a tile for every so many tokens of the largest group
+    assert sharing(engine, (5, 3), (2, 3), new=30) != sharing(engine, (5, 4), (2, 2), new=30)
+
+
+def test_the_rule_is_asked_once_for_every_kind_of_attention(engine, monkeypatch):
+    from llm_b200 import ops
+    asked = []
+    monkeypatch.setattr(ops, "prefix_attention_pays", lambda *a: asked.append(a) or a[1] > 1)
+    engine.sharing_shapes = ((4, 2, 64), (1, 1, 32), (8, 2, 64))
+    found = sharing(engine, (5, 3), (2, 2))
+    assert [a[1:4] for a in asked] == list(engine.sharing_shapes)
+    assert all(a[0] == torch.float32 and a[4:8] == (5, 1, 5, 2 * 5 + 2) for a in asked)
+    assert found[-1] == ((4, 2, 64), (8, 2, 64))
+
+
+def test_a_step_that_gains_nothing_is_an_ordinary_one(engine, monkeypatch):
+    """Nothing of the groups reaches the step, its buffer or its key."""
+    from llm_b200 import ops
+    seen, run = [], engine.model.forward
+
+    def forward(tokens, ctx, rows):
+        seen.append(ctx.sharing)
+        return run(tokens, ctx, rows)
+    monkeypatch.setattr(engine.model, "forward", forward)
+    slots = forked(engine, 1, 3)
+    engine.step([Entry(s, [3], [0]) for s in slots])
+    assert seen[0].shapes == engine.sharing_shapes
+    monkeypatch.setattr(ops, "prefix_attention_pays", lambda *a: False)
+    assert sharing(engine, (5, 3)) is None
+    engine.step([Entry(s, [3], [0]) for s in slots])
+    assert seen[1] is None
+
+
+def test_a_model_whose_attentions_read_for_themselves_asks_nothing(engine, monkeypatch):
+    engine.sharing_shapes = ()
+    monkeypatch.setattr(engine, "_groups", None)
+    slots = forked(engine, 1, 3)
+    engine.step([Entry(s, [3], [0]) for s in slots])
+    engine.cache.check()
+
+
+def test_what_is_counted_until_it_is_captured_is_bounded(engine):
+    for i in range(step_module.MAX_SEEN + 50):
+        assert engine._replay(i, 64, None, 0, None) is None
+    assert 0 < len(engine._graph_seen) <= step_module.MAX_SEEN

@@ -1,0 +1,40 @@
+"""Steps of forked sequences on the GPU by the engine's own rule: which of them read shared pages once, what is captured for them, and their logits."""
+import pytest
+import torch
+
+import plain_llama
+from test_model_gpu import close
+from tiny import make_folder, random_tokens
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def engine_for(folder, dtype, **options):
+    from llm_b200.engine import Engine, load_model
+    return Engine(load_model(folder, dtype, DEV), **{"max_tokens": 16384, **options})
+
+
+def test_another_number_of_shared_pages_replays_the_same_graph(tmp_path):
+    from llm_b200.engine import Entry
+    folder = make_folder(tmp_path, "F", F32)
+    config, weights = plain_llama.read_model_folder(folder)
+    engine = engine_for(folder, F32)
+    graphs = []
+    for pages in (5, 6, 7):
+        prompt = random_tokens(pages * 64 + 9, config["vocab_size"], pages)
+        (slot,) = engine.acquire()
+        engine.step([Entry(slot, prompt, [])])
+        slots, texts = [slot] + engine.fork(slot, 2), [prompt] * 3
+        for k in range(5):
+            new = [random_tokens(1, config["vocab_size"], 100 * pages + 10 * k + i) for i in range(3)]
+            texts = [t + n for t, n in zip(texts, new)]
+            logits = engine.step([Entry(s, n, [0]) for s, n in zip(slots, new)])
+        for row, text in zip(logits, texts):
+            assert close(row[None], plain_llama.forward(config, weights, text)[-1:], F32)
+        engine.release(slots)
+        graphs.append((len(engine._graphs), engine.graph_replays))
+    assert graphs == [(1, 3), (1, 8), (1, 13)]
+    engine.check()
