@@ -1,3 +1,4 @@
+#include "../prefix_plan.h"
 #include "cache.hpp"
 
 #include <algorithm>
@@ -154,12 +155,14 @@ using namespace llmh;
 
 // ------------------------------------------------------------------------------------ C boundary
 
-// The constants of plan.h for callers that cannot include it: 0 page, 1 gated block, 2 largest head size.
+// The constants of plan.h and prefix_plan.h for callers that cannot include them: 0 page, 1 gated block, 2 largest head size, 3 rows of a
+// sequence in prefix attention.
 LLMH_EXPORT int llmh_plan_constant(int which) {
     switch (which) {
         case 0: return LLMB_PAGE;
         case 1: return LLMB_GLU_BLOCK;
         case 2: return LLMB_MAX_HEAD_DIM;
+        case 3: return llmb_prefix::FEW_ROWS;
         default: return -1;
     }
 }

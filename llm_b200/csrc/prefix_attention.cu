@@ -17,17 +17,19 @@
 // weight whatever is stored there, and values beyond a tile's last position are taken for zero, so that what an earlier sequence
 // left in a page (infinities and NaN too) does not reach a result. A row that sees no key is zero.
 #include "mma.cuh"
+#include "prefix_plan.h"
 #include "tc.cuh"
 
 using namespace llmb;
 using namespace llmb::tc;
+using namespace llmb_prefix;
 
 LLMB_DEFINE_LAST_ERROR(llmb_prefix_attention)
 
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int MAX_SPLITS = 64, MAX_SLOTS = 2 * MAX_SPLITS;      // parts of the shared pages, of own ones; of a row
+constexpr int MAX_SLOTS = 2 * MAX_SPLITS;         // of a row: parts of the shared pages, of own ones
 
 struct Args {
     const void* q;
@@ -408,10 +410,10 @@ __global__ void __launch_bounds__(SIMT_THREADS) prefix_attention_simt_kernel(con
 // In both, weights are rounded to 8 bits, what the tensor cores take, and their sum is of the unrounded ones. The two are kernels of their own:
 // as branches of one, the own pages of a step took a third longer.
 
-constexpr int TC_ROWS = 128;                      // lanes of tensor memory
+constexpr int TC_ROWS = TILE_ROWS;                // lanes of tensor memory
 constexpr int KV_PIECE = LLMB_PAGE * 64 * 2;      // a page, 64 columns of the head: 8 KB
 constexpr int Q_PIECE = TC_ROWS * 64 * 2;         // 128 rows, 64 columns of the head: 16 KB
-constexpr int FEW_ROWS = 16, FEW_THREADS = 160, TILE_THREADS = 192;
+constexpr int FEW_THREADS = 160, TILE_THREADS = 192;
 constexpr int FEW_WARPS = 4;
 // tensor memory of an item: two buffers of scores (64 columns of 32-bit values, the weights over the first 32), O beside them
 constexpr uint32_t S_COL = 0, O_COL = 128, TMEM_COLS = 256;
@@ -1016,7 +1018,7 @@ prefix_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __
 // block has rows of. Only the rows of that sequence see those: the others' weights are zero, and the products leave their lanes of O
 // alone (a value that is not finite times a weight of zero would reach them).
 
-constexpr int WIDE_ROWS = 256, WIDE_THREADS = 384;           // warps 0 keys, 1 products, 2 values, 4-7 and 8-11 a tile's softmax
+constexpr int WIDE_THREADS = 384;           // warps 0 keys, 1 products, 2 values, 4-7 and 8-11 a tile's softmax
 constexpr int PAIR_PIECE = 128 * 128;                        // 128 positions, 64 columns of the head: 16 KB
 constexpr int WIDE_REGS_FEW = 104, WIDE_REGS_MANY = 200;      // 128 x 64 + 256 x 216 <= 384 x 168, what the block is launched with
 
@@ -1732,19 +1734,10 @@ struct Plan {
     long long part_rows;             // rows that are joined from parts
 };
 
-constexpr int SMS = 148;
-
 struct Sizes {
     int n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim, max_new, max_group, max_shared, max_own;
     bool tc;                         // the tensor-core kernels can take the call
 };
-
-// the least power of two that is no less than n: replayed steps of one bucket make the same launches
-int bucket(int n) {
-    int b = 1;
-    while (b < n) b *= 2;
-    return b;
-}
 
 // Which kernel, and into how many parts the shared and the own pages are cut: as many pages a block as make all blocks come to about the blocks
 // that the SMs hold at once, two pages at least.
@@ -1755,13 +1748,7 @@ Plan plan_for(const Sizes& z) {
     // sequences that bring few rows each would leave a tile of a group to walk many sequences' pages for a few of its rows
     p.whole = z.tc && (long long)z.max_new * share > FEW_ROWS;
     long long group_rows = shared > 0 ? (long long)z.max_group * share : 0;
-    // A few shared pages are read by every sequence itself: they come from L2, and a launch, its start and its parts are saved. One page always (three
-    // sequences of a small 32-bit model 14.5 us from the host for 22). Instead of the wide kernel up to 4,096 pages of a key head in all: heads of 128
-    // over 8, 64 sequences behind 2, 4 and 8 pages 12.3, 15.0, 20.3 us for 20.5, 22.5, 22.8; behind 16 pages 24 either way. Instead of the tile kernel up to
-    // 512, while no SM has two sequences: 8 behind 4, 8 and 16 pages 7.1, 7.7 and 12.7 for 9.3, 9.6 and 10.1; 32 behind 2 pages 12.7 for 11.2.
-    const long long walks = (long long)z.n_seqs * z.n_kv_heads;
-    p.alone = !p.whole && (shared == 1 || (z.tc && shared > 0 && group_rows > FEW_ROWS &&
-                                           (group_rows > TC_ROWS ? walks * shared <= 4096 : walks * shared <= 512 && walks <= SMS)));
+    p.alone = reads_alone((long long)z.n_seqs * z.n_kv_heads, shared, group_rows, z.tc, p.whole);
     if (p.alone) {
         own = bucket(own + shared);
         shared = 0;
@@ -1782,17 +1769,8 @@ Plan plan_for(const Sizes& z) {
     if (p.kernel == WIDE) {
         // whole rounds of tiles as they are, the tiles of the last round cut so that they fill one, into four pages at least
         p.full_tiles = p.whole ? (int)(prefix / SMS * SMS) : 0;
-        long long rest = prefix - p.full_tiles, best = 0;
-        p.prefix_splits = 1;
-        for (int n = 1; n <= MAX_SPLITS && (n == 1 || 4 * n <= walk) && rest > 0; ++n) {
-            // In pages' time (0.85 us): rounds of blocks times what one takes, its pages and about twelve for its start and its end, and the parts
-            // written and read again at some 5 TB/s.
-            long long time = (rest * n + SMS - 1) / SMS * (ceil_div(walk, n) + 12) + (n > 1 ? rest * n * WIDE_ROWS * z.head_dim * 8 / 4300000 : 0);
-            if (n == 1 || time < best) {
-                best = time;
-                p.prefix_splits = n;
-            }
-        }
+        const long long rest = prefix - p.full_tiles;
+        p.prefix_splits = wide_pieces(rest, walk, z.head_dim);
         wide_blocks = p.full_tiles + rest * p.prefix_splits;
         p.own_splits = p.own_tiles > 0 ? ceil_div(own, 32) : 0;      // own pages: a launch of their own, 32 pages a block at most
         if (even) {

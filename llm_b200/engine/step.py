@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import os
 from array import array
-from ctypes import byref, c_int, c_longlong
+from ctypes import byref, c_double, c_int, c_longlong
 from dataclasses import dataclass
 from itertools import chain
 
@@ -304,8 +304,16 @@ class Engine:
         n_groups, max_new, max_group, max_shared, max_own, saved = summary
         if n_groups == 0:
             return None
+
+        def times_of(shape):
+            def times():
+                apart, once = c_double(), c_double()
+                native.check(native.lib().llmh_step_attention_times(self.cache._handle, batch.n, batch.slots, batch.counts, n_groups, first, pages,
+                                                                    *shape, byref(apart), byref(once)))
+                return apart.value, once.value
+            return times
         shapes = tuple(s for s in self.sharing_shapes
-                       if ops.prefix_attention_pays(self.dtype, *s, batch.n, max_new, max_shared, saved))
+                       if ops.prefix_attention_pays(self.dtype, *s, batch.n, max_new, max_shared, saved, max_group, times_of(s)))
         if not shapes:
             return None
         at = self._group_room(batch.n)

@@ -22,7 +22,7 @@ OK, FORMAT, INVARIANT, CACHE_FULL, CONTEXT_FULL, IO = range(6)
 
 
 _P = c_void_p
-_INTS, _LONGS = POINTER(c_int), POINTER(c_longlong)
+_INTS, _LONGS, _DOUBLES = POINTER(c_int), POINTER(c_longlong), POINTER(c_double)
 _BATCH = [c_int, _INTS, _INTS, _INTS, _INTS, _INTS]      # n, slots, counts, tokens, want counts, wants
 
 # name: (result type, argument types); the declarations are in the .cpp files of csrc/host
@@ -58,6 +58,7 @@ _SIGNATURES = {
     "llmh_cache_plan_compact": (c_int, [_P, c_int, _INTS, _INTS, _INTS]),
     "llmh_cache_apply_moves": (c_int, [_P, c_int, c_int, _INTS, _INTS]),
     "llmh_step_groups": (c_int, [_P, c_int, _INTS, _INTS, _INTS, _INTS, _INTS]),
+    "llmh_step_attention_times": (c_int, [_P, c_int, _INTS, _INTS, c_int, _INTS, _INTS, c_int, c_int, c_int, _DOUBLES, _DOUBLES]),
     "llmh_prompt_runs": (c_int, [c_int, _INTS, _INTS, c_int, _INTS, _INTS, _INTS]),
     "llmh_step_check": (c_int, [_P, *_BATCH, c_int, c_int]),
     "llmh_step_reserve": (c_int, [_P, c_int, _INTS, _INTS]),
@@ -135,8 +136,8 @@ def ints(values, ctype=c_int):
 
 
 def plan_constant(name: str) -> int:
-    """A constant of csrc/plan.h, the one definition shared by kernels, host library and Python."""
-    return lib().llmh_plan_constant({"page": 0, "glu_block": 1, "max_head_dim": 2}[name])
+    """A constant of csrc/plan.h or prefix_plan.h, the one definition shared by kernels, host library and Python."""
+    return lib().llmh_plan_constant({"page": 0, "glu_block": 1, "max_head_dim": 2, "prefix_few_rows": 3}[name])
 
 
 def read_json(text, where: str = "text"):

@@ -1478,29 +1478,41 @@ def page_bucket(pages: int) -> int:
     return 1 << (pages - 1).bit_length() if pages > 0 else 0
 
 
-def prefix_attention_pays(dtype, n_heads, n_kv_heads, head_dim, n_seqs, max_new, max_shared, saved_pages) -> bool:
-    """Whether a step whose sequences share pages reads them once for each group (`prefix_attention`) or for each sequence
-    (`attention`); saved_pages: pages that are read once less for each further member of a group.
+_PREFIX_FEW_ROWS = native.plan_constant("prefix_few_rows")       # (csrc/prefix_plan.h)
 
-    In 32 bits always (two sequences behind one page 8 us for 33, eight behind 32 pages 19 for 361). In bfloat16 where
-    `attention` has a tensor-core kernel and this has none (32, 96) never, where neither has one always. Head sizes 64 and 128,
-    measured at 32 heads over 8 and over 32, with 2 to 64 sequences behind 1 to 128 pages; microseconds without and with:
+
+def prefix_attention_pays(dtype, n_heads, n_kv_heads, head_dim, n_seqs, max_new, max_shared, saved_pages, max_group=None, times=None) -> bool:
+    """Whether a step whose sequences share pages reads them once for each group (`prefix_attention`) or for each sequence
+    (`attention`); saved_pages: pages that are read once less for each further member of a group; times: for a step of several tokens, a function that estimates what the two take, apart and once.
+
+    In 32 bits always (one token a sequence 4 to 64 times as fast, 5 to 100 tokens 1.6 to 88 times, one pair beside 14 other prompts 4 to
+    18). In bfloat16 where `attention` has a tensor-core kernel and this has none (32, 96) never, where neither has one
+    always (80, 112, 256: 2 to 57 times). Head sizes 64 and 128, measured at 32 heads over 8 and over 32 (and over 1 and 2), with 2 to 80 sequences
+    behind 1 to 512 pages; microseconds without and with, from memory:
 
     * single tokens: reading a page again is cheap until the saved bytes outweigh the join, some 10 MB and 0.8 MB for every
       sequence. Heads of 128 over 8: 4 sequences behind 8 pages 6.1 / 7.4, 32 pages 10.9 / 9.0; 16 behind 4 pages 9.0 / 8.8, 16 pages
       16.7 / 11.1; 64 behind 2 pages 14.5 / 12.3, 4 pages 19 / 15, 8 pages 30 / 20, 128 pages 305 / 38; heads of 64: 8 behind 16 pages 6.7 / 9.2, 64
       behind 8 pages 17 / 15.
-    * several tokens: tiles of several sequences' rows fill up where query heads share a key head, so 32 pages pay (8 sequences
-      of 5 to 20 tokens 38 / 27, of 200 to 300 106 / 86; behind 8 pages 16 / 24 and 48 / 46); with a key head for each query head
-      128 pages do (8 sequences of 40 to 90 tokens 136 / 125, behind 32 pages 40 / 56)."""
+    * several tokens: 32 pages where query heads share a key head (2 questions of 17 to 93 tokens 29 / 21, 8 39 / 38; behind 8 pages 11.7 / 18.0 and
+      16.3 / 21.5), 128 with a key head for each (8 137 / 98; behind 32 pages 40 / 48). In steps of several groups tiles
+      are cut by their place, not by their length, so that a few questions among many prompts are one long chain: the estimates have
+      the last word. Two questions behind 32 pages with 6 and 62 prompts 30 / 46 and 70 / 81 (no), 4 groups of 4 questions 50 / 40, a prompt of 500
+      tokens beside 8 and 63 samples 42 / 50 (no) and 257 / 217."""
     if saved_pages <= 0 or tactics.is_disabled("prefix_attention"):
         return False
     if dtype is torch.float32:
         return True
     if head_dim not in (64, 128) or tactics.is_disabled("prefix_attention_tc"):
         return head_dim not in (32, 64, 96, 128)
+    share = n_heads // n_kv_heads
     if max_new > 1:
-        return max_shared >= (32 if n_heads > n_kv_heads else 128)
+        if max_shared < (32 if share > 1 else 128):
+            return False
+        if max_new * share <= _PREFIX_FEW_ROWS or times is None:
+            return True
+        apart, once = times()
+        return once <= apart
     return saved_pages * PAGE * n_kv_heads * head_dim * 4 >= 10e6 + 0.8e6 * n_seqs
 
 
