@@ -155,14 +155,15 @@ using namespace llmh;
 
 // ------------------------------------------------------------------------------------ C boundary
 
-// The constants of plan.h and prefix_plan.h for callers that cannot include them: 0 page, 1 gated block, 2 largest head size, 3 rows of a
-// sequence in prefix attention.
+// The constants of plan.h and prefix_plan.h for callers that cannot include them: 0 page, 1 gated block, 2 largest head size, 3 and 4 rows of a
+// sequence and of a group in prefix attention.
 LLMH_EXPORT int llmh_plan_constant(int which) {
     switch (which) {
         case 0: return LLMB_PAGE;
         case 1: return LLMB_GLU_BLOCK;
         case 2: return LLMB_MAX_HEAD_DIM;
         case 3: return llmb_prefix::FEW_ROWS;
+        case 4: return llmb_prefix::TILE_ROWS;
         default: return -1;
     }
 }

@@ -230,6 +230,11 @@ LLMH_EXPORT int llmh_step_groups(void* cache, int n, const int* slots, const int
     });
 }
 
+// Whether a step of single tokens in bfloat16 has every sequence read its shared pages itself (prefix_plan.h).
+LLMH_EXPORT int llmh_prefix_reads_alone(long long walks, int shared, long long group_rows) {
+    return llmb_prefix::reads_alone(walks, shared, group_rows, true, false) ? 1 : 0;
+}
+
 // About how many microseconds the attention of a prompt step in bfloat16 takes where every sequence reads its pages for itself (*apart: a block for 128
 // tokens and a query head, two on an SM) and where tiles of a group's rows read the shared ones once (*once: prefix_plan.h). A page takes a
 // block 0.77 apart and 0.57 of an SM's time where there are many; a tile of 256 rows 0.98, one of at most 128 rows 0.78, if its keys serve several

@@ -58,6 +58,7 @@ _SIGNATURES = {
     "llmh_cache_plan_compact": (c_int, [_P, c_int, _INTS, _INTS, _INTS]),
     "llmh_cache_apply_moves": (c_int, [_P, c_int, c_int, _INTS, _INTS]),
     "llmh_step_groups": (c_int, [_P, c_int, _INTS, _INTS, _INTS, _INTS, _INTS]),
+    "llmh_prefix_reads_alone": (c_int, [c_longlong, c_int, c_longlong]),
     "llmh_step_attention_times": (c_int, [_P, c_int, _INTS, _INTS, c_int, _INTS, _INTS, c_int, c_int, c_int, _DOUBLES, _DOUBLES]),
     "llmh_prompt_runs": (c_int, [c_int, _INTS, _INTS, c_int, _INTS, _INTS, _INTS]),
     "llmh_step_check": (c_int, [_P, *_BATCH, c_int, c_int]),
@@ -137,7 +138,7 @@ def ints(values, ctype=c_int):
 
 def plan_constant(name: str) -> int:
     """A constant of csrc/plan.h or prefix_plan.h, the one definition shared by kernels, host library and Python."""
-    return lib().llmh_plan_constant({"page": 0, "glu_block": 1, "max_head_dim": 2, "prefix_few_rows": 3}[name])
+    return lib().llmh_plan_constant({"page": 0, "glu_block": 1, "max_head_dim": 2, "prefix_few_rows": 3, "prefix_tile_rows": 4}[name])
 
 
 def read_json(text, where: str = "text"):

@@ -1479,41 +1479,54 @@ def page_bucket(pages: int) -> int:
 
 
 _PREFIX_FEW_ROWS = native.plan_constant("prefix_few_rows")       # (csrc/prefix_plan.h)
+_PREFIX_TILE_ROWS = native.plan_constant("prefix_tile_rows")
 
 
 def prefix_attention_pays(dtype, n_heads, n_kv_heads, head_dim, n_seqs, max_new, max_shared, saved_pages, max_group=None, times=None) -> bool:
     """Whether a step whose sequences share pages reads them once for each group (`prefix_attention`) or for each sequence
-    (`attention`); saved_pages: pages that are read once less for each further member of a group; times: for a step of several tokens, a function that estimates what the two take, apart and once.
+    (`attention`); saved_pages: pages that are read once less for each further member of a group; max_group: most new tokens of a
+    group (all if None); times: for a step of several tokens, a function that estimates what the two take, apart and once.
 
     In 32 bits always (one token a sequence 4 to 64 times as fast, 5 to 100 tokens 1.6 to 88 times, one pair beside 14 other prompts 4 to
     18). In bfloat16 where `attention` has a tensor-core kernel and this has none (32, 96) never, where neither has one
     always (80, 112, 256: 2 to 57 times). Head sizes 64 and 128, measured at 32 heads over 8 and over 32 (and over 1 and 2), with 2 to 80 sequences
     behind 1 to 512 pages; microseconds without and with, from memory:
 
-    * single tokens: reading a page again is cheap until the saved bytes outweigh the join, some 10 MB and 0.8 MB for every
-      sequence. Heads of 128 over 8: 4 sequences behind 8 pages 6.1 / 7.4, 32 pages 10.9 / 9.0; 16 behind 4 pages 9.0 / 8.8, 16 pages
-      16.7 / 11.1; 64 behind 2 pages 14.5 / 12.3, 4 pages 19 / 15, 8 pages 30 / 20, 128 pages 305 / 38; heads of 64: 8 behind 16 pages 6.7 / 9.2, 64
-      behind 8 pages 17 / 15.
+    * single tokens: reading a page again is cheap until the saved bytes outweigh launches and join: some 10 MB, 0.5 for every
+      sequence and 0.08 for every key head of one. Heads of 128 over 8: 4 sequences behind 8 pages 6.0 / 7.7, 32 pages 10.9 / 9.6; 16 behind 4
+      pages 8.8 / 9.2, 8 pages 11.6 / 10.7; 32 behind 4 pages 11.4 / 14.2, 8 pages 16.6 / 14.4; four groups of 16 behind up to 8 pages 21.5 / 24.3, 32 pages
+      62 / 29. A key head for each of 32: 16 behind 2 pages 13.3 / 15.7, 4 pages 17.9 / 15.8. Heads of 64: 32 behind 8 pages 9.1 / 11.1, 16 pages 14.9 / 12.3. Over
+      one key head: 16 behind 32 pages 18.4 / 22.9, 128 pages 53.7 / 24.7.
+      Where large groups read few pages in one launch without a join, a quarter of a MB for every sequence and 0.03 for every key head of
+      one: 64 behind 1, 2, 4, 8 pages 12.8 / 12.5, 14.5 / 13.4, 19.3 / 16.2, 29.4 / 21.7.
     * several tokens: 32 pages where query heads share a key head (2 questions of 17 to 93 tokens 29 / 21, 8 39 / 38; behind 8 pages 11.7 / 18.0 and
       16.3 / 21.5), 128 with a key head for each (8 137 / 98; behind 32 pages 40 / 48). In steps of several groups tiles
       are cut by their place, not by their length, so that a few questions among many prompts are one long chain: the estimates have
       the last word. Two questions behind 32 pages with 6 and 62 prompts 30 / 46 and 70 / 81 (no), 4 groups of 4 questions 50 / 40, a prompt of 500
-      tokens beside 8 and 63 samples 42 / 50 (no) and 257 / 217."""
+      tokens beside 8 and 63 samples 42 / 50 (no) and 257 / 217. A few tokens a sequence with a key head for each: as single ones
+      too (a pair of 16 tokens among 62 of one behind 128 pages 143 / 165, eight groups of 4 308 / 175)."""
     if saved_pages <= 0 or tactics.is_disabled("prefix_attention"):
         return False
     if dtype is torch.float32:
         return True
     if head_dim not in (64, 128) or tactics.is_disabled("prefix_attention_tc"):
         return head_dim not in (32, 64, 96, 128)
-    share = n_heads // n_kv_heads
+    share, walks = n_heads // n_kv_heads, n_seqs * n_kv_heads
+    group_rows = (n_seqs * max_new if max_group is None else max_group) * share
+    saved, enough = saved_pages * PAGE * n_kv_heads * head_dim * 4, 10e6 + 0.5e6 * n_seqs + 0.08e6 * walks
     if max_new > 1:
         if max_shared < (32 if share > 1 else 128):
             return False
-        if max_new * share <= _PREFIX_FEW_ROWS or times is None:
+        if max_new * share <= _PREFIX_FEW_ROWS:
+            return share > 1 or saved >= enough
+        if times is None:
             return True
         apart, once = times()
         return once <= apart
-    return saved_pages * PAGE * n_kv_heads * head_dim * 4 >= 10e6 + 0.8e6 * n_seqs
+    if max_new * share <= _PREFIX_FEW_ROWS and group_rows > _PREFIX_TILE_ROWS and \
+            native.lib().llmh_prefix_reads_alone(walks, page_bucket(max_shared), group_rows):
+        enough = 0.25e6 * n_seqs + 0.03e6 * walks
+    return saved >= enough
 
 
 def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, group_first, group_pages, n_heads, n_kv_heads, head_dim,

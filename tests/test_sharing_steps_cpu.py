@@ -85,6 +85,28 @@ def test_what_is_counted_until_it_is_captured_is_bounded(engine):
     assert 0 < len(engine._graph_seen) <= step_module.MAX_SEEN
 
 
+def pays(*a):
+    from llm_b200 import ops
+    return ops.prefix_attention_pays(torch.bfloat16, *a)
+
+
+def test_single_tokens_pay_where_reading_once_was_measured_faster():
+    """(query heads, key heads, head size, sequences, 1, shared pages, saved pages, tokens of the largest group) on both sides of each line."""
+    for heads, n, no, yes in [((32, 8, 128), 4, 8, 32), ((32, 8, 128), 16, 4, 8), ((32, 8, 128), 32, 4, 8), ((32, 32, 128), 16, 2, 4), ((32, 32, 128), 32, 2, 4),
+                              ((32, 8, 64), 32, 8, 16), ((32, 1, 128), 16, 32, 128), ((40, 2, 64), 64, 8, 32),
+                              ((32, 8, 128), 64, 1, 2), ((32, 8, 64), 64, 2, 8)]:            # these two are one launch
+        assert not pays(*heads, n, 1, no, (n - 1) * no, n), (heads, n, no)
+        assert pays(*heads, n, 1, yes, (n - 1) * yes, n), (heads, n, yes)
+    # four groups of 16 behind 2, 4, 6 and 8 pages 21.5 / 24.3 us, behind 8 to 32 62 / 29; a pair among many sequences
+    assert not pays(32, 8, 128, 64, 1, 8, 15 * 20, 16) and pays(32, 8, 128, 64, 1, 32, 15 * 80, 16)
+    assert not pays(32, 8, 128, 64, 1, 128, 128, 2)
+
+
+def test_few_tokens_a_sequence():
+    assert pays(32, 8, 128, 64, 4, 32, 32, 8, None) and not pays(32, 8, 128, 64, 4, 16, 16, 8, None)
+    assert not pays(32, 32, 128, 64, 16, 128, 128, 32, None) and pays(32, 32, 128, 32, 16, 128, 3 * 576, 64, None)
+
+
 @pytest.mark.parametrize("heads", [(32, 8, 128), (32, 8, 64)])
 def test_prompt_steps_of_several_groups_pay_where_their_tiles_fill_the_gpu(tmp_path, plain_kernels, heads):
     """A few questions behind a document among prompts that share nothing were slower read once (30 / 46, 101 / 148 us); several such groups were
