@@ -70,3 +70,59 @@ def test_bounds_of_any_size(wide, new):
     """Bounds are no sizes of anything: the widest serve."""
     b = make([(3, [(17 * i % 100, new) for i in range(7)]), (0, [(150, new)])], 8, 2, 64, BF16, seed=63)
     check(b, call(with_bounds(b, max_new=wide, max_group=wide, max_own=wide)))
+
+
+def even(n, low, high):
+    return [(low + (high - low) * (7 * i % n) // max(n - 1, 1), 1) for i in range(n)]
+
+
+REPLAYED = {                    # kernel: heads, groups of the captured step and of others of the same bounds, launches
+    "tile": ((8, 2, 64), [[(20, even(12, 0, 150))], [(31, even(12, 0, 30))], [(3, even(12, 60, 200))]], 3),
+    "tile, dealt out": ((8, 2, 64), [[(20, even(12, 0, 150)), (9, even(7, 3, 70)), (0, even(1, 9, 9))], [(5, even(4, 0, 90)), (31, even(14, 0, 128)), (2, even(2, 1, 64))],
+                                     [(0, even(15, 0, 150)), (30, even(1, 63, 63)), (7, even(4, 0, 20))]], 3),
+    "wide": ((32, 8, 128), [[(33, even(40, 0, 200))], [(20, even(40, 3, 900))], [(1, even(40, 0, 66))]], 3),
+    "wide, dealt out": ((32, 8, 128), [[(33, even(40, 0, 200)), (0, even(2, 5, 80)), (9, even(6, 0, 130))], [(4, even(10, 0, 128)), (40, even(37, 0, 64)), (0, even(1, 700, 700))],
+                                       [(0, even(40, 0, 100)), (0, even(2, 0, 3)), (0, even(6, 1, 300))]], 3),
+    "few": ((8, 2, 64), [[(20, even(4, 0, 150))], [(31, even(4, 0, 30))]], 2),
+    "on the cuda cores": ((8, 2, 48), [[(20, even(4, 0, 150)), (3, even(9, 0, 90))], [(31, even(12, 0, 30)), (0, even(1, 70, 70))]], 2),
+}
+
+
+@pytest.mark.parametrize("which", REPLAYED)
+def test_each_kernel_replays_on_other_lengths_and_groups(which):
+    """The bounds of a captured call hold for all its replays and are loose for each: unequal groups, groups that share nothing, short and long own parts."""
+    (heads, kv_heads, dim), steps, launches = REPLAYED[which]
+    made = [make(groups, heads, kv_heads, dim, BF16, seed=70 + i) for i, groups in enumerate(steps)]
+    n_pages, width = max(b["keys"].shape[0] for b in made), max(b["table"].shape[1] for b in made)
+    n = made[0]["cu"][-1]
+    held = dict(made[0], q=made[0]["q"].clone(), arrays=tuple(t.clone() for t in made[0]["arrays"]),
+                table=torch.zeros((n, width), dtype=torch.int32, device=DEV),
+                keys=torch.zeros((n_pages, kv_heads, 64, dim), dtype=BF16, device=DEV), values=torch.zeros((n_pages, kv_heads, 64, dim), dtype=BF16, device=DEV),
+                bounds={k: max(b["bounds"][k] for b in made) for k in made[0]["bounds"]})
+
+    def load(b):
+        held["keys"][:b["keys"].shape[0]] = b["keys"]
+        held["values"][:b["values"].shape[0]] = b["values"]
+        held["table"].zero_()
+        held["table"][:, :b["table"].shape[1]] = b["table"]
+        held["q"].copy_(b["q"])
+        for to, t in zip(held["arrays"], b["arrays"]):
+            to.copy_(t)
+    load(made[0])
+    before = ops().launch_count()
+    call(held)
+    assert ops().launch_count() - before == launches
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(held)
+    for b in made + made[:1]:
+        load(b)
+        graph.replay()
+        check(b, out)
+
+
+@pytest.mark.parametrize("groups", [[(33, even(40, 0, 300))], [(33, even(40, 0, 300)), (5, even(4, 0, 100))], [(20, even(12, 0, 150))], [(20, even(3, 0, 150))]])
+def test_shared_and_own_parts_behind_a_kernel_in_front(groups):
+    b = make(groups, 32, 8, 128, BF16, seed=64)
+    behind_a_kernel_in_front(b, 2 if len(groups[0][1]) == 3 else 3)
