@@ -111,23 +111,25 @@ def _start(engine, reqs, batch, prompts, slots):
         slots += engine.acquire(len(reqs))
         return engine.step([Entry(slot, r.prompt, [len(r.prompt) - 1]) for slot, r in zip(slots, reqs)])
     alone = [b for b, i in enumerate(batch) if b == 0 or not prompts.twin[i]]
+    runs = []                                            # of prompts that begin alike
+    for b in alone:
+        if runs and prompts.run[batch[b]] == prompts.run[batch[runs[-1][0]]]:
+            runs[-1].append(b)
+        else:
+            runs.append([b])
+    firsts = engine.acquire(len(runs))
+    slots += firsts
+    common = [prompts.common[batch[members[0]]] if len(members) > 1 else 0 for members in runs]
+    begun = [Entry(first, reqs[members[0]].prompt[:n], []) for first, members, n in zip(firsts, runs, common) if n]
+    if begun:
+        engine.step(begun)
     slot_of, done = {}, {}
-    at = 0
-    while at < len(alone):                               # runs of prompts that begin alike
-        end = at + 1
-        while end < len(alone) and prompts.run[batch[alone[end]]] == prompts.run[batch[alone[at]]]:
-            end += 1
-        common = prompts.common[batch[alone[at]]] if end - at > 1 else 0
-        (first,) = engine.acquire()
-        slots.append(first)
-        members = [first]
-        if common:
-            engine.step([Entry(first, reqs[alone[at]].prompt[:common], [])])
-            members += engine.fork(first, end - at - 1)
-            slots += members[1:]
-        for b, slot in zip(alone[at:end], members):
-            slot_of[b], done[b] = slot, common
-        at = end
+    for first, members, n in zip(firsts, runs, common):
+        forks = engine.fork(first, len(members) - 1) if n else []
+        slots += forks
+        # (a run of several prompts has a page in common at least)
+        slot_of.update(zip(members, [first] + forks))
+        done.update((b, n) for b in members)
     logits = engine.step([Entry(slot_of[b], reqs[b].prompt[done[b]:], [len(reqs[b].prompt) - done[b] - 1]) for b in alone])
     rows = []
     for k, b in enumerate(alone):                        # equal prompts: the rest of them

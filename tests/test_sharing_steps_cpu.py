@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tiny import make_folder
+from tiny import make_folder, random_tokens
 
 from llm_b200.cache import PAGE, KvRequest, PagedCache
 from llm_b200.engine import Engine, Entry, load_model
@@ -134,3 +134,20 @@ def test_prompt_steps_of_several_groups_pay_where_their_tiles_fill_the_gpu(tmp_p
         assert taken(*[(pages * (g + 1) // 16, [17, 54]) for g in range(16)])
         assert taken((pages, [50] * 64), *[(0, [30 + i]) for i in range(16)])
     assert not taken((0, [500]), (32, [1] * 8)) and taken((0, [500]), (32, [1] * 63))
+
+
+def test_what_runs_of_prompts_begin_with_is_prefilled_in_one_step(engine, monkeypatch):
+    """Two documents with their questions, a prompt alone and a repeated one: what is common once, in one step, then all the rest in another."""
+    from llm_b200.engine import GenerationRequest, generate
+    from llm_b200.sampling import SamplingParams
+    one, two = [random_tokens(n, engine.vocab, 5 + n) for n in (130, 200)]
+    prompts = [one + [3], one + [4, 5], [9, 8, 7], two + [1], two + [2], two + [2], two[:150] + [6]]
+    requests = [GenerationRequest(p, max_tokens=4, params=SamplingParams(temperature=0.8, seed=i)) for i, p in enumerate(prompts)]
+    apart = generate(engine, requests)
+    steps, step = [], engine.step
+    monkeypatch.setattr(engine, "step", lambda entries, *a, **k: steps.append([len(e.tokens) for e in entries]) or step(entries, *a, **k))
+    together = generate(engine, requests, share_prefix=True)
+    assert [r.tokens for r in together] == [r.tokens for r in apart]
+    assert steps[0] == [128, 128] and steps[1] == [3, 4, 3, 73, 73, 23]
+    assert engine.cache.slots.n_held == 0
+    engine.cache.check()
