@@ -58,6 +58,15 @@ def main(argv=None) -> int:
     return complete(args)
 
 
+def _held_by_samples(model, prompt_tokens: int, max_tokens: int, context: int, samples: int) -> int:
+    """Positions that the cache has to hold for `samples` continuations of one prompt: the prompt's full pages once, what each writes
+    for itself. The rings of windowed attentions are each sample's own, from the first position on."""
+    from .cache import PAGE, round_up
+    final = round_up(min(prompt_tokens + max(max_tokens, 0), context, model.spec.max_positions))
+    shared = 0 if any(r is not None and r.window for r in model.cache_requests()[0]) else min(prompt_tokens, final) // PAGE * PAGE
+    return shared + samples * (final - shared)
+
+
 def complete(args) -> int:
     model, context, max_tokens, temperature, dtype = None, DEFAULT_CONTEXT, DEFAULT_MAX_TOKENS, 0.7, "bfloat16"
     seed, prompt, samples = None, [], 1
@@ -85,9 +94,13 @@ def complete(args) -> int:
     if samples < 1:
         raise SystemExit("--samples needs a number of at least 1")
     import llm_b200
-    llm = llm_b200.LLM(model, dtype=dtype, context=context, batch=samples)
     options = {} if seed is None else {"seed": seed}
     if samples > 1:
+        from .api import parse_dtype
+        from .engine import load_model
+        bound = load_model(model, parse_dtype(dtype), "cuda:0")
+        llm = llm_b200.LLM(bound, context=context, batch=samples,
+                           max_tokens_held=_held_by_samples(bound, len(prompt), max_tokens, context, samples))
         (results,) = llm.generate([prompt], max_tokens=max_tokens, temperature=temperature, details=True, samples=samples, **options)
         for result in results:
             print(" ".join(map(str, result.tokens)))
@@ -95,6 +108,7 @@ def complete(args) -> int:
         print(f"[{results[0].prompt_tokens} prompt tokens, {drawn} generated in {samples} samples, ttft {results[0].ttft_ms:.0f} ms, "
               f"{sum(r.tokens_per_second for r in results):.1f} tok/s]", file=sys.stderr)
         return 0
+    llm = llm_b200.LLM(model, dtype=dtype, context=context, batch=1)
     (result,) = llm.generate([prompt], max_tokens=max_tokens, temperature=temperature, details=True,
                              on_token=lambda i, t: print(t, end=" ", flush=True), **options)
     print()

@@ -151,3 +151,23 @@ def test_what_runs_of_prompts_begin_with_is_prefilled_in_one_step(engine, monkey
     assert steps[0] == [128, 128] and steps[1] == [3, 4, 3, 73, 73, 23]
     assert engine.cache.slots.n_held == 0
     engine.cache.check()
+
+
+def test_the_command_line_holds_a_prompt_once(tmp_path, plain_kernels, monkeypatch):
+    """Whole contexts for every sample are more than a GPU has for a long prompt: what is asked for holds all samples at once, and no page more."""
+    import sys
+    import llm_b200
+    from llm_b200.cli import _held_by_samples
+    model = load_model(make_folder(tmp_path, "F", torch.float32), torch.float32, "cpu")
+    held = _held_by_samples(model, 200, 8, 2048, 5)
+    assert held == (3 + 5) * PAGE and _held_by_samples(model, 200, 100000, 2048, 5) == (3 + 5 * 29) * PAGE
+    assert _held_by_samples(model, 192, 0, 2048, 5) == 3 * PAGE
+    assert _held_by_samples(model, 200, 100000, 1 << 20, 5) == (3 + 5 * 29) * PAGE                    # the model's own limit
+    batches, module = [], sys.modules["llm_b200.engine.generate"]
+    run = module._run_batch
+    monkeypatch.setattr(module, "_run_batch", lambda engine, requests, batch, *rest: batches.append(len(batch)) or run(engine, requests, batch, *rest))
+    llm = llm_b200.LLM(model, context=2048, batch=5, max_tokens_held=held)
+    results = llm.generate([random_tokens(200, 5000, 3)], samples=5, max_tokens=8, stop_tokens=())
+    assert batches == [5] and [len(r) for r in results[0]] == [8] * 5
+    model.cache_requests = lambda: ([KvRequest(1, 2, window=70)], [None])
+    assert _held_by_samples(model, 200, 8, 2048, 5) == 5 * 4 * PAGE
