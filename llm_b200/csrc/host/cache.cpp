@@ -112,8 +112,8 @@ long long Cache::held_tokens() const {
     return total;
 }
 
-// No slot or page lost or held by more slots than it counts; a page that several slots hold is a full one of a `full` group, at the
-// same place in all of them; the table mirrors the lists.
+// No slot or page lost or held by more slots than it counts; a page that several slots hold is one of a `full` group, at the same place in all of
+// them; the table mirrors the lists. (A slot may have been set back onto a page that it shares: it cannot write there, require_writable.)
 void Cache::check() const {
     slots.check();
     for (const Group& group : groups) {

@@ -13,9 +13,10 @@
 // share = heads / kv_heads, so that one pass over a key head serves all query heads that share it.
 //
 // Everything that changes from step to step (lengths, tables, groups) is read from device arrays; the sizes of the launch are upper
-// bounds (most tokens of a group, most pages) and a block beyond the real work leaves. A key beyond a row's position has no
-// weight whatever is stored there, and values beyond a tile's last position are taken for zero, so that what an earlier sequence
-// left in a page (infinities and NaN too) does not reach a result. A row that sees no key is zero.
+// bounds (most tokens of a group, most pages) and a block beyond the real work leaves; a step of more tokens than its bounds say is
+// reported. A key beyond a row's position has no weight whatever is stored there, and values beyond the last position of a sequence's own pages are
+// taken for zero, so that what an earlier sequence left in a page (infinities and NaN too) does not reach a result. Shared pages are full: every
+// member of the group holds all their positions, and nothing in them is left over. A row that sees no key is zero.
 #include "mma.cuh"
 #include "prefix_plan.h"
 #include "tc.cuh"
@@ -1020,7 +1021,9 @@ prefix_attention_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __
 
 constexpr int WIDE_THREADS = 384;           // warps 0 keys, 1 products, 2 values, 4-7 and 8-11 a tile's softmax
 constexpr int PAIR_PIECE = 128 * 128;                        // 128 positions, 64 columns of the head: 16 KB
-constexpr int WIDE_REGS_FEW = 104, WIDE_REGS_MANY = 200;      // 128 x 64 + 256 x 216 <= 384 x 168, what the block is launched with
+// of the warps that issue and of the softmax's (64 and 216 spilled in the loop that issues)
+constexpr int WIDE_REGS_FEW = 104, WIDE_REGS_MANY = 200, WIDE_REGS_LAUNCHED = 168;
+static_assert(128 * WIDE_REGS_FEW + 256 * WIDE_REGS_MANY <= WIDE_THREADS * WIDE_REGS_LAUNCHED, "the shares come from what the block is launched with");
 
 // The pages of an item, one after the other: the shared ones, then those of each sequence in turn.
 struct Walk {
@@ -1835,6 +1838,9 @@ int launch_tc(const Args& a, const Plan& p, int n_pages, cudaStream_t stream) {
         LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tiles));
         LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_tile_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tiles));
         LLMB_CUDA(cudaFuncSetAttribute(prefix_attention_wide_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wide));
+        cudaFuncAttributes built;                // (its softmax warps would wait for registers that are not there)
+        LLMB_CUDA(cudaFuncGetAttributes(&built, prefix_attention_wide_kernel<HD>));
+        LLMB_REQUIRE(built.numRegs >= WIDE_REGS_LAUNCHED, "prefix_attention: built with %d registers a thread", built.numRegs);
         configured = true;
     }
     CUtensorMap map_k, map_v;
@@ -1894,17 +1900,12 @@ LLMB_EXPORT int llmb_prefix_attention_status() {
     return v;
 }
 
-// Whether the tensor-core kernels take these operands (rows and caches on 16-byte boundaries, a positive scale).
-LLMB_EXPORT int llmb_prefix_attention_tc_serves(int dtype, int head_dim, int aligned, float scale) {
-    return dtype == LLMB_DTYPE_BF16 && (head_dim == 64 || head_dim == 128) && aligned && scale > 0.f ? 1 : 0;
-}
-
 // The sizes of a call, one integer each.
 struct llmb_prefix_sizes {
     int q_stride, n_pages, table_stride, out_stride;         // elements between rows, pages of the caches
     int dtype, n_tokens, n_seqs, n_groups, n_heads, n_kv_heads, head_dim;
     int max_new, max_group, max_shared, max_own;             // upper bounds (ops.prefix_attention)
-    int tc;                                                  // what llmb_prefix_attention_tc_serves said, 0 to keep to the CUDA cores
+    int tc;                                                  // whether the tensor-core kernels take the call (refused where they cannot), 0: the CUDA cores
 };
 
 namespace {
@@ -1937,8 +1938,8 @@ LLMB_EXPORT int llmb_prefix_attention(const void* q, const void* k_cache, const 
     LLMB_REQUIRE(z.max_new > 0 && z.max_group >= z.max_new && z.max_shared >= 0 && z.max_own >= 0, "prefix_attention: bad sizes");
     LLMB_REQUIRE((long long)z.n_tokens * z.n_heads < (1ll << 31), "prefix_attention: %d tokens of %d heads", z.n_tokens, z.n_heads);
     auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-    LLMB_REQUIRE(!z.tc || llmb_prefix_attention_tc_serves(z.dtype, z.head_dim, aligned(q) && z.q_stride % 8 == 0 && aligned(out) && z.out_stride % 8 == 0 &&
-                                                          aligned(k_cache) && aligned(v_cache), scale),
+    LLMB_REQUIRE(!z.tc || (z.dtype == LLMB_DTYPE_BF16 && (z.head_dim == 64 || z.head_dim == 128) && scale > 0.f && z.q_stride % 8 == 0 && z.out_stride % 8 == 0 &&
+                           aligned(q) && aligned(out) && aligned(k_cache) && aligned(v_cache)),
                  "prefix_attention: the tensor-core kernels do not take these operands");
     LLMB_REQUIRE(z.n_pages > 0 && (long long)z.n_pages * z.n_kv_heads * LLMB_PAGE < (1ll << 31), "prefix_attention: %d pages", z.n_pages);
     Plan p = plan_for(sizes_of(z));

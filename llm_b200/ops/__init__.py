@@ -1533,7 +1533,8 @@ def prefix_attention(qkv, k_cache, v_cache, block_table, seq_lens, cu_seqlens, g
                      scale, *, max_new, max_group, max_shared, max_own, out=None):
     """Causal grouped-query attention, as `attention` without its options, for a batch whose sequences share pages: the
     sequences group_first[g] .. group_first[g + 1] - 1 have the same pages in the first group_pages[g] places of their rows of
-    `block_table`, and those keys and values are read once for all of them (by each, where they are few pages). `group_first` (int32 [G + 1], from 0 to the
+    `block_table`, and those keys and values are read once for all of them (by each, where they are few pages). These pages are full: each of
+    the sequences holds all their positions. `group_first` (int32 [G + 1], from 0 to the
     number of sequences) and `group_pages` (int32 [G]) are on the device, as `seq_lens` [B] (with the new tokens) and
     `cu_seqlens` [B + 1] are; a sequence that shares nothing is a group of its own with 0 pages. The cache already holds the
     new tokens' keys and values. Returns [T, Hq * D] in qkv's dtype.
