@@ -5,7 +5,7 @@
 namespace llmb_prefix {
 
 constexpr int SMS = 148;
-constexpr int FEW_ROWS = 16;         // rows of a sequence (new tokens times the query heads of a key head) from which on a group's tiles walk own pages too
+constexpr int FEW_ROWS = 16;         // rows of a sequence (new tokens times the query heads of a key head) above which a group's tiles walk own pages too
 constexpr int TILE_ROWS = 128;       // of a group, up to which two blocks share an SM
 constexpr int WIDE_ROWS = 256;       // of a tile of larger groups
 constexpr int MAX_SPLITS = 64;       // pieces of a tile
