@@ -16,6 +16,7 @@ import collections
 import ctypes
 import functools
 import itertools
+import math
 import os
 import sys
 
@@ -1110,9 +1111,12 @@ def check_device_status() -> None:
     bounds (prefix_attention). Cheap (it reads a word of host memory); meaningful after the stream was synchronised."""
     from .build import _loaded
     for name in ("gemm_tc", "attention_prefill_tc", "routed_experts", "latent_prefill_tc", "latent_attention",
-                 "sigmoid_attention_tc", "diff_attention_tc", "gated_recurrence", "prefix_attention"):
+                 "sigmoid_attention_tc", "diff_attention_tc", "gated_recurrence", "prefix_attention", "attention_int8", "int8_cache"):
         if name in _loaded:
             code = getattr(_loaded[name], f"llmb_{name}_status")()
+            if name in ("attention_int8", "int8_cache") and code in (_BEYOND_BOUNDS, _OUT_OF_RANGE):
+                said = "more tokens than max_new said" if code == _BEYOND_BOUNDS else "a position, sequence, token or page that there is not"
+                raise KernelError(f"{name}: a step brought {said}; its results are not valid")
             if name == "prefix_attention" and code == _BEYOND_BOUNDS:
                 raise KernelError("prefix_attention: a step brought more tokens than max_new or max_group said; its results are not valid")
             if code != 0:
@@ -1452,6 +1456,7 @@ def attention_replay_key(step, n_heads: int, n_kv_heads: int, window: int = 0):
 # ----------------------------------------------------------------------------- sequences that share pages
 
 _prefix_entry = None
+_OUT_OF_RANGE = 51              # what the kernels of a cache in 8 bits report of a place that there is not (csrc/attention_int8.cu, int8_cache.cu)
 _BEYOND_BOUNDS = 50             # its report of a step larger than its bounds (csrc/prefix_attention.cu)
 
 
@@ -1652,6 +1657,150 @@ def copy_slots(states, source, target) -> None:
             size = state.numel() // state.shape[0] * state.element_size()
             shapes.append((state.data_ptr(), 1, 1, 0, size, 0, size))
     _copy_items(shapes, states[0].shape[0] if states else 0, source, target, None, "copy_slots")
+
+
+# ----------------------------------------------------------------------------- a cache held in 8 bits
+
+class Int8Pages:
+    """Keys or values of a paged cache held in 8 bits: `values`, whole numbers (int8) [pages, Hkv, 64, D], and `scales`, float32 [pages,
+    Hkv, 64 / block], a power of two for each block of `block` positions (1, 2, 4 .. 64) of a head. values * scales is what is held. Both are
+    contiguous; a scale that is no number says that the block took in a value that is not finite."""
+    __slots__ = ("values", "scales", "block")
+
+    def __init__(self, values, scales):
+        if values.dim() != 4 or values.shape[2] != PAGE or values.dtype is not torch.int8 or not values.is_contiguous():
+            raise KernelError(f"Int8Pages: values must be contiguous int8 [pages, kv heads, {PAGE}, dim], not {tuple(values.shape)} {values.dtype}")
+        if (scales.dim() != 3 or scales.shape[:2] != values.shape[:2] or scales.shape[2] not in (1, 2, 4, 8, 16, 32, 64)
+                or scales.dtype is not torch.float32 or not scales.is_contiguous() or scales.device != values.device):
+            raise KernelError(f"Int8Pages: scales must be contiguous float32 [{values.shape[0]}, {values.shape[1]}, {PAGE} / block] beside the values")
+        if values.data_ptr() % 16:
+            raise KernelError("Int8Pages: values must start on 16 bytes")
+        self.values, self.scales, self.block = values, scales, PAGE // scales.shape[2]
+
+    def held(self, dtype=torch.bfloat16):
+        """What the pages stand for, [pages, Hkv, 64, D] (exact in bfloat16 and float32)."""
+        return (self.values.view(*self.scales.shape, -1) * self.scales[..., None]).to(dtype).view(self.values.shape)
+
+
+def _check_int8(keys, values, n_kv_heads, head_dim, what: str) -> None:
+    if not isinstance(keys, Int8Pages) or not isinstance(values, Int8Pages):
+        raise KernelError(f"{what}: keys and values are Int8Pages")
+    shape = keys.values.shape
+    if shape[1] != n_kv_heads or shape[3] != head_dim or values.values.shape != shape or values.block != keys.block:
+        raise KernelError(f"{what}: keys {tuple(shape)} in blocks of {keys.block} and values {tuple(values.values.shape)} in blocks of {values.block} "
+                          f"are no pages of {n_kv_heads} heads of {head_dim}, both alike")
+
+
+def _check_step(what: str, block_table, ring_pages, n_seqs, *vectors) -> None:
+    int32 = torch.int32
+    for t, count, name in vectors:
+        if t.dtype is not int32 or t.dim() != 1 or t.numel() != count or not t.is_contiguous():
+            raise KernelError(f"{what}: {name} must be contiguous int32 [{count}]")
+    if block_table.dtype is not int32 or block_table.dim() != 2 or block_table.shape[0] != n_seqs or block_table.stride(1) != 1:
+        raise KernelError(f"{what}: the page table must be int32 [{n_seqs}, pages]")
+    if not 1 <= ring_pages <= block_table.shape[1]:
+        raise KernelError(f"{what}: a ring of {ring_pages} pages in a table of {block_table.shape[1]}")
+
+
+def _on_current_device(what: str, *tensors) -> None:
+    """All tensors are on the current CUDA device: launches go to its current stream."""
+    _require_cuda(*tensors)
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != device:
+            raise KernelError(f"{what}: a tensor on {t.device}, while the current device is cuda:{device}")
+
+
+def rope_cache_write_int8(qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_table, ring_pages, keys, values, n_heads, n_kv_heads, head_dim,
+                          interleaved=False, write_cache=True, out=None):
+    """`rope_cache_write` for a cache held in 8 bits (`keys` and `values`: Int8Pages): the rotated queries of the fused
+    [T, (Hq + 2 Hkv) D] projection are the result ([T, Hq * D], qkv itself is left as it is), its keys, rotated, and its values are appended
+    to their sequences' pages. The tokens of sequence i are rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1, at consecutive
+    positions tok_pos; `block_table` [B, pages].
+
+    A block of positions has the smallest power of two for a scale with which its largest value is at most 127 steps. One that the
+    step continues keeps its scale where that is enough; where it grows, what the block holds is divided by the growth and rounded again. What
+    lies in a block behind the sequence's last position has no say. A value that is not finite makes its block's scale no number until the block is
+    begun anew; attention over it is then none either. No two sequences of a call may write to one page. A position, sequence or page that there is not
+    is left out and reported by `check_device_status`."""
+    what = "rope_cache_write_int8"
+    n, n_seqs = qkv.shape[0], cu_seqlens.numel() - 1
+    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or not qkv.is_contiguous():
+        raise KernelError(f"{what}: qkv {tuple(qkv.shape)} is not contiguous [T, ({n_heads} + 2 * {n_kv_heads}) * {head_dim}]")
+    code = _code(qkv.dtype)
+    _check_int8(keys, values, n_kv_heads, head_dim, what)
+    _check_step(what, block_table, ring_pages, n_seqs, (tok_pos, n, "tok_pos"), (tok_seq, n, "tok_seq"), (cu_seqlens, n_seqs + 1, "cu_seqlens"))
+    n_rot = n_positions = 0
+    if rope_table is not None:
+        if rope_table.dim() != 2 or rope_table.dtype is not torch.float32 or not rope_table.is_contiguous() or rope_table.shape[1] > head_dim \
+                or rope_table.shape[1] % 2:
+            raise KernelError(f"{what}: the table of angles must be contiguous float32 [positions, n_rot] with an even n_rot <= {head_dim}")
+        n_positions, n_rot = rope_table.shape
+    _on_current_device(what, qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_table, keys.values, keys.scales, values.values, values.scales, out)
+    _check_out(out, (n, n_heads * head_dim), qkv.dtype, what)
+    if out is None:
+        out = qkv.new_empty((n, n_heads * head_dim))
+    _call("int8_cache", "llmb_int8_append", _ptr(qkv), _c_int(code), _ptr(rope_table), _ptr(tok_pos), _ptr(tok_seq), _ptr(cu_seqlens),
+          _ptr(block_table), _c_int(block_table.stride(0)), _c_int(ring_pages), _ptr(out), _ptr(keys.values), _ptr(keys.scales), _ptr(values.values),
+          _ptr(values.scales), _c_int(n), _c_int(n_seqs), _c_int(keys.values.shape[0]), _c_int(n_heads), _c_int(n_kv_heads), _c_int(head_dim),
+          _c_int(n_rot), _c_int(n_positions), _c_int(1 if interleaved else 0), _c_int(keys.block), _c_int(1 if write_cache else 0), _stream())
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _int8_plan(*sizes) -> tuple:
+    """(the sizes of a call as the library takes them, floats of scratch, launches)."""
+    lib, kernels, packed = load_library("attention_int8"), ctypes.c_int(0), (_c_int * len(sizes))(*sizes)
+    lib.llmb_attention_int8_scratch_floats.restype = ctypes.c_longlong
+    lib.llmb_attention_int8.argtypes = [_c_void] * 11 + [ctypes.c_longlong, _c_float, _c_void, _c_void]
+    floats = lib.llmb_attention_int8_scratch_floats(packed, ctypes.byref(kernels))
+    return packed, ctypes.addressof(packed), floats, kernels.value
+
+
+def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seqlens, n_heads, n_kv_heads, head_dim, scale, window=0, *, max_new,
+                   max_len, out=None, seq_order=None):
+    """Causal grouped-query attention, as `attention` without its other options, over a cache held in 8 bits (`keys` and `values`:
+    Int8Pages), which already holds the new tokens' keys and values: the queries are the first Hq * D columns of `qkv`, sequence i has the rows
+    cu_seqlens[i] .. cu_seqlens[i + 1] - 1 and seq_lens[i] positions with them. `window` > 0: a query sees its own position and the window - 1
+    before it. Returns [T, Hq * D] in qkv's dtype.
+
+    max_new, max_len: most new tokens and most positions of a sequence, upper bounds that size the launches (a sequence longer than max_len is
+    served all the same). A step that brings more tokens than max_new says, and a page or token that there is not, are
+    reported by `check_device_status`; its results are not valid. `seq_order` (int32 [B]): the sequences by falling length, which start
+    in that order."""
+    what = "attention_int8"
+    if qkv.dim() != 2:
+        raise KernelError(f"{what}: queries must be rows")
+    (n, width), (q_stride, inner) = qkv.shape, qkv.stride()
+    if inner != 1 or width < n_heads * head_dim or n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads:
+        raise KernelError(f"{what}: queries must be rows of at least {n_heads} * {head_dim} contiguous values, for {n_kv_heads} key heads")
+    dtype, n_seqs = qkv.dtype, seq_lens.numel()
+    code = _code(dtype)
+    _check_int8(keys, values, n_kv_heads, head_dim, what)
+    _check_step(what, block_table, ring_pages, n_seqs, (seq_lens, n_seqs, "seq_lens"), (cu_seqlens, n_seqs + 1, "cu_seqlens"),
+                *(() if seq_order is None else ((seq_order, n_seqs, "seq_order"),)))
+    if max_new < 1 or max_len < 1 or window < 0 or not math.isfinite(scale):
+        raise KernelError(f"{what}: max_new {max_new}, max_len {max_len}, window {window}, scale {scale}")
+    _on_current_device(what, qkv, keys.values, keys.scales, values.values, values.scales, block_table, seq_lens, cu_seqlens, seq_order, out)
+    if out is None:
+        out = qkv.new_empty((n, n_heads * head_dim))
+    else:
+        _check_out(out, (n, n_heads * head_dim), dtype, what)
+    if n == 0:
+        return out
+    # no step goes beyond its tokens and its table; lengths count in powers of two of pages, so that a captured step serves the next lengths
+    max_new, max_len = min(max_new, n), page_bucket(-(-min(max_len, 1 << 30) // PAGE)) * PAGE
+    tc = 0
+    packed, at_sizes, floats, kernels = _int8_plan(q_stride, n_heads * head_dim, block_table.stride(0), ring_pages, keys.values.shape[0], code, n, n_seqs,
+                                                   n_heads, n_kv_heads, head_dim, keys.block, window, max_new, max_len, tc)
+    parts = _scratch(qkv.device, "attention", floats)[0] if floats else None
+    if _recording is not None:
+        _recording.keep += [qkv, keys, values, block_table, seq_lens, cu_seqlens, seq_order, out, parts, packed]
+    _call("attention_int8", "llmb_attention_int8", qkv.data_ptr(), keys.values.data_ptr(), keys.scales.data_ptr(), values.values.data_ptr(),
+          values.scales.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), cu_seqlens.data_ptr(),
+          None if seq_order is None else seq_order.data_ptr(), out.data_ptr(), parts.data_ptr() if floats else None, floats, float(scale), at_sizes,
+          _stream(), kernels=kernels)
+    return out
 
 
 # ----------------------------------------------------------------------------- latent attention, shared rotated keys
@@ -2107,7 +2256,7 @@ def required_libraries() -> list:
             "attention_decode", "attention_prefill", "attention_prefill_tc", "sampling"]
 
 
-__all__ = ["PAGE", "GLU_BLOCK", "glu_fusable", "embed", "scale_", "random_normal_", "begin_recording", "end_recording", "RecordedPass", "StepScope", "scratch_generation", "Emit", "FoldedNorm", "RopeWrite", "cast_sumsq", "SUMSQ_LD", "rmsnorm", "swiglu", "rope_cache_write", "linear", "attention", "prefix_attention", "prefix_attention_pays", "page_bucket", "copy_pages", "copy_slots",
+__all__ = ["PAGE", "GLU_BLOCK", "glu_fusable", "embed", "scale_", "random_normal_", "begin_recording", "end_recording", "RecordedPass", "StepScope", "scratch_generation", "Emit", "FoldedNorm", "RopeWrite", "cast_sumsq", "SUMSQ_LD", "rmsnorm", "swiglu", "rope_cache_write", "linear", "attention", "prefix_attention", "prefix_attention_pays", "page_bucket", "Int8Pages", "rope_cache_write_int8", "attention_int8", "copy_pages", "copy_slots",
            "softcap_", "add_rows_", "conv_rope_cache_write", "diff_attention", "tanh_norm", "norm_rope_cache_write",
            "sigmoid_attention", "gated_recurrence", "state_space", "attention_replay_key", "layernorm", "input_conv", "output_norm_add_", "forget_recurrence",
            "latent_write", "head_products", "latent_attention", "latent_prefill", "attention_decode_splits", "sigmoid_attention_replay_key", "sigmoid_decode_splits", "sigmoid_mixed_heads", "sigmoid_mixed_elements",
