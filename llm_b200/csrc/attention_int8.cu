@@ -42,11 +42,13 @@ struct Args {
     int q_stride, out_stride, table_stride, ring_pages, n_pages, n_tokens, n_seqs, n_heads, n_kv_heads, head_dim, block_shift, window;
     float scale_log2;
     int max_new, tiles, slots;
+    int few_tokens;                  // sequences that bring at most so many tokens are the kernel's for few rows (0: it is not launched)
+    int deal_blocks, deal_least;     // its blocks that all pages are dealt out to, in ranges of so many pages at least; 0: a block a (sequence, key head)
 };
 
 // What a kernel reports (no wait has these codes): a step that brings more tokens than max_new says; a place outside of what the call was given, which is
-// not read: a page, a token or a sequence that there is not.
-constexpr int BEYOND_BOUNDS = 50, OUT_OF_RANGE = 51;
+// not read: a page, a token or a sequence that there is not; a scale of what is seen that is no power of two.
+constexpr int BEYOND_BOUNDS = 50, OUT_OF_RANGE = 51, NOT_A_POWER = 52;
 __device__ __forceinline__ void report(int* status, int code) {
     if (status) atomicCAS(status, 0, code);
 }
@@ -214,6 +216,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_int8_simt_kernel(const
 #pragma unroll
         for (int c = 0; c < COLS * W; ++c) o[i][c] = 0;
     const bool idle = ty * RT >= w.n_rows;                     // a warp without rows
+    const int last = position_of(w, w.n_rows - 1, share), low = first_seen(a, position_of(w, 0, share));      // what a row of the tile sees at all
     if (w.page_begin < w.page_end) fetch(a.keys, page_at(a, pages, w.page_begin, status));
     for (int logical = w.page_begin; logical < w.page_end; ++logical) {
         const int key0 = logical * LLMB_PAGE, page = page_at(a, pages, logical, status);
@@ -243,7 +246,10 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_int8_simt_kernel(const
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int b = (tx + 32 * j) >> a.block_shift;
-                bad[j] = is_number(k_scales[b]) && is_number(v_scales[b]) ? 0.f : __uint_as_float(0x7fffffffu);
+                const float sk = k_scales[b], sv = v_scales[b];
+                bad[j] = is_number(sk) && is_number(sv) ? 0.f : __uint_as_float(0x7fffffffu);
+                if (bad[j] == 0.f && key0 + tx + 32 * j <= last && ((__float_as_uint(sk) | __float_as_uint(sv)) & 0x807fffffu) &&
+                    key0 + tx + 32 * j >= low) report(status, NOT_A_POWER);
             }
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
@@ -321,6 +327,628 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_int8_simt_kernel(const
                 for (int x = 0; x < W; ++x)
                     if ((c * 32 + tx) * W + x < D) a.acc[slot * D + (c * 32 + tx) * W + x] = half_of(o[i / 2][c * W + x], i & 1);
             if (tx == 0) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(l[i] != 0.f ? m[i] : -INFINITY, l[i]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ bfloat16, up to 16 rows
+//
+// What a decode step brings. Reading the cache is the work, and widening it: 16 bits would be twice the bytes, so the whole numbers stay what they are
+// until they are in registers. A byte b (two's complement) is exactly the fp16 number 1024 + 128 + b with the bits 0x6400 | (b ^ 0x80), one
+// logical operation for two of them; a multiply-add by (s, -1152 s) leaves b s, exact for s a power of two. Products are mma.sync with the cache's
+// positions (for the scores) or the head's columns (for the result) on the 16-row side and the queries' rows, 8 or 16, on the other: what is
+// widened is multiplied once.
+//
+//   scores^T [16 positions, rows] = K [16, D] Q^T        result^T [16 columns, rows] += V^T [16, positions] P^T
+//
+// fp16 holds 2^-24 to 65504. So queries are divided by the power of two that brings their row's largest to 2^14; scales count from the largest of the 32
+// positions that a warp works on (2^5 for that one, so that 29 powers of two fit); and a row keeps, beside the running maximum m of its scores, a
+// reference R of score plus exponent of the values' scale, to which its weights w = 2^(score - m) 2^(m + E - R + 14) and its sums refer: weights and
+// values that span more than fp16 does are lost only where they are nothing beside what the row has. All sums are in 32 bits.
+//
+// The pages of all (sequence, key head) pairs, one after the other, are dealt out to the blocks that the SMs hold at once in ranges of
+// equal length, so a block's range covers the end of one pair, some whole ones, and the beginning of another. Pairs that one block has done as a whole are
+// finished there, of the others each block leaves a part. A block has four warps, each with a ring of units of 32 positions of its own (TMA, rows
+// swizzled so that both the reads of keys, four lanes a row, and those of values, eight columns a lane, touch all banks once), which runs on over the
+// ends of pairs; warps meet where a pair ends.
+
+constexpr int FEW_THREADS = 128, FEW_WARPS = 4, UNIT = 32;      // UNIT: positions that a warp works on at a time
+constexpr int FEW_ROWS = 16;
+constexpr int SCALE_UP = 5, WEIGHT_UP = 14;                    // powers of two that the largest scale and weight are lifted to
+
+template <int HD, int NT> struct Few {
+    static constexpr int TILE = UNIT * HD;                      // bytes of a unit's keys
+    static constexpr int STAGES = HD == 64 ? 4 : 2;
+    static constexpr int BLOCKS = NT == 1 ? 3 : 2;              // of an SM
+    static constexpr int LD = HD + 4;
+    static constexpr int RING = FEW_WARPS * STAGES * 2 * TILE;
+    static constexpr int MERGE = 2 * (8 * NT * LD + 8 * NT * 4) * 4;            // two warps' rows, and their references
+    static constexpr int SCALES = FEW_WARPS * STAGES * 2 * UNIT * 4;
+    static constexpr int BYTES = RING + MERGE + SCALES + FEW_WARPS * STAGES * 8 + 16;
+    static_assert(BLOCKS * (BYTES + 1024) <= 227 * 1024, "blocks of an SM");
+};
+
+// the physical row of a tile of 8 that stands for index g of the products: see the banks above
+template <int HD> __device__ __forceinline__ int row_of(int g) {
+    if (HD == 128) return g ^ ((g & 1) << 2);
+    const int t = g >> 1, even = (t & 1) | ((t >> 1) << 2);
+    return g & 1 ? even ^ 3 : even;
+}
+template <int HD> __device__ __forceinline__ int byte_of(int row, int chunk) {
+    return HD == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+constexpr uint32_t BYTES_TO_F16 = 0x64806480u, MINUS_1152 = 0xe480e480u;
+// bytes 0 and 2 (1 and 3) of x as two fp16 numbers, times s (with off = -1152 s)
+__device__ __forceinline__ uint32_t even_bytes(uint32_t x, uint32_t s, uint32_t off) { return hfma2((x & 0x00ff00ffu) ^ BYTES_TO_F16, s, off); }
+__device__ __forceinline__ uint32_t odd_bytes(uint32_t x, uint32_t s, uint32_t off) { return hfma2(((x >> 8) & 0x00ff00ffu) ^ BYTES_TO_F16, s, off); }
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+    return d;
+}
+__device__ __forceinline__ void cp_async4(void* smem, const void* global) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_u32(smem)), "l"(global));
+}
+// 2^n as an fp16 number's bits, 0 below what it holds
+__device__ __forceinline__ uint32_t f16_power(int n) { return n >= -14 ? (uint32_t)(n + 15) << 10 : n >= -24 ? 1u << (n + 24) : 0u; }
+// 2^(a - b) for references that may be -inf (of nothing)
+__device__ __forceinline__ float ratio(float a, float b) { return a == -INFINITY ? 0.f : fast_exp2(a - b); }
+
+// The pages of a sequence that its rows see: places first .. first + pages - 1 of its table. 0 pages where it brings nothing, and (many) where it
+// brings more rows than `most`.
+struct Span {
+    int first, pages, first_token, n_new, first_pos;
+};
+__device__ __forceinline__ Span span_of(const Args& a, int seq, int most_tokens) {
+    Span s;
+    s.first_token = a.cu_seqlens[seq];
+    const int end = a.cu_seqlens[seq + 1];
+    s.n_new = end - s.first_token;
+    s.first_pos = a.seq_lens[seq] - s.n_new;
+    const bool fits = s.n_new > 0 && s.n_new <= most_tokens && s.first_token >= 0 && end <= a.n_tokens && s.first_pos >= 0;
+    s.first = a.window > 0 ? max(s.first_pos - a.window + 1, 0) / LLMB_PAGE : 0;
+    s.pages = fits ? (s.first_pos + s.n_new - 1) / LLMB_PAGE + 1 - s.first : 0;
+    return s;
+}
+// A (sequence, key head) pair and where its pages stand among all.
+struct Pair {
+    int seq, head;
+    long long start;
+    Span span;
+};
+// What does not fit is reported: places that there are not, more tokens than max_new says (where no other kernel takes those).
+__device__ __forceinline__ void check_span(const Args& a, const Span& s, int* status) {
+    if (s.n_new <= 0) return;
+    if (s.first_token < 0 || s.first_token + s.n_new > a.n_tokens || s.first_pos < 0) report(status, OUT_OF_RANGE);
+    else if (s.n_new > a.max_new) report(status, BEYOND_BOUNDS);
+}
+// The pages of all pairs, by every lane of a warp.
+__device__ __forceinline__ long long all_pages(const Args& a, int most_tokens, int lane) {
+    long long sum = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32)
+        sum += __reduce_add_sync(0xffffffffu, s0 + lane < a.n_seqs ? (unsigned)span_of(a, s0 + lane, most_tokens).pages : 0u);
+    return sum * a.n_kv_heads;
+}
+// The pair that page `at` of all belongs to.
+__device__ __forceinline__ Pair pair_at(const Args& a, long long at, int most_tokens, int lane) {
+    long long before = 0;
+    Pair p;
+    for (int s0 = 0;; s0 += 32) {
+        const int mine = s0 + lane < a.n_seqs ? span_of(a, s0 + lane, most_tokens).pages : 0;
+        unsigned up = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            unsigned left = __shfl_up_sync(0xffffffffu, up, d);
+            if (lane >= d) up += left;
+        }
+        const unsigned beyond = __ballot_sync(0xffffffffu, at < before + (long long)up * a.n_kv_heads);
+        if (beyond) {
+            const int k = __ffs(beyond) - 1;
+            p.seq = s0 + k;
+            p.span = span_of(a, p.seq, most_tokens);
+            p.start = before + (long long)(__shfl_sync(0xffffffffu, up, k) - p.span.pages) * a.n_kv_heads;
+            p.head = (int)((at - p.start) / p.span.pages);
+            p.start += (long long)p.head * p.span.pages;
+            return p;
+        }
+        before += (long long)__shfl_sync(0xffffffffu, up, 31) * a.n_kv_heads;
+    }
+}
+// the pair behind it (there is one)
+__device__ __forceinline__ void next_pair(const Args& a, Pair& p, int most_tokens) {
+    p.start += p.span.pages;
+    if (++p.head < a.n_kv_heads) return;
+    p.head = 0;
+    do p.span = span_of(a, ++p.seq, most_tokens); while (p.span.pages == 0 && p.seq + 1 < a.n_seqs);
+}
+// pages of a block's range: all in equal ranges, two pages at least
+__device__ __forceinline__ long long range_pages(const Args& a, long long all) {
+    const long long per = (all + a.deal_blocks - 1) / a.deal_blocks;
+    return per < a.deal_least ? a.deal_least : per;
+}
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(FEW_THREADS, Few<HD, NT>::BLOCKS)
+attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a, int* status) {
+    using F = Few<HD, NT>;
+    constexpr int TILE = F::TILE, STAGES = F::STAGES, LD = F::LD, DIMS = HD / 8, CHUNKS = HD / 64;     // DIMS: a lane's columns of the result
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* base = smem_raw;                            // (its alignment is the swizzle's)
+    const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    unsigned char* ring = base + warp * STAGES * 2 * TILE;
+    float* merge = reinterpret_cast<float*>(base + F::RING);                     // [2] a warp's rows [8 NT][LD], then (m, R, l, -) of each
+    float* scales = reinterpret_cast<float*>(base + F::RING + F::MERGE) + warp * STAGES * 2 * UNIT;         // of this warp: [stage][2][32]
+    uint64_t* full = reinterpret_cast<uint64_t*>(base + F::RING + F::MERGE + F::SCALES) + warp * STAGES;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(base + F::RING + F::MERGE + F::SCALES + FEW_WARPS * STAGES * 8);
+
+    griddep_launch();
+    if (lane == 0) {
+        for (int i = 0; i < STAGES; ++i) mbar_init(smem_u32(&full[i]), 1);
+        if (warp == 0) *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    griddep_wait();
+    __syncthreads();
+    const int share = a.n_heads / a.n_kv_heads, most_tokens = a.few_tokens;
+    Pair pair;
+    long long r0, r1;                                          // the block's range of all pages
+    if (a.deal_blocks == 0) {                                  // a pair a block
+        const int at = blockIdx.x / a.n_kv_heads;
+        pair.seq = a.seq_order ? a.seq_order[at] : at;
+        pair.head = blockIdx.x % a.n_kv_heads;
+        pair.start = r0 = 0;
+        if ((unsigned)pair.seq >= (unsigned)a.n_seqs) {
+            if (threadIdx.x == 0) report(status, OUT_OF_RANGE);
+            return;
+        }
+        pair.span = span_of(a, pair.seq, most_tokens);
+        r1 = pair.span.pages;
+        if (r1 == 0) {
+            if (threadIdx.x == 0) check_span(a, pair.span, status);
+            return;
+        }
+    } else {
+        const long long all = all_pages(a, most_tokens, lane), per = range_pages(a, all);
+        if (blockIdx.x == 0)
+            for (int s = threadIdx.x; s < a.n_seqs; s += FEW_THREADS) {
+                check_span(a, span_of(a, s, most_tokens), status);
+                if (a.seq_order && (unsigned)a.seq_order[s] >= (unsigned)a.n_seqs) report(status, OUT_OF_RANGE);
+            }
+        r0 = blockIdx.x * per;
+        r1 = r0 + per < all ? r0 + per : all;
+        if (r0 >= r1) return;
+        pair = pair_at(a, r0, most_tokens, lane);
+    }
+    const int units = (int)(r1 - r0) * (LLMB_PAGE / UNIT);
+    const __nv_bfloat16* q_all = behind_wait(static_cast<const __nv_bfloat16*>(a.q));
+    const int scales_per_page = LLMB_PAGE >> a.block_shift;
+
+    // What is asked for: unit `asked` of the range, of pair `ahead`; its page's number is on its way.
+    Pair ahead = pair;
+    int asked = warp, page_ahead = 0;
+    auto look_up = [&]() {
+        if (asked >= units) return;
+        const long long at = r0 + asked / (LLMB_PAGE / UNIT);
+        while (at >= ahead.start + ahead.span.pages) next_pair(a, ahead, most_tokens);
+        page_ahead = page_at(a, a.block_table + (size_t)ahead.seq * a.table_stride, ahead.span.first + (int)(at - ahead.start), status);
+    };
+    auto ask = [&](int stage) {
+        if (asked < units) {
+            const int head_row = page_ahead * a.n_kv_heads + ahead.head, row = asked % (LLMB_PAGE / UNIT) * UNIT;
+            const size_t at = (size_t)head_row * scales_per_page + ((row + lane) >> a.block_shift);
+            cp_async4(scales + stage * 2 * UNIT + lane, a.key_scales + at);
+            cp_async4(scales + stage * 2 * UNIT + UNIT + lane, a.value_scales + at);
+            if (elect_one()) {
+                const uint32_t bar = smem_u32(&full[stage]), to = smem_u32(ring + stage * 2 * TILE);
+                mbar_expect_tx(bar, 2 * TILE);
+                tma_load_2d(to, &map_k, bar, 0, head_row * LLMB_PAGE + row);
+                tma_load_2d(to + TILE, &map_v, bar, 0, head_row * LLMB_PAGE + row);
+            }
+            __syncwarp();
+            asked += FEW_WARPS;
+            look_up();
+        }
+        cp_async_commit();
+    };
+    look_up();
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) ask(i);
+
+    int done = warp, stage = 0;                                // the next unit, and where it arrives
+    uint32_t phase = 0;
+    bool ok = true;
+    for (;;) {
+        // ---- the pair's rows
+        const Span& span = pair.span;
+        const int n_rows = span.n_new * share;
+        const long long pair_end = pair.start + span.pages, end = pair_end < r1 ? pair_end : r1;
+        const int limit = span.first_pos + span.n_new - 1, low = first_seen(a, span.first_pos);       // positions that a row sees at all
+        uint32_t qb[NT][HD / 16][2];
+        float row_scale[NT][2];                                // of rows 2t and 2t + 1 of each tile
+        int pos[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = n * 8 + g;
+            const bool valid = r < n_rows;
+            const __nv_bfloat16* q = q_all + (size_t)(span.first_token + (valid ? r : 0) / share) * a.q_stride +
+                                     (size_t)(pair.head * share + (valid ? r : 0) % share) * HD + 16 * t;
+            uint4 raw[CHUNKS][2];
+            uint32_t most = 0;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    raw[c][i] = valid ? *reinterpret_cast<const uint4*>(q + 64 * c + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+                    const uint32_t x[4] = {raw[c][i].x, raw[c][i].y, raw[c][i].z, raw[c][i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) most = max(most, max(x[k] & 0x7fffu, (x[k] >> 16) & 0x7fffu));
+                }
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int exponent = max((int)(most >> 7), 27) - 127;                         // (rows below 2^-100 are as good as zero)
+            const float factor = __uint_as_float((uint32_t)(14 - exponent + 127) << 23);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint4& v = raw[c][w >> 1];
+                    const uint32_t x01 = w & 1 ? v.z : v.x, x23 = w & 1 ? v.w : v.y;       // columns 4w .. 4w + 3: two values each
+                    const float x0 = __uint_as_float(x01 << 16) * factor, x1 = __uint_as_float(x01 & 0xffff0000u) * factor;
+                    const float x2 = __uint_as_float(x23 << 16) * factor, x3 = __uint_as_float(x23 & 0xffff0000u) * factor;
+                    qb[n][c * 4 + w][0] = pack_f16(x0, x2);
+                    qb[n][c * 4 + w][1] = pack_f16(x1, x3);
+                }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int of = n * 8 + 2 * t + j, e = __shfl_sync(0xffffffffu, exponent, (2 * t + j) * 4);
+                row_scale[n][j] = a.scale_log2 * __uint_as_float((uint32_t)(max(e - 14 + 127, 1)) << 23);
+                pos[n][j] = of < n_rows ? span.first_pos + of / share : -1;
+            }
+        }
+        float acc[NT][DIMS / 2][4], m[NT][2], ref[NT][2], sum[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < DIMS / 2; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[n][i][k] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                m[n][j] = ref[n][j] = -INFINITY;
+                sum[n][j] = 0.f;
+            }
+        }
+        // ---- its units
+        for (; done < units; done += FEW_WARPS) {
+            const long long at = r0 + done / (LLMB_PAGE / UNIT);
+            if (at >= end) break;
+            const int key0 = (span.first + (int)(at - pair.start)) * LLMB_PAGE + done % (LLMB_PAGE / UNIT) * UNIT;
+            ok = ok && mbar_wait_warp(smem_u32(&full[stage]), phase, abort_flag, status, 21);
+            cp_async_wait<STAGES - 1>();
+            __syncwarp();
+            if (ok && key0 <= limit && key0 + UNIT > low) {
+                const unsigned char* k_tile = ring + stage * 2 * TILE;
+                const unsigned char* v_tile = k_tile + TILE;
+                // the unit's scales, a lane a position: the largest of those that are seen, then all as fp16 powers from it. (Blocks of 16 positions and
+                // more have one for all 16 of a tile, and it counts where any of these is seen.)
+                const int alike = a.block_shift >= 4 ? 15 : 0, nearest = key0 + (lane & ~alike);
+                const bool seen = nearest <= limit && nearest + alike >= low;
+                uint32_t ks = seen ? __float_as_uint(scales[stage * 2 * UNIT + lane]) : 0u, vs = seen ? __float_as_uint(scales[stage * 2 * UNIT + UNIT + lane]) : 0u;
+                const bool none = (ks & 0x7fffffffu) >= NOT_FINITE || (vs & 0x7fffffffu) >= NOT_FINITE;
+                if (!none && seen && ((ks | vs) & 0x807fffffu)) report(status, NOT_A_POWER);
+                const unsigned bad = __ballot_sync(0xffffffffu, none);
+                if (none) ks = vs = 0u;
+                const int ke = __reduce_max_sync(0xffffffffu, ks >> 23), ve = __reduce_max_sync(0xffffffffu, vs >> 23);
+                // (each lane's over its key's: fp16 scales, key's low, value's high)
+                uint32_t* packed = reinterpret_cast<uint32_t*>(scales + stage * 2 * UNIT);
+                packed[lane] = (ks ? f16_power((int)(ks >> 23) - ke + SCALE_UP) : 0u) | ((vs ? f16_power((int)(vs >> 23) - ve + SCALE_UP) : 0u) << 16);
+                __syncwarp();
+
+                float s[2][NT][4];
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) s[tile][n][k] = 0.f;
+                    uint32_t sa, sb;                           // of positions row_of(g) and 8 behind it
+                    const int row = tile * 16 + row_of<HD>(g);
+                    sa = packed[row];
+                    sb = a.block_shift >= 4 ? sa : packed[row + 8];
+                    sa = __byte_perm(sa, 0, 0x1010);
+                    sb = __byte_perm(sb, 0, 0x1010);
+                    const uint32_t oa = hmul2(sa, MINUS_1152), ob = hmul2(sb, MINUS_1152);
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; ++c) {
+                        const uint4 xa = *reinterpret_cast<const uint4*>(k_tile + byte_of<HD>(row, 4 * c + t));
+                        const uint4 xb = *reinterpret_cast<const uint4*>(k_tile + byte_of<HD>(row + 8, 4 * c + t));
+                        const uint32_t wa[4] = {xa.x, xa.y, xa.z, xa.w}, wb[4] = {xb.x, xb.y, xb.z, xb.w};
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t a0 = even_bytes(wa[w], sa, oa), a2 = odd_bytes(wa[w], sa, oa);
+                            const uint32_t a1 = even_bytes(wb[w], sb, ob), a3 = odd_bytes(wb[w], sb, ob);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_f16(s[tile][n], a0, a1, a2, a3, qb[n][c * 4 + w][0], qb[n][c * 4 + w][1]);
+                        }
+                    }
+                }
+                const float k_unit = __uint_as_float((uint32_t)max(ke - SCALE_UP, 1) << 23);                  // what a step of the keys stands for
+                const float v_unit = (float)(ve - 127);
+                uint32_t pb[2][NT][2];                         // the weights, positions on the contracted side
+                bool moved = false;
+                float shrink[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float weight[2][4];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float c = row_scale[n][j] * k_unit;
+                        float x[4] = {s[0][n][j] * c, s[0][n][2 + j] * c, s[1][n][j] * c, s[1][n][2 + j] * c};
+                        const int first = first_seen(a, pos[n][j]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {          // positions row_of(g) + 8 i of the unit
+                            const int at_row = row_of<HD>(g) + 8 * i, key = key0 + at_row;
+                            if (bad >> at_row & 1) x[i] = __uint_as_float(0x7fffffffu);
+                            if (key > pos[n][j] || key < first) x[i] = -INFINITY;
+                        }
+                        float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        const float new_m = fmaxf(m[n][j], top), against = new_m == -INFINITY ? 0.f : new_m;
+                        const float new_ref = fmaxf(ref[n][j], top + v_unit), from = new_ref == -INFINITY ? 0.f : new_ref;
+                        shrink[n][j] = ratio(ref[n][j], from);
+                        moved |= new_ref != ref[n][j];
+                        const float lift = fast_exp2(fminf(against + v_unit - from + (float)WEIGHT_UP, 126.f));
+                        float add = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            x[i] = fast_exp2(x[i] - against);
+                            add += x[i];
+                            weight[i >> 1][(i & 1) * 2 + j] = x[i] * lift;
+                        }
+                        sum[n][j] = sum[n][j] * ratio(m[n][j], against) + add;         // of this lane's positions
+                        m[n][j] = new_m;
+                        ref[n][j] = new_ref;
+                    }
+#pragma unroll
+                    for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) pb[tile][n][half] = transposed(pack_f16(weight[tile][2 * half], weight[tile][2 * half + 1]));
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < DIMS / 2; ++i)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) acc[n][i][k] *= shrink[n][k & 1];
+                }
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile) {
+                    // positions 2t, 2t + 1 of the products, and 8 behind them
+                    const int row[2] = {tile * 16 + row_of<HD>(2 * t), tile * 16 + row_of<HD>(2 * t + 1)};
+                    uint32_t s_low, s_high;
+                    if (a.block_shift >= 4) {
+                        s_low = s_high = __byte_perm(packed[row[0]], 0, 0x3232);
+                    } else {
+                        s_low = __byte_perm(packed[row[0]], packed[row[1]], 0x7632);
+                        s_high = __byte_perm(packed[row[0] + 8], packed[row[1] + 8], 0x7632);
+                    }
+                    const uint32_t o_low = hmul2(s_low, MINUS_1152), o_high = hmul2(s_high, MINUS_1152);
+                    uint32_t x[4][DIMS / 4];                   // positions 2t, 2t + 1, 2t + 8, 2t + 9: this lane's columns
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int from = row[i & 1] + (i >> 1) * 8;
+                        if constexpr (HD == 128) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(v_tile + byte_of<HD>(from, g));
+                            x[i][0] = v.x;
+                            x[i][1] = v.y;
+                            x[i][2] = v.z;
+                            x[i][3] = v.w;
+                        } else {
+                            const uint2 v = *reinterpret_cast<const uint2*>(v_tile + byte_of<HD>(from, g >> 1) + (g & 1) * 8);
+                            x[i][0] = v.x;
+                            x[i][1] = v.y;
+                        }
+                    }
+#pragma unroll
+                    for (int w = 0; w < DIMS / 4; ++w)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {                  // columns 4w + 2 half, + 1
+                            const uint32_t y_low = __byte_perm(x[0][w], x[1][w], half ? 0x7632 : 0x5410);
+                            const uint32_t y_high = __byte_perm(x[2][w], x[3][w], half ? 0x7632 : 0x5410);
+                            const uint32_t a0 = even_bytes(y_low, s_low, o_low), a1 = odd_bytes(y_low, s_low, o_low);
+                            const uint32_t a2 = even_bytes(y_high, s_high, o_high), a3 = odd_bytes(y_high, s_high, o_high);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_f16(acc[n][2 * w + half], a0, a1, a2, a3, pb[tile][n][0], pb[tile][n][1]);
+                        }
+                }
+            }
+            __syncwarp();                                      // everyone has read the unit: its room is free
+            ask(stage);
+            if (++stage == STAGES) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+        // ---- the four warps' sums, in a fixed order: 2 to 0 and 3 to 1, then 1 to 0
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                sum[n][j] += __shfl_xor_sync(0xffffffffu, sum[n][j], 4);
+                sum[n][j] += __shfl_xor_sync(0xffffffffu, sum[n][j], 8);
+                sum[n][j] += __shfl_xor_sync(0xffffffffu, sum[n][j], 16);
+            }
+        constexpr int HALF = 8 * NT * LD + 8 * NT * 4;
+#pragma unroll
+        for (int round = 0; round < 2; ++round) {
+            const int from = 2 >> round;                       // warps from .. 2 from - 1 hand over to those `from` below
+            float* rows = merge + (warp & (from - 1)) * HALF;
+            __syncthreads();
+            if (warp >= from && warp < 2 * from) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int r = n * 8 + 2 * t + j;
+#pragma unroll
+                        for (int i = 0; i < DIMS / 2; ++i)
+                            *reinterpret_cast<float2*>(rows + r * LD + g * DIMS + 2 * i) = make_float2(acc[n][i][j], acc[n][i][2 + j]);
+                        if (g == 0) *reinterpret_cast<float4*>(rows + 8 * NT * LD + r * 4) = make_float4(m[n][j], ref[n][j], sum[n][j], 0.f);
+                    }
+            }
+            __syncthreads();
+            if (warp < from) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int r = n * 8 + 2 * t + j;
+                        const float4 other = *reinterpret_cast<const float4*>(rows + 8 * NT * LD + r * 4);
+                        const float new_m = fmaxf(m[n][j], other.x), new_ref = fmaxf(ref[n][j], other.y);
+                        sum[n][j] = sum[n][j] * ratio(m[n][j], new_m) + other.z * ratio(other.x, new_m);
+                        const float mine = ratio(ref[n][j], new_ref), theirs = ratio(other.y, new_ref);
+#pragma unroll
+                        for (int i = 0; i < DIMS / 2; ++i) {
+                            const float2 x = *reinterpret_cast<const float2*>(rows + r * LD + g * DIMS + 2 * i);
+                            acc[n][i][j] = acc[n][i][j] * mine + x.x * theirs;
+                            acc[n][i][2 + j] = acc[n][i][2 + j] * mine + x.y * theirs;
+                        }
+                        m[n][j] = new_m;
+                        ref[n][j] = new_ref;
+                    }
+            }
+        }
+        if (warp == 0) {
+            const bool whole = pair.start >= r0 && pair_end <= r1;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int r = n * 8 + 2 * t + j;
+                    if (r >= n_rows) continue;
+                    float factor = sum[n][j] != 0.f ? fast_exp2(ref[n][j] - (float)(WEIGHT_UP + SCALE_UP) - m[n][j]) : 0.f;
+                    if (whole) {
+                        factor /= sum[n][j] != 0.f ? sum[n][j] : 1.f;
+                        uint32_t out[DIMS / 2];
+#pragma unroll
+                        for (int i = 0; i < DIMS / 2; ++i) out[i] = pack_bf16(acc[n][i][j] * factor, acc[n][i][2 + j] * factor);
+                        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first_token + r / share) * a.out_stride +
+                                            (size_t)(pair.head * share + r % share) * HD + g * DIMS;
+#pragma unroll
+                        for (int i = 0; i < DIMS / 2; i += 4) *reinterpret_cast<uint4*>(to + 2 * i) = make_uint4(out[i], out[i + 1], out[i + 2], out[i + 3]);
+                    } else {
+                        const size_t part = ((size_t)blockIdx.x * 2 + (pair.start >= r0 ? 1 : 0)) * FEW_ROWS + r;
+                        float* to = a.acc + part * HD + g * DIMS;
+#pragma unroll
+                        for (int i = 0; i < DIMS / 2; i += 2)
+                            *reinterpret_cast<float4*>(to + 2 * i) = make_float4(acc[n][i][j] * factor, acc[n][i][2 + j] * factor, acc[n][i + 1][j] * factor,
+                                                                                 acc[n][i + 1][2 + j] * factor);
+                        if (g == 0) *reinterpret_cast<float2*>(a.stats + part * 2) = make_float2(sum[n][j] != 0.f ? m[n][j] : -INFINITY, sum[n][j]);
+                    }
+                }
+        }
+        if (end >= r1) break;
+        next_pair(a, pair, most_tokens);
+    }
+    __syncthreads();
+    if (*abort_flag)                                           // a wait ran out: copies in flight get their time before the block leaves
+        for (int i = 0; i < 100; ++i) __nanosleep(10000);
+}
+
+// The parts of a (sequence, key head) pair that several blocks have worked on. A block a pair, a warp a row at a time (several for few rows, each with
+// its share of the parts; their sums are added in order).
+constexpr int JOIN_WARPS = 8;
+template <int HD>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_few_join_kernel(const __grid_constant__ Args a) {
+    constexpr int W = HD / 32;                                 // a lane's columns
+    __shared__ float shared_value[JOIN_WARPS][HD];
+    __shared__ float2 shared_stats[JOIN_WARPS];
+    griddep_launch();
+    griddep_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = a.n_heads / a.n_kv_heads;
+    const int seq = blockIdx.x / a.n_kv_heads, head = blockIdx.x % a.n_kv_heads;
+    const Span span = span_of(a, seq, a.few_tokens);
+    if (span.pages == 0) return;
+    long long all = 0, before = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+        const unsigned pages = s0 + lane < a.n_seqs ? (unsigned)span_of(a, s0 + lane, a.few_tokens).pages : 0u;
+        all += __reduce_add_sync(0xffffffffu, pages);
+        before += __reduce_add_sync(0xffffffffu, s0 + lane < seq ? pages : 0u);
+    }
+    const long long per = range_pages(a, all * a.n_kv_heads), start = before * a.n_kv_heads + (long long)head * span.pages;
+    const int first = (int)(start / per), last = (int)((start + span.pages - 1) / per), n_parts = last - first + 1, n_rows = span.n_new * share;
+    if (n_parts == 1) return;                                  // finished where it was worked on
+    const float* acc = behind_wait(a.acc);
+    const float2* stats = reinterpret_cast<const float2*>(behind_wait(a.stats));
+    int a_row = 1;                                             // warps of a row
+    while (a_row * 2 * n_rows <= JOIN_WARPS) a_row *= 2;
+    const int rows = JOIN_WARPS / a_row, mine = warp % a_row;
+    auto part_of = [&](int k, int r) { return ((size_t)(first + k) * 2 + (k == 0 ? 1 : 0)) * FEW_ROWS + r; };
+    for (int r0 = 0; r0 < n_rows; r0 += rows) {
+        const int r = r0 + warp / a_row;
+        float value[W], m = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < W; ++c) value[c] = 0.f;
+        if (r < n_rows) {
+            for (int k = lane; k < n_parts; k += 32) m = fmaxf(m, stats[part_of(k, r)].x);
+            m = warp_max(m);
+            const float against = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+            for (int k = mine; k < n_parts; k += a_row) {
+                const float2 s = stats[part_of(k, r)];
+                const float* from = acc + part_of(k, r) * HD + lane * W;
+                float x[W];
+                if constexpr (W == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from);
+                else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(from);
+                const float weight = s.y != 0.f ? exp2f(s.x - against) : 0.f;
+                sum += s.y * weight;
+#pragma unroll
+                for (int c = 0; c < W; ++c) value[c] = fmaf(x[c], weight, value[c]);
+            }
+        }
+        if (a_row > 1) {
+            if (r < n_rows) {
+#pragma unroll
+                for (int c = 0; c < W; ++c) shared_value[warp][lane * W + c] = value[c];
+                if (lane == 0) shared_stats[warp] = make_float2(m, sum);
+            }
+            __syncthreads();
+            if (mine == 0 && r < n_rows)
+                for (int k = 1; k < a_row; ++k) {
+                    sum += shared_stats[warp + k].y;
+#pragma unroll
+                    for (int c = 0; c < W; ++c) value[c] += shared_value[warp + k][lane * W + c];
+                }
+            __syncthreads();
+        }
+        if (mine == 0 && r < n_rows) {
+            const float inv = sum != 0.f ? 1.f / sum : 0.f;
+            __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first_token + r / share) * a.out_stride + (size_t)(head * share + r % share) * HD + lane * W;
+#pragma unroll
+            for (int c = 0; c < W; c += 2) *reinterpret_cast<uint32_t*>(to + c) = pack_bf16(value[c] * inv, value[c + 1] * inv);
         }
     }
 }
@@ -426,6 +1054,8 @@ __global__ void __launch_bounds__(256, CHUNKS == 1 ? 5 : 3) attention_int8_join_
 // ------------------------------------------------------------------------------------------------ the launches
 
 struct Plan {
+    bool few;                        // the kernel for few rows takes the step
+    int few_blocks, deal_blocks, deal_least;
     int tiles, slots;
     long long blocks;                // of a slot
     long long part_rows;             // rows that are joined from parts
@@ -436,12 +1066,33 @@ struct Sizes {
     bool tc;
 };
 
+// The kernel for few rows deals pages out where a sequence may have more than WHOLE_PAGES, LEAST_PAGES a block at least.
+constexpr int WHOLE_PAGES = 4, LEAST_PAGES = 2;
+
 // Into how many slices the pages are cut: as many as make all blocks come to about the blocks that the SMs hold at once, two pages each at least.
 Plan plan_for(const Sizes& z) {
     Plan p;
     const int share = z.n_heads / z.n_kv_heads;
     const int seen = z.window > 0 && z.window + z.max_new < z.max_len ? z.window + z.max_new : z.max_len;
     const int pages = ceil_div(seen > 0 ? seen : 1, LLMB_PAGE);
+    p.few = z.tc && (long long)z.max_new * share <= FEW_ROWS;
+    p.few_blocks = p.deal_blocks = p.deal_least = 0;
+    if (p.few) {
+        const long long pairs = (long long)z.n_seqs * z.n_kv_heads;
+        p.tiles = 1;
+        p.slots = 1;
+        p.part_rows = 0;
+        p.blocks = pairs;
+        if (pages > WHOLE_PAGES) {
+            const int held = SMS * ((long long)z.max_new * share <= 8 ? 3 : 2);
+            p.deal_least = LEAST_PAGES;
+            p.deal_blocks = (long long)ceil_div(pages, LEAST_PAGES) * pairs < held ? (int)(ceil_div(pages, LEAST_PAGES) * pairs) : held;
+            p.blocks = p.deal_blocks;
+            p.part_rows = 2ll * p.deal_blocks * FEW_ROWS;
+        }
+        p.few_blocks = (int)p.blocks;
+        return p;
+    }
     p.tiles = ceil_div((long long)z.max_new * share, SIMT_ROWS);
     p.blocks = (long long)z.n_seqs * p.tiles * z.n_kv_heads;
     const long long wave = (long long)SMS * (z.head_dim <= 128 ? 2 : 1);
@@ -485,8 +1136,41 @@ void launch_join(const Args& a, int rows, cudaStream_t stream) {
     else llmb::launch(attention_int8_join_kernel<T, 8, CHUNKS>, dim3(rows), 256, 0, stream, true, a, rows);
 }
 
+// 8-bit rows of a cache, boxes of UNIT of them
+int make_map_int8(CUtensorMap* map, const void* ptr, long long rows, int dim) {
+    EncodeTiled encode = encode_fn();
+    if (!encode) return fail(LLMB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)dim};
+    cuuint32_t box[2] = {(cuuint32_t)dim, (cuuint32_t)UNIT}, elem[2] = {1, 1};
+    CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(LLMB_ERR_CUDA, "cuTensorMapEncodeTiled (8 bits) failed with %d", (int)r);
+    return LLMB_OK;
+}
+
+template <int HD, int NT>
+int launch_few(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
+    static bool done[MAX_DEVICES] = {};
+    if (int code = allow_shared((const void*)attention_int8_few_kernel<HD, NT>, Few<HD, NT>::BYTES, done)) return code;
+    CUtensorMap map_k, map_v;
+    const long long rows = (long long)a.n_pages * a.n_kv_heads * LLMB_PAGE;
+    int code = make_map_int8(&map_k, a.keys, rows, HD);
+    if (!code) code = make_map_int8(&map_v, a.values, rows, HD);
+    if (code) return code;
+    llmb::launch(attention_int8_few_kernel<HD, NT>, dim3(p.few_blocks), FEW_THREADS, Few<HD, NT>::BYTES, stream, true, map_k, map_v, a, status);
+    if ((code = check_launch("attention_int8_few")) || p.deal_blocks == 0) return code;
+    llmb::launch(attention_int8_few_join_kernel<HD>, dim3(a.n_seqs * a.n_kv_heads), JOIN_WARPS * 32, 0, stream, true, a);
+    return check_launch("attention_int8_few_join");
+}
+
 template <typename T>
 int run(const Args& a, const Plan& p, const Sizes& z, int* status, cudaStream_t stream) {
+    if (p.few) {
+        const bool narrow = a.few_tokens * (a.n_heads / a.n_kv_heads) <= 8;
+        if (a.head_dim == 64) return narrow ? launch_few<64, 1>(a, p, status, stream) : launch_few<64, 2>(a, p, status, stream);
+        return narrow ? launch_few<128, 1>(a, p, status, stream) : launch_few<128, 2>(a, p, status, stream);
+    }
     int code = a.head_dim <= 64 ? launch_simt<T, 64>(a, p, status, stream) : a.head_dim <= 128 ? launch_simt<T, 128>(a, p, status, stream)
                                                                                                : launch_simt<T, 256>(a, p, status, stream);
     if (code || a.slots == 1) return code;
@@ -528,7 +1212,7 @@ LLMB_EXPORT long long llmb_attention_int8_scratch_floats(const llmb_int8_sizes* 
     *kernels = 1;
     if (!sane(*z)) return 0;
     const Plan p = plan_for(sizes_of(*z));
-    if (p.slots > 1) ++*kernels;
+    if (p.slots > 1 || p.deal_blocks > 0) ++*kernels;
     return scratch_floats_of(p.part_rows * p.slots, z->head_dim);
 }
 
@@ -548,6 +1232,9 @@ LLMB_EXPORT int llmb_attention_int8(const void* q, const void* keys, const float
     LLMB_REQUIRE((long long)z.n_tokens * z.n_heads < (1ll << 31), "attention_int8: %d tokens of %d heads", z.n_tokens, z.n_heads);
     auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     LLMB_REQUIRE(aligned(keys) && aligned(values), "attention_int8: pages must start on 16 bytes");
+    LLMB_REQUIRE(!z.tc || (z.dtype == LLMB_DTYPE_BF16 && (z.head_dim == 64 || z.head_dim == 128) && scale > 0.f && z.q_stride % 8 == 0 &&
+                           z.out_stride % 8 == 0 && aligned(q) && aligned(out) && (long long)z.n_pages * z.n_kv_heads * LLMB_PAGE < (1ll << 31)),
+                 "attention_int8: the tensor-core kernels do not take these operands");
     const Sizes s = sizes_of(z);
     const Plan p = plan_for(s);
     LLMB_REQUIRE(p.blocks < (1ll << 31), "attention_int8: too many blocks");
@@ -558,7 +1245,8 @@ LLMB_EXPORT int llmb_attention_int8(const void* q, const void* keys, const float
     if (status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status, status_word(), 0));
     const Args a{q, (const signed char*)keys, key_scales, (const signed char*)values, value_scales, block_table, seq_lens, cu_seqlens, seq_order, out, scratch,
                  scratch + value_floats(parts, z.head_dim), z.q_stride, z.out_stride, z.table_stride, z.ring_pages, z.n_pages, z.n_tokens, z.n_seqs,
-                 z.n_heads, z.n_kv_heads, z.head_dim, shift, z.window, scale * LOG2E, z.max_new, p.tiles, p.slots};
+                 z.n_heads, z.n_kv_heads, z.head_dim, shift, z.window, scale * LOG2E, z.max_new, p.tiles, p.slots,
+                 p.few ? z.max_new : 0, p.deal_blocks, p.deal_least};
     return z.dtype == LLMB_DTYPE_F32 ? run<float>(a, p, s, status, stream) : run<__nv_bfloat16>(a, p, s, status, stream);
 }
 

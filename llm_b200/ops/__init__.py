@@ -1114,8 +1114,8 @@ def check_device_status() -> None:
                  "sigmoid_attention_tc", "diff_attention_tc", "gated_recurrence", "prefix_attention", "attention_int8", "int8_cache"):
         if name in _loaded:
             code = getattr(_loaded[name], f"llmb_{name}_status")()
-            if name in ("attention_int8", "int8_cache") and code in (_BEYOND_BOUNDS, _OUT_OF_RANGE):
-                said = "more tokens than max_new said" if code == _BEYOND_BOUNDS else "a position, sequence, token or page that there is not"
+            if name in ("attention_int8", "int8_cache") and code in _INT8_REPORTS:
+                said = _INT8_REPORTS[code]
                 raise KernelError(f"{name}: a step brought {said}; its results are not valid")
             if name == "prefix_attention" and code == _BEYOND_BOUNDS:
                 raise KernelError("prefix_attention: a step brought more tokens than max_new or max_group said; its results are not valid")
@@ -1456,8 +1456,9 @@ def attention_replay_key(step, n_heads: int, n_kv_heads: int, window: int = 0):
 # ----------------------------------------------------------------------------- sequences that share pages
 
 _prefix_entry = None
-_OUT_OF_RANGE = 51              # what the kernels of a cache in 8 bits report of a place that there is not (csrc/attention_int8.cu, int8_cache.cu)
 _BEYOND_BOUNDS = 50             # its report of a step larger than its bounds (csrc/prefix_attention.cu)
+_INT8_REPORTS = {50: "more tokens than max_new said", 51: "a position, sequence, token or page that there is not",
+                 52: "a scale that is no power of two"}      # (csrc/attention_int8.cu, int8_cache.cu)
 
 
 def _declare_prefix():
@@ -1790,7 +1791,8 @@ def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seql
         return out
     # no step goes beyond its tokens and its table; lengths count in powers of two of pages, so that a captured step serves the next lengths
     max_new, max_len = min(max_new, n), page_bucket(-(-min(max_len, 1 << 30) // PAGE)) * PAGE
-    tc = 0
+    tc = int(dtype is torch.bfloat16 and head_dim in (64, 128) and scale > 0 and q_stride % 8 == 0 and not (qkv.data_ptr() | out.data_ptr()) & 15
+             and keys.values.numel() // head_dim < 1 << 31 and not tactics.is_disabled("attention_int8_tc"))
     packed, at_sizes, floats, kernels = _int8_plan(q_stride, n_heads * head_dim, block_table.stride(0), ring_pages, keys.values.shape[0], code, n, n_seqs,
                                                    n_heads, n_kv_heads, head_dim, keys.block, window, max_new, max_len, tc)
     parts = _scratch(qkv.device, "attention", floats)[0] if floats else None

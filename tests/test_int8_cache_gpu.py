@@ -260,8 +260,10 @@ def test_attention_reports():
     for dtype in (F32, BF16):
         b = make([100, 10], [1, 40], 4, 2, 128, dtype, seed=23)
         good = call(b)
-        for wrong in ("max_new", "page", "order"):
+        for wrong in ("max_new", "page", "order", "scale"):
             c = dict(b)
+            if wrong == "scale":
+                c["keys"] = ops().Int8Pages(b["keys"].values, b["keys"].scales * 1.5)
             if wrong == "page":
                 c["table"] = b["table"].clone()
                 c["table"][0, 1] = 1 << 20
