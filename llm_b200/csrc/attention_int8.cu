@@ -44,6 +44,9 @@ struct Args {
     int max_new, tiles, slots;
     int few_tokens;                  // sequences that bring at most so many tokens are the kernel's for few rows (0: it is not launched)
     int deal_blocks, deal_least;     // its blocks that all pages are dealt out to, in ranges of so many pages at least; 0: a block a (sequence, key head)
+    int wide_blocks, wide_least;     // the same of the kernel for many rows, in steps; 0: a block a tile
+    float* wide_acc;                 // parts of that kernel's blocks: [blocks, 2, 256, head_dim], and their maxima and sums
+    float* wide_stats;
 };
 
 // What a kernel reports (no wait has these codes): a step that brings more tokens than max_new says; a place outside of what the call was given, which is
@@ -953,6 +956,727 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_few_join_kerne
     }
 }
 
+// ------------------------------------------------------------------------------------------------ bfloat16, many rows
+//
+// 256 rows a block, one block an SM: two tiles of 128 rows with four softmax warps each share the keys and values of 128 positions (two pages), which
+// four more warps fetch as bytes and leave in shared memory as fp16, widened as above; one warp issues the products (tcgen05). Per tile one buffer of
+// scores [128, 128] and O [128, D] fill tensor memory; the two tiles take turns: while the softmax of one works on its scores, the products of
+// the other run (P V of these positions, then Q K^T of the next). Widening is a fifth of the instructions that 256 rows of softmax take, and 256 rows
+// share it.
+//
+// References as above, with two differences: keys' scales count from the largest of the 128 positions of a step, values' from the largest of each page (from
+// 2^-90 of the largest so far at least, which keeps the sums of the weights exact where a page's values are zeros), and R moves only when it is exceeded by 2^8.
+//
+// The steps of all (sequence, key head, tile), one after the other, are dealt out to the blocks in ranges of equal length, as pages are above; barriers
+// and buffers run on from one tile to the next, so the next tile's keys are fetched and widened while a result is written.
+
+constexpr int WIDE_THREADS = 512;           // warps 0 products, 4-7 and 8-11 a tile's softmax, 12-15 widening
+constexpr int WIDE_ROWS = 256, TILE_ROWS = 128, STEP = 128, STEP_PAGES = STEP / LLMB_PAGE;
+constexpr int TILE_PIECE = TILE_ROWS * 128, STEP_PIECE = STEP * 128;             // 64 columns of the head: 16 KB
+constexpr int REGS_ISSUE = 56, REGS_SOFTMAX = 176, REGS_WIDEN = 104, REGS_LAUNCHED = 128;
+static_assert(128 * (REGS_ISSUE + 2 * REGS_SOFTMAX + REGS_WIDEN) <= WIDE_THREADS * REGS_LAUNCHED, "the shares come from what the block is launched with");
+constexpr int WIDE_UP = 7;                  // power of two that weights are lifted to; R may lag 2^8 behind
+constexpr int VALUE_SPAN = 90;
+constexpr int INFOS = 4;                    // steps whose scales are on their way to the softmax: the step behind the next one may be widened by then
+
+// two 32-bit values to an instruction
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+
+struct StepInfo {
+    float k_unit, v_unit[2];         // what a step of the keys stands for; exponent of the values' reference, of each page
+    uint32_t any_bad;
+    uint32_t bad[4];                 // positions whose scale is no number
+};
+
+// A tile of a (sequence, key head) and its pages.
+struct Segment {
+    int seq, head, tile;
+    int row0, n_rows;
+    int first_page, pages, steps;
+    int low, limit;                  // positions that a row of the tile sees at all
+    Span span;
+    long long start;                 // its first step among all
+};
+__device__ __forceinline__ int tiles_of(const Args& a, const Span& s) { return (s.n_new * (a.n_heads / a.n_kv_heads) + WIDE_ROWS - 1) / WIDE_ROWS; }
+__device__ __forceinline__ void place_tile(const Args& a, Segment& g) {
+    const int share = a.n_heads / a.n_kv_heads;
+    g.row0 = g.tile * WIDE_ROWS;
+    g.n_rows = min(WIDE_ROWS, g.span.n_new * share - g.row0);
+    g.low = first_seen(a, g.span.first_pos + g.row0 / share);
+    g.limit = g.span.first_pos + (g.row0 + g.n_rows - 1) / share;
+    g.first_page = g.low / LLMB_PAGE;
+    g.pages = g.limit / LLMB_PAGE + 1 - g.first_page;
+    g.steps = (g.pages + STEP_PAGES - 1) / STEP_PAGES;
+}
+// The sequence as this kernel takes it: 0 pages where the kernel for few rows does, or nothing is brought.
+__device__ __forceinline__ Span wide_span(const Args& a, int seq) {
+    Span s = span_of(a, seq, a.max_new);
+    if (s.n_new <= a.few_tokens) s.pages = 0;
+    return s;
+}
+// The steps of all tiles of one of the sequence's key heads.
+__device__ __forceinline__ int steps_of(const Args& a, const Span& s) {
+    int sum = 0;
+    if (s.pages == 0) return 0;
+    Segment g;
+    g.span = s;
+    const int tiles = tiles_of(a, s);
+    for (g.tile = 0; g.tile < tiles; ++g.tile) {
+        place_tile(a, g);
+        sum += g.steps;
+    }
+    return sum;
+}
+__device__ __forceinline__ long long all_steps(const Args& a, int lane) {
+    long long sum = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32)
+        sum += __reduce_add_sync(0xffffffffu, s0 + lane < a.n_seqs ? (unsigned)steps_of(a, wide_span(a, s0 + lane)) : 0u);
+    return sum * a.n_kv_heads;
+}
+__device__ __forceinline__ Segment segment_at(const Args& a, long long at, int lane) {
+    long long before = 0;
+    Segment g;
+    for (int s0 = 0;; s0 += 32) {
+        const int mine = s0 + lane < a.n_seqs ? steps_of(a, wide_span(a, s0 + lane)) : 0;
+        unsigned up = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            unsigned left = __shfl_up_sync(0xffffffffu, up, d);
+            if (lane >= d) up += left;
+        }
+        const unsigned beyond = __ballot_sync(0xffffffffu, at < before + (long long)up * a.n_kv_heads);
+        if (beyond) {
+            const int k = __ffs(beyond) - 1, steps = __shfl_sync(0xffffffffu, mine, k);
+            g.seq = s0 + k;
+            g.span = wide_span(a, g.seq);
+            g.start = before + (long long)(__shfl_sync(0xffffffffu, up, k) - steps) * a.n_kv_heads;
+            g.head = (int)((at - g.start) / steps);
+            g.start += (long long)g.head * steps;
+            for (g.tile = 0;; ++g.tile) {
+                place_tile(a, g);
+                if (at < g.start + g.steps) return g;
+                g.start += g.steps;
+            }
+        }
+        before += (long long)__shfl_sync(0xffffffffu, up, 31) * a.n_kv_heads;
+    }
+}
+// the segment behind it (there is one)
+__device__ __forceinline__ void next_segment(const Args& a, Segment& g) {
+    g.start += g.steps;
+    if (++g.tile >= tiles_of(a, g.span)) {
+        g.tile = 0;
+        if (++g.head == a.n_kv_heads) {
+            g.head = 0;
+            do g.span = wide_span(a, ++g.seq); while (g.span.pages == 0 && g.seq + 1 < a.n_seqs);
+        }
+    }
+    place_tile(a, g);
+}
+__device__ __forceinline__ long long range_steps(const Args& a, long long all) {
+    const long long per = (all + a.wide_blocks - 1) / a.wide_blocks;
+    return per < a.wide_least ? a.wide_least : per;
+}
+
+// 16 bytes as 16 fp16 numbers times s, in their order
+__device__ __forceinline__ void widen16(const uint4& v, uint32_t s, uint4& low, uint4& high) {
+    const uint32_t off = hmul2(s, MINUS_1152), x[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
+    uint32_t y[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        y[2 * i] = hfma2(__byte_perm(x[i], 0x64646464u, 0x4140), s, off);
+        y[2 * i + 1] = hfma2(__byte_perm(x[i], 0x64646464u, 0x4342), s, off);
+    }
+    low = make_uint4(y[0], y[1], y[2], y[3]);
+    high = make_uint4(y[4], y[5], y[6], y[7]);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(const __grid_constant__ Args a, int* status) {
+    constexpr int PIECES = HD / 64, Q_BYTES = PIECES * TILE_PIECE, STEP_BYTES = PIECES * STEP_PIECE;
+    constexpr uint32_t SCORES = 128, O_FIRST = 256, COLS = 512;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* q_tile = smem_raw;                         // [2]
+    unsigned char* k_tile = q_tile + 2 * Q_BYTES;             // [2] steps
+    unsigned char* v_tile = k_tile + 2 * STEP_BYTES;          // [2]
+    StepInfo* infos = reinterpret_cast<StepInfo*>(v_tile + 2 * STEP_BYTES);      // [INFOS]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(infos + INFOS);
+    uint64_t* q_full = bars;                  // [2] a tile's queries are in shared memory, its last result is out of tensor memory
+    uint64_t* k_full = bars + 2;              // [2]
+    uint64_t* k_empty = bars + 4;             // [2]
+    uint64_t* v_full = bars + 6;              // [2]
+    uint64_t* v_empty = bars + 8;             // [2]
+    uint64_t* s_full = bars + 10;             // [2] a tile's scores are complete (and all its products before)
+    uint64_t* p_full = bars + 12;             // [2][2] its weights of 64 positions are written and O has been rescaled
+    uint64_t* o_full = bars + 16;             // [2] the tile's last P V is complete
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = warp_index(), lane = threadIdx.x & 31, share = a.n_heads / a.n_kv_heads;
+    if (threadIdx.x == 0) {
+#pragma unroll 1
+        for (int i = 0; i < 18; ++i) {
+            const bool by_group = i < 4 || i == 6 || i == 7 || (i >= 12 && i < 16);
+            mbar_init(smem_u32(&bars[i]), by_group ? 128 : 1);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // Tensor memory is taken when the kernel in front is done with it, and the next kernel may take some only when this one has it: two
+    // that wait for one another's would stand still.
+    griddep_wait();
+    Segment segment;
+    long long r0, r1;                                         // the block's range of all steps
+    if (a.wide_blocks == 0) {                                 // a tile a block, those that see most first
+        int x = blockIdx.x;
+        segment.head = x % a.n_kv_heads;
+        x /= a.n_kv_heads;
+        const int back = x % a.tiles, at = x / a.tiles;
+        segment.seq = a.seq_order ? a.seq_order[at] : at;
+        if ((unsigned)segment.seq >= (unsigned)a.n_seqs) {
+            if (threadIdx.x == 0) report(status, OUT_OF_RANGE);
+            return;
+        }
+        segment.span = wide_span(a, segment.seq);
+        if (threadIdx.x == 0 && back == 0) check_span(a, segment.span, status);
+        const int tiles = segment.span.pages > 0 ? tiles_of(a, segment.span) : 0;
+        if (back >= tiles) return;
+        segment.tile = tiles - 1 - back;
+        place_tile(a, segment);
+        segment.start = r0 = 0;
+        r1 = segment.steps;
+    } else {
+        const long long all = all_steps(a, lane), per = range_steps(a, all);
+        if (blockIdx.x == 0)
+            for (int s = threadIdx.x; s < a.n_seqs; s += WIDE_THREADS) {
+                check_span(a, span_of(a, s, a.max_new), status);
+                if (a.seq_order && (unsigned)a.seq_order[s] >= (unsigned)a.n_seqs) report(status, OUT_OF_RANGE);
+            }
+        r0 = blockIdx.x * per;
+        r1 = r0 + per < all ? r0 + per : all;
+        if (r0 >= r1) return;
+        segment = segment_at(a, r0, lane);
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    griddep_launch();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total = (int)(r1 - r0);                         // steps of the block, counted on over its segments
+    // what the block has of a segment: its steps skip .. skip + count - 1
+    auto share_of = [&](const Segment& g, int& skip, int& count) {
+        skip = g.start < r0 ? (int)(r0 - g.start) : 0;
+        const long long end = g.start + g.steps < r1 ? g.start + g.steps : r1;
+        count = (int)(end - g.start) - skip;
+    };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
+        if (warp == 0) {
+            // fp16 operands, 32-bit sums
+            constexpr uint32_t idesc_qk = (1u << 4) | ((uint32_t)(STEP >> 3) << 17) | ((uint32_t)(TILE_ROWS >> 4) << 24);
+            constexpr uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(TILE_ROWS >> 4) << 24);
+            const uint64_t q_desc = smem_desc(smem_u32(q_tile));
+            const uint64_t k_desc0 = smem_desc(smem_u32(k_tile)), v_desc0 = smem_desc_mn(smem_u32(v_tile), STEP_PIECE);
+            constexpr uint64_t BUFFER = (uint64_t)(STEP_BYTES >> 4), Q_TILE = (uint64_t)(Q_BYTES >> 4);
+            uint32_t turns[2] = {0, 0}, segments[2] = {0, 0};  // of each tile so far
+            auto issue_qk = [&](int tile, int n_tiles, int st) {
+                const int b = st & 1;
+                if (elect_one()) {
+#pragma unroll
+                    for (int j = 0; j < HD / 16; ++j) {
+                        uint64_t q_off = (uint64_t)(((j >> 2) * TILE_PIECE + (j & 3) * 32) >> 4);
+                        uint64_t k_off = (uint64_t)(((j >> 2) * STEP_PIECE + (j & 3) * 32) >> 4);
+                        tcgen05_mma(tmem_base + tile * SCORES, q_desc + tile * Q_TILE + q_off, k_desc0 + b * BUFFER + k_off, idesc_qk, j > 0 ? 1u : 0u);
+                    }
+                    tcgen05_commit(smem_u32(&s_full[tile]));
+                    if (tile == n_tiles - 1) tcgen05_commit(smem_u32(&k_empty[b]));
+                }
+                __syncwarp();
+            };
+            // the values of step st and the keys of the step behind it are in shared memory
+            auto arrived = [&](int st, bool last) {
+                return mbar_wait_warp(smem_u32(&v_full[st & 1]), (st >> 1) & 1, abort_flag, status, 36) &&
+                       (last || mbar_wait_warp(smem_u32(&k_full[(st + 1) & 1]), ((st + 1) >> 1) & 1, abort_flag, status, 37));
+            };
+            // A tile's products of step st, then its scores of the next.
+            auto turn = [&](int tile, int n_tiles, int st, bool first, bool last, bool last_but_one) -> bool {
+                const int b = st & 1;
+                const uint32_t o = tmem_base + O_FIRST + tile * HD, p = tmem_base + tile * SCORES;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {        // 64 positions each: the first are multiplied while the others' weights are formed
+                    if (!mbar_wait_warp(smem_u32(&p_full[2 * tile + half]), turns[tile] & 1, abort_flag, status, 35)) return false;
+                    tcgen05_fence_after();
+                    // 16 positions a product: 8 columns of weights, 2048 bytes of value rows; a segment's first one overwrites O
+                    if (elect_one()) {
+#pragma unroll
+                        for (int j = 4 * half; j < 4 * half + 4; ++j)
+                            tcgen05_mma_ts(o, p + j * 8, v_desc0 + b * BUFFER + (uint64_t)((j * 2048) >> 4), idesc_pv, first && j == 0 ? 0u : 1u);
+                    }
+                    __syncwarp();
+                }
+                ++turns[tile];
+                if (elect_one()) {
+                    if (last) tcgen05_commit(smem_u32(&o_full[tile]));
+                    if (tile == n_tiles - 1) tcgen05_commit(smem_u32(&v_empty[b]));
+                }
+                __syncwarp();
+                if (!last) {
+                    issue_qk(tile, n_tiles, st + 1);
+                    // the next keys and values are waited for where products are under way
+                    if (tile == 0) return arrived(st + 1, last_but_one);
+                }
+                return true;
+            };
+            bool ok = true;
+            for (int st = 0; st < total && ok;) {
+                int skip, count;
+                share_of(segment, skip, count);
+                const int n_tiles = segment.n_rows > TILE_ROWS ? 2 : 1, end = st + count;
+                ok = mbar_wait_warp(smem_u32(&k_full[st & 1]), (st >> 1) & 1, abort_flag, status, 34);
+                for (int tile = 0; tile < n_tiles && ok; ++tile) {
+                    ok = mbar_wait_warp(smem_u32(&q_full[tile]), segments[tile]++ & 1, abort_flag, status, 33);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    issue_qk(tile, n_tiles, st);
+                }
+                ok = ok && arrived(st, st + 1 == end);
+                for (int i = st; i < end && ok; ++i) {
+                    ok = turn(0, n_tiles, i, i == st, i + 1 == end, i + 2 == end);
+                    if (n_tiles == 2) ok = ok && turn(1, n_tiles, i, i == st, i + 1 == end, false);
+                }
+                st = end;
+                if (st < total) next_segment(a, segment);
+            }
+        }
+    } else if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_WIDEN));
+        constexpr int LANES = HD / 16, RPP = 128 / LANES, PASSES = STEP / RPP;        // lanes of a row, rows of a pass
+        const int t = threadIdx.x & 127, wq = warp & 3, c = t % LANES, row_in = t / LANES;
+        const int scales_per_page = LLMB_PAGE >> a.block_shift;
+        uint4 raw_k[PASSES], raw_v[PASSES];
+        uint32_t ks[4], vs[4];                                 // the scales of positions lane + 32 j of the step
+        // What is asked for: step `asked` of the block's; its pages' numbers are on their way.
+        Segment ahead = segment;
+        int asked = 0, begun, count, pages_ahead[STEP_PAGES];  // begun: the step that `ahead` begins with
+        int skip;
+        share_of(ahead, skip, count);
+        begun = 0;
+        auto look_up = [&]() {
+            if (asked >= total) return;
+            if (asked == begun + count) {
+                begun += count;
+                next_segment(a, ahead);
+                share_of(ahead, skip, count);
+            }
+            const int* table = a.block_table + (size_t)ahead.seq * a.table_stride;
+            const int place = (skip + asked - begun) * STEP_PAGES;
+#pragma unroll
+            for (int i = 0; i < STEP_PAGES; ++i)
+                pages_ahead[i] = place + i < ahead.pages ? page_at(a, table, ahead.first_page + place + i, status) * a.n_kv_heads + ahead.head : -1;
+        };
+        auto fetch = [&](uint4 (&raw)[PASSES], const signed char* cache) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                const int row = i * RPP + row_in, page = pages_ahead[i * RPP / LLMB_PAGE];
+                raw[i] = page >= 0 ? *reinterpret_cast<const uint4*>(cache + ((size_t)page * LLMB_PAGE + row % LLMB_PAGE) * HD + c * 16) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        };
+        auto fetch_scales = [&]() {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int page = pages_ahead[j >> 1], block = ((j & 1) * 32 + lane) >> a.block_shift;
+                ks[j] = page >= 0 ? __float_as_uint(a.key_scales[(size_t)page * scales_per_page + block]) : 0u;
+                vs[j] = page >= 0 ? __float_as_uint(a.value_scales[(size_t)page * scales_per_page + block]) : 0u;
+            }
+        };
+        // a step's rows to shared memory, times their scales
+        auto store = [&](unsigned char* to, const uint4 (&raw)[PASSES], const uint32_t (&packed)[4], uint32_t which) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                const int row = i * RPP + row_in, from = (i * RPP) % 32 + wq * (32 / LANES) + lane / LANES;
+                const uint32_t s = __byte_perm(__shfl_sync(0xffffffffu, packed[i * RPP / 32], from), 0, which);
+                uint4 low, high;
+                widen16(raw[i], s, low, high);
+                unsigned char* at = to + (c >> 2) * STEP_PIECE + row * 128;
+                const int chunk = 2 * (c & 3), flip = c >> 2;  // (lanes of the second piece write their halves the other way round: other banks)
+                *reinterpret_cast<uint4*>(at + (((chunk + flip) ^ (row & 7)) << 4)) = flip ? high : low;
+                *reinterpret_cast<uint4*>(at + (((chunk + 1 - flip) ^ (row & 7)) << 4)) = flip ? low : high;
+            }
+        };
+        look_up();
+        fetch(raw_k, a.keys);
+        fetch_scales();
+        fetch(raw_v, a.values);
+        int value_top = 0;                                     // the largest exponent of the segment's values so far
+        bool ok = true;
+        for (int st = 0; st < total && ok; ++st) {
+            const int b = st & 1;
+            // the step's scales from the largest of those that are seen
+            const Segment& of = ahead;                         // (asked == st here: the look-up for the next step comes below)
+            if (st == begun) value_top = 0;
+            const int alike = a.block_shift >= 4 ? 15 : 0, key0 = (of.first_page + (skip + st - begun) * STEP_PAGES) * LLMB_PAGE;
+            uint32_t packed[4], bad[4];
+            int ke = 0, ve[STEP_PAGES] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int nearest = key0 + ((lane + 32 * j) & ~alike);
+                const bool seen = nearest <= of.limit && nearest + alike >= of.low;
+                const uint32_t k = seen ? ks[j] : 0u, v = seen ? vs[j] : 0u;
+                const bool none = (k & 0x7fffffffu) >= NOT_FINITE || (v & 0x7fffffffu) >= NOT_FINITE;
+                if (!none && ((k | v) & 0x807fffffu)) report(status, NOT_A_POWER);
+                bad[j] = __ballot_sync(0xffffffffu, none);
+                ks[j] = none ? 0u : k >> 23;
+                vs[j] = none ? 0u : v >> 23;
+                ke = max(ke, (int)ks[j]);
+                ve[j >> 1] = max(ve[j >> 1], (int)vs[j]);
+            }
+            ke = __reduce_max_sync(0xffffffffu, ke);
+#pragma unroll
+            for (int i = 0; i < STEP_PAGES; ++i) {
+                ve[i] = __reduce_max_sync(0xffffffffu, ve[i]);
+                value_top = max(value_top, ve[i]);
+                ve[i] = max(ve[i], value_top - VALUE_SPAN);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                packed[j] = (ks[j] ? f16_power((int)(ks[j] & 0xffu) - ke + SCALE_UP) : 0u) |
+                            ((vs[j] ? f16_power((int)(vs[j] & 0xffu) - ve[j >> 1] + SCALE_UP) : 0u) << 16);
+            if (t == 0) {
+                StepInfo& info = infos[st % INFOS];
+                info.k_unit = __uint_as_float((uint32_t)max(ke - SCALE_UP, 1) << 23);
+                info.v_unit[0] = (float)(ve[0] - 127);
+                info.v_unit[1] = (float)(ve[1] - 127);
+                info.any_bad = bad[0] | bad[1] | bad[2] | bad[3];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) info.bad[j] = bad[j];
+            }
+            ++asked;
+            look_up();
+            ok = st < 2 || mbar_wait_warp(smem_u32(&k_empty[b]), ((st >> 1) - 1) & 1, abort_flag, status, 31);
+            if (!ok) break;
+            store(k_tile + b * STEP_BYTES, raw_k, packed, 0x1010);
+            fence_async_shared();
+            mbar_arrive(smem_u32(&k_full[b]));
+            if (st + 1 < total) {
+                fetch(raw_k, a.keys);
+                fetch_scales();
+            }
+            ok = st < 2 || mbar_wait_warp(smem_u32(&v_empty[b]), ((st >> 1) - 1) & 1, abort_flag, status, 32);
+            if (!ok) break;
+            store(v_tile + b * STEP_BYTES, raw_v, packed, 0x3232);
+            fence_async_shared();
+            mbar_arrive(smem_u32(&v_full[b]));
+            if (st + 1 < total) fetch(raw_v, a.values);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+        const int tile = (warp >> 2) - 1, quarter = warp & 3, r = quarter * 32 + lane;       // row of the tile = lane of tensor memory
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t s_addr = lane_addr + tile * SCORES, o_addr = lane_addr + O_FIRST + tile * HD;
+        unsigned char* my_row = q_tile + tile * Q_BYTES + r * 128;          // 128 bytes of each piece; its 16-byte chunks are swizzled
+        uint32_t turns = 0, segments = 0;
+        bool ok = true;
+        for (int st = 0; st < total && ok;) {
+            int skip, count;
+            share_of(segment, skip, count);
+            const int n_tiles = segment.n_rows > TILE_ROWS ? 2 : 1, end = st + count;
+            const int tile_rows = segment.n_rows - tile * TILE_ROWS;        // of this tile, above 128 where it is full
+            if (tile < n_tiles) {
+                const bool valid = r < tile_rows, idle = quarter * 32 >= tile_rows;      // idle: a warp without rows (its lanes' weights reach nobody's result)
+                const int at = segment.row0 + tile * TILE_ROWS + (valid ? r : 0);
+                const int token = segment.span.first_token + at / share, head = segment.head * share + at % share;
+                const int my_pos = valid ? segment.span.first_pos + at / share : -1, my_first = first_seen(a, my_pos);
+                float row_scale;
+                {   // the row's queries as fp16, their largest at 2^14
+                    const uint4* q = reinterpret_cast<const uint4*>(behind_wait(static_cast<const __nv_bfloat16*>(a.q)) + (size_t)token * a.q_stride + (size_t)head * HD);
+                    uint4 x[HD / 8];
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int i = 0; i < HD / 8; ++i) x[i] = valid ? q[i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                    for (int i = 0; i < HD / 8; ++i) {
+                        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) most = max(most, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+                    }
+                    const int exponent = max((int)(most >> 7), 27) - 127;
+                    const float factor = __uint_as_float((uint32_t)(14 - exponent + 127) << 23);
+                    row_scale = a.scale_log2 * __uint_as_float((uint32_t)max(exponent - 14 + 127, 1) << 23);
+#pragma unroll
+                    for (int i = 0; i < HD / 8; ++i) {
+                        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                        uint32_t y[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) y[k] = pack_f16(__uint_as_float(w[k] << 16) * factor, __uint_as_float(w[k] & 0xffff0000u) * factor);
+                        *reinterpret_cast<uint4*>(my_row + (i >> 3) * TILE_PIECE + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+                    }
+                }
+                fence_async_shared();
+                tcgen05_fence_before();                        // (the last result has been read)
+                mbar_arrive(smem_u32(&q_full[tile]));
+                float run_max = -INFINITY, ref = -INFINITY, run_sum = 0.f;
+                for (int i = st; i < end && ok; ++i) {
+                    ok = mbar_wait_warp(smem_u32(&s_full[tile]), turns++ & 1, abort_flag, status, 38);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    if (idle) {
+                        mbar_arrive(smem_u32(&p_full[2 * tile]));
+                        mbar_arrive(smem_u32(&p_full[2 * tile + 1]));
+                        continue;
+                    }
+                    const StepInfo& info = infos[i % INFOS];
+                    const float c = fmaxf(row_scale * info.k_unit, 1.1754944e-38f), v_unit0 = info.v_unit[0], v_unit1 = info.v_unit[1];
+                    const int key0 = (segment.first_page + (skip + i - st) * STEP_PAGES) * LLMB_PAGE;
+                    const int last = my_pos - key0, first = my_first - key0;       // the positions of the step that the row sees
+                    uint32_t r0s[32], r1s[32], r2s[32], r3s[32];
+                    // the second half of the scores comes while the first one's maximum is taken
+                    tmem_ld32_start(s_addr, r0s);
+                    tmem_ld32_start(s_addr + 32, r1s);
+                    tmem_ld32_wait(r0s);
+                    tmem_ld32_wait(r1s);
+                    tmem_ld32_start(s_addr + 64, r2s);
+                    tmem_ld32_start(s_addr + 96, r3s);
+                    auto mask = [&](uint32_t (&x)[32], int from) {
+                        if (info.any_bad) {
+                            const uint32_t bad = info.bad[from >> 5];
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (bad >> j & 1) x[j] = 0x7fffffffu;
+                        }
+                        if (last < from + 31) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (j + from > last) x[j] = __float_as_uint(-INFINITY);
+                        }
+                        if (first > from) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (j + from < first) x[j] = __float_as_uint(-INFINITY);
+                        }
+                    };
+                    mask(r0s, 0);
+                    mask(r1s, 32);
+                    float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        top0 = max3(top0, __uint_as_float(r0s[j]), __uint_as_float(r0s[j + 1]));
+                        top1 = max3(top1, __uint_as_float(r1s[j]), __uint_as_float(r1s[j + 1]));
+                    }
+                    tmem_ld32_wait(r2s);
+                    tmem_ld32_wait(r3s);
+                    mask(r2s, 64);
+                    mask(r3s, 96);
+                    top0 = fmaxf(top0, top1) * c;
+                    float top2 = -INFINITY, top3 = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        top2 = max3(top2, __uint_as_float(r2s[j]), __uint_as_float(r2s[j + 1]));
+                        top3 = max3(top3, __uint_as_float(r3s[j]), __uint_as_float(r3s[j + 1]));
+                    }
+                    top2 = fmaxf(top2, top3) * c;
+                    const float new_max = max3(run_max, top0, top2), candidate = fmaxf(top0 + v_unit0, top2 + v_unit1);
+                    // (a row that has seen no position yet keeps -inf, and all its weights are zero)
+                    const bool move = candidate - ref > 8.f;
+                    const float new_ref = move ? candidate : ref;
+                    const float alpha = move ? fast_exp2(ref - new_ref) : 1.f;
+                    const bool none = new_ref == -INFINITY;
+                    const float lift = none ? 0.f : (float)WIDE_UP - new_ref;
+                    if (i > st && __any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+                        for (int col = 0; col < HD; col += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o_addr + col, o);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                            tmem_st16(o_addr + col, o);
+                        }
+                    }
+                    const uint64_t scale2 = pair_of(c, c);
+                    uint64_t shift2 = pair_of(lift + v_unit0, lift + v_unit0), add = pair_of(0u, 0u);
+                    // what the page's weights are lifted by, taken off their sum
+                    auto page_sum = [&](float v_unit) {
+                        float lo, hi;
+                        unpair(add, lo, hi);
+                        return none ? lo + hi : (lo + hi) * fast_exp2(-lift - v_unit - new_max);
+                    };
+                    auto to_weights = [&](const uint32_t (&x)[32], int col) {
+                        uint32_t packed[16];
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float p0, p1;
+                            unpair(fma2(pair_of(x[j], x[j + 1]), scale2, shift2), p0, p1);
+                            p0 = fast_exp2(p0);
+                            p1 = fast_exp2(p1);
+                            add = add2(add, pair_of(p0, p1));
+                            packed[j >> 1] = pack_f16(p0, p1);
+                        }
+                        tmem_st16(s_addr + (col >> 1), packed);
+                    };
+                    to_weights(r0s, 0);
+                    to_weights(r1s, 32);
+                    tmem_st_wait();
+                    tcgen05_fence_before();
+                    mbar_arrive(smem_u32(&p_full[2 * tile]));
+                    run_sum = run_sum * ratio(run_max, new_max) + page_sum(v_unit0);
+                    shift2 = pair_of(lift + v_unit1, lift + v_unit1);
+                    add = pair_of(0u, 0u);
+                    to_weights(r2s, 64);
+                    to_weights(r3s, 96);
+                    run_sum += page_sum(v_unit1);
+                    run_max = new_max;
+                    ref = new_ref;
+                    tmem_st_wait();
+                    tcgen05_fence_before();
+                    mbar_arrive(smem_u32(&p_full[2 * tile + 1]));
+                }
+                // the result, or the block's part of it: by way of the queries' room, a warp's rows at a time, so that rows are written as a whole
+                ok = ok && mbar_wait_warp(smem_u32(&o_full[tile]), segments++ & 1, abort_flag, status, 40);
+                if (ok && !idle) {
+                    tcgen05_fence_after();
+                    const bool whole = segment.start >= r0 && segment.start + segment.steps <= r1;
+                    float factor = run_sum != 0.f ? fast_exp2(ref - (float)(WIDE_UP + SCALE_UP) - run_max) : 0.f;
+                    const size_t part = ((size_t)blockIdx.x * 2 + (segment.start >= r0 ? 1 : 0)) * WIDE_ROWS + tile * TILE_ROWS + r;
+                    unsigned char* to = nullptr;               // the row's place in memory
+                    if (whole) {
+                        factor /= run_sum != 0.f ? run_sum : 1.f;
+                        if (valid) to = reinterpret_cast<unsigned char*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD);
+                    } else if (valid) {
+                        to = reinterpret_cast<unsigned char*>(a.wide_acc + part * HD);
+                        *reinterpret_cast<float2*>(a.wide_stats + part * 2) = make_float2(run_sum != 0.f ? run_max : -INFINITY, run_sum);
+                    }
+                    constexpr int ROOM = HD * 2;               // bytes of a row that go out at a time
+                    for (int half = 0; half < (whole ? 1 : 2); ++half) {
+                        const int from = half * (HD / 2), columns = whole ? HD : HD / 2;
+#pragma unroll 1
+                        for (int col = 0; col < columns; col += 32) {
+                            uint32_t x[32];
+                            tmem_ld32(o_addr + from + col, x);
+#pragma unroll
+                            for (int d = 0; d < 32; ++d) x[d] = __float_as_uint(__uint_as_float(x[d]) * factor);
+                            const int chunk0 = col * (whole ? 2 : 4) / 16;
+                            auto put = [&](int chunk, uint4 v) {
+                                *reinterpret_cast<uint4*>(my_row + (chunk >> 3) * TILE_PIECE + (((chunk & 7) ^ (r & 7)) << 4)) = v;
+                            };
+                            if (whole) {
+#pragma unroll
+                                for (int d = 0; d < 32; d += 8)
+                                    put(chunk0 + d / 8, make_uint4(pack2(__uint_as_float(x[d]), __uint_as_float(x[d + 1])), pack2(__uint_as_float(x[d + 2]), __uint_as_float(x[d + 3])),
+                                                                   pack2(__uint_as_float(x[d + 4]), __uint_as_float(x[d + 5])), pack2(__uint_as_float(x[d + 6]), __uint_as_float(x[d + 7]))));
+                            } else {
+#pragma unroll
+                                for (int d = 0; d < 32; d += 4) put(chunk0 + d / 4, make_uint4(x[d], x[d + 1], x[d + 2], x[d + 3]));
+                            }
+                        }
+                        __syncwarp();
+                        constexpr int CHUNKS = ROOM / 16, ROWS = 32 / CHUNKS;    // ROWS rows to an instruction
+                        const int chunk = lane % CHUNKS;
+#pragma unroll 4
+                        for (int i = 0; i < 32; i += ROWS) {
+                            const int row = i + lane / CHUNKS, in_tile = quarter * 32 + row;
+                            unsigned char* there = reinterpret_cast<unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), row));
+                            if (there)
+                                *reinterpret_cast<uint4*>(there + half * ROOM + chunk * 16) = *reinterpret_cast<const uint4*>(
+                                    q_tile + tile * Q_BYTES + (chunk >> 3) * TILE_PIECE + in_tile * 128 + (((chunk & 7) ^ (in_tile & 7)) << 4));
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+            st = end;
+            if (st < total) next_segment(a, segment);
+        }
+    }
+
+    tcgen05_fence_before();
+    __syncthreads();
+    if (*abort_flag) {                                         // a wait ran out: products in flight get their time before the block leaves
+        for (int i = 0; i < 100; ++i) __nanosleep(10000);
+        __syncthreads();
+    }
+    if (warp == 0) {
+        tcgen05_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(COLS) : "memory");
+    }
+}
+
+// The parts of a tile that several blocks have worked on: a block 64 of its rows, a warp a row at a time.
+template <int HD>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_wide_join_kernel(const __grid_constant__ Args a) {
+    constexpr int W = HD / 32, SLICES = 4;                     // W: a lane's columns
+    griddep_launch();
+    griddep_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = a.n_heads / a.n_kv_heads;
+    int x = blockIdx.x;
+    const int slice = x % SLICES;
+    x /= SLICES;
+    Segment g;
+    g.head = x % a.n_kv_heads;
+    x /= a.n_kv_heads;
+    g.tile = x % a.tiles;
+    g.seq = x / a.tiles;
+    g.span = wide_span(a, g.seq);
+    if (g.span.pages == 0 || g.tile >= tiles_of(a, g.span)) return;
+    place_tile(a, g);
+    if (slice * (WIDE_ROWS / SLICES) >= g.n_rows) return;
+    long long all = 0, before = 0;
+    int mine = 0;                                              // steps of a key head of this sequence
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+        const unsigned steps = s0 + lane < a.n_seqs ? (unsigned)steps_of(a, wide_span(a, s0 + lane)) : 0u;
+        all += __reduce_add_sync(0xffffffffu, steps);
+        before += __reduce_add_sync(0xffffffffu, s0 + lane < g.seq ? steps : 0u);
+        if (g.seq >= s0 && g.seq < s0 + 32) mine = __shfl_sync(0xffffffffu, steps, g.seq - s0);
+    }
+    Segment up = g;
+    long long start = before * a.n_kv_heads + (long long)g.head * mine;
+    for (up.tile = 0; up.tile < g.tile; ++up.tile) {
+        place_tile(a, up);
+        start += up.steps;
+    }
+    const long long per = range_steps(a, all * a.n_kv_heads);
+    const int first = (int)(start / per), n_parts = (int)((start + g.steps - 1) / per) - first + 1;
+    if (n_parts == 1) return;                                  // finished where it was worked on
+    const float* acc = behind_wait(a.wide_acc);
+    const float2* stats = reinterpret_cast<const float2*>(behind_wait(a.wide_stats));
+    auto part_of = [&](int k, int r) { return ((size_t)(first + k) * 2 + (k == 0 ? 1 : 0)) * WIDE_ROWS + r; };
+    for (int i = warp; i < WIDE_ROWS / SLICES; i += JOIN_WARPS) {
+        const int r = slice * (WIDE_ROWS / SLICES) + i;
+        if (r >= g.n_rows) break;
+        float value[W], m = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < W; ++c) value[c] = 0.f;
+        for (int k = lane; k < n_parts; k += 32) m = fmaxf(m, stats[part_of(k, r)].x);
+        m = warp_max(m);
+        const float against = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+        for (int k = 0; k < n_parts; ++k) {
+            const float2 s = stats[part_of(k, r)];
+            const float* from = acc + part_of(k, r) * HD + lane * W;
+            float v[W];
+            if constexpr (W == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(from);
+            else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(from);
+            const float weight = s.y != 0.f ? exp2f(s.x - against) : 0.f;
+            sum += s.y * weight;
+#pragma unroll
+            for (int c = 0; c < W; ++c) value[c] = fmaf(v[c], weight, value[c]);
+        }
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+        const int token = g.span.first_token + (g.row0 + r) / share, head = g.head * share + (g.row0 + r) % share;
+        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD + lane * W;
+#pragma unroll
+        for (int c = 0; c < W; c += 2) *reinterpret_cast<uint32_t*>(to + c) = pack_bf16(value[c] * inv, value[c + 1] * inv);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ the parts joined
 //
 // WARPS warps a row: each reads all the maxima and sums, a lane two parts, and takes every WARPS-th part, several of them in flight; their
@@ -1053,53 +1777,76 @@ __global__ void __launch_bounds__(256, CHUNKS == 1 ? 5 : 3) attention_int8_join_
 
 // ------------------------------------------------------------------------------------------------ the launches
 
-struct Plan {
-    bool few;                        // the kernel for few rows takes the step
-    int few_blocks, deal_blocks, deal_least;
-    int tiles, slots;
-    long long blocks;                // of a slot
-    long long part_rows;             // rows that are joined from parts
-};
-
 struct Sizes {
     int n_tokens, n_seqs, n_heads, n_kv_heads, head_dim, window, max_new, max_len;
     bool tc;
 };
 
+struct Plan {
+    bool few, wide;                  // which of the tensor-core kernels run (neither: the CUDA cores)
+    int few_tokens;                  // sequences that bring at most so many tokens are the first one's
+    long long few_blocks, wide_grid, blocks;
+    int deal_blocks, deal_least, wide_blocks, wide_least;
+    int tiles, slots;
+    long long part_rows, wide_rows;  // rows that are joined from parts
+    int launches;
+};
+
 // The kernel for few rows deals pages out where a sequence may have more than WHOLE_PAGES, LEAST_PAGES a block at least.
 constexpr int WHOLE_PAGES = 4, LEAST_PAGES = 2;
+// The kernel for many rows deals steps out, LEAST_STEPS a block at least, unless no tile has more than WHOLE_STEPS.
+constexpr int WHOLE_STEPS = 4, LEAST_STEPS = 4;
 
-// Into how many slices the pages are cut: as many as make all blocks come to about the blocks that the SMs hold at once, two pages each at least.
 Plan plan_for(const Sizes& z) {
-    Plan p;
+    Plan p = {};
     const int share = z.n_heads / z.n_kv_heads;
     const int seen = z.window > 0 && z.window + z.max_new < z.max_len ? z.window + z.max_new : z.max_len;
     const int pages = ceil_div(seen > 0 ? seen : 1, LLMB_PAGE);
-    p.few = z.tc && (long long)z.max_new * share <= FEW_ROWS;
-    p.few_blocks = p.deal_blocks = p.deal_least = 0;
-    if (p.few) {
-        const long long pairs = (long long)z.n_seqs * z.n_kv_heads;
-        p.tiles = 1;
-        p.slots = 1;
-        p.part_rows = 0;
-        p.blocks = pairs;
-        if (pages > WHOLE_PAGES) {
-            const int held = SMS * ((long long)z.max_new * share <= 8 ? 3 : 2);
-            p.deal_least = LEAST_PAGES;
-            p.deal_blocks = (long long)ceil_div(pages, LEAST_PAGES) * pairs < held ? (int)(ceil_div(pages, LEAST_PAGES) * pairs) : held;
-            p.blocks = p.deal_blocks;
-            p.part_rows = 2ll * p.deal_blocks * FEW_ROWS;
+    const long long pairs = (long long)z.n_seqs * z.n_kv_heads;
+    p.slots = 1;
+    p.launches = 1;
+    if (z.tc) {
+        p.few_tokens = FEW_ROWS / share < z.max_new ? FEW_ROWS / share : z.max_new;
+        p.wide = (long long)z.max_new * share > FEW_ROWS;
+        // sequences that bring few tokens beside others that bring many: there are some for certain only where the tokens are too few for all to bring more
+        p.few = !p.wide || (p.few_tokens > 0 && z.n_tokens < (long long)z.n_seqs * (p.few_tokens + 1));
+        if (!p.few) p.few_tokens = 0;
+        p.launches = 0;
+        if (p.few) {
+            p.few_blocks = pairs;
+            ++p.launches;
+            if (pages > WHOLE_PAGES) {
+                const long long held = SMS * ((long long)p.few_tokens * share <= 8 ? 3 : 2), most = ceil_div(pages, LEAST_PAGES) * pairs;
+                p.deal_least = LEAST_PAGES;
+                p.deal_blocks = (int)(most < held ? most : held);
+                p.few_blocks = p.deal_blocks;
+                p.part_rows = 2ll * p.deal_blocks * FEW_ROWS;
+                ++p.launches;
+            }
         }
-        p.few_blocks = (int)p.blocks;
+        if (p.wide) {
+            p.tiles = ceil_div((long long)z.max_new * share, WIDE_ROWS);
+            p.wide_grid = pairs * p.tiles;
+            ++p.launches;
+            if (ceil_div(pages, STEP_PAGES) > WHOLE_STEPS) {
+                p.wide_blocks = SMS;
+                p.wide_least = LEAST_STEPS;
+                p.wide_grid = SMS;
+                p.wide_rows = 2ll * SMS * WIDE_ROWS;
+                ++p.launches;
+            }
+        }
         return p;
     }
+    // Into how many slices the pages are cut: as many as make all blocks come to about the blocks that the SMs hold at once, two pages each at least.
     p.tiles = ceil_div((long long)z.max_new * share, SIMT_ROWS);
-    p.blocks = (long long)z.n_seqs * p.tiles * z.n_kv_heads;
+    p.blocks = pairs * p.tiles;
     const long long wave = (long long)SMS * (z.head_dim <= 128 ? 2 : 1);
     long long slots = wave / p.blocks;
     if (slots > pages / 2) slots = pages / 2;
     p.slots = slots < 1 ? 1 : slots > MAX_SPLITS ? MAX_SPLITS : (int)slots;
     p.part_rows = p.slots == 1 ? 0 : (long long)z.n_tokens * z.n_heads;
+    if (p.slots > 1) ++p.launches;
     return p;
 }
 
@@ -1158,19 +1905,43 @@ int launch_few(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
     int code = make_map_int8(&map_k, a.keys, rows, HD);
     if (!code) code = make_map_int8(&map_v, a.values, rows, HD);
     if (code) return code;
-    llmb::launch(attention_int8_few_kernel<HD, NT>, dim3(p.few_blocks), FEW_THREADS, Few<HD, NT>::BYTES, stream, true, map_k, map_v, a, status);
+    llmb::launch(attention_int8_few_kernel<HD, NT>, dim3((unsigned)p.few_blocks), FEW_THREADS, Few<HD, NT>::BYTES, stream, true, map_k, map_v, a, status);
     if ((code = check_launch("attention_int8_few")) || p.deal_blocks == 0) return code;
     llmb::launch(attention_int8_few_join_kernel<HD>, dim3(a.n_seqs * a.n_kv_heads), JOIN_WARPS * 32, 0, stream, true, a);
     return check_launch("attention_int8_few_join");
 }
 
+template <int HD>
+int launch_wide(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
+    // (more than half of an SM's shared memory for the smaller head size too: tensor memory has room for one block)
+    constexpr size_t need = (HD / 64) * (2 * TILE_PIECE + 4 * STEP_PIECE) + INFOS * sizeof(StepInfo) + 19 * 8, bytes = need < 120 * 1024 ? 120 * 1024 : need;
+    static_assert(bytes + 1024 <= 227 * 1024, "one block an SM");
+    static bool done[MAX_DEVICES] = {};
+    static bool checked = false;
+    if (!checked) {                              // (its softmax warps would wait for registers that are not there)
+        cudaFuncAttributes built;
+        LLMB_CUDA(cudaFuncGetAttributes(&built, attention_int8_wide_kernel<HD>));
+        LLMB_REQUIRE(built.numRegs >= REGS_LAUNCHED, "attention_int8: built with %d registers a thread", built.numRegs);
+        checked = true;
+    }
+    if (int code = allow_shared((const void*)attention_int8_wide_kernel<HD>, bytes, done)) return code;
+    llmb::launch(attention_int8_wide_kernel<HD>, dim3((unsigned)p.wide_grid), WIDE_THREADS, bytes, stream, true, a, status);
+    if (int code = check_launch("attention_int8_wide")) return code;
+    if (p.wide_blocks == 0) return LLMB_OK;
+    llmb::launch(attention_int8_wide_join_kernel<HD>, dim3((unsigned)(4ll * a.n_seqs * a.n_kv_heads * a.tiles)), JOIN_WARPS * 32, 0, stream, true, a);
+    return check_launch("attention_int8_wide_join");
+}
+
+template <int HD>
+int launch_tc(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
+    int code = LLMB_OK;
+    if (p.few) code = a.few_tokens * (a.n_heads / a.n_kv_heads) <= 8 ? launch_few<HD, 1>(a, p, status, stream) : launch_few<HD, 2>(a, p, status, stream);
+    return code || !p.wide ? code : launch_wide<HD>(a, p, status, stream);
+}
+
 template <typename T>
 int run(const Args& a, const Plan& p, const Sizes& z, int* status, cudaStream_t stream) {
-    if (p.few) {
-        const bool narrow = a.few_tokens * (a.n_heads / a.n_kv_heads) <= 8;
-        if (a.head_dim == 64) return narrow ? launch_few<64, 1>(a, p, status, stream) : launch_few<64, 2>(a, p, status, stream);
-        return narrow ? launch_few<128, 1>(a, p, status, stream) : launch_few<128, 2>(a, p, status, stream);
-    }
+    if (p.few || p.wide) return a.head_dim == 64 ? launch_tc<64>(a, p, status, stream) : launch_tc<128>(a, p, status, stream);
     int code = a.head_dim <= 64 ? launch_simt<T, 64>(a, p, status, stream) : a.head_dim <= 128 ? launch_simt<T, 128>(a, p, status, stream)
                                                                                                : launch_simt<T, 256>(a, p, status, stream);
     if (code || a.slots == 1) return code;
@@ -1212,8 +1983,8 @@ LLMB_EXPORT long long llmb_attention_int8_scratch_floats(const llmb_int8_sizes* 
     *kernels = 1;
     if (!sane(*z)) return 0;
     const Plan p = plan_for(sizes_of(*z));
-    if (p.slots > 1 || p.deal_blocks > 0) ++*kernels;
-    return scratch_floats_of(p.part_rows * p.slots, z->head_dim);
+    *kernels = p.launches;
+    return scratch_floats_of(p.part_rows * p.slots + p.wide_rows, z->head_dim);
 }
 
 LLMB_EXPORT int llmb_attention_int8(const void* q, const void* keys, const float* key_scales, const void* values, const float* value_scales,
@@ -1237,16 +2008,18 @@ LLMB_EXPORT int llmb_attention_int8(const void* q, const void* keys, const float
                  "attention_int8: the tensor-core kernels do not take these operands");
     const Sizes s = sizes_of(z);
     const Plan p = plan_for(s);
-    LLMB_REQUIRE(p.blocks < (1ll << 31), "attention_int8: too many blocks");
-    const long long parts = p.part_rows * p.slots;
-    LLMB_REQUIRE(parts == 0 || (scratch != nullptr && aligned(scratch) && scratch_floats >= scratch_floats_of(parts, z.head_dim)),
+    LLMB_REQUIRE(p.blocks < (1ll << 31) && p.few_blocks < (1ll << 31) && 4 * p.wide_grid < (1ll << 31) &&
+                 4ll * z.n_seqs * z.n_kv_heads * p.tiles < (1ll << 31), "attention_int8: too many blocks");
+    const long long parts = p.part_rows * p.slots, all_parts = parts + p.wide_rows;
+    LLMB_REQUIRE(all_parts == 0 || (scratch != nullptr && aligned(scratch) && scratch_floats >= scratch_floats_of(all_parts, z.head_dim)),
                  "attention_int8: scratch too small");
     int* status = nullptr;
     if (status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status, status_word(), 0));
+    float* stats = scratch + value_floats(all_parts, z.head_dim);
     const Args a{q, (const signed char*)keys, key_scales, (const signed char*)values, value_scales, block_table, seq_lens, cu_seqlens, seq_order, out, scratch,
-                 scratch + value_floats(parts, z.head_dim), z.q_stride, z.out_stride, z.table_stride, z.ring_pages, z.n_pages, z.n_tokens, z.n_seqs,
-                 z.n_heads, z.n_kv_heads, z.head_dim, shift, z.window, scale * LOG2E, z.max_new, p.tiles, p.slots,
-                 p.few ? z.max_new : 0, p.deal_blocks, p.deal_least};
+                 stats, z.q_stride, z.out_stride, z.table_stride, z.ring_pages, z.n_pages, z.n_tokens, z.n_seqs, z.n_heads, z.n_kv_heads, z.head_dim,
+                 shift, z.window, scale * LOG2E, z.max_new, p.tiles, p.slots, p.few_tokens, p.deal_blocks, p.deal_least, p.wide_blocks, p.wide_least,
+                 scratch + parts * z.head_dim, stats + 2 * parts};
     return z.dtype == LLMB_DTYPE_F32 ? run<float>(a, p, s, status, stream) : run<__nv_bfloat16>(a, p, s, status, stream);
 }
 
