@@ -958,8 +958,10 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_few_join_kerne
 
 // ------------------------------------------------------------------------------------------------ bfloat16, many rows
 //
-// 256 rows a block, one block an SM: two tiles of 128 rows with four softmax warps each share the keys and values of 128 positions (two pages), which
-// four more warps fetch as bytes and leave in shared memory as fp16, widened as above; one warp issues the products (tcgen05). Per tile one buffer of
+// 256 rows a block, one block an SM: two tiles of 128 rows with four softmax warps each share the keys and values of 128 positions (two pages). One warp
+// has a step's bytes copied to shared memory and works out its scales, four widen them, as above, to the fp16 operands of the products (tcgen05), which
+// another one issues. (Fetched through the widening warps' registers a step took 9,000 cycles: the fence between their stores and the products
+// waits for their loads too.) Per tile one buffer of
 // scores [128, 128] and O [128, D] fill tensor memory; the two tiles take turns: while the softmax of one works on its scores, the products of
 // the other run (P V of these positions, then Q K^T of the next). Widening is a fifth of the instructions that 256 rows of softmax take, and 256 rows
 // share it.
@@ -970,10 +972,10 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_few_join_kerne
 // The steps of all (sequence, key head, tile), one after the other, are dealt out to the blocks in ranges of equal length, as pages are above; barriers
 // and buffers run on from one tile to the next, so the next tile's keys are fetched and widened while a result is written.
 
-constexpr int WIDE_THREADS = 512;           // warps 0 products, 4-7 and 8-11 a tile's softmax, 12-15 widening
+constexpr int WIDE_THREADS = 512;           // warps 0 products, 1 pages and scales, 4-7 and 8-11 a tile's softmax, 12-15 widening
 constexpr int WIDE_ROWS = 256, TILE_ROWS = 128, STEP = 128, STEP_PAGES = STEP / LLMB_PAGE;
 constexpr int TILE_PIECE = TILE_ROWS * 128, STEP_PIECE = STEP * 128;             // 64 columns of the head: 16 KB
-constexpr int REGS_ISSUE = 56, REGS_SOFTMAX = 176, REGS_WIDEN = 104, REGS_LAUNCHED = 128;
+constexpr int REGS_ISSUE = 96, REGS_SOFTMAX = 168, REGS_WIDEN = 80, REGS_LAUNCHED = 128;
 static_assert(128 * (REGS_ISSUE + 2 * REGS_SOFTMAX + REGS_WIDEN) <= WIDE_THREADS * REGS_LAUNCHED, "the shares come from what the block is launched with");
 constexpr int WIDE_UP = 7;                  // power of two that weights are lifted to; R may lag 2^8 behind
 constexpr int VALUE_SPAN = 90;
@@ -991,6 +993,7 @@ struct StepInfo {
     float k_unit, v_unit[2];         // what a step of the keys stands for; exponent of the values' reference, of each page
     uint32_t any_bad;
     uint32_t bad[4];                 // positions whose scale is no number
+    uint32_t packed[STEP];           // fp16 scales: key's low, value's high
 };
 
 // A tile of a (sequence, key head) and its pages.
@@ -1104,7 +1107,9 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
     unsigned char* q_tile = smem_raw;                         // [2]
     unsigned char* k_tile = q_tile + 2 * Q_BYTES;             // [2] steps
     unsigned char* v_tile = k_tile + 2 * STEP_BYTES;          // [2]
-    StepInfo* infos = reinterpret_cast<StepInfo*>(v_tile + 2 * STEP_BYTES);      // [INFOS]
+    unsigned char* raw_k = v_tile + 2 * STEP_BYTES;           // a step's bytes
+    unsigned char* raw_v = raw_k + STEP * HD;
+    StepInfo* infos = reinterpret_cast<StepInfo*>(raw_v + STEP * HD);            // [INFOS]
     uint64_t* bars = reinterpret_cast<uint64_t*>(infos + INFOS);
     uint64_t* q_full = bars;                  // [2] a tile's queries are in shared memory, its last result is out of tensor memory
     uint64_t* k_full = bars + 2;              // [2]
@@ -1114,15 +1119,17 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
     uint64_t* s_full = bars + 10;             // [2] a tile's scores are complete (and all its products before)
     uint64_t* p_full = bars + 12;             // [2][2] its weights of 64 positions are written and O has been rescaled
     uint64_t* o_full = bars + 16;             // [2] the tile's last P V is complete
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+    uint64_t* raw_full = bars + 18;           // [2] a step's keys as bytes and its scales, its values as bytes
+    uint64_t* raw_empty = bars + 20;          // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = warp_index(), lane = threadIdx.x & 31, share = a.n_heads / a.n_kv_heads;
     if (threadIdx.x == 0) {
 #pragma unroll 1
-        for (int i = 0; i < 18; ++i) {
-            const bool by_group = i < 4 || i == 6 || i == 7 || (i >= 12 && i < 16);
-            mbar_init(smem_u32(&bars[i]), by_group ? 128 : 1);
+        for (int i = 0; i < 22; ++i) {
+            const bool by_group = i < 4 || i == 6 || i == 7 || (i >= 12 && i < 16) || i >= 20;
+            mbar_init(smem_u32(&bars[i]), by_group ? 128 : i == 18 ? 2 : 1);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1257,126 +1264,133 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                 st = end;
                 if (st < total) next_segment(a, segment);
             }
+        } else if (warp == 1) {
+            const int scales_per_page = LLMB_PAGE >> a.block_shift, alike = a.block_shift >= 4 ? 15 : 0;
+            auto copy = [&](unsigned char* to, const signed char* from, uint64_t* bar, const int (&pages)[STEP_PAGES]) {
+                if (elect_one()) {
+                    mbar_expect_tx(smem_u32(bar), (pages[1] >= 0 ? 2 : 1) * LLMB_PAGE * HD);
+#pragma unroll
+                    for (int i = 0; i < STEP_PAGES; ++i)
+                        if (pages[i] >= 0)
+                            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                             smem_u32(to + i * LLMB_PAGE * HD)), "l"(from + (size_t)pages[i] * LLMB_PAGE * HD), "r"(LLMB_PAGE * HD), "r"(smem_u32(bar)) : "memory");
+                }
+                __syncwarp();
+            };
+            bool ok = true;
+            for (int st = 0; st < total && ok;) {
+                int skip, count;
+                share_of(segment, skip, count);
+                const int* table = a.block_table + (size_t)segment.seq * a.table_stride;
+                int value_top = 0;                             // the largest exponent of the segment's values so far
+                const int end = st + count;
+                int next[STEP_PAGES];                          // the next step's page numbers are on their way
+                auto look_up = [&](int i) {
+#pragma unroll
+                    for (int k = 0; k < STEP_PAGES; ++k) {
+                        const int place = i * STEP_PAGES + k;
+                        next[k] = place < segment.pages ? page_at(a, table, segment.first_page + place, status) * a.n_kv_heads + segment.head : -1;
+                    }
+                };
+                look_up(skip);
+                for (int i = skip; st < end && ok; ++st, ++i) {
+                    const int pages[STEP_PAGES] = {next[0], next[1]};
+                    uint32_t ks[4], vs[4];                     // the scales of positions lane + 32 j of the step
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int page = pages[j >> 1], block = ((j & 1) * 32 + lane) >> a.block_shift;
+                        ks[j] = page >= 0 ? __float_as_uint(a.key_scales[(size_t)page * scales_per_page + block]) : 0u;
+                        vs[j] = page >= 0 ? __float_as_uint(a.value_scales[(size_t)page * scales_per_page + block]) : 0u;
+                    }
+                    if (st + 1 < end) look_up(i + 1);
+                    ok = st == 0 || mbar_wait_warp(smem_u32(&raw_empty[0]), (st - 1) & 1, abort_flag, status, 43);
+                    if (!ok) break;
+                    copy(raw_k, a.keys, &raw_full[0], pages);
+                    // scales from the largest of those that are seen
+                    const int key0 = (segment.first_page + i * STEP_PAGES) * LLMB_PAGE;
+                    StepInfo& info = infos[st % INFOS];
+                    uint32_t bad[4];
+                    int ke = 0, ve[STEP_PAGES] = {0, 0};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int nearest = key0 + ((lane + 32 * j) & ~alike);
+                        const bool seen = nearest <= segment.limit && nearest + alike >= segment.low;
+                        const uint32_t k = seen ? ks[j] : 0u, v = seen ? vs[j] : 0u;
+                        const bool none = (k & 0x7fffffffu) >= NOT_FINITE || (v & 0x7fffffffu) >= NOT_FINITE;
+                        if (!none && ((k | v) & 0x807fffffu)) report(status, NOT_A_POWER);
+                        bad[j] = __ballot_sync(0xffffffffu, none);
+                        ks[j] = none ? 0u : k >> 23 & 0xffu;
+                        vs[j] = none ? 0u : v >> 23 & 0xffu;
+                        ke = max(ke, (int)ks[j]);
+                        ve[j >> 1] = max(ve[j >> 1], (int)vs[j]);
+                    }
+                    ke = __reduce_max_sync(0xffffffffu, ke);
+#pragma unroll
+                    for (int k = 0; k < STEP_PAGES; ++k) {
+                        ve[k] = __reduce_max_sync(0xffffffffu, ve[k]);
+                        value_top = max(value_top, ve[k]);
+                        ve[k] = max(ve[k], value_top - VALUE_SPAN);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        info.packed[lane + 32 * j] = (ks[j] ? f16_power((int)ks[j] - ke + SCALE_UP) : 0u) | ((vs[j] ? f16_power((int)vs[j] - ve[j >> 1] + SCALE_UP) : 0u) << 16);
+                    if (lane == 0) {
+                        info.k_unit = __uint_as_float((uint32_t)max(ke - SCALE_UP, 1) << 23);
+                        info.v_unit[0] = (float)(ve[0] - 127);
+                        info.v_unit[1] = (float)(ve[1] - 127);
+                        info.any_bad = bad[0] | bad[1] | bad[2] | bad[3];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) info.bad[j] = bad[j];
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&raw_full[0]));
+                    ok = st == 0 || mbar_wait_warp(smem_u32(&raw_empty[1]), (st - 1) & 1, abort_flag, status, 44);
+                    if (!ok) break;
+                    copy(raw_v, a.values, &raw_full[1], pages);
+                }
+                if (st < total && ok) next_segment(a, segment);
+            }
         }
     } else if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_WIDEN));
         constexpr int LANES = HD / 16, RPP = 128 / LANES, PASSES = STEP / RPP;        // lanes of a row, rows of a pass
-        const int t = threadIdx.x & 127, wq = warp & 3, c = t % LANES, row_in = t / LANES;
-        const int scales_per_page = LLMB_PAGE >> a.block_shift;
-        uint4 raw_k[PASSES], raw_v[PASSES];
-        uint32_t ks[4], vs[4];                                 // the scales of positions lane + 32 j of the step
-        // What is asked for: step `asked` of the block's; its pages' numbers are on their way.
-        Segment ahead = segment;
-        int asked = 0, begun, count, pages_ahead[STEP_PAGES];  // begun: the step that `ahead` begins with
-        int skip;
-        share_of(ahead, skip, count);
-        begun = 0;
-        auto look_up = [&]() {
-            if (asked >= total) return;
-            if (asked == begun + count) {
-                begun += count;
-                next_segment(a, ahead);
-                share_of(ahead, skip, count);
-            }
-            const int* table = a.block_table + (size_t)ahead.seq * a.table_stride;
-            const int place = (skip + asked - begun) * STEP_PAGES;
-#pragma unroll
-            for (int i = 0; i < STEP_PAGES; ++i)
-                pages_ahead[i] = place + i < ahead.pages ? page_at(a, table, ahead.first_page + place + i, status) * a.n_kv_heads + ahead.head : -1;
-        };
-        auto fetch = [&](uint4 (&raw)[PASSES], const signed char* cache) {
-#pragma unroll
-            for (int i = 0; i < PASSES; ++i) {
-                const int row = i * RPP + row_in, page = pages_ahead[i * RPP / LLMB_PAGE];
-                raw[i] = page >= 0 ? *reinterpret_cast<const uint4*>(cache + ((size_t)page * LLMB_PAGE + row % LLMB_PAGE) * HD + c * 16) : make_uint4(0u, 0u, 0u, 0u);
-            }
-        };
-        auto fetch_scales = [&]() {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int page = pages_ahead[j >> 1], block = ((j & 1) * 32 + lane) >> a.block_shift;
-                ks[j] = page >= 0 ? __float_as_uint(a.key_scales[(size_t)page * scales_per_page + block]) : 0u;
-                vs[j] = page >= 0 ? __float_as_uint(a.value_scales[(size_t)page * scales_per_page + block]) : 0u;
-            }
-        };
-        // a step's rows to shared memory, times their scales
-        auto store = [&](unsigned char* to, const uint4 (&raw)[PASSES], const uint32_t (&packed)[4], uint32_t which) {
-#pragma unroll
-            for (int i = 0; i < PASSES; ++i) {
-                const int row = i * RPP + row_in, from = (i * RPP) % 32 + wq * (32 / LANES) + lane / LANES;
-                const uint32_t s = __byte_perm(__shfl_sync(0xffffffffu, packed[i * RPP / 32], from), 0, which);
-                uint4 low, high;
-                widen16(raw[i], s, low, high);
-                unsigned char* at = to + (c >> 2) * STEP_PIECE + row * 128;
-                const int chunk = 2 * (c & 3), flip = c >> 2;  // (lanes of the second piece write their halves the other way round: other banks)
-                *reinterpret_cast<uint4*>(at + (((chunk + flip) ^ (row & 7)) << 4)) = flip ? high : low;
-                *reinterpret_cast<uint4*>(at + (((chunk + 1 - flip) ^ (row & 7)) << 4)) = flip ? low : high;
-            }
-        };
-        look_up();
-        fetch(raw_k, a.keys);
-        fetch_scales();
-        fetch(raw_v, a.values);
-        int value_top = 0;                                     // the largest exponent of the segment's values so far
+        const int t = threadIdx.x & 127, c = t % LANES, row_in = t / LANES;
+        const int chunk = 2 * (c & 3), flip = c >> 2;          // (lanes of the second piece write their halves the other way round: other banks)
         bool ok = true;
-        for (int st = 0; st < total && ok; ++st) {
-            const int b = st & 1;
-            // the step's scales from the largest of those that are seen
-            const Segment& of = ahead;                         // (asked == st here: the look-up for the next step comes below)
-            if (st == begun) value_top = 0;
-            const int alike = a.block_shift >= 4 ? 15 : 0, key0 = (of.first_page + (skip + st - begun) * STEP_PAGES) * LLMB_PAGE;
-            uint32_t packed[4], bad[4];
-            int ke = 0, ve[STEP_PAGES] = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int nearest = key0 + ((lane + 32 * j) & ~alike);
-                const bool seen = nearest <= of.limit && nearest + alike >= of.low;
-                const uint32_t k = seen ? ks[j] : 0u, v = seen ? vs[j] : 0u;
-                const bool none = (k & 0x7fffffffu) >= NOT_FINITE || (v & 0x7fffffffu) >= NOT_FINITE;
-                if (!none && ((k | v) & 0x807fffffu)) report(status, NOT_A_POWER);
-                bad[j] = __ballot_sync(0xffffffffu, none);
-                ks[j] = none ? 0u : k >> 23;
-                vs[j] = none ? 0u : v >> 23;
-                ke = max(ke, (int)ks[j]);
-                ve[j >> 1] = max(ve[j >> 1], (int)vs[j]);
-            }
-            ke = __reduce_max_sync(0xffffffffu, ke);
-#pragma unroll
-            for (int i = 0; i < STEP_PAGES; ++i) {
-                ve[i] = __reduce_max_sync(0xffffffffu, ve[i]);
-                value_top = max(value_top, ve[i]);
-                ve[i] = max(ve[i], value_top - VALUE_SPAN);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                packed[j] = (ks[j] ? f16_power((int)(ks[j] & 0xffu) - ke + SCALE_UP) : 0u) |
-                            ((vs[j] ? f16_power((int)(vs[j] & 0xffu) - ve[j >> 1] + SCALE_UP) : 0u) << 16);
-            if (t == 0) {
-                StepInfo& info = infos[st % INFOS];
-                info.k_unit = __uint_as_float((uint32_t)max(ke - SCALE_UP, 1) << 23);
-                info.v_unit[0] = (float)(ve[0] - 127);
-                info.v_unit[1] = (float)(ve[1] - 127);
-                info.any_bad = bad[0] | bad[1] | bad[2] | bad[3];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) info.bad[j] = bad[j];
-            }
-            ++asked;
-            look_up();
-            ok = st < 2 || mbar_wait_warp(smem_u32(&k_empty[b]), ((st >> 1) - 1) & 1, abort_flag, status, 31);
+        for (int i = 0; i < 2 * total && ok; ++i) {            // keys and values in turn
+            const int st = i >> 1, which = i & 1, b = st & 1;
+            uint64_t* full = bars + 2 + 4 * which + b;         // (k_full, v_full and their like)
+            uint64_t* empty = bars + 4 + 4 * which + b;
+            const uint32_t* packed = infos[st % INFOS].packed;
+            const unsigned char* raw = (which ? raw_v : raw_k) + c * 16;
+            unsigned char* to = (which ? v_tile : k_tile) + b * STEP_BYTES + (c >> 2) * STEP_PIECE;
+            const uint32_t select = which ? 0x3232u : 0x1010u;
+            ok = mbar_wait_warp(smem_u32(&raw_full[which]), st & 1, abort_flag, status, 41) &&
+                 (st < 2 || mbar_wait_warp(smem_u32(empty), ((st >> 1) - 1) & 1, abort_flag, status, 31));
             if (!ok) break;
-            store(k_tile + b * STEP_BYTES, raw_k, packed, 0x1010);
-            fence_async_shared();
-            mbar_arrive(smem_u32(&k_full[b]));
-            if (st + 1 < total) {
-                fetch(raw_k, a.keys);
-                fetch_scales();
+            // rows to the operands' place, times their scales
+#pragma unroll 1
+            for (int i0 = 0; i0 < PASSES; i0 += 4) {
+                uint4 x[4];
+                uint32_t s[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int row = (i0 + j) * RPP + row_in;
+                    x[j] = *reinterpret_cast<const uint4*>(raw + row * HD);
+                    s[j] = __byte_perm(packed[row], 0, select);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int row = (i0 + j) * RPP + row_in;
+                    uint4 low, high;
+                    widen16(x[j], s[j], low, high);
+                    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk + flip) ^ (row & 7)) << 4)) = flip ? high : low;
+                    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk + 1 - flip) ^ (row & 7)) << 4)) = flip ? low : high;
+                }
             }
-            ok = st < 2 || mbar_wait_warp(smem_u32(&v_empty[b]), ((st >> 1) - 1) & 1, abort_flag, status, 32);
-            if (!ok) break;
-            store(v_tile + b * STEP_BYTES, raw_v, packed, 0x3232);
+            mbar_arrive(smem_u32(&raw_empty[which]));          // the bytes' room is free
             fence_async_shared();
-            mbar_arrive(smem_u32(&v_full[b]));
-            if (st + 1 < total) fetch(raw_v, a.values);
+            mbar_arrive(smem_u32(full));
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
@@ -1395,7 +1409,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                 const bool valid = r < tile_rows, idle = quarter * 32 >= tile_rows;      // idle: a warp without rows (its lanes' weights reach nobody's result)
                 const int at = segment.row0 + tile * TILE_ROWS + (valid ? r : 0);
                 const int token = segment.span.first_token + at / share, head = segment.head * share + at % share;
-                const int my_pos = valid ? segment.span.first_pos + at / share : -1, my_first = first_seen(a, my_pos);
+                // (lanes without a row have queries of zero and see everything: nothing is masked for them)
+                const int my_pos = valid ? segment.span.first_pos + at / share : 0x3fffffff, my_first = valid ? first_seen(a, my_pos) : 0;
                 float row_scale;
                 {   // the row's queries as fp16, their largest at 2^14
                     const uint4* q = reinterpret_cast<const uint4*>(behind_wait(static_cast<const __nv_bfloat16*>(a.q)) + (size_t)token * a.q_stride + (size_t)head * HD);
@@ -1435,56 +1450,46 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                         continue;
                     }
                     const StepInfo& info = infos[i % INFOS];
-                    const float c = fmaxf(row_scale * info.k_unit, 1.1754944e-38f), v_unit0 = info.v_unit[0], v_unit1 = info.v_unit[1];
+                    const float c = fmaxf(row_scale * info.k_unit, 1.1754944e-38f);
                     const int key0 = (segment.first_page + (skip + i - st) * STEP_PAGES) * LLMB_PAGE;
                     const int last = my_pos - key0, first = my_first - key0;       // the positions of the step that the row sees
-                    uint32_t r0s[32], r1s[32], r2s[32], r3s[32];
-                    // the second half of the scores comes while the first one's maximum is taken
-                    tmem_ld32_start(s_addr, r0s);
-                    tmem_ld32_start(s_addr + 32, r1s);
-                    tmem_ld32_wait(r0s);
-                    tmem_ld32_wait(r1s);
-                    tmem_ld32_start(s_addr + 64, r2s);
-                    tmem_ld32_start(s_addr + 96, r3s);
-                    auto mask = [&](uint32_t (&x)[32], int from) {
-                        if (info.any_bad) {
-                            const uint32_t bad = info.bad[from >> 5];
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (bad >> j & 1) x[j] = 0x7fffffffu;
-                        }
-                        if (last < from + 31) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (j + from > last) x[j] = __float_as_uint(-INFINITY);
-                        }
-                        if (first > from) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (j + from < first) x[j] = __float_as_uint(-INFINITY);
-                        }
-                    };
-                    mask(r0s, 0);
-                    mask(r1s, 32);
+                    const bool masked = __any_sync(0xffffffffu, last < STEP - 1 || first > 0) || info.any_bad;
+                    // Scores are read twice, a page at a time, by loops that are not unrolled: kept in registers, with all four quarters' code in a
+                    // row, warps spent a fifth of their time waiting for instructions.
                     float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll 1
+                    for (int half = 0; half < STEP_PAGES; ++half) {
+                        uint32_t x0[32], x1[32];
+                        tmem_ld32_start(s_addr + half * LLMB_PAGE, x0);
+                        tmem_ld32_start(s_addr + half * LLMB_PAGE + 32, x1);
+                        tmem_ld32_wait(x0);
+                        tmem_ld32_wait(x1);
+                        if (masked) {                          // what the row does not see: -inf, in tensor memory too
+                            auto mask = [&](uint32_t (&x)[32], int from) {
+                                const uint32_t bad = info.bad[from >> 5];
+                                const int most = last - from, least = first - from;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        top0 = max3(top0, __uint_as_float(r0s[j]), __uint_as_float(r0s[j + 1]));
-                        top1 = max3(top1, __uint_as_float(r1s[j]), __uint_as_float(r1s[j + 1]));
-                    }
-                    tmem_ld32_wait(r2s);
-                    tmem_ld32_wait(r3s);
-                    mask(r2s, 64);
-                    mask(r3s, 96);
-                    top0 = fmaxf(top0, top1) * c;
-                    float top2 = -INFINITY, top3 = -INFINITY;
+                                for (int j = 0; j < 32; ++j) {
+                                    if (bad >> j & 1) x[j] = 0x7fffffffu;
+                                    if (j > most || j < least) x[j] = __float_as_uint(-INFINITY);
+                                }
+                                tmem_st32(s_addr + from, x);
+                            };
+                            mask(x0, half * LLMB_PAGE);
+                            mask(x1, half * LLMB_PAGE + 32);
+                            tmem_st_wait();
+                        }
+                        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        top2 = max3(top2, __uint_as_float(r2s[j]), __uint_as_float(r2s[j + 1]));
-                        top3 = max3(top3, __uint_as_float(r3s[j]), __uint_as_float(r3s[j + 1]));
+                        for (int j = 0; j < 32; j += 2) {
+                            t0 = max3(t0, __uint_as_float(x0[j]), __uint_as_float(x0[j + 1]));
+                            t1 = max3(t1, __uint_as_float(x1[j]), __uint_as_float(x1[j + 1]));
+                        }
+                        t0 = fmaxf(t0, t1) * c;
+                        if (half == 0) top0 = t0;
+                        else top1 = t0;
                     }
-                    top2 = fmaxf(top2, top3) * c;
-                    const float new_max = max3(run_max, top0, top2), candidate = fmaxf(top0 + v_unit0, top2 + v_unit1);
+                    const float new_max = max3(run_max, top0, top1), candidate = fmaxf(top0 + info.v_unit[0], top1 + info.v_unit[1]);
                     // (a row that has seen no position yet keeps -inf, and all its weights are zero)
                     const bool move = candidate - ref > 8.f;
                     const float new_ref = move ? candidate : ref;
@@ -1502,42 +1507,41 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                         }
                     }
                     const uint64_t scale2 = pair_of(c, c);
-                    uint64_t shift2 = pair_of(lift + v_unit0, lift + v_unit0), add = pair_of(0u, 0u);
-                    // what the page's weights are lifted by, taken off their sum
-                    auto page_sum = [&](float v_unit) {
-                        float lo, hi;
-                        unpair(add, lo, hi);
-                        return none ? lo + hi : (lo + hi) * fast_exp2(-lift - v_unit - new_max);
-                    };
-                    auto to_weights = [&](const uint32_t (&x)[32], int col) {
-                        uint32_t packed[16];
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            float p0, p1;
-                            unpair(fma2(pair_of(x[j], x[j + 1]), scale2, shift2), p0, p1);
-                            p0 = fast_exp2(p0);
-                            p1 = fast_exp2(p1);
-                            add = add2(add, pair_of(p0, p1));
-                            packed[j >> 1] = pack_f16(p0, p1);
-                        }
-                        tmem_st16(s_addr + (col >> 1), packed);
-                    };
-                    to_weights(r0s, 0);
-                    to_weights(r1s, 32);
-                    tmem_st_wait();
-                    tcgen05_fence_before();
-                    mbar_arrive(smem_u32(&p_full[2 * tile]));
-                    run_sum = run_sum * ratio(run_max, new_max) + page_sum(v_unit0);
-                    shift2 = pair_of(lift + v_unit1, lift + v_unit1);
-                    add = pair_of(0u, 0u);
-                    to_weights(r2s, 64);
-                    to_weights(r3s, 96);
-                    run_sum += page_sum(v_unit1);
+                    run_sum *= ratio(run_max, new_max);
                     run_max = new_max;
                     ref = new_ref;
-                    tmem_st_wait();
-                    tcgen05_fence_before();
-                    mbar_arrive(smem_u32(&p_full[2 * tile + 1]));
+#pragma unroll 1
+                    for (int half = 0; half < STEP_PAGES; ++half) {
+                        const float shift = lift + info.v_unit[half];
+                        const uint64_t shift2 = pair_of(shift, shift);
+                        uint64_t add = pair_of(0u, 0u);
+                        uint32_t x0[32], x1[32];
+                        tmem_ld32_start(s_addr + half * LLMB_PAGE, x0);
+                        tmem_ld32_start(s_addr + half * LLMB_PAGE + 32, x1);
+                        tmem_ld32_wait(x0);
+                        tmem_ld32_wait(x1);
+                        auto to_weights = [&](const uint32_t (&x)[32], int col) {
+                            uint32_t packed[16];
+#pragma unroll
+                            for (int j = 0; j < 32; j += 2) {
+                                float p0, p1;
+                                unpair(fma2(pair_of(x[j], x[j + 1]), scale2, shift2), p0, p1);
+                                p0 = fast_exp2(p0);
+                                p1 = fast_exp2(p1);
+                                add = add2(add, pair_of(p0, p1));
+                                packed[j >> 1] = pack_f16(p0, p1);
+                            }
+                            tmem_st16(s_addr + (col >> 1), packed);
+                        };
+                        to_weights(x0, half * LLMB_PAGE);
+                        to_weights(x1, half * LLMB_PAGE + 32);
+                        tmem_st_wait();
+                        tcgen05_fence_before();
+                        mbar_arrive(smem_u32(&p_full[2 * tile + half]));
+                        float lo, hi;                          // what the page's weights are lifted by is taken off their sum
+                        unpair(add, lo, hi);
+                        run_sum += none ? lo + hi : (lo + hi) * fast_exp2(-shift - new_max);
+                    }
                 }
                 // the result, or the block's part of it: by way of the queries' room, a warp's rows at a time, so that rows are written as a whole
                 ok = ok && mbar_wait_warp(smem_u32(&o_full[tile]), segments++ & 1, abort_flag, status, 40);
@@ -1599,7 +1603,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
 
     tcgen05_fence_before();
     __syncthreads();
-    if (*abort_flag) {                                         // a wait ran out: products in flight get their time before the block leaves
+    if (*abort_flag) {                                         // a wait ran out: copies and products in flight get their time before the block leaves
         for (int i = 0; i < 100; ++i) __nanosleep(10000);
         __syncthreads();
     }
@@ -1914,8 +1918,8 @@ int launch_few(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
 template <int HD>
 int launch_wide(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
     // (more than half of an SM's shared memory for the smaller head size too: tensor memory has room for one block)
-    constexpr size_t need = (HD / 64) * (2 * TILE_PIECE + 4 * STEP_PIECE) + INFOS * sizeof(StepInfo) + 19 * 8, bytes = need < 120 * 1024 ? 120 * 1024 : need;
-    static_assert(bytes + 1024 <= 227 * 1024, "one block an SM");
+    constexpr size_t need = (HD / 64) * (2 * TILE_PIECE + 4 * STEP_PIECE) + 2 * STEP * HD + INFOS * sizeof(StepInfo) + 23 * 8, bytes = need < 120 * 1024 ? 120 * 1024 : need;
+    static_assert(bytes <= 227 * 1024, "one block an SM");
     static bool done[MAX_DEVICES] = {};
     static bool checked = false;
     if (!checked) {                              // (its softmax warps would wait for registers that are not there)
