@@ -105,7 +105,8 @@ __device__ __forceinline__ int head_of(const Item& w, int r, int share) { return
 __device__ __forceinline__ int position_of(const Item& w, int r, int share) { return w.first_pos + (w.row0 + r) / share; }
 // the page of a place in the table; one that there is not is reported, and page 0 read in its place
 __device__ __forceinline__ int page_at(const Args& a, const int* pages, int logical, int* status) {
-    const int page = pages[logical % a.ring_pages];
+    if (logical >= a.ring_pages) logical %= a.ring_pages;      // (a division only where the ring has been gone round)
+    const int page = pages[logical];
     if ((unsigned)page < (unsigned)a.n_pages) return page;
     report(status, OUT_OF_RANGE);
     return 0;
@@ -344,29 +345,30 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_int8_simt_kernel(const
 //
 //   scores^T [16 positions, rows] = K [16, D] Q^T        result^T [16 columns, rows] += V^T [16, positions] P^T
 //
-// fp16 holds 2^-24 to 65504. So queries are divided by the power of two that brings their row's largest to 2^14; scales count from the largest of the 32
+// fp16 holds 2^-24 to 65504. So queries are divided by the power of two that brings their row's largest to 2^14; scales count from the largest of the
 // positions that a warp works on (2^5 for that one, so that 29 powers of two fit); and a row keeps, beside the running maximum m of its scores, a
 // reference R of score plus exponent of the values' scale, to which its weights w = 2^(score - m) 2^(m + E - R + 14) and its sums refer: weights and
 // values that span more than fp16 does are lost only where they are nothing beside what the row has. All sums are in 32 bits.
 //
 // The pages of all (sequence, key head) pairs, one after the other, are dealt out to the blocks that the SMs hold at once in ranges of
 // equal length, so a block's range covers the end of one pair, some whole ones, and the beginning of another. Pairs that one block has done as a whole are
-// finished there, of the others each block leaves a part. A block has four warps, each with a ring of units of 32 positions of its own (TMA, rows
+// finished there, of the others each block leaves a part. A block has four warps, each with a ring of units of its own, 32 positions or 64 (TMA, rows
 // swizzled so that both the reads of keys, four lanes a row, and those of values, eight columns a lane, touch all banks once), which runs on over the
 // ends of pairs; warps meet where a pair ends.
 
-constexpr int FEW_THREADS = 128, FEW_WARPS = 4, UNIT = 32;      // UNIT: positions that a warp works on at a time
+constexpr int FEW_THREADS = 128, FEW_WARPS = 4;
 constexpr int FEW_ROWS = 16;
 constexpr int SCALE_UP = 5, WEIGHT_UP = 14;                    // powers of two that the largest scale and weight are lifted to
 
+template <int HD> constexpr int UNIT = HD == 64 ? 64 : 32;      // positions that a warp works on at a time
 template <int HD, int NT> struct Few {
-    static constexpr int TILE = UNIT * HD;                      // bytes of a unit's keys
-    static constexpr int STAGES = HD == 64 ? 4 : 2;
+    static constexpr int TILE = UNIT<HD> * HD;                  // bytes of a unit's keys
+    static constexpr int STAGES = 2;
     static constexpr int BLOCKS = NT == 1 ? 3 : 2;              // of an SM
     static constexpr int LD = HD + 4;
     static constexpr int RING = FEW_WARPS * STAGES * 2 * TILE;
     static constexpr int MERGE = 2 * (8 * NT * LD + 8 * NT * 4) * 4;            // two warps' rows, and their references
-    static constexpr int SCALES = FEW_WARPS * STAGES * 2 * UNIT * 4;
+    static constexpr int SCALES = FEW_WARPS * STAGES * 2 * UNIT<HD> * 4;
     static constexpr int BYTES = RING + MERGE + SCALES + FEW_WARPS * STAGES * 8 + 16;
     static_assert(BLOCKS * (BYTES + 1024) <= 227 * 1024, "blocks of an SM");
 };
@@ -412,8 +414,8 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 __device__ __forceinline__ void cp_async4(void* smem, const void* global) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_u32(smem)), "l"(global));
 }
-// 2^n as an fp16 number's bits, 0 below what it holds
-__device__ __forceinline__ uint32_t f16_power(int n) { return n >= -14 ? (uint32_t)(n + 15) << 10 : n >= -24 ? 1u << (n + 24) : 0u; }
+// 2^(exponent - most + SCALE_UP) for the exponents of two scales, 0 for those without one, as fp16 numbers (0 below what it holds)
+__device__ __forceinline__ float power_of(int exponent, int most) { return exponent ? __uint_as_float((uint32_t)max(exponent - most + SCALE_UP + 127, 0) << 23) : 0.f; }
 // 2^(a - b) for references that may be -inf (of nothing)
 __device__ __forceinline__ float ratio(float a, float b) { return a == -INFINITY ? 0.f : fast_exp2(a - b); }
 
@@ -494,13 +496,13 @@ template <int HD, int NT>
 __global__ void __launch_bounds__(FEW_THREADS, Few<HD, NT>::BLOCKS)
 attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a, int* status) {
     using F = Few<HD, NT>;
-    constexpr int TILE = F::TILE, STAGES = F::STAGES, LD = F::LD, DIMS = HD / 8, CHUNKS = HD / 64;     // DIMS: a lane's columns of the result
+    constexpr int U = UNIT<HD>, TILE = F::TILE, STAGES = F::STAGES, LD = F::LD, DIMS = HD / 8, CHUNKS = HD / 64;     // DIMS: a lane's columns of the result
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* base = smem_raw;                            // (its alignment is the swizzle's)
     const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     unsigned char* ring = base + warp * STAGES * 2 * TILE;
     float* merge = reinterpret_cast<float*>(base + F::RING);                     // [2] a warp's rows [8 NT][LD], then (m, R, l, -) of each
-    float* scales = reinterpret_cast<float*>(base + F::RING + F::MERGE) + warp * STAGES * 2 * UNIT;         // of this warp: [stage][2][32]
+    float* scales = reinterpret_cast<float*>(base + F::RING + F::MERGE) + warp * STAGES * 2 * U;            // of this warp: [stage][2][U]
     uint64_t* full = reinterpret_cast<uint64_t*>(base + F::RING + F::MERGE + F::SCALES) + warp * STAGES;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(base + F::RING + F::MERGE + F::SCALES + FEW_WARPS * STAGES * 8);
 
@@ -542,25 +544,33 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         if (r0 >= r1) return;
         pair = pair_at(a, r0, most_tokens, lane);
     }
-    const int units = (int)(r1 - r0) * (LLMB_PAGE / UNIT);
+    constexpr int PER_PAGE = LLMB_PAGE / U, TILES = U / 16;
+    const int units = (int)(r1 - r0) * PER_PAGE;
     const __nv_bfloat16* q_all = behind_wait(static_cast<const __nv_bfloat16*>(a.q));
     const int scales_per_page = LLMB_PAGE >> a.block_shift;
 
-    // What is asked for: unit `asked` of the range, of pair `ahead`; its page's number is on its way.
+    // What is asked for: unit `asked` of the range, of pair `ahead` (up to page `ahead_end` of the range); its page's number is on its way.
     Pair ahead = pair;
-    int asked = warp, page_ahead = 0;
+    int asked = warp, page_ahead = 0, ahead_end = (int)(pair.start - r0) + pair.span.pages;
     auto look_up = [&]() {
         if (asked >= units) return;
-        const long long at = r0 + asked / (LLMB_PAGE / UNIT);
-        while (at >= ahead.start + ahead.span.pages) next_pair(a, ahead, most_tokens);
-        page_ahead = page_at(a, a.block_table + (size_t)ahead.seq * a.table_stride, ahead.span.first + (int)(at - ahead.start), status);
+        const int at = asked / PER_PAGE;
+        while (at >= ahead_end) {
+            next_pair(a, ahead, most_tokens);
+            ahead_end += ahead.span.pages;
+        }
+        page_ahead = page_at(a, a.block_table + (size_t)ahead.seq * a.table_stride, ahead.span.first + ahead.span.pages - (ahead_end - at), status);
     };
     auto ask = [&](int stage) {
         if (asked < units) {
-            const int head_row = page_ahead * a.n_kv_heads + ahead.head, row = asked % (LLMB_PAGE / UNIT) * UNIT;
-            const size_t at = (size_t)head_row * scales_per_page + ((row + lane) >> a.block_shift);
-            cp_async4(scales + stage * 2 * UNIT + lane, a.key_scales + at);
-            cp_async4(scales + stage * 2 * UNIT + UNIT + lane, a.value_scales + at);
+            const int head_row = page_ahead * a.n_kv_heads + ahead.head, row = asked % PER_PAGE * U;
+            float* to_scales = scales + stage * 2 * U + lane;
+#pragma unroll
+            for (int k = 0; k < U; k += 32) {
+                const int at = head_row * scales_per_page + ((row + lane + k) >> a.block_shift);
+                cp_async4(to_scales + k, a.key_scales + at);
+                cp_async4(to_scales + U + k, a.value_scales + at);
+            }
             if (elect_one()) {
                 const uint32_t bar = smem_u32(&full[stage]), to = smem_u32(ring + stage * 2 * TILE);
                 mbar_expect_tx(bar, 2 * TILE);
@@ -580,12 +590,15 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
     int done = warp, stage = 0;                                // the next unit, and where it arrives
     uint32_t phase = 0;
     bool ok = true;
+    const int my_row = row_of<HD>(g);
     for (;;) {
         // ---- the pair's rows
         const Span& span = pair.span;
         const int n_rows = span.n_new * share;
-        const long long pair_end = pair.start + span.pages, end = pair_end < r1 ? pair_end : r1;
-        const int limit = span.first_pos + span.n_new - 1, low = first_seen(a, span.first_pos);       // positions that a row sees at all
+        const int pair_begin = (int)(pair.start - r0), pair_end = pair_begin + span.pages, range_end = (int)(r1 - r0);      // in pages of the range
+        const int end = min(pair_end, range_end);
+        const int limit = span.first_pos + span.n_new - 1, low = first_seen(a, span.first_pos);       // positions that a row sees at all,
+        const int all_to = span.first_pos, all_from = first_seen(a, limit);                           // and that all rows see
         uint32_t qb[NT][HD / 16][2];
         float row_scale[NT][2];                                // of rows 2t and 2t + 1 of each tile
         int pos[NT][2];
@@ -625,7 +638,8 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
             for (int j = 0; j < 2; ++j) {
                 const int of = n * 8 + 2 * t + j, e = __shfl_sync(0xffffffffu, exponent, (2 * t + j) * 4);
                 row_scale[n][j] = a.scale_log2 * __uint_as_float((uint32_t)(max(e - 14 + 127, 1)) << 23);
-                pos[n][j] = of < n_rows ? span.first_pos + of / share : -1;
+                // (rows that are none have queries of zero and see everything: nothing is masked for them)
+                pos[n][j] = of < n_rows ? span.first_pos + of / share : limit;
             }
         }
         float acc[NT][DIMS / 2][4], m[NT][2], ref[NT][2], sum[NT][2];
@@ -642,42 +656,51 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
             }
         }
         // ---- its units
-        for (; done < units; done += FEW_WARPS) {
-            const long long at = r0 + done / (LLMB_PAGE / UNIT);
-            if (at >= end) break;
-            const int key0 = (span.first + (int)(at - pair.start)) * LLMB_PAGE + done % (LLMB_PAGE / UNIT) * UNIT;
+        for (; done < end * PER_PAGE; done += FEW_WARPS) {
+            const int key0 = (span.first + done / PER_PAGE - pair_begin) * LLMB_PAGE + done % PER_PAGE * U;
             ok = ok && mbar_wait_warp(smem_u32(&full[stage]), phase, abort_flag, status, 21);
             cp_async_wait<STAGES - 1>();
             __syncwarp();
-            if (ok && key0 <= limit && key0 + UNIT > low) {
+            if (ok && key0 <= limit && key0 + U > low) {
                 const unsigned char* k_tile = ring + stage * 2 * TILE;
                 const unsigned char* v_tile = k_tile + TILE;
                 // the unit's scales, a lane a position: the largest of those that are seen, then all as fp16 powers from it. (Blocks of 16 positions and
                 // more have one for all 16 of a tile, and it counts where any of these is seen.)
-                const int alike = a.block_shift >= 4 ? 15 : 0, nearest = key0 + (lane & ~alike);
-                const bool seen = nearest <= limit && nearest + alike >= low;
-                uint32_t ks = seen ? __float_as_uint(scales[stage * 2 * UNIT + lane]) : 0u, vs = seen ? __float_as_uint(scales[stage * 2 * UNIT + UNIT + lane]) : 0u;
-                const bool none = (ks & 0x7fffffffu) >= NOT_FINITE || (vs & 0x7fffffffu) >= NOT_FINITE;
-                if (!none && seen && ((ks | vs) & 0x807fffffu)) report(status, NOT_A_POWER);
-                const unsigned bad = __ballot_sync(0xffffffffu, none);
-                if (none) ks = vs = 0u;
-                const int ke = __reduce_max_sync(0xffffffffu, ks >> 23), ve = __reduce_max_sync(0xffffffffu, vs >> 23);
-                // (each lane's over its key's: fp16 scales, key's low, value's high)
-                uint32_t* packed = reinterpret_cast<uint32_t*>(scales + stage * 2 * UNIT);
-                packed[lane] = (ks ? f16_power((int)(ks >> 23) - ke + SCALE_UP) : 0u) | ((vs ? f16_power((int)(vs >> 23) - ve + SCALE_UP) : 0u) << 16);
+                const int alike = a.block_shift >= 4 ? 15 : 0;
+                uint32_t* packed = reinterpret_cast<uint32_t*>(scales + stage * 2 * U);       // (each lane's over its key's: key's low, value's high)
+                uint32_t ks[U / 32], vs[U / 32], bad[U / 32], any_bad = 0;
+                int ke = 0, ve = 0;
+#pragma unroll
+                for (int k = 0; k < U / 32; ++k) {
+                    const int nearest = key0 + ((lane + 32 * k) & ~alike);
+                    const bool seen = nearest <= limit && nearest + alike >= low;
+                    ks[k] = seen ? packed[lane + 32 * k] : 0u;
+                    vs[k] = seen ? packed[U + lane + 32 * k] : 0u;
+                    const bool none = max(ks[k] & 0x7fffffffu, vs[k] & 0x7fffffffu) >= NOT_FINITE;
+                    bad[k] = __ballot_sync(0xffffffffu, none);
+                    any_bad |= bad[k];
+                    if ((ks[k] | vs[k]) & 0x807fffffu && !none) report(status, NOT_A_POWER);
+                    ks[k] = none ? 0u : ks[k] >> 23 & 0xffu;
+                    vs[k] = none ? 0u : vs[k] >> 23 & 0xffu;
+                    ke = max(ke, (int)ks[k]);
+                    ve = max(ve, (int)vs[k]);
+                }
+                ke = __reduce_max_sync(0xffffffffu, ke);
+                ve = __reduce_max_sync(0xffffffffu, ve);
+#pragma unroll
+                for (int k = 0; k < U / 32; ++k) packed[lane + 32 * k] = pack_f16(power_of((int)ks[k], ke), power_of((int)vs[k], ve));
                 __syncwarp();
 
-                float s[2][NT][4];
+                float s[TILES][NT][4];
 #pragma unroll
-                for (int tile = 0; tile < 2; ++tile) {
+                for (int tile = 0; tile < TILES; ++tile) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) s[tile][n][k] = 0.f;
-                    uint32_t sa, sb;                           // of positions row_of(g) and 8 behind it
-                    const int row = tile * 16 + row_of<HD>(g);
-                    sa = packed[row];
-                    sb = a.block_shift >= 4 ? sa : packed[row + 8];
+                    const int row = tile * 16 + my_row;
+                    uint32_t sa = packed[row], sb = sa;        // of this position and the one 8 behind it
+                    if (a.block_shift < 4) sb = packed[row + 8];
                     sa = __byte_perm(sa, 0, 0x1010);
                     sb = __byte_perm(sb, 0, 0x1010);
                     const uint32_t oa = hmul2(sa, MINUS_1152), ob = hmul2(sb, MINUS_1152);
@@ -695,60 +718,78 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
                         }
                     }
                 }
+                if (key0 + U - 1 > all_to || key0 < all_from || any_bad) {        // some rows do not see all of the unit
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const int most = pos[n][j] - key0, least = first_seen(a, pos[n][j]) - key0;
+#pragma unroll
+                            for (int i = 0; i < 2 * TILES; ++i) {
+                                float& x = s[i >> 1][n][(i & 1) * 2 + j];
+                                const int at = my_row + 8 * i;
+                                if (bad[(8 * i) / 32] >> (at & 31) & 1) x = __uint_as_float(0x7fffffffu);
+                                if (at > most || at < least) x = -INFINITY;
+                            }
+                        }
+                }
                 const float k_unit = __uint_as_float((uint32_t)max(ke - SCALE_UP, 1) << 23);                  // what a step of the keys stands for
                 const float v_unit = (float)(ve - 127);
-                uint32_t pb[2][NT][2];                         // the weights, positions on the contracted side
+                float c[NT][2], top[NT][2];
                 bool moved = false;
-                float shrink[NT][2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float weight[2][4];
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const float c = row_scale[n][j] * k_unit;
-                        float x[4] = {s[0][n][j] * c, s[0][n][2 + j] * c, s[1][n][j] * c, s[1][n][2 + j] * c};
-                        const int first = first_seen(a, pos[n][j]);
+                        c[n][j] = fmaxf(row_scale[n][j] * k_unit, 1.1754944e-38f);
+                        float x = fmaxf(s[0][n][j], s[0][n][2 + j]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {          // positions row_of(g) + 8 i of the unit
-                            const int at_row = row_of<HD>(g) + 8 * i, key = key0 + at_row;
-                            if (bad >> at_row & 1) x[i] = __uint_as_float(0x7fffffffu);
-                            if (key > pos[n][j] || key < first) x[i] = -INFINITY;
-                        }
-                        float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        const float new_m = fmaxf(m[n][j], top), against = new_m == -INFINITY ? 0.f : new_m;
-                        const float new_ref = fmaxf(ref[n][j], top + v_unit), from = new_ref == -INFINITY ? 0.f : new_ref;
-                        shrink[n][j] = ratio(ref[n][j], from);
-                        moved |= new_ref != ref[n][j];
-                        const float lift = fast_exp2(fminf(against + v_unit - from + (float)WEIGHT_UP, 126.f));
-                        float add = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            x[i] = fast_exp2(x[i] - against);
-                            add += x[i];
-                            weight[i >> 1][(i & 1) * 2 + j] = x[i] * lift;
-                        }
-                        sum[n][j] = sum[n][j] * ratio(m[n][j], against) + add;         // of this lane's positions
-                        m[n][j] = new_m;
-                        ref[n][j] = new_ref;
+                        for (int tile = 1; tile < TILES; ++tile) x = max3(x, s[tile][n][j], s[tile][n][2 + j]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        top[n][j] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * c[n][j];
+                        moved |= top[n][j] > m[n][j] || top[n][j] + v_unit > ref[n][j];
                     }
-#pragma unroll
-                    for (int tile = 0; tile < 2; ++tile)
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) pb[tile][n][half] = transposed(pack_f16(weight[tile][2 * half], weight[tile][2 * half + 1]));
-                }
                 if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int i = 0; i < DIMS / 2; ++i)
+                        for (int j = 0; j < 2; ++j) {
+                            const float new_m = fmaxf(m[n][j], top[n][j]), new_ref = fmaxf(ref[n][j], top[n][j] + v_unit);
+                            sum[n][j] *= ratio(m[n][j], new_m);
+                            const float shrink = ratio(ref[n][j], new_ref);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) acc[n][i][k] *= shrink[n][k & 1];
+                            for (int i = 0; i < DIMS / 2; ++i) {
+                                acc[n][i][j] *= shrink;
+                                acc[n][i][2 + j] *= shrink;
+                            }
+                            m[n][j] = new_m;
+                            ref[n][j] = new_ref;
+                        }
+                }
+                uint32_t pb[TILES][NT][2];                     // the weights, positions on the contracted side
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float weight[TILES][4];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        // (a row that has seen nothing yet has references of -inf, and all its weights are zero)
+                        const float against = m[n][j] == -INFINITY ? 0.f : m[n][j], from = ref[n][j] == -INFINITY ? 0.f : ref[n][j];
+                        const float lift = fast_exp2(fminf(against + v_unit - from + (float)WEIGHT_UP, 126.f));
+#pragma unroll
+                        for (int i = 0; i < 2 * TILES; ++i) {
+                            const float p = fast_exp2(fmaf(s[i >> 1][n][(i & 1) * 2 + j], c[n][j], -against));
+                            sum[n][j] += p;                    // of this lane's positions
+                            weight[i >> 1][(i & 1) * 2 + j] = p * lift;
+                        }
+                    }
+#pragma unroll
+                    for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) pb[tile][n][half] = transposed(pack_f16(weight[tile][2 * half], weight[tile][2 * half + 1]));
                 }
 #pragma unroll
-                for (int tile = 0; tile < 2; ++tile) {
+                for (int tile = 0; tile < TILES; ++tile) {
                     // positions 2t, 2t + 1 of the products, and 8 behind them
                     const int row[2] = {tile * 16 + row_of<HD>(2 * t), tile * 16 + row_of<HD>(2 * t + 1)};
                     uint32_t s_low, s_high;
@@ -845,7 +886,7 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
             }
         }
         if (warp == 0) {
-            const bool whole = pair.start >= r0 && pair_end <= r1;
+            const bool whole = pair_begin >= 0 && pair_end <= range_end;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -873,7 +914,7 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
                     }
                 }
         }
-        if (end >= r1) break;
+        if (end >= range_end) break;
         next_pair(a, pair, most_tokens);
     }
     __syncthreads();
@@ -1022,17 +1063,30 @@ __device__ __forceinline__ Span wide_span(const Args& a, int seq) {
     if (s.n_new <= a.few_tokens) s.pages = 0;
     return s;
 }
-// The steps of all tiles of one of the sequence's key heads.
-__device__ __forceinline__ int steps_of(const Args& a, const Span& s) {
-    int sum = 0;
-    if (s.pages == 0) return 0;
-    Segment g;
-    g.span = s;
-    const int tiles = tiles_of(a, s);
-    for (g.tile = 0; g.tile < tiles; ++g.tile) {
-        place_tile(a, g);
-        sum += g.steps;
+// Steps of a key head's tiles, one after the other, without a division for each (with them a prompt of 32 tiles took a block 40,000 cycles to find
+// its place).
+struct TileWalk {
+    int tokens, rest;                // (tile * WIDE_ROWS) / share, and what is left
+    int tile, tiles;
+};
+__device__ __forceinline__ TileWalk walk_of(const Args& a, const Span& s) { return TileWalk{0, 0, 0, s.pages > 0 ? tiles_of(a, s) : 0}; }
+// the steps of the walk's tile; the walk goes on to the next
+__device__ __forceinline__ int walk_steps(const Args& a, const Span& s, TileWalk& w, int share, int tokens, int rest) {
+    const int low = first_seen(a, s.first_pos + w.tokens);
+    w.tokens += tokens;
+    w.rest += rest;
+    if (w.rest >= share) {
+        w.rest -= share;
+        ++w.tokens;
     }
+    const int last = ++w.tile == w.tiles ? s.n_new - 1 : w.rest ? w.tokens : w.tokens - 1;        // the tile's last token
+    return ((s.first_pos + last) / LLMB_PAGE - low / LLMB_PAGE) / STEP_PAGES + 1;
+}
+// The steps of the first `most` tiles of one of the sequence's key heads.
+__device__ __forceinline__ int steps_of(const Args& a, const Span& s, int most = 1 << 30) {
+    const int share = a.n_heads / a.n_kv_heads, tokens = WIDE_ROWS / share, rest = WIDE_ROWS - tokens * share;
+    int sum = 0;
+    for (TileWalk w = walk_of(a, s); w.tile < min(w.tiles, most);) sum += walk_steps(a, s, w, share, tokens, rest);
     return sum;
 }
 __device__ __forceinline__ long long all_steps(const Args& a, int lane) {
@@ -1060,11 +1114,15 @@ __device__ __forceinline__ Segment segment_at(const Args& a, long long at, int l
             g.start = before + (long long)(__shfl_sync(0xffffffffu, up, k) - steps) * a.n_kv_heads;
             g.head = (int)((at - g.start) / steps);
             g.start += (long long)g.head * steps;
-            for (g.tile = 0;; ++g.tile) {
-                place_tile(a, g);
-                if (at < g.start + g.steps) return g;
-                g.start += g.steps;
+            const int share = a.n_heads / a.n_kv_heads, tokens = WIDE_ROWS / share, rest = WIDE_ROWS - tokens * share;
+            for (TileWalk w = walk_of(a, g.span);;) {
+                g.tile = w.tile;
+                const int here = walk_steps(a, g.span, w, share, tokens, rest);
+                if (at < g.start + here) break;
+                g.start += here;
             }
+            place_tile(a, g);
+            return g;
         }
         before += (long long)__shfl_sync(0xffffffffu, up, 31) * a.n_kv_heads;
     }
@@ -1086,17 +1144,11 @@ __device__ __forceinline__ long long range_steps(const Args& a, long long all) {
     return per < a.wide_least ? a.wide_least : per;
 }
 
-// 16 bytes as 16 fp16 numbers times s, in their order
-__device__ __forceinline__ void widen16(const uint4& v, uint32_t s, uint4& low, uint4& high) {
-    const uint32_t off = hmul2(s, MINUS_1152), x[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
-    uint32_t y[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        y[2 * i] = hfma2(__byte_perm(x[i], 0x64646464u, 0x4140), s, off);
-        y[2 * i + 1] = hfma2(__byte_perm(x[i], 0x64646464u, 0x4342), s, off);
-    }
-    low = make_uint4(y[0], y[1], y[2], y[3]);
-    high = make_uint4(y[4], y[5], y[6], y[7]);
+// 8 bytes as 8 fp16 numbers times s (off = -1152 s), in their order
+__device__ __forceinline__ uint4 widen8(uint2 v, uint32_t s, uint32_t off) {
+    const uint32_t x = v.x ^ 0x80808080u, y = v.y ^ 0x80808080u;
+    return make_uint4(hfma2(__byte_perm(x, 0x64646464u, 0x4140), s, off), hfma2(__byte_perm(x, 0x64646464u, 0x4342), s, off),
+                      hfma2(__byte_perm(y, 0x64646464u, 0x4140), s, off), hfma2(__byte_perm(y, 0x64646464u, 0x4342), s, off));
 }
 
 template <int HD>
@@ -1333,7 +1385,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        info.packed[lane + 32 * j] = (ks[j] ? f16_power((int)ks[j] - ke + SCALE_UP) : 0u) | ((vs[j] ? f16_power((int)vs[j] - ve[j >> 1] + SCALE_UP) : 0u) << 16);
+                        info.packed[lane + 32 * j] = pack_f16(power_of((int)ks[j], ke), power_of((int)vs[j], ve[j >> 1]));
                     if (lane == 0) {
                         info.k_unit = __uint_as_float((uint32_t)max(ke - SCALE_UP, 1) << 23);
                         info.v_unit[0] = (float)(ve[0] - 127);
@@ -1371,21 +1423,21 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
             // rows to the operands' place, times their scales
 #pragma unroll 1
             for (int i0 = 0; i0 < PASSES; i0 += 4) {
-                uint4 x[4];
+                uint2 x[4][2];                                 // this lane's first half and the other one
                 uint32_t s[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int row = (i0 + j) * RPP + row_in;
-                    x[j] = *reinterpret_cast<const uint4*>(raw + row * HD);
+                    x[j][0] = *reinterpret_cast<const uint2*>(raw + row * HD + flip * 8);
+                    x[j][1] = *reinterpret_cast<const uint2*>(raw + row * HD + (1 - flip) * 8);
                     s[j] = __byte_perm(packed[row], 0, select);
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int row = (i0 + j) * RPP + row_in;
-                    uint4 low, high;
-                    widen16(x[j], s[j], low, high);
-                    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk + flip) ^ (row & 7)) << 4)) = flip ? high : low;
-                    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk + 1 - flip) ^ (row & 7)) << 4)) = flip ? low : high;
+                    const uint32_t off = hmul2(s[j], MINUS_1152);
+                    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk + flip) ^ (row & 7)) << 4)) = widen8(x[j][0], s[j], off);
+                    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk + 1 - flip) ^ (row & 7)) << 4)) = widen8(x[j][1], s[j], off);
                 }
             }
             mbar_arrive(smem_u32(&raw_empty[which]));          // the bytes' room is free
@@ -1411,29 +1463,42 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                 const int token = segment.span.first_token + at / share, head = segment.head * share + at % share;
                 // (lanes without a row have queries of zero and see everything: nothing is masked for them)
                 const int my_pos = valid ? segment.span.first_pos + at / share : 0x3fffffff, my_first = valid ? first_seen(a, my_pos) : 0;
+                // The queries come row by row, the whole warp's at once; then each lane brings its row to fp16, the largest at 2^14, in place. (What is run
+                // once a tile is written in short loops: its instructions are not at hand, and unrolled it took twice the time.)
                 float row_scale;
-                {   // the row's queries as fp16, their largest at 2^14
-                    const uint4* q = reinterpret_cast<const uint4*>(behind_wait(static_cast<const __nv_bfloat16*>(a.q)) + (size_t)token * a.q_stride + (size_t)head * HD);
-                    uint4 x[HD / 8];
-                    uint32_t most = 0;
-#pragma unroll
-                    for (int i = 0; i < HD / 8; ++i) x[i] = valid ? q[i] : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                    for (int i = 0; i < HD / 8; ++i) {
-                        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) most = max(most, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+                {
+                    constexpr int CHUNKS = HD / 8, ROWS = 32 / CHUNKS;           // 16-byte chunks of a row, rows to an instruction
+                    const int chunk = lane % CHUNKS;
+                    const __nv_bfloat16* q = behind_wait(static_cast<const __nv_bfloat16*>(a.q)) + (size_t)(segment.head * share) * HD + chunk * 8;
+                    int from = segment.row0 + tile * TILE_ROWS + quarter * 32 + lane / CHUNKS, token0 = from / share, head0 = from - token0 * share;
+                    token0 += segment.span.first_token;
+#pragma unroll 4
+                    for (int i = lane / CHUNKS; i < 32; i += ROWS) {
+                        const int row = quarter * 32 + i;
+                        unsigned char* to = q_tile + tile * Q_BYTES + (chunk >> 3) * TILE_PIECE + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+                        if (row < tile_rows) cp_async16(to, q + (size_t)token0 * a.q_stride + (size_t)head0 * HD);
+                        else *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
+                        for (head0 += ROWS; head0 >= share; head0 -= share) ++token0;
                     }
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    __syncwarp();
+                    auto place = [&](int i) { return reinterpret_cast<uint4*>(my_row + (i >> 3) * TILE_PIECE + (((i & 7) ^ (r & 7)) << 4)); };
+                    uint32_t most = 0;
+#pragma unroll 4
+                    for (int i = 0; i < CHUNKS; ++i) {
+                        const uint4 x = *place(i);
+                        most = __vmaxu2(most, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+                    }
+                    most = max(most & 0xffffu, most >> 16);
                     const int exponent = max((int)(most >> 7), 27) - 127;
                     const float factor = __uint_as_float((uint32_t)(14 - exponent + 127) << 23);
                     row_scale = a.scale_log2 * __uint_as_float((uint32_t)max(exponent - 14 + 127, 1) << 23);
-#pragma unroll
-                    for (int i = 0; i < HD / 8; ++i) {
-                        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                        uint32_t y[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) y[k] = pack_f16(__uint_as_float(w[k] << 16) * factor, __uint_as_float(w[k] & 0xffff0000u) * factor);
-                        *reinterpret_cast<uint4*>(my_row + (i >> 3) * TILE_PIECE + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+#pragma unroll 2
+                    for (int i = 0; i < CHUNKS; ++i) {
+                        const uint4 x = *place(i);
+                        auto both = [&](uint32_t w) { return pack_f16(__uint_as_float(w << 16) * factor, __uint_as_float(w & 0xffff0000u) * factor); };
+                        *place(i) = make_uint4(both(x.x), both(x.y), both(x.z), both(x.w));
                     }
                 }
                 fence_async_shared();
@@ -1559,26 +1624,27 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                         *reinterpret_cast<float2*>(a.wide_stats + part * 2) = make_float2(run_sum != 0.f ? run_max : -INFINITY, run_sum);
                     }
                     constexpr int ROOM = HD * 2;               // bytes of a row that go out at a time
-                    for (int half = 0; half < (whole ? 1 : 2); ++half) {
-                        const int from = half * (HD / 2), columns = whole ? HD : HD / 2;
+                    const int columns = whole ? HD : HD / 2;
 #pragma unroll 1
-                        for (int col = 0; col < columns; col += 32) {
-                            uint32_t x[32];
-                            tmem_ld32(o_addr + from + col, x);
+                    for (int from = 0; from < HD; from += columns) {
+#pragma unroll 1
+                        for (int col = 0; col < columns; col += 16) {
+                            uint32_t x[16];
+                            tmem_ld16(o_addr + from + col, x);
 #pragma unroll
-                            for (int d = 0; d < 32; ++d) x[d] = __float_as_uint(__uint_as_float(x[d]) * factor);
-                            const int chunk0 = col * (whole ? 2 : 4) / 16;
+                            for (int d = 0; d < 16; ++d) x[d] = __float_as_uint(__uint_as_float(x[d]) * factor);
+                            const int chunk0 = whole ? col / 8 : col / 4;
                             auto put = [&](int chunk, uint4 v) {
                                 *reinterpret_cast<uint4*>(my_row + (chunk >> 3) * TILE_PIECE + (((chunk & 7) ^ (r & 7)) << 4)) = v;
                             };
                             if (whole) {
 #pragma unroll
-                                for (int d = 0; d < 32; d += 8)
+                                for (int d = 0; d < 16; d += 8)
                                     put(chunk0 + d / 8, make_uint4(pack2(__uint_as_float(x[d]), __uint_as_float(x[d + 1])), pack2(__uint_as_float(x[d + 2]), __uint_as_float(x[d + 3])),
                                                                    pack2(__uint_as_float(x[d + 4]), __uint_as_float(x[d + 5])), pack2(__uint_as_float(x[d + 6]), __uint_as_float(x[d + 7]))));
                             } else {
 #pragma unroll
-                                for (int d = 0; d < 32; d += 4) put(chunk0 + d / 4, make_uint4(x[d], x[d + 1], x[d + 2], x[d + 3]));
+                                for (int d = 0; d < 16; d += 4) put(chunk0 + d / 4, make_uint4(x[d], x[d + 1], x[d + 2], x[d + 3]));
                             }
                         }
                         __syncwarp();
@@ -1589,7 +1655,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                             const int row = i + lane / CHUNKS, in_tile = quarter * 32 + row;
                             unsigned char* there = reinterpret_cast<unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), row));
                             if (there)
-                                *reinterpret_cast<uint4*>(there + half * ROOM + chunk * 16) = *reinterpret_cast<const uint4*>(
+                                *reinterpret_cast<uint4*>(there + from * 4 + chunk * 16) = *reinterpret_cast<const uint4*>(
                                     q_tile + tile * Q_BYTES + (chunk >> 3) * TILE_PIECE + in_tile * 128 + (((chunk & 7) ^ (in_tile & 7)) << 4));
                         }
                         __syncwarp();
@@ -1640,12 +1706,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_wide_join_kern
         before += __reduce_add_sync(0xffffffffu, s0 + lane < g.seq ? steps : 0u);
         if (g.seq >= s0 && g.seq < s0 + 32) mine = __shfl_sync(0xffffffffu, steps, g.seq - s0);
     }
-    Segment up = g;
-    long long start = before * a.n_kv_heads + (long long)g.head * mine;
-    for (up.tile = 0; up.tile < g.tile; ++up.tile) {
-        place_tile(a, up);
-        start += up.steps;
-    }
+    const long long start = before * a.n_kv_heads + (long long)g.head * mine + steps_of(a, g.span, g.tile);
     const long long per = range_steps(a, all * a.n_kv_heads);
     const int first = (int)(start / per), n_parts = (int)((start + g.steps - 1) / per) - first + 1;
     if (n_parts == 1) return;                                  // finished where it was worked on
@@ -1799,7 +1860,7 @@ struct Plan {
 // The kernel for few rows deals pages out where a sequence may have more than WHOLE_PAGES, LEAST_PAGES a block at least.
 constexpr int WHOLE_PAGES = 4, LEAST_PAGES = 2;
 // The kernel for many rows deals steps out, LEAST_STEPS a block at least, unless no tile has more than WHOLE_STEPS.
-constexpr int WHOLE_STEPS = 4, LEAST_STEPS = 4;
+constexpr int WHOLE_STEPS = 16, LEAST_STEPS = 4;
 
 Plan plan_for(const Sizes& z) {
     Plan p = {};
@@ -1887,12 +1948,12 @@ void launch_join(const Args& a, int rows, cudaStream_t stream) {
     else llmb::launch(attention_int8_join_kernel<T, 8, CHUNKS>, dim3(rows), 256, 0, stream, true, a, rows);
 }
 
-// 8-bit rows of a cache, boxes of UNIT of them
+// 8-bit rows of a cache, boxes of a unit of them
 int make_map_int8(CUtensorMap* map, const void* ptr, long long rows, int dim) {
     EncodeTiled encode = encode_fn();
     if (!encode) return fail(LLMB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)dim};
-    cuuint32_t box[2] = {(cuuint32_t)dim, (cuuint32_t)UNIT}, elem[2] = {1, 1};
+    cuuint32_t box[2] = {(cuuint32_t)dim, (cuuint32_t)(dim == 64 ? UNIT<64> : UNIT<128>)}, elem[2] = {1, 1};
     CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
