@@ -47,6 +47,8 @@ struct Args {
     int wide_blocks, wide_least;     // the same of the kernel for many rows, in steps; 0: a block a tile
     float* wide_acc;                 // parts of that kernel's blocks: [blocks, 2, 256, head_dim], and their maxima and sums
     float* wide_stats;
+    int2* few_blocks_of;             // [n_seqs, n_kv_heads] which blocks have parts of a pair, [n_seqs, n_kv_heads, tiles] of a tile
+    int2* wide_blocks_of;
 };
 
 // What a kernel reports (no wait has these codes): a step that brings more tokens than max_new says; a place outside of what the call was given, which is
@@ -419,8 +421,8 @@ __device__ __forceinline__ float power_of(int exponent, int most) { return expon
 // 2^(a - b) for references that may be -inf (of nothing)
 __device__ __forceinline__ float ratio(float a, float b) { return a == -INFINITY ? 0.f : fast_exp2(a - b); }
 
-// The pages of a sequence that its rows see: places first .. first + pages - 1 of its table. 0 pages where it brings nothing, and (many) where it
-// brings more rows than `most`.
+// The pages of a sequence that its rows see: places first .. first + pages - 1 of its table. 0 pages where it brings nothing or more than `most_tokens`,
+// and where it does not fit (check_span).
 struct Span {
     int first, pages, first_token, n_new, first_pos;
 };
@@ -430,53 +432,52 @@ __device__ __forceinline__ Span span_of(const Args& a, int seq, int most_tokens)
     const int end = a.cu_seqlens[seq + 1];
     s.n_new = end - s.first_token;
     s.first_pos = a.seq_lens[seq] - s.n_new;
-    const bool fits = s.n_new > 0 && s.n_new <= most_tokens && s.first_token >= 0 && end <= a.n_tokens && s.first_pos >= 0;
-    s.first = a.window > 0 ? max(s.first_pos - a.window + 1, 0) / LLMB_PAGE : 0;
-    s.pages = fits ? (s.first_pos + s.n_new - 1) / LLMB_PAGE + 1 - s.first : 0;
+    s.first = first_seen(a, s.first_pos) / LLMB_PAGE;
+    s.pages = (s.first_pos + s.n_new - 1) / LLMB_PAGE + 1 - s.first;
+    if (s.n_new <= 0 || s.n_new > most_tokens || s.first_token < 0 || end > a.n_tokens || s.first_pos < 0 || s.pages > a.ring_pages) s.pages = 0;
     return s;
 }
-// A (sequence, key head) pair and where its pages stand among all.
-struct Pair {
-    int seq, head;
-    long long start;
-    Span span;
-};
-// What does not fit is reported: places that there are not, more tokens than max_new says (where no other kernel takes those).
+// What does not fit is reported: places that there are not, more tokens than max_new says.
 __device__ __forceinline__ void check_span(const Args& a, const Span& s, int* status) {
     if (s.n_new <= 0) return;
-    if (s.first_token < 0 || s.first_token + s.n_new > a.n_tokens || s.first_pos < 0) report(status, OUT_OF_RANGE);
+    if (s.first_token < 0 || s.first_token + s.n_new > a.n_tokens || s.first_pos < 0 ||
+        (s.first_pos + s.n_new - 1) / LLMB_PAGE + 1 - s.first > a.ring_pages) report(status, OUT_OF_RANGE);
     else if (s.n_new > a.max_new) report(status, BEYOND_BOUNDS);
 }
+// A (sequence, key head) pair and where its pages stand among all. (There are fewer than 2^31: a sequence has no more than its ring.)
+struct Pair {
+    int seq, head, start;
+    Span span;
+};
 // The pages of all pairs, by every lane of a warp.
-__device__ __forceinline__ long long all_pages(const Args& a, int most_tokens, int lane) {
-    long long sum = 0;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32)
-        sum += __reduce_add_sync(0xffffffffu, s0 + lane < a.n_seqs ? (unsigned)span_of(a, s0 + lane, most_tokens).pages : 0u);
+__device__ __forceinline__ int all_pages(const Args& a, int most_tokens, int lane) {
+    int sum = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) sum += __reduce_add_sync(0xffffffffu, s0 + lane < a.n_seqs ? span_of(a, s0 + lane, most_tokens).pages : 0);
     return sum * a.n_kv_heads;
 }
 // The pair that page `at` of all belongs to.
-__device__ __forceinline__ Pair pair_at(const Args& a, long long at, int most_tokens, int lane) {
-    long long before = 0;
+__device__ __forceinline__ Pair pair_at(const Args& a, int at, int most_tokens, int lane) {
+    int before = 0;
     Pair p;
     for (int s0 = 0;; s0 += 32) {
         const int mine = s0 + lane < a.n_seqs ? span_of(a, s0 + lane, most_tokens).pages : 0;
-        unsigned up = mine;
+        int up = mine;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
-            unsigned left = __shfl_up_sync(0xffffffffu, up, d);
+            int left = __shfl_up_sync(0xffffffffu, up, d);
             if (lane >= d) up += left;
         }
-        const unsigned beyond = __ballot_sync(0xffffffffu, at < before + (long long)up * a.n_kv_heads);
+        const unsigned beyond = __ballot_sync(0xffffffffu, at < before + up * a.n_kv_heads);
         if (beyond) {
             const int k = __ffs(beyond) - 1;
             p.seq = s0 + k;
             p.span = span_of(a, p.seq, most_tokens);
-            p.start = before + (long long)(__shfl_sync(0xffffffffu, up, k) - p.span.pages) * a.n_kv_heads;
-            p.head = (int)((at - p.start) / p.span.pages);
-            p.start += (long long)p.head * p.span.pages;
+            p.start = before + (__shfl_sync(0xffffffffu, up, k) - p.span.pages) * a.n_kv_heads;
+            p.head = (at - p.start) / p.span.pages;
+            p.start += p.head * p.span.pages;
             return p;
         }
-        before += (long long)__shfl_sync(0xffffffffu, up, 31) * a.n_kv_heads;
+        before += __shfl_sync(0xffffffffu, up, 31) * a.n_kv_heads;
     }
 }
 // the pair behind it (there is one)
@@ -486,10 +487,12 @@ __device__ __forceinline__ void next_pair(const Args& a, Pair& p, int most_token
     p.head = 0;
     do p.span = span_of(a, ++p.seq, most_tokens); while (p.span.pages == 0 && p.seq + 1 < a.n_seqs);
 }
-// pages of a block's range: all in equal ranges, two pages at least
-__device__ __forceinline__ long long range_pages(const Args& a, long long all) {
-    const long long per = (all + a.deal_blocks - 1) / a.deal_blocks;
-    return per < a.deal_least ? a.deal_least : per;
+// A block's range of `all` things that are dealt out to so many blocks, `least` at least.
+__device__ __forceinline__ int range_of(int all, int blocks, int least) { return max((all + blocks - 1) / blocks, least); }
+// The block that begins with something says which blocks have parts of it: x the first one, y how many.
+__device__ __forceinline__ int2 blocks_of(int start, int count, int per) {
+    const int first = start / per;
+    return make_int2(first, (start + count - 1) / per - first + 1);
 }
 
 template <int HD, int NT>
@@ -512,46 +515,42 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         if (warp == 0) *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    griddep_wait();
     __syncthreads();
+    // (lengths, tables and the order are not written by the kernels of a step: a block finds its place before the kernel in front is done)
     const int share = a.n_heads / a.n_kv_heads, most_tokens = a.few_tokens;
     Pair pair;
-    long long r0, r1;                                          // the block's range of all pages
+    int r0, r1, per = 0;                                       // the block's range of all pages
     if (a.deal_blocks == 0) {                                  // a pair a block
         const int at = blockIdx.x / a.n_kv_heads;
         pair.seq = a.seq_order ? a.seq_order[at] : at;
         pair.head = blockIdx.x % a.n_kv_heads;
         pair.start = r0 = 0;
-        if ((unsigned)pair.seq >= (unsigned)a.n_seqs) {
-            if (threadIdx.x == 0) report(status, OUT_OF_RANGE);
-            return;
-        }
-        pair.span = span_of(a, pair.seq, most_tokens);
-        r1 = pair.span.pages;
-        if (r1 == 0) {
-            if (threadIdx.x == 0) check_span(a, pair.span, status);
-            return;
-        }
+        const bool there = (unsigned)pair.seq < (unsigned)a.n_seqs;
+        pair.span = span_of(a, there ? pair.seq : 0, most_tokens);
+        r1 = there ? pair.span.pages : 0;
+        if (threadIdx.x == 0) there ? check_span(a, pair.span, status) : report(status, OUT_OF_RANGE);
     } else {
-        const long long all = all_pages(a, most_tokens, lane), per = range_pages(a, all);
+        const int all = all_pages(a, most_tokens, lane);
+        per = range_of(all, a.deal_blocks, a.deal_least);
         if (blockIdx.x == 0)
             for (int s = threadIdx.x; s < a.n_seqs; s += FEW_THREADS) {
                 check_span(a, span_of(a, s, most_tokens), status);
                 if (a.seq_order && (unsigned)a.seq_order[s] >= (unsigned)a.n_seqs) report(status, OUT_OF_RANGE);
             }
-        r0 = blockIdx.x * per;
-        r1 = r0 + per < all ? r0 + per : all;
-        if (r0 >= r1) return;
-        pair = pair_at(a, r0, most_tokens, lane);
+        r0 = min((long long)blockIdx.x * per, (long long)all);
+        r1 = min(r0 + per, all);
+        if (r0 < r1) pair = pair_at(a, r0, most_tokens, lane);
     }
+    griddep_wait();
+    if (r0 >= r1) return;
     constexpr int PER_PAGE = LLMB_PAGE / U, TILES = U / 16;
-    const int units = (int)(r1 - r0) * PER_PAGE;
+    const int units = (r1 - r0) * PER_PAGE;
     const __nv_bfloat16* q_all = behind_wait(static_cast<const __nv_bfloat16*>(a.q));
     const int scales_per_page = LLMB_PAGE >> a.block_shift;
 
     // What is asked for: unit `asked` of the range, of pair `ahead` (up to page `ahead_end` of the range); its page's number is on its way.
     Pair ahead = pair;
-    int asked = warp, page_ahead = 0, ahead_end = (int)(pair.start - r0) + pair.span.pages;
+    int asked = warp, page_ahead = 0, ahead_end = pair.start - r0 + pair.span.pages;
     auto look_up = [&]() {
         if (asked >= units) return;
         const int at = asked / PER_PAGE;
@@ -595,7 +594,8 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         // ---- the pair's rows
         const Span& span = pair.span;
         const int n_rows = span.n_new * share;
-        const int pair_begin = (int)(pair.start - r0), pair_end = pair_begin + span.pages, range_end = (int)(r1 - r0);      // in pages of the range
+        const int pair_begin = pair.start - r0, pair_end = pair_begin + span.pages, range_end = r1 - r0;       // in pages of the range
+        if (per && pair_begin >= 0 && threadIdx.x == 0) a.few_blocks_of[pair.seq * a.n_kv_heads + pair.head] = blocks_of(pair.start, span.pages, per);
         const int end = min(pair_end, range_end);
         const int limit = span.first_pos + span.n_new - 1, low = first_seen(a, span.first_pos);       // positions that a row sees at all,
         const int all_to = span.first_pos, all_from = first_seen(a, limit);                           // and that all rows see
@@ -922,79 +922,83 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         for (int i = 0; i < 100; ++i) __nanosleep(10000);
 }
 
-// The parts of a (sequence, key head) pair that several blocks have worked on. A block a pair, a warp a row at a time (several for few rows, each with
-// its share of the parts; their sums are added in order).
-constexpr int JOIN_WARPS = 8;
-template <int HD>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_few_join_kernel(const __grid_constant__ Args a) {
+// The parts that several blocks have of a row: a row is one of `stride` of a (sequence, key head) pair, or of a pair's tile, `of` says which blocks. WARPS
+// warps a row, each with every WARPS-th part; their sums are added in order.
+constexpr int JOIN_WARPS = 8, JOIN_AHEAD = 4;
+template <int HD, int WARPS>
+__device__ __forceinline__ void join_row(const float* acc, const float2* stats, int2 of, int stride, int r, bool there, __nv_bfloat16* to) {
     constexpr int W = HD / 32;                                 // a lane's columns
     __shared__ float shared_value[JOIN_WARPS][HD];
-    __shared__ float2 shared_stats[JOIN_WARPS];
-    griddep_launch();
-    griddep_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = a.n_heads / a.n_kv_heads;
-    const int seq = blockIdx.x / a.n_kv_heads, head = blockIdx.x % a.n_kv_heads;
-    const Span span = span_of(a, seq, a.few_tokens);
-    if (span.pages == 0) return;
-    long long all = 0, before = 0;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-        const unsigned pages = s0 + lane < a.n_seqs ? (unsigned)span_of(a, s0 + lane, a.few_tokens).pages : 0u;
-        all += __reduce_add_sync(0xffffffffu, pages);
-        before += __reduce_add_sync(0xffffffffu, s0 + lane < seq ? pages : 0u);
-    }
-    const long long per = range_pages(a, all * a.n_kv_heads), start = before * a.n_kv_heads + (long long)head * span.pages;
-    const int first = (int)(start / per), last = (int)((start + span.pages - 1) / per), n_parts = last - first + 1, n_rows = span.n_new * share;
-    if (n_parts == 1) return;                                  // finished where it was worked on
-    const float* acc = behind_wait(a.acc);
-    const float2* stats = reinterpret_cast<const float2*>(behind_wait(a.stats));
-    int a_row = 1;                                             // warps of a row
-    while (a_row * 2 * n_rows <= JOIN_WARPS) a_row *= 2;
-    const int rows = JOIN_WARPS / a_row, mine = warp % a_row;
-    auto part_of = [&](int k, int r) { return ((size_t)(first + k) * 2 + (k == 0 ? 1 : 0)) * FEW_ROWS + r; };
-    for (int r0 = 0; r0 < n_rows; r0 += rows) {
-        const int r = r0 + warp / a_row;
-        float value[W], m = -INFINITY, sum = 0.f;
+    __shared__ float shared_sum[JOIN_WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp % WARPS;
+    auto part_of = [&](int k) { return ((size_t)(of.x + k) * 2 + (k == 0 ? 1 : 0)) * stride + r; };
+    float value[W], sum = 0.f;
 #pragma unroll
-        for (int c = 0; c < W; ++c) value[c] = 0.f;
-        if (r < n_rows) {
-            for (int k = lane; k < n_parts; k += 32) m = fmaxf(m, stats[part_of(k, r)].x);
-            m = warp_max(m);
-            const float against = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-            for (int k = mine; k < n_parts; k += a_row) {
-                const float2 s = stats[part_of(k, r)];
-                const float* from = acc + part_of(k, r) * HD + lane * W;
-                float x[W];
-                if constexpr (W == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from);
-                else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(from);
-                const float weight = s.y != 0.f ? exp2f(s.x - against) : 0.f;
-                sum += s.y * weight;
+    for (int c = 0; c < W; ++c) value[c] = 0.f;
+    if (there) {
+        float m = -INFINITY;
+        for (int k = lane; k < of.y; k += 32) m = fmaxf(m, stats[part_of(k)].x);
+        for (int k0 = mine; k0 < of.y; k0 += WARPS * JOIN_AHEAD) {
+            float x[JOIN_AHEAD][W];
+            float2 st[JOIN_AHEAD];
 #pragma unroll
-                for (int c = 0; c < W; ++c) value[c] = fmaf(x[c], weight, value[c]);
-            }
-        }
-        if (a_row > 1) {
-            if (r < n_rows) {
+            for (int j = 0; j < JOIN_AHEAD; ++j) {
+                const int k = k0 + j * WARPS;
+                st[j] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-                for (int c = 0; c < W; ++c) shared_value[warp][lane * W + c] = value[c];
-                if (lane == 0) shared_stats[warp] = make_float2(m, sum);
-            }
-            __syncthreads();
-            if (mine == 0 && r < n_rows)
-                for (int k = 1; k < a_row; ++k) {
-                    sum += shared_stats[warp + k].y;
-#pragma unroll
-                    for (int c = 0; c < W; ++c) value[c] += shared_value[warp + k][lane * W + c];
+                for (int c = 0; c < W; ++c) x[j][c] = 0.f;
+                if (k < of.y) {
+                    st[j] = stats[part_of(k)];
+                    const float* from = acc + part_of(k) * HD + lane * W;
+                    if constexpr (W == 4) *reinterpret_cast<float4*>(x[j]) = *reinterpret_cast<const float4*>(from);
+                    else *reinterpret_cast<float2*>(x[j]) = *reinterpret_cast<const float2*>(from);
                 }
-            __syncthreads();
-        }
-        if (mine == 0 && r < n_rows) {
-            const float inv = sum != 0.f ? 1.f / sum : 0.f;
-            __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first_token + r / share) * a.out_stride + (size_t)(head * share + r % share) * HD + lane * W;
+            }
+            if (k0 == mine) m = warp_max(m);                   // (the loads above are under way)
+            const float against = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int c = 0; c < W; c += 2) *reinterpret_cast<uint32_t*>(to + c) = pack_bf16(value[c] * inv, value[c + 1] * inv);
+            for (int j = 0; j < JOIN_AHEAD; ++j) {
+                const float weight = st[j].y != 0.f ? exp2f(st[j].x - against) : 0.f;
+                sum += st[j].y * weight;
+#pragma unroll
+                for (int c = 0; c < W; ++c) value[c] = fmaf(x[j][c], weight, value[c]);
+            }
         }
     }
+    if (WARPS > 1) {
+#pragma unroll
+        for (int c = 0; c < W; ++c) shared_value[warp][lane * W + c] = value[c];
+        if (lane == 0) shared_sum[warp] = sum;
+        __syncthreads();
+        if (mine == 0)
+#pragma unroll
+            for (int k = 1; k < WARPS; ++k) {
+                sum += shared_sum[warp + k];
+#pragma unroll
+                for (int c = 0; c < W; ++c) value[c] += shared_value[warp + k][lane * W + c];
+            }
+    }
+    if (mine == 0 && there) {
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+        for (int c = 0; c < W; c += 2) *reinterpret_cast<uint32_t*>(to + lane * W + c) = pack_bf16(value[c] * inv, value[c + 1] * inv);
+    }
+}
+
+template <int HD, int WARPS>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_few_join_kernel(const __grid_constant__ Args a, int rows) {
+    griddep_launch();
+    const int share = a.n_heads / a.n_kv_heads, most = a.few_tokens * share;      // rows of a pair
+    const int row = blockIdx.x * (JOIN_WARPS / WARPS) + (threadIdx.x >> 5) / WARPS;
+    const int pair = row / most, r = row - pair * most, seq = pair / a.n_kv_heads, head = pair - seq * a.n_kv_heads;
+    Span span{};
+    if (row < rows) span = span_of(a, seq, a.few_tokens);
+    griddep_wait();
+    bool there = span.pages > 0 && r < span.n_new * share;
+    const int2 of = there ? behind_wait(a.few_blocks_of)[pair] : make_int2(0, 0);
+    there = there && of.y > 1;                                 // (one block has finished it where it was worked on)
+    join_row<HD, WARPS>(behind_wait(a.acc), reinterpret_cast<const float2*>(behind_wait(a.stats)), of, FEW_ROWS, r, there,
+                        static_cast<__nv_bfloat16*>(a.out) + (size_t)(span.first_token + r / share) * a.out_stride + (size_t)(head * share + r % share) * HD);
 }
 
 // ------------------------------------------------------------------------------------------------ bfloat16, many rows
@@ -1044,7 +1048,7 @@ struct Segment {
     int first_page, pages, steps;
     int low, limit;                  // positions that a row of the tile sees at all
     Span span;
-    long long start;                 // its first step among all
+    int start;                       // its first step among all
 };
 __device__ __forceinline__ int tiles_of(const Args& a, const Span& s) { return (s.n_new * (a.n_heads / a.n_kv_heads) + WIDE_ROWS - 1) / WIDE_ROWS; }
 __device__ __forceinline__ void place_tile(const Args& a, Segment& g) {
@@ -1089,31 +1093,30 @@ __device__ __forceinline__ int steps_of(const Args& a, const Span& s, int most =
     for (TileWalk w = walk_of(a, s); w.tile < min(w.tiles, most);) sum += walk_steps(a, s, w, share, tokens, rest);
     return sum;
 }
-__device__ __forceinline__ long long all_steps(const Args& a, int lane) {
-    long long sum = 0;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32)
-        sum += __reduce_add_sync(0xffffffffu, s0 + lane < a.n_seqs ? (unsigned)steps_of(a, wide_span(a, s0 + lane)) : 0u);
+__device__ __forceinline__ int all_steps(const Args& a, int lane) {
+    int sum = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) sum += __reduce_add_sync(0xffffffffu, s0 + lane < a.n_seqs ? steps_of(a, wide_span(a, s0 + lane)) : 0);
     return sum * a.n_kv_heads;
 }
-__device__ __forceinline__ Segment segment_at(const Args& a, long long at, int lane) {
-    long long before = 0;
+__device__ __forceinline__ Segment segment_at(const Args& a, int at, int lane) {
+    int before = 0;
     Segment g;
     for (int s0 = 0;; s0 += 32) {
         const int mine = s0 + lane < a.n_seqs ? steps_of(a, wide_span(a, s0 + lane)) : 0;
-        unsigned up = mine;
+        int up = mine;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
-            unsigned left = __shfl_up_sync(0xffffffffu, up, d);
+            int left = __shfl_up_sync(0xffffffffu, up, d);
             if (lane >= d) up += left;
         }
-        const unsigned beyond = __ballot_sync(0xffffffffu, at < before + (long long)up * a.n_kv_heads);
+        const unsigned beyond = __ballot_sync(0xffffffffu, at < before + up * a.n_kv_heads);
         if (beyond) {
             const int k = __ffs(beyond) - 1, steps = __shfl_sync(0xffffffffu, mine, k);
             g.seq = s0 + k;
             g.span = wide_span(a, g.seq);
-            g.start = before + (long long)(__shfl_sync(0xffffffffu, up, k) - steps) * a.n_kv_heads;
-            g.head = (int)((at - g.start) / steps);
-            g.start += (long long)g.head * steps;
+            g.start = before + (__shfl_sync(0xffffffffu, up, k) - steps) * a.n_kv_heads;
+            g.head = (at - g.start) / steps;
+            g.start += g.head * steps;
             const int share = a.n_heads / a.n_kv_heads, tokens = WIDE_ROWS / share, rest = WIDE_ROWS - tokens * share;
             for (TileWalk w = walk_of(a, g.span);;) {
                 g.tile = w.tile;
@@ -1124,7 +1127,7 @@ __device__ __forceinline__ Segment segment_at(const Args& a, long long at, int l
             place_tile(a, g);
             return g;
         }
-        before += (long long)__shfl_sync(0xffffffffu, up, 31) * a.n_kv_heads;
+        before += __shfl_sync(0xffffffffu, up, 31) * a.n_kv_heads;
     }
 }
 // the segment behind it (there is one)
@@ -1139,11 +1142,6 @@ __device__ __forceinline__ void next_segment(const Args& a, Segment& g) {
     }
     place_tile(a, g);
 }
-__device__ __forceinline__ long long range_steps(const Args& a, long long all) {
-    const long long per = (all + a.wide_blocks - 1) / a.wide_blocks;
-    return per < a.wide_least ? a.wide_least : per;
-}
-
 // 8 bytes as 8 fp16 numbers times s (off = -1152 s), in their order
 __device__ __forceinline__ uint4 widen8(uint2 v, uint32_t s, uint32_t off) {
     const uint32_t x = v.x ^ 0x80808080u, y = v.y ^ 0x80808080u;
@@ -1190,7 +1188,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
     // that wait for one another's would stand still.
     griddep_wait();
     Segment segment;
-    long long r0, r1;                                         // the block's range of all steps
+    int r0, r1, per = 0;                                      // the block's range of all steps
     if (a.wide_blocks == 0) {                                 // a tile a block, those that see most first
         int x = blockIdx.x;
         segment.head = x % a.n_kv_heads;
@@ -1210,14 +1208,15 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
         segment.start = r0 = 0;
         r1 = segment.steps;
     } else {
-        const long long all = all_steps(a, lane), per = range_steps(a, all);
+        const int all = all_steps(a, lane);
+        per = range_of(all, a.wide_blocks, a.wide_least);
         if (blockIdx.x == 0)
             for (int s = threadIdx.x; s < a.n_seqs; s += WIDE_THREADS) {
                 check_span(a, span_of(a, s, a.max_new), status);
                 if (a.seq_order && (unsigned)a.seq_order[s] >= (unsigned)a.n_seqs) report(status, OUT_OF_RANGE);
             }
-        r0 = blockIdx.x * per;
-        r1 = r0 + per < all ? r0 + per : all;
+        r0 = min((long long)blockIdx.x * per, (long long)all);
+        r1 = min(r0 + per, all);
         if (r0 >= r1) return;
         segment = segment_at(a, r0, lane);
     }
@@ -1230,12 +1229,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
     tcgen05_fence_after();
     griddep_launch();
     const uint32_t tmem_base = *tmem_slot;
-    const int total = (int)(r1 - r0);                         // steps of the block, counted on over its segments
+    const int total = r1 - r0;                                // steps of the block, counted on over its segments
     // what the block has of a segment: its steps skip .. skip + count - 1
     auto share_of = [&](const Segment& g, int& skip, int& count) {
-        skip = g.start < r0 ? (int)(r0 - g.start) : 0;
-        const long long end = g.start + g.steps < r1 ? g.start + g.steps : r1;
-        count = (int)(end - g.start) - skip;
+        skip = max(r0 - g.start, 0);
+        count = min(g.start + g.steps, r1) - g.start - skip;
     };
 
     if (warp < 4) {
@@ -1345,6 +1343,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                     }
                 };
                 look_up(skip);
+                if (per && segment.start >= r0 && lane == 0)
+                    a.wide_blocks_of[(segment.seq * a.n_kv_heads + segment.head) * a.tiles + segment.tile] = blocks_of(segment.start, segment.steps, per);
                 for (int i = skip; st < end && ok; ++st, ++i) {
                     const int pages[STEP_PAGES] = {next[0], next[1]};
                     uint32_t ks[4], vs[4];                     // the scales of positions lane + 32 j of the step
@@ -1679,67 +1679,25 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
     }
 }
 
-// The parts of a tile that several blocks have worked on: a block 64 of its rows, a warp a row at a time.
-template <int HD>
+template <int HD, int WARPS>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_wide_join_kernel(const __grid_constant__ Args a) {
-    constexpr int W = HD / 32, SLICES = 4;                     // W: a lane's columns
     griddep_launch();
-    griddep_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = a.n_heads / a.n_kv_heads;
-    int x = blockIdx.x;
-    const int slice = x % SLICES;
-    x /= SLICES;
+    constexpr int ROWS = JOIN_WARPS / WARPS, BLOCKS = WIDE_ROWS / ROWS;          // of a block; of a tile
+    const int share = a.n_heads / a.n_kv_heads, tile = blockIdx.x / BLOCKS, r = blockIdx.x % BLOCKS * ROWS + (threadIdx.x >> 5) / WARPS;
     Segment g;
-    g.head = x % a.n_kv_heads;
-    x /= a.n_kv_heads;
-    g.tile = x % a.tiles;
-    g.seq = x / a.tiles;
+    g.tile = tile % a.tiles;
+    const int pair = tile / a.tiles;
+    g.seq = pair / a.n_kv_heads;
+    g.head = pair % a.n_kv_heads;
     g.span = wide_span(a, g.seq);
-    if (g.span.pages == 0 || g.tile >= tiles_of(a, g.span)) return;
-    place_tile(a, g);
-    if (slice * (WIDE_ROWS / SLICES) >= g.n_rows) return;
-    long long all = 0, before = 0;
-    int mine = 0;                                              // steps of a key head of this sequence
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-        const unsigned steps = s0 + lane < a.n_seqs ? (unsigned)steps_of(a, wide_span(a, s0 + lane)) : 0u;
-        all += __reduce_add_sync(0xffffffffu, steps);
-        before += __reduce_add_sync(0xffffffffu, s0 + lane < g.seq ? steps : 0u);
-        if (g.seq >= s0 && g.seq < s0 + 32) mine = __shfl_sync(0xffffffffu, steps, g.seq - s0);
-    }
-    const long long start = before * a.n_kv_heads + (long long)g.head * mine + steps_of(a, g.span, g.tile);
-    const long long per = range_steps(a, all * a.n_kv_heads);
-    const int first = (int)(start / per), n_parts = (int)((start + g.steps - 1) / per) - first + 1;
-    if (n_parts == 1) return;                                  // finished where it was worked on
-    const float* acc = behind_wait(a.wide_acc);
-    const float2* stats = reinterpret_cast<const float2*>(behind_wait(a.wide_stats));
-    auto part_of = [&](int k, int r) { return ((size_t)(first + k) * 2 + (k == 0 ? 1 : 0)) * WIDE_ROWS + r; };
-    for (int i = warp; i < WIDE_ROWS / SLICES; i += JOIN_WARPS) {
-        const int r = slice * (WIDE_ROWS / SLICES) + i;
-        if (r >= g.n_rows) break;
-        float value[W], m = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int c = 0; c < W; ++c) value[c] = 0.f;
-        for (int k = lane; k < n_parts; k += 32) m = fmaxf(m, stats[part_of(k, r)].x);
-        m = warp_max(m);
-        const float against = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-        for (int k = 0; k < n_parts; ++k) {
-            const float2 s = stats[part_of(k, r)];
-            const float* from = acc + part_of(k, r) * HD + lane * W;
-            float v[W];
-            if constexpr (W == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(from);
-            else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(from);
-            const float weight = s.y != 0.f ? exp2f(s.x - against) : 0.f;
-            sum += s.y * weight;
-#pragma unroll
-            for (int c = 0; c < W; ++c) value[c] = fmaf(v[c], weight, value[c]);
-        }
-        const float inv = sum != 0.f ? 1.f / sum : 0.f;
-        const int token = g.span.first_token + (g.row0 + r) / share, head = g.head * share + (g.row0 + r) % share;
-        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD + lane * W;
-#pragma unroll
-        for (int c = 0; c < W; c += 2) *reinterpret_cast<uint32_t*>(to + c) = pack_bf16(value[c] * inv, value[c + 1] * inv);
-    }
+    const int at = g.tile * WIDE_ROWS + r;                     // the row of the sequence
+    bool there = g.span.pages > 0 && at < g.span.n_new * share;
+    griddep_wait();
+    const int2 of = there ? behind_wait(a.wide_blocks_of)[tile] : make_int2(0, 0);
+    there = there && of.y > 1;
+    if (WARPS == 1 && !there) return;
+    join_row<HD, WARPS>(behind_wait(a.wide_acc), reinterpret_cast<const float2*>(behind_wait(a.wide_stats)), of, WIDE_ROWS, r, there,
+                        static_cast<__nv_bfloat16*>(a.out) + (size_t)(g.span.first_token + at / share) * a.out_stride + (size_t)(g.head * share + at % share) * HD);
 }
 
 // ------------------------------------------------------------------------------------------------ the parts joined
@@ -1918,6 +1876,11 @@ Plan plan_for(const Sizes& z) {
 // of the parts' weighted values (their maxima and sums start on 16 bytes behind them), and of both
 long long value_floats(long long parts, int head_dim) { return (parts * head_dim + 3) / 4 * 4; }
 long long scratch_floats_of(long long parts, int head_dim) { return value_floats(parts, head_dim) + 2 * parts; }
+// and of what says which blocks have them
+long long places_of(const Plan& p, const Sizes& z) {
+    const long long pairs = (long long)z.n_seqs * z.n_kv_heads;
+    return (p.deal_blocks ? pairs : 0) + (p.wide_blocks ? pairs * p.tiles : 0);
+}
 
 // A kernel's shared memory is a setting of each device.
 constexpr int MAX_DEVICES = 64;
@@ -1972,7 +1935,11 @@ int launch_few(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
     if (code) return code;
     llmb::launch(attention_int8_few_kernel<HD, NT>, dim3((unsigned)p.few_blocks), FEW_THREADS, Few<HD, NT>::BYTES, stream, true, map_k, map_v, a, status);
     if ((code = check_launch("attention_int8_few")) || p.deal_blocks == 0) return code;
-    llmb::launch(attention_int8_few_join_kernel<HD>, dim3(a.n_seqs * a.n_kv_heads), JOIN_WARPS * 32, 0, stream, true, a);
+    // as many warps a row as there is room for: a few rows have many parts each
+    const int joined = a.n_seqs * a.n_kv_heads * a.few_tokens * (a.n_heads / a.n_kv_heads);
+    if (joined <= 4 * SMS) llmb::launch(attention_int8_few_join_kernel<HD, 8>, dim3(joined), JOIN_WARPS * 32, 0, stream, true, a, joined);
+    else if (joined <= 16 * SMS) llmb::launch(attention_int8_few_join_kernel<HD, 2>, dim3((joined + 3) / 4), JOIN_WARPS * 32, 0, stream, true, a, joined);
+    else llmb::launch(attention_int8_few_join_kernel<HD, 1>, dim3((joined + 7) / 8), JOIN_WARPS * 32, 0, stream, true, a, joined);
     return check_launch("attention_int8_few_join");
 }
 
@@ -1993,7 +1960,9 @@ int launch_wide(const Args& a, const Plan& p, int* status, cudaStream_t stream) 
     llmb::launch(attention_int8_wide_kernel<HD>, dim3((unsigned)p.wide_grid), WIDE_THREADS, bytes, stream, true, a, status);
     if (int code = check_launch("attention_int8_wide")) return code;
     if (p.wide_blocks == 0) return LLMB_OK;
-    llmb::launch(attention_int8_wide_join_kernel<HD>, dim3((unsigned)(4ll * a.n_seqs * a.n_kv_heads * a.tiles)), JOIN_WARPS * 32, 0, stream, true, a);
+    const unsigned tiles = (unsigned)a.n_seqs * a.n_kv_heads * a.tiles;
+    if (tiles <= 32) llmb::launch(attention_int8_wide_join_kernel<HD, 4>, dim3(tiles * (WIDE_ROWS / 2)), JOIN_WARPS * 32, 0, stream, true, a);
+    else llmb::launch(attention_int8_wide_join_kernel<HD, 1>, dim3(tiles * (WIDE_ROWS / JOIN_WARPS)), JOIN_WARPS * 32, 0, stream, true, a);
     return check_launch("attention_int8_wide_join");
 }
 
@@ -2049,7 +2018,7 @@ LLMB_EXPORT long long llmb_attention_int8_scratch_floats(const llmb_int8_sizes* 
     if (!sane(*z)) return 0;
     const Plan p = plan_for(sizes_of(*z));
     *kernels = p.launches;
-    return scratch_floats_of(p.part_rows * p.slots + p.wide_rows, z->head_dim);
+    return scratch_floats_of(p.part_rows * p.slots + p.wide_rows, z->head_dim) + 2 * places_of(p, sizes_of(*z));
 }
 
 LLMB_EXPORT int llmb_attention_int8(const void* q, const void* keys, const float* key_scales, const void* values, const float* value_scales,
@@ -2073,18 +2042,21 @@ LLMB_EXPORT int llmb_attention_int8(const void* q, const void* keys, const float
                  "attention_int8: the tensor-core kernels do not take these operands");
     const Sizes s = sizes_of(z);
     const Plan p = plan_for(s);
-    LLMB_REQUIRE(p.blocks < (1ll << 31) && p.few_blocks < (1ll << 31) && 4 * p.wide_grid < (1ll << 31) &&
-                 4ll * z.n_seqs * z.n_kv_heads * p.tiles < (1ll << 31), "attention_int8: too many blocks");
+    const long long pairs = (long long)z.n_seqs * z.n_kv_heads;
+    LLMB_REQUIRE(p.blocks < (1ll << 31) && p.few_blocks < (1ll << 31) && p.wide_grid < (1ll << 31) && pairs * p.tiles * (WIDE_ROWS / 2) < (1ll << 31) &&
+                 pairs * FEW_ROWS < (1ll << 31), "attention_int8: too many blocks");
+    LLMB_REQUIRE(!z.tc || pairs * z.ring_pages * (p.wide ? p.tiles : 1) < (1ll << 31), "attention_int8: too many pages to deal out");
     const long long parts = p.part_rows * p.slots, all_parts = parts + p.wide_rows;
-    LLMB_REQUIRE(all_parts == 0 || (scratch != nullptr && aligned(scratch) && scratch_floats >= scratch_floats_of(all_parts, z.head_dim)),
+    LLMB_REQUIRE(all_parts == 0 || (scratch != nullptr && aligned(scratch) && scratch_floats >= scratch_floats_of(all_parts, z.head_dim) + 2 * places_of(p, s)),
                  "attention_int8: scratch too small");
     int* status = nullptr;
     if (status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status, status_word(), 0));
     float* stats = scratch + value_floats(all_parts, z.head_dim);
+    int2* places = reinterpret_cast<int2*>(stats + 2 * all_parts);
     const Args a{q, (const signed char*)keys, key_scales, (const signed char*)values, value_scales, block_table, seq_lens, cu_seqlens, seq_order, out, scratch,
                  stats, z.q_stride, z.out_stride, z.table_stride, z.ring_pages, z.n_pages, z.n_tokens, z.n_seqs, z.n_heads, z.n_kv_heads, z.head_dim,
                  shift, z.window, scale * LOG2E, z.max_new, p.tiles, p.slots, p.few_tokens, p.deal_blocks, p.deal_least, p.wide_blocks, p.wide_least,
-                 scratch + parts * z.head_dim, stats + 2 * parts};
+                 scratch + parts * z.head_dim, stats + 2 * parts, places, places + (p.deal_blocks ? pairs : 0)};
     return z.dtype == LLMB_DTYPE_F32 ? run<float>(a, p, s, status, stream) : run<__nv_bfloat16>(a, p, s, status, stream);
 }
 

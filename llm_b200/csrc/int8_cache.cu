@@ -160,28 +160,35 @@ LLMB_EXPORT int llmb_int8_cache_status() {
     return v;
 }
 
-LLMB_EXPORT int llmb_int8_append(const void* qkv, int dtype, const float* angles, const int* tok_pos, const int* tok_seq,
-                                 const int* cu_seqlens, const int* block_table, int table_stride, int ring_pages, void* queries, void* keys,
-                                 float* key_scales, void* values, float* value_scales, int n_tokens, int n_seqs, int n_pages,
-                                 int n_heads, int n_kv_heads, int head_dim, int n_rot, int n_positions, int interleaved, int block, int write_cache,
-                                 cudaStream_t stream) {
-    if (n_tokens == 0) return LLMB_OK;
-    LLMB_REQUIRE(dtype == LLMB_DTYPE_F32 || dtype == LLMB_DTYPE_BF16, "int8_append: unknown dtype %d", dtype);
-    LLMB_REQUIRE(n_tokens > 0 && n_heads > 0 && n_kv_heads > 0 && ring_pages > 0, "int8_append: bad sizes");
-    LLMB_REQUIRE(head_dim > 0 && head_dim % 2 == 0 && head_dim <= LLMB_MAX_HEAD_DIM, "int8_append: head_dim %d must be even and at most %d", head_dim,
+// The sizes of a call, one integer each.
+struct llmb_int8_append_sizes {
+    int dtype, table_stride, ring_pages, n_tokens, n_seqs, n_pages;
+    int n_heads, n_kv_heads, head_dim, n_rot, n_positions, interleaved, block, write_cache;
+};
+
+LLMB_EXPORT int llmb_int8_append(const void* qkv, const float* angles, const int* tok_pos, const int* tok_seq, const int* cu_seqlens,
+                                 const int* block_table, void* queries, void* keys, float* key_scales, void* values, float* value_scales,
+                                 const llmb_int8_append_sizes* sizes, cudaStream_t stream) {
+    const llmb_int8_append_sizes& z = *sizes;
+    if (z.n_tokens == 0) return LLMB_OK;
+    LLMB_REQUIRE(z.dtype == LLMB_DTYPE_F32 || z.dtype == LLMB_DTYPE_BF16, "int8_append: unknown dtype %d", z.dtype);
+    LLMB_REQUIRE(z.n_tokens > 0 && z.n_seqs > 0 && z.n_heads > 0 && z.n_kv_heads > 0 && z.ring_pages > 0, "int8_append: bad sizes");
+    LLMB_REQUIRE(z.head_dim > 0 && z.head_dim % 2 == 0 && z.head_dim <= LLMB_MAX_HEAD_DIM, "int8_append: head_dim %d must be even and at most %d", z.head_dim,
                  LLMB_MAX_HEAD_DIM);
-    LLMB_REQUIRE(n_rot >= 0 && n_rot <= head_dim && n_rot % 2 == 0, "int8_append: the rotated part %d must be even and at most head_dim %d", n_rot, head_dim);
-    LLMB_REQUIRE(block >= 1 && block <= LLMB_PAGE && (block & (block - 1)) == 0, "int8_append: blocks of %d positions", block);
-    Args a{qkv, n_rot ? angles : nullptr, tok_pos, tok_seq, cu_seqlens, block_table, queries, (signed char*)keys, key_scales, (signed char*)values,
-           value_scales, table_stride, ring_pages, n_heads, n_kv_heads, head_dim, angles ? n_rot : 0, interleaved, write_cache, block,
-           n_tokens, n_seqs, n_pages, n_positions};
-    const int units = n_heads + (write_cache ? 2 * n_kv_heads : 0);
+    LLMB_REQUIRE(z.n_rot >= 0 && z.n_rot <= z.head_dim && z.n_rot % 2 == 0, "int8_append: the rotated part %d must be even and at most head_dim %d", z.n_rot,
+                 z.head_dim);
+    LLMB_REQUIRE(z.block >= 1 && z.block <= LLMB_PAGE && (z.block & (z.block - 1)) == 0, "int8_append: blocks of %d positions", z.block);
+    const bool turns = angles != nullptr && z.n_rot > 0;
+    Args a{qkv, turns ? angles : nullptr, tok_pos, tok_seq, cu_seqlens, block_table, queries, (signed char*)keys, key_scales, (signed char*)values,
+           value_scales, z.table_stride, z.ring_pages, z.n_heads, z.n_kv_heads, z.head_dim, turns ? z.n_rot : 0, z.interleaved, z.write_cache, z.block,
+           z.n_tokens, z.n_seqs, z.n_pages, z.n_positions};
+    const int units = z.n_heads + (z.write_cache ? 2 * z.n_kv_heads : 0);
     const int rows = ceil_div(units, WARPS);
     LLMB_REQUIRE(rows <= 65535, "int8_append: too many heads");
     int* status = nullptr;
     if (tc::status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status, tc::status_word(), 0));
-    dim3 grid(n_tokens, rows);
-    if (dtype == LLMB_DTYPE_F32) llmb::launch(int8_append_kernel<float>, grid, dim3(THREADS), 0, stream, true, a, status);
+    dim3 grid(z.n_tokens, rows);
+    if (z.dtype == LLMB_DTYPE_F32) llmb::launch(int8_append_kernel<float>, grid, dim3(THREADS), 0, stream, true, a, status);
     else llmb::launch(int8_append_kernel<__nv_bfloat16>, grid, dim3(THREADS), 0, stream, true, a, status);
     return check_launch("int8_append");
 }

@@ -1666,7 +1666,7 @@ class Int8Pages:
     """Keys or values of a paged cache held in 8 bits: `values`, whole numbers (int8) [pages, Hkv, 64, D], and `scales`, float32 [pages,
     Hkv, 64 / block], a power of two for each block of `block` positions (1, 2, 4 .. 64) of a head. values * scales is what is held. Both are
     contiguous; a scale that is no number says that the block took in a value that is not finite."""
-    __slots__ = ("values", "scales", "block")
+    __slots__ = ("values", "scales", "block", "shape", "device")
 
     def __init__(self, values, scales):
         if values.dim() != 4 or values.shape[2] != PAGE or values.dtype is not torch.int8 or not values.is_contiguous():
@@ -1677,6 +1677,7 @@ class Int8Pages:
         if values.data_ptr() % 16:
             raise KernelError("Int8Pages: values must start on 16 bytes")
         self.values, self.scales, self.block = values, scales, PAGE // scales.shape[2]
+        self.shape, self.device = tuple(values.shape), values.get_device()
 
     def held(self, dtype=torch.bfloat16):
         """What the pages stand for, [pages, Hkv, 64, D] (exact in bfloat16 and float32)."""
@@ -1684,18 +1685,17 @@ class Int8Pages:
 
 
 def _check_int8(keys, values, n_kv_heads, head_dim, what: str) -> None:
-    if not isinstance(keys, Int8Pages) or not isinstance(values, Int8Pages):
+    if type(keys) is not Int8Pages or type(values) is not Int8Pages:
         raise KernelError(f"{what}: keys and values are Int8Pages")
-    shape = keys.values.shape
-    if shape[1] != n_kv_heads or shape[3] != head_dim or values.values.shape != shape or values.block != keys.block:
-        raise KernelError(f"{what}: keys {tuple(shape)} in blocks of {keys.block} and values {tuple(values.values.shape)} in blocks of {values.block} "
+    if keys.shape[1:] != (n_kv_heads, PAGE, head_dim) or values.shape != keys.shape or values.block != keys.block:
+        raise KernelError(f"{what}: keys {keys.shape} in blocks of {keys.block} and values {values.shape} in blocks of {values.block} "
                           f"are no pages of {n_kv_heads} heads of {head_dim}, both alike")
 
 
-def _check_step(what: str, block_table, ring_pages, n_seqs, *vectors) -> None:
+def _check_step(what: str, block_table, ring_pages, n_seqs, vectors) -> None:
     int32 = torch.int32
     for t, count, name in vectors:
-        if t.dtype is not int32 or t.dim() != 1 or t.numel() != count or not t.is_contiguous():
+        if t.dtype is not int32 or t.shape != (count,) or not t.is_contiguous():
             raise KernelError(f"{what}: {name} must be contiguous int32 [{count}]")
     if block_table.dtype is not int32 or block_table.dim() != 2 or block_table.shape[0] != n_seqs or block_table.stride(1) != 1:
         raise KernelError(f"{what}: the page table must be int32 [{n_seqs}, pages]")
@@ -1703,13 +1703,30 @@ def _check_step(what: str, block_table, ring_pages, n_seqs, *vectors) -> None:
         raise KernelError(f"{what}: a ring of {ring_pages} pages in a table of {block_table.shape[1]}")
 
 
-def _on_current_device(what: str, *tensors) -> None:
+def _check_device(what: str, keys, values, tensors) -> None:
     """All tensors are on the current CUDA device: launches go to its current stream."""
-    _require_cuda(*tensors)
-    device = torch.cuda.current_device()
+    device = keys.device
     for t in tensors:
-        if t is not None and t.device.index != device:
-            raise KernelError(f"{what}: a tensor on {t.device}, while the current device is cuda:{device}")
+        if t is not None and t.get_device() != device:
+            device = -1
+    if device < 0 or values.device != device:
+        _require_cuda(keys.values, values.values, *tensors)
+        raise KernelError(f"{what}: its tensors are on several devices")
+    if device != (_current_device() if _current_device is not None else torch.cuda.current_device()):
+        raise KernelError(f"{what}: its tensors are on cuda:{device}, which is not the current device")
+
+
+def _declare(lib_name: str, fn_name: str, argtypes):
+    """An entry point with its argument types, so that a call hands over plain numbers (its launch is short, and a ctypes object for each
+    argument costs the host as much)."""
+    getattr(load_library(lib_name), fn_name).argtypes = argtypes
+
+
+@functools.lru_cache(maxsize=4096)
+def _int8_append_sizes(*sizes) -> tuple:
+    _declare("int8_cache", "llmb_int8_append", [_c_void] * 13)
+    packed = (_c_int * len(sizes))(*sizes)
+    return packed, ctypes.addressof(packed)
 
 
 def rope_cache_write_int8(qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_table, ring_pages, keys, values, n_heads, n_kv_heads, head_dim,
@@ -1725,35 +1742,39 @@ def rope_cache_write_int8(qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_t
     begun anew; attention over it is then none either. No two sequences of a call may write to one page. A position, sequence or page that there is not
     is left out and reported by `check_device_status`."""
     what = "rope_cache_write_int8"
-    n, n_seqs = qkv.shape[0], cu_seqlens.numel() - 1
     if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or not qkv.is_contiguous():
         raise KernelError(f"{what}: qkv {tuple(qkv.shape)} is not contiguous [T, ({n_heads} + 2 * {n_kv_heads}) * {head_dim}]")
-    code = _code(qkv.dtype)
+    n, n_seqs, dtype = qkv.shape[0], cu_seqlens.numel() - 1, qkv.dtype
+    code = _code(dtype)
     _check_int8(keys, values, n_kv_heads, head_dim, what)
-    _check_step(what, block_table, ring_pages, n_seqs, (tok_pos, n, "tok_pos"), (tok_seq, n, "tok_seq"), (cu_seqlens, n_seqs + 1, "cu_seqlens"))
+    _check_step(what, block_table, ring_pages, n_seqs, ((tok_pos, n, "tok_pos"), (tok_seq, n, "tok_seq"), (cu_seqlens, n_seqs + 1, "cu_seqlens")))
     n_rot = n_positions = 0
     if rope_table is not None:
         if rope_table.dim() != 2 or rope_table.dtype is not torch.float32 or not rope_table.is_contiguous() or rope_table.shape[1] > head_dim \
                 or rope_table.shape[1] % 2:
             raise KernelError(f"{what}: the table of angles must be contiguous float32 [positions, n_rot] with an even n_rot <= {head_dim}")
         n_positions, n_rot = rope_table.shape
-    _on_current_device(what, qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_table, keys.values, keys.scales, values.values, values.scales, out)
-    _check_out(out, (n, n_heads * head_dim), qkv.dtype, what)
+    _check_device(what, keys, values, (qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_table, out))
     if out is None:
         out = qkv.new_empty((n, n_heads * head_dim))
-    _call("int8_cache", "llmb_int8_append", _ptr(qkv), _c_int(code), _ptr(rope_table), _ptr(tok_pos), _ptr(tok_seq), _ptr(cu_seqlens),
-          _ptr(block_table), _c_int(block_table.stride(0)), _c_int(ring_pages), _ptr(out), _ptr(keys.values), _ptr(keys.scales), _ptr(values.values),
-          _ptr(values.scales), _c_int(n), _c_int(n_seqs), _c_int(keys.values.shape[0]), _c_int(n_heads), _c_int(n_kv_heads), _c_int(head_dim),
-          _c_int(n_rot), _c_int(n_positions), _c_int(1 if interleaved else 0), _c_int(keys.block), _c_int(1 if write_cache else 0), _stream())
+    else:
+        _check_out(out, (n, n_heads * head_dim), dtype, what)
+    packed, at_sizes = _int8_append_sizes(code, block_table.stride(0), ring_pages, n, n_seqs, keys.shape[0], n_heads, n_kv_heads, head_dim, n_rot,
+                                          n_positions, 1 if interleaved else 0, keys.block, 1 if write_cache else 0)
+    if _recording is not None:
+        _recording.keep += [qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_table, keys, values, out, packed]
+    _call("int8_cache", "llmb_int8_append", qkv.data_ptr(), None if rope_table is None else rope_table.data_ptr(), tok_pos.data_ptr(), tok_seq.data_ptr(),
+          cu_seqlens.data_ptr(), block_table.data_ptr(), out.data_ptr(), keys.values.data_ptr(), keys.scales.data_ptr(), values.values.data_ptr(),
+          values.scales.data_ptr(), at_sizes, _stream())
     return out
 
 
 @functools.lru_cache(maxsize=4096)
 def _int8_plan(*sizes) -> tuple:
     """(the sizes of a call as the library takes them, floats of scratch, launches)."""
+    _declare("attention_int8", "llmb_attention_int8", [_c_void] * 11 + [ctypes.c_longlong, _c_float, _c_void, _c_void])
     lib, kernels, packed = load_library("attention_int8"), ctypes.c_int(0), (_c_int * len(sizes))(*sizes)
     lib.llmb_attention_int8_scratch_floats.restype = ctypes.c_longlong
-    lib.llmb_attention_int8.argtypes = [_c_void] * 11 + [ctypes.c_longlong, _c_float, _c_void, _c_void]
     floats = lib.llmb_attention_int8_scratch_floats(packed, ctypes.byref(kernels))
     return packed, ctypes.addressof(packed), floats, kernels.value
 
@@ -1766,8 +1787,8 @@ def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seql
     before it. Returns [T, Hq * D] in qkv's dtype.
 
     max_new, max_len: most new tokens and most positions of a sequence, upper bounds that size the launches (a sequence longer than max_len is
-    served all the same). A step that brings more tokens than max_new says, and a page or token that there is not, are
-    reported by `check_device_status`; its results are not valid. `seq_order` (int32 [B]): the sequences by falling length, which start
+    served all the same). A step that brings more tokens than max_new says, a page or token that there is not, and a scale that is no
+    power of two are reported by `check_device_status`; its results are not valid. `seq_order` (int32 [B]): the sequences by falling length, which start
     in that order."""
     what = "attention_int8"
     if qkv.dim() != 2:
@@ -1778,29 +1799,32 @@ def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seql
     dtype, n_seqs = qkv.dtype, seq_lens.numel()
     code = _code(dtype)
     _check_int8(keys, values, n_kv_heads, head_dim, what)
-    _check_step(what, block_table, ring_pages, n_seqs, (seq_lens, n_seqs, "seq_lens"), (cu_seqlens, n_seqs + 1, "cu_seqlens"),
-                *(() if seq_order is None else ((seq_order, n_seqs, "seq_order"),)))
+    vectors = ((seq_lens, n_seqs, "seq_lens"), (cu_seqlens, n_seqs + 1, "cu_seqlens"))
+    if seq_order is not None:
+        vectors += ((seq_order, n_seqs, "seq_order"),)
+    _check_step(what, block_table, ring_pages, n_seqs, vectors)
     if max_new < 1 or max_len < 1 or window < 0 or not math.isfinite(scale):
         raise KernelError(f"{what}: max_new {max_new}, max_len {max_len}, window {window}, scale {scale}")
-    _on_current_device(what, qkv, keys.values, keys.scales, values.values, values.scales, block_table, seq_lens, cu_seqlens, seq_order, out)
+    _check_device(what, keys, values, (qkv, block_table, seq_lens, cu_seqlens, seq_order, out))
     if out is None:
         out = qkv.new_empty((n, n_heads * head_dim))
     else:
         _check_out(out, (n, n_heads * head_dim), dtype, what)
     if n == 0:
         return out
-    # no step goes beyond its tokens and its table; lengths count in powers of two of pages, so that a captured step serves the next lengths
+    # no step goes beyond its tokens; lengths count in powers of two of pages, so that a captured step serves the next lengths
     max_new, max_len = min(max_new, n), page_bucket(-(-min(max_len, 1 << 30) // PAGE)) * PAGE
-    tc = int(dtype is torch.bfloat16 and head_dim in (64, 128) and scale > 0 and q_stride % 8 == 0 and not (qkv.data_ptr() | out.data_ptr()) & 15
-             and keys.values.numel() // head_dim < 1 << 31 and not tactics.is_disabled("attention_int8_tc"))
-    packed, at_sizes, floats, kernels = _int8_plan(q_stride, n_heads * head_dim, block_table.stride(0), ring_pages, keys.values.shape[0], code, n, n_seqs,
+    at_q, at_out = qkv.data_ptr(), out.data_ptr()
+    tc = int(dtype is torch.bfloat16 and head_dim in (64, 128) and scale > 0 and q_stride % 8 == 0 and not (at_q | at_out) & 15
+             and keys.shape[0] * n_kv_heads * PAGE < 1 << 31 and not tactics.is_disabled("attention_int8_tc"))
+    packed, at_sizes, floats, kernels = _int8_plan(q_stride, n_heads * head_dim, block_table.stride(0), ring_pages, keys.shape[0], code, n, n_seqs,
                                                    n_heads, n_kv_heads, head_dim, keys.block, window, max_new, max_len, tc)
     parts = _scratch(qkv.device, "attention", floats)[0] if floats else None
     if _recording is not None:
         _recording.keep += [qkv, keys, values, block_table, seq_lens, cu_seqlens, seq_order, out, parts, packed]
-    _call("attention_int8", "llmb_attention_int8", qkv.data_ptr(), keys.values.data_ptr(), keys.scales.data_ptr(), values.values.data_ptr(),
+    _call("attention_int8", "llmb_attention_int8", at_q, keys.values.data_ptr(), keys.scales.data_ptr(), values.values.data_ptr(),
           values.scales.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), cu_seqlens.data_ptr(),
-          None if seq_order is None else seq_order.data_ptr(), out.data_ptr(), parts.data_ptr() if floats else None, floats, float(scale), at_sizes,
+          None if seq_order is None else seq_order.data_ptr(), at_out, parts.data_ptr() if floats else None, floats, float(scale), at_sizes,
           _stream(), kernels=kernels)
     return out
 
