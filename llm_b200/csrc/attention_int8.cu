@@ -1861,12 +1861,14 @@ Plan plan_for(const Sizes& z) {
         }
         return p;
     }
-    // Into how many slices the pages are cut: as many as make all blocks come to about the blocks that the SMs hold at once, two pages each at least.
+    // Into how many slices the pages are cut: as many as make all blocks come to about the blocks that the SMs hold at once, two pages each at least; up
+    // to WHOLE_PAGES are one block's, since joining takes a launch.
     p.tiles = ceil_div((long long)z.max_new * share, SIMT_ROWS);
     p.blocks = pairs * p.tiles;
     const long long wave = (long long)SMS * (z.head_dim <= 128 ? 2 : 1);
     long long slots = wave / p.blocks;
     if (slots > pages / 2) slots = pages / 2;
+    if (pages <= WHOLE_PAGES) slots = 1;
     p.slots = slots < 1 ? 1 : slots > MAX_SPLITS ? MAX_SPLITS : (int)slots;
     p.part_rows = p.slots == 1 ? 0 : (long long)z.n_tokens * z.n_heads;
     if (p.slots > 1) ++p.launches;
@@ -2049,8 +2051,8 @@ LLMB_EXPORT int llmb_attention_int8(const void* q, const void* keys, const float
     const long long parts = p.part_rows * p.slots, all_parts = parts + p.wide_rows;
     LLMB_REQUIRE(all_parts == 0 || (scratch != nullptr && aligned(scratch) && scratch_floats >= scratch_floats_of(all_parts, z.head_dim) + 2 * places_of(p, s)),
                  "attention_int8: scratch too small");
-    int* status = nullptr;
-    if (status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status, status_word(), 0));
+    static int* status = nullptr;                // (one address for all devices)
+    if (!status && status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status, status_word(), 0));
     float* stats = scratch + value_floats(all_parts, z.head_dim);
     int2* places = reinterpret_cast<int2*>(stats + 2 * all_parts);
     const Args a{q, (const signed char*)keys, key_scales, (const signed char*)values, value_scales, block_table, seq_lens, cu_seqlens, seq_order, out, scratch,

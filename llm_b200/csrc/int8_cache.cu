@@ -150,6 +150,244 @@ __global__ void __launch_bounds__(THREADS) int8_append_kernel(const __grid_const
     if (lane == 0) *scale_at = scale;
 }
 
+// ------------------------------------------------------------------------------------------------ 16 bytes at a time
+//
+// Heads of 64 and 128 that rotate as a whole or not at all. Eight pairs of elements are a lane's: two pieces of a row, which with the angles it holds
+// in registers for all of a token's queries; D / 16 lanes a row, so a warp has 4 rows (8) to an instruction. A block of the cache is one warp's, up to
+// 16 new rows of it in registers between the largest magnitude and the whole numbers (more are read twice).
+//
+// A block of threads does `run` neighbouring tokens: their first rows in blocks of the cache are looked up by one warp, then the eight warps take
+// blocks and queries in turn. Memory bounds long steps: 16,889 tokens of 32 heads over 8 of 128 in FIXME; what a step of
+// 64 tokens takes is a launch and three dependent reads.
+
+constexpr int MAX_RUN = 16, HELD = 16, QUERIES = 4;            // tokens of a block of threads; rows that a warp holds; rows of queries, in instructions
+
+struct Begun {                                                 // a block of the cache that begins to be written with a token
+    int token, position, n_rows, page;
+};
+
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    } else {
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+        *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(tc::pack2(x[0], x[1]), tc::pack2(x[2], x[3]), tc::pack2(x[4], x[5]), tc::pack2(x[6], x[7]));
+    } else {
+        *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(x);
+        *reinterpret_cast<float4*>(p + 4) = *reinterpret_cast<const float4*>(x + 4);
+    }
+}
+__device__ __forceinline__ uint2 whole8(const float (&x)[8], float inverse) {
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)__float2int_rn(__fmul_rn(x[i], inverse)) & 0xffu) << (8 * (i & 3));
+    return make_uint2(w[0], w[1]);
+}
+
+// A lane's part of a row: eight pairs. Interleaved, the two pieces adjoin and the pairs lie inside; otherwise they are half a head apart.
+template <typename T, int D, bool INTERLEAVED> struct Row {
+    static constexpr int LANES = D / 16, ROWS = 32 / LANES;
+    static __device__ __forceinline__ int first(int lane) { return (lane % LANES) * (INTERLEAVED ? 16 : 8); }
+    static constexpr int APART = INTERLEAVED ? 8 : D / 2;
+    static __device__ __forceinline__ void turn(float (&a)[8], float (&b)[8], const float (&c)[8], const float (&s)[8]) {
+        auto pair = [&](float& low, float& high, int i) {
+            const float x = low;
+            low = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(high, s[i]));
+            high = __fadd_rn(__fmul_rn(high, c[i]), __fmul_rn(x, s[i]));
+        };
+        if constexpr (INTERLEAVED) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                pair(a[2 * i], a[2 * i + 1], i);
+                pair(b[2 * i], b[2 * i + 1], 4 + i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pair(a[i], b[i], i);
+        }
+    }
+};
+__device__ __forceinline__ uint32_t largest8(const float (&x)[8]) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+    return most;
+}
+
+template <typename T, int D, bool INTERLEAVED>
+__global__ void __launch_bounds__(THREADS) int8_append_vec_kernel(const __grid_constant__ Args a, int run, int* status) {
+    using R = Row<T, D, INTERLEAVED>;
+    constexpr int LANES = R::LANES, ROWS = R::ROWS, STEPS = HELD / ROWS, HALF = D / 2;
+    __shared__ Begun begun[MAX_RUN];
+    __shared__ int n_begun, positions[MAX_RUN];
+    griddep_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row_in = lane / LANES, first_pair = lane % LANES * 8;
+    const int token0 = blockIdx.x * run, n_here = min(run, a.n_tokens - token0), units = a.n_heads + 2 * a.n_kv_heads;
+    // (positions, sequences and tables are not written by the kernels of a step)
+    if (warp == 0) {
+        Begun b{};
+        bool mine = false;
+        if (lane < n_here) {
+            b.token = token0 + lane;
+            b.position = a.tok_pos[b.token];
+            const int seq = a.tok_seq[b.token];
+            bool there = b.position >= 0 && !(a.angles && b.position >= a.n_positions);
+            positions[lane] = there ? b.position : -1;
+            if (there && a.write_cache) {
+                there = (unsigned)seq < (unsigned)a.n_seqs;
+                if (there && (b.position % a.block == 0 || b.token == a.cu_seqlens[seq])) {
+                    int place = b.position / LLMB_PAGE;
+                    if (place >= a.ring_pages) place %= a.ring_pages;
+                    b.n_rows = min(a.block - b.position % a.block, a.cu_seqlens[seq + 1] - b.token);
+                    b.page = a.block_table[(size_t)seq * a.table_stride + place];
+                    there = mine = (unsigned)b.page < (unsigned)a.n_pages && b.n_rows > 0 && b.token + b.n_rows <= a.n_tokens &&
+                                   !(a.angles && b.position + b.n_rows > a.n_positions);
+                }
+            }
+            if (!there && status) atomicCAS(status, 0, OUT_OF_RANGE);
+        }
+        const unsigned which = __ballot_sync(0xffffffffu, mine);
+        if (mine) begun[__popc(which & ((1u << lane) - 1u))] = b;
+        if (lane == 0) n_begun = __popc(which);
+    }
+    __syncthreads();
+    griddep_wait();
+    const T* qkv = behind_wait(static_cast<const T*>(a.qkv));
+    const size_t row_stride = (size_t)units * D;
+    auto angles_of = [&](int position, float (&c)[8], float (&s)[8]) {
+        const float* from = a.angles + (size_t)position * D + first_pair;
+        load8(from, c);
+        load8(from + HALF, s);
+    };
+    // ---- blocks of the cache: (begun block, keys or values, head)
+    const int n_blocks = n_begun * 2 * a.n_kv_heads, stride = gridDim.y * WARPS;
+    int task = blockIdx.y * WARPS + warp;
+    for (; task < n_blocks; task += stride) {
+        const Begun b = begun[task / (2 * a.n_kv_heads)];
+        const int unit = task % (2 * a.n_kv_heads);            // of the projection, behind the queries
+        const bool keys = unit < a.n_kv_heads, turned = keys && a.angles;
+        const int head = keys ? unit : unit - a.n_kv_heads, first = b.position % a.block, row = b.position % LLMB_PAGE;
+        const T* from = qkv + b.token * row_stride + (size_t)(a.n_heads + unit) * D + R::first(lane);
+        const size_t at = (size_t)b.page * a.n_kv_heads + head;
+        signed char* block_rows = (keys ? a.keys : a.values) + (at * LLMB_PAGE + row) * D;
+        signed char* to = block_rows + R::first(lane);
+        float* scale_at = (keys ? a.key_scales : a.value_scales) + at * (LLMB_PAGE / a.block) + row / a.block;
+        const float before = first != 0 ? *scale_at : 0.f;
+        float x[STEPS][8], y[STEPS][8];
+        auto fetch = [&](int r0, int i) {                      // rows r0 + i * ROWS + row_in: to place i
+            const int r = r0 + i * ROWS + row_in;
+            if (r < b.n_rows) {
+                load8(from + r * row_stride, x[i]);
+                load8(from + r * row_stride + R::APART, y[i]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[i][k] = y[i][k] = 0.f;
+            }
+        };
+        auto rotate = [&](int r0, int i) {
+            const int r = r0 + i * ROWS + row_in;
+            if (turned && r < b.n_rows) {
+                float c[8], s[8];
+                angles_of(b.position + r, c, s);
+                R::turn(x[i], y[i], c, s);
+            }
+        };
+        uint32_t most = 0;
+        for (int r0 = 0; r0 < b.n_rows; r0 += HELD) {
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) fetch(r0, i);
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                rotate(r0, i);
+                most = max(most, max(largest8(x[i]), largest8(y[i])));
+            }
+        }
+        float scale = __uint_as_float(scale_bits(__reduce_max_sync(0xffffffffu, most)));
+        if (first != 0) {                                      // the block is continued
+            __syncwarp();                                      // (everyone has read its scale)
+            if (!is_number(scale) || !is_number(before)) {
+                scale = __uint_as_float(0x7fffffffu);
+            } else if (scale > before) {
+                const float shrink = before / scale;
+                signed char* older = block_rows - first * D;
+                for (int i = lane; i < first * D / 16; i += 32) {
+                    uint4 v = reinterpret_cast<uint4*>(older)[i];
+                    signed char* q = reinterpret_cast<signed char*>(&v);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) q[k] = whole((float)q[k], shrink);
+                    reinterpret_cast<uint4*>(older)[i] = v;
+                }
+            } else {
+                scale = before;
+            }
+        }
+        const float inverse = is_number(scale) ? 1.f / scale : 0.f;
+        for (int r0 = 0; r0 < b.n_rows; r0 += HELD) {
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                if (b.n_rows > HELD) {
+                    fetch(r0, i);
+                    rotate(r0, i);
+                }
+                const int r = r0 + i * ROWS + row_in;
+                if (r < b.n_rows) {
+                    *reinterpret_cast<uint2*>(to + r * D) = inverse != 0.f ? whole8(x[i], inverse) : make_uint2(0u, 0u);
+                    *reinterpret_cast<uint2*>(to + r * D + R::APART) = inverse != 0.f ? whole8(y[i], inverse) : make_uint2(0u, 0u);
+                }
+            }
+        }
+        if (lane == 0) *scale_at = scale;
+    }
+    // ---- queries: (token, QUERIES times ROWS heads), all of them under way at once
+    const int chunks = (a.n_heads + ROWS * QUERIES - 1) / (ROWS * QUERIES), n_chunks = n_here * chunks;
+    for (task -= n_blocks; task < n_chunks; task += stride) {
+        const int t = task / chunks, head0 = (task - t * chunks) * ROWS * QUERIES + row_in, position = positions[t];
+        if (position < 0) continue;
+        const T* from = qkv + (token0 + t) * row_stride + R::first(lane);
+        T* to = static_cast<T*>(a.queries) + (size_t)(token0 + t) * a.n_heads * D + R::first(lane);
+        float x[QUERIES][8], y[QUERIES][8], c[8], s[8];
+        if (a.angles) angles_of(position, c, s);
+#pragma unroll
+        for (int i = 0; i < QUERIES; ++i)
+            if (head0 + i * ROWS < a.n_heads) {
+                load8(from + (head0 + i * ROWS) * D, x[i]);
+                load8(from + (head0 + i * ROWS) * D + R::APART, y[i]);
+            }
+#pragma unroll
+        for (int i = 0; i < QUERIES; ++i)
+            if (head0 + i * ROWS < a.n_heads) {
+                if (a.angles) R::turn(x[i], y[i], c, s);
+                store8(to + (head0 + i * ROWS) * D, x[i]);
+                store8(to + (head0 + i * ROWS) * D + R::APART, y[i]);
+            }
+    }
+}
+
+template <typename T, int D>
+void launch_vec(const Args& a, int* status, cudaStream_t stream) {
+    // blocks of threads for every SM several times, up to MAX_RUN tokens each
+    int run = a.n_tokens / (148 * 4);
+    run = run < 1 ? 1 : run > MAX_RUN ? MAX_RUN : run;
+    // few tokens: a token's work over several blocks of threads
+    const int blocks = (a.n_tokens + run - 1) / run, tasks = (a.write_cache ? 2 * a.n_kv_heads : 0) + (a.n_heads * D / 512 + QUERIES - 1) / QUERIES;
+    int slices = 148 * 4 / blocks;
+    slices = slices > (tasks + WARPS - 1) / WARPS ? (tasks + WARPS - 1) / WARPS : slices < 1 ? 1 : slices;
+    const dim3 grid(blocks, slices);
+    if (a.interleaved) llmb::launch(int8_append_vec_kernel<T, D, true>, grid, dim3(THREADS), 0, stream, true, a, run, status);
+    else llmb::launch(int8_append_vec_kernel<T, D, false>, grid, dim3(THREADS), 0, stream, true, a, run, status);
+}
+
 }  // namespace
 
 LLMB_EXPORT int llmb_int8_cache_status() {
@@ -185,8 +423,15 @@ LLMB_EXPORT int llmb_int8_append(const void* qkv, const float* angles, const int
     const int units = z.n_heads + (z.write_cache ? 2 * z.n_kv_heads : 0);
     const int rows = ceil_div(units, WARPS);
     LLMB_REQUIRE(rows <= 65535, "int8_append: too many heads");
-    int* status = nullptr;
-    if (tc::status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status, tc::status_word(), 0));
+    static int* status = nullptr;                // (one address for all devices)
+    if (!status && tc::status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status, tc::status_word(), 0));
+    auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+    if ((z.head_dim == 64 || z.head_dim == 128) && (a.n_rot == 0 || a.n_rot == z.head_dim) && aligned(qkv) && aligned(queries) && aligned(keys) &&
+        aligned(values) && aligned(angles)) {
+        if (z.dtype == LLMB_DTYPE_F32) z.head_dim == 64 ? launch_vec<float, 64>(a, status, stream) : launch_vec<float, 128>(a, status, stream);
+        else z.head_dim == 64 ? launch_vec<__nv_bfloat16, 64>(a, status, stream) : launch_vec<__nv_bfloat16, 128>(a, status, stream);
+        return check_launch("int8_append_vec");
+    }
     dim3 grid(z.n_tokens, rows);
     if (z.dtype == LLMB_DTYPE_F32) llmb::launch(int8_append_kernel<float>, grid, dim3(THREADS), 0, stream, true, a, status);
     else llmb::launch(int8_append_kernel<__nv_bfloat16>, grid, dim3(THREADS), 0, stream, true, a, status);

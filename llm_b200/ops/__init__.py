@@ -1669,15 +1669,16 @@ class Int8Pages:
     __slots__ = ("values", "scales", "block", "shape", "device")
 
     def __init__(self, values, scales):
-        if values.dim() != 4 or values.shape[2] != PAGE or values.dtype is not torch.int8 or not values.is_contiguous():
+        self.values, self.scales, self.shape, self.device = values, scales, values.shape, values.get_device()
+        if len(self.shape) != 4 or self.shape[2] != PAGE or values.dtype is not torch.int8 or not values.is_contiguous():
             raise KernelError(f"Int8Pages: values must be contiguous int8 [pages, kv heads, {PAGE}, dim], not {tuple(values.shape)} {values.dtype}")
-        if (scales.dim() != 3 or scales.shape[:2] != values.shape[:2] or scales.shape[2] not in (1, 2, 4, 8, 16, 32, 64)
-                or scales.dtype is not torch.float32 or not scales.is_contiguous() or scales.device != values.device):
-            raise KernelError(f"Int8Pages: scales must be contiguous float32 [{values.shape[0]}, {values.shape[1]}, {PAGE} / block] beside the values")
+        blocks = scales.shape
+        if (len(blocks) != 3 or blocks[0] != self.shape[0] or blocks[1] != self.shape[1] or blocks[2] not in (1, 2, 4, 8, 16, 32, 64)
+                or scales.dtype is not torch.float32 or not scales.is_contiguous() or scales.get_device() != self.device):
+            raise KernelError(f"Int8Pages: scales must be contiguous float32 [{self.shape[0]}, {self.shape[1]}, {PAGE} / block] beside the values")
         if values.data_ptr() % 16:
             raise KernelError("Int8Pages: values must start on 16 bytes")
-        self.values, self.scales, self.block = values, scales, PAGE // scales.shape[2]
-        self.shape, self.device = tuple(values.shape), values.get_device()
+        self.block = PAGE // blocks[2]
 
     def held(self, dtype=torch.bfloat16):
         """What the pages stand for, [pages, Hkv, 64, D] (exact in bfloat16 and float32)."""
@@ -1687,8 +1688,9 @@ class Int8Pages:
 def _check_int8(keys, values, n_kv_heads, head_dim, what: str) -> None:
     if type(keys) is not Int8Pages or type(values) is not Int8Pages:
         raise KernelError(f"{what}: keys and values are Int8Pages")
-    if keys.shape[1:] != (n_kv_heads, PAGE, head_dim) or values.shape != keys.shape or values.block != keys.block:
-        raise KernelError(f"{what}: keys {keys.shape} in blocks of {keys.block} and values {values.shape} in blocks of {values.block} "
+    shape = keys.shape
+    if shape[1] != n_kv_heads or shape[3] != head_dim or values.shape != shape or values.block != keys.block:
+        raise KernelError(f"{what}: keys {tuple(shape)} in blocks of {keys.block} and values {tuple(values.shape)} in blocks of {values.block} "
                           f"are no pages of {n_kv_heads} heads of {head_dim}, both alike")
 
 
@@ -1799,10 +1801,12 @@ def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seql
     dtype, n_seqs = qkv.dtype, seq_lens.numel()
     code = _code(dtype)
     _check_int8(keys, values, n_kv_heads, head_dim, what)
-    vectors = ((seq_lens, n_seqs, "seq_lens"), (cu_seqlens, n_seqs + 1, "cu_seqlens"))
-    if seq_order is not None:
-        vectors += ((seq_order, n_seqs, "seq_order"),)
-    _check_step(what, block_table, ring_pages, n_seqs, vectors)
+    int32, table = torch.int32, block_table.shape
+    if not (seq_lens.dtype is int32 and cu_seqlens.dtype is int32 and block_table.dtype is int32 and seq_order is None and len(table) == 2
+            and table[0] == n_seqs and 1 <= ring_pages <= table[1] and block_table.stride(1) == 1 and seq_lens.dim() == 1 and cu_seqlens.dim() == 1
+            and cu_seqlens.numel() == n_seqs + 1 and seq_lens.is_contiguous() and cu_seqlens.is_contiguous()):
+        vectors = ((seq_lens, n_seqs, "seq_lens"), (cu_seqlens, n_seqs + 1, "cu_seqlens"))
+        _check_step(what, block_table, ring_pages, n_seqs, vectors if seq_order is None else vectors + ((seq_order, n_seqs, "seq_order"),))
     if max_new < 1 or max_len < 1 or window < 0 or not math.isfinite(scale):
         raise KernelError(f"{what}: max_new {max_new}, max_len {max_len}, window {window}, scale {scale}")
     _check_device(what, keys, values, (qkv, block_table, seq_lens, cu_seqlens, seq_order, out))
