@@ -166,20 +166,25 @@ struct Begun {                                                 // a block of the
     int token, position, n_rows, page;
 };
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-    if constexpr (sizeof(T) == 2) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// eight values as they are in memory
+template <typename T> struct Raw {
+    uint4 v[sizeof(T) / 2];
+};
+template <typename T> __device__ __forceinline__ Raw<T> raw8(const T* p) {
+    Raw<T> r;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    } else {
-        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
-        *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+    return r;
+}
+template <typename T> __device__ __forceinline__ void unpack8(const Raw<T>& r, float (&x)[8]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (sizeof(T) == 2) x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+        else x[i] = __uint_as_float(w[i]);
     }
 }
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) { unpack8(raw8(p), x); }
 template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
     if constexpr (sizeof(T) == 2) {
         *reinterpret_cast<uint4*>(p) = make_uint4(tc::pack2(x[0], x[1]), tc::pack2(x[2], x[3]), tc::pack2(x[4], x[5]), tc::pack2(x[6], x[7]));
@@ -284,33 +289,37 @@ __global__ void __launch_bounds__(THREADS) int8_append_vec_kernel(const __grid_c
         signed char* to = block_rows + R::first(lane);
         float* scale_at = (keys ? a.key_scales : a.value_scales) + at * (LLMB_PAGE / a.block) + row / a.block;
         const float before = first != 0 ? *scale_at : 0.f;
-        float x[STEPS][8], y[STEPS][8];
-        auto fetch = [&](int r0, int i) {                      // rows r0 + i * ROWS + row_in: to place i
-            const int r = r0 + i * ROWS + row_in;
-            if (r < b.n_rows) {
-                load8(from + r * row_stride, x[i]);
-                load8(from + r * row_stride + R::APART, y[i]);
-            } else {
+        Raw<T> low[STEPS], high[STEPS];                        // as they came: rotated for the magnitude, and again for the whole numbers
+        auto fetch = [&](int r0) {                             // rows r0 + i * ROWS + row_in: to place i
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[i][k] = y[i][k] = 0.f;
+            for (int i = 0; i < STEPS; ++i) {
+                const int r = r0 + i * ROWS + row_in;
+                if (r < b.n_rows) {
+                    low[i] = raw8(from + r * row_stride);
+                    high[i] = raw8(from + r * row_stride + R::APART);
+                }
             }
         };
-        auto rotate = [&](int r0, int i) {
-            const int r = r0 + i * ROWS + row_in;
-            if (turned && r < b.n_rows) {
+        auto values_of = [&](int r, int i, float (&x)[8], float (&y)[8]) {
+            unpack8(low[i], x);
+            unpack8(high[i], y);
+            if (turned) {
                 float c[8], s[8];
                 angles_of(b.position + r, c, s);
-                R::turn(x[i], y[i], c, s);
+                R::turn(x, y, c, s);
             }
         };
         uint32_t most = 0;
         for (int r0 = 0; r0 < b.n_rows; r0 += HELD) {
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i) fetch(r0, i);
+            fetch(r0);
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) {
-                rotate(r0, i);
-                most = max(most, max(largest8(x[i]), largest8(y[i])));
+                const int r = r0 + i * ROWS + row_in;
+                if (r < b.n_rows) {
+                    float x[8], y[8];
+                    values_of(r, i, x, y);
+                    most = max(most, max(largest8(x), largest8(y)));
+                }
             }
         }
         float scale = __uint_as_float(scale_bits(__reduce_max_sync(0xffffffffu, most)));
@@ -334,16 +343,15 @@ __global__ void __launch_bounds__(THREADS) int8_append_vec_kernel(const __grid_c
         }
         const float inverse = is_number(scale) ? 1.f / scale : 0.f;
         for (int r0 = 0; r0 < b.n_rows; r0 += HELD) {
+            if (b.n_rows > HELD) fetch(r0);
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) {
-                if (b.n_rows > HELD) {
-                    fetch(r0, i);
-                    rotate(r0, i);
-                }
                 const int r = r0 + i * ROWS + row_in;
                 if (r < b.n_rows) {
-                    *reinterpret_cast<uint2*>(to + r * D) = inverse != 0.f ? whole8(x[i], inverse) : make_uint2(0u, 0u);
-                    *reinterpret_cast<uint2*>(to + r * D + R::APART) = inverse != 0.f ? whole8(y[i], inverse) : make_uint2(0u, 0u);
+                    float x[8], y[8];
+                    values_of(r, i, x, y);
+                    *reinterpret_cast<uint2*>(to + r * D) = inverse != 0.f ? whole8(x, inverse) : make_uint2(0u, 0u);
+                    *reinterpret_cast<uint2*>(to + r * D + R::APART) = inverse != 0.f ? whole8(y, inverse) : make_uint2(0u, 0u);
                 }
             }
         }
@@ -356,20 +364,24 @@ __global__ void __launch_bounds__(THREADS) int8_append_vec_kernel(const __grid_c
         if (position < 0) continue;
         const T* from = qkv + (token0 + t) * row_stride + R::first(lane);
         T* to = static_cast<T*>(a.queries) + (size_t)(token0 + t) * a.n_heads * D + R::first(lane);
-        float x[QUERIES][8], y[QUERIES][8], c[8], s[8];
+        Raw<T> low[QUERIES], high[QUERIES];
+        float c[8], s[8];
         if (a.angles) angles_of(position, c, s);
 #pragma unroll
         for (int i = 0; i < QUERIES; ++i)
             if (head0 + i * ROWS < a.n_heads) {
-                load8(from + (head0 + i * ROWS) * D, x[i]);
-                load8(from + (head0 + i * ROWS) * D + R::APART, y[i]);
+                low[i] = raw8(from + (head0 + i * ROWS) * D);
+                high[i] = raw8(from + (head0 + i * ROWS) * D + R::APART);
             }
 #pragma unroll
         for (int i = 0; i < QUERIES; ++i)
             if (head0 + i * ROWS < a.n_heads) {
-                if (a.angles) R::turn(x[i], y[i], c, s);
-                store8(to + (head0 + i * ROWS) * D, x[i]);
-                store8(to + (head0 + i * ROWS) * D + R::APART, y[i]);
+                float x[8], y[8];
+                unpack8(low[i], x);
+                unpack8(high[i], y);
+                if (a.angles) R::turn(x, y, c, s);
+                store8(to + (head0 + i * ROWS) * D, x);
+                store8(to + (head0 + i * ROWS) * D + R::APART, y);
             }
     }
 }
