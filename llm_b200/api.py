@@ -34,16 +34,17 @@ class LLM:
     model: a folder with config.json and model.safetensors, or a bound DecoderModel.
     context: most positions one sequence may hold (its prompt and what it generates).
     batch: most sequences generated together.
+    cache_dtype: "int8" holds the cache in 8 bits, half of bfloat16 (`Engine`).
     """
 
     def __init__(self, model, dtype="bfloat16", device="cuda:0", context: int = DEFAULT_CONTEXT,
-                 batch: int = 8, max_tokens_held: int | None = None):
+                 batch: int = 8, max_tokens_held: int | None = None, cache_dtype=None, cache_block: int = 16):
         if isinstance(model, (str, bytes)) or hasattr(model, "__fspath__"):
             model = load_model(model, parse_dtype(dtype), device)
         self.model = model
         context = min(context, model.spec.max_positions)
         held = max_tokens_held or batch * round_up(context)
-        self.engine = Engine(model, max_tokens=held, max_seq_len=context, max_slots=batch)
+        self.engine = Engine(model, max_tokens=held, max_seq_len=context, max_slots=batch, cache_dtype=cache_dtype, cache_block=cache_block)
         self.default_stop_tokens = tuple(model.spec.stop_tokens)
 
     def generate(self, prompts, max_tokens: int = DEFAULT_MAX_TOKENS, temperature: float = 0.7,
@@ -82,7 +83,7 @@ def load(model, **options) -> LLM:
 
 def generate(model, prompts, **options):
     """One call: load `model` (a folder) and generate. Options of `LLM` (dtype,
-    device, context, batch) and of `LLM.generate` may both be given."""
-    load_keys = ("dtype", "device", "context", "batch", "max_tokens_held")
+    device, context, batch, cache_dtype, cache_block) and of `LLM.generate` may both be given."""
+    load_keys = ("dtype", "device", "context", "batch", "max_tokens_held", "cache_dtype", "cache_block")
     llm = LLM(model, **{k: options.pop(k) for k in load_keys if k in options})
     return llm.generate(prompts, **options)

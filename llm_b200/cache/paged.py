@@ -14,6 +14,8 @@ serves a batch:
   values are wider or narrower than its keys, one tensor for the keys and one
   for the values) and, per slot, its own list of pages: logical page i of a
   sequence is `pages[i % ring]`;
+* with `kv_dtype` int8 the pages of every group hold keys and values in 8 bits with a scale
+  for each block of `kv_block` positions and head (ops.Int8Pages);
 * `state` tensors [slots, ...] hold what a mixer keeps per sequence at a fixed
   size; a slot's rows are zeroed when the slot is taken.
 
@@ -33,6 +35,7 @@ from dataclasses import dataclass, field
 import torch
 
 from .. import native
+from ..errors import LlmError
 from .allocator import FreeList
 
 PAGE = native.plan_constant("page")      # positions per cache page (csrc/plan.h)
@@ -100,6 +103,8 @@ class Group:
     storage: torch.Tensor | None = None               # [entries, 2, pages, Hkv, PAGE, D] (keys and values alike)
     keys: torch.Tensor | None = None                  # [entries, pages, Hkv, PAGE, D] and
     values: torch.Tensor | None = None                # [entries, pages, Hkv, PAGE, value_dim] where they differ
+    scales: torch.Tensor | None = None                # [entries, 2, pages, Hkv, PAGE / kv_block]: of a cache held in 8 bits
+    int8_views: list | None = None                    # (keys, values) of each entry as ops.Int8Pages
     slot_pages: _SlotPages | None = None              # slot -> list of physical pages
 
 
@@ -112,12 +117,17 @@ class PagedCache:
     the ring of window groups)."""
 
     def __init__(self, requests, states, max_tokens: int, max_seq_len: int, max_slots: int,
-                 dtype, device, step_tokens: int | None = None, block_states=None):
+                 dtype, device, step_tokens: int | None = None, block_states=None, kv_dtype=None, kv_block: int = 16):
         self.max_seq_len = max_seq_len
         self.max_slots = max_slots
         self.dtype = dtype
         self.device = torch.device(device)
         self.step_tokens = step_tokens or max_seq_len
+        if kv_dtype not in (None, dtype, torch.int8) or kv_block not in (1, 2, 4, 8, 16, 32, 64):
+            raise LlmError(f"a cache of {kv_dtype} in blocks of {kv_block} positions (int8, and a power of two up to {PAGE})")
+        self.int8 = kv_dtype is torch.int8
+        if self.int8 and any(r is not None and (r.values_are_keys or r.value_dim not in (None, r.head_dim) or r.head_dim % 2) for r in requests):
+            raise LlmError("a cache in 8 bits holds keys and values of one and the same even size")
         self.groups: list[Group] = []
         self.entry_group: list = []          # schedule entry -> (group index, index in group) or None
         by_key = {}
@@ -154,7 +164,11 @@ class PagedCache:
             elif group.value_dim == group.head_dim:
                 group.storage = torch.zeros(
                     (len(group.entries), 2, n_pages.value, group.n_kv_heads, PAGE, group.head_dim),
-                    dtype=dtype, device=self.device)
+                    dtype=torch.int8 if self.int8 else dtype, device=self.device)
+                if self.int8:
+                    from ..ops import Int8Pages
+                    group.scales = torch.zeros(group.storage.shape[:4] + (PAGE // kv_block,), dtype=torch.float32, device=self.device)
+                    group.int8_views = [tuple(Int8Pages(group.storage[i, j], group.scales[i, j]) for j in (0, 1)) for i in range(len(group.entries))]
             else:
                 shape = (len(group.entries), n_pages.value, group.n_kv_heads, PAGE)
                 group.keys = torch.zeros(shape + (group.head_dim,), dtype=dtype, device=self.device)
@@ -203,7 +217,7 @@ class PagedCache:
             flat = copies[:4 * n_copies.value]
             for g in set(flat[0::4]):
                 mine = [i for i in range(0, len(flat), 4) if flat[i] == g]
-                ops.copy_pages(self._pools(g), [flat[i + 1] for i in mine], [flat[i + 2] for i in mine], [flat[i + 3] for i in mine])
+                self._copy_pages(g, [flat[i + 1] for i in mine], [flat[i + 2] for i in mine], [flat[i + 3] for i in mine])
             states = [s for s in self.states + self.block_states if s is not None]
             if states:
                 ops.copy_slots(states, [int(slot)] * len(children), children)
@@ -216,17 +230,22 @@ class PagedCache:
     def compact(self) -> int:
         """Move the held pages of every group to the front of its pool, on the current stream: the first `pool.n_held` pages of a group's
         tensors are then all that is held (a cache to be saved or moved is one piece). Returns the number of pages moved."""
-        from .. import ops
         moved = 0
         for g, group in enumerate(self.groups):
             n = group.pool.count
             source, target, count = (c_int * n)(), (c_int * n)(), c_int()
             native.check(native.lib().llmh_cache_plan_compact(self._handle, g, source, target, byref(count)))
             if count.value:
-                ops.copy_pages(self._pools(g), source[:count.value], target[:count.value])
+                self._copy_pages(g, source[:count.value], target[:count.value])
                 native.check(native.lib().llmh_cache_apply_moves(self._handle, g, count, source, target))
                 moved += count.value
         return moved
+
+    def _copy_pages(self, group_index: int, source, target, rows=None) -> None:
+        from .. import ops
+        ops.copy_pages(self._pools(group_index), source, target, rows)
+        if self.groups[group_index].scales is not None:
+            ops.copy_page_scales(self.groups[group_index].scales, source, target)
 
     def _pools(self, group_index: int) -> list:
         group = self.groups[group_index]
@@ -279,12 +298,14 @@ class PagedCache:
 
     def layer_view(self, entry: int):
         """(group index, keys, values) of the schedule entry that owns storage:
-        keys and values are [pages, Hkv, 64, D]."""
+        keys and values are [pages, Hkv, 64, D] (ops.Int8Pages of a cache held in 8 bits)."""
         where = self.entry_group[entry]
         if where is None:
             return None
         g, i = where
         group = self.groups[g]
+        if group.int8_views is not None:
+            return (g, *group.int8_views[i])
         if group.storage is None:
             return g, group.keys[i], group.values[i]
         return g, group.storage[i, 0], group.storage[i, 1]
@@ -301,7 +322,7 @@ class PagedCache:
 
     def bytes(self) -> int:
         total = sum(t.numel() * t.element_size() for g in self.groups
-                    for t in (g.storage, g.keys, g.values if g.values is not g.keys else None) if t is not None)
+                    for t in (g.storage, g.scales, g.keys, g.values if g.values is not g.keys else None) if t is not None)
         total += sum(s.numel() * s.element_size() for s in self.states + self.block_states if s is not None)
         return total
 

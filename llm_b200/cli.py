@@ -1,7 +1,7 @@
 """Command line of the library, in the manner of MythEclipse/llm's `llm-cli`.
 
-    python -m llm_b200 [--model DIR] [--context 4096] [--max-tokens 256] [--temperature 0.7] [--samples 1] ID ...
-    python -m llm_b200 bench [-m DIR | --random SHAPE] [-c 4096] [-p 512] [-n 128] [-b 1] [-r 5] [-o json]
+    python -m llm_b200 [--model DIR] [--context 4096] [--max-tokens 256] [--temperature 0.7] [--samples 1] [--cache-dtype int8] ID ...
+    python -m llm_b200 bench [-m DIR | --random SHAPE] [-c 4096] [-p 512] [-n 128] [-b 1] [-r 5] [-o json] [--cache-dtype int8]
     python -m llm_b200 inspect DIR
     python -m llm_b200 random (--shape NAME | --config FILE) --out DIR [--seed S]
 
@@ -13,7 +13,7 @@ flags of apps/cli/src/bench.rs:45-71 (-m, -c, -p, -n, -r, -o with comma lists)
 and its two tests: `pp<N>` times the prefill of N tokens and nothing else,
 `tg<N>` prefills a 16-token prompt and times only the decoding of N tokens
 (bench.rs:10-12,27); `-b` adds the batch size; every test runs once uncounted before its `-r`
-repetitions. `inspect` prints the model's
+repetitions. `--cache-dtype int8` holds keys and values in 8 bits. `inspect` prints the model's
 geometry, checks the checkpoint's tensors and names the kernel variant each
 product and attention shape gets (apps/cli/src/inspect.rs:16-131).
 """
@@ -69,7 +69,7 @@ def _held_by_samples(model, prompt_tokens: int, max_tokens: int, context: int, s
 
 def complete(args) -> int:
     model, context, max_tokens, temperature, dtype = None, DEFAULT_CONTEXT, DEFAULT_MAX_TOKENS, 0.7, "bfloat16"
-    seed, prompt, samples = None, [], 1
+    seed, prompt, samples, cache_dtype = None, [], 1, None
     while args:
         a = args.pop(0)
         if a == "--model":
@@ -82,6 +82,8 @@ def complete(args) -> int:
             temperature = float(_value(args, a))
         elif a == "--dtype":
             dtype = _value(args, a)
+        elif a == "--cache-dtype":
+            cache_dtype = _value(args, a)
         elif a == "--seed":
             seed = int(_value(args, a))
         elif a == "--samples":
@@ -90,7 +92,8 @@ def complete(args) -> int:
             prompt += _int_list(a, "the prompt")
     if model is None or not prompt:
         raise SystemExit("usage: python -m llm_b200 --model DIR [--context N] [--max-tokens N] "
-                         "[--temperature T] [--dtype bfloat16|float32] [--seed S] [--samples N] TOKEN_ID ...")
+                         "[--temperature T] [--dtype bfloat16|float32] [--seed S] [--samples N] "
+                         "[--cache-dtype int8] TOKEN_ID ...")
     if samples < 1:
         raise SystemExit("--samples needs a number of at least 1")
     import llm_b200
@@ -99,7 +102,7 @@ def complete(args) -> int:
         from .api import parse_dtype
         from .engine import load_model
         bound = load_model(model, parse_dtype(dtype), "cuda:0")
-        llm = llm_b200.LLM(bound, context=context, batch=samples,
+        llm = llm_b200.LLM(bound, context=context, batch=samples, cache_dtype=cache_dtype,
                            max_tokens_held=_held_by_samples(bound, len(prompt), max_tokens, context, samples))
         (results,) = llm.generate([prompt], max_tokens=max_tokens, temperature=temperature, details=True, samples=samples, **options)
         for result in results:
@@ -108,7 +111,7 @@ def complete(args) -> int:
         print(f"[{results[0].prompt_tokens} prompt tokens, {drawn} generated in {samples} samples, ttft {results[0].ttft_ms:.0f} ms, "
               f"{sum(r.tokens_per_second for r in results):.1f} tok/s]", file=sys.stderr)
         return 0
-    llm = llm_b200.LLM(model, dtype=dtype, context=context, batch=1)
+    llm = llm_b200.LLM(model, dtype=dtype, context=context, batch=1, cache_dtype=cache_dtype)
     (result,) = llm.generate([prompt], max_tokens=max_tokens, temperature=temperature, details=True,
                              on_token=lambda i, t: print(t, end=" ", flush=True), **options)
     print()
@@ -120,7 +123,7 @@ def complete(args) -> int:
 
 def bench(args) -> int:
     model_dir, random_shape, context, dtype = None, None, DEFAULT_CONTEXT, "bfloat16"
-    prompts, gens, batches, reps, as_json, layers = [512], [128], [1], 5, False, None
+    prompts, gens, batches, reps, as_json, layers, cache_dtype = [512], [128], [1], 5, False, None, None
     while args:
         a = args.pop(0)
         if a in ("-m", "--model"):
@@ -143,6 +146,8 @@ def bench(args) -> int:
             as_json = _value(args, a).lower() == "json"
         elif a == "--dtype":
             dtype = _value(args, a)
+        elif a == "--cache-dtype":
+            cache_dtype = _value(args, a)
         else:
             raise SystemExit(f"unknown bench flag {a}")
     if (model_dir is None) == (random_shape is None):
@@ -166,7 +171,7 @@ def bench(args) -> int:
     rows = []
     for batch in batches:
         per_seq = round_up(context)
-        engine = Engine(model, max_tokens=batch * per_seq, max_seq_len=context, max_slots=batch)
+        engine = Engine(model, max_tokens=batch * per_seq, max_seq_len=context, max_slots=batch, cache_dtype=cache_dtype)
         for n in prompts:
             samples = []
             for rep in range(reps + 1):            # the first run is not counted: it plans the scratch

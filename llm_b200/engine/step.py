@@ -23,7 +23,7 @@ from .. import native, ops
 from ..cache import PAGE, PagedCache, round_up
 from ..errors import FormatError, LlmError
 from ..parts.base import SharedPages, StepContext
-from .workspace import Workspace
+from .workspace import BufferRequest, Workspace
 
 
 GRAPH_AFTER_STEPS = 2      # plain steps of a shape before it is captured
@@ -92,11 +92,15 @@ class Engine:
         arena); a larger step is run as several passes over subsets of its tokens.
     use_graphs: replay decode steps from CUDA graphs (only if every part of the
         model says it can be captured).
+    cache_dtype: "int8" holds keys and values in 8 bits with a scale for each block of
+        `cache_block` positions and head (for models whose attentions say that they can
+        read that); None: in the run's type. Forked sequences hold shared pages once there
+        too, and each reads them for itself.
     """
 
     def __init__(self, model, max_tokens: int, max_seq_len: int | None = None,
                  max_slots: int | None = None, step_tokens: int | None = None,
-                 use_graphs: bool = True, pass_tokens: int = 65536):
+                 use_graphs: bool = True, pass_tokens: int = 65536, cache_dtype=None, cache_block: int = 16):
         if model.embedding is None:
             raise LlmError("the model has no weights bound")
         self.model = model
@@ -108,7 +112,15 @@ class Engine:
         self.max_slots = max_slots or max(1, max_tokens // PAGE)
         self.step_tokens = step_tokens or self.max_seq_len
         self.pass_tokens = max(int(pass_tokens), 1)
-        ops.ensure_built(model.libraries())
+        if cache_dtype not in (None, "int8", torch.int8):
+            raise LlmError(f"a cache of {cache_dtype} (int8, or None for the run's type)")
+        int8 = cache_dtype is not None
+        mixers = [model.blocks[item.layer].mixer for item in model.spec.schedule]
+        if int8:
+            for mixer in mixers:
+                if mixer.kv_request() is not None and not mixer.serves_int8_cache:
+                    raise LlmError(f"{type(mixer).__name__} does not read a cache in 8 bits")
+        ops.ensure_built(model.libraries() + (["int8_cache", "attention_int8"] if int8 else []))
         # every product and attention shape of this model must have a kernel: a size that none
         # accepts (a head size above the kernels' limit) is refused here, not in the first step
         self.kernel_plan = model.plan_identity()
@@ -116,16 +128,23 @@ class Engine:
         kv, states = model.cache_requests()
         self.cache = PagedCache(kv, states, max_tokens, self.max_seq_len, self.max_slots,
                                 self.dtype, self.device, self.step_tokens,
-                                block_states=model.block_state_requests())
+                                block_states=model.block_state_requests(), kv_dtype=torch.int8 if int8 else None, kv_block=cache_block)
         self.vocab = model.spec.vocab
         self.steps_run = 0
-        self.workspace = Workspace(self.device, model.scratch_requests)
+        queries = max((m.int8_queries for m in mixers), default=0) if int8 else 0
+
+        def scratch_requests(n_tokens):
+            wanted = model.scratch_requests(n_tokens)
+            if queries:                   # nobody else's for the whole of a layer
+                wanted = wanted + [BufferRequest("int8_queries", (n_tokens, queries), self.dtype, 0, max((r.last_use for r in wanted), default=0))]
+            return wanted
+        self.workspace = Workspace(self.device, scratch_requests)
         self.scope = ops.StepScope()      # the kernels' own scratch: one for all steps, as they have one arena
         self.use_graphs = (use_graphs and self.device.type == "cuda"
                            and os.environ.get("LLMB_NO_GRAPHS", "0") in ("", "0")
                            and not ops.PROFILING
                            and getattr(model, "graph_safe", lambda: False)())
-        self.sharing_shapes = model.sharing_shapes()      # the attentions that can read shared pages once
+        self.sharing_shapes = () if int8 else model.sharing_shapes()      # the attentions that can read shared pages once
         self._graphs, self._graph_seen, self._graph_pool = {}, {}, None
         self.graph_replays = 0            # decode steps run from a captured graph so far
         # passes that are not replayed from a graph (prompts, mixed steps, the first steps of a
@@ -273,6 +292,8 @@ class Engine:
         if logits is None and self.use_records and not graphable:
             step = _HostStep(n_tokens, batch.n, decode, *lengths(), max_len)
             key = self.model.replay_key(step, sizes[6])
+            if key is not None and self.cache.int8:
+                key = (key, ops.attention_int8_replay_key(step))
             if key is not None and sizes[6] * self.vocab <= MAX_RECORDED_LOGITS:
                 if sharing is not None:
                     key = (key, sharing)

@@ -1660,6 +1660,18 @@ def copy_slots(states, source, target) -> None:
     _copy_items(shapes, states[0].shape[0] if states else 0, source, target, None, "copy_slots")
 
 
+def copy_page_scales(scales, source, target) -> None:
+    """scales[..., target[i], :, :] = scales[..., source[i], :, :] for all i, in place: the scales that belong to copied pages of a cache held
+    in 8 bits. `scales`: contiguous [..., pages, heads, blocks]; the rest as in `copy_pages`."""
+    _require_cuda(scales)
+    if scales.dim() < 3 or not scales.is_contiguous():
+        raise KernelError("copy_page_scales: scales must be contiguous [..., pages, heads, blocks]")
+    pages, heads, blocks = scales.shape[-3:]
+    page = heads * blocks * scales.element_size()
+    outers = scales.numel() // max(pages * heads * blocks, 1)
+    _copy_items([(scales.data_ptr(), outers, 1, pages * page, page, 0, page)] if scales.numel() else [], pages, source, target, None, "copy_page_scales")
+
+
 # ----------------------------------------------------------------------------- a cache held in 8 bits
 
 class Int8Pages:
@@ -1831,6 +1843,11 @@ def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seql
           None if seq_order is None else seq_order.data_ptr(), at_out, parts.data_ptr() if floats else None, floats, float(scale), at_sizes,
           _stream(), kernels=kernels)
     return out
+
+
+def attention_int8_replay_key(step):
+    """What the launches of `attention_int8` depend on beyond the token and sequence counts (Part.replay_key)."""
+    return (max(step.new_counts), page_bucket(-(-step.max_len // PAGE)))
 
 
 # ----------------------------------------------------------------------------- latent attention, shared rotated keys
@@ -2286,7 +2303,7 @@ def required_libraries() -> list:
             "attention_decode", "attention_prefill", "attention_prefill_tc", "sampling"]
 
 
-__all__ = ["PAGE", "GLU_BLOCK", "glu_fusable", "embed", "scale_", "random_normal_", "begin_recording", "end_recording", "RecordedPass", "StepScope", "scratch_generation", "Emit", "FoldedNorm", "RopeWrite", "cast_sumsq", "SUMSQ_LD", "rmsnorm", "swiglu", "rope_cache_write", "linear", "attention", "prefix_attention", "prefix_attention_pays", "page_bucket", "Int8Pages", "rope_cache_write_int8", "attention_int8", "copy_pages", "copy_slots",
+__all__ = ["PAGE", "GLU_BLOCK", "glu_fusable", "embed", "scale_", "random_normal_", "begin_recording", "end_recording", "RecordedPass", "StepScope", "scratch_generation", "Emit", "FoldedNorm", "RopeWrite", "cast_sumsq", "SUMSQ_LD", "rmsnorm", "swiglu", "rope_cache_write", "linear", "attention", "prefix_attention", "prefix_attention_pays", "page_bucket", "Int8Pages", "rope_cache_write_int8", "attention_int8", "attention_int8_replay_key", "copy_page_scales", "copy_pages", "copy_slots",
            "softcap_", "add_rows_", "conv_rope_cache_write", "diff_attention", "tanh_norm", "norm_rope_cache_write",
            "sigmoid_attention", "gated_recurrence", "state_space", "attention_replay_key", "layernorm", "input_conv", "output_norm_add_", "forget_recurrence",
            "latent_write", "head_products", "latent_attention", "latent_prefill", "attention_decode_splits", "sigmoid_attention_replay_key", "sigmoid_decode_splits", "sigmoid_mixed_heads", "sigmoid_mixed_elements",

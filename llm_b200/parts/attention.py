@@ -17,6 +17,7 @@ class AttentionMixer(Mixer):
     scale, the window, the biases and the position encoding as parameters."""
     graph_safe = True
     emits = True
+    serves_int8_cache = True
     libraries = ("elementwise", "gemm_simt", "gemm_skinny", "gemm_tc", "attention_generic", "attention_decode", "attention_decode_window", "attention_prefill", "attention_prefill_tc", "prefix_attention")
 
     def __init__(self, spec):
@@ -27,6 +28,10 @@ class AttentionMixer(Mixer):
     @property
     def q_width(self):
         return self.spec.n_heads * self.spec.head_dim
+
+    @property
+    def int8_queries(self):
+        return self.q_width
 
     @property
     def kv_width(self):
@@ -112,6 +117,16 @@ class AttentionMixer(Mixer):
         angles = self.position.table if self.position is not None else None
         interleaved = self.position.interleaved if self.position is not None else False
         out = ctx.scratch("qkv", (n, self.q_width + 2 * self.kv_width), h.dtype)
+        mixed = ctx.scratch("mixed", (n, self.q_width), h.dtype)
+        if isinstance(keys, ops.Int8Pages):
+            qkv = ops.linear(h, self.w_qkv, self.b_qkv, out=out, norm=norm)
+            queries = ops.rope_cache_write_int8(qkv, angles, ctx.tok_pos, ctx.tok_seq, ctx.cu_seqlens, table, ring, keys, values, s.n_heads,
+                                                s.n_kv_heads, s.head_dim, interleaved=interleaved, write_cache=(entry == cache_entry),
+                                                out=ctx.scratch("int8_queries", (n, self.q_width), h.dtype))
+            mixed = ops.attention_int8(queries, keys, values, table, ring, ctx.seq_lens, ctx.cu_seqlens, s.n_heads, s.n_kv_heads, s.head_dim,
+                                       s.scale, s.window, max_new=max(ctx.new_counts), max_len=ctx.max_len, out=mixed, seq_order=ctx.seq_order)
+            ops.linear(mixed, self.w_o, self.b_o, residual=residual, emit=emit)
+            return
         if h.dtype == torch.bfloat16 and (angles is None or angles.shape[1] == s.head_dim):
             # the rotation and the cache write ride in the product's epilogue where its kernel has them
             qkv = ops.linear(h, self.w_qkv, self.b_qkv, out=out, norm=norm, rope=ops.RopeWrite(
@@ -122,7 +137,6 @@ class AttentionMixer(Mixer):
             ops.rope_cache_write(qkv, angles, ctx.tok_pos, ctx.tok_seq, table, ring, keys, values, s.n_heads,
                                  s.n_kv_heads, s.head_dim, interleaved=interleaved,
                                  write_cache=(entry == cache_entry))
-        mixed = ctx.scratch("mixed", (n, self.q_width), h.dtype)
         share = ctx.sharing
         if share is not None and s.window == 0 and (s.n_heads, s.n_kv_heads, s.head_dim) in share.shapes:
             mixed = ops.prefix_attention(qkv, keys, values, table, ctx.seq_lens, ctx.cu_seqlens, share.group_first, share.group_pages,
