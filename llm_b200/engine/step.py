@@ -131,14 +131,13 @@ class Engine:
                                 block_states=model.block_state_requests(), kv_dtype=torch.int8 if int8 else None, kv_block=cache_block)
         self.vocab = model.spec.vocab
         self.steps_run = 0
-        queries = max((m.int8_queries for m in mixers), default=0) if int8 else 0
-
-        def scratch_requests(n_tokens):
-            wanted = model.scratch_requests(n_tokens)
-            if queries:                   # nobody else's for the whole of a layer
-                wanted = wanted + [BufferRequest("int8_queries", (n_tokens, queries), self.dtype, 0, max((r.last_use for r in wanted), default=0))]
-            return wanted
-        self.workspace = Workspace(self.device, scratch_requests)
+        wanted = model.scratch_requests
+        if int8:
+            # (nothing here refers to the engine: its captured steps go when its last name does, not whenever garbage is collected)
+            def wanted(n_tokens, requests=model.scratch_requests, columns=max((m.int8_queries for m in mixers), default=0), dtype=self.dtype):
+                buffers = requests(n_tokens)
+                return buffers + [BufferRequest("int8_queries", (n_tokens, columns), dtype, 0, max((r.last_use for r in buffers), default=0))]
+        self.workspace = Workspace(self.device, wanted)
         self.scope = ops.StepScope()      # the kernels' own scratch: one for all steps, as they have one arena
         self.use_graphs = (use_graphs and self.device.type == "cuda"
                            and os.environ.get("LLMB_NO_GRAPHS", "0") in ("", "0")

@@ -1,5 +1,8 @@
 """The engine with a cache held in 8 bits: host logic on the CPU, the kernels replaced by their plain statements. What is under test is which rows,
 pages, scales and slots the operators are given."""
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -114,6 +117,22 @@ def test_half_the_bytes_and_refusals(tmp_path, plain_kernels, monkeypatch):
         monkeypatch.setattr(mixer, "serves_int8_cache", False)
     with pytest.raises(LlmError, match="does not read"):
         Engine(engine.model, max_tokens=2048, cache_dtype="int8")
+
+
+@pytest.mark.parametrize("options", [{}, {"cache_dtype": None}])
+def test_an_engine_goes_with_its_last_name(tmp_path, plain_kernels, monkeypatch, options):
+    """Captured steps that are destroyed by the garbage collector while another engine captures end that capture."""
+    config, weights, engine = setup(tmp_path, monkeypatch, sorted(CONFIGS)[0], **options)
+    (slot,) = engine.acquire()
+    engine.step([Entry(slot, [1, 2, 3], [2])])
+    gone = weakref.ref(engine)
+    gc.collect()
+    gc.disable()
+    try:
+        del engine
+        assert gone() is None
+    finally:
+        gc.enable()
 
 
 def test_mixers_of_other_designs_are_refused(tmp_path, plain_kernels):
