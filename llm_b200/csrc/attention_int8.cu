@@ -1017,11 +1017,11 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_few_join_kerne
 // The steps of all (sequence, key head, tile), one after the other, are dealt out to the blocks in ranges of equal length, as pages are above; barriers
 // and buffers run on from one tile to the next, so the next tile's keys are fetched and widened while a result is written.
 
-constexpr int WIDE_THREADS = 512;           // warps 0 products, 1 pages and scales, 4-7 and 8-11 a tile's softmax, 12-15 widening
+constexpr int WIDE_THREADS = 768;           // warps 0 products, 1 pages and scales, 4-11 and 12-19 a tile's softmax (four for each page), 20-23 widening
 constexpr int WIDE_ROWS = 256, TILE_ROWS = 128, STEP = 128, STEP_PAGES = STEP / LLMB_PAGE;
 constexpr int TILE_PIECE = TILE_ROWS * 128, STEP_PIECE = STEP * 128;             // 64 columns of the head: 16 KB
-constexpr int REGS_ISSUE = 96, REGS_SOFTMAX = 168, REGS_WIDEN = 80, REGS_LAUNCHED = 128;
-static_assert(128 * (REGS_ISSUE + 2 * REGS_SOFTMAX + REGS_WIDEN) <= WIDE_THREADS * REGS_LAUNCHED, "the shares come from what the block is launched with");
+constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 88, REGS_WIDEN = 56, REGS_LAUNCHED = 80;
+static_assert(128 * (REGS_ISSUE + 4 * REGS_SOFTMAX + REGS_WIDEN) <= WIDE_THREADS * REGS_LAUNCHED, "the shares come from what the block is launched with");
 constexpr int WIDE_UP = 7;                  // power of two that weights are lifted to; R may lag 2^8 behind
 constexpr int VALUE_SPAN = 90;
 constexpr int INFOS = 4;                    // steps whose scales are on their way to the softmax: the step behind the next one may be widened by then
@@ -1038,7 +1038,6 @@ struct StepInfo {
     float k_unit, v_unit[2];         // what a step of the keys stands for; exponent of the values' reference, of each page
     uint32_t any_bad;
     uint32_t bad[4];                 // positions whose scale is no number
-    uint32_t packed[STEP];           // fp16 scales: key's low, value's high
 };
 
 // A tile of a (sequence, key head) and its pages.
@@ -1160,16 +1159,18 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
     unsigned char* raw_k = v_tile + 2 * STEP_BYTES;           // a step's bytes
     unsigned char* raw_v = raw_k + STEP * HD;
     StepInfo* infos = reinterpret_cast<StepInfo*>(raw_v + STEP * HD);            // [INFOS]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(infos + INFOS);
+    unsigned short* step_scales = reinterpret_cast<unsigned short*>(infos + INFOS);      // [2][STEP] fp16 scales of the bytes' positions
+    uint32_t* shared_rows = reinterpret_cast<uint32_t*>(step_scales + 2 * STEP);         // [tile][page][row] what the two warps of a row tell one another
+    uint64_t* bars = reinterpret_cast<uint64_t*>(shared_rows + 4 * TILE_ROWS);
     uint64_t* q_full = bars;                  // [2] a tile's queries are in shared memory, its last result is out of tensor memory
     uint64_t* k_full = bars + 2;              // [2]
     uint64_t* k_empty = bars + 4;             // [2]
     uint64_t* v_full = bars + 6;              // [2]
     uint64_t* v_empty = bars + 8;             // [2]
     uint64_t* s_full = bars + 10;             // [2] a tile's scores are complete (and all its products before)
-    uint64_t* p_full = bars + 12;             // [2][2] its weights of 64 positions are written and O has been rescaled
+    uint64_t* p_full = bars + 12;             // [2][2] its weights of a page are written, and (with the first page's) O has been rescaled
     uint64_t* o_full = bars + 16;             // [2] the tile's last P V is complete
-    uint64_t* raw_full = bars + 18;           // [2] a step's keys as bytes and its scales, its values as bytes
+    uint64_t* raw_full = bars + 18;           // [2] a step's keys as bytes and their scales, its values and theirs
     uint64_t* raw_empty = bars + 20;          // [2]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -1178,8 +1179,9 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
     if (threadIdx.x == 0) {
 #pragma unroll 1
         for (int i = 0; i < 22; ++i) {
-            const bool by_group = i < 4 || i == 6 || i == 7 || (i >= 12 && i < 16) || i >= 20;
-            mbar_init(smem_u32(&bars[i]), by_group ? 128 : i == 18 ? 2 : 1);
+            const bool by_all = i < 2 || i == 12 || i == 14;                      // a tile's eight warps; four below
+            const bool by_group = i == 2 || i == 3 || i == 6 || i == 7 || i == 13 || i == 15 || i >= 20;
+            mbar_init(smem_u32(&bars[i]), by_all ? 256 : by_group ? 128 : i >= 18 ? 2 : 1);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1276,8 +1278,9 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                     // 16 positions a product: 8 columns of weights, 2048 bytes of value rows; a segment's first one overwrites O
                     if (elect_one()) {
 #pragma unroll
-                        for (int j = 4 * half; j < 4 * half + 4; ++j)
-                            tcgen05_mma_ts(o, p + j * 8, v_desc0 + b * BUFFER + (uint64_t)((j * 2048) >> 4), idesc_pv, first && j == 0 ? 0u : 1u);
+                        for (int j = 0; j < 4; ++j)
+                            tcgen05_mma_ts(o, p + half * LLMB_PAGE + j * 8, v_desc0 + b * BUFFER + (uint64_t)(((half * 4 + j) * 2048) >> 4), idesc_pv,
+                                           first && half == 0 && j == 0 ? 0u : 1u);
                     }
                     __syncwarp();
                 }
@@ -1384,8 +1387,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                         ve[k] = max(ve[k], value_top - VALUE_SPAN);
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        info.packed[lane + 32 * j] = pack_f16(power_of((int)ks[j], ke), power_of((int)vs[j], ve[j >> 1]));
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t both = pack_f16(power_of((int)ks[j], ke), power_of((int)vs[j], ve[j >> 1]));
+                        step_scales[lane + 32 * j] = (unsigned short)both;
+                        vs[j] = both >> 16;
+                    }
                     if (lane == 0) {
                         info.k_unit = __uint_as_float((uint32_t)max(ke - SCALE_UP, 1) << 23);
                         info.v_unit[0] = (float)(ve[0] - 127);
@@ -1399,11 +1405,15 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                     ok = st == 0 || mbar_wait_warp(smem_u32(&raw_empty[1]), (st - 1) & 1, abort_flag, status, 44);
                     if (!ok) break;
                     copy(raw_v, a.values, &raw_full[1], pages);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) step_scales[STEP + lane + 32 * j] = (unsigned short)vs[j];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&raw_full[1]));
                 }
                 if (st < total && ok) next_segment(a, segment);
             }
         }
-    } else if (warp >= 12) {
+    } else if (warp >= 20) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_WIDEN));
         constexpr int LANES = HD / 16, RPP = 128 / LANES, PASSES = STEP / RPP;        // lanes of a row, rows of a pass
         const int t = threadIdx.x & 127, c = t % LANES, row_in = t / LANES;
@@ -1413,10 +1423,9 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
             const int st = i >> 1, which = i & 1, b = st & 1;
             uint64_t* full = bars + 2 + 4 * which + b;         // (k_full, v_full and their like)
             uint64_t* empty = bars + 4 + 4 * which + b;
-            const uint32_t* packed = infos[st % INFOS].packed;
+            const unsigned short* scale = step_scales + which * STEP;
             const unsigned char* raw = (which ? raw_v : raw_k) + c * 16;
             unsigned char* to = (which ? v_tile : k_tile) + b * STEP_BYTES + (c >> 2) * STEP_PIECE;
-            const uint32_t select = which ? 0x3232u : 0x1010u;
             ok = mbar_wait_warp(smem_u32(&raw_full[which]), st & 1, abort_flag, status, 41) &&
                  (st < 2 || mbar_wait_warp(smem_u32(empty), ((st >> 1) - 1) & 1, abort_flag, status, 31));
             if (!ok) break;
@@ -1430,7 +1439,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                     const int row = (i0 + j) * RPP + row_in;
                     x[j][0] = *reinterpret_cast<const uint2*>(raw + row * HD + flip * 8);
                     x[j][1] = *reinterpret_cast<const uint2*>(raw + row * HD + (1 - flip) * 8);
-                    s[j] = __byte_perm(packed[row], 0, select);
+                    s[j] = scale[row] * 0x10001u;
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -1446,13 +1455,20 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
-        const int tile = (warp >> 2) - 1, quarter = warp & 3, r = quarter * 32 + lane;       // row of the tile = lane of tensor memory
+        // Two warps a row, one for each page of a step: they agree on the maximum, and each has its half of O's columns. (With one warp a row, 128 scores
+        // one after the other, a step took 4,300 cycles; the loops stay short all the same.)
+        const int tile = ((warp >> 2) - 1) >> 1, part = ((warp >> 2) - 1) & 1, quarter = warp & 3, r = quarter * 32 + lane;       // r: row of the tile = lane of tensor memory
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t s_addr = lane_addr + tile * SCORES, o_addr = lane_addr + O_FIRST + tile * HD;
-        unsigned char* my_row = q_tile + tile * Q_BYTES + r * 128;          // 128 bytes of each piece; its 16-byte chunks are swizzled
+        const uint32_t s_addr = lane_addr + tile * SCORES, o_addr = lane_addr + O_FIRST + tile * HD + part * (HD / 2);
+        constexpr int PART_CHUNKS = HD / 16;                   // 16-byte chunks of this warp's half of a row of queries, or of a result on its way
+        unsigned char* region = q_tile + tile * Q_BYTES + (HD == 128 ? part * TILE_PIECE : 0);
+        auto place = [&](int row, int chunk) { return reinterpret_cast<uint4*>(region + row * 128 + (((chunk + (HD == 128 ? 0 : part * PART_CHUNKS)) ^ (row & 7)) << 4)); };
+        uint32_t* mine = shared_rows + (tile * 2 + part) * TILE_ROWS + r;
+        const uint32_t* theirs = shared_rows + (tile * 2 + 1 - part) * TILE_ROWS + r;
+        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + quarter) : "memory"); };         // the two warps of these rows
         uint32_t turns = 0, segments = 0;
         bool ok = true;
-        for (int st = 0; st < total && ok;) {
+        for (int st = 0; st < total;) {
             int skip, count;
             share_of(segment, skip, count);
             const int n_tiles = segment.n_rows > TILE_ROWS ? 2 : 1, end = st + count;
@@ -1467,196 +1483,187 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                 // once a tile is written in short loops: its instructions are not at hand, and unrolled it took twice the time.)
                 float row_scale;
                 {
-                    constexpr int CHUNKS = HD / 8, ROWS = 32 / CHUNKS;           // 16-byte chunks of a row, rows to an instruction
-                    const int chunk = lane % CHUNKS;
-                    const __nv_bfloat16* q = behind_wait(static_cast<const __nv_bfloat16*>(a.q)) + (size_t)(segment.head * share) * HD + chunk * 8;
-                    int from = segment.row0 + tile * TILE_ROWS + quarter * 32 + lane / CHUNKS, token0 = from / share, head0 = from - token0 * share;
+                    constexpr int ROWS = 32 / PART_CHUNKS;                       // rows to an instruction
+                    const int chunk = lane % PART_CHUNKS;
+                    const __nv_bfloat16* q = behind_wait(static_cast<const __nv_bfloat16*>(a.q)) + (size_t)(segment.head * share) * HD + part * (HD / 2) + chunk * 8;
+                    int from = segment.row0 + tile * TILE_ROWS + quarter * 32 + lane / PART_CHUNKS, token0 = from / share, head0 = from - token0 * share;
                     token0 += segment.span.first_token;
-#pragma unroll 4
-                    for (int i = lane / CHUNKS; i < 32; i += ROWS) {
+#pragma unroll 2
+                    for (int i = lane / PART_CHUNKS; i < 32; i += ROWS) {
                         const int row = quarter * 32 + i;
-                        unsigned char* to = q_tile + tile * Q_BYTES + (chunk >> 3) * TILE_PIECE + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
-                        if (row < tile_rows) cp_async16(to, q + (size_t)token0 * a.q_stride + (size_t)head0 * HD);
-                        else *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
+                        if (row < tile_rows) cp_async16(place(row, chunk), q + (size_t)token0 * a.q_stride + (size_t)head0 * HD);
+                        else *place(row, chunk) = make_uint4(0u, 0u, 0u, 0u);
                         for (head0 += ROWS; head0 >= share; head0 -= share) ++token0;
                     }
                     cp_async_commit();
                     cp_async_wait<0>();
                     __syncwarp();
-                    auto place = [&](int i) { return reinterpret_cast<uint4*>(my_row + (i >> 3) * TILE_PIECE + (((i & 7) ^ (r & 7)) << 4)); };
                     uint32_t most = 0;
-#pragma unroll 4
-                    for (int i = 0; i < CHUNKS; ++i) {
-                        const uint4 x = *place(i);
+#pragma unroll 2
+                    for (int i = 0; i < PART_CHUNKS; ++i) {
+                        const uint4 x = *place(r, i);
                         most = __vmaxu2(most, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
                     }
-                    most = max(most & 0xffffu, most >> 16);
-                    const int exponent = max((int)(most >> 7), 27) - 127;
+                    *mine = max(most & 0xffffu, most >> 16);
+                    meet();
+                    const int exponent = max((int)(max(*mine, *theirs) >> 7), 27) - 127;
                     const float factor = __uint_as_float((uint32_t)(14 - exponent + 127) << 23);
                     row_scale = a.scale_log2 * __uint_as_float((uint32_t)max(exponent - 14 + 127, 1) << 23);
 #pragma unroll 2
-                    for (int i = 0; i < CHUNKS; ++i) {
-                        const uint4 x = *place(i);
+                    for (int i = 0; i < PART_CHUNKS; ++i) {
+                        const uint4 x = *place(r, i);
                         auto both = [&](uint32_t w) { return pack_f16(__uint_as_float(w << 16) * factor, __uint_as_float(w & 0xffff0000u) * factor); };
-                        *place(i) = make_uint4(both(x.x), both(x.y), both(x.z), both(x.w));
+                        *place(r, i) = make_uint4(both(x.x), both(x.y), both(x.z), both(x.w));
                     }
                 }
                 fence_async_shared();
                 tcgen05_fence_before();                        // (the last result has been read)
                 mbar_arrive(smem_u32(&q_full[tile]));
                 float run_max = -INFINITY, ref = -INFINITY, run_sum = 0.f;
-                for (int i = st; i < end && ok; ++i) {
-                    ok = mbar_wait_warp(smem_u32(&s_full[tile]), turns++ & 1, abort_flag, status, 38);
-                    if (!ok) break;
+                for (int i = st; i < end; ++i) {
+                    ok = ok && mbar_wait_warp(smem_u32(&s_full[tile]), turns++ & 1, abort_flag, status, 38);
                     tcgen05_fence_after();
+                    if (!ok) {                                 // (a wait has run out: the other warp of the rows may not know yet, and is met all the same)
+                        if (!idle) meet();
+                        continue;
+                    }
                     if (idle) {
                         mbar_arrive(smem_u32(&p_full[2 * tile]));
-                        mbar_arrive(smem_u32(&p_full[2 * tile + 1]));
+                        if (part) mbar_arrive(smem_u32(&p_full[2 * tile + 1]));
                         continue;
                     }
                     const StepInfo& info = infos[i % INFOS];
                     const float c = fmaxf(row_scale * info.k_unit, 1.1754944e-38f);
-                    const int key0 = (segment.first_page + (skip + i - st) * STEP_PAGES) * LLMB_PAGE;
-                    const int last = my_pos - key0, first = my_first - key0;       // the positions of the step that the row sees
-                    const bool masked = __any_sync(0xffffffffu, last < STEP - 1 || first > 0) || info.any_bad;
-                    // Scores are read twice, a page at a time, by loops that are not unrolled: kept in registers, with all four quarters' code in a
-                    // row, warps spent a fifth of their time waiting for instructions.
-                    float top0 = -INFINITY, top1 = -INFINITY;
+                    const int key0 = (segment.first_page + (skip + i - st) * STEP_PAGES + part) * LLMB_PAGE;
+                    const int last = my_pos - key0, first = my_first - key0;       // the positions of the page that the row sees
+                    const uint32_t page_addr = s_addr + part * LLMB_PAGE;
+                    const bool masked = __any_sync(0xffffffffu, last < LLMB_PAGE - 1 || first > 0) || info.any_bad;
+                    float top = -INFINITY;
 #pragma unroll 1
-                    for (int half = 0; half < STEP_PAGES; ++half) {
-                        uint32_t x0[32], x1[32];
-                        tmem_ld32_start(s_addr + half * LLMB_PAGE, x0);
-                        tmem_ld32_start(s_addr + half * LLMB_PAGE + 32, x1);
-                        tmem_ld32_wait(x0);
-                        tmem_ld32_wait(x1);
+                    for (int from = 0; from < LLMB_PAGE; from += 32) {
+                        uint32_t x[32];
+                        tmem_ld32(page_addr + from, x);
                         if (masked) {                          // what the row does not see: -inf, in tensor memory too
-                            auto mask = [&](uint32_t (&x)[32], int from) {
-                                const uint32_t bad = info.bad[from >> 5];
-                                const int most = last - from, least = first - from;
+                            const uint32_t bad = info.bad[2 * part + (from >> 5)];
+                            const int most = last - from, least = first - from;
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) {
-                                    if (bad >> j & 1) x[j] = 0x7fffffffu;
-                                    if (j > most || j < least) x[j] = __float_as_uint(-INFINITY);
-                                }
-                                tmem_st32(s_addr + from, x);
-                            };
-                            mask(x0, half * LLMB_PAGE);
-                            mask(x1, half * LLMB_PAGE + 32);
-                            tmem_st_wait();
+                            for (int j = 0; j < 32; ++j) {
+                                if (bad >> j & 1) x[j] = 0x7fffffffu;
+                                if (j > most || j < least) x[j] = __float_as_uint(-INFINITY);
+                            }
+                            tmem_st32(page_addr + from, x);
                         }
                         float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            t0 = max3(t0, __uint_as_float(x0[j]), __uint_as_float(x0[j + 1]));
-                            t1 = max3(t1, __uint_as_float(x1[j]), __uint_as_float(x1[j + 1]));
+                        for (int j = 0; j < 32; j += 4) {
+                            t0 = max3(t0, __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
+                            t1 = max3(t1, __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]));
                         }
-                        t0 = fmaxf(t0, t1) * c;
-                        if (half == 0) top0 = t0;
-                        else top1 = t0;
+                        top = max3(top, t0, t1);
                     }
-                    const float new_max = max3(run_max, top0, top1), candidate = fmaxf(top0 + info.v_unit[0], top1 + info.v_unit[1]);
+                    tmem_st_wait();
+                    top *= c;
+                    *mine = __float_as_uint(top);
+                    meet();
+                    const float other = __uint_as_float(*theirs);
+                    const float new_max = max3(run_max, top, other), candidate = fmaxf(top + info.v_unit[part], other + info.v_unit[1 - part]);
                     // (a row that has seen no position yet keeps -inf, and all its weights are zero)
                     const bool move = candidate - ref > 8.f;
                     const float new_ref = move ? candidate : ref;
                     const float alpha = move ? fast_exp2(ref - new_ref) : 1.f;
                     const bool none = new_ref == -INFINITY;
-                    const float lift = none ? 0.f : (float)WIDE_UP - new_ref;
+                    const float shift = (none ? 0.f : (float)WIDE_UP - new_ref) + info.v_unit[part];
                     if (i > st && __any_sync(0xffffffffu, move)) {
 #pragma unroll 1
-                        for (int col = 0; col < HD; col += 16) {
+                        for (int col = 0; col < HD / 2; col += 16) {
                             uint32_t o[16];
                             tmem_ld16(o_addr + col, o);
 #pragma unroll
                             for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
                             tmem_st16(o_addr + col, o);
                         }
+                        tmem_st_wait();
                     }
-                    const uint64_t scale2 = pair_of(c, c);
-                    run_sum *= ratio(run_max, new_max);
+                    if (part) {                                // this half of O is ready for the first page's products
+                        tcgen05_fence_before();
+                        mbar_arrive(smem_u32(&p_full[2 * tile]));
+                    }
+                    const uint64_t scale2 = pair_of(c, c), shift2 = pair_of(shift, shift);
+                    uint64_t add = pair_of(0u, 0u);
+#pragma unroll 1
+                    for (int from = 0; from < LLMB_PAGE; from += 32) {
+                        uint32_t x[32], weights[16];
+                        tmem_ld32(page_addr + from, x);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float p0, p1;
+                            unpair(fma2(pair_of(x[j], x[j + 1]), scale2, shift2), p0, p1);
+                            p0 = fast_exp2(p0);
+                            p1 = fast_exp2(p1);
+                            add = add2(add, pair_of(p0, p1));
+                            weights[j >> 1] = pack_f16(p0, p1);
+                        }
+                        tmem_st16(page_addr + from / 2, weights);      // over this page's scores that have been read
+                    }
+                    tmem_st_wait();
+                    tcgen05_fence_before();
+                    mbar_arrive(smem_u32(&p_full[2 * tile + part]));
+                    float lo, hi;                              // what the page's weights are lifted by is taken off their sum
+                    unpair(add, lo, hi);
+                    run_sum = run_sum * ratio(run_max, new_max) + (none ? lo + hi : (lo + hi) * fast_exp2(-shift - new_max));
                     run_max = new_max;
                     ref = new_ref;
-#pragma unroll 1
-                    for (int half = 0; half < STEP_PAGES; ++half) {
-                        const float shift = lift + info.v_unit[half];
-                        const uint64_t shift2 = pair_of(shift, shift);
-                        uint64_t add = pair_of(0u, 0u);
-                        uint32_t x0[32], x1[32];
-                        tmem_ld32_start(s_addr + half * LLMB_PAGE, x0);
-                        tmem_ld32_start(s_addr + half * LLMB_PAGE + 32, x1);
-                        tmem_ld32_wait(x0);
-                        tmem_ld32_wait(x1);
-                        auto to_weights = [&](const uint32_t (&x)[32], int col) {
-                            uint32_t packed[16];
-#pragma unroll
-                            for (int j = 0; j < 32; j += 2) {
-                                float p0, p1;
-                                unpair(fma2(pair_of(x[j], x[j + 1]), scale2, shift2), p0, p1);
-                                p0 = fast_exp2(p0);
-                                p1 = fast_exp2(p1);
-                                add = add2(add, pair_of(p0, p1));
-                                packed[j >> 1] = pack_f16(p0, p1);
-                            }
-                            tmem_st16(s_addr + (col >> 1), packed);
-                        };
-                        to_weights(x0, half * LLMB_PAGE);
-                        to_weights(x1, half * LLMB_PAGE + 32);
-                        tmem_st_wait();
-                        tcgen05_fence_before();
-                        mbar_arrive(smem_u32(&p_full[2 * tile + half]));
-                        float lo, hi;                          // what the page's weights are lifted by is taken off their sum
-                        unpair(add, lo, hi);
-                        run_sum += none ? lo + hi : (lo + hi) * fast_exp2(-shift - new_max);
-                    }
                 }
                 // the result, or the block's part of it: by way of the queries' room, a warp's rows at a time, so that rows are written as a whole
                 ok = ok && mbar_wait_warp(smem_u32(&o_full[tile]), segments++ & 1, abort_flag, status, 40);
-                if (ok && !idle) {
+                if (!ok && !idle) {
+                    meet();
+                    meet();
+                } else if (!idle) {
                     tcgen05_fence_after();
+                    *mine = __float_as_uint(run_sum);
+                    meet();
+                    run_sum += __uint_as_float(*theirs);
+                    meet();                                    // (both have read)
                     const bool whole = segment.start >= r0 && segment.start + segment.steps <= r1;
                     float factor = run_sum != 0.f ? fast_exp2(ref - (float)(WIDE_UP + SCALE_UP) - run_max) : 0.f;
-                    const size_t part = ((size_t)blockIdx.x * 2 + (segment.start >= r0 ? 1 : 0)) * WIDE_ROWS + tile * TILE_ROWS + r;
-                    unsigned char* to = nullptr;               // the row's place in memory
+                    const size_t row = ((size_t)blockIdx.x * 2 + (segment.start >= r0 ? 1 : 0)) * WIDE_ROWS + tile * TILE_ROWS + r;
+                    unsigned char* to = nullptr;               // this half of the row in memory
                     if (whole) {
                         factor /= run_sum != 0.f ? run_sum : 1.f;
-                        if (valid) to = reinterpret_cast<unsigned char*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD);
+                        if (valid) to = reinterpret_cast<unsigned char*>(static_cast<__nv_bfloat16*>(a.out) + (size_t)token * a.out_stride + (size_t)head * HD + part * (HD / 2));
                     } else if (valid) {
-                        to = reinterpret_cast<unsigned char*>(a.wide_acc + part * HD);
-                        *reinterpret_cast<float2*>(a.wide_stats + part * 2) = make_float2(run_sum != 0.f ? run_max : -INFINITY, run_sum);
+                        to = reinterpret_cast<unsigned char*>(a.wide_acc + row * HD + part * (HD / 2));
+                        if (part == 0) *reinterpret_cast<float2*>(a.wide_stats + row * 2) = make_float2(run_sum != 0.f ? run_max : -INFINITY, run_sum);
                     }
-                    constexpr int ROOM = HD * 2;               // bytes of a row that go out at a time
-                    const int columns = whole ? HD : HD / 2;
+                    const int columns = whole ? HD / 2 : HD / 4;                 // that go out at a time: HD bytes
 #pragma unroll 1
-                    for (int from = 0; from < HD; from += columns) {
+                    for (int from = 0; from < HD / 2; from += columns) {
 #pragma unroll 1
                         for (int col = 0; col < columns; col += 16) {
                             uint32_t x[16];
                             tmem_ld16(o_addr + from + col, x);
 #pragma unroll
                             for (int d = 0; d < 16; ++d) x[d] = __float_as_uint(__uint_as_float(x[d]) * factor);
-                            const int chunk0 = whole ? col / 8 : col / 4;
-                            auto put = [&](int chunk, uint4 v) {
-                                *reinterpret_cast<uint4*>(my_row + (chunk >> 3) * TILE_PIECE + (((chunk & 7) ^ (r & 7)) << 4)) = v;
-                            };
                             if (whole) {
 #pragma unroll
                                 for (int d = 0; d < 16; d += 8)
-                                    put(chunk0 + d / 8, make_uint4(pack2(__uint_as_float(x[d]), __uint_as_float(x[d + 1])), pack2(__uint_as_float(x[d + 2]), __uint_as_float(x[d + 3])),
-                                                                   pack2(__uint_as_float(x[d + 4]), __uint_as_float(x[d + 5])), pack2(__uint_as_float(x[d + 6]), __uint_as_float(x[d + 7]))));
+                                    *place(r, (col + d) / 8) =
+                                        make_uint4(pack2(__uint_as_float(x[d]), __uint_as_float(x[d + 1])), pack2(__uint_as_float(x[d + 2]), __uint_as_float(x[d + 3])),
+                                                   pack2(__uint_as_float(x[d + 4]), __uint_as_float(x[d + 5])), pack2(__uint_as_float(x[d + 6]), __uint_as_float(x[d + 7])));
                             } else {
 #pragma unroll
-                                for (int d = 0; d < 16; d += 4) put(chunk0 + d / 4, make_uint4(x[d], x[d + 1], x[d + 2], x[d + 3]));
+                                for (int d = 0; d < 16; d += 4) *place(r, (col + d) / 4) = make_uint4(x[d], x[d + 1], x[d + 2], x[d + 3]);
                             }
                         }
                         __syncwarp();
-                        constexpr int CHUNKS = ROOM / 16, ROWS = 32 / CHUNKS;    // ROWS rows to an instruction
-                        const int chunk = lane % CHUNKS;
-#pragma unroll 4
+                        constexpr int ROWS = 32 / PART_CHUNKS;
+                        const int chunk = lane % PART_CHUNKS;
+#pragma unroll 2
                         for (int i = 0; i < 32; i += ROWS) {
-                            const int row = i + lane / CHUNKS, in_tile = quarter * 32 + row;
-                            unsigned char* there = reinterpret_cast<unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), row));
-                            if (there)
-                                *reinterpret_cast<uint4*>(there + from * 4 + chunk * 16) = *reinterpret_cast<const uint4*>(
-                                    q_tile + tile * Q_BYTES + (chunk >> 3) * TILE_PIECE + in_tile * 128 + (((chunk & 7) ^ (in_tile & 7)) << 4));
+                            const int from_row = i + lane / PART_CHUNKS;
+                            unsigned char* there = reinterpret_cast<unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), from_row));
+                            if (there) *reinterpret_cast<uint4*>(there + from * 4 + chunk * 16) = *place(quarter * 32 + from_row, chunk);
                         }
                         __syncwarp();
                     }
@@ -1948,7 +1955,7 @@ int launch_few(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
 template <int HD>
 int launch_wide(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
     // (more than half of an SM's shared memory for the smaller head size too: tensor memory has room for one block)
-    constexpr size_t need = (HD / 64) * (2 * TILE_PIECE + 4 * STEP_PIECE) + 2 * STEP * HD + INFOS * sizeof(StepInfo) + 23 * 8, bytes = need < 120 * 1024 ? 120 * 1024 : need;
+    constexpr size_t need = (HD / 64) * (2 * TILE_PIECE + 4 * STEP_PIECE) + 2 * STEP * HD + INFOS * sizeof(StepInfo) + 4 * STEP + 16 * TILE_ROWS + 23 * 8, bytes = need < 120 * 1024 ? 120 * 1024 : need;
     static_assert(bytes <= 227 * 1024, "one block an SM");
     static bool done[MAX_DEVICES] = {};
     static bool checked = false;
