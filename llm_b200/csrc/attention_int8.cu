@@ -396,8 +396,14 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
 }
 constexpr uint32_t BYTES_TO_F16 = 0x64806480u, MINUS_1152 = 0xe480e480u;
 // bytes 0 and 2 (1 and 3) of x as two fp16 numbers, times s (with off = -1152 s)
-__device__ __forceinline__ uint32_t even_bytes(uint32_t x, uint32_t s, uint32_t off) { return hfma2((x & 0x00ff00ffu) ^ BYTES_TO_F16, s, off); }
-__device__ __forceinline__ uint32_t odd_bytes(uint32_t x, uint32_t s, uint32_t off) { return hfma2(((x >> 8) & 0x00ff00ffu) ^ BYTES_TO_F16, s, off); }
+// (one operation of three operands; written as (x & a) ^ b it was two)
+__device__ __forceinline__ uint32_t biased(uint32_t x) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(d) : "r"(x), "r"(0x00ff00ffu), "r"(BYTES_TO_F16));
+    return d;
+}
+__device__ __forceinline__ uint32_t even_bytes(uint32_t x, uint32_t s, uint32_t off) { return hfma2(biased(x), s, off); }
+__device__ __forceinline__ uint32_t odd_bytes(uint32_t x, uint32_t s, uint32_t off) { return hfma2(biased(x >> 8), s, off); }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     uint32_t d;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
@@ -1415,38 +1421,41 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
         }
     } else if (warp >= 20) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_WIDEN));
-        constexpr int LANES = HD / 16, RPP = 128 / LANES, PASSES = STEP / RPP;        // lanes of a row, rows of a pass
-        const int t = threadIdx.x & 127, c = t % LANES, row_in = t / LANES;
-        const int chunk = 2 * (c & 3), flip = c >> 2;          // (lanes of the second piece write their halves the other way round: other banks)
+        // A pass is 16 bytes a thread. Of eight lanes four have half a row and four half of the next one: in the same columns where a row is 64 bytes,
+        // the other half where it is 128, so that both what they read and the two chunks that each writes lie in different banks.
+        constexpr int PASSES = HD / 16;
+        const int t = threadIdx.x & 127, quad = t & 3, other = (t >> 2) & 1;
         bool ok = true;
         for (int i = 0; i < 2 * total && ok; ++i) {            // keys and values in turn
             const int st = i >> 1, which = i & 1, b = st & 1;
             uint64_t* full = bars + 2 + 4 * which + b;         // (k_full, v_full and their like)
             uint64_t* empty = bars + 4 + 4 * which + b;
             const unsigned short* scale = step_scales + which * STEP;
-            const unsigned char* raw = (which ? raw_v : raw_k) + c * 16;
-            unsigned char* to = (which ? v_tile : k_tile) + b * STEP_BYTES + (c >> 2) * STEP_PIECE;
+            const unsigned char* raw = which ? raw_v : raw_k;
+            unsigned char* to = (which ? v_tile : k_tile) + b * STEP_BYTES;
             ok = mbar_wait_warp(smem_u32(&raw_full[which]), st & 1, abort_flag, status, 41) &&
                  (st < 2 || mbar_wait_warp(smem_u32(empty), ((st >> 1) - 1) & 1, abort_flag, status, 31));
             if (!ok) break;
             // rows to the operands' place, times their scales
 #pragma unroll 1
             for (int i0 = 0; i0 < PASSES; i0 += 4) {
-                uint2 x[4][2];                                 // this lane's first half and the other one
+                uint4 x[4];
                 uint32_t s[4];
+                auto row_of_pass = [&](int j) { return HD == 128 ? (i0 + j) / 2 * 32 + t / 4 : (i0 + j) * 32 + t / 4; };
+                auto piece_of_pass = [&](int j) { return HD == 128 ? (j & 1) ^ other : 0; };
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int row = (i0 + j) * RPP + row_in;
-                    x[j][0] = *reinterpret_cast<const uint2*>(raw + row * HD + flip * 8);
-                    x[j][1] = *reinterpret_cast<const uint2*>(raw + row * HD + (1 - flip) * 8);
+                    const int row = row_of_pass(j);
+                    x[j] = *reinterpret_cast<const uint4*>(raw + row * HD + piece_of_pass(j) * 64 + quad * 16);
                     s[j] = scale[row] * 0x10001u;
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int row = (i0 + j) * RPP + row_in;
+                    const int row = row_of_pass(j);
                     const uint32_t off = hmul2(s[j], MINUS_1152);
-                    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk + flip) ^ (row & 7)) << 4)) = widen8(x[j][0], s[j], off);
-                    *reinterpret_cast<uint4*>(to + row * 128 + (((chunk + 1 - flip) ^ (row & 7)) << 4)) = widen8(x[j][1], s[j], off);
+                    unsigned char* at = to + piece_of_pass(j) * STEP_PIECE + row * 128;
+                    *reinterpret_cast<uint4*>(at + (((2 * quad) ^ (row & 7)) << 4)) = widen8(make_uint2(x[j].x, x[j].y), s[j], off);
+                    *reinterpret_cast<uint4*>(at + (((2 * quad + 1) ^ (row & 7)) << 4)) = widen8(make_uint2(x[j].z, x[j].w), s[j], off);
                 }
             }
             mbar_arrive(smem_u32(&raw_empty[which]));          // the bytes' room is free
