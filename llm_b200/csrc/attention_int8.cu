@@ -337,6 +337,230 @@ __global__ void __launch_bounds__(SIMT_THREADS) attention_int8_simt_kernel(const
     }
 }
 
+// ------------------------------------------------------------------------------------------------ any type, any head size, up to 8 rows
+//
+// The same arithmetic for what a decode step brings: with 32 rows a block one warp of eight would have all the work. Here each warp walks pages of its
+// own. A lane forms the scores of all rows with keys `lane` and `lane + 32`, whose bytes it reads itself and widens to 32 bits in registers; the
+// weights, times the values' scales, go through shared memory; then a lane adds the weighted values of its columns. The eight warps' sums meet at
+// the end. Eight sequences of 4,096 positions (32 heads over 8 of 64, 32-bit) take 30 us, with 32 rows a block 73. What bounds it is a page's chain: with the
+// keys' and values' loads where they are used it was 77; with one block of eight warps an SM and 165 registers a thread 44, with two and 16 values at a
+// time 34, four blocks of four warps 31.
+
+constexpr int ROWS_THREADS = 256, ROWS_WARPS = ROWS_THREADS / 32;
+
+// Four bytes as 32-bit values: 0x4b000000 | (b ^ 0x80) is 8388608 + 128 + b.
+__device__ __forceinline__ void widen4(uint32_t x, float (&v)[4]) {
+    x ^= 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7650 + i)) - 8388736.f;
+}
+template <int DMAX, int R> constexpr int rows_floats() { return R * DMAX + ROWS_WARPS * (R * DMAX > LLMB_PAGE * R ? R * DMAX : LLMB_PAGE * R) + ROWS_WARPS * R * 2; }
+
+template <typename T, int DMAX, int R>
+__global__ void __launch_bounds__(ROWS_THREADS, DMAX == 64 ? 2 : 1) attention_int8_rows_kernel(const __grid_constant__ Args a, int* status) {
+    constexpr int W = DMAX / 32;                   // a lane's columns, which adjoin
+    extern __shared__ __align__(16) float smem[];
+    float* qs = smem;                              // [R][DMAX], scaled; zeros behind the head's last column
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int ROOM = R * DMAX > LLMB_PAGE * R ? R * DMAX : LLMB_PAGE * R;
+    float* room = smem + R * DMAX;                 // of each warp: its weights [64][R], at the end its sums [R][DMAX]
+    float* weights = room + warp * ROOM;
+    float2* stats = reinterpret_cast<float2*>(room + ROWS_WARPS * ROOM);         // [warp][R]
+    griddep_launch();
+    Item w;
+    const bool work = item_of(a, blockIdx.x, blockIdx.y, R, w, status);
+    griddep_wait();
+    if (!work) return;
+    const int D = a.head_dim, share = a.n_heads / a.n_kv_heads;
+    const T* q = behind_wait(static_cast<const T*>(a.q));
+    const int* pages = a.block_table + (size_t)w.seq * a.table_stride;
+    const int scales_per_page = LLMB_PAGE >> a.block_shift;
+    for (int i = threadIdx.x; i < R * DMAX; i += ROWS_THREADS) {
+        const int r = i / DMAX, d = i - r * DMAX;
+        qs[i] = r < w.n_rows && d < D ? to_float(q[(size_t)token_of(w, r, share) * a.q_stride + (size_t)head_of(w, r, share) * D + d]) * a.scale_log2 : 0.f;
+    }
+    __syncthreads();
+    float m[R], l[R], o[R][W];
+    int pos[R], seen[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        pos[r] = r < w.n_rows ? position_of(w, r, share) : -1;
+        seen[r] = first_seen(a, pos[r]);
+#pragma unroll
+        for (int c = 0; c < W; ++c) o[r][c] = 0.f;
+    }
+    const int last = position_of(w, w.n_rows - 1, share), low = first_seen(a, position_of(w, 0, share));      // what a row sees at all
+    // A page's loads are under way before anything is worked out: the keys' bytes of this lane's two (where the head is not too large for the
+    // registers), the scales, the first values; then each group of values under the products with the one before.
+    constexpr int HALVES = DMAX <= 128 ? 2 : 1, GROUP = 8, WORDS = (W + 3) / 4;
+    const bool vectors = D % 16 == 0, all = lane * W + W <= D && D % W == 0;     // a key's bytes can be read 16 at a time, this lane's columns at once
+    int next = w.page_begin + warp < w.page_end ? page_at(a, pages, w.page_begin + warp, status) : 0;
+    for (int logical = w.page_begin + warp; logical < w.page_end; logical += ROWS_WARPS) {
+        const int key0 = logical * LLMB_PAGE, from = max(low - key0, 0), to = min(last + 1 - key0, LLMB_PAGE);      // what of the page a row sees at all
+        const size_t at = (size_t)next * a.n_kv_heads + w.kv_head;
+        const signed char* keys = a.keys + at * LLMB_PAGE * D;
+        const signed char* values = a.values + at * LLMB_PAGE * D + lane * W;
+        if (logical + ROWS_WARPS < w.page_end) next = page_at(a, pages, logical + ROWS_WARPS, status);
+        uint4 raw[HALVES][DMAX / 16];
+        auto fetch_keys = [&](int half, uint4 (&x)[DMAX / 16]) {
+            const int k = lane + 32 * half;
+            const uint4* row = reinterpret_cast<const uint4*>(keys + (size_t)k * D);
+#pragma unroll
+            for (int i = 0; i < DMAX / 16; ++i)
+                if (vectors && i * 16 < D && k >= from && k < to) x[i] = row[i];
+        };
+        uint32_t held[2][GROUP][WORDS];
+        auto fetch_values = [&](int k0, uint32_t (&x)[GROUP][WORDS]) {
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j) {
+                const int k = k0 + j;
+                const signed char* row = values + (size_t)k * D;
+                if (k >= to || lane * W >= D) continue;
+                if (!all) {
+#pragma unroll
+                    for (int c = 0; c < W; ++c) {
+                        if (c % 4 == 0) x[j][c / 4] = 0;
+                        if (lane * W + c < D) x[j][c / 4] |= (uint32_t)(unsigned char)row[c] << (8 * (c % 4));
+                    }
+                } else if constexpr (W == 2) {
+                    x[j][0] = *reinterpret_cast<const unsigned short*>(row);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < WORDS; ++c) x[j][c] = reinterpret_cast<const uint32_t*>(row)[c];
+                }
+            }
+        };
+        float s[2][R], ks[2], vs[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int k = lane + 32 * half;
+            const bool there = k >= from && k < to;
+            ks[half] = there ? a.key_scales[at * scales_per_page + (k >> a.block_shift)] : 0.f;
+            vs[half] = there ? a.value_scales[at * scales_per_page + (k >> a.block_shift)] : 0.f;
+            if (half < HALVES) fetch_keys(half, raw[half]);
+        }
+        fetch_values(from, held[0]);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int k = lane + 32 * half, key = key0 + k;
+            if (half >= HALVES) fetch_keys(half, raw[0]);
+            const uint4 (&x)[DMAX / 16] = raw[half < HALVES ? half : 0];
+            const bool bad = !is_number(ks[half]) || !is_number(vs[half]);
+            if (!bad && ((__float_as_uint(ks[half]) | __float_as_uint(vs[half])) & 0x807fffffu)) report(status, NOT_A_POWER);
+            uint64_t dot[R];                       // even and odd columns apart
+#pragma unroll
+            for (int r = 0; r < R; ++r) dot[r] = 0;
+            auto add = [&](uint32_t bytes, int d) {
+                float v[4];
+                widen4(bytes, v);
+                const uint64_t v01 = pair_of(v[0], v[1]), v23 = pair_of(v[2], v[3]);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const ulonglong2 qv = *reinterpret_cast<const ulonglong2*>(qs + r * DMAX + d);
+                    dot[r] = fma2(qv.x, v01, fma2(qv.y, v23, dot[r]));
+                }
+            };
+            if (k >= from && k < to) {
+                if (vectors) {
+#pragma unroll
+                    for (int i = 0; i < DMAX / 16; ++i) {
+                        if (i * 16 >= D) break;
+                        add(x[i].x, i * 16);
+                        add(x[i].y, i * 16 + 4);
+                        add(x[i].z, i * 16 + 8);
+                        add(x[i].w, i * 16 + 12);
+                    }
+                } else {
+                    const signed char* row = keys + (size_t)k * D;
+                    for (int d = 0; d < D; d += 4) {             // (heads are even; the last two columns may be none)
+                        uint32_t y = *reinterpret_cast<const unsigned short*>(row + d);
+                        if (d + 2 < D) y |= (uint32_t)*reinterpret_cast<const unsigned short*>(row + d + 2) << 16;
+                        add(y, d);
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                s[half][r] = bad ? __uint_as_float(0x7fffffffu) : (half_of(dot[r], 0) + half_of(dot[r], 1)) * ks[half];
+                if (key > pos[r] || key < seen[r]) s[half][r] = -INFINITY;
+            }
+            if (bad) vs[half] = 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float top = warp_max(fmaxf(s[0][r], s[1][r]));
+            const float new_m = fmaxf(m[r], top), against = new_m == -INFINITY ? 0.f : new_m, alpha = exp2f(m[r] - against);
+            m[r] = new_m;
+            float add = 0.f;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float p = exp2f(s[half][r] - against);
+                add += p;
+                weights[(lane + 32 * half) * R + r] = p * vs[half];
+            }
+            l[r] = l[r] * alpha + add;             // of this lane's keys
+#pragma unroll
+            for (int c = 0; c < W; ++c) o[r][c] *= alpha;
+        }
+        __syncwarp();
+        auto multiply = [&](int k0, const uint32_t (&x)[GROUP][WORDS]) {
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j) {
+                if (k0 + j >= to) break;
+                float v[WORDS * 4];
+#pragma unroll
+                for (int c = 0; c < WORDS; ++c) widen4(x[j][c], *reinterpret_cast<float (*)[4]>(v + 4 * c));
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float p = weights[(k0 + j) * R + r];
+#pragma unroll
+                    for (int c = 0; c < W; ++c) o[r][c] = fmaf(p, v[c], o[r][c]);
+                }
+            }
+        };
+        for (int k = from; k < to; k += 2 * GROUP) {
+            fetch_values(k + GROUP, held[1]);
+            multiply(k, held[0]);
+            fetch_values(k + 2 * GROUP, held[0]);
+            multiply(k + GROUP, held[1]);
+        }
+        __syncwarp();                              // the weights are read before the next page's are written
+    }
+    // the warps' sums in order
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        l[r] = warp_sum(l[r]);
+        if (lane == 0) stats[warp * R + r] = make_float2(m[r], l[r]);
+#pragma unroll
+        for (int c = 0; c < W; ++c) room[warp * ROOM + r * DMAX + lane * W + c] = o[r][c];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < w.n_rows * D; i += ROWS_THREADS) {
+        const int r = i / D, d = i - r * D;
+        float top = -INFINITY, value = 0.f, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < ROWS_WARPS; ++k) top = fmaxf(top, stats[k * R + r].x);
+        const float against = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int k = 0; k < ROWS_WARPS; ++k) {
+            const float2 of = stats[k * R + r];
+            const float weight = of.y != 0.f ? exp2f(of.x - against) : 0.f;
+            sum += of.y * weight;
+            value = fmaf(room[k * ROOM + r * DMAX + d], weight, value);
+        }
+        const int token = token_of(w, r, share), head = head_of(w, r, share);
+        if (a.slots == 1) {
+            static_cast<T*>(a.out)[(size_t)token * a.out_stride + (size_t)head * D + d] = from_float<T>(sum != 0.f ? value / sum : 0.f);
+        } else {
+            const size_t slot = ((size_t)token * a.n_heads + head) * a.slots + w.slot;
+            a.acc[slot * D + d] = value;
+            if (d == 0) *reinterpret_cast<float2*>(a.stats + slot * 2) = make_float2(sum != 0.f ? top : -INFINITY, sum);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ bfloat16, up to 16 rows
 //
 // What a decode step brings. Reading the cache is the work, and widening it: 16 bits would be twice the bytes, so the whole numbers stay what they are
@@ -547,11 +771,9 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         r1 = min(r0 + per, all);
         if (r0 < r1) pair = pair_at(a, r0, most_tokens, lane);
     }
-    griddep_wait();
-    if (r0 >= r1) return;
+    if (r0 >= r1) return griddep_wait();
     constexpr int PER_PAGE = LLMB_PAGE / U, TILES = U / 16;
     const int units = (r1 - r0) * PER_PAGE;
-    const __nv_bfloat16* q_all = behind_wait(static_cast<const __nv_bfloat16*>(a.q));
     const int scales_per_page = LLMB_PAGE >> a.block_shift;
 
     // What is asked for: unit `asked` of the range, of pair `ahead` (up to page `ahead_end` of the range); its page's number is on its way.
@@ -589,9 +811,11 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         cp_async_commit();
     };
     look_up();
+    griddep_wait();
 #pragma unroll
     for (int i = 0; i < STAGES; ++i) ask(i);
 
+    const __nv_bfloat16* q_all = behind_wait(static_cast<const __nv_bfloat16*>(a.q));
     int done = warp, stage = 0;                                // the next unit, and where it arrives
     uint32_t phase = 0;
     bool ok = true;
@@ -1826,13 +2050,14 @@ struct Plan {
     int few_tokens;                  // sequences that bring at most so many tokens are the first one's
     long long few_blocks, wide_grid, blocks;
     int deal_blocks, deal_least, wide_blocks, wide_least;
+    int rows;                        // of a block on the CUDA cores: 4 or 8 where a step has no more, 0: 32
     int tiles, slots;
     long long part_rows, wide_rows;  // rows that are joined from parts
     int launches;
 };
 
 // The kernel for few rows deals pages out where a sequence may have more than WHOLE_PAGES, LEAST_PAGES a block at least.
-constexpr int WHOLE_PAGES = 4, LEAST_PAGES = 2;
+constexpr int WHOLE_PAGES = 4, LEAST_PAGES = 4;
 // The kernel for many rows deals steps out, LEAST_STEPS a block at least, unless no tile has more than WHOLE_STEPS.
 constexpr int WHOLE_STEPS = 16, LEAST_STEPS = 4;
 
@@ -1877,6 +2102,18 @@ Plan plan_for(const Sizes& z) {
         }
         return p;
     }
+    p.rows = (long long)z.max_new * share <= 4 ? 4 : (long long)z.max_new * share <= 8 ? 8 : 0;
+    if (p.rows) {
+        // a page for each of a block's warps at least, as many slices as make two blocks an SM
+        p.tiles = 1;
+        p.blocks = pairs;
+        const long long slots = 2ll * SMS / pairs, most = ceil_div(pages, ROWS_WARPS);
+        p.slots = (int)(slots < 1 ? 1 : slots > most ? most : slots);
+        if (p.slots > MAX_SPLITS) p.slots = MAX_SPLITS;
+        p.part_rows = p.slots == 1 ? 0 : (long long)z.n_tokens * z.n_heads;
+        if (p.slots > 1) ++p.launches;
+        return p;
+    }
     // Into how many slices the pages are cut: as many as make all blocks come to about the blocks that the SMs hold at once, two pages each at least; up
     // to WHOLE_PAGES are one block's, since joining takes a launch.
     p.tiles = ceil_div((long long)z.max_new * share, SIMT_ROWS);
@@ -1918,6 +2155,20 @@ int launch_simt(const Args& a, const Plan& p, int* status, cudaStream_t stream) 
     if (int code = allow_shared((const void*)attention_int8_simt_kernel<T, DMAX>, smem, done)) return code;
     llmb::launch(attention_int8_simt_kernel<T, DMAX>, dim3((unsigned)p.blocks, p.slots), SIMT_THREADS, smem, stream, true, a, status);
     return check_launch("attention_int8_simt");
+}
+
+template <typename T, int DMAX, int R>
+int launch_rows(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
+    constexpr size_t smem = rows_floats<DMAX, R>() * sizeof(float);
+    static bool done[MAX_DEVICES] = {};
+    if (int code = allow_shared((const void*)attention_int8_rows_kernel<T, DMAX, R>, smem, done)) return code;
+    llmb::launch(attention_int8_rows_kernel<T, DMAX, R>, dim3((unsigned)p.blocks, p.slots), ROWS_THREADS, smem, stream, true, a, status);
+    return check_launch("attention_int8_rows");
+}
+template <typename T, int DMAX>
+int launch_cores(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
+    return p.rows == 4 ? launch_rows<T, DMAX, 4>(a, p, status, stream) : p.rows == 8 ? launch_rows<T, DMAX, 8>(a, p, status, stream)
+                                                                                    : launch_simt<T, DMAX>(a, p, status, stream);
 }
 
 // a warp for four parts, as many as fit
@@ -1994,8 +2245,8 @@ int launch_tc(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
 template <typename T>
 int run(const Args& a, const Plan& p, const Sizes& z, int* status, cudaStream_t stream) {
     if (p.few || p.wide) return a.head_dim == 64 ? launch_tc<64>(a, p, status, stream) : launch_tc<128>(a, p, status, stream);
-    int code = a.head_dim <= 64 ? launch_simt<T, 64>(a, p, status, stream) : a.head_dim <= 128 ? launch_simt<T, 128>(a, p, status, stream)
-                                                                                               : launch_simt<T, 256>(a, p, status, stream);
+    int code = a.head_dim <= 64 ? launch_cores<T, 64>(a, p, status, stream) : a.head_dim <= 128 ? launch_cores<T, 128>(a, p, status, stream)
+                                                                                                : launch_cores<T, 256>(a, p, status, stream);
     if (code || a.slots == 1) return code;
     if (a.head_dim <= 128) launch_join<T, 1>(a, (int)p.part_rows, stream);
     else launch_join<T, 2>(a, (int)p.part_rows, stream);
