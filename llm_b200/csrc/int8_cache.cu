@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(THREADS) int8_append_kernel(const __grid_const
     if (unit >= units) return;
     const T* qkv = behind_wait(static_cast<const T*>(a.qkv));
     const size_t row_stride = (size_t)units * D;
+    if (token >= a.cu_seqlens[a.n_seqs]) return;              // a row behind the last sequence's
     const int position = a.tok_pos[token];
     const bool turned = unit < a.n_heads + a.n_kv_heads;      // queries and keys
     auto angles_of = [&](int pos) { return a.angles + (size_t)pos * a.n_rot; };
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(THREADS) int8_append_kernel(const __grid_const
         n_rows = min(a.block - first, a.cu_seqlens[seq + 1] - token);
         page = a.block_table[(size_t)seq * a.table_stride + (position / LLMB_PAGE) % a.ring_pages];
     }
-    if ((unsigned)page >= (unsigned)a.n_pages || token + n_rows > a.n_tokens || (a.angles && position + n_rows > a.n_positions)) {
+    if ((unsigned)page >= (unsigned)a.n_pages || n_rows <= 0 || token < a.cu_seqlens[seq] || token + n_rows > a.n_tokens || (a.angles && position + n_rows > a.n_positions)) {
         if (lane == 0 && status) atomicCAS(status, 0, OUT_OF_RANGE);
         return;
     }
@@ -157,8 +158,10 @@ __global__ void __launch_bounds__(THREADS) int8_append_kernel(const __grid_const
 // 16 new rows of it in registers between the largest magnitude and the whole numbers (more are read twice).
 //
 // A block of threads does `run` neighbouring tokens: their first rows in blocks of the cache are looked up by one warp, then the eight warps take
-// blocks and queries in turn. Memory bounds long steps: 16,889 tokens of 32 heads over 8 of 128 in FIXME; what a step of
-// 64 tokens takes is a launch and three dependent reads.
+// blocks and queries in turn. Rows are
+// held as they came and rotated again for the whole numbers: with the rotated values in registers there was room for half as many warps (16,889 tokens 95 us
+// for 80). Those tokens (32 heads over 8 of 128) move 389 MB, at 4.9 TB/s: a warp's loads are 4 KB, with 16 to 24 warps on an SM. Three and four blocks of
+// 80 and 64 registers spilled (78 and 104 us; 64 tokens 3.9 and 4.9). What a step of 64 tokens takes (3.1 us) is a launch and three dependent reads.
 
 constexpr int MAX_RUN = 16, HELD = 16, QUERIES = 4;            // tokens of a block of threads; rows that a warp holds; rows of queries, in instructions
 
@@ -243,14 +246,15 @@ __global__ void __launch_bounds__(THREADS) int8_append_vec_kernel(const __grid_c
     if (warp == 0) {
         Begun b{};
         bool mine = false;
-        if (lane < n_here) {
+        if (lane < n_here) positions[lane] = -1;
+        if (lane < n_here && token0 + lane < a.cu_seqlens[a.n_seqs]) {           // (rows behind the last sequence's are left as they are)
             b.token = token0 + lane;
             b.position = a.tok_pos[b.token];
             const int seq = a.tok_seq[b.token];
             bool there = b.position >= 0 && !(a.angles && b.position >= a.n_positions);
-            positions[lane] = there ? b.position : -1;
+            if (there) positions[lane] = b.position;
             if (there && a.write_cache) {
-                there = (unsigned)seq < (unsigned)a.n_seqs;
+                there = (unsigned)seq < (unsigned)a.n_seqs && b.token >= a.cu_seqlens[seq] && b.token < a.cu_seqlens[seq + 1];
                 if (there && (b.position % a.block == 0 || b.token == a.cu_seqlens[seq])) {
                     int place = b.position / LLMB_PAGE;
                     if (place >= a.ring_pages) place %= a.ring_pages;

@@ -1747,8 +1747,8 @@ def rope_cache_write_int8(qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_t
                           interleaved=False, write_cache=True, out=None):
     """`rope_cache_write` for a cache held in 8 bits (`keys` and `values`: Int8Pages): the rotated queries of the fused
     [T, (Hq + 2 Hkv) D] projection are the result ([T, Hq * D], qkv itself is left as it is), its keys, rotated, and its values are appended
-    to their sequences' pages. The tokens of sequence i are rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1, at consecutive
-    positions tok_pos; `block_table` [B, pages].
+    to their sequences' pages. The tokens of sequence i are rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (none overlap; rows behind the last one's
+    are left as they are), at consecutive positions tok_pos; `block_table` [B, pages].
 
     A block of positions has the smallest power of two for a scale with which its largest value is at most 127 steps. One that the
     step continues keeps its scale where that is enough; where it grows, what the block holds is divided by the growth and rounded again. What

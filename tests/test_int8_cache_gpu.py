@@ -462,6 +462,81 @@ def test_append_ring_and_reports():
             ops().check_device_status()
 
 
+@pytest.mark.parametrize("dtype, dim, n_rot", [(F32, 16, 16), (BF16, 128, 128), (BF16, 128, 64)])
+def test_append_rows_behind_the_last_sequence(dtype, dim, n_rot):
+    """A padded batch: the padding's queries and pages are left as they are, whatever its positions and sequences say."""
+    b = make([5, 40], [3, 30], 4, 2, dim, dtype, seed=43)
+    x, angles = projection(b, n_rot, False, 13)
+    padded = torch.cat([x, torch.full((9, *x.shape[1:]), math.nan, dtype=dtype, device=DEV)])
+    pos, seq = places(b)
+    pos, seq = torch.cat([pos, ints([0, 16, 64, 3, -7, 1 << 30, 0, 1, 2])]), torch.cat([seq, ints([0, 1, 1, 0, 0, 1, 99, -1, 0])])
+    out = torch.full((42, 4 * dim), 7.0, dtype=dtype, device=DEV)
+    before = copies(b)
+    ops().rope_cache_write_int8(padded.flatten(1), angles, pos, seq, b["arrays"][1], b["table"], b["ring"], b["keys"], b["values"], 4, 2, dim, out=out)
+    check_append(b, x, angles, False, before, out[:33])
+    assert bool((out[33:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype, dim", [(F32, 16), (BF16, 128), (BF16, 80)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [20, 1, 90]])
+def test_attention_rows_behind_the_last_sequence_and_wide_tables(dtype, dim, new):
+    """A padded batch, and a table inside a wider one."""
+    b = make([200, 3, 70], new, 4, 2, dim, dtype, seed=47)
+    n = b["cu"][-1]
+    wide = torch.full((3, b["ring"] + 5), 1 << 20, dtype=torch.int32, device=DEV)
+    wide[:, :b["ring"]] = b["table"]
+    padded = torch.cat([b["q"], torch.full((6, 4 * dim), math.nan, dtype=dtype, device=DEV)])
+    out = torch.full((n + 6, 4 * dim), 7.0, dtype=dtype, device=DEV)
+    call({**b, "q": padded, "table": wide[:, :b["ring"]]}, out=out)
+    check(b, out[:n].contiguous())
+    assert bool((out[n:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_attention_scales_of_the_scores(dtype, scale):
+    for new in ([1, 2], [60, 1]):
+        b = make([100, 30], new, 4, 2, 64, dtype, seed=53)
+        b["scale"] = scale
+        got = call(b)
+        torch.cuda.synchronize()
+        for s, length in enumerate(b["lengths"]):
+            t = b["cu"][s]
+            page = b["table"][s].long()[torch.arange(length, device=DEV) // PAGE]
+            row = torch.arange(length, device=DEV) % PAGE
+            seen = length - new[s] + 1                         # of the sequence's first new token
+            k, v = (c.held(torch.float64)[page, 0, row][:seen] for c in (b["keys"], b["values"]))
+            weights = torch.softmax(b["q"][t, :64].double() @ k.T * scale, -1)
+            assert bool(((got[t, :64].double() - weights @ v).abs() <= 2.0 ** -7 * (weights @ v.abs())).all())
+
+
+def test_pages_behind_two_to_the_31_bytes():
+    """Pools of more than 2^31 whole numbers, whose last pages are in use."""
+    n_pages, kv, dim = 34000, 8, 128                           # 2.2 * 10^9 whole numbers each of keys and values
+    small = make([300, 90], [1, 1], 32, kv, dim, BF16, seed=59)
+    big = []
+    for cache in (small["keys"], small["values"]):
+        n = cache.values.shape[0]
+        whole = torch.zeros((n_pages, kv, PAGE, dim), dtype=torch.int8, device=DEV)
+        scales = torch.full((n_pages, kv, cache.scales.shape[2]), math.nan, device=DEV)
+        whole[-n:], scales[-n:] = cache.values, cache.scales
+        big.append(ops().Int8Pages(whole, scales))
+    shift = n_pages - small["keys"].values.shape[0]
+    table = small["table"] + shift
+    for new in (1, 20):
+        b = make([301 - new, 91 - new], [new, new], 32, kv, dim, BF16, seed=61)
+        b.update(keys=small["keys"], values=small["values"], table=small["table"], ring=small["ring"])
+        want = call(b)
+        check(b, want)
+        assert torch.equal(call({**b, "keys": big[0], "values": big[1], "table": table}), want)
+    x, angles = projection(b, dim, False, 15)
+    append(b, x, angles)
+    append({**b, "keys": big[0], "values": big[1], "table": table}, x, angles)
+    for cache, whole in zip((b["keys"], b["values"]), big):
+        n = cache.values.shape[0]
+        assert torch.equal(whole.values[-n:], cache.values) and torch.equal(whole.scales[-n:].nan_to_num(7.0), cache.scales.nan_to_num(7.0))
+
+
 # ----------------------------------------------------------------------------- together
 
 @pytest.mark.parametrize("dtype, heads, kv_heads, dim", [(F32, 4, 2, 16), (BF16, 8, 2, 128), (BF16, 8, 8, 64), (BF16, 6, 2, 80)])
