@@ -581,6 +581,11 @@ __global__ void __launch_bounds__(ROWS_THREADS, DMAX == 64 ? 2 : 1) attention_in
 // finished there, of the others each block leaves a part. A block has four warps, each with a ring of units of its own, 32 positions or 64 (TMA, rows
 // swizzled so that both the reads of keys, four lanes a row, and those of values, eight columns a lane, touch all banks once), which runs on over the
 // ends of pairs; warps meet where a pair ends.
+//
+// 64 sequences of 8,192 positions (32 heads over 8 of 128, 1.08 GB) take 173 us in short bursts, 6.2 TB/s, and 204 in long loops at the power cap: reading
+// is the limit, and the energy of some 780 instructions for 8 KB. Eight take 37 us, one 11 on the device: 10 of them are a block's start (lengths, table,
+// first pages: dependent reads), its end and the join. Three blocks an SM of 165 registers; with maximum, reference and masks worked out anew for every unit,
+// and 32 positions for heads of 64 too, a unit took 1,130 instructions.
 
 constexpr int FEW_THREADS = 128, FEW_WARPS = 4;
 constexpr int FEW_ROWS = 16;
@@ -1238,8 +1243,11 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_few_join_kerne
 // another one issues. (Fetched through the widening warps' registers a step took 9,000 cycles: the fence between their stores and the products
 // waits for their loads too.) Per tile one buffer of
 // scores [128, 128] and O [128, D] fill tensor memory; the two tiles take turns: while the softmax of one works on its scores, the products of
-// the other run (P V of these positions, then Q K^T of the next). Widening is a fifth of the instructions that 256 rows of softmax take, and 256 rows
-// share it.
+// the other run (P V of these positions, then Q K^T of the next). Widening is a quarter of all instructions, and 256 rows share it.
+//
+// Four prompts of 120 to 510 tokens behind 16,384 positions take 380 us in short bursts (0.54 of the products' burst rate), 415 in long loops; a prompt of 2,048
+// tokens 55. A step takes some 4,300 cycles; its products alone are 2,048, its exponentials as many on their unit, its instructions 2,560 of a
+// scheduler's slots and its traffic through shared memory some 2,800.
 //
 // References as above, with two differences: keys' scales count from the largest of the 128 positions of a step, values' from the largest of each page (from
 // 2^-90 of the largest so far at least, which keeps the sums of the weights exact where a page's values are zeros), and R moves only when it is exceeded by 2^8.
@@ -2056,8 +2064,12 @@ struct Plan {
     int launches;
 };
 
-// The kernel for few rows deals pages out where a sequence may have more than WHOLE_PAGES, LEAST_PAGES a block at least.
-constexpr int WHOLE_PAGES = 4, LEAST_PAGES = 4;
+// The kernel for few rows deals pages out where a sequence may have more than WHOLE_PAGES, LEAST_PAGES a block at least. Below, a sequence and head are one
+// block's, which saves the launch that joins, 4 us of the host's time: with 500 positions one sequence takes 8.3 us on the device, dealt out 7.7, 64
+// take 20.1 and 20.8; with 1,000 positions one takes 13.5 and 8.0, 16 take 19.2 and 15.2.
+constexpr int WHOLE_PAGES = 8, LEAST_PAGES = 4;
+// The kernel for any shape cuts a sequence where it may have more pages than this.
+constexpr int SIMT_WHOLE_PAGES = 4;
 // The kernel for many rows deals steps out, LEAST_STEPS a block at least, unless no tile has more than WHOLE_STEPS.
 constexpr int WHOLE_STEPS = 16, LEAST_STEPS = 4;
 
@@ -2115,13 +2127,13 @@ Plan plan_for(const Sizes& z) {
         return p;
     }
     // Into how many slices the pages are cut: as many as make all blocks come to about the blocks that the SMs hold at once, two pages each at least; up
-    // to WHOLE_PAGES are one block's, since joining takes a launch.
+    // to SIMT_WHOLE_PAGES are one block's, since joining takes a launch.
     p.tiles = ceil_div((long long)z.max_new * share, SIMT_ROWS);
     p.blocks = pairs * p.tiles;
     const long long wave = (long long)SMS * (z.head_dim <= 128 ? 2 : 1);
     long long slots = wave / p.blocks;
     if (slots > pages / 2) slots = pages / 2;
-    if (pages <= WHOLE_PAGES) slots = 1;
+    if (pages <= SIMT_WHOLE_PAGES) slots = 1;
     p.slots = slots < 1 ? 1 : slots > MAX_SPLITS ? MAX_SPLITS : (int)slots;
     p.part_rows = p.slots == 1 ? 0 : (long long)z.n_tokens * z.n_heads;
     if (p.slots > 1) ++p.launches;

@@ -1761,7 +1761,12 @@ def rope_cache_write_int8(qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_t
     n, n_seqs, dtype = qkv.shape[0], cu_seqlens.numel() - 1, qkv.dtype
     code = _code(dtype)
     _check_int8(keys, values, n_kv_heads, head_dim, what)
-    _check_step(what, block_table, ring_pages, n_seqs, ((tok_pos, n, "tok_pos"), (tok_seq, n, "tok_seq"), (cu_seqlens, n_seqs + 1, "cu_seqlens")))
+    int32, table = torch.int32, block_table.shape
+    if not (tok_pos.dtype is int32 and tok_seq.dtype is int32 and cu_seqlens.dtype is int32 and block_table.dtype is int32 and len(table) == 2
+            and table[0] == n_seqs and 1 <= ring_pages <= table[1] and block_table.stride(1) == 1 and tok_pos.dim() == 1 and tok_seq.dim() == 1
+            and cu_seqlens.dim() == 1 and tok_pos.numel() == n and tok_seq.numel() == n and tok_pos.is_contiguous() and tok_seq.is_contiguous()
+            and cu_seqlens.is_contiguous()):
+        _check_step(what, block_table, ring_pages, n_seqs, ((tok_pos, n, "tok_pos"), (tok_seq, n, "tok_seq"), (cu_seqlens, n_seqs + 1, "cu_seqlens")))
     n_rot = n_positions = 0
     if rope_table is not None:
         if rope_table.dim() != 2 or rope_table.dtype is not torch.float32 or not rope_table.is_contiguous() or rope_table.shape[1] > head_dim \

@@ -21,6 +21,7 @@ _LEAST = {"products": (148 * 2 * 128 * 256, 1 << 14),     # what a product on pa
 generation = 0                            # grows with that of every scope and stream
 _line = threading.local()                 # .entered: the scopes that this thread is inside of
 _lock = threading.Lock()
+_recent = None                            # (stream, device, its StepScope): who asked last
 _of_stream: dict = {}                     # (device, stream) -> StepScope, the one that was asked last at the end
 
 
@@ -72,11 +73,17 @@ def inside() -> bool:
 
 def of_call(device, stream: int, capturing: bool, kind: str, floats: int, counters: int = 0) -> tuple:
     """(float32 [>= floats], int32 [>= counters], zero, or None) for a call that is launched on `stream`."""
+    global _recent
     entered = getattr(_line, "entered", None)
     if entered:
         return entered[-1].room(device, kind, floats, counters, capturing)
     if capturing:
         return _new(device, floats, counters)
+    recent = _recent                      # the stream that asked last asks again, as a rule: its scope is not looked for
+    if recent is not None and recent[0] == stream and recent[1] == device:
+        held = recent[2]._held.get((device, kind))
+        if held is not None and held[0].numel() >= floats and (held[1].numel() if held[1] is not None else 0) >= counters:
+            return held
     with _lock:
         scope = _of_stream.pop((device, stream), None)
         if scope is None:
@@ -86,4 +93,5 @@ def of_call(device, stream: int, capturing: bool, kind: str, floats: int, counte
         _of_stream[(device, stream)] = scope
         found = scope.room(device, kind, floats, counters, False)
         scope._outgrown.clear()           # nothing but records points at it, and those keep it themselves
+        _recent = (stream, device, scope)
         return found
