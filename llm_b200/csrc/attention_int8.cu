@@ -49,6 +49,7 @@ struct Args {
     float* wide_stats;
     int2* few_blocks_of;             // [n_seqs, n_kv_heads] which blocks have parts of a pair, [n_seqs, n_kv_heads, tiles] of a tile
     int2* wide_blocks_of;
+    int* arrived;                    // [n_seqs, n_kv_heads] zeros: how many of a pair's parts are there, where its last block joins them (null: a launch does)
 };
 
 // What a kernel reports (no wait has these codes): a step that brings more tokens than max_new says; a place outside of what the call was given, which is
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, DMAX == 64 ? 2 : 1) attention_in
 // equal length, so a block's range covers the end of one pair, some whole ones, and the beginning of another. Pairs that one block has done as a whole are
 // finished there, of the others each block leaves a part. A block has four warps, each with a ring of units of its own, 32 positions or 64 (TMA, rows
 // swizzled so that both the reads of keys, four lanes a row, and those of values, eight columns a lane, touch all banks once), which runs on over the
-// ends of pairs; warps meet where a pair ends.
+// ends of pairs; warps meet where a pair ends. Of a pair that several blocks have, the last one to come joins the parts, or a launch does (plan_for).
 //
 // 64 sequences of 8,192 positions (32 heads over 8 of 128, 1.08 GB) take 173 us in short bursts, 6.2 TB/s, and 204 in long loops at the power cap: reading
 // is the limit, and the energy of some 780 instructions for 8 KB. Eight take 37 us, one 11 on the device: 10 of them are a block's start (lengths, table,
@@ -600,7 +601,7 @@ template <int HD, int NT> struct Few {
     static constexpr int RING = FEW_WARPS * STAGES * 2 * TILE;
     static constexpr int MERGE = 2 * (8 * NT * LD + 8 * NT * 4) * 4;            // two warps' rows, and their references
     static constexpr int SCALES = FEW_WARPS * STAGES * 2 * UNIT<HD> * 4;
-    static constexpr int BYTES = RING + MERGE + SCALES + FEW_WARPS * STAGES * 8 + 16;
+    static constexpr int BYTES = RING + MERGE + SCALES + FEW_WARPS * STAGES * 8 + 16 + 64;                       // 64: Edge twice, and two answers
     static_assert(BLOCKS * (BYTES + 1024) <= 227 * 1024, "blocks of an SM");
 };
 
@@ -730,6 +731,53 @@ __device__ __forceinline__ int2 blocks_of(int start, int count, int per) {
     return make_int2(first, (start + count - 1) / per - first + 1);
 }
 
+// A pair that the block has a part of, as the joining needs it.
+struct Edge {
+    int pair, start, pages, first_token, n_rows, out_column;
+};
+// A warp joins the parts of row r of a pair that blocks of.x .. of.x + of.y - 1 have, in their order whoever joins. (Read from L2: other blocks wrote them.)
+template <int HD>
+__device__ __forceinline__ void join_here(const float* acc, const float2* stats, int2 of, int r, __nv_bfloat16* to, int lane) {
+    constexpr int W = HD / 32, AHEAD = 16;                     // a lane's columns, parts under way
+    auto part_of = [&](int k) { return ((size_t)(of.x + k) * 2 + (k == 0 ? 1 : 0)) * FEW_ROWS + r; };
+    float x[AHEAD][W], value[W], sum = 0.f, m = -INFINITY;
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+#pragma unroll
+            for (int c = 0; c < W; ++c) x[j][c] = 0.f;
+            if (k0 + j >= of.y) continue;
+            const float* from = acc + part_of(k0 + j) * HD + lane * W;
+            if constexpr (W == 4) *reinterpret_cast<float4*>(x[j]) = __ldcg(reinterpret_cast<const float4*>(from));
+            else *reinterpret_cast<float2*>(x[j]) = __ldcg(reinterpret_cast<const float2*>(from));
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < W; ++c) value[c] = 0.f;
+    fetch(0);
+    for (int k = lane; k < of.y; k += 32) m = fmaxf(m, __ldcg(stats + part_of(k)).x);
+    m = warp_max(m);
+    const float against = m == -INFINITY ? 0.f : m;
+    for (int k0 = 0; k0 < of.y; k0 += 32) {
+        const float2 st = k0 + lane < of.y ? __ldcg(stats + part_of(k0 + lane)) : make_float2(-INFINITY, 0.f);
+        const float weight = st.y != 0.f ? exp2f(st.x - against) : 0.f;
+        sum += st.y * weight;
+        for (int j0 = 0; j0 < 32 && k0 + j0 < of.y; j0 += AHEAD) {
+            if (k0 + j0) fetch(k0 + j0);
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const float of_part = __shfl_sync(0xffffffffu, weight, j0 + j);
+#pragma unroll
+                for (int c = 0; c < W; ++c) value[c] = fmaf(x[j][c], of_part, value[c]);
+            }
+        }
+    }
+    sum = warp_sum(sum);
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int c = 0; c < W; c += 2) *reinterpret_cast<uint32_t*>(to + lane * W + c) = pack_bf16(value[c] * inv, value[c + 1] * inv);
+}
+
 template <int HD, int NT>
 __global__ void __launch_bounds__(FEW_THREADS, Few<HD, NT>::BLOCKS)
 attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a, int* status) {
@@ -744,10 +792,16 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
     uint64_t* full = reinterpret_cast<uint64_t*>(base + F::RING + F::MERGE + F::SCALES) + warp * STAGES;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(base + F::RING + F::MERGE + F::SCALES + FEW_WARPS * STAGES * 8);
 
+    // the block's first pair, where another block begins it, and its last, where another one ends it; whether this block joins them
+    Edge* edges = reinterpret_cast<Edge*>(base + F::RING + F::MERGE + F::SCALES + FEW_WARPS * STAGES * 8 + 16);
+    int* joins = reinterpret_cast<int*>(edges + 2);
     griddep_launch();
     if (lane == 0) {
         for (int i = 0; i < STAGES; ++i) mbar_init(smem_u32(&full[i]), 1);
-        if (warp == 0) *abort_flag = 0;
+        if (warp == 0) {
+            *abort_flag = 0;
+            edges[0].n_rows = edges[1].n_rows = 0;
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -830,7 +884,7 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         const Span& span = pair.span;
         const int n_rows = span.n_new * share;
         const int pair_begin = pair.start - r0, pair_end = pair_begin + span.pages, range_end = r1 - r0;       // in pages of the range
-        if (per && pair_begin >= 0 && threadIdx.x == 0) a.few_blocks_of[pair.seq * a.n_kv_heads + pair.head] = blocks_of(pair.start, span.pages, per);
+        if (per && !a.arrived && pair_begin >= 0 && threadIdx.x == 0) a.few_blocks_of[pair.seq * a.n_kv_heads + pair.head] = blocks_of(pair.start, span.pages, per);
         const int end = min(pair_end, range_end);
         const int limit = span.first_pos + span.n_new - 1, low = first_seen(a, span.first_pos);       // positions that a row sees at all,
         const int all_to = span.first_pos, all_from = first_seen(a, limit);                           // and that all rows see
@@ -1122,6 +1176,8 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         }
         if (warp == 0) {
             const bool whole = pair_begin >= 0 && pair_end <= range_end;
+            if (!whole && lane == 0)
+                edges[pair_begin >= 0] = Edge{pair.seq * a.n_kv_heads + pair.head, pair.start, span.pages, span.first_token, n_rows, pair.head * share * HD};
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -1151,6 +1207,28 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         }
         if (end >= range_end) break;
         next_pair(a, pair, most_tokens);
+    }
+    if (NT == 1 && a.arrived) {
+        // the block whose part of a pair comes last joins all, and leaves the count as it was
+        if (warp == 0) {
+            __threadfence();
+            __syncwarp();
+            if (lane < 2) {
+                const Edge& e = edges[lane];
+                const bool last = e.n_rows > 0 && atomicAdd(a.arrived + e.pair, 1) == blocks_of(e.start, e.pages, per).y - 1;
+                if (last) a.arrived[e.pair] = 0;
+                joins[lane] = last;
+            }
+        }
+        __syncthreads();
+        for (int i = 0; i < 2; ++i) {
+            if (!joins[i]) continue;
+            __threadfence();
+            const Edge e = edges[i];
+            for (int r = warp; r < e.n_rows; r += FEW_WARPS)
+                join_here<HD>(a.acc, reinterpret_cast<const float2*>(a.stats), blocks_of(e.start, e.pages, per), r,
+                              static_cast<__nv_bfloat16*>(a.out) + (size_t)(e.first_token + r / share) * a.out_stride + e.out_column + r % share * HD, lane);
+        }
     }
     __syncthreads();
     if (*abort_flag)                                           // a wait ran out: copies in flight get their time before the block leaves
@@ -2060,6 +2138,7 @@ struct Plan {
     int deal_blocks, deal_least, wide_blocks, wide_least;
     int rows;                        // of a block on the CUDA cores: 4 or 8 where a step has no more, 0: 32
     int tiles, slots;
+    bool joins;                      // the kernel for few rows joins its parts itself
     long long part_rows, wide_rows;  // rows that are joined from parts
     int launches;
 };
@@ -2068,6 +2147,10 @@ struct Plan {
 // block's, which saves the launch that joins, 4 us of the host's time: with 500 positions one sequence takes 8.3 us on the device, dealt out 7.7, 64
 // take 20.1 and 20.8; with 1,000 positions one takes 13.5 and 8.0, 16 take 19.2 and 15.2.
 constexpr int WHOLE_PAGES = 8, LEAST_PAGES = 4;
+// The blocks join their parts themselves where a pair has up to 8 rows and no more than so many parts (a block joins one after another what a launch of its own
+// spreads), and where a block has no more than so many pages: the end of a block, a fence and a count take 2 us, a launch 4 of the host's and 4 of the
+// device's. Eight sequences of 8,192 positions (19 pages a block) take 35.5 us, with a launch 38.3; 64 (148 pages, and all blocks end at once) 207 and 203.
+constexpr int JOIN_PARTS = 64, JOIN_PAGES = 48;
 // The kernel for any shape cuts a sequence where it may have more pages than this.
 constexpr int SIMT_WHOLE_PAGES = 4;
 // The kernel for many rows deals steps out, LEAST_STEPS a block at least, unless no tile has more than WHOLE_STEPS.
@@ -2097,7 +2180,8 @@ Plan plan_for(const Sizes& z) {
                 p.deal_blocks = (int)(most < held ? most : held);
                 p.few_blocks = p.deal_blocks;
                 p.part_rows = 2ll * p.deal_blocks * FEW_ROWS;
-                ++p.launches;
+                p.joins = (long long)p.few_tokens * share <= 8 && p.deal_blocks <= JOIN_PARTS * z.n_kv_heads && pages * pairs <= (long long)JOIN_PAGES * p.deal_blocks;
+                if (!p.joins) ++p.launches;
             }
         }
         if (p.wide) {
@@ -2146,7 +2230,7 @@ long long scratch_floats_of(long long parts, int head_dim) { return value_floats
 // and of what says which blocks have them
 long long places_of(const Plan& p, const Sizes& z) {
     const long long pairs = (long long)z.n_seqs * z.n_kv_heads;
-    return (p.deal_blocks ? pairs : 0) + (p.wide_blocks ? pairs * p.tiles : 0);
+    return (p.deal_blocks && !p.joins ? pairs : 0) + (p.wide_blocks ? pairs * p.tiles : 0);
 }
 
 // A kernel's shared memory is a setting of each device.
@@ -2215,7 +2299,7 @@ int launch_few(const Args& a, const Plan& p, int* status, cudaStream_t stream) {
     if (!code) code = make_map_int8(&map_v, a.values, rows, HD);
     if (code) return code;
     llmb::launch(attention_int8_few_kernel<HD, NT>, dim3((unsigned)p.few_blocks), FEW_THREADS, Few<HD, NT>::BYTES, stream, true, map_k, map_v, a, status);
-    if ((code = check_launch("attention_int8_few")) || p.deal_blocks == 0) return code;
+    if ((code = check_launch("attention_int8_few")) || p.deal_blocks == 0 || p.joins) return code;
     // as many warps a row as there is room for: a few rows have many parts each
     const int joined = a.n_seqs * a.n_kv_heads * a.few_tokens * (a.n_heads / a.n_kv_heads);
     if (joined <= 4 * SMS) llmb::launch(attention_int8_few_join_kernel<HD, 8>, dim3(joined), JOIN_WARPS * 32, 0, stream, true, a, joined);
@@ -2293,18 +2377,20 @@ bool sane(const llmb_int8_sizes& z) {
 }
 }  // namespace
 
-// Floats of scratch that a call of these sizes needs, and the number of its launches in *kernels.
-LLMB_EXPORT long long llmb_attention_int8_scratch_floats(const llmb_int8_sizes* z, int* kernels) {
-    *kernels = 1;
+// Floats of scratch that a call of these sizes needs, the number of its launches in counts[0] and of its counters in counts[1].
+LLMB_EXPORT long long llmb_attention_int8_scratch_floats(const llmb_int8_sizes* z, int* counts) {
+    counts[0] = 1;
+    counts[1] = 0;
     if (!sane(*z)) return 0;
     const Plan p = plan_for(sizes_of(*z));
-    *kernels = p.launches;
+    counts[0] = p.launches;
+    counts[1] = p.joins ? z->n_seqs * z->n_kv_heads : 0;
     return scratch_floats_of(p.part_rows * p.slots + p.wide_rows, z->head_dim) + 2 * places_of(p, sizes_of(*z));
 }
 
 LLMB_EXPORT int llmb_attention_int8(const void* q, const void* keys, const float* key_scales, const void* values, const float* value_scales,
                                     const int* block_table, const int* seq_lens, const int* cu_seqlens, const int* seq_order, void* out, float* scratch,
-                                    long long scratch_floats, float scale, const llmb_int8_sizes* sizes, cudaStream_t stream) {
+                                    long long scratch_floats, int* arrived, int n_arrived, float scale, const llmb_int8_sizes* sizes, cudaStream_t stream) {
     const llmb_int8_sizes& z = *sizes;
     if (z.n_tokens == 0 || z.n_seqs == 0) return LLMB_OK;
     LLMB_REQUIRE(z.dtype == LLMB_DTYPE_F32 || z.dtype == LLMB_DTYPE_BF16, "attention_int8: float32 and bfloat16 are built");
@@ -2330,6 +2416,7 @@ LLMB_EXPORT int llmb_attention_int8(const void* q, const void* keys, const float
     const long long parts = p.part_rows * p.slots, all_parts = parts + p.wide_rows;
     LLMB_REQUIRE(all_parts == 0 || (scratch != nullptr && aligned(scratch) && scratch_floats >= scratch_floats_of(all_parts, z.head_dim) + 2 * places_of(p, s)),
                  "attention_int8: scratch too small");
+    LLMB_REQUIRE(!p.joins || (arrived && n_arrived >= pairs), "attention_int8: %d counters for %lld sequences' heads", n_arrived, pairs);
     static int* status = nullptr;                // (one address for all devices)
     if (!status && status_word()) LLMB_CUDA(cudaHostGetDevicePointer((void**)&status, status_word(), 0));
     float* stats = scratch + value_floats(all_parts, z.head_dim);
@@ -2337,7 +2424,8 @@ LLMB_EXPORT int llmb_attention_int8(const void* q, const void* keys, const float
     const Args a{q, (const signed char*)keys, key_scales, (const signed char*)values, value_scales, block_table, seq_lens, cu_seqlens, seq_order, out, scratch,
                  stats, z.q_stride, z.out_stride, z.table_stride, z.ring_pages, z.n_pages, z.n_tokens, z.n_seqs, z.n_heads, z.n_kv_heads, z.head_dim,
                  shift, z.window, scale * LOG2E, z.max_new, p.tiles, p.slots, p.few_tokens, p.deal_blocks, p.deal_least, p.wide_blocks, p.wide_least,
-                 scratch + parts * z.head_dim, stats + 2 * parts, places, places + (p.deal_blocks ? pairs : 0)};
+                 scratch + parts * z.head_dim, stats + 2 * parts, places, places + (p.deal_blocks && !p.joins ? pairs : 0),
+                 p.joins ? arrived : nullptr};
     return z.dtype == LLMB_DTYPE_F32 ? run<float>(a, p, s, status, stream) : run<__nv_bfloat16>(a, p, s, status, stream);
 }
 

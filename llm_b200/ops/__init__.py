@@ -1790,12 +1790,12 @@ def rope_cache_write_int8(qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_t
 
 @functools.lru_cache(maxsize=4096)
 def _int8_plan(*sizes) -> tuple:
-    """(the sizes of a call as the library takes them, floats of scratch, launches)."""
-    _declare("attention_int8", "llmb_attention_int8", [_c_void] * 11 + [ctypes.c_longlong, _c_float, _c_void, _c_void])
-    lib, kernels, packed = load_library("attention_int8"), ctypes.c_int(0), (_c_int * len(sizes))(*sizes)
+    """(the sizes of a call as the library takes them, floats and counters of scratch, launches)."""
+    _declare("attention_int8", "llmb_attention_int8", [_c_void] * 11 + [ctypes.c_longlong, _c_void, _c_int, _c_float, _c_void, _c_void])
+    lib, counts, packed = load_library("attention_int8"), (_c_int * 2)(), (_c_int * len(sizes))(*sizes)
     lib.llmb_attention_int8_scratch_floats.restype = ctypes.c_longlong
-    floats = lib.llmb_attention_int8_scratch_floats(packed, ctypes.byref(kernels))
-    return packed, ctypes.addressof(packed), floats, kernels.value
+    floats = lib.llmb_attention_int8_scratch_floats(packed, counts)
+    return packed, ctypes.addressof(packed), floats, counts[1], counts[0]
 
 
 def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seqlens, n_heads, n_kv_heads, head_dim, scale, window=0, *, max_new,
@@ -1838,15 +1838,15 @@ def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seql
     at_q, at_out = qkv.data_ptr(), out.data_ptr()
     tc = int(dtype is torch.bfloat16 and head_dim in (64, 128) and scale > 0 and q_stride % 8 == 0 and not (at_q | at_out) & 15
              and keys.shape[0] * n_kv_heads * PAGE < 1 << 31 and not tactics.is_disabled("attention_int8_tc"))
-    packed, at_sizes, floats, kernels = _int8_plan(q_stride, n_heads * head_dim, block_table.stride(0), ring_pages, keys.shape[0], code, n, n_seqs,
-                                                   n_heads, n_kv_heads, head_dim, keys.block, window, max_new, max_len, tc)
-    parts = _scratch(qkv.device, "attention", floats)[0] if floats else None
+    packed, at_sizes, floats, counters, kernels = _int8_plan(q_stride, n_heads * head_dim, block_table.stride(0), ring_pages, keys.shape[0], code, n,
+                                                             n_seqs, n_heads, n_kv_heads, head_dim, keys.block, window, max_new, max_len, tc)
+    parts, arrived = _scratch(qkv.device, "attention", floats, counters) if floats else (None, None)
     if _recording is not None:
-        _recording.keep += [qkv, keys, values, block_table, seq_lens, cu_seqlens, seq_order, out, parts, packed]
+        _recording.keep += [qkv, keys, values, block_table, seq_lens, cu_seqlens, seq_order, out, parts, arrived, packed]
     _call("attention_int8", "llmb_attention_int8", at_q, keys.values.data_ptr(), keys.scales.data_ptr(), values.values.data_ptr(),
           values.scales.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), cu_seqlens.data_ptr(),
-          None if seq_order is None else seq_order.data_ptr(), at_out, parts.data_ptr() if floats else None, floats, float(scale), at_sizes,
-          _stream(), kernels=kernels)
+          None if seq_order is None else seq_order.data_ptr(), at_out, parts.data_ptr() if floats else None, floats,
+          arrived.data_ptr() if counters else None, counters, float(scale), at_sizes, _stream(), kernels=kernels)
     return out
 
 

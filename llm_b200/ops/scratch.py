@@ -16,7 +16,7 @@ import torch
 
 STREAMS = 8
 _LEAST = {"products": (148 * 2 * 128 * 256, 1 << 14),     # what a product on pairs of SMs asks for at most; tile counters
-          "attention": (1 << 23, 0)}
+          "attention": (1 << 23, 1 << 12)}                 # parts of rows; how many of a sequence's there are
 
 generation = 0                            # grows with that of every scope and stream
 _line = threading.local()                 # .entered: the scopes that this thread is inside of

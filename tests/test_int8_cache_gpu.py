@@ -563,3 +563,75 @@ def test_a_prompt_and_its_next_tokens(dtype, heads, kv_heads, dim, block):
         scale = keys.scales.double()[table[s].long()[row // PAGE], :, row % PAGE // block]
         # half a step, and half of each step that the block was in before it grew: less than one step in all
         assert bool(((got - torch.cat(exact[s])).abs() <= scale[..., None] * (0.5 if block == 1 else 1.0) + 1e-5).all())
+
+
+# (held, new, heads, kv_heads, dim, window): sequences that many blocks share, one long one among many short, few heads, up to 8 rows and above
+SHARED = [
+    ([8190], [1], 32, 8, 128, 0),
+    ([30000] + [3] * 20, [1] * 21, 16, 8, 64, 0),
+    ([4000, 0, 900], [2, 1, 0], 32, 8, 128, 0),
+    ([20000], [1], 8, 1, 128, 0),
+    ([2000, 2500, 700], [1, 1, 1], 4, 4, 64, 1500),
+    ([3000, 5000], [4, 2], 16, 4, 128, 0),
+    ([640 + 7 * i for i in range(40)], [1] * 40, 8, 8, 64, 0),
+]
+
+
+def test_attention_parts_that_meet():
+    """Parts of a pair are joined in their own order whichever block ends last, and counts of one shape's parts do not show in another's: calls of all
+    shapes in turn, some of them captured, give the same bits each time."""
+    batches = [make(held, new, heads, kv_heads, dim, BF16, window=window, seed=60 + i)
+               for i, (held, new, heads, kv_heads, dim, window) in enumerate(SHARED)]
+    first = [call(b) for b in batches]
+    for b, got in zip(batches, first):
+        check(b, got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [call(b) for b in batches]
+    for _ in range(10):
+        graph.replay()
+        for b, got, again in zip(batches, first, captured):
+            assert torch.equal(again, got)
+            again.zero_()
+        for b, got in zip(batches, first):
+            assert torch.equal(call(b), got)
+
+
+@pytest.mark.parametrize("dtype, heads, kv_heads, dim", [(BF16, 8, 2, 128), (F32, 4, 2, 64)])
+def test_steps_whose_lengths_are_counted_on_the_device(dtype, heads, kv_heads, dim):
+    """Lengths, positions and the table written by a tensor operation right in front of the calls, as a loop on the device has them: the same as
+    with everything waited for in between."""
+    held = [700, 5, 60, 0]
+    b = make(held, [1] * 4, heads, kv_heads, dim, dtype, seed=71)
+    steps = 60
+    n_pages, width = b["keys"].values.shape[0], 16
+    start = torch.stack([torch.randperm(64)[:width] + 64 * s for s in range(4)]).to(torch.int32).to(DEV)
+    x, angles = projection(dict(b, lengths=[1000]), dim, False, 72)
+    more = torch.randn(steps, *x.flatten(1).shape, generator=torch.Generator().manual_seed(73)).to(dtype).to(DEV)
+    _, seq = places(b)
+
+    def loop(wait):
+        gen = torch.Generator().manual_seed(74)
+        keys, values = (pages_of(256, kv_heads, dim, 16, gen) for _ in range(2))
+        for cache in (keys, values):
+            cache.scales.fill_(2.0 ** -5)
+        pos, lens, table, outs = ints(held), ints([h + 1 for h in held]), start.clone(), []
+        for i in range(steps):
+            if wait:
+                torch.cuda.synchronize()
+            q = ops().rope_cache_write_int8(more[i], angles, pos, seq, b["arrays"][1], table, width, keys, values, heads, kv_heads, dim)
+            if wait:
+                torch.cuda.synchronize()
+            outs.append(ops().attention_int8(q, keys, values, table, width, lens, b["arrays"][1], heads, kv_heads, dim, b["scale"], max_new=1, max_len=1024))
+            if wait:
+                torch.cuda.synchronize()
+            table.copy_((table + 1) % 256)                     # (other pages each time: what a stale table names holds something else)
+            lens.add_(1)
+            pos.add_(1)
+        torch.cuda.synchronize()
+        ops().check_device_status()
+        return torch.stack(outs)
+
+    want = loop(True)
+    for _ in range(5):
+        assert torch.equal(loop(False), want)
