@@ -1457,6 +1457,7 @@ def attention_replay_key(step, n_heads: int, n_kv_heads: int, window: int = 0):
 
 _prefix_entry = None
 _BEYOND_BOUNDS = 50             # its report of a step larger than its bounds (csrc/prefix_attention.cu)
+_FARTHEST = (1 << 31) - 1       # elements between rows, as the kernels count them
 _INT8_REPORTS = {50: "more tokens than max_new said", 51: "a position, sequence, token or page that there is not",
                  52: "a scale that is no power of two"}      # (csrc/attention_int8.cu, int8_cache.cu)
 
@@ -1770,9 +1771,11 @@ def rope_cache_write_int8(qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_t
     n_rot = n_positions = 0
     if rope_table is not None:
         if rope_table.dim() != 2 or rope_table.dtype is not torch.float32 or not rope_table.is_contiguous() or rope_table.shape[1] > head_dim \
-                or rope_table.shape[1] % 2:
+                or rope_table.shape[1] % 2 or rope_table.shape[0] == 0:
             raise KernelError(f"{what}: the table of angles must be contiguous float32 [positions, n_rot] with an even n_rot <= {head_dim}")
         n_positions, n_rot = rope_table.shape
+    if block_table.stride(0) > _FARTHEST:
+        raise KernelError(f"{what}: rows of the page table lie {block_table.stride(0)} apart")
     _check_device(what, keys, values, (qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_table, out))
     if out is None:
         out = qkv.new_empty((n, n_heads * head_dim))
@@ -1826,6 +1829,10 @@ def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seql
         _check_step(what, block_table, ring_pages, n_seqs, vectors if seq_order is None else vectors + ((seq_order, n_seqs, "seq_order"),))
     if max_new < 1 or max_len < 1 or window < 0 or not math.isfinite(scale):
         raise KernelError(f"{what}: max_new {max_new}, max_len {max_len}, window {window}, scale {scale}")
+    if q_stride > _FARTHEST or block_table.stride(0) > _FARTHEST:
+        raise KernelError(f"{what}: rows lie {q_stride} and {block_table.stride(0)} (of the page table) apart")
+    if window > ring_pages * PAGE:                             # more than a sequence holds
+        window = 0
     _check_device(what, keys, values, (qkv, block_table, seq_lens, cu_seqlens, seq_order, out))
     if out is None:
         out = qkv.new_empty((n, n_heads * head_dim))

@@ -65,3 +65,16 @@ def attended(n=4, heads=4, kv=2, dim=16):
 def test_attentions_that_are_refused(wrong):
     with pytest.raises(KernelError):
         ops.attention_int8(**{**attended(), **wrong})
+
+
+def test_what_an_integer_does_not_hold_is_refused():
+    far = torch.empty_strided((4, 64), (1 << 31, 1), device="meta")
+    with pytest.raises(KernelError, match="apart"):
+        ops.attention_int8(**{**attended(), "qkv": far})
+    table = torch.empty_strided((1, 2), (1 << 31, 1), dtype=torch.int32, device="meta")
+    with pytest.raises(KernelError, match="apart"):
+        ops.attention_int8(**{**attended(), "block_table": table})
+    with pytest.raises(KernelError, match="apart"):
+        ops.rope_cache_write_int8(**{**step(), "block_table": table})
+    with pytest.raises(KernelError, match="table of angles"):                              # (no rows: not the same as no table)
+        ops.rope_cache_write_int8(**{**step(), "rope_table": torch.zeros(0, 16)})

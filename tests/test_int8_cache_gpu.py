@@ -635,3 +635,13 @@ def test_steps_whose_lengths_are_counted_on_the_device(dtype, heads, kv_heads, d
     want = loop(True)
     for _ in range(5):
         assert torch.equal(loop(False), want)
+
+
+@pytest.mark.parametrize("dtype, new", [(BF16, [1, 1]), (BF16, [70, 3]), (F32, [2, 1])])
+def test_attention_windows_beyond_all_positions(dtype, new):
+    """A window that no sequence fills, whatever its number, is none."""
+    b = make([900, 40], new, 8, 2, 64, dtype, seed=81)
+    want = call(b)
+    for window in (b["ring"] * PAGE + 1, 2 ** 31 - 1, 2 ** 32 + 5):
+        assert torch.equal(call(dict(b, window=window)), want)
+    check(dict(b, window=b["ring"] * PAGE), call(dict(b, window=b["ring"] * PAGE)))
