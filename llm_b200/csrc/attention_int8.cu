@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, DMAX == 64 ? 2 : 1) attention_in
 // equal length, so a block's range covers the end of one pair, some whole ones, and the beginning of another. Pairs that one block has done as a whole are
 // finished there, of the others each block leaves a part. A block has four warps, each with a ring of units of its own, 32 positions or 64 (TMA, rows
 // swizzled so that both the reads of keys, four lanes a row, and those of values, eight columns a lane, touch all banks once), which runs on over the
-// ends of pairs; warps meet where a pair ends. Of a pair that several blocks have, the last one to come joins the parts, or a launch does (plan_for).
+// ends of pairs; warps meet where a pair ends. Of a pair that several blocks have, a launch joins the parts, or the last block to come (plan_for).
 //
 // 64 sequences of 8,192 positions (32 heads over 8 of 128, 1.08 GB) take 173 us in short bursts, 6.2 TB/s, and 204 in long loops at the power cap: reading
 // is the limit, and the energy of some 780 instructions for 8 KB. Eight take 37 us, one 11 on the device: 10 of them are a block's start (lengths, table,
@@ -1209,15 +1209,14 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
         next_pair(a, pair, most_tokens);
     }
     if (NT == 1 && a.arrived) {
-        // the block whose part of a pair comes last joins all, and leaves the count as it was
+        // the block whose part of a pair comes last joins all, and the count is zero again
         if (warp == 0) {
             __threadfence();
             __syncwarp();
             if (lane < 2) {
                 const Edge& e = edges[lane];
-                const bool last = e.n_rows > 0 && atomicAdd(a.arrived + e.pair, 1) == blocks_of(e.start, e.pages, per).y - 1;
-                if (last) a.arrived[e.pair] = 0;
-                joins[lane] = last;
+                const unsigned last = blocks_of(e.start, e.pages, per).y - 1;
+                joins[lane] = e.n_rows > 0 && atomicInc(reinterpret_cast<unsigned*>(a.arrived) + e.pair, last) == last;
             }
         }
         __syncthreads();
@@ -2128,7 +2127,7 @@ __global__ void __launch_bounds__(256, CHUNKS == 1 ? 5 : 3) attention_int8_join_
 
 struct Sizes {
     int n_tokens, n_seqs, n_heads, n_kv_heads, head_dim, window, max_new, max_len;
-    bool tc;
+    bool tc, alone;
 };
 
 struct Plan {
@@ -2147,9 +2146,11 @@ struct Plan {
 // block's, which saves the launch that joins, 4 us of the host's time: with 500 positions one sequence takes 8.3 us on the device, dealt out 7.7, 64
 // take 20.1 and 20.8; with 1,000 positions one takes 13.5 and 8.0, 16 take 19.2 and 15.2.
 constexpr int WHOLE_PAGES = 8, LEAST_PAGES = 4;
-// The blocks join their parts themselves where a pair has up to 8 rows and no more than so many parts (a block joins one after another what a launch of its own
-// spreads), and where a block has no more than so many pages: the end of a block, a fence and a count take 2 us, a launch 4 of the host's and 4 of the
-// device's. Eight sequences of 8,192 positions (19 pages a block) take 35.5 us, with a launch 38.3; 64 (148 pages, and all blocks end at once) 207 and 203.
+// The blocks join their parts themselves in calls outside of a step that is replayed, where a pair has up to 8 rows and no more than so many parts (a block joins
+// one after another what a launch of its own spreads), and a block has no more than so many pages. A launch costs the host 2.5 us and, behind the kernel in a
+// captured step, next to nothing; the end of a block, a fence, a count and the parts' way through L2 take 3. Calls one by one: eight sequences of 8,192
+// positions (19 pages a block) take 35.8 us and with a launch 38.4, one 18.1 and 20.5, 64 (148 pages, all blocks end at once) 207 and 203. Captured: one 14.1 and
+// 11.0, eight 38.2 and 37.7.
 constexpr int JOIN_PARTS = 64, JOIN_PAGES = 48;
 // The kernel for any shape cuts a sequence where it may have more pages than this.
 constexpr int SIMT_WHOLE_PAGES = 4;
@@ -2180,7 +2181,7 @@ Plan plan_for(const Sizes& z) {
                 p.deal_blocks = (int)(most < held ? most : held);
                 p.few_blocks = p.deal_blocks;
                 p.part_rows = 2ll * p.deal_blocks * FEW_ROWS;
-                p.joins = (long long)p.few_tokens * share <= 8 && p.deal_blocks <= JOIN_PARTS * z.n_kv_heads && pages * pairs <= (long long)JOIN_PAGES * p.deal_blocks;
+                p.joins = z.alone && (long long)p.few_tokens * share <= 8 && p.deal_blocks <= JOIN_PARTS * z.n_kv_heads && pages * pairs <= (long long)JOIN_PAGES * p.deal_blocks;
                 if (!p.joins) ++p.launches;
             }
         }
@@ -2365,11 +2366,12 @@ struct llmb_int8_sizes {
     int dtype, n_tokens, n_seqs, n_heads, n_kv_heads, head_dim, block, window;
     int max_new, max_len;                                           // upper bounds (ops.attention_int8)
     int tc;                                                         // whether the tensor-core kernels take the call (refused where they cannot), 0: the CUDA cores
+    int alone;                                                      // the call is no part of a step that is replayed: a launch costs the host its time
 };
 
 namespace {
 Sizes sizes_of(const llmb_int8_sizes& z) {
-    return Sizes{z.n_tokens, z.n_seqs, z.n_heads, z.n_kv_heads, z.head_dim, z.window, z.max_new, z.max_len, z.tc != 0};
+    return Sizes{z.n_tokens, z.n_seqs, z.n_heads, z.n_kv_heads, z.head_dim, z.window, z.max_new, z.max_len, z.tc != 0, z.alone != 0};
 }
 bool sane(const llmb_int8_sizes& z) {
     return z.n_tokens > 0 && z.n_seqs > 0 && z.n_kv_heads > 0 && z.n_heads > 0 && z.n_heads % z.n_kv_heads == 0 && z.max_new > 0 && z.max_len > 0 &&

@@ -1846,7 +1846,8 @@ def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seql
     tc = int(dtype is torch.bfloat16 and head_dim in (64, 128) and scale > 0 and q_stride % 8 == 0 and not (at_q | at_out) & 15
              and keys.shape[0] * n_kv_heads * PAGE < 1 << 31 and not tactics.is_disabled("attention_int8_tc"))
     packed, at_sizes, floats, counters, kernels = _int8_plan(q_stride, n_heads * head_dim, block_table.stride(0), ring_pages, keys.shape[0], code, n,
-                                                             n_seqs, n_heads, n_kv_heads, head_dim, keys.block, window, max_new, max_len, tc)
+                                                             n_seqs, n_heads, n_kv_heads, head_dim, keys.block, window, max_new, max_len, tc,
+                                                             0 if scratch.inside() else 1)
     parts, arrived = _scratch(qkv.device, "attention", floats, counters) if floats else (None, None)
     if _recording is not None:
         _recording.keep += [qkv, keys, values, block_table, seq_lens, cu_seqlens, seq_order, out, parts, arrived, packed]

@@ -645,3 +645,19 @@ def test_attention_windows_beyond_all_positions(dtype, new):
     for window in (b["ring"] * PAGE + 1, 2 ** 31 - 1, 2 ** 32 + 5):
         assert torch.equal(call(dict(b, window=window)), want)
     check(dict(b, window=b["ring"] * PAGE), call(dict(b, window=b["ring"] * PAGE)))
+
+
+@pytest.mark.parametrize("which", range(len(SHARED)))
+def test_attention_parts_inside_a_step(which):
+    """The same shapes inside a step's scope, where a launch of its own joins the parts."""
+    held, new, heads, kv_heads, dim, window = SHARED[which]
+    b = make(held, new, heads, kv_heads, dim, BF16, window=window, seed=90 + which)
+    with ops().StepScope():
+        check(b, call(b))
+        first, graph = call(b), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            again = call(b)
+    for _ in range(3):
+        again.zero_()
+        graph.replay()
+        assert torch.equal(again, first)
