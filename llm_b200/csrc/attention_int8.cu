@@ -2028,17 +2028,18 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_wide_join_kern
 // ------------------------------------------------------------------------------------------------ the parts joined
 //
 // WARPS warps a row: each reads all the maxima and sums, a lane two parts, and takes every WARPS-th part, several of them in flight; their
-// sums are added in order. CHUNKS: 128 columns of the head each.
+// sums are added in order. CHUNKS: 128 columns of the head each. Rows of tokens that no sequence has (a padded batch) have no parts, and are left as they are.
 template <typename T, int WARPS, int CHUNKS>
 __global__ void __launch_bounds__(256, CHUNKS == 1 ? 5 : 3) attention_int8_join_kernel(const __grid_constant__ Args a, int n_rows) {
     constexpr int ROWS = 8 / WARPS, AHEAD = 4;
     __shared__ float4 shared_value[8][CHUNKS * 32];
     griddep_launch();
+    const int first_token = a.cu_seqlens[0], end_token = a.cu_seqlens[a.n_seqs];
     griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp % WARPS;
-    const int row = blockIdx.x * ROWS + warp / WARPS;
+    const int row = blockIdx.x * ROWS + warp / WARPS, token = row / a.n_heads;
     const int D = a.head_dim, slots = a.slots, width = (D + 3) / 4;
-    const bool valid = row < n_rows, vectors = D % 4 == 0;
+    const bool valid = row < n_rows && token >= first_token && token < end_token, vectors = D % 4 == 0;
     float4 value[CHUNKS];
     float sum = 0.f;
 #pragma unroll
@@ -2112,7 +2113,7 @@ __global__ void __launch_bounds__(256, CHUNKS == 1 ? 5 : 3) attention_int8_join_
     }
     if (!valid) return;
     const float inv = sum != 0.f ? 1.f / sum : 0.f;
-    T* out = static_cast<T*>(a.out) + (size_t)(row / a.n_heads) * a.out_stride + (size_t)(row % a.n_heads) * D;
+    T* out = static_cast<T*>(a.out) + (size_t)token * a.out_stride + (size_t)(row % a.n_heads) * D;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
         const int col = (c * 32 + lane) * 4;

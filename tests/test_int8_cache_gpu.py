@@ -661,3 +661,42 @@ def test_attention_parts_inside_a_step(which):
         again.zero_()
         graph.replay()
         assert torch.equal(again, first)
+
+
+# ----------------------------------------------------------------------------- long padded batches
+
+def padded(b, rows):
+    """The batch with `rows` rows behind its last sequence's, and a result whose every element is 7."""
+    width = b["heads"] * b["dim"]
+    q = torch.cat([b["q"], torch.full((rows, width), math.nan, dtype=b["dtype"], device=DEV)])
+    return {**b, "q": q}, torch.full((q.shape[0], width), 7.0, dtype=b["dtype"], device=DEV)
+
+
+@pytest.mark.parametrize("dtype, dim", [(F32, 16), (F32, 64), (F32, 128), (BF16, 80), (BF16, 256), (BF16, 64), (BF16, 128)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [20, 1, 90], [3, 0, 2]])
+def test_attention_rows_behind_the_last_sequence_of_cut_ones(dtype, dim, new):
+    """A padded batch whose sequences are cut into parts: the padding is left as it is by what joins them, in calls one by one, inside of a
+    step, and in captured ones that are replayed on fewer tokens."""
+    b = make([2000, 3, 700], new, 4, 2, dim, dtype, seed=101)
+    n = b["cu"][-1]
+    wide, out = padded(b, 6)
+    call(wide, out=out)
+    check(b, out[:n].contiguous())
+    assert bool((out[n:] == 7).all())
+    with ops().StepScope():
+        out.fill_(7)
+        call(wide, out=out)
+        check(b, out[:n].contiguous())
+        assert bool((out[n:] == 7).all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(wide, out=out)
+    kept = n - new[2]
+    b["arrays"][1][3] = kept                                   # the last sequence brings nothing
+    b["arrays"][0][2] = 700
+    fewer = {**b, "new": new[:2] + [0], "cu": b["cu"][:3] + [kept], "lengths": b["lengths"][:2] + [700]}
+    for _ in range(2):
+        out.fill_(7)
+        graph.replay()
+        check(fewer, out[:kept].contiguous())
+        assert bool((out[kept:] == 7).all())
