@@ -67,6 +67,13 @@ struct Item {
     int page_begin, page_end;        // places in the table, before the ring
 };
 
+// the first key that a position sees
+__device__ __forceinline__ int first_seen(const Args& a, int position) { return a.window > 0 ? max(position - a.window + 1, 0) : 0; }
+// How many pages the new tokens of a sequence see: more than its ring has are not there any more (one would be read in another's place).
+__device__ __forceinline__ int pages_seen(const Args& a, int first_pos, int n_new) {
+    return (first_pos + n_new - 1) / LLMB_PAGE + 1 - first_seen(a, first_pos) / LLMB_PAGE;
+}
+
 // false where nothing is left for the block
 __device__ __forceinline__ bool item_of(const Args& a, int x, int slot, int tile_rows, Item& w, int* status) {
     w.kv_head = x % a.n_kv_heads;
@@ -83,7 +90,7 @@ __device__ __forceinline__ bool item_of(const Args& a, int x, int slot, int tile
     const int end_token = a.cu_seqlens[w.seq + 1];
     int n_new = end_token - w.first_token;
     w.first_pos = a.seq_lens[w.seq] - n_new;
-    if (w.first_token < 0 || end_token > a.n_tokens || (n_new > 0 && w.first_pos < 0)) {
+    if (w.first_token < 0 || end_token > a.n_tokens || (n_new > 0 && (w.first_pos < 0 || pages_seen(a, w.first_pos, n_new) > a.ring_pages))) {
         if (threadIdx.x == 0) report(status, OUT_OF_RANGE);
         return false;
     }
@@ -114,8 +121,6 @@ __device__ __forceinline__ int page_at(const Args& a, const int* pages, int logi
     report(status, OUT_OF_RANGE);
     return 0;
 }
-// the first key that a position sees
-__device__ __forceinline__ int first_seen(const Args& a, int position) { return a.window > 0 ? max(position - a.window + 1, 0) : 0; }
 
 // ------------------------------------------------------------------------------------------------ any type, any head size
 //
@@ -669,15 +674,14 @@ __device__ __forceinline__ Span span_of(const Args& a, int seq, int most_tokens)
     s.n_new = end - s.first_token;
     s.first_pos = a.seq_lens[seq] - s.n_new;
     s.first = first_seen(a, s.first_pos) / LLMB_PAGE;
-    s.pages = (s.first_pos + s.n_new - 1) / LLMB_PAGE + 1 - s.first;
+    s.pages = pages_seen(a, s.first_pos, s.n_new);
     if (s.n_new <= 0 || s.n_new > most_tokens || s.first_token < 0 || end > a.n_tokens || s.first_pos < 0 || s.pages > a.ring_pages) s.pages = 0;
     return s;
 }
 // What does not fit is reported: places that there are not, more tokens than max_new says.
 __device__ __forceinline__ void check_span(const Args& a, const Span& s, int* status) {
     if (s.n_new <= 0) return;
-    if (s.first_token < 0 || s.first_token + s.n_new > a.n_tokens || s.first_pos < 0 ||
-        (s.first_pos + s.n_new - 1) / LLMB_PAGE + 1 - s.first > a.ring_pages) report(status, OUT_OF_RANGE);
+    if (s.first_token < 0 || s.first_token + s.n_new > a.n_tokens || s.first_pos < 0 || pages_seen(a, s.first_pos, s.n_new) > a.ring_pages) report(status, OUT_OF_RANGE);
     else if (s.n_new > a.max_new) report(status, BEYOND_BOUNDS);
 }
 // A (sequence, key head) pair and where its pages stand among all. (There are fewer than 2^31: a sequence has no more than its ring.)

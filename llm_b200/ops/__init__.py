@@ -1809,8 +1809,8 @@ def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seql
     before it. Returns [T, Hq * D] in qkv's dtype.
 
     max_new, max_len: most new tokens and most positions of a sequence, upper bounds that size the launches (a sequence longer than max_len is
-    served all the same). A step that brings more tokens than max_new says, a page or token that there is not, and a scale that is no
-    power of two are reported by `check_device_status`; its results are not valid. `seq_order` (int32 [B]): the sequences by falling length, which start
+    served all the same). A step that brings more tokens than max_new says, a page or token that there is not, a sequence whose queries see more
+    pages than its ring has, and a scale that is no power of two are reported by `check_device_status`; its results are not valid. `seq_order` (int32 [B]): the sequences by falling length, which start
     in that order."""
     what = "attention_int8"
     if qkv.dim() != 2:

@@ -700,3 +700,21 @@ def test_attention_rows_behind_the_last_sequence_of_cut_ones(dtype, dim, new):
         graph.replay()
         check(fewer, out[:kept].contiguous())
         assert bool((out[kept:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype, dim", [(F32, 16), (F32, 128), (BF16, 80), (BF16, 64), (BF16, 128)])
+@pytest.mark.parametrize("held, new, window", [([1000, 20], [1, 1], 0), ([1000, 20], [40, 3], 0), ([700, 9], [1, 1], 300), ([190, 9], [70, 1], 0)])
+def test_attention_reports_sequences_longer_than_their_ring(dtype, dim, held, new, window):
+    """A sequence of which a step sees more pages than its ring has is reported, whichever kernel serves it; one that fits is not."""
+    from llm_b200.errors import KernelError
+    b = make(held, new, 4, 2, dim, dtype, window=window, seed=103)
+    check(b, call(b))
+    small = {**b, "ring": 4}                                   # (4 pages of the table)
+    call(small)
+    torch.cuda.synchronize()
+    with pytest.raises(KernelError, match="a step brought"):
+        ops().check_device_status()
+    check(b, call(b))
+    call({**small, "window": 50} if held[0] > 300 and max(new) < 50 else {**b, "ring": 5})
+    torch.cuda.synchronize()
+    ops().check_device_status()
