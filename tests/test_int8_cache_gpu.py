@@ -718,3 +718,64 @@ def test_attention_reports_sequences_longer_than_their_ring(dtype, dim, held, ne
     call({**small, "window": 50} if held[0] > 300 and max(new) < 50 else {**b, "ring": 5})
     torch.cuda.synchronize()
     ops().check_device_status()
+
+
+@pytest.mark.parametrize("dtype, heads, kv_heads, dim, new", [
+    (BF16, 8, 2, 128, [1, 1, 1]), (BF16, 8, 2, 128, [30, 1, 5]), (BF16, 4, 4, 64, [2, 1, 1]), (BF16, 4, 4, 64, [5, 300, 1]), (BF16, 4, 2, 80, [1, 1, 1]),
+    (BF16, 4, 2, 80, [30, 1, 5]), (F32, 8, 2, 128, [1, 2, 1]), (F32, 8, 2, 64, [30, 1, 5])])
+@pytest.mark.parametrize("inside", [False, True])
+def test_attention_replayed_on_another_batch(dtype, heads, kv_heads, dim, new, inside):
+    """A captured call replayed with other lengths, queries, pages and scales, and with the new tokens of the sequences dealt out another way."""
+    import contextlib
+    ring = 22
+    b = make([700, 80, 1000], new, heads, kv_heads, dim, dtype, ring=ring, seed=107)
+    others = [make([900, 5, 300], new, heads, kv_heads, dim, dtype, ring=ring, seed=108),
+              make([3, 600, 70], new[1:] + new[:1], heads, kv_heads, dim, dtype, ring=ring, seed=109)]
+    scope = ops().StepScope() if inside else contextlib.nullcontext()
+    with scope:
+        check(b, call(b, max_len=1300))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(b, max_len=1300)
+    graph.replay()
+    check(b, out)
+    for other in others:
+        n = other["keys"].values.shape[0]
+        assert n <= b["keys"].values.shape[0] and other["table"].shape == b["table"].shape and other["cu"][-1] == b["cu"][-1]
+        b["q"].copy_(other["q"])
+        b["table"].copy_(other["table"])
+        for mine, theirs in zip(b["arrays"], other["arrays"]):
+            mine.copy_(theirs)
+        for name in ("keys", "values"):
+            b[name].values[:n].copy_(other[name].values)
+            b[name].scales[:n].copy_(other[name].scales)
+        out.zero_()
+        graph.replay()
+        check(other, out)
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim", [(32, 8, 128), (8, 8, 64), (10, 2, 128)])
+@pytest.mark.parametrize("window", [0, 2100])
+def test_attention_single_tokens_beside_a_prompt(heads, kv_heads, dim, window):
+    """Steps that two kernels serve, each with its work dealt out and its parts in the same scratch: sequences of a few tokens at long and short
+    positions among prompts of 60 and 30."""
+    share = heads // kv_heads
+    held = [5000, 0, 3000, 4500, 200, 4000, 64, 2300] + [700 + 61 * i for i in range(24)]
+    new = [1, 60, 1, 30, 1, 16 // share, 0, 1] + [1] * 24
+    assert sum(new) < len(new) * (16 // share + 1)             # (some bring up to 16 rows for certain: both kernels are launched)
+    b = make(held, new, heads, kv_heads, dim, BF16, window=window, seed=113)
+    first = call(b)
+    check(b, first)
+    with ops().StepScope():
+        check(b, call(b))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            again = call(b)
+    for _ in range(2):
+        again.zero_()
+        graph.replay()
+        assert torch.equal(again, first)
+    b["arrays"][0][0] = 900                                    # (shorter, in the same captured launches)
+    b["lengths"][0] = 900
+    graph.replay()
+    check(b, again)
