@@ -23,7 +23,7 @@ from .. import native, ops
 from ..cache import PAGE, PagedCache, round_up
 from ..errors import FormatError, LlmError
 from ..parts.base import SharedPages, StepContext
-from .workspace import BufferRequest, Workspace
+from .workspace import Workspace
 
 
 GRAPH_AFTER_STEPS = 2      # plain steps of a shape before it is captured
@@ -115,9 +115,8 @@ class Engine:
         if cache_dtype not in (None, "int8", torch.int8):
             raise LlmError(f"a cache of {cache_dtype} (int8, or None for the run's type)")
         int8 = cache_dtype is not None
-        mixers = [model.blocks[item.layer].mixer for item in model.spec.schedule]
         if int8:
-            for mixer in mixers:
+            for mixer in (model.blocks[item.layer].mixer for item in model.spec.schedule):
                 if mixer.kv_request() is not None and not mixer.serves_int8_cache:
                     raise LlmError(f"{type(mixer).__name__} does not read a cache in 8 bits")
         ops.ensure_built(model.libraries() + (["int8_cache", "attention_int8"] if int8 else []))
@@ -131,13 +130,7 @@ class Engine:
                                 block_states=model.block_state_requests(), kv_dtype=torch.int8 if int8 else None, kv_block=cache_block)
         self.vocab = model.spec.vocab
         self.steps_run = 0
-        wanted = model.scratch_requests
-        if int8:
-            # (nothing here refers to the engine: its captured steps go when its last name does, not whenever garbage is collected)
-            def wanted(n_tokens, requests=model.scratch_requests, columns=max((m.int8_queries for m in mixers), default=0), dtype=self.dtype):
-                buffers = requests(n_tokens)
-                return buffers + [BufferRequest("int8_queries", (n_tokens, columns), dtype, 0, max((r.last_use for r in buffers), default=0))]
-        self.workspace = Workspace(self.device, wanted)
+        self.workspace = Workspace(self.device, model.scratch_requests)
         self.scope = ops.StepScope()      # the kernels' own scratch: one for all steps, as they have one arena
         self.use_graphs = (use_graphs and self.device.type == "cuda"
                            and os.environ.get("LLMB_NO_GRAPHS", "0") in ("", "0")

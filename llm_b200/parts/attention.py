@@ -30,10 +30,6 @@ class AttentionMixer(Mixer):
         return self.spec.n_heads * self.spec.head_dim
 
     @property
-    def int8_queries(self):
-        return self.q_width
-
-    @property
     def kv_width(self):
         return self.spec.n_kv_heads * self.spec.head_dim
 
@@ -78,8 +74,9 @@ class AttentionMixer(Mixer):
         from ..engine.workspace import BufferRequest
         s = self.spec
         # phases: 0 projections, 1 rotation + cache write, 2 attention, 3 output projection
-        return [BufferRequest("qkv", (n_tokens, self.q_width + 2 * self.kv_width), dtype, 0, 2),
-                BufferRequest("mixed", (n_tokens, self.q_width), dtype, 2, 3)]
+        # (with a cache in 8 bits "mixed" holds the rotated queries from phase 1 on, and the result of the attention lies in "qkv")
+        return [BufferRequest("qkv", (n_tokens, self.q_width + 2 * self.kv_width), dtype, 0, 3),
+                BufferRequest("mixed", (n_tokens, self.q_width), dtype, 1, 3)]
 
     def kernel_shapes(self, dtype, token_counts):
         s, out = self.spec, []
@@ -121,11 +118,12 @@ class AttentionMixer(Mixer):
         if isinstance(keys, ops.Int8Pages):
             qkv = ops.linear(h, self.w_qkv, self.b_qkv, out=out, norm=norm)
             queries = ops.rope_cache_write_int8(qkv, angles, ctx.tok_pos, ctx.tok_seq, ctx.cu_seqlens, table, ring, keys, values, s.n_heads,
-                                                s.n_kv_heads, s.head_dim, interleaved=interleaved, write_cache=(entry == cache_entry),
-                                                out=ctx.scratch("int8_queries", (n, self.q_width), h.dtype))
-            mixed = ops.attention_int8(queries, keys, values, table, ring, ctx.seq_lens, ctx.cu_seqlens, s.n_heads, s.n_kv_heads, s.head_dim,
-                                       s.scale, s.window, max_new=max(ctx.new_counts), max_len=ctx.max_len, out=mixed, seq_order=ctx.seq_order)
-            ops.linear(mixed, self.w_o, self.b_o, residual=residual, emit=emit)
+                                                s.n_kv_heads, s.head_dim, interleaved=interleaved, write_cache=(entry == cache_entry), out=mixed)
+            # (the projection is read: the result takes its place)
+            result = ops.attention_int8(queries, keys, values, table, ring, ctx.seq_lens, ctx.cu_seqlens, s.n_heads, s.n_kv_heads, s.head_dim,
+                                        s.scale, s.window, max_new=max(ctx.new_counts), max_len=ctx.max_len,
+                                        out=ctx.scratch("qkv", (n, self.q_width), h.dtype), seq_order=ctx.seq_order)
+            ops.linear(result, self.w_o, self.b_o, residual=residual, emit=emit)
             return
         if h.dtype == torch.bfloat16 and (angles is None or angles.shape[1] == s.head_dim):
             # the rotation and the cache write ride in the product's epilogue where its kernel has them

@@ -80,10 +80,8 @@ class Part:
     #: squares); a block runs ops.cast_sumsq behind parts that do not
     emits: bool = False
 
-    #: True if `forward` also works on a cache held in 8 bits (`ctx.cache.layer_view` then gives ops.Int8Pages), and
-    #: `int8_queries` columns of its scratch buffer "int8_queries" are wanted for that
+    #: True if `forward` also works on a cache held in 8 bits (`ctx.cache.layer_view` then gives ops.Int8Pages)
     serves_int8_cache: bool = False
-    int8_queries: int = 0
 
     #: True if `forward` takes `fresh=True` and then WRITES its result into `residual` (float32
     #: [T * result_terms, hidden]) instead of adding to it: what a block that norms a part's result needs

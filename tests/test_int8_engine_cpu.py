@@ -141,3 +141,42 @@ def test_mixers_of_other_designs_are_refused(tmp_path, plain_kernels):
     engine_of()
     with pytest.raises(LlmError, match="does not read a cache in 8 bits"):
         engine_of(cache_dtype="int8")
+
+
+@pytest.mark.parametrize("which", sorted(CONFIGS))
+def test_queries_and_results_lie_in_the_arena(tmp_path, plain_kernels, monkeypatch, which):
+    """The operators of a layer are given where to write to: buffers of the arena that do not overlap, and that an engine with a cache in the
+    run's type has too. (A result that is allocated in each call would be kept once for each layer and recorded step.)"""
+    from llm_b200 import ops
+    config, weights, engine = setup(tmp_path, monkeypatch, which)
+    seen = []
+
+    def inside(t, n, width):
+        begin, size = engine.workspace.arena.data_ptr(), engine.workspace.arena.numel()
+        assert t is not None and tuple(t.shape) == (n, width) and t.is_contiguous()
+        assert begin <= t.data_ptr() and t.data_ptr() + t.numel() * t.element_size() <= begin + size
+        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
+    def append(qkv, *args, out=None, **more):
+        a, b = inside(out, qkv.shape[0], args[8] * args[10])
+        assert b <= qkv.data_ptr() or qkv.data_ptr() + qkv.numel() * qkv.element_size() <= a
+        seen.append("append")
+        return plain_int8.rope_cache_write_int8(qkv, *args, out=out, **more)
+
+    def attention(q, *args, out=None, **more):
+        a, b = inside(out, q.shape[0], args[6] * args[8])
+        assert b <= q.data_ptr() or q.data_ptr() + q.numel() * q.element_size() <= a
+        seen.append("attention")
+        return plain_int8.attention_int8(q, *args, out=out, **more)
+
+    monkeypatch.setattr(ops, "rope_cache_write_int8", append)
+    monkeypatch.setattr(ops, "attention_int8", attention)
+    (slot,) = engine.acquire()
+    engine.step([Entry(slot, [1, 2, 3], [2])])
+    engine.step([Entry(slot, [4], [0])])
+    assert seen.count("append") == seen.count("attention") > 0
+    other = Engine(engine.model, max_tokens=2048)
+    for n in (1, 3, 100):
+        plan = engine.workspace.plan_for(n)
+        plan.check()
+        assert plan.total == other.workspace.plan_for(n).total

@@ -143,3 +143,30 @@ def test_generation_and_the_command_line(tmp_path, capsys):
     assert cli.main(arguments + [str(t) for t in prompt]) == 0
     assert [int(x) for x in capsys.readouterr().out.split()] == ids[0]
     assert cli.main(["bench", "-m", str(folder), "-c", "64", "-p", "16", "-n", "4", "-r", "1", "--cache-dtype", "int8"]) == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_recorded_passes_keep_no_results(tmp_path, dtype):
+    """Passes recorded under many keys hold addresses of one arena: a record keeps no more than one of an engine with a cache in the run's type."""
+    from llm_b200.engine import Entry
+    folder = make_folder(tmp_path, sorted(CONFIGS)[0], BF16)
+
+    def grown(cache_dtype):
+        """What a record of a pass of n - 1 tokens adds to what the device has allocated, behind one of n."""
+        engine = engine_for(folder, dtype, use_graphs=False, max_tokens=4096, cache_dtype=cache_dtype)
+        longest, held = min(engine.max_seq_len - 8, 120), []
+        for n in (longest, longest - 1):
+            for _ in range(4):
+                (slot,) = engine.acquire()
+                engine.step([Entry(slot, random_tokens(n, engine.vocab, n), [n - 1])])
+                engine.release([slot])
+            torch.cuda.synchronize()
+            held.append((torch.cuda.memory_allocated(), len(engine._records)))
+        engine.check()
+        (before, keys), (after, more) = held
+        assert engine.records_run > 0 and more > keys
+        queries = sum(block.mixer.q_width for block in engine.model.blocks) * (longest - 1) * torch.empty((), dtype=dtype).element_size()
+        return after - before, queries
+
+    (plain, queries), (int8, _) = grown(None), grown("int8")
+    assert int8 - plain < queries
