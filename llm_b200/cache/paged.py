@@ -15,7 +15,8 @@ serves a batch:
   for the values) and, per slot, its own list of pages: logical page i of a
   sequence is `pages[i % ring]`;
 * with `kv_dtype` int8 the pages of every group hold keys and values in 8 bits with a scale
-  for each block of `kv_block` positions and head (ops.Int8Pages);
+  for each block of `kv_block` positions and head (ops.Int8Pages); a sequence is shortened to where a
+  block begins;
 * `state` tensors [slots, ...] hold what a mixer keeps per sequence at a fixed
   size; a slot's rows are zeroed when the slot is taken.
 
@@ -126,6 +127,7 @@ class PagedCache:
         if kv_dtype not in (None, dtype, torch.int8) or kv_block not in (1, 2, 4, 8, 16, 32, 64):
             raise LlmError(f"a cache of {kv_dtype} in blocks of {kv_block} positions (int8, and a power of two up to {PAGE})")
         self.int8 = kv_dtype is torch.int8
+        self.kv_block = kv_block
         if self.int8 and any(r is not None and (r.values_are_keys or r.value_dim not in (None, r.head_dim) or r.head_dim % 2) for r in requests):
             raise LlmError("a cache in 8 bits holds keys and values of one and the same even size")
         self.groups: list[Group] = []
@@ -275,6 +277,11 @@ class PagedCache:
                                                             native.ints(shared, c_longlong)))
 
     def set_length(self, slot: int, length: int) -> None:
+        """The slot stands at `length`. Positions behind it are dropped; a cache held in 8 bits goes back to where a block of `kv_block`
+        positions begins (or anywhere with blocks of one position), since dropped positions would keep their say in the scale of
+        a block that is continued."""
+        if self.int8 and length % self.kv_block and length < self.length(slot):
+            raise LlmError(f"slot {slot} cannot go back to {length} positions: its cache in 8 bits has blocks of {self.kv_block}")
         native.check(native.lib().llmh_cache_set_length(self._handle, int(slot), int(length)))
 
     def length(self, slot: int) -> int:

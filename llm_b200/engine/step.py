@@ -95,7 +95,8 @@ class Engine:
     cache_dtype: "int8" holds keys and values in 8 bits with a scale for each block of
         `cache_block` positions and head (for models whose attentions say that they can
         read that); None: in the run's type. Forked sequences hold shared pages once there
-        too, and each reads them for itself.
+        too, and each reads them for itself. A sequence is shortened (`cache.set_length`) to
+        where a block begins, or to any length with `cache_block=1`.
     """
 
     def __init__(self, model, max_tokens: int, max_seq_len: int | None = None,
@@ -159,7 +160,7 @@ class Engine:
 
     def fork(self, slot: int, count: int = 1) -> list:
         """`count` new sequences that stand where `slot` stands: they share its full pages, and attention reads those once
-        for all of them in steps where they stand next to each other (ops.prefix_attention)."""
+        for all of them in steps where they stand next to each other (ops.prefix_attention; with a cache in 8 bits each reads them for itself)."""
         return self.cache.fork(slot, count)
 
     def length(self, slot: int) -> int:

@@ -180,3 +180,32 @@ def test_queries_and_results_lie_in_the_arena(tmp_path, plain_kernels, monkeypat
         plan = engine.workspace.plan_for(n)
         plan.check()
         assert plan.total == other.workspace.plan_for(n).total
+
+
+def test_sequences_go_back_to_where_a_block_begins(tmp_path, plain_kernels, monkeypatch):
+    """Positions that are dropped keep their say in the scale of a block that is continued, and one that was not finite its block: going back into the
+    middle of a block is refused, and what is dropped from a block's beginning on leaves nothing behind."""
+    config, weights, engine = setup(tmp_path, monkeypatch, sorted(CONFIGS)[0], cache_block=16)
+    tokens = random_tokens(40, config["vocab_size"], 3)
+    (slot,) = engine.acquire()
+    engine.step([Entry(slot, tokens[:32], [])])
+    want = engine.step([Entry(slot, tokens[32:], list(range(8)))])
+    for length in (39, 33, 31, 17, 1):
+        with pytest.raises(LlmError, match="block"):
+            engine.cache.set_length(slot, length)
+        assert engine.length(slot) == 40
+    engine.step([Entry(slot, random_tokens(5, config["vocab_size"], 4), [])])
+    engine.cache.set_length(slot, 32)
+    for group in engine.cache.groups:                          # (what the dropped positions may have left: no number at all)
+        page = group.slot_pages[slot][0]
+        group.scales[:, :, page, :, 2:] = float("nan")
+    assert torch.equal(engine.step([Entry(slot, tokens[32:], list(range(8)))]), want)
+    engine.cache.set_length(slot, 40)
+    engine.cache.set_length(slot, 0)
+    engine.cache.set_length(slot, 5)                           # (forward, as before)
+    for options in ({"cache_block": 1}, {"cache_dtype": None}):
+        other = Engine(engine.model, **{"max_tokens": 2048, "cache_dtype": "int8", **options})
+        (slot,) = other.acquire()
+        want = other.step([Entry(slot, tokens, [39])])
+        other.cache.set_length(slot, 37)
+        assert torch.allclose(other.step([Entry(slot, tokens[37:], [2])]), want, atol=2e-4, rtol=1e-4)
