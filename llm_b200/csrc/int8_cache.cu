@@ -396,9 +396,10 @@ void launch_vec(const Args& a, int* status, cudaStream_t stream) {
     int run = a.n_tokens / (148 * 4);
     run = run < 1 ? 1 : run > MAX_RUN ? MAX_RUN : run;
     // few tokens: a token's work over several blocks of threads
-    const int blocks = (a.n_tokens + run - 1) / run, tasks = (a.write_cache ? 2 * a.n_kv_heads : 0) + (a.n_heads * D / 512 + QUERIES - 1) / QUERIES;
+    const int blocks = (a.n_tokens + run - 1) / run, heads = Row<T, D, false>::ROWS * QUERIES;                // of queries, to a task
+    const int tasks = (a.write_cache ? 2 * a.n_kv_heads : 0) + (a.n_heads + heads - 1) / heads, most = (tasks + WARPS - 1) / WARPS;
     int slices = 148 * 4 / blocks;
-    slices = slices > (tasks + WARPS - 1) / WARPS ? (tasks + WARPS - 1) / WARPS : slices < 1 ? 1 : slices;
+    slices = slices > most ? most : slices < 1 ? 1 : slices;
     const dim3 grid(blocks, slices);
     if (a.interleaved) llmb::launch(int8_append_vec_kernel<T, D, true>, grid, dim3(THREADS), 0, stream, true, a, run, status);
     else llmb::launch(int8_append_vec_kernel<T, D, false>, grid, dim3(THREADS), 0, stream, true, a, run, status);

@@ -779,3 +779,16 @@ def test_attention_single_tokens_beside_a_prompt(heads, kv_heads, dim, window):
     b["lengths"][0] = 900
     graph.replay()
     check(b, again)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("heads, kv_heads, dim", [(1, 1, 64), (4, 2, 64), (7, 7, 64), (3, 1, 128), (33, 1, 128)])
+@pytest.mark.parametrize("new", [1, 700])
+def test_append_queries_of_any_number_of_heads(dtype, heads, kv_heads, dim, new):
+    """Queries alone (a layer that reads another's cache), of fewer heads than an instruction has rows, and more than a task has."""
+    b = make([70, 3], [new, 1], heads, kv_heads, dim, dtype, seed=151)
+    x, angles = projection(b, dim, False, 31)
+    before = copies(b)
+    alone = append(b, x, angles, write_cache=False)
+    check_append(b, x, angles, False, before, append(b, x, angles))
+    assert torch.equal(append(b, x, angles), alone)
