@@ -38,8 +38,8 @@ struct Args {
     int n_tokens, n_seqs, n_pages, n_positions;
 };
 
-// What the kernel reports of a place outside of what the call was given: a position without angles, a sequence or a page that there is not. Nothing is
-// read or written there.
+// What the kernel reports of a place outside of what the call was given: a position without angles, a sequence or a page that there is not, a token
+// that is not its sequence's. Nothing is read or written there.
 constexpr int OUT_OF_RANGE = 51;
 
 // the two elements of pair p: rotated pairs first, then neighbours of the part that is not
@@ -100,11 +100,14 @@ __global__ void __launch_bounds__(THREADS) int8_append_kernel(const __grid_const
     const int seq = a.tok_seq[token], first = position % a.block;
     int page = -1, n_rows = 0;
     if ((unsigned)seq < (unsigned)a.n_seqs) {
-        if (first != 0 && token != a.cu_seqlens[seq]) return; // another warp has this block
-        n_rows = min(a.block - first, a.cu_seqlens[seq + 1] - token);
-        page = a.block_table[(size_t)seq * a.table_stride + (position / LLMB_PAGE) % a.ring_pages];
+        const int begin = a.cu_seqlens[seq], end = a.cu_seqlens[seq + 1];
+        if (token >= begin && token < end) {
+            if (first != 0 && token != begin) return;         // another warp has this block
+            n_rows = min(a.block - first, end - token);
+            page = a.block_table[(size_t)seq * a.table_stride + (position / LLMB_PAGE) % a.ring_pages];
+        }
     }
-    if ((unsigned)page >= (unsigned)a.n_pages || n_rows <= 0 || token < a.cu_seqlens[seq] || token + n_rows > a.n_tokens || (a.angles && position + n_rows > a.n_positions)) {
+    if ((unsigned)page >= (unsigned)a.n_pages || token + n_rows > a.n_tokens || (a.angles && position + n_rows > a.n_positions)) {
         if (lane == 0 && status) atomicCAS(status, 0, OUT_OF_RANGE);
         return;
     }
@@ -254,13 +257,18 @@ __global__ void __launch_bounds__(THREADS) int8_append_vec_kernel(const __grid_c
             bool there = b.position >= 0 && !(a.angles && b.position >= a.n_positions);
             if (there) positions[lane] = b.position;
             if (there && a.write_cache) {
-                there = (unsigned)seq < (unsigned)a.n_seqs && b.token >= a.cu_seqlens[seq] && b.token < a.cu_seqlens[seq + 1];
-                if (there && (b.position % a.block == 0 || b.token == a.cu_seqlens[seq])) {
+                int begin = 0, end = 0;
+                if ((unsigned)seq < (unsigned)a.n_seqs) {
+                    begin = a.cu_seqlens[seq];
+                    end = a.cu_seqlens[seq + 1];
+                }
+                there = b.token >= begin && b.token < end;
+                if (there && (b.position % a.block == 0 || b.token == begin)) {
                     int place = b.position / LLMB_PAGE;
                     if (place >= a.ring_pages) place %= a.ring_pages;
-                    b.n_rows = min(a.block - b.position % a.block, a.cu_seqlens[seq + 1] - b.token);
+                    b.n_rows = min(a.block - b.position % a.block, end - b.token);
                     b.page = a.block_table[(size_t)seq * a.table_stride + place];
-                    there = mine = (unsigned)b.page < (unsigned)a.n_pages && b.n_rows > 0 && b.token + b.n_rows <= a.n_tokens &&
+                    there = mine = (unsigned)b.page < (unsigned)a.n_pages && b.token + b.n_rows <= a.n_tokens &&
                                    !(a.angles && b.position + b.n_rows > a.n_positions);
                 }
             }

@@ -792,3 +792,32 @@ def test_append_queries_of_any_number_of_heads(dtype, heads, kv_heads, dim, new)
     alone = append(b, x, angles, write_cache=False)
     check_append(b, x, angles, False, before, append(b, x, angles))
     assert torch.equal(append(b, x, angles), alone)
+
+
+# ----------------------------------------------------------------------------- appends that leave something out
+
+def same_pages(a, b):
+    return all(torch.equal(x.values, y.values) and torch.equal(x.scales.nan_to_num(7.0), y.scales.nan_to_num(7.0)) for x, y in zip(a, b))
+
+
+def cloned(b):
+    return [ops().Int8Pages(c.values.clone(), c.scales.clone()) for c in (b["keys"], b["values"])]
+
+
+APPENDERS = [(F32, 16, 16), (F32, 128, 128), (BF16, 64, 64), (BF16, 128, 128), (BF16, 128, 64), (BF16, 80, 0)]
+
+
+@pytest.mark.parametrize("dtype, dim, n_rot", APPENDERS)
+def test_append_of_tokens_that_are_not_their_sequences(dtype, dim, n_rot):
+    """A token whose sequence says other rows: reported, wherever it stands in its block."""
+    from llm_b200.errors import KernelError
+    b = make([5, 16], [20, 30], 4, 2, dim, dtype, seed=137)
+    x, angles = projection(b, n_rot, False, 23)
+    pos, seq = places(b)
+    for token, says in ((3, 1), (11, 1), (0, 1), (20, 0), (40, 0)):       # in the middle of a block, at its beginning, a sequence's first
+        wrong = seq.clone()
+        wrong[token] = says
+        ops().rope_cache_write_int8(x.flatten(1), angles, pos, wrong, b["arrays"][1], b["table"], b["ring"], b["keys"], b["values"], 4, 2, dim)
+        torch.cuda.synchronize()
+        with pytest.raises(KernelError, match="int8_cache: a step brought"):
+            ops().check_device_status()
