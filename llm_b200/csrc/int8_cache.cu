@@ -39,8 +39,15 @@ struct Args {
 };
 
 // What the kernel reports of a place outside of what the call was given: a position without angles, a sequence or a page that there is not, a token
-// that is not its sequence's. Nothing is read or written there.
+// that is not its sequence's, a sequence that brings more than its ring holds. Nothing is read or written there.
 constexpr int OUT_OF_RANGE = 51;
+
+// Whether the rows begin .. end - 1 of a sequence, of which `token` has `position`, go to pages of their own: with more of them than the ring has, two
+// warps would write to one block.
+__device__ __forceinline__ bool fits_ring(const Args& a, int token, int position, int begin, int end) {
+    const int first = max(position - (token - begin), 0), last = position + (end - 1 - token);
+    return last / LLMB_PAGE - first / LLMB_PAGE < a.ring_pages;
+}
 
 // the two elements of pair p: rotated pairs first, then neighbours of the part that is not
 __device__ __forceinline__ void pair_at(const Args& a, int p, bool turned, int& i0, int& i1) {
@@ -104,7 +111,7 @@ __global__ void __launch_bounds__(THREADS) int8_append_kernel(const __grid_const
         if (token >= begin && token < end) {
             if (first != 0 && token != begin) return;         // another warp has this block
             n_rows = min(a.block - first, end - token);
-            page = a.block_table[(size_t)seq * a.table_stride + (position / LLMB_PAGE) % a.ring_pages];
+            if (fits_ring(a, token, position, begin, end)) page = a.block_table[(size_t)seq * a.table_stride + (position / LLMB_PAGE) % a.ring_pages];
         }
     }
     if ((unsigned)page >= (unsigned)a.n_pages || token + n_rows > a.n_tokens || (a.angles && position + n_rows > a.n_positions)) {
@@ -269,7 +276,7 @@ __global__ void __launch_bounds__(THREADS) int8_append_vec_kernel(const __grid_c
                     b.n_rows = min(a.block - b.position % a.block, end - b.token);
                     b.page = a.block_table[(size_t)seq * a.table_stride + place];
                     there = mine = (unsigned)b.page < (unsigned)a.n_pages && b.token + b.n_rows <= a.n_tokens &&
-                                   !(a.angles && b.position + b.n_rows > a.n_positions);
+                                   !(a.angles && b.position + b.n_rows > a.n_positions) && fits_ring(a, b.token, b.position, begin, end);
                 }
             }
             if (!there && status) atomicCAS(status, 0, OUT_OF_RANGE);

@@ -1755,8 +1755,9 @@ def rope_cache_write_int8(qkv, rope_table, tok_pos, tok_seq, cu_seqlens, block_t
     step continues keeps its scale where that is enough; where it grows, what the block holds is divided by the growth and rounded again. A block that
     the step begins has no memory of what lay there. One that is continued at a position that was written before (a sequence that went back) does: what
     is overwritten keeps its say in the scale, so go back to where a block begins. A value that is not finite makes its block's scale no number until the
-    block is begun anew; attention over it is then none either. No two sequences of a call may write to one page. A position, sequence or page that there is not
-    is left out and reported by `check_device_status`, as is a token that is none of its sequence's rows."""
+    block is begun anew; attention over it is then none either. No two sequences of a call may write to one page. A position, sequence or page that there is not,
+    a token that is none of its sequence's rows, and a sequence that brings more than its ring of pages holds, are left out and reported
+    by `check_device_status`."""
     what = "rope_cache_write_int8"
     if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or not qkv.is_contiguous():
         raise KernelError(f"{what}: qkv {tuple(qkv.shape)} is not contiguous [T, ({n_heads} + 2 * {n_kv_heads}) * {head_dim}]")

@@ -808,6 +808,36 @@ APPENDERS = [(F32, 16, 16), (F32, 128, 128), (BF16, 64, 64), (BF16, 128, 128), (
 
 
 @pytest.mark.parametrize("dtype, dim, n_rot", APPENDERS)
+@pytest.mark.parametrize("held, new", [(10, 300), (0, 257), (63, 194), (250, 2000)])
+def test_append_of_more_than_a_ring_holds(dtype, dim, n_rot, held, new):
+    """A sequence that brings more pages than its ring has is left out and reported; the others of the step, and all queries, are as without it."""
+    from llm_b200.errors import KernelError
+    b = make([held, 3], [new, 2], 4, 2, dim, dtype, ring=4, seed=127)
+    x, angles = projection(b, n_rot, False, 17)
+    keys, values = cloned(b)
+    alone = dict(b, keys=keys, values=values, table=b["table"][1:], lengths=[5], new=[2], cu=[0, 2], arrays=(ints([5]), ints([0, 2])))
+    want = append(alone, x[new:].contiguous(), angles)
+    queries = append(b, x, angles, write_cache=False)
+    torch.cuda.synchronize()
+    ops().check_device_status()
+    got = append(b, x, angles)
+    torch.cuda.synchronize()
+    with pytest.raises(KernelError, match="int8_cache: a step brought"):
+        ops().check_device_status()
+    assert torch.equal(got, queries) and torch.equal(got[new:], want)
+    assert same_pages((b["keys"], b["values"]), (keys, values))
+
+
+@pytest.mark.parametrize("dtype, dim, n_rot", APPENDERS)
+@pytest.mark.parametrize("held, new", [(0, 256), (63, 193), (255, 1), (64 * 9 + 1, 200)])
+def test_append_of_what_a_ring_just_holds(dtype, dim, n_rot, held, new):
+    b = make([held, 3], [new, 2], 4, 2, dim, dtype, ring=4, seed=131)
+    x, angles = projection(b, n_rot, False, 19)
+    before = copies(b)
+    check_append(b, x, angles, False, before, append(b, x, angles))
+
+
+@pytest.mark.parametrize("dtype, dim, n_rot", APPENDERS)
 def test_append_of_tokens_that_are_not_their_sequences(dtype, dim, n_rot):
     """A token whose sequence says other rows: reported, wherever it stands in its block."""
     from llm_b200.errors import KernelError
