@@ -440,7 +440,7 @@ LLMB_EXPORT int llmb_int8_append(const void* qkv, const float* angles, const int
                                  const int* block_table, void* queries, void* keys, float* key_scales, void* values, float* value_scales,
                                  const llmb_int8_append_sizes* sizes, cudaStream_t stream) {
     const llmb_int8_append_sizes& z = *sizes;
-    if (z.n_tokens == 0) return LLMB_OK;
+    if (z.n_tokens == 0 || z.n_seqs == 0) return LLMB_OK;
     LLMB_REQUIRE(z.dtype == LLMB_DTYPE_F32 || z.dtype == LLMB_DTYPE_BF16, "int8_append: unknown dtype %d", z.dtype);
     LLMB_REQUIRE(z.n_tokens > 0 && z.n_seqs > 0 && z.n_heads > 0 && z.n_kv_heads > 0 && z.ring_pages > 0, "int8_append: bad sizes");
     LLMB_REQUIRE(z.head_dim > 0 && z.head_dim % 2 == 0 && z.head_dim <= LLMB_MAX_HEAD_DIM, "int8_append: head_dim %d must be even and at most %d", z.head_dim,

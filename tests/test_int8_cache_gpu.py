@@ -851,3 +851,18 @@ def test_append_of_tokens_that_are_not_their_sequences(dtype, dim, n_rot):
         torch.cuda.synchronize()
         with pytest.raises(KernelError, match="int8_cache: a step brought"):
             ops().check_device_status()
+
+
+@pytest.mark.parametrize("dtype, dim, n_rot", APPENDERS)
+def test_steps_without_sequences(dtype, dim, n_rot):
+    """A padded batch that has no sequence at all: nothing is written."""
+    b = make([5], [3], 4, 2, dim, dtype, seed=139)
+    x, angles = projection(b, n_rot, False, 29)
+    pos, seq = places(b)
+    kept, out = cloned(b), torch.full((3, 4 * dim), 7.0, dtype=dtype, device=DEV)
+    none, table = ints([0]), b["table"][:0]
+    ops().rope_cache_write_int8(x.flatten(1), angles, pos, seq, none, table, b["ring"], b["keys"], b["values"], 4, 2, dim, out=out)
+    ops().attention_int8(b["q"], b["keys"], b["values"], table, b["ring"], ints([]), none, 4, 2, dim, b["scale"], max_new=1, max_len=1, out=out)
+    torch.cuda.synchronize()
+    ops().check_device_status()
+    assert bool((out == 7).all()) and same_pages((b["keys"], b["values"]), kept)
