@@ -53,8 +53,8 @@ struct Args {
 };
 
 // What a kernel reports (no wait has these codes): a step that brings more tokens than max_new says; a place outside of what the call was given, which is
-// not read: a page, a token or a sequence that there is not; a scale of what is seen that is no power of two.
-constexpr int BEYOND_BOUNDS = 50, OUT_OF_RANGE = 51, NOT_A_POWER = 52;
+// not read: a page, a token or a sequence that there is not; a scale of what is seen that is no power of two; scores beyond LARGEST_SCORE.
+constexpr int BEYOND_BOUNDS = 50, OUT_OF_RANGE = 51, NOT_A_POWER = 52, LARGE_SCORES = 53;
 __device__ __forceinline__ void report(int* status, int code) {
     if (status) atomicCAS(status, 0, code);
 }
@@ -145,6 +145,17 @@ __device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
     return v;
 }
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
 
 template <int DMAX>
 constexpr int simt_floats() { return (SIMT_ROWS + 2 * LLMB_PAGE) * (DMAX + 4) + SIMT_ROWS * LLMB_PAGE; }
@@ -579,8 +590,10 @@ __global__ void __launch_bounds__(ROWS_THREADS, DMAX == 64 ? 2 : 1) attention_in
 //
 // fp16 holds 2^-24 to 65504. So queries are divided by the power of two that brings their row's largest to 2^14; scales count from the largest of the
 // positions that a warp works on (2^5 for that one, so that 29 powers of two fit); and a row keeps, beside the running maximum m of its scores, a
-// reference R of score plus exponent of the values' scale, to which its weights w = 2^(score - m) 2^(m + E - R + 14) and its sums refer: weights and
-// values that span more than fp16 does are lost only where they are nothing beside what the row has. All sums are in 32 bits.
+// reference R of score plus exponent of the values' scale, to which its weights w = 2^(score - m) 2^(m + E - R + 14) and its sums refer (what is held is R - m,
+// so that large scores take nothing from it). All sums are in 32 bits. What is lost: values below 2^-29, and weights below 2^-38, of the largest that counts there. That is the
+// largest of what any of the rows sees, in a unit for values and so far for weights: a loud position that one row is not to see takes from the others
+// what is 2^29 below it.
 //
 // The pages of all (sequence, key head) pairs, one after the other, are dealt out to the blocks that the SMs hold at once in ranges of
 // equal length, so a block's range covers the end of one pair, some whole ones, and the beginning of another. Pairs that one block has done as a whole are
@@ -659,6 +672,8 @@ __device__ __forceinline__ void cp_async4(void* smem, const void* global) {
 }
 // 2^(exponent - most + SCALE_UP) for the exponents of two scales, 0 for those without one, as fp16 numbers (0 below what it holds)
 __device__ __forceinline__ float power_of(int exponent, int most) { return exponent ? __uint_as_float((uint32_t)max(exponent - most + SCALE_UP + 127, 0) << 23) : 0.f; }
+// How far a maximum of `from` (-inf: nothing yet) lies below one of `to`, which is no smaller
+__device__ __forceinline__ float moved_by(float from, float to) { return from == -INFINITY ? -INFINITY : from - to; }
 // 2^(a - b) for references that may be -inf (of nothing)
 __device__ __forceinline__ float ratio(float a, float b) { return a == -INFINITY ? 0.f : fast_exp2(a - b); }
 
@@ -935,7 +950,7 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
                 pos[n][j] = of < n_rows ? span.first_pos + of / share : limit;
             }
         }
-        float acc[NT][DIMS / 2][4], m[NT][2], ref[NT][2], sum[NT][2];
+        float acc[NT][DIMS / 2][4], m[NT][2], lag[NT][2], sum[NT][2];            // lag: the reference, from the maximum
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -944,7 +959,7 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
                 for (int k = 0; k < 4; ++k) acc[n][i][k] = 0.f;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                m[n][j] = ref[n][j] = -INFINITY;
+                m[n][j] = lag[n][j] = -INFINITY;
                 sum[n][j] = 0.f;
             }
         }
@@ -1028,54 +1043,68 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
                 }
                 const float k_unit = __uint_as_float((uint32_t)max(ke - SCALE_UP, 1) << 23);                  // what a step of the keys stands for
                 const float v_unit = (float)(ve - 127);
-                float c[NT][2], top[NT][2];
+                float top[NT][2];
                 bool moved = false;
+                // scores in base-2 units: rounded before the maximum is taken off, so that the largest is off by nothing whatever its size
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        c[n][j] = fmaxf(row_scale[n][j] * k_unit, 1.1754944e-38f);
+                        const float c = fmaxf(row_scale[n][j] * k_unit, 1.1754944e-38f);
+#pragma unroll
+                        for (int i = 0; i < 2 * TILES; ++i) {
+                            float& score = s[i >> 1][n][(i & 1) * 2 + j];
+                            score = __fmul_rn(score, c);       // (a packed product would be joined with the packed sum below)
+                        }
                         float x = fmaxf(s[0][n][j], s[0][n][2 + j]);
 #pragma unroll
                         for (int tile = 1; tile < TILES; ++tile) x = max3(x, s[tile][n][j], s[tile][n][2 + j]);
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                        top[n][j] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * c[n][j];
-                        moved |= top[n][j] > m[n][j] || top[n][j] + v_unit > ref[n][j];
+                        top[n][j] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        moved |= top[n][j] > m[n][j] || top[n][j] - m[n][j] + v_unit > lag[n][j];
                     }
+                }
                 if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const float new_m = fmaxf(m[n][j], top[n][j]), new_ref = fmaxf(ref[n][j], top[n][j] + v_unit);
-                            sum[n][j] *= ratio(m[n][j], new_m);
-                            const float shrink = ratio(ref[n][j], new_ref);
+                            const float new_m = fmaxf(m[n][j], top[n][j]), by = moved_by(m[n][j], new_m), held = lag[n][j] + by;
+                            const float new_lag = fmaxf(held, moved_by(top[n][j], new_m) + v_unit);
+                            sum[n][j] *= fast_exp2(by);
+                            const float shrink = ratio(held, new_lag);
 #pragma unroll
                             for (int i = 0; i < DIMS / 2; ++i) {
                                 acc[n][i][j] *= shrink;
                                 acc[n][i][2 + j] *= shrink;
                             }
                             m[n][j] = new_m;
-                            ref[n][j] = new_ref;
+                            lag[n][j] = new_lag;
                         }
                 }
                 uint32_t pb[TILES][NT][2];                     // the weights, positions on the contracted side
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float weight[TILES][4];
+                    float weight[TILES][4], against[2], lift[2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        // (a row that has seen nothing yet has references of -inf, and all its weights are zero)
-                        const float against = m[n][j] == -INFINITY ? 0.f : m[n][j], from = ref[n][j] == -INFINITY ? 0.f : ref[n][j];
-                        const float lift = fast_exp2(fminf(against + v_unit - from + (float)WEIGHT_UP, 126.f));
-#pragma unroll
-                        for (int i = 0; i < 2 * TILES; ++i) {
-                            const float p = fast_exp2(fmaf(s[i >> 1][n][(i & 1) * 2 + j], c[n][j], -against));
-                            sum[n][j] += p;                    // of this lane's positions
-                            weight[i >> 1][(i & 1) * 2 + j] = p * lift;
-                        }
+                        // (a row that has seen nothing yet has a maximum of -inf, and all its weights are zero)
+                        against[j] = m[n][j] == -INFINITY ? 0.f : -m[n][j];
+                        lift[j] = fast_exp2(fminf(v_unit + (float)WEIGHT_UP - lag[n][j], 126.f));
                     }
+                    const uint64_t against2 = pair_of(against[0], against[1]), lift2 = pair_of(lift[0], lift[1]);
+                    uint64_t sum2 = pair_of(sum[n][0], sum[n][1]);
+#pragma unroll
+                    for (int i = 0; i < 2 * TILES; ++i) {
+                        const float(&x)[4] = s[i >> 1][n];
+                        float p0, p1;
+                        unpair(add2(pair_of(x[(i & 1) * 2], x[(i & 1) * 2 + 1]), against2), p0, p1);
+                        const uint64_t p = pair_of(fast_exp2(p0), fast_exp2(p1));
+                        sum2 = add2(sum2, p);                  // of this lane's positions
+                        unpair(mul2(p, lift2), weight[i >> 1][(i & 1) * 2], weight[i >> 1][(i & 1) * 2 + 1]);
+                    }
+                    unpair(sum2, sum[n][0], sum[n][1]);
 #pragma unroll
                     for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
@@ -1153,7 +1182,7 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
 #pragma unroll
                         for (int i = 0; i < DIMS / 2; ++i)
                             *reinterpret_cast<float2*>(rows + r * LD + g * DIMS + 2 * i) = make_float2(acc[n][i][j], acc[n][i][2 + j]);
-                        if (g == 0) *reinterpret_cast<float4*>(rows + 8 * NT * LD + r * 4) = make_float4(m[n][j], ref[n][j], sum[n][j], 0.f);
+                        if (g == 0) *reinterpret_cast<float4*>(rows + 8 * NT * LD + r * 4) = make_float4(m[n][j], lag[n][j], sum[n][j], 0.f);
                     }
             }
             __syncthreads();
@@ -1164,9 +1193,10 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
                     for (int j = 0; j < 2; ++j) {
                         const int r = n * 8 + 2 * t + j;
                         const float4 other = *reinterpret_cast<const float4*>(rows + 8 * NT * LD + r * 4);
-                        const float new_m = fmaxf(m[n][j], other.x), new_ref = fmaxf(ref[n][j], other.y);
-                        sum[n][j] = sum[n][j] * ratio(m[n][j], new_m) + other.z * ratio(other.x, new_m);
-                        const float mine = ratio(ref[n][j], new_ref), theirs = ratio(other.y, new_ref);
+                        const float new_m = fmaxf(m[n][j], other.x), by = moved_by(m[n][j], new_m), other_by = moved_by(other.x, new_m);
+                        const float held = lag[n][j] + by, other_held = other.y + other_by, new_lag = fmaxf(held, other_held);
+                        sum[n][j] = sum[n][j] * fast_exp2(by) + other.z * fast_exp2(other_by);
+                        const float mine = ratio(held, new_lag), theirs = ratio(other_held, new_lag);
 #pragma unroll
                         for (int i = 0; i < DIMS / 2; ++i) {
                             const float2 x = *reinterpret_cast<const float2*>(rows + r * LD + g * DIMS + 2 * i);
@@ -1174,7 +1204,7 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
                             acc[n][i][2 + j] = acc[n][i][2 + j] * mine + x.y * theirs;
                         }
                         m[n][j] = new_m;
-                        ref[n][j] = new_ref;
+                        lag[n][j] = new_lag;
                     }
             }
         }
@@ -1188,7 +1218,7 @@ attention_int8_few_kernel(const __grid_constant__ CUtensorMap map_k, const __gri
                 for (int j = 0; j < 2; ++j) {
                     const int r = n * 8 + 2 * t + j;
                     if (r >= n_rows) continue;
-                    float factor = sum[n][j] != 0.f ? fast_exp2(ref[n][j] - (float)(WEIGHT_UP + SCALE_UP) - m[n][j]) : 0.f;
+                    float factor = sum[n][j] != 0.f ? fast_exp2(lag[n][j] - (float)(WEIGHT_UP + SCALE_UP)) : 0.f;
                     if (whole) {
                         factor /= sum[n][j] != 0.f ? sum[n][j] : 1.f;
                         uint32_t out[DIMS / 2];
@@ -1343,15 +1373,8 @@ constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 88, REGS_WIDEN = 56, REGS_LAUNCHED
 static_assert(128 * (REGS_ISSUE + 4 * REGS_SOFTMAX + REGS_WIDEN) <= WIDE_THREADS * REGS_LAUNCHED, "the shares come from what the block is launched with");
 constexpr int WIDE_UP = 7;                  // power of two that weights are lifted to; R may lag 2^8 behind
 constexpr int VALUE_SPAN = 90;
+constexpr float LARGEST_SCORE = 8388608.f;  // 2^23, in base-2 units: beyond, a reference (integers away from a score) is not exact and weights leave fp16; reported
 constexpr int INFOS = 4;                    // steps whose scales are on their way to the softmax: the step behind the next one may be widened by then
-
-// two 32-bit values to an instruction
-__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
-    uint64_t v;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
-    return v;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
 
 struct StepInfo {
     float k_unit, v_unit[2];         // what a step of the keys stands for; exponent of the values' reference, of each page
@@ -1841,7 +1864,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                 fence_async_shared();
                 tcgen05_fence_before();                        // (the last result has been read)
                 mbar_arrive(smem_u32(&q_full[tile]));
-                float run_max = -INFINITY, ref = -INFINITY, run_sum = 0.f;
+                float run_max = -INFINITY, ref = -INFINITY, run_sum = 0.f, lowest = -INFINITY;      // lowest: the first maximum, as maxima only grow
                 for (int i = st; i < end; ++i) {
                     ok = ok && mbar_wait_warp(smem_u32(&s_full[tile]), turns++ & 1, abort_flag, status, 38);
                     tcgen05_fence_after();
@@ -1884,7 +1907,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                         top = max3(top, t0, t1);
                     }
                     tmem_st_wait();
-                    top *= c;
+                    top = __fmul_rn(top, c);                   // (not joined with a sum behind it: both warps of a row decide by the rounded one)
                     *mine = __float_as_uint(top);
                     meet();
                     const float other = __uint_as_float(*theirs);
@@ -1933,6 +1956,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                     float lo, hi;                              // what the page's weights are lifted by is taken off their sum
                     unpair(add, lo, hi);
                     run_sum = run_sum * ratio(run_max, new_max) + (none ? lo + hi : (lo + hi) * fast_exp2(-shift - new_max));
+                    lowest = run_max == -INFINITY ? new_max : lowest;
                     run_max = new_max;
                     ref = new_ref;
                 }
@@ -1948,6 +1972,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) attention_int8_wide_kernel(co
                     run_sum += __uint_as_float(*theirs);
                     meet();                                    // (both have read)
                     const bool whole = segment.start >= r0 && segment.start + segment.steps <= r1;
+                    if (valid && ((run_max > LARGEST_SCORE && run_max != INFINITY) || (lowest < -LARGEST_SCORE && lowest != -INFINITY))) report(status, LARGE_SCORES);
                     float factor = run_sum != 0.f ? fast_exp2(ref - (float)(WIDE_UP + SCALE_UP) - run_max) : 0.f;
                     const size_t row = ((size_t)blockIdx.x * 2 + (segment.start >= r0 ? 1 : 0)) * WIDE_ROWS + tile * TILE_ROWS + r;
                     unsigned char* to = nullptr;               // this half of the row in memory

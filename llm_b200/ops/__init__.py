@@ -1459,7 +1459,7 @@ _prefix_entry = None
 _BEYOND_BOUNDS = 50             # its report of a step larger than its bounds (csrc/prefix_attention.cu)
 _FARTHEST = (1 << 31) - 1       # elements between rows, as the kernels count them
 _INT8_REPORTS = {50: "more tokens than max_new said", 51: "a position, sequence, token or page that there is not",
-                 52: "a scale that is no power of two"}      # (csrc/attention_int8.cu, int8_cache.cu)
+                 52: "a scale that is no power of two", 53: "scores beyond 2^23 in base-2 units"}      # (csrc/attention_int8.cu, int8_cache.cu)
 
 
 def _declare_prefix():
@@ -1812,7 +1812,8 @@ def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seql
 
     max_new, max_len: most new tokens and most positions of a sequence, upper bounds that size the launches (a sequence longer than max_len is
     served all the same). A step that brings more tokens than max_new says, a page or token that there is not, a sequence whose queries see more
-    pages than its ring has, and a scale that is no power of two are reported by `check_device_status`; its results are not valid. `seq_order` (int32 [B]): the sequences by falling length, which start
+    pages than its ring has, a scale that is no power of two, and (in bfloat16, where a sequence brings more than 16 queries to a key head) scores
+    beyond 2^23 / log2(e) are reported by `check_device_status`; its results are not valid. `seq_order` (int32 [B]): the sequences by falling length, which start
     in that order."""
     what = "attention_int8"
     if qkv.dim() != 2:

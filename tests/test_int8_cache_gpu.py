@@ -866,3 +866,105 @@ def test_steps_without_sequences(dtype, dim, n_rot):
     torch.cuda.synchronize()
     ops().check_device_status()
     assert bool((out == 7).all()) and same_pages((b["keys"], b["values"]), kept)
+
+
+# ----------------------------------------------------------------------------- loud positions that a row does not see
+
+def check_rows(b, got):
+    """`check` with each row's own share of what may be lost: n 2^-32 times the largest value that the row itself sees."""
+    heads, dim, share = b["heads"], b["dim"], b["heads"] // b["kv_heads"]
+    weight, half = (0.0, 0.0) if b["dtype"] == F32 else (2.0 ** -11, 2.0 ** -8)
+    torch.cuda.synchronize()
+    ops().check_device_status()
+    got, (length,), (n_new,) = got.double().view(-1, heads, dim), b["lengths"], b["new"]
+    row = torch.arange(length, device=DEV)
+    seen = row[None, :] <= torch.arange(length - n_new, length, device=DEV)[:, None]
+    page = b["table"][0].long()[row // PAGE]
+    for a in range(heads):
+        k, v = (cache.held(torch.float64)[page, a // share, row % PAGE] for cache in (b["keys"], b["values"]))
+        q = b["q"][:, a * dim:(a + 1) * dim].double()
+        weights = torch.softmax((q @ k.T * b["scale"]).masked_fill(~seen, -math.inf), -1)
+        want, size = weights @ v, weights @ v.abs()
+        worst = ((q.abs() @ k.abs().T) * b["scale"]).masked_fill(~seen, 0).amax(-1, keepdim=True)
+        bound = (4 * (2 * (dim + 8) * worst + length + 16) * U + weight + half) * size + half * want.abs() + 1e-30
+        if weight:
+            bound = bound + length * 2.0 ** -32 * (seen * v.abs().amax(-1)).amax(-1, keepdim=True)
+        off = (got[:, a] - want).abs()
+        assert bool((off <= bound).all()), (a, float((off / bound).max()))
+
+
+@pytest.mark.parametrize("dtype, dim, apart", [(BF16, 64, 28), (BF16, 128, 28), (F32, 64, 28), (F32, 128, 90), (BF16, 80, 90)])
+@pytest.mark.parametrize("held, new", [(14, 4), (0, 64), (100, 70), (0, 500)])
+@pytest.mark.parametrize("which", ["keys", "values"])
+def test_attention_loud_positions_that_a_row_does_not_see(dtype, dim, apart, held, new, which):
+    """A block of later positions that is 2^apart times as loud as all others, in the same page, under the causal mask: rows in front of it are as near as
+    without it, and those that see it are right. (The tensor cores' kernels hold scales within 29 powers of two of the largest that a row of the tile sees.)"""
+    b = make([held], [new], 8, 2, dim, dtype, seed=157)
+    first = -(-(held + new // 2) // 16) * 16                   # of the loud block
+    assert held < first < held + new
+    if which == "keys" and dtype == BF16 and dim != 80 and new > 4:
+        apart = 17                                             # (scores beyond 2^23 are reported there: the next test)
+    for name in ("keys", "values"):
+        base = -6.0 if name == "keys" or apart < 60 else -50.0
+        for p in range(0, held + new, 16):
+            b[name].scales[b["table"][0, p // PAGE], :, p % PAGE // 16] = 2.0 ** (base + (apart if name == which and p == first else 0))
+    got = call(b)
+    check_rows(b, got)
+    check(b, got)
+
+
+@pytest.mark.parametrize("dtype, dim", [(BF16, 64), (BF16, 128), (F32, 64), (BF16, 80)])
+@pytest.mark.parametrize("held, new", [(300, 1), (300, 3), (14, 4), (300, 40), (0, 70), (2500, 40)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attention_large_scores(dtype, dim, held, new, sign):
+    """One key that has all of a row's weight by scores of up to 2^35: its value comes back, or the call is reported. At negative scores (all of a row's) the
+    smallest wins."""
+    from llm_b200.errors import KernelError
+    for size in (14, 20, 26, 33):
+        b = make([held], [new], 8, 2, dim, dtype, seed=167)
+        b["q"].fill_(1.0)
+        pages = b["table"][0].long()
+        at = [min(5 + 64 * i, held) for i in range(2)] + [held]            # keys that stand out, a little more each time
+        b["keys"].values.fill_(0 if sign > 0 else -64)
+        for i, p in enumerate(at):
+            b["keys"].values[pages[p // PAGE], :, p % PAGE] = int((64 + 8 * i) if sign > 0 else -(40 - 8 * i))
+        b["keys"].scales[pages] = 2.0 ** (size - 6 - round(math.log2(dim * b["scale"])))
+        b["values"].scales[pages] = 2.0 ** -9
+        b["values"].scales[pages[-1:]] = 2.0 ** -3
+        got = call(b)
+        torch.cuda.synchronize()
+        scores = 1.4427 * b["scale"] * dim * 64 * 2.0 ** (size - 6 - round(math.log2(dim * b["scale"])))
+        if dtype == BF16 and dim != 80 and new > 4 and scores > 2.0 ** 23:
+            with pytest.raises(KernelError, match="scores beyond"):
+                ops().check_device_status()
+            continue
+        ops().check_device_status()
+        got, want = got.double().view(new, 8, dim), b["values"].held(torch.float64)[pages[held // PAGE], :, held % PAGE]
+        want = want.repeat_interleave(4, 0)
+        assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -10 if size == 14 else 0.0)).all()), (size, float((got - want).abs().max()))
+
+
+def test_attention_references_at_the_border_of_a_move():
+    """Scores whose rounded product lies at the border of where a reference moves, and the unrounded one beyond it: both warps of a row decide alike."""
+    import numpy as np
+    log2e, held, new = np.float32(1.4426950408889634), 150, 50
+    b = make([held], [new], 4, 1, 128, BF16, seed=173)
+    pages = b["table"][0].long()
+    b["keys"].scales[pages[:4]] = 2.0 ** -4
+    b["values"].scales[pages[:4]] = 2.0 ** -3
+    b["keys"].values.zero_()
+    b["keys"].values[pages[2], 0, 7, 0] = 64                   # scores of 0, and one of 8 in the second step
+    tried = 0
+    for m in range(128):
+        product = (1 + m / 128) * 64 * 2.0 ** -4
+        at = int(np.float32(8 / product / float(log2e)).view(np.int32))
+        scale = next((float(s) for s in (np.int32(at + d).view(np.float32) for d in range(-40, 41))
+                      if 8 + 2.0 ** -22 < float(np.float32(s * log2e)) * product < 8 + 2.0 ** -21), None)
+        if scale is None:
+            continue
+        b["q"].zero_()
+        b["q"].view(new, 4, 128)[:, :, 0] = 1 + m / 128
+        b["scale"] = scale
+        check(b, call(b))
+        tried += 1
+    assert tried > 20
