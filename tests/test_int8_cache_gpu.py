@@ -968,3 +968,15 @@ def test_attention_references_at_the_border_of_a_move():
         check(b, call(b))
         tried += 1
     assert tried > 20
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("apart", [12, 28, 45])
+@pytest.mark.parametrize("held, new, window", [(40, 4, 0), (0, 64, 0), (100, 90, 0), (300, 4, 30), (300, 90, 50), (1000, 60, 300)])
+def test_attention_values_lost_beside_loud_ones(dim, apart, held, new, window):
+    """Values beside much louder ones, some of which a row does not see: what is lost is small beside the largest that a row of the tile sees."""
+    b = make([held], [new], 8, 2, dim, BF16, window=window, seed=163)
+    for p in range(0, held + new, 16):
+        loud = p // 16 % 3 == 1
+        b["values"].scales[b["table"][0, p // PAGE], :, p % PAGE // 16] = 2.0 ** (-20 + (apart if loud else 0))
+    check(b, call(b))
