@@ -13,7 +13,7 @@ flags of apps/cli/src/bench.rs:45-71 (-m, -c, -p, -n, -r, -o with comma lists)
 and its two tests: `pp<N>` times the prefill of N tokens and nothing else,
 `tg<N>` prefills a 16-token prompt and times only the decoding of N tokens
 (bench.rs:10-12,27); `-b` adds the batch size; every test runs once uncounted before its `-r`
-repetitions. `--cache-dtype int8` holds keys and values in 8 bits. `inspect` prints the model's
+repetitions. `--cache-dtype int8` holds keys and values in 8 bits, `--cache-block N` positions to a scale (16). `inspect` prints the model's
 geometry, checks the checkpoint's tensors and names the kernel variant each
 product and attention shape gets (apps/cli/src/inspect.rs:16-131).
 """
@@ -69,7 +69,7 @@ def _held_by_samples(model, prompt_tokens: int, max_tokens: int, context: int, s
 
 def complete(args) -> int:
     model, context, max_tokens, temperature, dtype = None, DEFAULT_CONTEXT, DEFAULT_MAX_TOKENS, 0.7, "bfloat16"
-    seed, prompt, samples, cache_dtype = None, [], 1, None
+    seed, prompt, samples, cache_dtype, cache_block = None, [], 1, None, 16
     while args:
         a = args.pop(0)
         if a == "--model":
@@ -84,6 +84,8 @@ def complete(args) -> int:
             dtype = _value(args, a)
         elif a == "--cache-dtype":
             cache_dtype = _value(args, a)
+        elif a == "--cache-block":
+            cache_block = int(_value(args, a))
         elif a == "--seed":
             seed = int(_value(args, a))
         elif a == "--samples":
@@ -93,7 +95,7 @@ def complete(args) -> int:
     if model is None or not prompt:
         raise SystemExit("usage: python -m llm_b200 --model DIR [--context N] [--max-tokens N] "
                          "[--temperature T] [--dtype bfloat16|float32] [--seed S] [--samples N] "
-                         "[--cache-dtype int8] TOKEN_ID ...")
+                         "[--cache-dtype int8 [--cache-block N]] TOKEN_ID ...")
     if samples < 1:
         raise SystemExit("--samples needs a number of at least 1")
     import llm_b200
@@ -102,7 +104,7 @@ def complete(args) -> int:
         from .api import parse_dtype
         from .engine import load_model
         bound = load_model(model, parse_dtype(dtype), "cuda:0")
-        llm = llm_b200.LLM(bound, context=context, batch=samples, cache_dtype=cache_dtype,
+        llm = llm_b200.LLM(bound, context=context, batch=samples, cache_dtype=cache_dtype, cache_block=cache_block,
                            max_tokens_held=_held_by_samples(bound, len(prompt), max_tokens, context, samples))
         (results,) = llm.generate([prompt], max_tokens=max_tokens, temperature=temperature, details=True, samples=samples, **options)
         for result in results:
@@ -111,7 +113,7 @@ def complete(args) -> int:
         print(f"[{results[0].prompt_tokens} prompt tokens, {drawn} generated in {samples} samples, ttft {results[0].ttft_ms:.0f} ms, "
               f"{sum(r.tokens_per_second for r in results):.1f} tok/s]", file=sys.stderr)
         return 0
-    llm = llm_b200.LLM(model, dtype=dtype, context=context, batch=1, cache_dtype=cache_dtype)
+    llm = llm_b200.LLM(model, dtype=dtype, context=context, batch=1, cache_dtype=cache_dtype, cache_block=cache_block)
     (result,) = llm.generate([prompt], max_tokens=max_tokens, temperature=temperature, details=True,
                              on_token=lambda i, t: print(t, end=" ", flush=True), **options)
     print()
@@ -123,7 +125,7 @@ def complete(args) -> int:
 
 def bench(args) -> int:
     model_dir, random_shape, context, dtype = None, None, DEFAULT_CONTEXT, "bfloat16"
-    prompts, gens, batches, reps, as_json, layers, cache_dtype = [512], [128], [1], 5, False, None, None
+    prompts, gens, batches, reps, as_json, layers, cache_dtype, cache_block = [512], [128], [1], 5, False, None, None, 16
     while args:
         a = args.pop(0)
         if a in ("-m", "--model"):
@@ -148,6 +150,8 @@ def bench(args) -> int:
             dtype = _value(args, a)
         elif a == "--cache-dtype":
             cache_dtype = _value(args, a)
+        elif a == "--cache-block":
+            cache_block = int(_value(args, a))
         else:
             raise SystemExit(f"unknown bench flag {a}")
     if (model_dir is None) == (random_shape is None):
@@ -171,7 +175,7 @@ def bench(args) -> int:
     rows = []
     for batch in batches:
         per_seq = round_up(context)
-        engine = Engine(model, max_tokens=batch * per_seq, max_seq_len=context, max_slots=batch, cache_dtype=cache_dtype)
+        engine = Engine(model, max_tokens=batch * per_seq, max_seq_len=context, max_slots=batch, cache_dtype=cache_dtype, cache_block=cache_block)
         for n in prompts:
             samples = []
             for rep in range(reps + 1):            # the first run is not counted: it plans the scratch

@@ -170,3 +170,21 @@ def test_recorded_passes_keep_no_results(tmp_path, dtype):
 
     (plain, queries), (int8, _) = grown(None), grown("int8")
     assert int8 - plain < queries
+
+
+def test_blocks_of_the_command_line(tmp_path, capsys):
+    """--cache-block reaches the engine: the same tokens as LLM(cache_block=...) gives, and numbers that are none refused."""
+    import llm_b200
+    from llm_b200 import cli
+    from llm_b200.errors import LlmError
+    folder = make_folder(tmp_path, sorted(CONFIGS)[0], BF16)
+    prompt = random_tokens(30, llm_b200.LLM(str(folder), context=100).engine.vocab, 9)
+    for block in (1, 64):
+        (want,) = llm_b200.LLM(str(folder), context=100, batch=1, cache_dtype="int8", cache_block=block).generate([prompt], max_tokens=12, temperature=0)
+        arguments = ["--model", str(folder), "--context", "100", "--max-tokens", "12", "--temperature", "0", "--cache-dtype", "int8", "--cache-block", str(block)]
+        capsys.readouterr()
+        assert cli.main(arguments + [str(t) for t in prompt]) == 0
+        assert [int(x) for x in capsys.readouterr().out.split()] == want
+    assert cli.main(["bench", "-m", str(folder), "-c", "64", "-p", "16", "-n", "4", "-r", "1", "--cache-dtype", "int8", "--cache-block", "32"]) == 0
+    with pytest.raises(LlmError, match="blocks of 3 positions"):
+        llm_b200.LLM(str(folder), context=100, cache_dtype="int8", cache_block=3)
