@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, DMAX == 64 ? 2 : 1) attention_in
 // ends of pairs; warps meet where a pair ends. Of a pair that several blocks have, a launch joins the parts, or the last block to come (plan_for).
 //
 // 64 sequences of 8,192 positions (32 heads over 8 of 128, 1.08 GB) take 173 us in short bursts, 6.2 TB/s, and 204 in long loops at the power cap: reading
-// is the limit, and the energy of some 780 instructions for 8 KB. Eight take 37 us, one 11 on the device: 10 of them are a block's start (lengths, table,
+// is the limit, and the energy of some 770 instructions for 8 KB. Eight take 37 us, one 11 on the device: 10 of them are a block's start (lengths, table,
 // first pages: dependent reads), its end and the join. Three blocks an SM of 165 registers; with maximum, reference and masks worked out anew for every unit,
 // and 32 positions for heads of 64 too, a unit took 1,130 instructions.
 
@@ -1361,7 +1361,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attention_int8_few_join_kerne
 // scheduler's slots and its traffic through shared memory some 2,800.
 //
 // References as above, with two differences: keys' scales count from the largest of the 128 positions of a step, values' from the largest of each page (from
-// 2^-90 of the largest so far at least, which keeps the sums of the weights exact where a page's values are zeros), and R moves only when it is exceeded by 2^8.
+// 2^-90 of the largest so far at least, which keeps the sums of the weights exact where a page's values are zeros), and R moves only when it is exceeded by 2^8
+// (weights below 2^-31 of the row's largest contribution may be lost).
 //
 // The steps of all (sequence, key head, tile), one after the other, are dealt out to the blocks in ranges of equal length, as pages are above; barriers
 // and buffers run on from one tile to the next, so the next tile's keys are fetched and widened while a result is written.

@@ -94,8 +94,9 @@ class Engine:
         model says it can be captured).
     cache_dtype: "int8" holds keys and values in 8 bits with a scale for each block of
         `cache_block` positions and head (for models whose attentions say that they can
-        read that); None: in the run's type. Forked sequences hold shared pages once there
-        too, and each reads them for itself. A sequence is shortened (`cache.set_length`) to
+        read that); None: in the run's type. All columns of a head share a scale: a model whose
+        keys have columns much louder than the rest loses more by it than others. Forked
+        sequences hold shared pages once there too, and each reads them for itself. A sequence is shortened (`cache.set_length`) to
         where a block begins, or to any length with `cache_block=1`.
     """
 

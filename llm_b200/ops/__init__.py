@@ -1812,9 +1812,12 @@ def attention_int8(qkv, keys, values, block_table, ring_pages, seq_lens, cu_seql
 
     max_new, max_len: most new tokens and most positions of a sequence, upper bounds that size the launches (a sequence longer than max_len is
     served all the same). A step that brings more tokens than max_new says, a page or token that there is not, a sequence whose queries see more
-    pages than its ring has, a scale that is no power of two, and (in bfloat16, where a sequence brings more than 16 queries to a key head) scores
-    beyond 2^23 / log2(e) are reported by `check_device_status`; its results are not valid. `seq_order` (int32 [B]): the sequences by falling length, which start
-    in that order."""
+    pages than its ring has, a scale that is no power of two, and scores beyond 2^23 / log2(e) (in bfloat16 with heads of 64 and 128, where max_new
+    says more than 16 queries to a key head) are reported by `check_device_status`; its results are not valid. `seq_order` (int32 [B]): the sequences by
+    falling length, which start in that order.
+
+    The same call gives the same bits each time; a call inside of a step's scope (`StepScope`) may add the parts of a long sequence in another order than
+    one outside. In bfloat16 with heads of 64 and 128, n positions lose n 2^-32 of the largest value in 8 bits that a query of the same tile sees."""
     what = "attention_int8"
     if qkv.dim() != 2:
         raise KernelError(f"{what}: queries must be rows")
