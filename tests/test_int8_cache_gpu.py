@@ -980,3 +980,28 @@ def test_attention_values_lost_beside_loud_ones(dim, apart, held, new, window):
         loud = p // 16 % 3 == 1
         b["values"].scales[b["table"][0, p // PAGE], :, p % PAGE // 16] = 2.0 ** (-20 + (apart if loud else 0))
     check(b, call(b))
+
+
+@pytest.mark.parametrize("dtype, dim", [(F32, 64), (F32, 128), (BF16, 64), (BF16, 128), (BF16, 80), (BF16, 256)])
+@pytest.mark.parametrize("held, new", [([3000, 70], [1, 1]), ([300, 70], [4, 3]), ([300, 0], [60, 90]), ([9000], [33])])
+def test_attention_queries_that_are_not_finite_and_extreme_scales(dtype, dim, held, new):
+    """A query that is not finite has no number for a result, and no other query's result changes by a bit; whole numbers of -128, and scales at
+    both ends of what 32 bits hold."""
+    b = make(held, new, 8, 2, dim, dtype, seed=179)
+    want, n = call(b).clone(), b["cu"][-1]
+    spoilt = torch.zeros(n, 8, dtype=torch.bool, device=DEV)
+    spoilt[0, 1] = spoilt[n - 1, 5] = True
+    for bad in (math.nan, math.inf, -math.inf):
+        q = b["q"].clone()
+        q[0, dim + 3] = q[n - 1, 5 * dim + 3] = bad
+        got = call({**b, "q": q}).view(n, 8, dim)
+        torch.cuda.synchronize()
+        ops().check_device_status()
+        assert bool(got[spoilt].isnan().all()) and torch.equal(got[~spoilt], want.view(n, 8, dim)[~spoilt])
+    for which, exponent in (("values", -126), ("values", 110), ("keys", -126)):
+        c = make(held, new, 8, 2, dim, dtype, seed=181)
+        c[which].values[:, :, ::3] = -128
+        c[which].scales[~c[which].scales.isnan()] = 2.0 ** exponent
+        check(c, call(c))
+    c["values"].scales[~c["values"].scales.isnan()] = 0.0
+    assert not bool(call(c).any())
